@@ -20,6 +20,7 @@ _f = ctypes.c_void_p  # device pointers
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
 _sz = ctypes.c_size_t
+_strides = ctypes.POINTER(ctypes.c_int64)  # a host array
 
 # name -> argtypes, restype (int status unless stated)
 SIGNATURES = {
@@ -89,6 +90,15 @@ SIGNATURES = {
     "csn_spatial_generators_partials": ([_i64, _i64, _int], _i64),
     "csn_spatial_generators_fwd": ([_f, _f, _f, _f, _f, _f, _f, _f, _i64, _i64, _i64, _int, _f], _int),
     "csn_spatial_generators_bwd": ([_f] * 13 + [_i64, _i64, _i64, _int, _f], _int),
+    "csn_gated_scan_marks": ([_i64, _i64, _i64, _int], _i64),
+    "csn_gated_scan_fwd": ([_f, _f, _f, _strides, _f, _f, _f, _f, _f, _i64, _i64, _i64, _int, _f], _int),
+    "csn_gated_scan_bwd": ([_f, _f, _f, _f, _strides, _f, _f, _f, _f, _f, _f, _f, _i64, _i64, _i64, _int, _f], _int),
+    "csn_gated_step": ([_f, _f, _f, _strides, _f, _f, _i64, _i64, _int, _f], _int),
+    "csn_silu_gated_linear_workspace_bytes": ([_i64, _i64, _i64, _int], _sz),
+    "csn_silu_gated_linear_fwd": ([_f, _i64, _f, _i64, _f, _i64, _f, _i64, _i64, _i64, _int, _f, _sz, _f], _int),
+    "csn_silu_gated_linear_bwd": ([_f, _i64, _f, _i64, _f, _i64, _f, _i64, _f, _f, _f, _i64, _i64, _i64, _int, _f,
+                                   _sz, _f], _int),
+    "csn_dropout_add": ([_f, _f, _f, _f, _i64, _int, _int, _f], _int),
     "csn_timing_enable": ([_int], _int),
     "csn_timing_reset": ([], _int),
     "csn_timing_read": ([ctypes.c_char_p, ctypes.POINTER(ctypes.c_double),

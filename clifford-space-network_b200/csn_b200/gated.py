@@ -1,0 +1,295 @@
+"""PyTorch front end of the gated recurrent block's kernels (csrc/csn_gated_scan.cu, csn_ffn.cu,
+csn_dropout.cu): the channelwise recurrence and its step, the gated feed-forward product, and
+dropout on the residual path.
+
+Unlike the rotor ops these read and write float32, bfloat16 and float16 tensors as they are (all
+tensors of a call of one type; recurrence states are float32) and take strided rows in place: only
+the last axis has to be contiguous, so slices of one projection's output are not copied.  Every op
+runs on the current stream of its tensors' device.  Gradients are first-order: a second backward
+pass through them raises.
+
+The reference has no counterpart of these; its matrix recurrence is python/clifford_cl6.py:150-171
+and its gated product python/clifford_model.py:42-43.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .ops import _ptr, _require_cuda, _stream, _workspace
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _dtype_of(name, allowed, *ts):
+    """The dtype code of tensors that have to share one of the allowed types."""
+    dtype = ts[0].dtype
+    if dtype not in allowed or any(t is not None and t.dtype != dtype for t in ts):
+        raise ValueError(f"{name}: tensors of one type among {', '.join(str(d) for d in allowed)} expected, got "
+                         f"{', '.join(str(t.dtype) for t in ts if t is not None)}")
+    return DTYPES[dtype]
+
+
+def _same_device(name, *ts):
+    _require_cuda(*ts)
+    if len({t.device for t in ts if t is not None}) > 1:
+        raise ValueError(f"{name}: tensors are on different devices")
+
+
+def _on(device):
+    """Makes `device` current for a launch, where it is not."""
+    if torch.cuda.current_device() == device.index:
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _rows(t):
+    """t detached, with a contiguous last axis (itself where it has one)."""
+    if t is None:
+        return None
+    t = t.detach()
+    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def _packed(t):
+    """Contiguous and 16-byte aligned (itself where it is)."""
+    if t is None:
+        return None
+    t = t.detach().contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
+def _row_strides(*ts):
+    """Strides of every axis but the last of each tensor, as a host array; 0 where an axis has one
+    entry (its stride means nothing) or a tensor is absent.  [rows, C] gives (0, row)."""
+    out = []
+    for t in ts:
+        st = [] if t is None else [t.stride(i) if t.shape[i] > 1 else 0 for i in range(t.dim() - 1)]
+        out += [0] * (2 - len(st)) + st
+    return (ctypes.c_int64 * len(out))(*out)
+
+
+def _wants_grad(*ts):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+# ------------------------------------------------------------- gated recurrence
+def _scan_sizes(f, cu):
+    if cu is None:
+        return f.shape[0], f.shape[1], f.shape[2]
+    return cu.shape[0] - 1, f.shape[0], f.shape[1]
+
+
+def _gated_scan_fwd(f, x, h0, gate, cu, keep):
+    """(y, h_last, marks or None) of rows as they lie; h0 float32."""
+    f, x, gate, h0 = _rows(f), _rows(x), _rows(gate), _packed(h0)
+    S, T, C = _scan_sizes(f, cu)
+    dev = f.device
+    y = torch.empty(f.shape, dtype=f.dtype, device=dev)
+    h_last = torch.empty(S, C, dtype=torch.float32, device=dev)
+    marks = None
+    if keep:
+        marks = torch.empty(_lib.load().csn_gated_scan_marks(S, T, C, int(cu is not None)), dtype=torch.float32,
+                            device=dev)
+    with _on(dev):
+        _lib.call("csn_gated_scan_fwd", _ptr(f), _ptr(x), _ptr(gate), _row_strides(f, x, gate), _ptr(h0), _ptr(cu),
+                  _ptr(y), _ptr(h_last), _ptr(marks), S, T, C, DTYPES[f.dtype], _stream(dev))
+    return y, h_last, marks
+
+
+def _gated_scan_bwd(f, x, gate, cu, marks, dy, dh_last, need):
+    """Gradients (df, dx, dh0, dgate) where `need` asks for them, None elsewhere."""
+    f, x, gate, dy, dh_last = _rows(f), _rows(x), _rows(gate), _rows(dy), _packed(dh_last)
+    S, T, C = _scan_sizes(f, cu)
+    dev = f.device
+    like = lambda want: torch.empty(f.shape, dtype=f.dtype, device=dev) if want else None  # noqa: E731
+    df, dx, dgate = like(need[0]), like(need[1]), like(need[3] and gate is not None)
+    dh0 = torch.empty(S, C, dtype=torch.float32, device=dev) if need[2] else None
+    with _on(dev):
+        _lib.call("csn_gated_scan_bwd", _ptr(f), _ptr(x), _ptr(gate), _ptr(dy), _row_strides(f, x, gate, dy),
+                  _ptr(cu), _ptr(marks), _ptr(dh_last), _ptr(df), _ptr(dx), _ptr(dgate), _ptr(dh0), S, T, C,
+                  DTYPES[f.dtype], _stream(dev))
+    return df, dx, dh0, dgate
+
+
+class GatedScanFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, f, x, h0, gate, cu):
+        ctx.set_materialize_grads(False)
+        y, h_last, marks = _gated_scan_fwd(f, x, h0, gate, cu, True)
+        ctx.save_for_backward(f, x, gate, cu, marks)
+        return y, h_last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh_last):
+        if dy is None and dh_last is None:
+            return None, None, None, None, None
+        f, x, gate, cu, marks = ctx.saved_tensors
+        return (*_gated_scan_bwd(f, x, gate, cu, marks, dy, dh_last, ctx.needs_input_grad), None)
+
+
+def _check_scan(f, x, h0, gate, cu):
+    _same_device("gated_scan", f, x, h0, gate, cu)
+    _dtype_of("gated_scan", DTYPES, f, x, gate)
+    if f.dim() != (3 if cu is None else 2) or x.shape != f.shape or (gate is not None and gate.shape != f.shape):
+        raise ValueError("gated_scan: f, x and gate [B, T, C], or [L, C] with cu_seqlens, of one shape expected, got "
+                         f"{', '.join(str(tuple(t.shape)) for t in (f, x, gate) if t is not None)}")
+    if cu is not None and (cu.dtype != torch.int32 or cu.dim() != 1 or cu.shape[0] < 2 or not cu.is_contiguous()):
+        raise ValueError("gated_scan: cu_seqlens is a contiguous int32 vector of at least 2 row numbers")
+    S, _, C = _scan_sizes(f, cu)
+    if h0 is not None and (tuple(h0.shape) != (S, C) or not h0.is_floating_point()):
+        raise ValueError(f"gated_scan: h0 [{S}, {C}] of a floating type expected, got {tuple(h0.shape)} {h0.dtype}")
+
+
+def gated_scan(f, x, h0=None, gate=None, cu_seqlens=None):
+    """The gated linear recurrence over channels, (y, h_last):
+
+        a_t = sigmoid(f_t),  h_t = a_t h_{t-1} + (1 - a_t) x_t,  y_t = h_t silu(gate_t)
+
+    (y = h without a gate).  f, x, gate: [B, T, C], or [L, C] with ``cu_seqlens`` (int32 row numbers
+    [S + 1] on the device, rising from 0): sequence s has the rows cu_seqlens[s] .. cu_seqlens[s+1] - 1
+    and may have none; rows of no sequence come out as 0.  h0: the states before the first steps
+    ([B, C] or [S, C], zero if absent); h_last: the float32 states after the last ones, h0 for a
+    sequence without steps.  Differentiable in f, x, h0 and gate."""
+    _check_scan(f, x, h0, gate, cu_seqlens)
+    h0 = None if h0 is None else h0.to(torch.float32)
+    if not _wants_grad(f, x, h0, gate):
+        return _gated_scan_fwd(f, x, h0, gate, cu_seqlens, False)[:2]
+    return GatedScanFunction.apply(f, x, h0, gate, cu_seqlens)
+
+
+def gated_step(f, x, h, gate=None):
+    """One step of :func:`gated_scan` for B streams: h [B, C] (float32, contiguous) is advanced in
+    place and y [B, C] returned; f, x, gate [B, C].  One launch and, but for y, no allocation.  For
+    generation: not differentiable."""
+    _same_device("gated_step", f, x, h, gate)
+    code = _dtype_of("gated_step", DTYPES, f, x, gate)
+    if f.dim() != 2 or x.shape != f.shape or h.shape != f.shape or (gate is not None and gate.shape != f.shape):
+        raise ValueError("gated_step: f, x, h and gate [B, C] of one shape expected")
+    if h.dtype != torch.float32 or not h.is_contiguous() or h.data_ptr() % 16:
+        raise ValueError("gated_step: h is a contiguous float32 state, 16-byte aligned")
+    if _wants_grad(f, x, h, gate):
+        raise ValueError("gated_step: not differentiable; call it under torch.no_grad() or use gated_scan")
+    f, x, gate = _rows(f), _rows(x), _rows(gate)
+    y = torch.empty(f.shape, dtype=f.dtype, device=f.device)
+    strides = (ctypes.c_int64 * 3)(f.stride(0), x.stride(0), 0 if gate is None else gate.stride(0))
+    with _on(f.device):
+        _lib.call("csn_gated_step", _ptr(f), _ptr(x), _ptr(gate), strides, _ptr(h), _ptr(y), f.shape[0], f.shape[1],
+                  code, _stream(f.device))
+    return y
+
+
+# ---------------------------------------------------- gated feed-forward product
+HALF_TYPES = (torch.bfloat16, torch.float16)
+
+
+def _ld(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _silu_gated_linear_fwd(x, wg, wu):
+    x, wg, wu = _rows(x), _rows(wg), _rows(wu)
+    R, C, F = x.shape[0], x.shape[1], wg.shape[0]
+    y = torch.empty(R, F, dtype=x.dtype, device=x.device)
+    nb = _lib.load().csn_silu_gated_linear_workspace_bytes(R, C, F, 0)
+    with _on(x.device):
+        ws = _workspace(nb, x.device) if nb else None
+        _lib.call("csn_silu_gated_linear_fwd", _ptr(x), _ld(x), _ptr(wg), _ld(wg), _ptr(wu), _ld(wu), _ptr(y), R, C,
+                  F, DTYPES[x.dtype], _ptr(ws), nb, _stream(x.device))
+    return y
+
+
+def _silu_gated_linear_bwd(x, wg, wu, dy, need):
+    x, wg, wu, dy = _rows(x), _rows(wg), _rows(wu), _rows(dy)
+    R, C, F = x.shape[0], x.shape[1], wg.shape[0]
+    dev, typ = x.device, x.dtype
+    dx = torch.empty(R, C, dtype=typ, device=dev) if need[0] else None
+    dwg = torch.empty(F, C, dtype=typ, device=dev) if need[1] else None
+    dwu = torch.empty(F, C, dtype=typ, device=dev) if need[2] else None
+    nb = _lib.load().csn_silu_gated_linear_workspace_bytes(R, C, F, 1)
+    with _on(dev):
+        ws = _workspace(nb, dev) if nb else None
+        _lib.call("csn_silu_gated_linear_bwd", _ptr(x), _ld(x), _ptr(wg), _ld(wg), _ptr(wu), _ld(wu), _ptr(dy),
+                  _ld(dy), _ptr(dx), _ptr(dwg), _ptr(dwu), R, C, F, DTYPES[typ], _ptr(ws), nb, _stream(dev))
+    return dx, dwg, dwu
+
+
+class SiluGatedLinearFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, wg, wu):
+        ctx.save_for_backward(x, wg, wu)
+        return _silu_gated_linear_fwd(x, wg, wu)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        return _silu_gated_linear_bwd(*ctx.saved_tensors, dy, ctx.needs_input_grad)
+
+
+def silu_gated_linear(x, w_gate, w_up):
+    """silu(x w_gate^T) * (x w_up^T) in one kernel: x [..., C], w_gate and w_up [F, C], result [..., F]
+    (what :func:`silu_gate` makes of the library product of both weights).  bfloat16 or float16 on the
+    tensor cores, sums in float32, one rounding at the end; the backward pass forms both products
+    again instead of keeping them.  float32 layers use ``silu_gate(linear(x, cat))``."""
+    _same_device("silu_gated_linear", x, w_gate, w_up)
+    _dtype_of("silu_gated_linear", HALF_TYPES, x, w_gate, w_up)
+    if x.dim() < 1 or w_gate.dim() != 2 or w_up.shape != w_gate.shape or x.shape[-1] != w_gate.shape[1]:
+        raise ValueError("silu_gated_linear: x [..., C] and w_gate, w_up [F, C] expected, got "
+                         f"{tuple(x.shape)}, {tuple(w_gate.shape)}, {tuple(w_up.shape)}")
+    lead, C, F = x.shape[:-1], w_gate.shape[1], w_gate.shape[0]
+    x2 = x.reshape(lead.numel(), C)
+    y = (SiluGatedLinearFunction.apply(x2, w_gate, w_up) if _wants_grad(x, w_gate, w_up)
+         else _silu_gated_linear_fwd(x2, w_gate, w_up))
+    return y.view(*lead, F)
+
+
+# ------------------------------------------------------------------------ dropout
+def _dropout_add(x, residual, cut, rng):
+    x, residual = _packed(x), _packed(residual)
+    y = torch.empty_like(x)
+    with _on(x.device):
+        _lib.call("csn_dropout_add", _ptr(x), _ptr(residual), _ptr(rng), _ptr(y), x.numel(), cut, DTYPES[x.dtype],
+                  _stream(x.device))
+    return y
+
+
+class DropoutAddFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, cut, rng):
+        ctx.save_for_backward(rng)  # changing rng in place before the backward pass raises there
+        ctx.cut = cut
+        return _dropout_add(x, residual, cut, rng)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        (rng,) = ctx.saved_tensors
+        dx = _dropout_add(dy, None, ctx.cut, rng) if ctx.needs_input_grad[0] else None
+        return dx, (dy if ctx.needs_input_grad[1] else None), None, None
+
+
+def dropout_add(x, residual, p: float, rng):
+    """residual + dropout(x, p) in one kernel each way, without a stored mask (residual None: dropout
+    alone).  rng: int64 [2] on the device, (seed, offset): the mask is a function of these and of the
+    place alone (Philox4x32-10, see csn_dropout_add in include/csn_b200.h), so equal numbers give equal
+    masks and a captured graph draws a new one when the numbers are changed between replays
+    (csn_b200.modules.DropoutAdd counts for itself).  p is taken in steps of 2^-16 and kept places
+    are scaled by one over the probability of being kept."""
+    _same_device("dropout_add", x, residual, rng)
+    _dtype_of("dropout_add", DTYPES, x, residual)
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"dropout_add: x and residual of one shape expected, got {tuple(x.shape)}, "
+                         f"{tuple(residual.shape)}")
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"dropout_add: 0 <= p <= 1 expected, got {p}")
+    if rng.dtype != torch.int64 or tuple(rng.shape) != (2,) or not rng.is_contiguous():
+        raise ValueError("dropout_add: rng is a contiguous int64 tensor (seed, offset)")
+    cut = round(p * 65536)
+    if not _wants_grad(x, residual):
+        return _dropout_add(x, residual, cut, rng)
+    return DropoutAddFunction.apply(x, residual, cut, rng)

@@ -17,6 +17,10 @@ Ops (reference functions they replace, paths relative to the reference root):
 * :func:`cell_step`         -- python/clifford_layer.py:50-115 CliffordTENNCell.forward
 * :func:`ga3_rotor_scan`    -- Cl(3,0) blade-basis form of the two-sided scan
                                (layout include/clifford_configs.cuh:38-51)
+
+The gated recurrent block's ops (:func:`gated_scan`, :func:`gated_step`,
+:func:`silu_gated_linear`, :func:`dropout_add`, in ``gated.py``) take float32 and 16-bit tensors as
+they are instead.
 """
 from __future__ import annotations
 
@@ -29,7 +33,8 @@ from . import _lib
 
 __all__ = ["rotor_scan", "fused_rotor_scan", "fused_rotor_scan_heads", "cayley", "cell_step", "ga3_rotor_scan",
            "rotor_step", "RotorStepGraph", "state_spike", "layer_norm", "ln_conv_silu",
-           "generator_action", "linear", "projection_epilogue", "silu_gate", "column_sum", "BASIS"]
+           "generator_action", "linear", "projection_epilogue", "silu_gate", "column_sum", "gated_scan", "gated_step",
+           "silu_gated_linear", "dropout_add", "BASIS"]
 
 BASIS = {"triu": 0, "ga": 1}
 
@@ -836,5 +841,7 @@ def spatial_generators(in_proj, biv_proj, metric, lambda_sw, gamma_log, D: int):
     return SpatialGeneratorsFunction.apply(in_proj, biv_proj, metric, lambda_sw, gamma_log, D)
 
 
-# torch.ops.csn.* registrations (needs the helpers above; imported last on purpose)
+# the gated recurrent block's ops and the torch.ops.csn.* registrations (both need the helpers
+# above; imported last on purpose)
+from .gated import dropout_add, gated_scan, gated_step, silu_gated_linear  # noqa: E402
 from . import library  # noqa: E402,F401

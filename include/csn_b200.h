@@ -398,6 +398,68 @@ int csn_spatial_generators_bwd(const float* in_proj, const float* biv_proj, cons
                                float* d_metric, float* dlambda_part, float* dgamma_part, int64_t B,
                                int64_t HW, int64_t N, int D, void* stream);
 
+/* ------------------------------------------------------ gated recurrent block */
+/* The operators of a gated recurrent block: the channelwise (diagonal) counterpart of the
+ * matrix recurrence above, the gated feed-forward product, and dropout on the residual path.
+ * The reference has none of them; the recurrence is python/clifford_cl6.py:150-171's
+ * X_t = a M X_{t-1} M^T + (1 - a) S with scalars in place of the matrices, the product is
+ * python/clifford_model.py:42-43's.  Tensors are float32, bfloat16 or float16 as given by
+ * `dtype`; states are float32 and every sum is one. */
+enum csn_dtype { CSN_F32 = 0, CSN_BF16 = 1, CSN_F16 = 2 };
+
+/* a_t = sigmoid(f_t),  h_t = a_t h_{t-1} + (1 - a_t) x_t,  y_t = h_t silu(gate_t) (gate NULL: y = h)
+ * for each of C channels.  Two forms:
+ *   cu_seqlens NULL: S sequences of T steps; f, x, gate element (s, t, c) at
+ *     ptr + s * strides[2i] + t * strides[2i + 1] + c  for i = 0, 1, 2 (strides in elements, a
+ *     host array), y [S, T, C];
+ *   cu_seqlens [S + 1] (device): T rows in all, sequence s has the rows cu[s] .. cu[s+1] - 1
+ *     (none if they are equal); strides[2i] is not used, y [T, C].  Rows of no sequence come
+ *     out as 0.  Borders are cut to 0 .. T and to their order; they must not fall.
+ * h0 [S, C] (NULL = 0), h_last [S, C] (the state after the last step; NULL = not wanted).
+ * marks: NULL, or csn_gated_scan_marks(S, T, C, packed) floats that csn_gated_scan_bwd reads.
+ * f, x, gate aligned to their type; everything else 16-byte aligned. */
+int64_t csn_gated_scan_marks(int64_t S, int64_t T, int64_t C, int packed);
+int csn_gated_scan_fwd(const void* f, const void* x, const void* gate, const int64_t* strides,
+                       const float* h0, const int32_t* cu_seqlens, void* y, float* h_last,
+                       float* marks, int64_t S, int64_t T, int64_t C, int dtype, void* stream);
+
+/* Adjoint of csn_gated_scan_fwd on the same inputs and its marks: dy (NULL = 0; strides[6],
+ * strides[7]) and dh_last [S, C] (NULL = 0) to df, dx, dgate (contiguous, in y's layout) and
+ * dh0 [S, C]; each output may be NULL. */
+int csn_gated_scan_bwd(const void* f, const void* x, const void* gate, const void* dy,
+                       const int64_t* strides, const int32_t* cu_seqlens, const float* marks,
+                       const float* dh_last, void* df, void* dx, void* dgate, float* dh0,
+                       int64_t S, int64_t T, int64_t C, int dtype, void* stream);
+
+/* One step of the same recurrence for B streams, h [B, C] in place (as csn_rotor_step):
+ * f, x, gate element (b, c) at ptr + b * strides[i] + c; y [B, C]. */
+int csn_gated_step(const void* f, const void* x, const void* gate, const int64_t* strides, float* h,
+                   void* y, int64_t B, int64_t C, int dtype, void* stream);
+
+/* y = silu(x w_gate^T) * (x w_up^T) in one pass (csn_silu_gate_fwd on the product that feeds it):
+ * x [R, C], w_gate, w_up [F, C] with row strides ldx, ld_gate, ld_up (elements), y [R, F];
+ * bfloat16 or float16, sums in float32.  The backward forms both products again, writes
+ * dx [R, C], dw_gate, dw_up [F, C] (each may be NULL) from dy [R, F] (row stride ld_dy).
+ * The workspace is required where its size is not 0, and is 16-byte aligned. */
+size_t csn_silu_gated_linear_workspace_bytes(int64_t R, int64_t C, int64_t F, int backward);
+int csn_silu_gated_linear_fwd(const void* x, int64_t ldx, const void* w_gate, int64_t ld_gate,
+                              const void* w_up, int64_t ld_up, void* y, int64_t R, int64_t C,
+                              int64_t F, int dtype, void* workspace, size_t workspace_bytes,
+                              void* stream);
+int csn_silu_gated_linear_bwd(const void* x, int64_t ldx, const void* w_gate, int64_t ld_gate,
+                              const void* w_up, int64_t ld_up, const void* dy, int64_t ld_dy,
+                              void* dx, void* dw_gate, void* dw_up, int64_t R, int64_t C, int64_t F,
+                              int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* y[i] = residual[i] + keep_i x[i] 65536 / (65536 - cut) over n elements (residual NULL: 0), a
+ * dropped place giving residual[i] whatever x[i] is.  keep_i = (r_i >= cut) for 16 random bits
+ * r_i: bits 16 (i % 2) .. of word (i % 8) / 2 of the Philox4x32-10 block with the counter words
+ * (i / 8 low, i / 8 high, offset low, offset high) and the key (seed low, seed high);
+ * rng = {seed, offset} on the device.  The gradient of x is the same call on dy without a
+ * residual.  0 <= cut <= 65536 is the drop probability times 65536. */
+int csn_dropout_add(const void* x, const void* residual, const int64_t* rng, void* y, int64_t n,
+                    int cut, int dtype, void* stream);
+
 /* -------------------------------------------------------------- kernel timing */
 /* Measurement hook with no counterpart in the reference (which times with wall clock,
  * tests/profile_performance.py:41-71).  While enabled, every kernel the library

@@ -1,0 +1,126 @@
+"""The gated recurrent block's entry points without a GPU: sizes of their buffers, and what the C ABI
+refuses before it touches a device."""
+import ctypes
+
+import pytest
+
+NULL = ctypes.c_void_p(0)
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from csn_b200 import _build, _lib
+    _build.build()
+    return _lib.load()
+
+
+def strides(*v):
+    return (ctypes.c_int64 * 8)(*v)
+
+
+def fake(offset=0):
+    """A pointer that is looked at, never followed."""
+    return ctypes.c_void_p(4096 + offset)
+
+
+def refused(lib, rc, code, text):
+    assert rc == code and text in lib.csn_last_error().decode()
+
+
+@pytest.mark.parametrize("packed,S,T", [(0, 1, 1), (0, 3, 64), (0, 5, 129), (1, 4, 1000), (1, 100, 7)])
+def test_marks_hold_every_pass_of_every_sequence(lib, packed, S, T):
+    """Sequence s keeps its states from row0 // 64 + s on: rooms do not overlap and end inside."""
+    import random
+    rng = random.Random(S * T)
+    C = 3
+    have = lib.csn_gated_scan_marks(S, T, C, packed)
+    assert have % C == 0
+    for _ in range(50):
+        if packed:
+            cu = sorted(rng.randint(0, T) for _ in range(S + 1))
+        else:
+            cu = [s * T for s in range(S + 1)]
+        end = 0
+        for s in range(S):
+            first = cu[s] // 64 + s
+            assert first >= end
+            end = first + -(-(cu[s + 1] - cu[s]) // 64)
+            assert end * C <= have
+
+
+def test_marks_of_nothing(lib):
+    assert lib.csn_gated_scan_marks(0, 5, 8, 0) == 0 and lib.csn_gated_scan_marks(5, 5, 0, 0) == 0
+
+
+def test_scan_refuses(lib):
+    p, st = fake(), strides()
+
+    def fwd(f=p, x=p, g=NULL, s=st, h0=NULL, cu=NULL, y=p, S=2, T=4, C=8, dtype=1):
+        return lib.csn_gated_scan_fwd(f, x, g, s, h0, cu, y, NULL, NULL, S, T, C, dtype, NULL)
+
+    refused(lib, fwd(S=-1), 1, "S, T, C >= 0")
+    refused(lib, fwd(T=-1), 1, "S, T, C >= 0")
+    refused(lib, fwd(dtype=3), 2, "dtype")
+    refused(lib, fwd(S=2 ** 31, C=64), 1, "tiles")
+    refused(lib, fwd(f=NULL), 1, "required")
+    refused(lib, fwd(y=NULL), 1, "required")
+    refused(lib, fwd(s=None), 1, "required")
+    refused(lib, fwd(x=fake(1)), 1, "aligned")
+    refused(lib, fwd(h0=fake(8)), 1, "aligned")
+    refused(lib, fwd(y=fake(2)), 1, "aligned")
+    assert fwd(S=0) == 0 and fwd(C=0) == 0
+
+    def bwd(marks=p, dy=p, df=p, dh0=NULL, T=4):
+        return lib.csn_gated_scan_bwd(p, p, NULL, dy, st, NULL, marks, NULL, df, p, NULL, dh0, 2, T, 8, 1, NULL)
+
+    refused(lib, bwd(marks=NULL), 1, "required")
+    refused(lib, bwd(marks=fake(4)), 1, "aligned")
+    refused(lib, bwd(dy=fake(1)), 1, "aligned")
+    refused(lib, bwd(df=fake(2)), 1, "aligned")
+    refused(lib, bwd(dh0=fake(4)), 1, "aligned")
+
+
+def test_step_refuses(lib):
+    p, st = fake(), strides()
+    step = lambda f=p, h=p, y=p, B=2, C=8, dtype=1: lib.csn_gated_step(f, p, NULL, st, h, y, B, C, dtype, NULL)  # noqa: E731
+    refused(lib, step(B=-1), 1, "negative")
+    refused(lib, step(dtype=-1), 2, "dtype")
+    refused(lib, step(h=NULL), 1, "missing")
+    refused(lib, step(h=fake(4)), 1, "misaligned")
+    refused(lib, step(f=fake(1)), 1, "misaligned")
+    assert step(B=0) == 0
+
+
+def test_ffn_refuses(lib):
+    p = fake()
+
+    def fwd(x=p, y=p, R=4, C=8, F=8, dtype=1, ws=p, nb=1 << 30):
+        return lib.csn_silu_gated_linear_fwd(x, C, p, C, p, C, y, R, C, F, dtype, ws, nb, NULL)
+
+    refused(lib, fwd(R=-1), 1, "R, C, F")
+    refused(lib, fwd(F=2 ** 22), 1, "R, C, F")
+    refused(lib, fwd(dtype=0), 2, "dtype")
+    refused(lib, fwd(x=NULL), 1, "missing")
+    refused(lib, fwd(y=fake(2)), 1, "misaligned")
+    assert fwd(R=0) == 0 and fwd(F=0) == 0
+
+    def bwd(dy=p, dx=p, R=4, C=8, F=8, ws=p, nb=1 << 30):
+        return lib.csn_silu_gated_linear_bwd(p, C, p, C, p, C, dy, F, dx, p, p, R, C, F, 1, ws, nb, NULL)
+
+    refused(lib, bwd(dy=NULL), 1, "missing")
+    refused(lib, bwd(dx=fake(2)), 1, "misaligned")
+    refused(lib, bwd(ws=NULL, nb=0), 1, "workspace")
+    refused(lib, bwd(nb=8), 1, "workspace")
+    refused(lib, bwd(C=-2), 1, "R, C, F")
+
+
+def test_dropout_refuses(lib):
+    p = fake()
+    drop = lambda x=p, rng=p, n=8, cut=100, dtype=0: lib.csn_dropout_add(x, NULL, rng, p, n, cut, dtype, NULL)  # noqa: E731
+    refused(lib, drop(n=-1), 1, "n >= 0")
+    refused(lib, drop(cut=65537), 1, "cut")
+    refused(lib, drop(cut=-1), 1, "cut")
+    refused(lib, drop(dtype=7), 2, "dtype")
+    refused(lib, drop(x=fake(4)), 1, "misaligned")
+    refused(lib, drop(rng=NULL), 1, "missing")
+    assert drop(n=0) == 0
