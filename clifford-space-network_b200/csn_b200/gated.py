@@ -188,34 +188,42 @@ def gated_step(f, x, h, gate=None):
 HALF_TYPES = (torch.bfloat16, torch.float16)
 
 
-def _ld(t):
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _tiled(t):
+    """(rows, row stride) of a 16-bit matrix whose rows start on 16 bytes: t itself where its rows do,
+    otherwise a copy with padded rows."""
+    t = _rows(t)
+    n, c = t.shape
+    ld = t.stride(0) if n > 1 else (c + 7) // 8 * 8
+    if t.data_ptr() % 16 == 0 and ld % 8 == 0 and ld >= c:
+        return t, ld
+    ld = (c + 7) // 8 * 8
+    room = torch.empty(n, ld, dtype=t.dtype, device=t.device)
+    room[:, :c].copy_(t)
+    return room, ld
 
 
 def _silu_gated_linear_fwd(x, wg, wu):
-    x, wg, wu = _rows(x), _rows(wg), _rows(wu)
     R, C, F = x.shape[0], x.shape[1], wg.shape[0]
+    (x, ldx), (wg, ldg), (wu, ldu) = _tiled(x), _tiled(wg), _tiled(wu)
     y = torch.empty(R, F, dtype=x.dtype, device=x.device)
-    nb = _lib.load().csn_silu_gated_linear_workspace_bytes(R, C, F, 0)
     with _on(x.device):
-        ws = _workspace(nb, x.device) if nb else None
-        _lib.call("csn_silu_gated_linear_fwd", _ptr(x), _ld(x), _ptr(wg), _ld(wg), _ptr(wu), _ld(wu), _ptr(y), R, C,
-                  F, DTYPES[x.dtype], _ptr(ws), nb, _stream(x.device))
+        _lib.call("csn_silu_gated_linear_fwd", _ptr(x), ldx, _ptr(wg), ldg, _ptr(wu), ldu, _ptr(y), R, C, F,
+                  DTYPES[x.dtype], _stream(x.device))
     return y
 
 
 def _silu_gated_linear_bwd(x, wg, wu, dy, need):
-    x, wg, wu, dy = _rows(x), _rows(wg), _rows(wu), _rows(dy)
     R, C, F = x.shape[0], x.shape[1], wg.shape[0]
+    (x, ldx), (wg, ldg), (wu, ldu), dy = _tiled(x), _tiled(wg), _tiled(wu), _rows(dy)
     dev, typ = x.device, x.dtype
     dx = torch.empty(R, C, dtype=typ, device=dev) if need[0] else None
     dwg = torch.empty(F, C, dtype=typ, device=dev) if need[1] else None
     dwu = torch.empty(F, C, dtype=typ, device=dev) if need[2] else None
-    nb = _lib.load().csn_silu_gated_linear_workspace_bytes(R, C, F, 1)
+    nb = _lib.load().csn_silu_gated_linear_bwd_workspace_bytes(R, C, F)
     with _on(dev):
-        ws = _workspace(nb, dev) if nb else None
-        _lib.call("csn_silu_gated_linear_bwd", _ptr(x), _ld(x), _ptr(wg), _ld(wg), _ptr(wu), _ld(wu), _ptr(dy),
-                  _ld(dy), _ptr(dx), _ptr(dwg), _ptr(dwu), R, C, F, DTYPES[typ], _ptr(ws), nb, _stream(dev))
+        ws = _workspace(nb, dev)
+        _lib.call("csn_silu_gated_linear_bwd", _ptr(x), ldx, _ptr(wg), ldg, _ptr(wu), ldu, _ptr(dy), dy.stride(0),
+                  _ptr(dx), _ptr(dwg), _ptr(dwu), R, C, F, DTYPES[typ], _ptr(ws), nb, _stream(dev))
     return dx, dwg, dwu
 
 

@@ -1,122 +1,676 @@
-// csn_ffn.cu -- the gated feed-forward product of 16-bit tensors and its adjoint.
+// csn_ffn.cu -- the gated feed-forward product of 16-bit tensors and its adjoint, on the tensor cores.
 //
 //   g = x Wg^T,  u = x Wu^T,  y = silu(g) * u          x [R, C], Wg, Wu [F, C], y [R, F]
 // Adjoint, with w = sigmoid(g):
 //   dg = dy u w (1 + g (1 - w)),  du = dy g w,  dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x
 // The backward pass forms g and u again in float32 (they are never stored): keeping them would cost 8 bytes written
 // and read an element in float32, or, rounded to 16 bits, a third of the gradients' precision.
-// dg and du are rounded to the tensors' own type once, as the operands of the products that follow.
+// dg and du are rounded to the tensors' own type once, as the operands of the products that follow.  In float16,
+// whose smallest number is 2^-24, they are first scaled by the power of two that brings the largest |dy| into [1, 2),
+// and the products are scaled back in float32.
+//
+// mm_kernel is one persistent kernel for the four products (Mode).  A CTA owns an SM: one thread feeds a ring of
+// shared-memory stages by TMA, one issues tcgen05.mma into one of two accumulators in tensor memory, and eight warps
+// finish the other accumulator, so that loads, products and epilogue overlap across tiles.  A tile is 128 x BN.  For
+// the gate, BN = 2 FN: FN rows of Wg and the same FN rows of Wu lie one after the other in shared memory as one
+// operand, so g and u of a place sit in one tensor-memory lane and the gate is a per-lane epilogue.  The transposed
+// products read the same row-major tensors with an MN-major operand: nothing is transposed in memory.
+//
+// few_rows_kernel takes R <= 64 rows (generation): there the weights are what is read, so they take the 128-row side
+// of the product (64 rows of Wg and 64 of Wu) and x the narrow side, and a cluster splits C where F alone gives too
+// few CTAs, its partial sums joined through distributed shared memory in a fixed order.
+#include <atomic>
 #include <cstdint>
 
 #include "csn_internal.h"
+#include "csn_tc.cuh"
 #include "csn_types.cuh"
 
 namespace csn {
 namespace {
 
-constexpr int TILE = 64, KT = 16;
+using namespace tc;
 
-// A matrix as products read it: element (i, k) at p + i * si + k * sk
-template <typename T>
-struct Mat2 {
-  const T* p;
-  int64_t si, sk;
+enum Mode { GATE, GATE_BWD, DX, DW };
+
+constexpr int BM = 128, BK = 64;
+constexpr int EPI_WARPS = 8;
+constexpr int THREADS = (EPI_WARPS + 2) * 32;
+constexpr int STAGE_ROW = 80;                       // a lane's 64 bytes, padded against bank conflicts
+constexpr int STAGING = EPI_WARPS * 32 * STAGE_ROW;
+constexpr int SMS = 148;                            // what the work is cut up for
+
+__host__ __device__ constexpr int stage_bytes(int bn) { return (BM + bn) * BK * 2; }
+__host__ __device__ constexpr int stages(int bn) { return bn == 256 ? 4 : 6; }
+constexpr int smem_bytes(int bn) { return stages(bn) * stage_bytes(bn) + STAGING + 1024; }
+
+struct Maps {
+  CUtensorMap a[2], b[2];
 };
 
-// acc += rows of A times rows of B over k, for the 64 x 64 tile at (m0, n0); 256 threads with 4 x 4 values each
-template <typename T>
-__device__ __forceinline__ void tile_product(const Mat2<T>& A, const Mat2<T>& B, int64_t M, int64_t N, int64_t K,
-                                             int64_t m0, int64_t n0, float (*as)[TILE + 4], float (*bs)[TILE + 4],
-                                             float (*acc)[4]) {
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  for (int64_t k0 = 0; k0 < K; k0 += KT) {
-    for (int i = threadIdx.x; i < TILE * KT; i += 256) {
-      // neighbouring threads take neighbouring elements of whichever axis is contiguous
-      const int ak = A.sk == 1 ? i % KT : i / TILE, am = A.sk == 1 ? i / KT : i % TILE;
-      const int bk = B.sk == 1 ? i % KT : i / TILE, bn = B.sk == 1 ? i / KT : i % TILE;
-      as[ak][am] = m0 + am < M && k0 + ak < K ? to_float(A.p[(m0 + am) * A.si + (k0 + ak) * A.sk]) : 0.0f;
-      bs[bk][bn] = n0 + bn < N && k0 + bk < K ? to_float(B.p[(n0 + bn) * B.si + (k0 + bk) * B.sk]) : 0.0f;
+struct Args {
+  int m, n;           // the output's rows and columns (of one half, for DW)
+  int mt, nt;         // its tiles
+  int kb;             // k blocks of one half
+  int halves_m;       // 2 for DW: dWg, then dWu
+  int halves_k;       // 2 for DX: dg Wg, then du Wu
+  int splits, kper;   // k blocks are cut into `splits` ranges of kper
+  void* out[2];       // y; dg, du; dx; dWg, dWu
+  int64_t ldo;
+  const void* dy;
+  int64_t ldy;
+  float* part;        // splits > 1: [splits][halves_m][m][n]
+  const uint32_t* amax;  // float16 backward: bits of the largest |dy|
+};
+
+// the power of two that brings amax into [1, 2), and its inverse; 1 where there is no such
+__device__ __forceinline__ float scale_up(const uint32_t* amax) {
+  if (!amax) return 1.0f;
+  const uint32_t b = *amax;
+  return b == 0 || b >= 0x7f800000u ? 1.0f : __uint_as_float((254u - (b >> 23)) << 23);
+}
+__device__ __forceinline__ float scale_down(const uint32_t* amax) {
+  if (!amax) return 1.0f;
+  const uint32_t b = *amax;
+  return b == 0 || b >= 0x7f800000u ? 1.0f : __uint_as_float((b >> 23) << 23);
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if (BF16) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&v);
+  }
+  __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+template <bool BF16>
+__device__ __forceinline__ float2 unpack2(uint32_t v) {
+  if (BF16) return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v));
+  return __half22float2(*reinterpret_cast<__half2*>(&v));
+}
+
+// A warp's 32 rows x 64 bytes, one row a lane, to memory in whole row pieces (4 lanes a row, 8 rows an access);
+// `vec`: rows start on 16 bytes and hold multiples of 16.
+__device__ __forceinline__ void put_rows(char* stage, int lane, const uint32_t* v, char* out, int64_t row_bytes,
+                                         int rows, int bytes, bool vec) {
+  uint4* mine = reinterpret_cast<uint4*>(stage + lane * STAGE_ROW);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) mine[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+  __syncwarp();
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = i * 8 + lane / 4, at = lane % 4 * 16;
+      if (r < rows && at < bytes)
+        *reinterpret_cast<uint4*>(out + r * row_bytes + at) = *reinterpret_cast<uint4*>(stage + r * STAGE_ROW + at);
     }
-    __syncthreads();
+  } else if (lane * 2 < bytes) {
+    for (int r = 0; r < rows; ++r)
+      *reinterpret_cast<uint16_t*>(out + r * row_bytes + lane * 2) =
+          *reinterpret_cast<uint16_t*>(stage + r * STAGE_ROW + lane * 2);
+  }
+  __syncwarp();
+}
+
+// the same the other way: what lies outside comes as 0
+__device__ __forceinline__ void get_rows(char* stage, int lane, uint32_t* v, const char* in, int64_t row_bytes, int rows,
+                                         int bytes, bool vec) {
+  if (vec) {
+    uint4 got[4];
 #pragma unroll
-    for (int k = 0; k < KT; ++k)
+    for (int i = 0; i < 4; ++i) {
+      const int r = i * 8 + lane / 4, at = lane % 4 * 16;
+      got[i] = r < rows && at < bytes ? *reinterpret_cast<const uint4*>(in + r * row_bytes + at) : make_uint4(0, 0, 0, 0);
+    }
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<uint4*>(stage + (i * 8 + lane / 4) * STAGE_ROW + lane % 4 * 16) = got[i];
+  } else {
+    for (int r = 0; r < 32; ++r)
+      *reinterpret_cast<uint16_t*>(stage + r * STAGE_ROW + lane * 2) =
+          r < rows && lane * 2 < bytes ? *reinterpret_cast<const uint16_t*>(in + r * row_bytes + lane * 2) : (uint16_t)0;
+  }
+  __syncwarp();
+  const uint4* mine = reinterpret_cast<const uint4*>(stage + lane * STAGE_ROW);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(as[k][ty * 4 + i], bs[k][tx * 4 + j], acc[i][j]);
-    __syncthreads();
+  for (int i = 0; i < 4; ++i) {
+    const uint4 q = mine[i];
+    v[4 * i] = q.x, v[4 * i + 1] = q.y, v[4 * i + 2] = q.z, v[4 * i + 3] = q.w;
+  }
+  __syncwarp();
+}
+
+// Tiles are walked in groups of 16 rows of tiles, column by column: the operands of the tiles under way at one time
+// (16 x 9) are read from HBM once and stay in L2.
+struct Tile {
+  int m, n, half, split;
+  __device__ __forceinline__ Tile(const Args& P, int t) {
+    const int per_unit = P.mt * P.nt;
+    const int unit = t / per_unit;
+    t -= unit * per_unit;
+    half = unit % P.halves_m;
+    split = unit / P.halves_m;
+    const int per = 16 * P.nt, g = t / per, rem = t - g * per;
+    const int gm = min(16, P.mt - g * 16);
+    m = g * 16 + rem % gm;
+    n = rem / gm;
+  }
+};
+
+template <Mode MODE, bool BF16, int BN>
+__global__ void __launch_bounds__(THREADS, 1) mm_kernel(const __grid_constant__ Maps maps, const Args P) {
+  constexpr int ST = stages(BN), SB = stage_bytes(BN);
+  constexpr bool A_MN = MODE == DW, B_MN = MODE == DX || MODE == DW;
+  constexpr int FN = BN / 2;
+  extern __shared__ char raw[];
+  __shared__ uint64_t full[ST], empty[ST], acc_full[2], acc_empty[2], drained;
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile uint32_t gave_up;
+  char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tiles = P.mt * P.nt * P.halves_m * P.splits;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ST; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], EPI_WARPS);
+    mbar_init(&drained, 1);
+    mbar_init_fence();
+    gave_up = 0;
+  }
+  if (warp == EPI_WARPS) tmem_alloc<2 * BN>(&tmem_slot);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_slot;
+
+  if (warp == EPI_WARPS) {
+    if (lane == 0) {  // TMA
+      int it = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        const Tile T(P, t);
+        const int k0 = T.split * P.kper, k1 = min(k0 + P.kper, P.kb * P.halves_k);
+        for (int k = k0; k < k1; ++k, ++it) {
+          const int s = it % ST;
+          if (!(ok = mbar_wait(&empty[s], (it / ST + 1) & 1, &gave_up))) break;
+          mbar_expect(&full[s], SB);
+          char* a = smem + s * SB;
+          char* b = a + BM * BK * 2;
+          if (MODE == GATE || MODE == GATE_BWD) {
+            tma_load(a, &maps.a[0], k * BK, T.m * BM, &full[s]);
+            tma_load(b, &maps.b[0], k * BK, T.n * FN, &full[s]);
+            tma_load(b + FN * BK * 2, &maps.b[1], k * BK, T.n * FN, &full[s]);
+          } else if (MODE == DX) {
+            const int h = k >= P.kb, kk = (k - h * P.kb) * BK;
+            tma_load(a, &maps.a[h], kk, T.m * BM, &full[s]);
+#pragma unroll
+            for (int j = 0; j < BN / 64; ++j) tma_load(b + j * 8192, &maps.b[h], T.n * BN + j * 64, kk, &full[s]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < BM / 64; ++j) tma_load(a + j * 8192, &maps.a[T.half], T.m * BM + j * 64, k * BK, &full[s]);
+#pragma unroll
+            for (int j = 0; j < BN / 64; ++j) tma_load(b + j * 8192, &maps.b[0], T.n * BN + j * 64, k * BK, &full[s]);
+          }
+        }
+      }
+      if (!ok)  // copies in flight end before the shared memory does
+        for (int j = it > ST ? it - ST : 0; j < it; ++j)
+          for (uint32_t i = 0; i < POLLS && !mbar_try(&full[j % ST], (j / ST) & 1); ++i) {}
+    }
+  } else if (warp == EPI_WARPS + 1) {
+    if (lane == 0) {  // MMA
+      constexpr uint32_t IDESC = instruction(BF16, A_MN, B_MN, BM, BN);
+      int it = 0, n = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++n) {
+        const Tile T(P, t);
+        const int k0 = T.split * P.kper, k1 = min(k0 + P.kper, P.kb * P.halves_k);
+        const uint32_t d = tmem + (n & 1) * BN;
+        if (!(ok = mbar_wait(&acc_empty[n & 1], ((n >> 1) + 1) & 1, &gave_up))) break;
+        fence_after();
+        for (int k = k0; k < k1; ++k, ++it) {
+          const int s = it % ST;
+          if (!(ok = mbar_wait(&full[s], (it / ST) & 1, &gave_up))) break;
+          fence_after();
+          const uint32_t a = smem_addr(smem + s * SB), b = a + BM * BK * 2;
+          const uint64_t ad = operand(a, 8192), bd = operand(b, 8192);
+#pragma unroll
+          for (int j = 0; j < BK / 16; ++j)
+            mma(d, ad + j * (A_MN ? 2048 >> 4 : 32 >> 4), bd + j * (B_MN ? 2048 >> 4 : 32 >> 4), IDESC, k > k0 || j > 0);
+          mma_commit(&empty[s]);
+        }
+        if (ok) mma_commit(&acc_full[n & 1]);
+      }
+      if (!ok) {
+        mma_commit(&drained);
+        for (uint32_t i = 0; i < POLLS && !mbar_try(&drained, 0); ++i) {}
+      }
+    }
+  } else {
+    // epilogue: warp w reads the tensor-memory lanes of quarter w % 4 and half of the columns
+    char* stage = smem + ST * SB + warp * 32 * STAGE_ROW;
+    const int quarter = warp % 4, side = warp / 4;
+    const float up = MODE == GATE_BWD ? scale_up(P.amax) : 1.0f;
+    const float down = MODE == DX || MODE == DW ? scale_down(P.amax) : 1.0f;
+    int n = 0;
+    for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++n) {
+      const Tile T(P, t);
+      const uint32_t d = tmem + (n & 1) * BN + ((uint32_t)(quarter * 32) << 16);
+      const int64_t row0 = (int64_t)T.m * BM + quarter * 32;
+      const int rows = (int)min((int64_t)32, P.m - row0);
+      const bool ok = mbar_wait(&acc_full[n & 1], (n >> 1) & 1, &gave_up);
+      __syncwarp();
+      fence_after();
+      if (MODE == GATE || MODE == GATE_BWD) {
+        const bool vec = P.ldo % 8 == 0;
+        const bool vec_dy = MODE == GATE_BWD && P.ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(P.dy) & 15) == 0 && P.n % 8 == 0;
+#pragma unroll 1
+        for (int c = side * (FN / 2); c < (side + 1) * (FN / 2); c += 32) {
+          const int64_t col = (int64_t)T.n * FN + c;
+          const int bytes = (int)min((int64_t)32, P.n - col) * 2;
+          if (rows <= 0 || bytes <= 0) continue;
+          uint32_t dy[16];
+          if (MODE == GATE_BWD)
+            get_rows(stage, lane, dy, static_cast<const char*>(P.dy) + (row0 * P.ldy + col) * 2, P.ldy * 2, rows, bytes,
+                     vec_dy);
+          float g[32], u[32];
+          tmem_load32(d + c, g);
+          tmem_load32(d + FN + c, u);
+          tmem_load_wait();
+          if (!ok)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) g[i] = __int_as_float(0x7fffffff);
+          uint32_t o0[16], o1[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float r0[2], r1[2];
+            const float2 dv = MODE == GATE_BWD ? unpack2<BF16>(dy[i]) : make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const float gv = g[2 * i + j], uv = u[2 * i + j];
+              const float w = __fdividef(1.0f, 1.0f + __expf(-gv));
+              if (MODE == GATE) {
+                r0[j] = gv * w * uv;
+              } else {
+                const float e = (j ? dv.y : dv.x) * up;
+                r0[j] = e * uv * (w * fmaf(gv, 1.0f - w, 1.0f));
+                r1[j] = e * gv * w;
+              }
+            }
+            o0[i] = pack2<BF16>(r0[0], r0[1]);
+            if (MODE == GATE_BWD) o1[i] = pack2<BF16>(r1[0], r1[1]);
+          }
+          const int64_t at = (row0 * P.ldo + col) * 2;
+          put_rows(stage, lane, o0, static_cast<char*>(P.out[0]) + at, P.ldo * 2, rows, bytes, vec);
+          if (MODE == GATE_BWD) put_rows(stage, lane, o1, static_cast<char*>(P.out[1]) + at, P.ldo * 2, rows, bytes, vec);
+        }
+      } else {
+#pragma unroll 1
+        for (int c = side * (BN / 2); c < (side + 1) * (BN / 2); c += 32) {
+          const int64_t col = (int64_t)T.n * BN + c;
+          const int cols = (int)min((int64_t)32, P.n - col);
+          if (rows <= 0 || cols <= 0) continue;
+          float v[32];
+          tmem_load32(d + c, v);
+          tmem_load_wait();
+          if (!ok)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = __int_as_float(0x7fffffff);
+          if (P.splits > 1) {
+            char* out = reinterpret_cast<char*>(P.part) +
+                        ((((int64_t)T.split * P.halves_m + T.half) * P.m + row0) * P.n + col) * 4;
+            put_rows(stage, lane, reinterpret_cast<uint32_t*>(v), out, (int64_t)P.n * 4, rows, min(cols, 16) * 4, P.n % 4 == 0);
+            if (cols > 16)
+              put_rows(stage, lane, reinterpret_cast<uint32_t*>(v + 16), out + 64, (int64_t)P.n * 4, rows, (cols - 16) * 4,
+                       P.n % 4 == 0);
+          } else if (void* to = T.half ? P.out[1] : P.out[0]) {
+            uint32_t o[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = pack2<BF16>(v[2 * i] * down, v[2 * i + 1] * down);
+            put_rows(stage, lane, o, static_cast<char*>(to) + (row0 * P.ldo + col) * 2, P.ldo * 2, rows, cols * 2,
+                     P.ldo % 8 == 0);
+          }
+        }
+      }
+      fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acc_empty[n & 1]);
+    }
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (warp == EPI_WARPS) tmem_free<2 * BN>(tmem);
+}
+
+// sums of the k ranges, in their order
+template <bool BF16>
+__global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ part, void* out, int64_t n, int64_t stride,
+                                                   int splits, const uint32_t* amax) {
+  const float down = scale_down(amax);
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+    float v = 0.0f;
+    for (int s = 0; s < splits; ++s) v += part[s * stride + i];
+    v *= down;
+    if (BF16) static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(v);
+    else static_cast<__half*>(out)[i] = __float2half_rn(v);
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) gate_kernel(Mat2<T> x, Mat2<T> wg, Mat2<T> wu, const T* dy, int64_t ldy, T* y,
-                                                   T* dg, T* du, int64_t R, int64_t C, int64_t F) {
-  __shared__ float as[KT][TILE + 4], bs[KT][TILE + 4];
-  const int64_t m0 = (int64_t)blockIdx.y * TILE, n0 = (int64_t)blockIdx.x * TILE;
-  float g[4][4] = {}, u[4][4] = {};
-  tile_product(x, wg, R, F, C, m0, n0, as, bs, g);
-  tile_product(x, wu, R, F, C, m0, n0, as, bs, u);
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int64_t r = m0 + threadIdx.x / 16 * 4 + i, c = n0 + threadIdx.x % 16 * 4 + j;
-      if (r >= R || c >= F) continue;
-      float w, wn;
-      sigmoid_pair(g[i][j], w, wn);
-      if (y) y[r * F + c] = from_float<T>(g[i][j] * w * u[i][j]);
-      if (dy) {
-        const float d = to_float(dy[r * ldy + c]);
-        dg[r * F + c] = from_float<T>(d * u[i][j] * (w * fmaf(g[i][j], wn, 1.0f)));
-        du[r * F + c] = from_float<T>(d * g[i][j] * w);
+// bits of the largest |dy| (0 before): a maximum does not depend on the order
+__global__ void __launch_bounds__(256) amax_kernel(const __half* __restrict__ dy, int64_t ld, int64_t R, int64_t F,
+                                                   uint32_t* amax) {
+  float m = 0.0f;
+  for (int64_t r = blockIdx.x; r < R; r += gridDim.x)
+    for (int64_t c = threadIdx.x; c < F; c += 256) m = fmaxf(m, fabsf(__half2float(dy[r * ld + c])));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if ((threadIdx.x & 31) == 0) atomicMax(amax, __float_as_uint(m));
+}
+
+// ------------------------------------------------------------------------ few rows
+constexpr int FEW = 64, HALF_ROWS = 64, FEW_THREADS = 6 * 32;
+
+__host__ __device__ constexpr int few_stage(int nr) { return (2 * HALF_ROWS + nr) * BK * 2; }
+__host__ __device__ constexpr int few_stages(int nr) { return nr == 64 ? 4 : 5; }
+constexpr int few_smem(int nr) { return few_stages(nr) * few_stage(nr) + 1024; }
+
+struct FewArgs {
+  int R, F, kb, kper;
+  void* y;
+};
+
+__device__ __forceinline__ float peer_float(uint32_t addr, uint32_t rank) {
+  uint32_t a;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <bool BF16, int NR>
+__global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(const __grid_constant__ Maps maps, const FewArgs P) {
+  constexpr int ST = few_stages(NR), SB = few_stage(NR), COLS = NR < 32 ? 32 : NR;
+  extern __shared__ char raw[];
+  __shared__ uint64_t full[ST], empty[ST], done;
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile uint32_t gave_up;
+  char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t rank, ranks;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
+  const int f0 = blockIdx.x / ranks * HALF_ROWS;
+  const int k0 = rank * P.kper, k1 = min(k0 + P.kper, P.kb);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ST; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+    mbar_init(&done, 1);
+    mbar_init_fence();
+    gave_up = 0;
+  }
+  if (warp == 4) tmem_alloc<COLS>(&tmem_slot);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_slot;
+  float* sums = reinterpret_cast<float*>(smem);  // [128][NR + 1], in the stages once they are done with
+
+  bool ok = true;
+  if (warp == 4) {
+    if (lane == 0) {
+      int k = k0;
+      for (; k < k1; ++k) {
+        const int it = k - k0, s = it % ST;
+        if (!mbar_wait(&empty[s], (it / ST + 1) & 1, &gave_up)) break;
+        mbar_expect(&full[s], SB);
+        char* a = smem + s * SB;
+        tma_load(a, &maps.a[0], k * BK, f0, &full[s]);
+        tma_load(a + HALF_ROWS * BK * 2, &maps.a[1], k * BK, f0, &full[s]);
+        tma_load(a + 2 * HALF_ROWS * BK * 2, &maps.b[0], k * BK, 0, &full[s]);
       }
+      if (k < k1)
+        for (int j = max(0, k - k0 - ST); j < k - k0; ++j)
+          for (uint32_t i = 0; i < POLLS && !mbar_try(&full[j % ST], (j / ST) & 1); ++i) {}
     }
-}
-
-// out[m, n] = sum_k A(m, k) B(n, k) + A2(m, k) B2(n, k)
-template <typename T>
-__global__ void __launch_bounds__(256) product_kernel(Mat2<T> a, Mat2<T> b, Mat2<T> a2, Mat2<T> b2, T* out, int64_t M,
-                                                      int64_t N, int64_t K) {
-  __shared__ float as[KT][TILE + 4], bs[KT][TILE + 4];
-  const int64_t m0 = (int64_t)blockIdx.y * TILE, n0 = (int64_t)blockIdx.x * TILE;
-  float acc[4][4] = {};
-  tile_product(a, b, M, N, K, m0, n0, as, bs, acc);
-  if (a2.p) tile_product(a2, b2, M, N, K, m0, n0, as, bs, acc);
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int64_t r = m0 + threadIdx.x / 16 * 4 + i, c = n0 + threadIdx.x % 16 * 4 + j;
-      if (r < M && c < N) out[r * N + c] = from_float<T>(acc[i][j]);
+  } else if (warp == 5) {
+    if (lane == 0) {
+      constexpr uint32_t IDESC = instruction(BF16, false, false, 128, NR);
+      for (int k = k0; k < k1; ++k) {
+        const int it = k - k0, s = it % ST;
+        if (!mbar_wait(&full[s], (it / ST) & 1, &gave_up)) break;
+        fence_after();
+        const uint32_t a = smem_addr(smem + s * SB);
+        const uint64_t ad = operand(a, 0), bd = operand(a + 2 * HALF_ROWS * BK * 2, 0);
+#pragma unroll
+        for (int j = 0; j < BK / 16; ++j) mma(tmem, ad + j * 2, bd + j * 2, IDESC, k > k0 || j > 0);
+        mma_commit(&empty[s]);
+      }
+      mma_commit(&done);
     }
+  } else {
+    // `done` counts the products issued: complete, unless a wait gave up
+    ok = mbar_wait(&done, 0, &gave_up);
+    __syncwarp();
+    fence_after();
+    const int row = warp * 32 + lane;
+#pragma unroll
+    for (int c = 0; c < NR; c += 16) {
+      uint32_t r[16];
+      asm volatile(
+          "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+          : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+            "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+          : "r"(tmem + ((uint32_t)(warp * 32) << 16) + c));
+      tmem_load_wait();
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        sums[row * (NR + 1) + c + i] = ok && !gave_up ? __uint_as_float(r[i]) : __int_as_float(0x7fffffff);
+    }
+    fence_before();
+  }
+  __syncthreads();
+  cluster_sync();
+  const uint32_t base = smem_addr(sums);
+  for (int i = rank * FEW_THREADS + threadIdx.x; i < P.R * HALF_ROWS; i += ranks * FEW_THREADS) {
+    const int r = i / HALF_ROWS, f = i % HALF_ROWS;
+    if (f0 + f >= P.F) continue;
+    float g = 0.0f, u = 0.0f;
+    for (uint32_t k = 0; k < ranks; ++k) {
+      g += peer_float(base + (f * (NR + 1) + r) * 4, k);
+      u += peer_float(base + ((f + HALF_ROWS) * (NR + 1) + r) * 4, k);
+    }
+    float w, wn;
+    sigmoid_pair(g, w, wn);
+    const float v = g * w * u;
+    const int64_t at = (int64_t)r * P.F + f0 + f;
+    if (BF16) static_cast<__nv_bfloat16*>(P.y)[at] = __float2bfloat16_rn(v);
+    else static_cast<__half*>(P.y)[at] = __float2half_rn(v);
+  }
+  cluster_sync();  // the peers have read this CTA's sums
+  if (warp == 4) {
+    fence_after();
+    tmem_free<COLS>(tmem);
+  }
 }
 
-dim3 tiles(int64_t M, int64_t N) { return dim3((unsigned)((N + TILE - 1) / TILE), (unsigned)((M + TILE - 1) / TILE)); }
+// ---------------------------------------------------------------------------- host
+int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to; }
 
-template <typename T>
-void forward(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void* wu, int64_t ldu, void* y, int64_t R,
-             int64_t C, int64_t F, cudaStream_t st) {
-  gate_kernel<T><<<tiles(R, F), 256, 0, st>>>({static_cast<const T*>(x), ldx, 1}, {static_cast<const T*>(wg), ldg, 1},
-                                              {static_cast<const T*>(wu), ldu, 1}, nullptr, 0, static_cast<T*>(y),
-                                              nullptr, nullptr, R, C, F);
+// How a product of m x n over k blocks is cut up.  Narrow tiles where 256 columns would leave SMs idle (or the
+// columns are few); and where even those leave more than half of the SMs idle, ranges of k of at least 4 blocks.
+struct Plan {
+  int bn, mt, nt, splits, kper;
+  Plan(int64_t m, int64_t n, int64_t blocks, int halves, bool gate) {
+    mt = (int)up(m, BM);
+    const int wide = gate ? 128 : 256;  // columns of a 256-wide tile
+    bn = n <= wide / 2 || mt * up(n, wide) * halves < SMS ? 128 : 256;
+    nt = (int)up(n, gate ? bn / 2 : bn);
+    splits = 1;
+    const int64_t tiles = (int64_t)mt * nt * halves;
+    if (!gate && tiles * 2 <= SMS) {
+      int64_t s = SMS / tiles;
+      s = s < blocks / 4 ? s : blocks / 4;
+      splits = s > 1 ? (int)s : 1;
+    }
+    kper = (int)up(blocks, splits);
+    splits = (int)up(blocks, kper);
+  }
+};
+
+size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// the backward pass's scratch: dg, du [R, ld], the largest |dy|, and the partial sums of split products
+struct Scratch {
+  int64_t ld;
+  size_t dg, du, amax, part, total;
+  Scratch(int64_t R, int64_t C, int64_t F) {
+    ld = up(F, 8) * 8;
+    const Plan px(R, C, 2 * up(F, BK), 1, false), pw(F, C, up(R, BK), 2, false);
+    const size_t sx = px.splits > 1 ? (size_t)px.splits * R * C * 4 : 0;
+    const size_t sw = pw.splits > 1 ? (size_t)pw.splits * 2 * F * C * 4 : 0;
+    dg = 0;
+    du = align256((size_t)R * ld * 2);
+    amax = 2 * du;
+    part = amax + 256;
+    total = part + align256(sx > sw ? sx : sw);
+  }
+};
+
+template <typename K>
+cudaError_t allow_smem(K kernel, int bytes) {
+  return cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
-template <typename T>
-void backward(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void* wu, int64_t ldu, const void* dy,
-              int64_t ldy, void* dx, void* dwg, void* dwu, int64_t R, int64_t C, int64_t F, void* ws, cudaStream_t st) {
-  const T *xt = static_cast<const T*>(x), *gt = static_cast<const T*>(wg), *ut = static_cast<const T*>(wu);
-  T* dg = static_cast<T*>(ws);
-  T* du = dg + R * F;
-  gate_kernel<T><<<tiles(R, F), 256, 0, st>>>({xt, ldx, 1}, {gt, ldg, 1}, {ut, ldu, 1}, static_cast<const T*>(dy), ldy,
-                                              nullptr, dg, du, R, C, F);
-  if (dx)
-    product_kernel<T><<<tiles(R, C), 256, 0, st>>>({dg, F, 1}, {gt, 1, ldg}, {du, F, 1}, {ut, 1, ldu},
-                                                   static_cast<T*>(dx), R, C, F);
-  const Mat2<T> none = {nullptr, 0, 0};
-  if (dwg) product_kernel<T><<<tiles(F, C), 256, 0, st>>>({dg, 1, F}, {xt, 1, ldx}, none, none, static_cast<T*>(dwg), F, C, R);
-  if (dwu) product_kernel<T><<<tiles(F, C), 256, 0, st>>>({du, 1, F}, {xt, 1, ldx}, none, none, static_cast<T*>(dwu), F, C, R);
+template <Mode MODE, bool BF16, int BN>
+int run_mm(const Maps& maps, const Args& P, cudaStream_t st, const char* who) {
+  if (cudaError_t e = allow_smem(mm_kernel<MODE, BF16, BN>, smem_bytes(BN))) return set_cuda_error(e, who);
+  const int64_t tiles = (int64_t)P.mt * P.nt * P.halves_m * P.splits;
+  const unsigned grid = (unsigned)(tiles < sm_count() ? tiles : sm_count());
+  mm_kernel<MODE, BF16, BN><<<grid, THREADS, smem_bytes(BN), st>>>(maps, P);
+  return check_launch(who);
+}
+
+template <bool BF16>
+int run_gate(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void* wu, int64_t ldu, const void* dy,
+             int64_t ldy, void* o0, void* o1, int64_t ldo, const uint32_t* amax, int64_t R, int64_t C, int64_t F,
+             cudaStream_t st, const char* who) {
+  const Plan p(R, F, up(C, BK), 1, true);
+  Maps maps;
+  if (!make_map(&maps.a[0], x, R, C, ldx, BM, BF16) || !make_map(&maps.b[0], wg, F, C, ldg, p.bn / 2, BF16) ||
+      !make_map(&maps.b[1], wu, F, C, ldu, p.bn / 2, BF16))
+    return set_error(CSN_ERR_CUDA, "silu_gated_linear: cuTensorMapEncodeTiled");
+  maps.a[1] = maps.a[0];
+  Args P = {};
+  P.m = (int)R, P.n = (int)F, P.mt = p.mt, P.nt = p.nt, P.kb = (int)up(C, BK), P.halves_m = P.halves_k = 1;
+  P.splits = p.splits, P.kper = p.kper, P.out[0] = o0, P.out[1] = o1, P.ldo = ldo, P.dy = dy, P.ldy = ldy, P.amax = amax;
+  if (dy) return p.bn == 256 ? run_mm<GATE_BWD, BF16, 256>(maps, P, st, who) : run_mm<GATE_BWD, BF16, 128>(maps, P, st, who);
+  return p.bn == 256 ? run_mm<GATE, BF16, 256>(maps, P, st, who) : run_mm<GATE, BF16, 128>(maps, P, st, who);
+}
+
+template <bool BF16, int NR>
+int run_few(const Maps& maps, const FewArgs& P, int ranks, cudaStream_t st, const char* who) {
+  if (cudaError_t e = allow_smem(few_rows_kernel<BF16, NR>, few_smem(NR))) return set_cuda_error(e, who);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(up(P.F, HALF_ROWS) * ranks));
+  cfg.blockDim = dim3(FEW_THREADS);
+  cfg.dynamicSmemBytes = few_smem(NR);
+  cfg.stream = st;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = ranks, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  if (cudaError_t e = cudaLaunchKernelEx(&cfg, few_rows_kernel<BF16, NR>, maps, P)) return set_cuda_error(e, who);
+  return check_launch(who);
+}
+
+template <bool BF16>
+int forward(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void* wu, int64_t ldu, void* y, int64_t R,
+            int64_t C, int64_t F, cudaStream_t st) {
+  const char* who = "csn_silu_gated_linear_fwd";
+  if (R > FEW) return run_gate<BF16>(x, ldx, wg, ldg, wu, ldu, nullptr, 0, y, nullptr, F, nullptr, R, C, F, st, who);
+  const int nr = R <= 16 ? 16 : R <= 32 ? 32 : 64;
+  Maps maps;
+  if (!make_map(&maps.a[0], wg, F, C, ldg, HALF_ROWS, BF16) || !make_map(&maps.a[1], wu, F, C, ldu, HALF_ROWS, BF16) ||
+      !make_map(&maps.b[0], x, R, C, ldx, nr, BF16))
+    return set_error(CSN_ERR_CUDA, "silu_gated_linear: cuTensorMapEncodeTiled");
+  maps.b[1] = maps.b[0];
+  FewArgs P = {(int)R, (int)F, (int)up(C, BK), 0, y};
+  // two CTAs fit on an SM: ranges of C (at least 4 blocks each) until there are as many
+  int ranks = 1;
+  while (ranks < 8 && up(F, HALF_ROWS) * ranks * 2 <= 2 * SMS && P.kb >= ranks * 2 * 4) ranks *= 2;
+  P.kper = (int)up(P.kb, ranks);
+  return nr == 16 ? run_few<BF16, 16>(maps, P, ranks, st, who)
+                  : nr == 32 ? run_few<BF16, 32>(maps, P, ranks, st, who) : run_few<BF16, 64>(maps, P, ranks, st, who);
+}
+
+template <Mode MODE, bool BF16>
+int run_product(const Maps& maps, Args P, int64_t blocks, const Plan& p, float* part, int64_t outs, cudaStream_t st,
+                const char* who) {
+  P.mt = p.mt, P.nt = p.nt, P.kb = (int)(blocks / P.halves_k), P.splits = p.splits, P.kper = p.kper, P.part = part;
+  int rc = p.bn == 256 ? run_mm<MODE, BF16, 256>(maps, P, st, who) : run_mm<MODE, BF16, 128>(maps, P, st, who);
+  if (rc || p.splits == 1) return rc;
+  const int64_t n = (int64_t)P.m * P.n, ctas = up(n, 256);
+  for (int h = 0; h < outs; ++h)
+    if (P.out[h])
+      join_kernel<BF16><<<(unsigned)(ctas < 8 * SMS ? ctas : 8 * SMS), 256, 0, st>>>(part + h * n, P.out[h], n, outs * n,
+                                                                                     p.splits, P.amax);
+  return check_launch(who);
+}
+
+template <bool BF16>
+int backward(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void* wu, int64_t ldu, const void* dy,
+             int64_t ldy, void* dx, void* dwg, void* dwu, int64_t R, int64_t C, int64_t F, void* ws, cudaStream_t st) {
+  const char* who = "csn_silu_gated_linear_bwd";
+  const Scratch s(R, C, F);
+  char* base = static_cast<char*>(ws);
+  void *dg = base + s.dg, *du = base + s.du;
+  float* part = reinterpret_cast<float*>(base + s.part);
+  uint32_t* amax = nullptr;
+  if (!BF16) {
+    amax = reinterpret_cast<uint32_t*>(base + s.amax);
+    if (cudaError_t e = cudaMemsetAsync(amax, 0, 4, st)) return set_cuda_error(e, who);
+    amax_kernel<<<(unsigned)(R < 8 * SMS ? R : 8 * SMS), 256, 0, st>>>(static_cast<const __half*>(dy), ldy, R, F, amax);
+  }
+  if (int rc = run_gate<BF16>(x, ldx, wg, ldg, wu, ldu, dy, ldy, dg, du, s.ld, amax, R, C, F, st, who)) return rc;
+  if (dx) {
+    const Plan p(R, C, 2 * up(F, BK), 1, false);
+    Maps maps;
+    if (!make_map(&maps.a[0], dg, R, F, s.ld, BM, BF16) || !make_map(&maps.a[1], du, R, F, s.ld, BM, BF16) ||
+        !make_map(&maps.b[0], wg, F, C, ldg, BK, BF16) || !make_map(&maps.b[1], wu, F, C, ldu, BK, BF16))
+      return set_error(CSN_ERR_CUDA, "silu_gated_linear: cuTensorMapEncodeTiled");
+    Args P = {};
+    P.m = (int)R, P.n = (int)C, P.halves_m = 1, P.halves_k = 2, P.out[0] = dx, P.ldo = C, P.amax = amax;
+    if (int rc = run_product<DX, BF16>(maps, P, 2 * up(F, BK), p, part, 1, st, who)) return rc;
+  }
+  if (dwg || dwu) {
+    const Plan p(F, C, up(R, BK), 2, false);
+    Maps maps;
+    if (!make_map(&maps.a[0], dg, R, F, s.ld, BK, BF16) || !make_map(&maps.a[1], du, R, F, s.ld, BK, BF16) ||
+        !make_map(&maps.b[0], x, R, C, ldx, BK, BF16))
+      return set_error(CSN_ERR_CUDA, "silu_gated_linear: cuTensorMapEncodeTiled");
+    maps.b[1] = maps.b[0];
+    Args P = {};
+    P.m = (int)F, P.n = (int)C, P.halves_m = 2, P.halves_k = 1, P.out[0] = dwg, P.out[1] = dwu, P.ldo = C, P.amax = amax;
+    if (int rc = run_product<DW, BF16>(maps, P, up(R, BK), p, part, 2, st, who)) return rc;
+  }
+  return CSN_OK;
 }
 
 bool al16b(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// what TMA reads in place: rows that start on 16 bytes
+bool tiled(const void* p, int64_t rows, int64_t cols, int64_t ld) {
+  return p && al16b(p) && ld % 8 == 0 && (rows == 1 || ld >= cols) && ld > 0 && ld < ((int64_t)1 << 38);
+}
+
 int check_ffn(const char* who, int64_t R, int64_t C, int64_t F, int dtype) {
-  // rows, channels and hidden units are 32-bit coordinates of the tiles
+  // tile coordinates and counts are 32-bit
   if (R < 0 || C < 0 || F < 0 || R > (1 << 21) || C > (1 << 21) || F > (1 << 21)) return set_error(CSN_ERR_INVALID, who);
   if (dtype != CSN_BF16 && dtype != CSN_F16) return set_error(CSN_ERR_UNSUPPORTED, who);
   return CSN_OK;
@@ -127,30 +681,29 @@ int check_ffn(const char* who, int64_t R, int64_t C, int64_t F, int dtype) {
 
 using namespace csn;
 
-extern "C" size_t csn_silu_gated_linear_workspace_bytes(int64_t R, int64_t C, int64_t F, int backward) {
-  if (R <= 0 || C <= 0 || F <= 0) return 0;
-  return backward ? (size_t)R * F * 4 : 0;
+extern "C" size_t csn_silu_gated_linear_bwd_workspace_bytes(int64_t R, int64_t C, int64_t F) {
+  if (R <= 0 || C <= 0 || F <= 0 || R > (1 << 21) || C > (1 << 21) || F > (1 << 21)) return 0;
+  return Scratch(R, C, F).total;
 }
 
 extern "C" int csn_silu_gated_linear_fwd(const void* x, int64_t ldx, const void* w_gate, int64_t ld_gate,
                                          const void* w_up, int64_t ld_up, void* y, int64_t R, int64_t C, int64_t F,
-                                         int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+                                         int dtype, void* stream) {
   if (int rc = check_ffn("csn_silu_gated_linear_fwd: needs 0 <= R, C, F <= 2^21 and dtype bfloat16 or float16", R, C, F, dtype))
     return rc;
   if (R == 0 || F == 0) return CSN_OK;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (!y || (C > 0 && (!x || !w_gate || !w_up)) || !al16b(y))
-    return set_error(CSN_ERR_INVALID, "csn_silu_gated_linear_fwd: missing or misaligned pointer");
-  if (C == 0)
-    return cudaMemsetAsync(y, 0, (size_t)R * F * 2, st) == cudaSuccess
-               ? CSN_OK : set_error(CSN_ERR_CUDA, "csn_silu_gated_linear_fwd: cudaMemsetAsync");
-  const size_t need = csn_silu_gated_linear_workspace_bytes(R, C, F, 0);
-  if (need && (!workspace || !al16b(workspace) || workspace_bytes < need))
-    return set_error(CSN_ERR_INVALID, "csn_silu_gated_linear_fwd: workspace smaller than csn_silu_gated_linear_workspace_bytes");
+  if (!y || !al16b(y)) return set_error(CSN_ERR_INVALID, "csn_silu_gated_linear_fwd: y missing or misaligned");
+  if (C == 0) {
+    const cudaError_t e = cudaMemsetAsync(y, 0, (size_t)R * F * 2, st);
+    return e == cudaSuccess ? CSN_OK : set_cuda_error(e, "csn_silu_gated_linear_fwd");
+  }
+  if (!tiled(x, R, C, ldx) || !tiled(w_gate, F, C, ld_gate) || !tiled(w_up, F, C, ld_up))
+    return set_error(CSN_ERR_INVALID, "csn_silu_gated_linear_fwd: x, w_gate and w_up need rows that start on 16 bytes "
+                                      "(row strides of at least C that are multiples of 8)");
   KernelTimer kt("silu_gated_linear_fwd", st);
-  if (dtype == CSN_BF16) forward<__nv_bfloat16>(x, ldx, w_gate, ld_gate, w_up, ld_up, y, R, C, F, st);
-  else forward<__half>(x, ldx, w_gate, ld_gate, w_up, ld_up, y, R, C, F, st);
-  return check_launch("csn_silu_gated_linear_fwd");
+  return dtype == CSN_BF16 ? forward<true>(x, ldx, w_gate, ld_gate, w_up, ld_up, y, R, C, F, st)
+                           : forward<false>(x, ldx, w_gate, ld_gate, w_up, ld_up, y, R, C, F, st);
 }
 
 extern "C" int csn_silu_gated_linear_bwd(const void* x, int64_t ldx, const void* w_gate, int64_t ld_gate,
@@ -168,15 +721,15 @@ extern "C" int csn_silu_gated_linear_bwd(const void* x, int64_t ldx, const void*
         return set_error(CSN_ERR_CUDA, "csn_silu_gated_linear_bwd: cudaMemsetAsync");
     return CSN_OK;
   }
-  if (!x || !w_gate || !w_up || !dy || !al16b(dx) || !al16b(dw_gate) || !al16b(dw_up))
+  if (!dy || (reinterpret_cast<uintptr_t>(dy) & 1) || !al16b(dx) || !al16b(dw_gate) || !al16b(dw_up))
     return set_error(CSN_ERR_INVALID, "csn_silu_gated_linear_bwd: missing or misaligned pointer");
-  const size_t need = csn_silu_gated_linear_workspace_bytes(R, C, F, 1);
-  if (need && (!workspace || !al16b(workspace) || workspace_bytes < need))
-    return set_error(CSN_ERR_INVALID, "csn_silu_gated_linear_bwd: workspace smaller than csn_silu_gated_linear_workspace_bytes");
+  if (!tiled(x, R, C, ldx) || !tiled(w_gate, F, C, ld_gate) || !tiled(w_up, F, C, ld_up))
+    return set_error(CSN_ERR_INVALID, "csn_silu_gated_linear_bwd: x, w_gate and w_up need rows that start on 16 bytes "
+                                      "(row strides of at least C that are multiples of 8)");
+  if (!workspace || !al16b(workspace) || workspace_bytes < csn_silu_gated_linear_bwd_workspace_bytes(R, C, F))
+    return set_error(CSN_ERR_INVALID, "csn_silu_gated_linear_bwd: workspace smaller than csn_silu_gated_linear_bwd_workspace_bytes");
   KernelTimer kt("silu_gated_linear_bwd", st);
-  if (dtype == CSN_BF16)
-    backward<__nv_bfloat16>(x, ldx, w_gate, ld_gate, w_up, ld_up, dy, ld_dy, dx, dw_gate, dw_up, R, C, F, workspace, st);
-  else
-    backward<__half>(x, ldx, w_gate, ld_gate, w_up, ld_up, dy, ld_dy, dx, dw_gate, dw_up, R, C, F, workspace, st);
-  return check_launch("csn_silu_gated_linear_bwd");
+  return dtype == CSN_BF16
+             ? backward<true>(x, ldx, w_gate, ld_gate, w_up, ld_up, dy, ld_dy, dx, dw_gate, dw_up, R, C, F, workspace, st)
+             : backward<false>(x, ldx, w_gate, ld_gate, w_up, ld_up, dy, ld_dy, dx, dw_gate, dw_up, R, C, F, workspace, st);
 }

@@ -1,0 +1,129 @@
+// csn_tc.cuh -- tensor-core building blocks for sm_100a: mbarriers, TMA tile loads, tensor memory and tcgen05.mma,
+// as inline PTX, and the tensor maps on the host.
+//
+// Every wait is bounded.  A wait that runs out sets the CTA's `gave_up` word; every other wait of the CTA then ends
+// too, the CTA drains what it has in flight, frees its tensor memory and returns, and its epilogue writes NaN in
+// place of results.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace csn {
+namespace tc {
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void mbar_init(uint64_t* b, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(b)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_init_fence() {
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* b) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(b)) : "memory");
+}
+__device__ __forceinline__ void mbar_expect(uint64_t* b, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(b)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint64_t* b, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_addr(b)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// Waits for the phase `parity` of b to end.  A poll takes tens of nanoseconds at least, so the limit is some tenths
+// of a second, a thousand times the longest tile.
+constexpr uint32_t POLLS = 1u << 23;
+__device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, volatile uint32_t* gave_up) {
+  for (uint32_t i = 0; i < POLLS; ++i) {
+    if (mbar_try(b, parity)) return true;
+    if ((i & 1023) == 1023 && *gave_up) return false;
+  }
+  *gave_up = 1;
+  return false;
+}
+
+// ------------------------------------------------------------------------- TMA
+// the box of `map` at (x, y) to shared memory, counted on b
+__device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int x, int y, uint64_t* b) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+          smem_addr(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(smem_addr(b))
+      : "memory");
+}
+
+// ---------------------------------------------------------------- tensor memory
+template <int COLS>
+__device__ __forceinline__ void tmem_alloc(uint32_t* slot) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(slot)), "n"(COLS)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+template <int COLS>
+__device__ __forceinline__ void tmem_free(uint32_t base) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "n"(COLS));
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// 32 columns of this warp's 32 lanes: thread = lane, register = column
+__device__ __forceinline__ void tmem_load32(uint32_t addr, float* v) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
+      "%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// -------------------------------------------------------------------------- MMA
+// Shared-memory operand of 16-bit elements in 128-byte swizzled rows (what a TMA box of 64 elements a row leaves).
+//   K-major: a row is 64 neighbouring k of one m (n); 8 rows make a 1024-byte group (SBO), a k step of 16 is 32 bytes.
+//   MN-major: a row is 64 neighbouring m of one k; 8 rows of k make a 1024-byte group (SBO), the next 64 m are `lbo`
+//   bytes on, a k step of 16 is 2048 bytes.
+__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lbo) {
+  return (uint64_t)((addr & 0x3ffff) >> 4) | (uint64_t)((lbo & 0x3ffff) >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+// kind::f16 instruction: float32 accumulators, both operands bf16 or both fp16, each K-major or MN-major, M x N
+__host__ __device__ constexpr uint32_t instruction(bool bf16, bool a_mn, bool b_mn, int m, int n) {
+  return 1u << 4 | (bf16 ? 1u : 0u) << 7 | (bf16 ? 1u : 0u) << 10 | (a_mn ? 1u : 0u) << 15 | (b_mn ? 1u : 0u) << 16 |
+         (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24;
+}
+
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      : "memory");
+}
+// b counts one arrival when every MMA issued so far by this thread is done
+__device__ __forceinline__ void mma_commit(uint64_t* b) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(b))
+               : "memory");
+}
+
+// ------------------------------------------------------------------------- host
+// Tensor map of a row-major 16-bit matrix [rows, cols] with `ld` elements a row (ld % 8 == 0, p 16-byte aligned),
+// read in boxes of 64 columns x box_rows rows with 128-byte swizzle; what lies outside reads as 0.
+bool make_map(CUtensorMap* map, const void* p, int64_t rows, int64_t cols, int64_t ld, int box_rows, bool bf16);
+int sm_count();
+
+}  // namespace tc
+}  // namespace csn

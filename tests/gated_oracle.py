@@ -79,23 +79,28 @@ def gated_scan(f, x, h0, gate, borders, dy=None, dh=None):
 
 def silu_gated_linear(x, wg, wu, kind, dy=None):
     """Sums over K products in float32, in any order: off by at most (K + 16) 2 U of the sum of their
-    sizes (2 U an addition: an accumulator may cut instead of rounding)."""
+    sizes (2 U an addition: an accumulator may cut instead of rounding).  The fast exp rounds its
+    argument too: off by (4 + 2 |g|) U.  float16 gradients dg, du are rounded after scaling by a power
+    of two that brings the largest |dy| into [1, 2): numbers below 2^-14 of that keep 2^-25 of it."""
     C, F, R = x.shape[1], wg.shape[0], x.shape[0]
     g, u = x @ wg.T, x @ wu.T
     sum_err = lambda k: (k + 16) * 2 * U  # noqa: E731
     ge, ue = sum_err(C) * (np.abs(x) @ np.abs(wg).T), sum_err(C) * (np.abs(x) @ np.abs(wu).T)
     w = sigmoid(g)
     silu, slope = g * w, w * (1 + g * (1 - w))
-    se = 1.1 * ge + 14 * U * np.abs(silu)  # |silu'| <= 1.1
+    fast = (14 + 2 * np.abs(g)) * U
+    se = 1.1 * ge + fast * np.abs(silu)  # |silu'| <= 1.1
     out = {"y": (silu * u, se * np.abs(u) + np.abs(silu) * ue + U * np.abs(silu * u))}
     if dy is None:
         return out
     dg, du = dy * u * slope, dy * silu
-    slope_err = 0.5 * ge + w * (8 * U * np.abs(g) + 16 * U * (1 + np.abs(g) * (1 - w)))  # |silu''| <= 0.5
+    # |silu''| <= 0.5; 1 - w is off by `fast` at most, and 1 + g (1 - w) by that times |g|
+    slope_err = 0.5 * ge + w * (fast * np.abs(g) + 2 * fast * (1 + np.abs(g) * (1 - w)))
     dge = np.abs(dy) * (ue * np.abs(slope) + np.abs(u) * slope_err) + 4 * U * np.abs(dg)
     due = np.abs(dy) * se + 2 * U * np.abs(du)
     # the operands of the products that follow are rounded to the type once
-    dge, due = dge + rounding(dg, kind), due + rounding(du, kind)
+    floor = TINY[kind] * (2.0 * np.abs(dy).max() if kind == "float16" and dy.size else 1.0)
+    dge, due = dge + HALF_STEP[kind] * np.abs(dg) + floor, due + HALF_STEP[kind] * np.abs(du) + floor
     aw, au, ax = np.abs(wg), np.abs(wu), np.abs(x)
     out["dx"] = (dg @ wg + du @ wu, dge @ aw + due @ au + sum_err(2 * F) * (np.abs(dg) @ aw + np.abs(du) @ au))
     out["dwg"] = (dg.T @ x, dge.T @ ax + sum_err(R) * (np.abs(dg).T @ ax))

@@ -94,13 +94,17 @@ def test_step_refuses(lib):
 def test_ffn_refuses(lib):
     p = fake()
 
-    def fwd(x=p, y=p, R=4, C=8, F=8, dtype=1, ws=p, nb=1 << 30):
-        return lib.csn_silu_gated_linear_fwd(x, C, p, C, p, C, y, R, C, F, dtype, ws, nb, NULL)
+    def fwd(x=p, y=p, R=4, C=8, F=8, ldx=8, dtype=1):
+        return lib.csn_silu_gated_linear_fwd(x, ldx, p, C, p, C, y, R, C, F, dtype, NULL)
 
     refused(lib, fwd(R=-1), 1, "R, C, F")
     refused(lib, fwd(F=2 ** 22), 1, "R, C, F")
     refused(lib, fwd(dtype=0), 2, "dtype")
-    refused(lib, fwd(x=NULL), 1, "missing")
+    refused(lib, fwd(x=NULL), 1, "16 bytes")
+    refused(lib, fwd(x=fake(8)), 1, "16 bytes")
+    refused(lib, fwd(ldx=12), 1, "16 bytes")
+    refused(lib, fwd(ldx=0), 1, "16 bytes")
+    refused(lib, fwd(C=9, ldx=16), 1, "16 bytes")
     refused(lib, fwd(y=fake(2)), 1, "misaligned")
     assert fwd(R=0) == 0 and fwd(F=0) == 0
 
