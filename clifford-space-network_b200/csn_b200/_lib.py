@@ -121,6 +121,8 @@ class CsnError(RuntimeError):
 def load(path: Path | None = None):
     """Load (once) and return the ctypes handle of libcsn_b200.so."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib

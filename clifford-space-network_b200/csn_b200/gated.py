@@ -13,53 +13,74 @@ and its gated product python/clifford_model.py:42-43.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _ptr, _require_cuda, _stream, _workspace
+from .ops import _require_cuda, _workspace
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_NAMES = {t: str(t).replace("torch.", "") for t in DTYPES}
+
+# a generation step is one small kernel, so what its call costs on the host is what it costs: the
+# index forms of current_device() and current_stream() take a tenth of the time
+_current_device = torch._C._cuda_getDevice
+_current_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _dtype_of(name, allowed, *ts):
-    """The dtype code of tensors that have to share one of the allowed types."""
-    dtype = ts[0].dtype
-    if dtype not in allowed or any(t is not None and t.dtype != dtype for t in ts):
-        raise ValueError(f"{name}: tensors of one type among {', '.join(str(d) for d in allowed)} expected, got "
-                         f"{', '.join(str(t.dtype) for t in ts if t is not None)}")
-    return DTYPES[dtype]
+def _launch(name, index, *args):
+    """Calls an entry point on the current stream of device `index`; None is a null pointer."""
+    if _current_device() == index:
+        rc = getattr(_lib.load(), name)(*args, _current_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = getattr(_lib.load(), name)(*args, _current_stream(index))
+    if rc:
+        raise _lib.CsnError(name, rc, _lib.load().csn_last_error().decode(errors="replace"))
 
 
-def _same_device(name, *ts):
-    _require_cuda(*ts)
-    if len({t.device for t in ts if t is not None}) > 1:
+def _device_of(name, first, *rest):
+    """The index of the device that all tensors are on."""
+    index = first.get_device()
+    for t in rest:
+        if t is not None and t.get_device() != index:
+            index = -1
+            break
+    if index < 0:
+        _require_cuda(first, *rest)
         raise ValueError(f"{name}: tensors are on different devices")
+    return index
 
 
-def _on(device):
-    """Makes `device` current for a launch, where it is not."""
-    if torch.cuda.current_device() == device.index:
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+def _dtype_of(name, allowed, first, *rest):
+    """The dtype code of tensors that have to share one of the allowed types."""
+    dtype = first.dtype
+    if dtype in allowed:
+        for t in rest:
+            if t is not None and t.dtype != dtype:
+                break
+        else:
+            return DTYPES[dtype]
+    raise ValueError(f"{name}: tensors of one type among {', '.join(_NAMES[d] for d in allowed)} expected, got "
+                     f"{', '.join(str(t.dtype) for t in (first, *rest) if t is not None)}")
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _rows(t):
-    """t detached, with a contiguous last axis (itself where it has one)."""
-    if t is None:
-        return None
-    t = t.detach()
-    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+    """t with a contiguous last axis (itself where it has one)."""
+    return t if t is None or t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
 def _packed(t):
-    """Contiguous and 16-byte aligned (itself where it is)."""
+    """t contiguous and 16-byte aligned (itself where it is)."""
     if t is None:
         return None
-    t = t.detach().contiguous()
+    t = t.contiguous()
     return t.clone() if t.data_ptr() % 16 else t
 
 
@@ -68,36 +89,46 @@ def _row_strides(*ts):
     entry (its stride means nothing) or a tensor is absent.  [rows, C] gives (0, row)."""
     out = []
     for t in ts:
-        st = [] if t is None else [t.stride(i) if t.shape[i] > 1 else 0 for i in range(t.dim() - 1)]
-        out += [0] * (2 - len(st)) + st
-    return (ctypes.c_int64 * len(out))(*out)
+        if t is None:
+            out += (0, 0)
+            continue
+        n, st = t.shape, t.stride()
+        if len(n) == 2:
+            out += (0, st[0] if n[0] > 1 else 0)
+        else:
+            out += (st[0] if n[0] > 1 else 0, st[1] if n[1] > 1 else 0)
+    return _STRIDES[len(out)](*out)
+
+
+_STRIDES = {n: ctypes.c_int64 * n for n in (3, 6, 8)}
 
 
 def _wants_grad(*ts):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 # ------------------------------------------------------------- gated recurrence
 def _scan_sizes(f, cu):
-    if cu is None:
-        return f.shape[0], f.shape[1], f.shape[2]
-    return cu.shape[0] - 1, f.shape[0], f.shape[1]
+    n = f.shape
+    return (n[0], n[1], n[2]) if cu is None else (cu.shape[0] - 1, n[0], n[1])
 
 
 def _gated_scan_fwd(f, x, h0, gate, cu, keep):
     """(y, h_last, marks or None) of rows as they lie; h0 float32."""
     f, x, gate, h0 = _rows(f), _rows(x), _rows(gate), _packed(h0)
     S, T, C = _scan_sizes(f, cu)
-    dev = f.device
-    y = torch.empty(f.shape, dtype=f.dtype, device=dev)
-    h_last = torch.empty(S, C, dtype=torch.float32, device=dev)
+    index = f.get_device()
+    y = f.new_empty(f.shape)
+    h_last = f.new_empty((S, C), dtype=torch.float32)
     marks = None
     if keep:
-        marks = torch.empty(_lib.load().csn_gated_scan_marks(S, T, C, int(cu is not None)), dtype=torch.float32,
-                            device=dev)
-    with _on(dev):
-        _lib.call("csn_gated_scan_fwd", _ptr(f), _ptr(x), _ptr(gate), _row_strides(f, x, gate), _ptr(h0), _ptr(cu),
-                  _ptr(y), _ptr(h_last), _ptr(marks), S, T, C, DTYPES[f.dtype], _stream(dev))
+        marks = f.new_empty((_lib.load().csn_gated_scan_marks(S, T, C, int(cu is not None)),), dtype=torch.float32)
+    _launch("csn_gated_scan_fwd", index, _ptr(f), _ptr(x), _ptr(gate), _row_strides(f, x, gate), _ptr(h0), _ptr(cu),
+            _ptr(y), _ptr(h_last), _ptr(marks), S, T, C, DTYPES[f.dtype])
     return y, h_last, marks
 
 
@@ -105,14 +136,13 @@ def _gated_scan_bwd(f, x, gate, cu, marks, dy, dh_last, need):
     """Gradients (df, dx, dh0, dgate) where `need` asks for them, None elsewhere."""
     f, x, gate, dy, dh_last = _rows(f), _rows(x), _rows(gate), _rows(dy), _packed(dh_last)
     S, T, C = _scan_sizes(f, cu)
-    dev = f.device
-    like = lambda want: torch.empty(f.shape, dtype=f.dtype, device=dev) if want else None  # noqa: E731
-    df, dx, dgate = like(need[0]), like(need[1]), like(need[3] and gate is not None)
-    dh0 = torch.empty(S, C, dtype=torch.float32, device=dev) if need[2] else None
-    with _on(dev):
-        _lib.call("csn_gated_scan_bwd", _ptr(f), _ptr(x), _ptr(gate), _ptr(dy), _row_strides(f, x, gate, dy),
-                  _ptr(cu), _ptr(marks), _ptr(dh_last), _ptr(df), _ptr(dx), _ptr(dgate), _ptr(dh0), S, T, C,
-                  DTYPES[f.dtype], _stream(dev))
+    df = f.new_empty(f.shape) if need[0] else None
+    dx = f.new_empty(f.shape) if need[1] else None
+    dh0 = f.new_empty((S, C), dtype=torch.float32) if need[2] else None
+    dgate = f.new_empty(f.shape) if need[3] and gate is not None else None
+    _launch("csn_gated_scan_bwd", f.get_device(), _ptr(f), _ptr(x), _ptr(gate), _ptr(dy),
+            _row_strides(f, x, gate, dy), _ptr(cu), _ptr(marks), _ptr(dh_last), _ptr(df), _ptr(dx), _ptr(dgate),
+            _ptr(dh0), S, T, C, DTYPES[f.dtype])
     return df, dx, dh0, dgate
 
 
@@ -134,9 +164,10 @@ class GatedScanFunction(torch.autograd.Function):
 
 
 def _check_scan(f, x, h0, gate, cu):
-    _same_device("gated_scan", f, x, h0, gate, cu)
+    _device_of("gated_scan", f, x, h0, gate, cu)
     _dtype_of("gated_scan", DTYPES, f, x, gate)
-    if f.dim() != (3 if cu is None else 2) or x.shape != f.shape or (gate is not None and gate.shape != f.shape):
+    n = f.shape
+    if len(n) != (3 if cu is None else 2) or x.shape != n or (gate is not None and gate.shape != n):
         raise ValueError("gated_scan: f, x and gate [B, T, C], or [L, C] with cu_seqlens, of one shape expected, got "
                          f"{', '.join(str(tuple(t.shape)) for t in (f, x, gate) if t is not None)}")
     if cu is not None and (cu.dtype != torch.int32 or cu.dim() != 1 or cu.shape[0] < 2 or not cu.is_contiguous()):
@@ -157,7 +188,8 @@ def gated_scan(f, x, h0=None, gate=None, cu_seqlens=None):
     ([B, C] or [S, C], zero if absent); h_last: the float32 states after the last ones, h0 for a
     sequence without steps.  Differentiable in f, x, h0 and gate."""
     _check_scan(f, x, h0, gate, cu_seqlens)
-    h0 = None if h0 is None else h0.to(torch.float32)
+    if h0 is not None and h0.dtype != torch.float32:
+        h0 = h0.to(torch.float32)
     if not _wants_grad(f, x, h0, gate):
         return _gated_scan_fwd(f, x, h0, gate, cu_seqlens, False)[:2]
     return GatedScanFunction.apply(f, x, h0, gate, cu_seqlens)
@@ -167,20 +199,19 @@ def gated_step(f, x, h, gate=None):
     """One step of :func:`gated_scan` for B streams: h [B, C] (float32, contiguous) is advanced in
     place and y [B, C] returned; f, x, gate [B, C].  One launch and, but for y, no allocation.  For
     generation: not differentiable."""
-    _same_device("gated_step", f, x, h, gate)
+    index = _device_of("gated_step", f, x, h, gate)
     code = _dtype_of("gated_step", DTYPES, f, x, gate)
-    if f.dim() != 2 or x.shape != f.shape or h.shape != f.shape or (gate is not None and gate.shape != f.shape):
+    n = f.shape
+    if len(n) != 2 or x.shape != n or h.shape != n or (gate is not None and gate.shape != n):
         raise ValueError("gated_step: f, x, h and gate [B, C] of one shape expected")
     if h.dtype != torch.float32 or not h.is_contiguous() or h.data_ptr() % 16:
         raise ValueError("gated_step: h is a contiguous float32 state, 16-byte aligned")
     if _wants_grad(f, x, h, gate):
         raise ValueError("gated_step: not differentiable; call it under torch.no_grad() or use gated_scan")
     f, x, gate = _rows(f), _rows(x), _rows(gate)
-    y = torch.empty(f.shape, dtype=f.dtype, device=f.device)
-    strides = (ctypes.c_int64 * 3)(f.stride(0), x.stride(0), 0 if gate is None else gate.stride(0))
-    with _on(f.device):
-        _lib.call("csn_gated_step", _ptr(f), _ptr(x), _ptr(gate), strides, _ptr(h), _ptr(y), f.shape[0], f.shape[1],
-                  code, _stream(f.device))
+    y = f.new_empty(n)
+    strides = _STRIDES[3](f.stride(0), x.stride(0), 0 if gate is None else gate.stride(0))
+    _launch("csn_gated_step", index, _ptr(f), _ptr(x), _ptr(gate), strides, _ptr(h), _ptr(y), n[0], n[1], code)
     return y
 
 
@@ -197,7 +228,7 @@ def _tiled(t):
     if t.data_ptr() % 16 == 0 and ld % 8 == 0 and ld >= c:
         return t, ld
     ld = (c + 7) // 8 * 8
-    room = torch.empty(n, ld, dtype=t.dtype, device=t.device)
+    room = t.new_empty((n, ld))
     room[:, :c].copy_(t)
     return room, ld
 
@@ -205,25 +236,22 @@ def _tiled(t):
 def _silu_gated_linear_fwd(x, wg, wu):
     R, C, F = x.shape[0], x.shape[1], wg.shape[0]
     (x, ldx), (wg, ldg), (wu, ldu) = _tiled(x), _tiled(wg), _tiled(wu)
-    y = torch.empty(R, F, dtype=x.dtype, device=x.device)
-    with _on(x.device):
-        _lib.call("csn_silu_gated_linear_fwd", _ptr(x), ldx, _ptr(wg), ldg, _ptr(wu), ldu, _ptr(y), R, C, F,
-                  DTYPES[x.dtype], _stream(x.device))
+    y = x.new_empty((R, F))
+    _launch("csn_silu_gated_linear_fwd", x.get_device(), _ptr(x), ldx, _ptr(wg), ldg, _ptr(wu), ldu, _ptr(y), R, C, F,
+            DTYPES[x.dtype])
     return y
 
 
 def _silu_gated_linear_bwd(x, wg, wu, dy, need):
     R, C, F = x.shape[0], x.shape[1], wg.shape[0]
     (x, ldx), (wg, ldg), (wu, ldu), dy = _tiled(x), _tiled(wg), _tiled(wu), _rows(dy)
-    dev, typ = x.device, x.dtype
-    dx = torch.empty(R, C, dtype=typ, device=dev) if need[0] else None
-    dwg = torch.empty(F, C, dtype=typ, device=dev) if need[1] else None
-    dwu = torch.empty(F, C, dtype=typ, device=dev) if need[2] else None
+    dx = x.new_empty((R, C)) if need[0] else None
+    dwg = x.new_empty((F, C)) if need[1] else None
+    dwu = x.new_empty((F, C)) if need[2] else None
     nb = _lib.load().csn_silu_gated_linear_bwd_workspace_bytes(R, C, F)
-    with _on(dev):
-        ws = _workspace(nb, dev)
-        _lib.call("csn_silu_gated_linear_bwd", _ptr(x), ldx, _ptr(wg), ldg, _ptr(wu), ldu, _ptr(dy), dy.stride(0),
-                  _ptr(dx), _ptr(dwg), _ptr(dwu), R, C, F, DTYPES[typ], _ptr(ws), nb, _stream(dev))
+    ws = _workspace(nb, x.device)
+    _launch("csn_silu_gated_linear_bwd", x.get_device(), _ptr(x), ldx, _ptr(wg), ldg, _ptr(wu), ldu, _ptr(dy),
+            dy.stride(0), _ptr(dx), _ptr(dwg), _ptr(dwu), R, C, F, DTYPES[x.dtype], _ptr(ws), nb)
     return dx, dwg, dwu
 
 
@@ -244,25 +272,24 @@ def silu_gated_linear(x, w_gate, w_up):
     (what :func:`silu_gate` makes of the library product of both weights).  bfloat16 or float16 on the
     tensor cores, sums in float32, one rounding at the end; the backward pass forms both products
     again instead of keeping them.  float32 layers use ``silu_gate(linear(x, cat))``."""
-    _same_device("silu_gated_linear", x, w_gate, w_up)
+    _device_of("silu_gated_linear", x, w_gate, w_up)
     _dtype_of("silu_gated_linear", HALF_TYPES, x, w_gate, w_up)
     if x.dim() < 1 or w_gate.dim() != 2 or w_up.shape != w_gate.shape or x.shape[-1] != w_gate.shape[1]:
         raise ValueError("silu_gated_linear: x [..., C] and w_gate, w_up [F, C] expected, got "
                          f"{tuple(x.shape)}, {tuple(w_gate.shape)}, {tuple(w_up.shape)}")
-    lead, C, F = x.shape[:-1], w_gate.shape[1], w_gate.shape[0]
-    x2 = x.reshape(lead.numel(), C)
+    C, F = w_gate.shape[1], w_gate.shape[0]
+    x2 = x if x.dim() == 2 else x.reshape(x.shape[:-1].numel(), C)
     y = (SiluGatedLinearFunction.apply(x2, w_gate, w_up) if _wants_grad(x, w_gate, w_up)
          else _silu_gated_linear_fwd(x2, w_gate, w_up))
-    return y.view(*lead, F)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], F)
 
 
 # ------------------------------------------------------------------------ dropout
 def _dropout_add(x, residual, cut, rng):
     x, residual = _packed(x), _packed(residual)
-    y = torch.empty_like(x)
-    with _on(x.device):
-        _lib.call("csn_dropout_add", _ptr(x), _ptr(residual), _ptr(rng), _ptr(y), x.numel(), cut, DTYPES[x.dtype],
-                  _stream(x.device))
+    y = x.new_empty(x.shape)
+    _launch("csn_dropout_add", x.get_device(), _ptr(x), _ptr(residual), _ptr(rng), _ptr(y), x.numel(), cut,
+            DTYPES[x.dtype])
     return y
 
 
@@ -288,7 +315,7 @@ def dropout_add(x, residual, p: float, rng):
     masks and a captured graph draws a new one when the numbers are changed between replays
     (csn_b200.modules.DropoutAdd counts for itself).  p is taken in steps of 2^-16 and kept places
     are scaled by one over the probability of being kept."""
-    _same_device("dropout_add", x, residual, rng)
+    _device_of("dropout_add", x, residual, rng)
     _dtype_of("dropout_add", DTYPES, x, residual)
     if residual is not None and residual.shape != x.shape:
         raise ValueError(f"dropout_add: x and residual of one shape expected, got {tuple(x.shape)}, "

@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(THREADS, 1) mm_kernel(const __grid_constant__ 
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               const float gv = g[2 * i + j], uv = u[2 * i + j];
-              const float w = __fdividef(1.0f, 1.0f + __expf(-gv));
+              const float w = sigmoid(gv);
               if (MODE == GATE) {
                 r0[j] = gv * w * uv;
               } else {
@@ -484,9 +484,7 @@ __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(const __grid_cons
       g += peer_float(base + (f * (NR + 1) + r) * 4, k);
       u += peer_float(base + ((f + HALF_ROWS) * (NR + 1) + r) * 4, k);
     }
-    float w, wn;
-    sigmoid_pair(g, w, wn);
-    const float v = g * w * u;
+    const float v = g * sigmoid(g) * u;
     const int64_t at = (int64_t)r * P.F + f0 + f;
     if (BF16) static_cast<__nv_bfloat16*>(P.y)[at] = __float2bfloat16_rn(v);
     else static_cast<__half*>(P.y)[at] = __float2half_rn(v);

@@ -4,11 +4,16 @@
 // Adjoint, with D_t = h_{t-1} - x_t, dh_t = dy_t silu(g_t) and lam_t = dh_t + a_{t+1} lam_{t+1} (the gradient of
 // the last state enters at the end):
 //   dx = q lam,  df = lam D a q,  dg = dy h silu'(g),  dh0 = a_0 lam_0
-// Each step is the affine map h -> a h + b, and maps compose: (A2, B2) o (A1, B1) = (A2 A1, A2 B1 + B2).  A warp
-// takes STEPS neighbouring steps of 32 * V neighbouring channels (a lane keeps V channels; a row of a warp is one
-// 128-byte access for 16-bit pairs and for float32), composes its steps in registers, the warps of a CTA pass their
-// composed maps through shared memory, and every step is then finished from the state that enters its warp.  So the
-// inputs are read once.  All sums, products and states are float32.
+//
+// With s = min(a, q), exact in its relative precision, a step is h + s (x - h) or x + s (h - x): rounding a itself
+// near 1 would drift a long memory, rounding h does not.  c = s, or -s where q is the larger, keeps both.
+//
+// Each step is an affine map h -> A h + B, and maps compose: (A2, B2) o (A1, B1) = (A2 A1, A2 B1 + B2).  A warp takes
+// STEPS neighbouring steps of 32 * V neighbouring channels (a lane keeps V channels; a row of a warp is one 128-byte
+// access for 16-bit pairs and for float32) and composes them in registers; the warps of a CTA pass their maps through
+// shared memory, the CTAs of a cluster, which take neighbouring MARK-step pieces of one sequence, through distributed
+// shared memory; then every warp runs its steps again from the state that enters them.  So inputs are read once,
+// one pass ahead of their use, and sums, products and states are float32 and in a fixed order.
 //
 // The forward pass keeps the float32 state before every MARK-th step ("marks") where a backward pass will follow:
 // the adjoint forms the states between two marks again instead of reading rounded outputs (y is not h where there is
@@ -81,12 +86,12 @@ __device__ __forceinline__ void store(T* p, const float* v) {
 
 // Rows that belong to no sequence (before the first, behind the last) are written as 0.
 template <typename T, int V>
-__device__ void clear_outside(const ScanArgs& A, const Seq& q, int64_t s, int64_t c, bool live, int warp,
+__device__ void clear_outside(const ScanArgs& A, const Seq& q, int64_t s, int64_t c, bool live, int warp, int warps,
                               T* o0, T* o1, T* o2) {
   if (!A.cu || !live) return;
   const float zero[V] = {};
   auto clear = [&](int64_t from, int64_t to) {
-    for (int64_t r = from + warp; r < to; r += WARPS) {
+    for (int64_t r = from + warp; r < to; r += warps) {
       if (o0) store<T, V>(o0 + r * A.C + c, zero);
       if (o1) store<T, V>(o1 + r * A.C + c, zero);
       if (o2) store<T, V>(o2 + r * A.C + c, zero);
@@ -96,13 +101,57 @@ __device__ void clear_outside(const ScanArgs& A, const Seq& q, int64_t s, int64_
   if (s == A.S - 1) clear(q.row0 + q.len, A.T);
 }
 
+// ------------------------------------------------------------------------ one step
+__device__ __forceinline__ bool keeps(float c) { return __float_as_int(c) >= 0; }  // a >= q
+__device__ __forceinline__ float coefficient(float f) {
+  const float s = sigmoid_small(f);
+  return f >= 0.0f ? s : -s;
+}
+__device__ __forceinline__ float step(float c, float h, float x) { return fmaf(c, x - h, keeps(c) ? h : x); }
+__device__ __forceinline__ float times_a(float c, float v) { return fmaf(-c, v, keeps(c) ? v : 0.0f); }
+__device__ __forceinline__ float times_q(float c, float v) { return fmaf(c, v, keeps(c) ? 0.0f : v); }
+
+// -------------------------------------------------------------------- the cluster
+struct Cluster {
+  uint32_t rank, size;
+  __device__ __forceinline__ Cluster() {
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
+  }
+  // *p of CTA `to` = v
+  __device__ __forceinline__ void put(float2* p, uint32_t to, float2 v) const {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(to));
+    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(a), "f"(v.x), "f"(v.y) : "memory");
+  }
+  __device__ __forceinline__ void sync() const {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+};
+constexpr int MOST_CTAS = 16;  // of a cluster
+
+// The raw inputs of a warp's steps.  Steps behind the end read the last row, channels behind the last read the last
+// ones: every address is inside, and what does not count is left out where it is used.
+template <typename T, int V, int N>
+struct Raw {
+  Pack<T, V> v[N][STEPS];
+  __device__ __forceinline__ void read(int i, const T* p, int64_t row, int64_t t1, int64_t len) {
+#pragma unroll
+    for (int l = 0; l < STEPS; ++l) v[i][l] = load<T, V>(p + min(t1 + l, len - 1) * row);
+  }
+};
+
 template <typename T, int V, bool GATE>
-__global__ void __launch_bounds__(WARPS * 32) gated_scan_fwd_kernel(const ScanArgs A) {
+__global__ void __launch_bounds__(WARPS * 32, 2) gated_scan_fwd_kernel(const ScanArgs A) {
   __shared__ float2 maps[2][WARPS][32 * V];
+  __shared__ float2 peers[2][MOST_CTAS][32 * V];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t s = blockIdx.x / A.tiles;
-  const int64_t c = (int64_t)(blockIdx.x % A.tiles) * (32 * V) + lane * V;
-  const bool live = c < A.C;
+  const Cluster K;
+  const int64_t unit = blockIdx.x / K.size;
+  const int64_t s = unit / A.tiles;
+  const int64_t c0 = (unit % A.tiles) * (32 * V) + lane * V;
+  const bool live = c0 < A.C;
+  const int64_t c = live ? c0 : A.C - V;
   const Seq q(A, s);
   const T* f = q.in<T>(A.f, A, s) + c;
   const T* x = q.in<T>(A.x, A, s) + c;
@@ -110,83 +159,121 @@ __global__ void __launch_bounds__(WARPS * 32) gated_scan_fwd_kernel(const ScanAr
   T* y = static_cast<T*>(A.y);
   float carry[V];
 #pragma unroll
-  for (int v = 0; v < V; ++v) carry[v] = A.h0 && live ? A.h0[s * A.C + c + v] : 0.0f;
+  for (int v = 0; v < V; ++v) carry[v] = A.h0 ? A.h0[s * A.C + c + v] : 0.0f;
 
+  const int64_t pass = (int64_t)K.size * MARK;
+  int64_t t1 = K.rank * MARK + warp * STEPS;
+  Raw<T, V, GATE ? 3 : 2> next;
+  auto fetch = [&](int64_t t) {
+    next.read(0, f, A.f.row, t, q.len);
+    next.read(1, x, A.x.row, t, q.len);
+    if (GATE) next.read(2, g, A.g.row, t, q.len);
+  };
+  if (q.len > 0) fetch(t1);
+  if (K.size > 1) K.sync();  // shared memory of a CTA is there once it has started
   int half = 0;
-  for (int64_t t0 = 0; t0 < q.len; t0 += MARK, half ^= 1) {
-    const int64_t t1 = t0 + warp * STEPS;
-    // P, H: the composed map from the state that enters this warp to the state after each step
-    float P[STEPS][V], H[STEPS][V];
-    Pack<T, V> gr[STEPS];
-    {
-      Pack<T, V> fr[STEPS], xr[STEPS];
+  for (int64_t t0 = 0; t0 < q.len; t0 += pass, t1 += pass, half ^= 1) {
+    const int n = (int)max((int64_t)0, min((int64_t)STEPS, q.len - t1));
+    float cs[STEPS][V];
+    Pack<T, V> xr[STEPS], gr[STEPS];
 #pragma unroll
-      for (int l = 0; l < STEPS; ++l)
-        if (live && t1 + l < q.len) {
-          fr[l] = load<T, V>(f + (t1 + l) * A.f.row);
-          xr[l] = load<T, V>(x + (t1 + l) * A.x.row);
-          if (GATE) gr[l] = load<T, V>(g + (t1 + l) * A.g.row);
-        }
+    for (int l = 0; l < STEPS; ++l) {
+      xr[l] = next.v[1][l];
+      if (GATE) gr[l] = next.v[GATE ? 2 : 0][l];
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float p = 1.0f, h = 0.0f;
-#pragma unroll
-        for (int l = 0; l < STEPS; ++l) {
-          if (live && t1 + l < q.len) {
-            float a, b;
-            sigmoid_pair(to_float(fr[l].v[v]), a, b);
-            p *= a;
-            h = fmaf(a, h, b * to_float(xr[l].v[v]));
-          }
-          P[l][v] = p;
-          H[l][v] = h;
-        }
-      }
+      for (int v = 0; v < V; ++v) cs[l][v] = coefficient(to_float(next.v[0][l].v[v]));
     }
-#pragma unroll
-    for (int v = 0; v < V; ++v) maps[half][warp][lane * V + v] = make_float2(P[STEPS - 1][v], H[STEPS - 1][v]);
-    __syncthreads();
-    float in[V];
+    if (t0 + pass < q.len) fetch(t1 + pass);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      float h = carry[v];
+      float p = 1.0f, h = 0.0f;
+      auto compose = [&](int l) {
+        p = times_a(cs[l][v], p);
+        h = step(cs[l][v], h, to_float(xr[l].v[v]));
+      };
+      if (n == STEPS) {
+#pragma unroll
+        for (int l = 0; l < STEPS; ++l) compose(l);
+      } else {
+#pragma unroll
+        for (int l = 0; l < STEPS; ++l)
+          if (l < n) compose(l);
+      }
+      maps[half][warp][lane * V + v] = make_float2(p, h);
+    }
+    __syncthreads();
+    // (p, b) of this thread: the warps before its own; then of the whole CTA
+    float p[V], b[V], in[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      float tp = 1.0f, tb = 0.0f;
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) {
-        if (w == warp) in[v] = h;
+        if (w == warp) p[v] = tp, b[v] = tb;
         const float2 m = maps[half][w][lane * V + v];
-        h = fmaf(m.x, h, m.y);
+        tb = fmaf(m.x, tb, m.y);
+        tp *= m.x;
       }
-      carry[v] = h;
+      if (K.size > 1) {
+        for (uint32_t r = warp; r < K.size; r += WARPS) K.put(&peers[half][K.rank][lane * V + v], r, make_float2(tp, tb));
+      } else {
+        in[v] = fmaf(p[v], carry[v], b[v]);
+        carry[v] = fmaf(tp, carry[v], tb);
+      }
     }
-    if (A.marks && warp == 0 && live) store<float, V>(A.marks + (q.mark0 + t0 / MARK) * A.C + c, in);
+    if (K.size > 1) {
+      K.sync();
 #pragma unroll
-    for (int l = 0; l < STEPS; ++l)
-      if (live && t1 + l < q.len) {
-        float o[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          o[v] = fmaf(P[l][v], in[v], H[l][v]);
-          if (GATE) {
-            float z = to_float(gr[l].v[v]), sg, sn;
-            sigmoid_pair(z, sg, sn);
-            o[v] *= z * sg;
-          }
+      for (int v = 0; v < V; ++v) {
+        float h = carry[v];
+        for (uint32_t r = 0; r < K.size; ++r) {
+          if (r == K.rank) in[v] = fmaf(p[v], h, b[v]);
+          const float2 m = peers[half][r][lane * V + v];
+          h = fmaf(m.x, h, m.y);
         }
-        store<T, V>(y + (q.row0 + t1 + l) * A.C + c, o);
+        carry[v] = h;
       }
+    }
+    if (A.marks && warp == 0 && live && t1 < q.len) store<float, V>(A.marks + (q.mark0 + t1 / MARK) * A.C + c, in);
+    T* out = y + (q.row0 + t1) * A.C + c;
+    auto finish = [&](int l) {
+      float o[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        o[v] = in[v] = step(cs[l][v], in[v], to_float(xr[l].v[v]));
+        if (GATE) {
+          const float z = to_float(gr[l].v[v]);
+          o[v] *= z * sigmoid(z);
+        }
+      }
+      if (live) store<T, V>(out + l * A.C, o);
+    };
+    if (n == STEPS) {
+#pragma unroll
+      for (int l = 0; l < STEPS; ++l) finish(l);
+    } else {
+#pragma unroll
+      for (int l = 0; l < STEPS; ++l)
+        if (l < n) finish(l);
+    }
   }
-  if (warp == 0 && live && A.h_last) store<float, V>(A.h_last + s * A.C + c, carry);
-  clear_outside<T, V>(A, q, s, c, live, warp, y, static_cast<T*>(nullptr), static_cast<T*>(nullptr));
+  if (K.rank == 0 && warp == 0 && live && A.h_last) store<float, V>(A.h_last + s * A.C + c, carry);
+  clear_outside<T, V>(A, q, s, c, live, K.rank * WARPS + warp, K.size * WARPS, y, static_cast<T*>(nullptr),
+                      static_cast<T*>(nullptr));
 }
 
 template <typename T, int V, bool GATE>
-__global__ void __launch_bounds__(WARPS * 32) gated_scan_bwd_kernel(const ScanArgs A) {
+__global__ void __launch_bounds__(WARPS * 32, 2) gated_scan_bwd_kernel(const ScanArgs A) {
   __shared__ float2 maps[2][WARPS][32 * V];  // the forward map of a warp's steps
   __shared__ float back[2][WARPS][32 * V];   // what leaves a warp's first step when nothing enters its last
+  __shared__ float2 peers[2][MOST_CTAS][32 * V];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t s = blockIdx.x / A.tiles;
-  const int64_t c = (int64_t)(blockIdx.x % A.tiles) * (32 * V) + lane * V;
-  const bool live = c < A.C;
+  const Cluster K;
+  const int64_t unit = blockIdx.x / K.size;
+  const int64_t s = unit / A.tiles;
+  const int64_t c0 = (unit % A.tiles) * (32 * V) + lane * V;
+  const bool live = c0 < A.C;
+  const int64_t c = live ? c0 : A.C - V;
   const Seq q(A, s);
   const T* f = q.in<T>(A.f, A, s) + c;
   const T* x = q.in<T>(A.x, A, s) + c;
@@ -195,110 +282,155 @@ __global__ void __launch_bounds__(WARPS * 32) gated_scan_bwd_kernel(const ScanAr
   T *df = static_cast<T*>(A.df), *dx = static_cast<T*>(A.dx), *dg = static_cast<T*>(A.dg);
   float mu[V];  // the gradient that enters the pass from behind: a lam of the step after it
 #pragma unroll
-  for (int v = 0; v < V; ++v) mu[v] = A.dh_last && live ? A.dh_last[s * A.C + c + v] : 0.0f;
+  for (int v = 0; v < V; ++v) mu[v] = A.dh_last ? A.dh_last[s * A.C + c + v] : 0.0f;
 
+  const int64_t pass = (int64_t)K.size * MARK;
+  const int64_t last = q.len > 0 ? (q.len - 1) / pass * pass : -pass;
+  int64_t t1 = last + K.rank * MARK + warp * STEPS;
+  Raw<T, V, GATE ? 4 : 3> next;
+  auto fetch = [&](int64_t t) {
+    next.read(0, f, A.f.row, t, q.len);
+    next.read(1, x, A.x.row, t, q.len);
+    if (dy) next.read(2, dy, A.dy.row, t, q.len);
+    if (GATE) next.read(GATE ? 3 : 0, g, A.g.row, t, q.len);
+  };
+  if (q.len > 0) fetch(t1);
+  if (K.size > 1) K.sync();  // shared memory of a CTA is there once it has started
   int half = 0;
-  for (int64_t t0 = (q.len - 1) / MARK * MARK; t0 >= 0 && q.len > 0; t0 -= MARK, half ^= 1) {
-    const int64_t t1 = t0 + warp * STEPS;
-    float a[STEPS][V], b[STEPS][V], xs[STEPS][V], e[STEPS][V], sg[STEPS][V];
-    Pack<T, V> gr[STEPS], dr[STEPS];
-    {
-      Pack<T, V> fr[STEPS], xr[STEPS];
+  for (int64_t t0 = last; t0 >= 0; t0 -= pass, t1 -= pass, half ^= 1) {
+    const int n = (int)max((int64_t)0, min((int64_t)STEPS, q.len - t1));
+    float cs[STEPS][V], e[STEPS][V];  // e = dh
+    Pack<T, V> xr[STEPS], dr[STEPS], gr[STEPS];
 #pragma unroll
-      for (int l = 0; l < STEPS; ++l)
-        if (live && t1 + l < q.len) {
-          fr[l] = load<T, V>(f + (t1 + l) * A.f.row);
-          xr[l] = load<T, V>(x + (t1 + l) * A.x.row);
-          if (dy) dr[l] = load<T, V>(dy + (t1 + l) * A.dy.row);
-          if (GATE) gr[l] = load<T, V>(g + (t1 + l) * A.g.row);
-        }
+    for (int l = 0; l < STEPS; ++l) {
+      xr[l] = next.v[1][l];
+      dr[l] = next.v[2][l];
+      if (GATE) gr[l] = next.v[GATE ? 3 : 0][l];
 #pragma unroll
-      for (int l = 0; l < STEPS; ++l) {
-        const bool in = live && t1 + l < q.len;
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          a[l][v] = 1.0f;  // a step behind the end passes state and gradient on
-          b[l][v] = xs[l][v] = e[l][v] = sg[l][v] = 0.0f;
-          if (in) {
-            sigmoid_pair(to_float(fr[l].v[v]), a[l][v], b[l][v]);
-            xs[l][v] = to_float(xr[l].v[v]);
-            e[l][v] = dy ? to_float(dr[l].v[v]) : 0.0f;
-            if (GATE) {
-              float sn;
-              sigmoid_pair(to_float(gr[l].v[v]), sg[l][v], sn);
-              e[l][v] *= to_float(gr[l].v[v]) * sg[l][v];
-            }
-          }
+      for (int v = 0; v < V; ++v) {
+        cs[l][v] = coefficient(to_float(next.v[0][l].v[v]));
+        e[l][v] = dy ? to_float(dr[l].v[v]) : 0.0f;
+        if (GATE && dy) {
+          const float z = to_float(gr[l].v[v]);
+          e[l][v] *= z * sigmoid(z);
         }
       }
     }
+    // the state that enters this CTA's steps
+    float h[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      h[v] = t0 + K.rank * MARK < q.len ? A.marks[(q.mark0 + t0 / MARK + K.rank) * A.C + c + v] : 0.0f;
+    if (t0 > 0) fetch(t1 - pass);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      float p = 1.0f, h = 0.0f, r = 0.0f;
+      float p = 1.0f, b = 0.0f, r = 0.0f;
+      auto compose = [&](int l) {
+        p = times_a(cs[l][v], p);
+        b = step(cs[l][v], b, to_float(xr[l].v[v]));
+      };
+      auto onward = [&](int l) { r = times_a(cs[l][v], e[l][v] + r); };
+      if (n == STEPS) {
 #pragma unroll
-      for (int l = 0; l < STEPS; ++l) {
-        p *= a[l][v];
-        h = fmaf(a[l][v], h, b[l][v] * xs[l][v]);
+        for (int l = 0; l < STEPS; ++l) compose(l);
+#pragma unroll
+        for (int l = STEPS - 1; l >= 0; --l) onward(l);
+      } else {
+#pragma unroll
+        for (int l = 0; l < STEPS; ++l)
+          if (l < n) compose(l);
+#pragma unroll
+        for (int l = STEPS - 1; l >= 0; --l)
+          if (l < n) onward(l);
       }
-#pragma unroll
-      for (int l = STEPS - 1; l >= 0; --l) r = a[l][v] * (e[l][v] + r);
-      maps[half][warp][lane * V + v] = make_float2(p, h);
+      maps[half][warp][lane * V + v] = make_float2(p, b);
       back[half][warp][lane * V + v] = r;
     }
     __syncthreads();
-    float h[V], m[V];
+    // (p, b) of this thread: the warps behind its own, in the direction of the gradient; then of the whole CTA
+    float p[V], b[V], m[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      h[v] = live ? A.marks[(q.mark0 + t0 / MARK) * A.C + c + v] : 0.0f;
+      float tp = 1.0f, tb = 0.0f;
+#pragma unroll
+      for (int w = WARPS - 1; w >= 0; --w) {
+        if (w == warp) p[v] = tp, b[v] = tb;
+        const float k = maps[half][w][lane * V + v].x;
+        tb = fmaf(k, tb, back[half][w][lane * V + v]);
+        tp *= k;
+      }
 #pragma unroll
       for (int w = 0; w < WARPS - 1; ++w)
         if (w < warp) {
           const float2 k = maps[half][w][lane * V + v];
           h[v] = fmaf(k.x, h[v], k.y);
         }
-      float r = mu[v];
-#pragma unroll
-      for (int w = WARPS - 1; w >= 0; --w) {
-        if (w == warp) m[v] = r;
-        r = fmaf(maps[half][w][lane * V + v].x, r, back[half][w][lane * V + v]);
+      if (K.size > 1) {
+        for (uint32_t r = warp; r < K.size; r += WARPS) K.put(&peers[half][K.rank][lane * V + v], r, make_float2(tp, tb));
+      } else {
+        m[v] = fmaf(p[v], mu[v], b[v]);
+        mu[v] = fmaf(tp, mu[v], tb);
       }
-      mu[v] = r;
     }
-    // forward over the steps: xs becomes D_t = h_{t-1} - x_t, and dg is done
+    if (K.size > 1) {
+      K.sync();
 #pragma unroll
-    for (int l = 0; l < STEPS; ++l) {
+      for (int v = 0; v < V; ++v) {
+        float r = mu[v];
+        for (int k = (int)K.size - 1; k >= 0; --k) {
+          if (k == (int)K.rank) m[v] = fmaf(p[v], r, b[v]);
+          const float2 w = peers[half][k][lane * V + v];
+          r = fmaf(w.x, r, w.y);
+        }
+        mu[v] = r;
+      }
+    }
+    const int64_t at = (q.row0 + t1) * A.C + c;
+    float D[STEPS][V];
+    // forward over the steps: D_t = h_{t-1} - x_t, and dg is done
+    auto ahead = [&](int l) {
       float o[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const float hn = fmaf(a[l][v], h[v], b[l][v] * xs[l][v]);
-        xs[l][v] = h[v] - xs[l][v];
-        h[v] = hn;
+        const float xv = to_float(xr[l].v[v]);
+        D[l][v] = h[v] - xv;
+        h[v] = step(cs[l][v], h[v], xv);
         if (GATE) {
-          const float z = to_float(gr[l].v[v]), w = sg[l][v];
-          o[v] = dy ? to_float(dr[l].v[v]) * hn * (w * fmaf(z, 1.0f - w, 1.0f)) : 0.0f;
+          const float z = to_float(gr[l].v[v]), w = sigmoid(z);
+          o[v] = dy ? to_float(dr[l].v[v]) * h[v] * (w * fmaf(z, 1.0f - w, 1.0f)) : 0.0f;
         }
       }
-      if (GATE && dg && live && t1 + l < q.len) store<T, V>(dg + (q.row0 + t1 + l) * A.C + c, o);
-    }
+      if (GATE && dg && live) store<T, V>(dg + at + l * A.C, o);
+    };
     // and back: lam_t = dh_t + a_{t+1} lam_{t+1}
-#pragma unroll
-    for (int l = STEPS - 1; l >= 0; --l) {
+    auto finish = [&](int l) {
       float of[V], ox[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const float lam = e[l][v] + m[v];
-        m[v] = a[l][v] * lam;
-        ox[v] = b[l][v] * lam;
-        of[v] = ox[v] * a[l][v] * xs[l][v];
+        const float lam = e[l][v] + m[v], sm = fabsf(cs[l][v]);
+        m[v] = times_a(cs[l][v], lam);
+        ox[v] = times_q(cs[l][v], lam);
+        of[v] = lam * D[l][v] * fmaf(-sm, sm, sm);
       }
-      if (live && t1 + l < q.len) {
-        if (dx) store<T, V>(dx + (q.row0 + t1 + l) * A.C + c, ox);
-        if (df) store<T, V>(df + (q.row0 + t1 + l) * A.C + c, of);
-      }
+      if (dx && live) store<T, V>(dx + at + l * A.C, ox);
+      if (df && live) store<T, V>(df + at + l * A.C, of);
+    };
+    if (n == STEPS) {
+#pragma unroll
+      for (int l = 0; l < STEPS; ++l) ahead(l);
+#pragma unroll
+      for (int l = STEPS - 1; l >= 0; --l) finish(l);
+    } else {
+#pragma unroll
+      for (int l = 0; l < STEPS; ++l)
+        if (l < n) ahead(l);
+#pragma unroll
+      for (int l = STEPS - 1; l >= 0; --l)
+        if (l < n) finish(l);
     }
   }
-  if (warp == 0 && live && A.dh0) store<float, V>(A.dh0 + s * A.C + c, mu);
-  clear_outside<T, V>(A, q, s, c, live, warp, df, dx, dg);
+  if (K.rank == 0 && warp == 0 && live && A.dh0) store<float, V>(A.dh0 + s * A.C + c, mu);
+  clear_outside<T, V>(A, q, s, c, live, K.rank * WARPS + warp, K.size * WARPS, df, dx, dg);
 }
 
 struct StepArgs {
@@ -322,13 +454,10 @@ __global__ void __launch_bounds__(256) gated_step_kernel(const StepArgs A) {
     float hn[V], o[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      float a, b;
-      sigmoid_pair(to_float(f.v[v]), a, b);
-      o[v] = hn[v] = fmaf(a, h.v[v], b * to_float(x.v[v]));
+      o[v] = hn[v] = step(coefficient(to_float(f.v[v])), h.v[v], to_float(x.v[v]));
       if (GATE) {
-        float z = to_float(g.v[v]), sg, sn;
-        sigmoid_pair(z, sg, sn);
-        o[v] *= z * sg;
+        const float z = to_float(g.v[v]);
+        o[v] *= z * sigmoid(z);
       }
     }
     store<float, V>(A.h + r * A.C + c, hn);
@@ -343,26 +472,46 @@ bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) 
 // Two channels a lane need even strides and 4-byte aligned rows; otherwise a lane takes one.
 bool pairs(const Rows& r) { return !r.p || (r.seq % 2 == 0 && r.row % 2 == 0 && aligned(r.p, 4)); }
 
-template <typename T, int V>
-void launch_scan(ScanArgs A, bool bwd, cudaStream_t st) {
-  A.tiles = (int)((A.C + 32 * V - 1) / (32 * V));
-  const unsigned grid = (unsigned)(A.S * A.tiles);
-  if (!bwd) {
-    if (A.g.p) gated_scan_fwd_kernel<T, V, true><<<grid, WARPS * 32, 0, st>>>(A);
-    else gated_scan_fwd_kernel<T, V, false><<<grid, WARPS * 32, 0, st>>>(A);
-  } else {
-    if (A.g.p) gated_scan_bwd_kernel<T, V, true><<<grid, WARPS * 32, 0, st>>>(A);
-    else gated_scan_bwd_kernel<T, V, false><<<grid, WARPS * 32, 0, st>>>(A);
-  }
+// CTAs of a cluster: the time axis is split until the GPU has enough CTAs to hide its memory's latency, as far as the
+// (mean) length has pieces for them.  Packed sequences are split further, since a few of them may hold most rows.
+int cluster_size(const ScanArgs& A) {
+  const int64_t units = A.S * A.tiles, len = A.cu ? A.T / 4 : A.T;
+  int k = 1;
+  while (k < MOST_CTAS && units * k < 3 * 148 && len > (int64_t)k * MARK) k *= 2;
+  return k;
 }
 
-void dispatch_scan(const ScanArgs& A, int dtype, bool bwd, cudaStream_t st) {
+template <typename T, int V>
+cudaError_t launch_scan(ScanArgs A, bool bwd, cudaStream_t st) {
+  A.tiles = (int)((A.C + 32 * V - 1) / (32 * V));
+  void (*kernel)(const ScanArgs) = bwd ? (A.g.p ? gated_scan_bwd_kernel<T, V, true> : gated_scan_bwd_kernel<T, V, false>)
+                                       : (A.g.p ? gated_scan_fwd_kernel<T, V, true> : gated_scan_fwd_kernel<T, V, false>);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = cluster_size(A), at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
+  if (at.val.clusterDim.x > 8)  // 8 is the size that every GPU takes; sm_100a takes 16 when asked to
+    if (cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                             cudaFuncAttributeNonPortableClusterSizeAllowed, 1))
+      return e;
+  cfg.gridDim = dim3((unsigned)(A.S * A.tiles * at.val.clusterDim.x));
+  cfg.blockDim = dim3(WARPS * 32);
+  cfg.stream = st;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, (const ScanArgs)A);
+}
+
+int dispatch_scan(const ScanArgs& A, int dtype, bool bwd, cudaStream_t st, const char* who) {
   const bool two = A.C % 2 == 0 && pairs(A.f) && pairs(A.x) && pairs(A.g) && pairs(A.dy);
-  if (dtype == CSN_F32) launch_scan<float, 1>(A, bwd, st);
-  else if (dtype == CSN_BF16 && two) launch_scan<__nv_bfloat16, 2>(A, bwd, st);
-  else if (dtype == CSN_BF16) launch_scan<__nv_bfloat16, 1>(A, bwd, st);
-  else if (two) launch_scan<__half, 2>(A, bwd, st);
-  else launch_scan<__half, 1>(A, bwd, st);
+  cudaError_t e;
+  if (dtype == CSN_F32) e = launch_scan<float, 1>(A, bwd, st);
+  else if (dtype == CSN_BF16 && two) e = launch_scan<__nv_bfloat16, 2>(A, bwd, st);
+  else if (dtype == CSN_BF16) e = launch_scan<__nv_bfloat16, 1>(A, bwd, st);
+  else if (two) e = launch_scan<__half, 2>(A, bwd, st);
+  else e = launch_scan<__half, 1>(A, bwd, st);
+  if (e != cudaSuccess) return set_cuda_error(e, who);
+  return check_launch(who);
 }
 
 int check_scan(const char* who, const ScanArgs& A, int dtype) {
@@ -405,8 +554,7 @@ extern "C" int csn_gated_scan_fwd(const void* f, const void* x, const void* gate
   A.h0 = h0, A.cu = cu_seqlens, A.y = y, A.h_last = h_last, A.marks = marks;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   KernelTimer kt("gated_scan_fwd", st);
-  dispatch_scan(A, dtype, false, st);
-  return check_launch("csn_gated_scan_fwd");
+  return dispatch_scan(A, dtype, false, st, "csn_gated_scan_fwd");
 }
 
 extern "C" int csn_gated_scan_bwd(const void* f, const void* x, const void* gate, const void* dy,
@@ -436,8 +584,7 @@ extern "C" int csn_gated_scan_bwd(const void* f, const void* x, const void* gate
   A.df = df, A.dx = dx, A.dg = gate ? dgate : nullptr, A.dh0 = dh0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   KernelTimer kt("gated_scan_bwd", st);
-  dispatch_scan(A, dtype, true, st);
-  return check_launch("csn_gated_scan_bwd");
+  return dispatch_scan(A, dtype, true, st, "csn_gated_scan_bwd");
 }
 
 namespace csn {

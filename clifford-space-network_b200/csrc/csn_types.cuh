@@ -35,14 +35,15 @@ struct alignas(sizeof(T) * V) Pack {
   T v[V];
 };
 
-// sigmoid(z) and 1 - sigmoid(z) = sigmoid(-z), both to full relative precision: with
-// e = exp(-|z|), the larger is 1 / (1 + e) and the smaller e / (1 + e).
-__device__ __forceinline__ void sigmoid_pair(float z, float& a, float& q) {
-  const float e = expf(-fabsf(z));
-  const float r = __fdividef(1.0f, 1.0f + e);
-  const float er = e * r;
-  a = z >= 0.0f ? r : er;
-  q = z >= 0.0f ? er : r;
+// min(sigmoid(z), sigmoid(-z)) = e / (1 + e) with e = exp(-|z|), to full relative precision; the other of the two is
+// one minus it.  The fast exponential rounds its argument: off by (4 + 2 |z|) 2^-24 relative, and the quotient by
+// 2^-22, which a recurrence sees at random and not as a drift.
+__device__ __forceinline__ float sigmoid_small(float z) {
+  const float e = __expf(-fabsf(z));
+  return __fdividef(e, 1.0f + e);
 }
+
+// sigmoid(z); 0 where exp(-z) is too large for float32
+__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
 
 }  // namespace csn

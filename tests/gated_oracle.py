@@ -1,10 +1,10 @@
 """64-bit forms of the gated recurrent block's operators, each with a bound on the rounding of a
 float32 computation of it (numpy, element by element, no code of the package).
 
-Units: U = 2^-24 is half a step of float32.  exp is off by at most 2 steps (4 U), a quotient by 2
-steps (4 U), a product, sum or fused product by 1 U.  So the larger of sigmoid(z), sigmoid(-z) is off
-by at most 7 U, the smaller by 12 U, and with the products around them a step of the recurrence
-adds at most 16 U of the sizes of its two terms."""
+Units: U = 2^-24 is half a step of float32.  A product, sum or fused product is off by at most 1 U, a
+quotient by 2 steps (4 U), the fast exp(z) by 2 steps and, since it rounds its argument, 2 |z| U.  So
+s = min(sigmoid(z), sigmoid(-z)) = e / (1 + e) is off by at most (12 + 2 |z|) U of itself, and so is
+sigmoid(z) where it is the smaller (the larger by less)."""
 import numpy as np
 
 U = 2.0 ** -24
@@ -31,7 +31,11 @@ def gated_scan(f, x, h0, gate, borders, dy=None, dh=None):
     z = gate if gate is not None else None
     w = sigmoid(z) if z is not None else None
     silu = z * w if z is not None else np.ones_like(f)
-    silu_err = 14 * U * np.abs(silu) if z is not None else np.zeros_like(f)
+    # the recurrence is h + s (x - h) or x + s (h - x); composing steps rounds the products of a and the
+    # partial states once more each
+    small, s_err = np.minimum(a, q), (12 + 2 * np.abs(f)) * U
+    fast = (14 + 2 * np.abs(z)) * U if z is not None else np.zeros_like(f)
+    silu_err = fast * np.abs(silu)
     h, he = np.zeros((L, C)), np.zeros((L, C))
     before, be = np.zeros((L, C)), np.zeros((L, C))
     last, laste = np.zeros_like(h0), np.zeros_like(h0)
@@ -41,7 +45,7 @@ def gated_scan(f, x, h0, gate, borders, dy=None, dh=None):
         v, err = h0[s].copy(), np.zeros(C)
         for t in range(b, e):
             before[t], be[t] = v, err
-            err = a[t] * err + 16 * U * (a[t] * np.abs(v) + q[t] * np.abs(x[t]))
+            err = a[t] * err + s_err[t] * small[t] * np.abs(x[t] - v) + 4 * U * (np.abs(v) + np.abs(x[t]))
             v = a[t] * v + q[t] * x[t]
             h[t], he[t] = v, err
         last[s], laste[s] = v, err
@@ -60,18 +64,18 @@ def gated_scan(f, x, h0, gate, borders, dy=None, dh=None):
         for t in range(e - 1, b - 1, -1):
             lam[t] = e_t[t] + m
             le[t] = e_err[t] + me + 2 * U * (np.abs(e_t[t]) + np.abs(m))
-            m, me = a[t] * lam[t], a[t] * le[t] + 16 * U * a[t] * (np.abs(e_t[t]) + np.abs(m))
+            m, me = a[t] * lam[t], a[t] * le[t] + (s_err[t] * small[t] + 4 * U) * np.abs(lam[t])
         dh0[s], dh0e[s] = m, me
     D = before - x
     De = be + U * (np.abs(before) + np.abs(x))
     df, dx = lam * D * a * q, lam * q
-    out["dx"] = (dx, q * le + 14 * U * np.abs(dx))
-    out["df"] = (df, np.abs(lam * a * q) * De + np.abs(D * a * q) * le + 28 * U * np.abs(df))
+    out["dx"] = (dx, q * le + (s_err * small + 2 * U * q) * np.abs(lam))
+    out["df"] = (df, np.abs(lam * a * q) * De + np.abs(D * a * q) * le + (s_err + 6 * U) * np.abs(df))
     out["dh0"] = (dh0, dh0e)
     if z is not None:
         slope = w * (1 + z * (1 - w))
-        # 1 - w is off by 8 U at most, and 1 + z (1 - w) by that times |z| and its own rounding
-        slope_err = w * (8 * U * np.abs(z) + 10 * U * (1 + np.abs(z) * (1 - w)))
+        # 1 - w is off by `fast` at most, and 1 + z (1 - w) by that times |z| and its own rounding
+        slope_err = w * (fast * np.abs(z) + 2 * fast * (1 + np.abs(z) * (1 - w)))
         out["dgate"] = (inside * dy * h * slope, inside * np.abs(dy) * (he * np.abs(slope) + np.abs(h) * slope_err
                                                                         + 2 * U * np.abs(h * slope)))
     return out
