@@ -133,13 +133,14 @@ def _gated_scan_fwd(f, x, h0, gate, cu, keep):
 
 
 def _gated_scan_bwd(f, x, gate, cu, marks, dy, dh_last, need):
-    """Gradients (df, dx, dh0, dgate) where `need` asks for them, None elsewhere."""
+    """Gradients (df, dx, dh0, dgate); dh0 where `need` asks for it, dgate where there is a gate."""
+    if dy is None:  # only the last states are used
+        dy = f.new_zeros((1,) * f.dim()).expand(f.shape)
     f, x, gate, dy, dh_last = _rows(f), _rows(x), _rows(gate), _rows(dy), _packed(dh_last)
     S, T, C = _scan_sizes(f, cu)
-    df = f.new_empty(f.shape) if need[0] else None
-    dx = f.new_empty(f.shape) if need[1] else None
+    df, dx = f.new_empty(f.shape), f.new_empty(f.shape)
     dh0 = f.new_empty((S, C), dtype=torch.float32) if need[2] else None
-    dgate = f.new_empty(f.shape) if need[3] and gate is not None else None
+    dgate = f.new_empty(f.shape) if gate is not None else None
     _launch("csn_gated_scan_bwd", f.get_device(), _ptr(f), _ptr(x), _ptr(gate), _ptr(dy),
             _row_strides(f, x, gate, dy), _ptr(cu), _ptr(marks), _ptr(dh_last), _ptr(df), _ptr(dx), _ptr(dgate),
             _ptr(dh0), S, T, C, DTYPES[f.dtype])

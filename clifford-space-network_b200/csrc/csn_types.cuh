@@ -29,21 +29,101 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { re
 template <>
 __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
+// two floats rounded to a pair of 16-bit numbers, the first in the low half
+template <typename T>
+__device__ __forceinline__ uint32_t pack(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack<float>(float a, float) { return __float_as_uint(a); }
+template <>
+__device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float a, float b) {
+  __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack<__half>(float a, float b) {
+  __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+
 // V neighbouring elements of type T as they lie in memory: one access
 template <typename T, int V>
 struct alignas(sizeof(T) * V) Pack {
   T v[V];
 };
 
-// min(sigmoid(z), sigmoid(-z)) = e / (1 + e) with e = exp(-|z|), to full relative precision; the other of the two is
-// one minus it.  The fast exponential rounds its argument: off by (4 + 2 |z|) 2^-24 relative, and the quotient by
-// 2^-22, which a recurrence sees at random and not as a drift.
-__device__ __forceinline__ float sigmoid_small(float z) {
-  const float e = __expf(-fabsf(z));
-  return __fdividef(e, 1.0f + e);
+// ------------------------------------------------------------- V float32 values
+// One or two channels of a lane.
+template <int V>
+struct Vals {
+  float v[V];
+  __device__ __forceinline__ float get(int i) const { return v[i]; }
+  static __device__ __forceinline__ Vals make(float a, float b) {
+    Vals r;
+    r.v[0] = a;
+    if (V > 1) r.v[V - 1] = b;
+    return r;
+  }
+};
+template <int V>
+__device__ __forceinline__ Vals<V> splat(float a) { return Vals<V>::make(a, a); }
+template <int V>
+__device__ __forceinline__ Vals<V> fma(Vals<V> a, Vals<V> b, Vals<V> c) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) c.v[i] = fmaf(a.v[i], b.v[i], c.v[i]);
+  return c;
+}
+template <int V>
+__device__ __forceinline__ Vals<V> operator*(Vals<V> a, Vals<V> b) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) a.v[i] *= b.v[i];
+  return a;
+}
+template <int V>
+__device__ __forceinline__ Vals<V> operator+(Vals<V> a, Vals<V> b) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) a.v[i] += b.v[i];
+  return a;
+}
+template <int V>
+__device__ __forceinline__ Vals<V> operator-(Vals<V> a, Vals<V> b) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) a.v[i] -= b.v[i];
+  return a;
 }
 
-// sigmoid(z); 0 where exp(-z) is too large for float32
-__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float inverse_fast(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+constexpr float LOG2E = 1.4426950408889634f;
+
+// a = sigmoid(z) and q = 1 - a = sigmoid(-z): the smaller is s = e / (1 + e) with e = exp(-|z|), off by a few units of
+// its own (and 2 |z| 2^-24 relative, since the exponential's argument is rounded); the larger is 1 - s, rounded once.
+template <int V>
+__device__ __forceinline__ void sigmoid_pair(Vals<V> z, Vals<V>& a, Vals<V>& q) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const float e = exp2_fast(-LOG2E * fabsf(z.v[i]));
+    const float s = e * inverse_fast(1.0f + e), l = 1.0f - s;
+    const bool up = z.v[i] >= 0.0f;
+    a.v[i] = up ? l : s;
+    q.v[i] = up ? s : l;
+  }
+}
+
+// sigmoid(z), with the same error; 0 where exp(-z) is too large for float32
+__device__ __forceinline__ float sigmoid(float z) { return inverse_fast(1.0f + exp2_fast(-LOG2E * z)); }
+template <int V>
+__device__ __forceinline__ Vals<V> sigmoid(Vals<V> z) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) z.v[i] = sigmoid(z.v[i]);
+  return z;
+}
 
 }  // namespace csn

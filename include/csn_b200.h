@@ -417,15 +417,15 @@ enum csn_dtype { CSN_F32 = 0, CSN_BF16 = 1, CSN_F16 = 2 };
  *     out as 0.  Borders are cut to 0 .. T and to their order; they must not fall.
  * h0 [S, C] (NULL = 0), h_last [S, C] (the state after the last step; NULL = not wanted).
  * marks: NULL, or csn_gated_scan_marks(S, T, C, packed) floats that csn_gated_scan_bwd reads.
- * f, x, gate aligned to their type; everything else 16-byte aligned. */
+ * f, x, gate aligned to their type; everything else 16-byte aligned.  T <= 2^30. */
 int64_t csn_gated_scan_marks(int64_t S, int64_t T, int64_t C, int packed);
 int csn_gated_scan_fwd(const void* f, const void* x, const void* gate, const int64_t* strides,
                        const float* h0, const int32_t* cu_seqlens, void* y, float* h_last,
                        float* marks, int64_t S, int64_t T, int64_t C, int dtype, void* stream);
 
-/* Adjoint of csn_gated_scan_fwd on the same inputs and its marks: dy (NULL = 0; strides[6],
- * strides[7]) and dh_last [S, C] (NULL = 0) to df, dx, dgate (contiguous, in y's layout) and
- * dh0 [S, C]; each output may be NULL. */
+/* Adjoint of csn_gated_scan_fwd on the same inputs and its marks: dy (strides[6], strides[7]) and
+ * dh_last [S, C] (NULL = 0) to df, dx, with a gate dgate (contiguous, in y's layout) and dh0
+ * [S, C] (NULL = not wanted). */
 int csn_gated_scan_bwd(const void* f, const void* x, const void* gate, const void* dy,
                        const int64_t* strides, const int32_t* cu_seqlens, const float* marks,
                        const float* dh_last, void* df, void* dx, void* dgate, float* dh0,
