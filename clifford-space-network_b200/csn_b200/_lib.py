@@ -91,8 +91,10 @@ SIGNATURES = {
     "csn_spatial_generators_fwd": ([_f, _f, _f, _f, _f, _f, _f, _f, _i64, _i64, _i64, _int, _f], _int),
     "csn_spatial_generators_bwd": ([_f] * 13 + [_i64, _i64, _i64, _int, _f], _int),
     "csn_gated_scan_marks": ([_i64, _i64, _i64, _int], _i64),
-    "csn_gated_scan_fwd": ([_f, _f, _f, _strides, _f, _f, _f, _f, _f, _i64, _i64, _i64, _int, _f], _int),
-    "csn_gated_scan_bwd": ([_f, _f, _f, _f, _strides, _f, _f, _f, _f, _f, _f, _f, _i64, _i64, _i64, _int, _f], _int),
+    "csn_gated_scan_workspace_bytes": ([_i64, _i64, _i64, _int, _int, _int], _sz),
+    "csn_gated_scan_fwd": ([_f, _f, _f, _strides, _f, _f, _f, _f, _f, _i64, _i64, _i64, _int, _f, _sz, _f], _int),
+    "csn_gated_scan_bwd": ([_f, _f, _f, _f, _strides, _f, _f, _f, _f, _f, _f, _f, _i64, _i64, _i64, _int, _f, _sz, _f],
+                           _int),
     "csn_gated_step": ([_f, _f, _f, _strides, _f, _f, _i64, _i64, _int, _f], _int),
     "csn_silu_gated_linear_bwd_workspace_bytes": ([_i64, _i64, _i64], _sz),
     "csn_silu_gated_linear_fwd": ([_f, _i64, _f, _i64, _f, _i64, _f, _i64, _i64, _i64, _int, _f], _int),

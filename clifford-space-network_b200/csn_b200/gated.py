@@ -117,6 +117,11 @@ def _scan_sizes(f, cu):
     return (n[0], n[1], n[2]) if cu is None else (cu.shape[0] - 1, n[0], n[1])
 
 
+def _scan_workspace(f, S, T, C, cu, backward):
+    nb = _lib.load().csn_gated_scan_workspace_bytes(S, T, C, int(cu is not None), DTYPES[f.dtype], backward)
+    return (f.new_empty((nb,), dtype=torch.uint8) if nb else None), nb
+
+
 def _gated_scan_fwd(f, x, h0, gate, cu, keep):
     """(y, h_last, marks or None) of rows as they lie; h0 float32."""
     f, x, gate, h0 = _rows(f), _rows(x), _rows(gate), _packed(h0)
@@ -127,8 +132,9 @@ def _gated_scan_fwd(f, x, h0, gate, cu, keep):
     marks = None
     if keep:
         marks = f.new_empty((_lib.load().csn_gated_scan_marks(S, T, C, int(cu is not None)),), dtype=torch.float32)
+    ws, nb = _scan_workspace(f, S, T, C, cu, 0)
     _launch("csn_gated_scan_fwd", index, _ptr(f), _ptr(x), _ptr(gate), _row_strides(f, x, gate), _ptr(h0), _ptr(cu),
-            _ptr(y), _ptr(h_last), _ptr(marks), S, T, C, DTYPES[f.dtype])
+            _ptr(y), _ptr(h_last), _ptr(marks), S, T, C, DTYPES[f.dtype], _ptr(ws), nb)
     return y, h_last, marks
 
 
@@ -141,9 +147,10 @@ def _gated_scan_bwd(f, x, gate, cu, marks, dy, dh_last, need):
     df, dx = f.new_empty(f.shape), f.new_empty(f.shape)
     dh0 = f.new_empty((S, C), dtype=torch.float32) if need[2] else None
     dgate = f.new_empty(f.shape) if gate is not None else None
+    ws, nb = _scan_workspace(f, S, T, C, cu, 1)
     _launch("csn_gated_scan_bwd", f.get_device(), _ptr(f), _ptr(x), _ptr(gate), _ptr(dy),
             _row_strides(f, x, gate, dy), _ptr(cu), _ptr(marks), _ptr(dh_last), _ptr(df), _ptr(dx), _ptr(dgate),
-            _ptr(dh0), S, T, C, DTYPES[f.dtype])
+            _ptr(dh0), S, T, C, DTYPES[f.dtype], _ptr(ws), nb)
     return df, dx, dh0, dgate
 
 

@@ -7,11 +7,14 @@
 //
 // Each step is an affine map h -> a h + b, and maps compose: (a2, b2) o (a1, b1) = (a2 a1, a2 b1 + b2).  A warp takes
 // STEPS neighbouring steps of 128 bytes of neighbouring channels (two to a lane in 16 bits, one in float32) and
-// composes them in registers; the warps of a CTA pass their maps through
-// shared memory, the CTAs of a cluster, which take neighbouring MARK-step pieces of one sequence, through distributed
-// shared memory; then every warp runs its steps again from the state that enters them.  So inputs are read once: each
-// warp copies its rows into shared memory with cp.async one pass ahead of their use.  Sums, products and states are
-// float32 and in a fixed order.
+// composes them in registers; the warps of a CTA, which take neighbouring steps, pass their maps through shared
+// memory; then every warp runs its steps again from the state that enters them.  So the inputs are read once: each
+// warp copies its rows into shared memory with cp.async one pass (MARK steps) ahead of their use.
+//
+// Where there are too few sequences and channels to fill the GPU, sequences are cut into chunks: reduce_kernel composes
+// the map of every chunk that another follows (it reads f and x once more, mostly from L2), and the CTA of a chunk
+// composes those before it into the state that enters it.  All sums, products and states are float32 and in an order
+// that the sizes alone fix.
 //
 // The forward pass keeps the float32 state before every MARK-th step ("marks") where a backward pass will follow:
 // the adjoint forms the states between two marks again instead of reading rounded outputs (y is not h where there is
@@ -44,31 +47,62 @@ struct ScanArgs {
   void *df, *dx, *dg;
   float* dh0;
   int64_t S, T, C;
+  float2* maps;  // [units][C]: the maps of chunks that another follows (backward: that follow another)
   int tiles;
+  int chunk;     // steps of a chunk, a multiple of MARK
+  int chunks;    // of a sequence, where all have one length
   bool wide;  // every row starts on 16 bytes and holds multiples of 16
 };
 
-// The rows of sequence s.  Borders outside 0..T, or falling ones, are cut to what is there.
-struct Seq {
-  int64_t row0;  // its first row in the outputs
-  int len;
-  int64_t mark0;  // its first mark: room for ceil(len / MARK) of them whatever the other lengths are
-  __device__ __forceinline__ Seq(const ScanArgs& A, int64_t s) {
+// The part of a sequence that a CTA works on.  Unit u is chunk u % chunks of sequence u / chunks, or, in a packed
+// batch, where sequence s begins with unit cu[s] / chunk + s (room for its chunks whatever the other lengths are), the
+// one that the borders give; some units are empty.  Borders outside 0..T, or falling ones, are cut to what is there.
+struct Part {
+  int64_t s;      // sequence; -1: none
+  int64_t row0;   // its first row in the outputs
+  int64_t unit;
+  int len;        // its steps
+  int k;          // chunk of the sequence
+  int from, to;   // steps of the chunk
+  int64_t mark0;  // the sequence's first mark: room for ceil(len / MARK) of them
+
+  __device__ __forceinline__ int64_t border(const ScanArgs& A, int64_t i) const {
+    return min(max((int64_t)A.cu[i], (int64_t)0), A.T);
+  }
+  __device__ __forceinline__ Part(const ScanArgs& A, int64_t u) : unit(u) {
     if (A.cu) {
-      const int64_t b = min(max((int64_t)A.cu[s], (int64_t)0), A.T);
-      const int64_t e = min(max((int64_t)A.cu[s + 1], b), A.T);
-      row0 = b;
-      len = (int)(e - b);
+      // the last s that begins at unit u or before: each round, 32 lanes look at 32 places of what is left
+      int64_t lo = 0, n = A.S;
+      while (n > 0) {
+        const int64_t step = (n + 31) / 32, i = lo + (threadIdx.x & 31) * step;
+        const bool yes = i < lo + n && border(A, i) / A.chunk + i <= u;
+        const int c = __popc(__ballot_sync(0xffffffffu, yes));
+        if (c == 0) break;
+        lo += (c - 1) * step;
+        n = step == 1 ? 0 : min(step, A.S - lo);
+      }
+      s = border(A, lo) / A.chunk + lo <= u ? lo : -1;
+      if (s < 0) return;
+      row0 = border(A, s);
+      len = (int)(max(border(A, s + 1), row0) - row0);
+      k = (int)(u - (row0 / A.chunk + s));
     } else {
+      s = u / A.chunks;
       row0 = s * A.T;
       len = (int)A.T;
+      k = (int)(u - s * A.chunks);
     }
     mark0 = row0 / MARK + s;
+    const int64_t first = (int64_t)k * A.chunk;
+    from = (int)min(first, (int64_t)len);
+    to = (int)min(first + A.chunk, (int64_t)len);
+    if (k > 0 && from >= len) s = -1;
   }
 };
 
-constexpr int ROW = 144;            // bytes of a tile's row in shared memory: 128, and a word more where rows are odd
-constexpr int PIECE = MARK * ROW;   // of one tensor's rows of one CTA pass
+// bytes of a tile's row in shared memory: 128, and a word more (kept to 16 bytes) where rows are odd
+__host__ __device__ constexpr int row_bytes(bool odd) { return odd ? 144 : 128; }
+__host__ __device__ constexpr int piece_bytes(bool odd) { return MARK * row_bytes(odd); }  // of one tensor's rows of one CTA pass
 
 template <typename T>
 struct Lane {
@@ -110,17 +144,18 @@ struct Input {
   int64_t row;    // bytes
   int left;       // ODD: bytes of the tile
 
-  __device__ __forceinline__ Input(const Rows& r, const ScanArgs& A, const Seq& q, int64_t s, int64_t tile, int t1) {
+  __device__ __forceinline__ Input(const Rows& r, const ScanArgs& A, const Part& q, int64_t tile, int t1) {
     p = nullptr;
     row = r.row * (int64_t)sizeof(T);
     left = (int)min((int64_t)32 * Lane<T>::V, A.C - tile) * (int)sizeof(T);
     if (!r.p) return;
     const int lane = threadIdx.x & 31;
-    p = static_cast<const char*>(r.p) + ((A.cu ? q.row0 * r.row : s * r.seq) + tile) * (int64_t)sizeof(T) + t1 * row;
+    p = static_cast<const char*>(r.p) + ((A.cu ? q.row0 * r.row : q.s * r.seq) + tile) * (int64_t)sizeof(T) + t1 * row;
     if (!ODD) p += A.wide ? (lane >> 3) * row + (lane & 7) * 16 : lane * 4;
   }
   // the warp's n rows into shared memory at `to`, then `step` rows on
   __device__ __forceinline__ void copy(char* to, int n, bool wide, int step) {
+    constexpr int ROW = row_bytes(ODD);
     const int lane = threadIdx.x & 31;
     const uint32_t at = (uint32_t)__cvta_generic_to_shared(to);
     if (ODD) {
@@ -180,13 +215,14 @@ __device__ __forceinline__ void store_row(T* p, Vals<Lane<T>::V> o, int have) {
 
 // Rows that belong to no sequence (before the first, behind the last) are written as 0.
 template <typename T, bool ODD>
-__device__ __noinline__ void clear_outside(const ScanArgs& A, const Seq& q, int64_t s, int64_t c, int have, int first,
-                                           int step, T* o) {
+__device__ __noinline__ void clear_outside(const ScanArgs& A, const Part& q, int64_t c, int have, void* out) {
+  T* o = static_cast<T*>(out);
   const Vals<Lane<T>::V> zero = splat<Lane<T>::V>(0.0f);
-  if (s == 0)
-    for (int64_t r = first; r < q.row0; r += step) store_row<T, ODD>(o + r * A.C + c, zero, have);
-  if (s == A.S - 1)
-    for (int64_t r = q.row0 + q.len + first; r < A.T; r += step) store_row<T, ODD>(o + r * A.C + c, zero, have);
+  const int warp = threadIdx.x >> 5;
+  if (q.s == 0)
+    for (int64_t r = warp; r < q.row0; r += WARPS) store_row<T, ODD>(o + r * A.C + c, zero, have);
+  if (q.s == A.S - 1)
+    for (int64_t r = q.row0 + q.len + warp; r < A.T; r += WARPS) store_row<T, ODD>(o + r * A.C + c, zero, have);
 }
 
 __device__ __forceinline__ void copies_queued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -194,70 +230,145 @@ __device__ __forceinline__ void copies_done() {
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncwarp();
 }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ int cluster_rank() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return (int)r;
-}
-__device__ __forceinline__ int cluster_ranks() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return (int)r;
-}
 
-// A map h -> p h + b of V channels, and its copy in another CTA's shared memory
+// A map h -> p h + b of V channels
 template <int V>
 struct alignas(8 * V) Map {
   Vals<V> p, b;
-  __device__ __forceinline__ void put(Map* to, int cta) const {
-    uint32_t a;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(to)), "r"(cta));
-    if (V == 1)
-      asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(a), "f"(p.get(0)), "f"(b.get(0)) : "memory");
-    else
-      asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(a), "f"(p.get(0)), "f"(p.get(V - 1)),
-                   "f"(b.get(0)), "f"(b.get(V - 1))
-                   : "memory");
-  }
+  __device__ __forceinline__ Vals<V> of(Vals<V> h) const { return fma(p, h, b); }
+  __device__ __forceinline__ Map after(const Map& m) const { return {p * m.p, fma(p, m.b, b)}; }
+  static __device__ __forceinline__ Map none() { return {splat<V>(1.0f), splat<V>(0.0f)}; }
 };
-constexpr int MOST_CTAS = 16;  // of a cluster
+
+// A chunk's map in memory
+template <int V>
+__device__ __forceinline__ Map<V> load_map(const float2* p, int have) {
+  const float2 u = have > 0 ? p[0] : make_float2(1.0f, 0.0f), w = V > 1 && have > 1 ? p[V - 1] : u;
+  return {Vals<V>::make(u.x, w.x), Vals<V>::make(u.y, w.y)};
+}
+template <int V>
+__device__ __forceinline__ void store_map(float2* p, const Map<V>& m, int have) {
+  if (have > 0) p[0] = make_float2(m.p.get(0), m.b.get(0));
+  if (V > 1 && have > 1) p[V - 1] = make_float2(m.p.get(V - 1), m.b.get(V - 1));
+}
+
+// The value that enters a chunk: `v` through the maps of n chunks from unit u on, each `step` units further.  The warps
+// compose n / WARPS neighbouring ones each.
+template <int V>
+__device__ __forceinline__ Vals<V> enter(const ScanArgs& A, Map<V> (*maps)[32], Vals<V> v, int64_t u, int n, int step,
+                                         int64_t c, int have) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  Map<V> m = Map<V>::none();
+#pragma unroll 4
+  for (int j = n * warp / WARPS; j < n * (warp + 1) / WARPS; ++j) m = load_map<V>(A.maps + (u + j * step) * A.C + c, have).after(m);
+  maps[warp][lane] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) v = maps[w][lane].of(v);
+  return v;
+}
+
+// The map of a chunk that another follows; BACK: of the gradient, through a chunk that follows another.  Each warp
+// composes a contiguous eighth of the chunk.
+template <typename T, bool GATE, bool ODD, bool BACK>
+__global__ void __launch_bounds__(WARPS * 32, 3) reduce_kernel(const __grid_constant__ ScanArgs A) {
+  using F = typename Lane<T>::F;
+  constexpr int V = Lane<T>::V, N = BACK && GATE ? 3 : 2, ROW = row_bytes(ODD), PIECE = piece_bytes(ODD);
+  extern __shared__ __align__(128) char ring[];  // [2][N][MARK rows]
+  __shared__ Map<V> maps[WARPS][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Part q(A, blockIdx.x / A.tiles);
+  if (q.s < 0 || (BACK ? q.k == 0 : q.to == q.len)) return;
+  const int64_t tile = (int64_t)(blockIdx.x % A.tiles) * Lane<T>::CHANNELS, c = tile + lane * V;
+  const int have = (int)max((int64_t)0, min((int64_t)V, A.C - c));
+  const int share = A.chunk / WARPS, first = q.from + warp * share, past = min(first + share, q.to);
+  char* mine = ring + warp * STEPS * ROW;
+  // BACK goes from the last steps to the first
+  int t = BACK ? first + (max(past - first, 1) - 1) / STEPS * STEPS : first;
+  const int step = BACK ? -STEPS : STEPS;
+  Input<T, ODD> f(A.f, A, q, tile, t), x(BACK ? A.dy : A.x, A, q, tile, t), g(A.g, A, q, tile, t);
+  const char *f0 = f.p, *x0 = x.p, *g0 = g.p;  // ODD: STEPS rows are whole words, so the skews never change
+  auto fetch = [&](int half, int n) {
+    char* to = mine + half * N * PIECE;
+    f.copy(to, n, A.wide, step);
+    x.copy(to + PIECE, n, A.wide, step);
+    if (N > 2) g.copy(to + 2 * PIECE, n, A.wide, step);
+    copies_queued();
+  };
+  Map<V> m = Map<V>::none();
+  if (past > first) fetch(0, past - t);
+  for (int half = 0; BACK ? t >= first && past > first : t < past; t += step, half ^= 1) {
+    copies_done();
+    const int u = t + step;
+    if (BACK ? u >= first : u < past) fetch(half ^ 1, past - u);
+    const char* in = mine + half * N * PIECE;
+    const int n = past - t;
+    auto take = [&](int l) {
+      F a, w;
+      sigmoid_pair(read<T, ODD>(in + l * ROW, f.skew(f0, f.row, l)), a, w);
+      F v = read<T, ODD>(in + PIECE + l * ROW, x.skew(x0, x.row, l));
+      if (BACK) {
+        if (GATE) {
+          const F z = read<T, ODD>(in + 2 * PIECE + l * ROW, g.skew(g0, g.row, l));
+          v = v * (z * sigmoid(z));
+        }
+        m.b = a * (v + m.b);
+      } else {
+        m.b = fma(a, m.b, w * v);
+      }
+      m.p = a * m.p;
+    };
+    if (n >= STEPS) {
+#pragma unroll
+      for (int l = 0; l < STEPS; ++l) take(BACK ? STEPS - 1 - l : l);
+    } else {
+#pragma unroll
+      for (int l = 0; l < STEPS; ++l)
+        if ((BACK ? STEPS - 1 - l : l) < n) take(BACK ? STEPS - 1 - l : l);
+    }
+  }
+  maps[warp][lane] = m;
+  __syncthreads();
+  if (warp == 0) {
+    m = Map<V>::none();
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) m = maps[BACK ? WARPS - 1 - w : w][lane].after(m);
+    store_map<V>(A.maps + q.unit * A.C + c, m, have);
+  }
+}
 
 template <typename T, bool GATE, bool ODD>
 __global__ void __launch_bounds__(WARPS * 32, 3) gated_scan_fwd_kernel(const __grid_constant__ ScanArgs A) {
   using F = typename Lane<T>::F;
-  constexpr int V = Lane<T>::V, N = GATE ? 3 : 2;
+  constexpr int V = Lane<T>::V, N = GATE ? 3 : 2, ROW = row_bytes(ODD), PIECE = piece_bytes(ODD);
   extern __shared__ __align__(128) char ring[];  // [2][N][MARK rows]
-  __shared__ Map<V> maps[2][WARPS][32], peers[2][MOST_CTAS][32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = cluster_rank(), ranks = cluster_ranks();
-  const int unit = blockIdx.x / ranks;
-  const int64_t s = unit / A.tiles, tile = (int64_t)(unit % A.tiles) * Lane<T>::CHANNELS, c = tile + lane * V;
+  __shared__ Map<V> maps[2][WARPS][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Part q(A, blockIdx.x / A.tiles);
+  if (q.s < 0) return;
+  const int64_t tile = (int64_t)(blockIdx.x % A.tiles) * Lane<T>::CHANNELS, c = tile + lane * V;
   const int have = (int)max((int64_t)0, min((int64_t)V, A.C - c));
-  const Seq q(A, s);
-  T* y = static_cast<T*>(A.y);
-  F carry = A.h0 ? load_state<V>(A.h0 + s * A.C + c, have) : splat<V>(0.0f);
-  const int pass = ranks * MARK;
-  int t1 = rank * MARK + warp * STEPS;
+  int t1 = q.from + warp * STEPS;
   char* mine = ring + warp * STEPS * ROW;
-  Input<T, ODD> f(A.f, A, q, s, tile, t1), x(A.x, A, q, s, tile, t1), g(A.g, A, q, s, tile, t1);
+  Input<T, ODD> f(A.f, A, q, tile, t1), x(A.x, A, q, tile, t1), g(A.g, A, q, tile, t1);
+  const char *f0 = f.p, *x0 = x.p, *g0 = g.p;  // ODD: MARK rows are whole words, so the skews never change
   auto fetch = [&](int half, int n) {
     char* to = mine + half * N * PIECE;
-    f.copy(to, n, A.wide, pass);
-    x.copy(to + PIECE, n, A.wide, pass);
-    if (GATE) g.copy(to + 2 * PIECE, n, A.wide, pass);
+    f.copy(to, n, A.wide, MARK);
+    x.copy(to + PIECE, n, A.wide, MARK);
+    if (GATE) g.copy(to + 2 * PIECE, n, A.wide, MARK);
     copies_queued();
   };
-  const char *f0 = f.p, *x0 = x.p, *g0 = g.p;  // ODD: MARK rows are whole words, so the first pass's skews are every pass's
-  fetch(0, q.len - t1);
-  T* out = y + (q.row0 + t1) * A.C + c;
-  if (ranks > 1) cluster_sync();  // shared memory of a CTA is there once it has started
+  fetch(0, q.to - t1);
+  F carry = A.h0 ? load_state<V>(A.h0 + q.s * A.C + c, have) : splat<V>(0.0f);
+  if (q.k > 0) carry = enter<V>(A, maps[1], carry, q.unit - q.k, q.k, 1, c, have);
+  T* out = static_cast<T*>(A.y) + (q.row0 + t1) * A.C + c;
+  float* mark = A.marks + (q.mark0 + q.from / MARK) * A.C + c;
   int half = 0;
-  for (int t0 = 0; t0 < q.len; t0 += pass, t1 += pass, out += pass * A.C, half ^= 1) {
-    const int n = q.len - t1;  // steps left
+  for (int t0 = q.from; t0 < q.to; t0 += MARK, t1 += MARK, out += MARK * A.C, half ^= 1) {
+    const int n = q.to - t1;  // steps left
     copies_done();
-    if (t0 + pass < q.len) fetch(half ^ 1, n - pass);
+    if (t0 + MARK < q.to) fetch(half ^ 1, n - MARK);
     const char* in = mine + half * N * PIECE;
     F a[STEPS], b[STEPS];
 #pragma unroll
@@ -273,40 +384,19 @@ __global__ void __launch_bounds__(WARPS * 32, 3) gated_scan_fwd_kernel(const __g
     }
     Map<V> m = {a[0], b[0]};
 #pragma unroll
-    for (int l = 1; l < STEPS; ++l) {
-      m.p = a[l] * m.p;
-      m.b = fma(a[l], m.b, b[l]);
-    }
+    for (int l = 1; l < STEPS; ++l) m = Map<V>{a[l], b[l]}.after(m);
     maps[half][warp][lane] = m;
     __syncthreads();
     F h;
-    if (ranks == 1) {
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        if (w == warp) h = carry;
-        const Map<V> k = maps[half][w][lane];
-        carry = fma(k.p, carry, k.b);
-      }
-    } else {
-      // the warps before this one, and then the whole CTA
-      Map<V> before, all = {splat<V>(1.0f), splat<V>(0.0f)};
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        if (w == warp) before = all;
-        const Map<V> k = maps[half][w][lane];
-        all.b = fma(k.p, all.b, k.b);
-        all.p = k.p * all.p;
-      }
-      for (int r = warp; r < ranks; r += WARPS) all.put(&peers[half][rank][lane], r);
-      cluster_sync();
-#pragma unroll 4
-      for (int r = 0; r < ranks; ++r) {
-        if (r == rank) h = fma(before.p, carry, before.b);
-        const Map<V> k = peers[half][r][lane];
-        carry = fma(k.p, carry, k.b);
-      }
+    for (int w = 0; w < WARPS; ++w) {
+      if (w == warp) h = carry;
+      carry = maps[half][w][lane].of(carry);
     }
-    if (A.marks && warp == 0 && n > 0) store_state<V>(A.marks + (q.mark0 + t1 / MARK) * A.C + c, h, have);
+    if (A.marks) {
+      if (warp == 0) store_state<V>(mark, h, have);
+      mark += A.C;
+    }
     auto finish = [&](int l) {
       h = fma(a[l], h, b[l]);
       F o = h;
@@ -325,56 +415,57 @@ __global__ void __launch_bounds__(WARPS * 32, 3) gated_scan_fwd_kernel(const __g
         if (l < n) finish(l);
     }
   }
-  if (rank == 0 && warp == 0 && A.h_last) store_state<V>(A.h_last + s * A.C + c, carry, have);
-  if (A.cu) clear_outside<T, ODD>(A, q, s, c, have, rank * WARPS + warp, ranks * WARPS, y);
+  if (q.to == q.len && warp == 0 && A.h_last) store_state<V>(A.h_last + q.s * A.C + c, carry, have);
+  if (A.cu && q.k == 0) clear_outside<T, ODD>(A, q, c, have, A.y);
 }
 
 template <typename T, bool GATE, bool ODD>
 __global__ void __launch_bounds__(WARPS * 32, 2) gated_scan_bwd_kernel(const __grid_constant__ ScanArgs A) {
   using F = typename Lane<T>::F;
-  constexpr int V = Lane<T>::V, N = GATE ? 4 : 3;
+  constexpr int V = Lane<T>::V, N = GATE ? 4 : 3, ROW = row_bytes(ODD), PIECE = piece_bytes(ODD);
   extern __shared__ __align__(128) char ring[];  // [2][N][MARK rows]
   // a warp's steps forward, and back: what leaves its first step when nothing enters its last
-  __shared__ Map<V> maps[2][WARPS][32], peers[2][MOST_CTAS][32];
+  __shared__ Map<V> maps[2][WARPS][32];
   __shared__ F back[2][WARPS][32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = cluster_rank(), ranks = cluster_ranks();
-  const int unit = blockIdx.x / ranks;
-  const int64_t s = unit / A.tiles, tile = (int64_t)(unit % A.tiles) * Lane<T>::CHANNELS, c = tile + lane * V;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Part q(A, blockIdx.x / A.tiles);
+  if (q.s < 0) return;
+  const int64_t tile = (int64_t)(blockIdx.x % A.tiles) * Lane<T>::CHANNELS, c = tile + lane * V;
   const int have = (int)max((int64_t)0, min((int64_t)V, A.C - c));
-  const Seq q(A, s);
-  // the gradient that enters the pass from behind: a lam of the step after it
-  F mu = A.dh_last ? load_state<V>(A.dh_last + s * A.C + c, have) : splat<V>(0.0f);
-  const int pass = ranks * MARK;
-  const int last = q.len > 0 ? (q.len - 1) / pass * pass : -pass;
-  int t1 = last + rank * MARK + warp * STEPS;
+  const int last = q.to > q.from ? q.from + (q.to - q.from - 1) / MARK * MARK : q.from - MARK;
+  int t1 = last + warp * STEPS;
   char* mine = ring + warp * STEPS * ROW;
-  Input<T, ODD> f(A.f, A, q, s, tile, t1), x(A.x, A, q, s, tile, t1), d(A.dy, A, q, s, tile, t1), g(A.g, A, q, s, tile, t1);
+  Input<T, ODD> f(A.f, A, q, tile, t1), x(A.x, A, q, tile, t1), d(A.dy, A, q, tile, t1), g(A.g, A, q, tile, t1);
+  const char *f0 = f.p, *x0 = x.p, *d0 = d.p, *g0 = g.p;  // ODD: as above
   auto fetch = [&](int half, int n) {
     char* to = mine + half * N * PIECE;
-    f.copy(to, n, A.wide, -pass);
-    x.copy(to + PIECE, n, A.wide, -pass);
-    d.copy(to + 2 * PIECE, n, A.wide, -pass);
-    if (GATE) g.copy(to + 3 * PIECE, n, A.wide, -pass);
+    f.copy(to, n, A.wide, -MARK);
+    x.copy(to + PIECE, n, A.wide, -MARK);
+    d.copy(to + 2 * PIECE, n, A.wide, -MARK);
+    if (GATE) g.copy(to + 3 * PIECE, n, A.wide, -MARK);
     copies_queued();
   };
-  const char *f0 = f.p, *x0 = x.p, *d0 = d.p, *g0 = g.p;  // ODD: as above
-  if (last >= 0) fetch(0, q.len - t1);
+  if (last >= q.from) fetch(0, q.to - t1);
+  // the gradient that enters from behind: a lam of the step after
+  F mu = A.dh_last ? load_state<V>(A.dh_last + q.s * A.C + c, have) : splat<V>(0.0f);
+  if (q.to < q.len) {
+    const int behind = (q.len - 1) / A.chunk - q.k;
+    mu = enter<V>(A, maps[1], mu, q.unit + behind, behind, -1, c, have);
+  }
   int64_t at = (q.row0 + t1) * A.C + c;
-  const float* mark = A.marks + (q.mark0 + last / MARK + rank) * A.C + c;
-  if (ranks > 1) cluster_sync();  // shared memory of a CTA is there once it has started
+  const float* mark = A.marks + (q.mark0 + last / MARK) * A.C + c;
   int half = 0;
-  for (int t0 = last; t0 >= 0; t0 -= pass, t1 -= pass, at -= pass * A.C, mark -= ranks * A.C, half ^= 1) {
-    const int n = q.len - t1;  // steps left
-    // the state that enters this CTA's steps
-    F h = t0 + rank * MARK < q.len ? load_state<V>(mark, have) : splat<V>(0.0f);
+  for (int t0 = last; t0 >= q.from; t0 -= MARK, t1 -= MARK, at -= MARK * A.C, mark -= A.C, half ^= 1) {
+    const int n = q.to - t1;  // steps left
+    F h = load_state<V>(mark, have);  // the state that enters the pass
     copies_done();
-    if (t0 > 0) fetch(half ^ 1, n + pass);
+    if (t0 > q.from) fetch(half ^ 1, n + MARK);
     const char* in = mine + half * N * PIECE;
     auto x_of = [&](int l) { return read<T, ODD>(in + PIECE + l * ROW, x.skew(x0, x.row, l)); };
     auto d_of = [&](int l) { return read<T, ODD>(in + 2 * PIECE + l * ROW, d.skew(d0, d.row, l)); };
     auto g_of = [&](int l) { return read<T, ODD>(in + 3 * PIECE + l * ROW, g.skew(g0, g.row, l)); };
     F a[STEPS], w[STEPS], e[STEPS];  // w = 1 - a, e = dh
-    Map<V> m = {splat<V>(1.0f), splat<V>(0.0f)};
+    Map<V> m = Map<V>::none();
     F r = splat<V>(0.0f);
     auto take = [&](int l) {
       sigmoid_pair(read<T, ODD>(in + l * ROW, f.skew(f0, f.row, l)), a[l], w[l]);
@@ -383,8 +474,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) gated_scan_bwd_kernel(const __g
         const F z = g_of(l);
         e[l] = e[l] * (z * sigmoid(z));
       }
-      m.p = a[l] * m.p;
-      m.b = fma(a[l], m.b, w[l] * x_of(l));
+      m = Map<V>{a[l], w[l] * x_of(l)}.after(m);
     };
     if (n >= STEPS) {
 #pragma unroll
@@ -403,34 +493,11 @@ __global__ void __launch_bounds__(WARPS * 32, 2) gated_scan_bwd_kernel(const __g
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < WARPS - 1; ++k)
-      if (k < warp) {
-        const Map<V> u = maps[half][k][lane];
-        h = fma(u.p, h, u.b);
-      }
-    if (ranks == 1) {
+      if (k < warp) h = maps[half][k][lane].of(h);
 #pragma unroll
-      for (int k = WARPS - 1; k >= 0; --k) {
-        if (k == warp) r = mu;
-        mu = fma(maps[half][k][lane].p, mu, back[half][k][lane]);
-      }
-    } else {
-      // the warps behind this one, in the direction of the gradient, and then the whole CTA
-      Map<V> before, all = {splat<V>(1.0f), splat<V>(0.0f)};
-#pragma unroll
-      for (int k = WARPS - 1; k >= 0; --k) {
-        if (k == warp) before = all;
-        const F u = maps[half][k][lane].p;
-        all.b = fma(u, all.b, back[half][k][lane]);
-        all.p = u * all.p;
-      }
-      for (int k = warp; k < ranks; k += WARPS) all.put(&peers[half][rank][lane], k);
-      cluster_sync();
-#pragma unroll 4
-      for (int k = ranks - 1; k >= 0; --k) {
-        if (k == rank) r = fma(before.p, mu, before.b);
-        const Map<V> u = peers[half][k][lane];
-        mu = fma(u.p, mu, u.b);
-      }
+    for (int k = WARPS - 1; k >= 0; --k) {
+      if (k == warp) r = mu;
+      mu = fma(maps[half][k][lane].p, mu, back[half][k][lane]);
     }
     // forward over the steps: D_t = h_{t-1} - x_t, and dg is done
     F D[STEPS];
@@ -465,12 +532,11 @@ __global__ void __launch_bounds__(WARPS * 32, 2) gated_scan_bwd_kernel(const __g
         if (l < n) finish(l);
     }
   }
-  if (rank == 0 && warp == 0 && A.dh0) store_state<V>(A.dh0 + s * A.C + c, mu, have);
-  if (A.cu) {
-    const int first = rank * WARPS + warp, step = ranks * WARPS;
-    clear_outside<T, ODD>(A, q, s, c, have, first, step, static_cast<T*>(A.df));
-    clear_outside<T, ODD>(A, q, s, c, have, first, step, static_cast<T*>(A.dx));
-    if (GATE) clear_outside<T, ODD>(A, q, s, c, have, first, step, static_cast<T*>(A.dg));
+  if (q.k == 0 && warp == 0 && A.dh0) store_state<V>(A.dh0 + q.s * A.C + c, mu, have);
+  if (A.cu && q.k == 0) {
+    clear_outside<T, ODD>(A, q, c, have, A.df);
+    clear_outside<T, ODD>(A, q, c, have, A.dx);
+    if (GATE) clear_outside<T, ODD>(A, q, c, have, A.dg);
   }
 }
 
@@ -529,59 +595,80 @@ bool rows_align(const Rows& r, int size, int bytes) {
   return !r.p || (r.seq * size % bytes == 0 && r.row * size % bytes == 0 && aligned(r.p, bytes));
 }
 
-// CTAs of a cluster: the time axis is split until the GPU has enough CTAs to hide its memory's latency, as far as the
-// (mean) length has pieces for them.  Packed sequences are split further, since a few of them may hold most rows.
-int cluster_size(const ScanArgs& A) {
-  const int64_t units = A.S * A.tiles, len = A.cu ? A.T / 4 : A.T;
-  int k = 1;
-  while (k < MOST_CTAS && units * k < 3 * 148 && len > (int64_t)k * MARK) k *= 2;
-  return k;
+// How sequences are cut.  The GPU holds 148 x per_sm CTAs at a time.  Where sequences and tiles alone do not fill half
+// of them, each sequence gets as many chunks as fit at one time; packed sequences, whose lengths are not known here and
+// may be anything, are cut at an even share of all rows.  Chunks have 4 passes at least: below that the second
+// reading and its launch cost more than they bring.
+struct Cut {
+  int tiles, chunk, chunks;
+  int64_t units;
+  Cut(int64_t S, int64_t T, int64_t C, bool packed, int dtype, bool bwd) {
+    const int channels = dtype == CSN_F32 ? 32 : 64;
+    const int64_t slots = 148 * (bwd ? 2 : 3);
+    tiles = (int)((C + channels - 1) / channels);
+    int64_t n = packed ? 1 : slots / (S * tiles);
+    int64_t len = packed ? T * tiles / slots : n > 1 ? T / n : T;
+    len = (len + MARK - 1) / MARK * MARK;
+    if (len < 4 * MARK) len = 4 * MARK;
+    chunk = (int)(len < T ? len : (T + MARK - 1) / MARK * MARK);
+    if (chunk == 0) chunk = MARK;
+    chunks = (int)((T + chunk - 1) / chunk);
+    if (chunks == 0) chunks = 1;
+    units = packed ? T / chunk + S : S * chunks;
+  }
+  bool split(int64_t T) const { return T > chunk; }
+};
+
+template <typename K>
+cudaError_t launch_part(K kernel, int64_t grid, int smem, const ScanArgs& A, cudaStream_t st) {
+  if (cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, smem))
+    return e;
+  kernel<<<(unsigned)grid, WARPS * 32, smem, st>>>(A);
+  return cudaGetLastError();
 }
 
+template <typename T, bool GATE, bool ODD>
+cudaError_t launch_scan(const ScanArgs& A, bool bwd, const Cut& cut, cudaStream_t st) {
+  const int64_t grid = cut.units * cut.tiles;
+  const int piece = 2 * piece_bytes(ODD);
+  if (cut.split(A.T)) {
+    const cudaError_t e = bwd ? launch_part(reduce_kernel<T, GATE, ODD, true>, grid, (GATE ? 3 : 2) * piece, A, st)
+                              : launch_part(reduce_kernel<T, false, ODD, false>, grid, 2 * piece, A, st);
+    if (e != cudaSuccess) return e;
+  }
+  return bwd ? launch_part(gated_scan_bwd_kernel<T, GATE, ODD>, grid, (GATE ? 4 : 3) * piece, A, st)
+             : launch_part(gated_scan_fwd_kernel<T, GATE, ODD>, grid, (GATE ? 3 : 2) * piece, A, st);
+}
 template <typename T, bool ODD>
-cudaError_t launch_scan(ScanArgs A, bool bwd, cudaStream_t st) {
-  A.tiles = (int)((A.C + Lane<T>::CHANNELS - 1) / Lane<T>::CHANNELS);
-  const bool gate = A.g.p;
-  void (*kernel)(const ScanArgs) =
-      bwd ? (gate ? gated_scan_bwd_kernel<T, true, ODD> : gated_scan_bwd_kernel<T, false, ODD>)
-          : (gate ? gated_scan_fwd_kernel<T, true, ODD> : gated_scan_fwd_kernel<T, false, ODD>);
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute at;
-  at.id = cudaLaunchAttributeClusterDimension;
-  at.val.clusterDim.x = cluster_size(A), at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
-  cfg.gridDim = dim3((unsigned)(A.S * A.tiles * at.val.clusterDim.x));
-  cfg.blockDim = dim3(WARPS * 32);
-  cfg.dynamicSmemBytes = 2 * ((bwd ? 3 : 2) + gate) * PIECE;
-  cfg.stream = st;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  const void* k = reinterpret_cast<const void*>(kernel);
-  if (cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes)) return e;
-  if (at.val.clusterDim.x > 8)  // 8 is the size that every GPU takes; sm_100a takes 16 when asked to
-    if (cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) return e;
-  return cudaLaunchKernelEx(&cfg, kernel, (const ScanArgs)A);
+cudaError_t launch_scan(const ScanArgs& A, bool bwd, const Cut& cut, cudaStream_t st) {
+  return A.g.p ? launch_scan<T, true, ODD>(A, bwd, cut, st) : launch_scan<T, false, ODD>(A, bwd, cut, st);
 }
 
-int dispatch_scan(ScanArgs A, int dtype, bool bwd, cudaStream_t st, const char* who) {
+int dispatch_scan(ScanArgs A, int dtype, bool bwd, void* workspace, size_t bytes, cudaStream_t st, const char* who) {
   const int size = width_of(dtype);
-  auto all = [&](int bytes) {
-    return A.C * size % bytes == 0 && rows_align(A.f, size, bytes) && rows_align(A.x, size, bytes) &&
-           rows_align(A.g, size, bytes) && rows_align(A.dy, size, bytes);
+  const Cut cut(A.S, A.T, A.C, A.cu != nullptr, dtype, bwd);
+  A.tiles = cut.tiles, A.chunk = cut.chunk, A.chunks = cut.chunks, A.maps = static_cast<float2*>(workspace);
+  if (cut.units * cut.tiles > 0x7fffffff) return set_error(CSN_ERR_INVALID, "csn_gated_scan: more than 2^31 - 1 tiles of work");
+  if (cut.split(A.T) && (!workspace || !aligned(workspace, 16) || bytes < (size_t)cut.units * A.C * sizeof(float2)))
+    return set_error(CSN_ERR_INVALID, "csn_gated_scan: workspace smaller than csn_gated_scan_workspace_bytes");
+  auto all = [&](int to) {
+    return A.C * size % to == 0 && rows_align(A.f, size, to) && rows_align(A.x, size, to) && rows_align(A.g, size, to) &&
+           rows_align(A.dy, size, to);
   };
   A.wide = all(16);
   const bool odd = !all(4);
-  const cudaError_t e = dtype == CSN_F32 ? launch_scan<float, false>(A, bwd, st)
-                        : dtype == CSN_BF16
-                            ? (odd ? launch_scan<__nv_bfloat16, true>(A, bwd, st) : launch_scan<__nv_bfloat16, false>(A, bwd, st))
-                            : (odd ? launch_scan<__half, true>(A, bwd, st) : launch_scan<__half, false>(A, bwd, st));
-  if (e != cudaSuccess) return set_cuda_error(e, who);
-  return check_launch(who);
+  const cudaError_t e =
+      dtype == CSN_F32 ? launch_scan<float, false>(A, bwd, cut, st)
+      : dtype == CSN_BF16
+          ? (odd ? launch_scan<__nv_bfloat16, true>(A, bwd, cut, st) : launch_scan<__nv_bfloat16, false>(A, bwd, cut, st))
+          : (odd ? launch_scan<__half, true>(A, bwd, cut, st) : launch_scan<__half, false>(A, bwd, cut, st));
+  return e == cudaSuccess ? CSN_OK : set_cuda_error(e, who);
 }
 
 int check_scan(const char* who, const ScanArgs& A, int dtype) {
   if (A.S < 0 || A.T < 0 || A.C < 0 || A.T > (1 << 30)) return set_error(CSN_ERR_INVALID, who);
   if (!width_of(dtype)) return set_error(CSN_ERR_UNSUPPORTED, who);
-  // the grid has one CTA for each 32 channels of a sequence at most
+  // a CTA for each 32 channels of a sequence
   if (A.S > 0 && A.C > 0 && (A.C + 31) / 32 > (int64_t)0x7fffffff / A.S) return set_error(CSN_ERR_INVALID, who);
   return CSN_OK;
 }
@@ -596,9 +683,18 @@ extern "C" int64_t csn_gated_scan_marks(int64_t S, int64_t T, int64_t C, int pac
   return ((packed ? T : S * T) / MARK + S) * C;
 }
 
+extern "C" size_t csn_gated_scan_workspace_bytes(int64_t S, int64_t T, int64_t C, int packed, int dtype, int backward) {
+  ScanArgs A = {};
+  A.S = S, A.T = T, A.C = C;
+  if (S <= 0 || T <= 0 || C <= 0 || check_scan("", A, dtype)) return 0;
+  const Cut cut(S, T, C, packed != 0, dtype, backward != 0);
+  return cut.split(T) ? (size_t)cut.units * C * sizeof(float2) : 0;
+}
+
 extern "C" int csn_gated_scan_fwd(const void* f, const void* x, const void* gate, const int64_t* strides,
                                   const float* h0, const int32_t* cu_seqlens, void* y, float* h_last, float* marks,
-                                  int64_t S, int64_t T, int64_t C, int dtype, void* stream) {
+                                  int64_t S, int64_t T, int64_t C, int dtype, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
   ScanArgs A = {};
   A.S = S, A.T = T, A.C = C;
   if (int rc = check_scan("csn_gated_scan_fwd: needs S, T, C >= 0, T <= 2^30, dtype float32, bfloat16 or float16, and at most "
@@ -618,13 +714,14 @@ extern "C" int csn_gated_scan_fwd(const void* f, const void* x, const void* gate
   A.h0 = h0, A.cu = cu_seqlens, A.y = y, A.h_last = h_last, A.marks = marks;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   KernelTimer kt("gated_scan_fwd", st);
-  return dispatch_scan(A, dtype, false, st, "csn_gated_scan_fwd");
+  return dispatch_scan(A, dtype, false, workspace, workspace_bytes, st, "csn_gated_scan_fwd");
 }
 
 extern "C" int csn_gated_scan_bwd(const void* f, const void* x, const void* gate, const void* dy,
                                   const int64_t* strides, const int32_t* cu_seqlens, const float* marks,
                                   const float* dh_last, void* df, void* dx, void* dgate, float* dh0, int64_t S,
-                                  int64_t T, int64_t C, int dtype, void* stream) {
+                                  int64_t T, int64_t C, int dtype, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
   ScanArgs A = {};
   A.S = S, A.T = T, A.C = C;
   if (int rc = check_scan("csn_gated_scan_bwd: needs S, T, C >= 0, T <= 2^30, dtype float32, bfloat16 or float16, and at most "
@@ -649,7 +746,7 @@ extern "C" int csn_gated_scan_bwd(const void* f, const void* x, const void* gate
   A.df = df, A.dx = dx, A.dg = gate ? dgate : nullptr, A.dh0 = dh0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   KernelTimer kt("gated_scan_bwd", st);
-  return dispatch_scan(A, dtype, true, st, "csn_gated_scan_bwd");
+  return dispatch_scan(A, dtype, true, workspace, workspace_bytes, st, "csn_gated_scan_bwd");
 }
 
 namespace csn {

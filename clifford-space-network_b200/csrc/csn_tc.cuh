@@ -1,4 +1,4 @@
-// csn_tc.cuh -- tensor-core building blocks for sm_100a: mbarriers, TMA tile loads, tensor memory and tcgen05.mma,
+// csn_tc.cuh -- asynchronous and tensor-core building blocks for sm_100a: mbarriers, TMA tile loads, tensor memory and tcgen05.mma,
 // as inline PTX, and the tensor maps on the host.
 //
 // Every wait is bounded.  A wait that runs out sets the CTA's `gave_up` word; every other wait of the CTA then ends

@@ -103,17 +103,15 @@ __device__ __forceinline__ float inverse_fast(float x) {
 }
 constexpr float LOG2E = 1.4426950408889634f;
 
-// a = sigmoid(z) and q = 1 - a = sigmoid(-z): the smaller is s = e / (1 + e) with e = exp(-|z|), off by a few units of
-// its own (and 2 |z| 2^-24 relative, since the exponential's argument is rounded); the larger is 1 - s, rounded once.
+// q = sigmoid(-z) = 1 / (1 + exp(z)), off by a few units of its own (and 2 |z| 2^-24 relative, since the exponential's
+// argument is rounded), and a = 1 - q, rounded once.  So a near 1 has the rounding of a float32 number, without a
+// drift, and a near 0 is off by 2^-25: what a h loses by it is half a unit of h.  exp(z) too large for float32: q = 0.
 template <int V>
 __device__ __forceinline__ void sigmoid_pair(Vals<V> z, Vals<V>& a, Vals<V>& q) {
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const float e = exp2_fast(-LOG2E * fabsf(z.v[i]));
-    const float s = e * inverse_fast(1.0f + e), l = 1.0f - s;
-    const bool up = z.v[i] >= 0.0f;
-    a.v[i] = up ? l : s;
-    q.v[i] = up ? s : l;
+    q.v[i] = inverse_fast(1.0f + exp2_fast(LOG2E * z.v[i]));
+    a.v[i] = 1.0f - q.v[i];
   }
 }
 

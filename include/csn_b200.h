@@ -417,11 +417,15 @@ enum csn_dtype { CSN_F32 = 0, CSN_BF16 = 1, CSN_F16 = 2 };
  *     out as 0.  Borders are cut to 0 .. T and to their order; they must not fall.
  * h0 [S, C] (NULL = 0), h_last [S, C] (the state after the last step; NULL = not wanted).
  * marks: NULL, or csn_gated_scan_marks(S, T, C, packed) floats that csn_gated_scan_bwd reads.
+ * The workspace is required where csn_gated_scan_workspace_bytes is not 0.
  * f, x, gate aligned to their type; everything else 16-byte aligned.  T <= 2^30. */
 int64_t csn_gated_scan_marks(int64_t S, int64_t T, int64_t C, int packed);
+size_t csn_gated_scan_workspace_bytes(int64_t S, int64_t T, int64_t C, int packed, int dtype,
+                                      int backward);
 int csn_gated_scan_fwd(const void* f, const void* x, const void* gate, const int64_t* strides,
                        const float* h0, const int32_t* cu_seqlens, void* y, float* h_last,
-                       float* marks, int64_t S, int64_t T, int64_t C, int dtype, void* stream);
+                       float* marks, int64_t S, int64_t T, int64_t C, int dtype, void* workspace,
+                       size_t workspace_bytes, void* stream);
 
 /* Adjoint of csn_gated_scan_fwd on the same inputs and its marks: dy (strides[6], strides[7]) and
  * dh_last [S, C] (NULL = 0) to df, dx, with a gate dgate (contiguous, in y's layout) and dh0
@@ -429,7 +433,8 @@ int csn_gated_scan_fwd(const void* f, const void* x, const void* gate, const int
 int csn_gated_scan_bwd(const void* f, const void* x, const void* gate, const void* dy,
                        const int64_t* strides, const int32_t* cu_seqlens, const float* marks,
                        const float* dh_last, void* df, void* dx, void* dgate, float* dh0,
-                       int64_t S, int64_t T, int64_t C, int dtype, void* stream);
+                       int64_t S, int64_t T, int64_t C, int dtype, void* workspace,
+                       size_t workspace_bytes, void* stream);
 
 /* One step of the same recurrence for B streams, h [B, C] in place (as csn_rotor_step):
  * f, x, gate element (b, c) at ptr + b * strides[i] + c; y [B, C]. */

@@ -3,8 +3,8 @@ float32 computation of it (numpy, element by element, no code of the package).
 
 Units: U = 2^-24 is half a step of float32.  A product, sum or fused product is off by at most 1 U, a
 quotient by 2 steps (4 U), the fast exp(z) by 2 steps and, since it rounds its argument, 2 |z| U.  So
-s = min(sigmoid(z), sigmoid(-z)) = e / (1 + e) is off by at most (12 + 2 |z|) U of itself, and so is
-sigmoid(z) where it is the smaller (the larger by less)."""
+q = sigmoid(-f) = 1 / (1 + exp(f)) is off by at most (12 + 2 |f|) U of itself, and a = 1 - q by that and
+half a unit of its own range, U."""
 import numpy as np
 
 U = 2.0 ** -24
@@ -31,9 +31,11 @@ def gated_scan(f, x, h0, gate, borders, dy=None, dh=None):
     z = gate if gate is not None else None
     w = sigmoid(z) if z is not None else None
     silu = z * w if z is not None else np.ones_like(f)
-    # the recurrence is h + s (x - h) or x + s (h - x); composing steps rounds the products of a and the
-    # partial states once more each
-    small, s_err = np.minimum(a, q), (12 + 2 * np.abs(f)) * U
+    # q itself is off by q_err, and as exp(f) is what carries the error, min(a, q) by that share of it; a = 1 - q
+    # by the same and its rounding.  Composing steps rounds the products of a and the partial states once more
+    small, q_err = np.minimum(a, q), (12 + 2 * np.abs(f)) * U
+    q_off = np.minimum(q, q_err * small + 8 * U * q)
+    a_off = q_off + U
     fast = (14 + 2 * np.abs(z)) * U if z is not None else np.zeros_like(f)
     silu_err = fast * np.abs(silu)
     h, he = np.zeros((L, C)), np.zeros((L, C))
@@ -45,7 +47,7 @@ def gated_scan(f, x, h0, gate, borders, dy=None, dh=None):
         v, err = h0[s].copy(), np.zeros(C)
         for t in range(b, e):
             before[t], be[t] = v, err
-            err = a[t] * err + s_err[t] * small[t] * np.abs(x[t] - v) + 4 * U * (np.abs(v) + np.abs(x[t]))
+            err = a[t] * err + a_off[t] * np.abs(v) + q_off[t] * np.abs(x[t]) + 4 * U * (a[t] * np.abs(v) + np.abs(x[t]))
             v = a[t] * v + q[t] * x[t]
             h[t], he[t] = v, err
         last[s], laste[s] = v, err
@@ -64,13 +66,14 @@ def gated_scan(f, x, h0, gate, borders, dy=None, dh=None):
         for t in range(e - 1, b - 1, -1):
             lam[t] = e_t[t] + m
             le[t] = e_err[t] + me + 2 * U * (np.abs(e_t[t]) + np.abs(m))
-            m, me = a[t] * lam[t], a[t] * le[t] + (s_err[t] * small[t] + 4 * U) * np.abs(lam[t])
+            m, me = a[t] * lam[t], a[t] * le[t] + (a_off[t] + 4 * U * a[t]) * np.abs(lam[t])
         dh0[s], dh0e[s] = m, me
     D = before - x
     De = be + U * (np.abs(before) + np.abs(x))
     df, dx = lam * D * a * q, lam * q
-    out["dx"] = (dx, q * le + (s_err * small + 2 * U * q) * np.abs(lam))
-    out["df"] = (df, np.abs(lam * a * q) * De + np.abs(D * a * q) * le + (s_err + 6 * U) * np.abs(df))
+    out["dx"] = (dx, q * le + (q_off + 2 * U * q) * np.abs(lam))
+    out["df"] = (df, np.abs(lam * a * q) * De + np.abs(D * a * q) * le + (a_off * q + a * q_off) * np.abs(lam * D)
+                 + 6 * U * np.abs(df))
     out["dh0"] = (dh0, dh0e)
     if z is not None:
         slope = w * (1 + z * (1 - w))

@@ -56,7 +56,7 @@ def test_scan_refuses(lib):
     p, st = fake(), strides()
 
     def fwd(f=p, x=p, g=NULL, s=st, h0=NULL, cu=NULL, y=p, S=2, T=4, C=8, dtype=1):
-        return lib.csn_gated_scan_fwd(f, x, g, s, h0, cu, y, NULL, NULL, S, T, C, dtype, NULL)
+        return lib.csn_gated_scan_fwd(f, x, g, s, h0, cu, y, NULL, NULL, S, T, C, dtype, NULL, 0, NULL)
 
     refused(lib, fwd(S=-1), 1, "S, T, C >= 0")
     refused(lib, fwd(T=-1), 1, "S, T, C >= 0")
@@ -71,13 +71,30 @@ def test_scan_refuses(lib):
     assert fwd(S=0) == 0 and fwd(C=0) == 0
 
     def bwd(marks=p, dy=p, df=p, dh0=NULL, T=4):
-        return lib.csn_gated_scan_bwd(p, p, NULL, dy, st, NULL, marks, NULL, df, p, NULL, dh0, 2, T, 8, 1, NULL)
+        return lib.csn_gated_scan_bwd(p, p, NULL, dy, st, NULL, marks, NULL, df, p, NULL, dh0, 2, T, 8, 1, NULL, 0, NULL)
 
     refused(lib, bwd(marks=NULL), 1, "required")
+    refused(lib, bwd(dy=NULL), 1, "required")
+    refused(lib, bwd(df=NULL), 1, "required")
     refused(lib, bwd(marks=fake(4)), 1, "aligned")
     refused(lib, bwd(dy=fake(1)), 1, "aligned")
     refused(lib, bwd(df=fake(2)), 1, "aligned")
     refused(lib, bwd(dh0=fake(4)), 1, "aligned")
+
+
+def test_long_scans_need_their_workspace(lib):
+    p, st = fake(), strides()
+    need = lib.csn_gated_scan_workspace_bytes(1, 65536, 64, 0, 1, 0)
+    assert need > 0 and need % (64 * 8) == 0
+    rc = lib.csn_gated_scan_fwd(p, p, NULL, st, NULL, NULL, p, NULL, NULL, 1, 65536, 64, 1, p, need - 1, NULL)
+    refused(lib, rc, 1, "workspace")
+    assert lib.csn_gated_scan_workspace_bytes(256, 4096, 4096, 0, 1, 0) == 0
+    # a packed batch has room for the chunks of every sequence, whatever their lengths
+    for S, T, C in ((1, 5000, 64), (37, 20011, 771), (400, 900, 64), (3, 1 << 20, 128)):
+        for backward in (0, 1):
+            units = lib.csn_gated_scan_workspace_bytes(S, T, C, 1, 1, backward) // (C * 8)
+            assert units == 0 or units >= S + 1
+    assert lib.csn_gated_scan_workspace_bytes(1, 65536, 64, 0, 9, 0) == 0
 
 
 def test_step_refuses(lib):
