@@ -137,21 +137,33 @@ __device__ __forceinline__ void store_state(float* p, Vals<V> h, int have) {
 }
 
 // Rows of one input as a warp copies and reads them.  ODD: 16-bit rows that do not all start on 4 bytes; such a row is
-// copied in the whole words that hold it and shifted when it is read.
+// copied in the whole words that hold it and shifted when it is read.  A warp's rows lie an even number of rows from
+// where they lay in its last pass, so only a row's place among the warp's, even or odd, says how far it is shifted.
 template <typename T, bool ODD>
 struct Input {
-  const char* p;  // this lane's first bytes of the warp's first row of the next pass
+  const char* p;  // this lane's first bytes of the warp's first row of the next pass (ODD: word of the second row: q)
+  const char* q;
   int64_t row;    // bytes
-  int left;       // ODD: bytes of the tile
+  int left;       // bytes of the tile
+  int skew[2];    // ODD: bits
 
-  __device__ __forceinline__ Input(const Rows& r, const ScanArgs& A, const Part& q, int64_t tile, int t1) {
-    p = nullptr;
+  __device__ __forceinline__ Input(const Rows& r, const ScanArgs& A, const Part& part, int64_t tile, int t1) {
+    p = q = nullptr;
     row = r.row * (int64_t)sizeof(T);
     left = (int)min((int64_t)32 * Lane<T>::V, A.C - tile) * (int)sizeof(T);
+    skew[0] = skew[1] = 0;
     if (!r.p) return;
     const int lane = threadIdx.x & 31;
-    p = static_cast<const char*>(r.p) + ((A.cu ? q.row0 * r.row : q.s * r.seq) + tile) * (int64_t)sizeof(T) + t1 * row;
-    if (!ODD) p += A.wide ? (lane >> 3) * row + (lane & 7) * 16 : lane * 4;
+    p = static_cast<const char*>(r.p) + ((A.cu ? part.row0 * r.row : part.s * r.seq) + tile) * (int64_t)sizeof(T) + t1 * row;
+    if (ODD) {
+      q = p + row;
+      skew[0] = (int)(reinterpret_cast<uintptr_t>(p) & 2) * 8;
+      skew[1] = (int)(reinterpret_cast<uintptr_t>(q) & 2) * 8;
+      p += lane * 4 - skew[0] / 8;
+      q += lane * 4 - skew[1] / 8;
+    } else {
+      p += A.wide ? (lane >> 3) * row + (lane & 7) * 16 : lane * 4;
+    }
   }
   // the warp's n rows into shared memory at `to`, then `step` rows on
   __device__ __forceinline__ void copy(char* to, int n, bool wide, int step) {
@@ -160,14 +172,20 @@ struct Input {
     const uint32_t at = (uint32_t)__cvta_generic_to_shared(to);
     if (ODD) {
 #pragma unroll
-      for (int l = 0; l < STEPS; ++l)
-        if (l < n) {
-          const char* w = p + l * row;
-          const int skew = (int)(reinterpret_cast<uintptr_t>(w) & 2);
-          w -= skew;
-          if (lane * 4 < left + skew) copy4(at + l * ROW + lane * 4, w + lane * 4);
-          if (lane == 0 && 128 < left + skew) copy4(at + l * ROW + 128, w + 128);
+      for (int o = 0; o < 2; ++o) {
+        const char* w = o ? q : p;
+        if (lane * 4 < left + skew[o] / 8) {
+#pragma unroll
+          for (int l = o; l < STEPS; l += 2)
+            if (l < n) copy4(at + l * ROW + lane * 4, w + (l - o) * row);
         }
+        if (lane == 0 && 128 < left + skew[o] / 8) {
+#pragma unroll
+          for (int l = o; l < STEPS; l += 2)
+            if (l < n) copy4(at + l * ROW + 128, w + (l - o) * row + 128);
+        }
+      }
+      q += step * row;
     } else if (wide) {
       const int l = lane >> 3;
       if ((lane & 7) * 16 < left) {
@@ -188,18 +206,12 @@ struct Input {
   static __device__ __forceinline__ void copy4(uint32_t to, const char* from) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
   }
-  // how far (in bits) the lanes' words of row l lie beyond the words' start; `p` as it was when the rows were copied
-  __device__ __forceinline__ static uint32_t skew(const char* p, int64_t row, int l) {
-    return (uint32_t)(reinterpret_cast<uintptr_t>(p + l * row) & 2) * 8;
+  // this lane's channels of the warp's row l, which was copied to `at`
+  __device__ __forceinline__ Vals<Lane<T>::V> read(const char* at, int l) const {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(at + l * row_bytes(ODD)) + (threadIdx.x & 31);
+    return unpack<T>(ODD ? __funnelshift_r(w[0], w[1], skew[l & 1]) : w[0]);
   }
 };
-
-// a lane's channels of a row in shared memory
-template <typename T, bool ODD>
-__device__ __forceinline__ Vals<Lane<T>::V> read(const char* row, uint32_t skew) {
-  const uint32_t* w = reinterpret_cast<const uint32_t*>(row) + (threadIdx.x & 31);
-  return unpack<T>(ODD ? __funnelshift_r(w[0], w[1], skew) : w[0]);
-}
 
 // a lane's channels of one output row
 template <typename T, bool ODD>
@@ -273,7 +285,7 @@ __device__ __forceinline__ Vals<V> enter(const ScanArgs& A, Map<V> (*maps)[32], 
 template <typename T, bool GATE, bool ODD, bool BACK>
 __global__ void __launch_bounds__(WARPS * 32, 3) reduce_kernel(const __grid_constant__ ScanArgs A) {
   using F = typename Lane<T>::F;
-  constexpr int V = Lane<T>::V, N = BACK && GATE ? 3 : 2, ROW = row_bytes(ODD), PIECE = piece_bytes(ODD);
+  constexpr int V = Lane<T>::V, N = BACK && GATE ? 3 : 2, PIECE = piece_bytes(ODD);
   extern __shared__ __align__(128) char ring[];  // [2][N][MARK rows]
   __shared__ Map<V> maps[WARPS][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -282,12 +294,11 @@ __global__ void __launch_bounds__(WARPS * 32, 3) reduce_kernel(const __grid_cons
   const int64_t tile = (int64_t)(blockIdx.x % A.tiles) * Lane<T>::CHANNELS, c = tile + lane * V;
   const int have = (int)max((int64_t)0, min((int64_t)V, A.C - c));
   const int share = A.chunk / WARPS, first = q.from + warp * share, past = min(first + share, q.to);
-  char* mine = ring + warp * STEPS * ROW;
+  char* mine = ring + warp * STEPS * row_bytes(ODD);
   // BACK goes from the last steps to the first
   int t = BACK ? first + (max(past - first, 1) - 1) / STEPS * STEPS : first;
   const int step = BACK ? -STEPS : STEPS;
   Input<T, ODD> f(A.f, A, q, tile, t), x(BACK ? A.dy : A.x, A, q, tile, t), g(A.g, A, q, tile, t);
-  const char *f0 = f.p, *x0 = x.p, *g0 = g.p;  // ODD: STEPS rows are whole words, so the skews never change
   auto fetch = [&](int half, int n) {
     char* to = mine + half * N * PIECE;
     f.copy(to, n, A.wide, step);
@@ -305,11 +316,11 @@ __global__ void __launch_bounds__(WARPS * 32, 3) reduce_kernel(const __grid_cons
     const int n = past - t;
     auto take = [&](int l) {
       F a, w;
-      sigmoid_pair(read<T, ODD>(in + l * ROW, f.skew(f0, f.row, l)), a, w);
-      F v = read<T, ODD>(in + PIECE + l * ROW, x.skew(x0, x.row, l));
+      sigmoid_pair(f.read(in, l), a, w);
+      F v = x.read(in + PIECE, l);
       if (BACK) {
         if (GATE) {
-          const F z = read<T, ODD>(in + 2 * PIECE + l * ROW, g.skew(g0, g.row, l));
+          const F z = g.read(in + 2 * PIECE, l);
           v = v * (z * sigmoid(z));
         }
         m.b = a * (v + m.b);
@@ -340,7 +351,7 @@ __global__ void __launch_bounds__(WARPS * 32, 3) reduce_kernel(const __grid_cons
 template <typename T, bool GATE, bool ODD>
 __global__ void __launch_bounds__(WARPS * 32, 3) gated_scan_fwd_kernel(const __grid_constant__ ScanArgs A) {
   using F = typename Lane<T>::F;
-  constexpr int V = Lane<T>::V, N = GATE ? 3 : 2, ROW = row_bytes(ODD), PIECE = piece_bytes(ODD);
+  constexpr int V = Lane<T>::V, N = GATE ? 3 : 2, PIECE = piece_bytes(ODD);
   extern __shared__ __align__(128) char ring[];  // [2][N][MARK rows]
   __shared__ Map<V> maps[2][WARPS][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -349,9 +360,8 @@ __global__ void __launch_bounds__(WARPS * 32, 3) gated_scan_fwd_kernel(const __g
   const int64_t tile = (int64_t)(blockIdx.x % A.tiles) * Lane<T>::CHANNELS, c = tile + lane * V;
   const int have = (int)max((int64_t)0, min((int64_t)V, A.C - c));
   int t1 = q.from + warp * STEPS;
-  char* mine = ring + warp * STEPS * ROW;
+  char* mine = ring + warp * STEPS * row_bytes(ODD);
   Input<T, ODD> f(A.f, A, q, tile, t1), x(A.x, A, q, tile, t1), g(A.g, A, q, tile, t1);
-  const char *f0 = f.p, *x0 = x.p, *g0 = g.p;  // ODD: MARK rows are whole words, so the skews never change
   auto fetch = [&](int half, int n) {
     char* to = mine + half * N * PIECE;
     f.copy(to, n, A.wide, MARK);
@@ -374,8 +384,8 @@ __global__ void __launch_bounds__(WARPS * 32, 3) gated_scan_fwd_kernel(const __g
 #pragma unroll
     for (int l = 0; l < STEPS; ++l) {
       F w;
-      sigmoid_pair(read<T, ODD>(in + l * ROW, f.skew(f0, f.row, l)), a[l], w);
-      b[l] = w * read<T, ODD>(in + PIECE + l * ROW, x.skew(x0, x.row, l));
+      sigmoid_pair(f.read(in, l), a[l], w);
+      b[l] = w * x.read(in + PIECE, l);
     }
     if (n < STEPS) {
 #pragma unroll
@@ -401,7 +411,7 @@ __global__ void __launch_bounds__(WARPS * 32, 3) gated_scan_fwd_kernel(const __g
       h = fma(a[l], h, b[l]);
       F o = h;
       if (GATE) {
-        const F z = read<T, ODD>(in + 2 * PIECE + l * ROW, g.skew(g0, g.row, l));
+        const F z = g.read(in + 2 * PIECE, l);
         o = h * (z * sigmoid(z));
       }
       store_row<T, ODD>(out + l * A.C, o, have);
@@ -422,7 +432,7 @@ __global__ void __launch_bounds__(WARPS * 32, 3) gated_scan_fwd_kernel(const __g
 template <typename T, bool GATE, bool ODD>
 __global__ void __launch_bounds__(WARPS * 32, 2) gated_scan_bwd_kernel(const __grid_constant__ ScanArgs A) {
   using F = typename Lane<T>::F;
-  constexpr int V = Lane<T>::V, N = GATE ? 4 : 3, ROW = row_bytes(ODD), PIECE = piece_bytes(ODD);
+  constexpr int V = Lane<T>::V, N = GATE ? 4 : 3, PIECE = piece_bytes(ODD);
   extern __shared__ __align__(128) char ring[];  // [2][N][MARK rows]
   // a warp's steps forward, and back: what leaves its first step when nothing enters its last
   __shared__ Map<V> maps[2][WARPS][32];
@@ -434,9 +444,8 @@ __global__ void __launch_bounds__(WARPS * 32, 2) gated_scan_bwd_kernel(const __g
   const int have = (int)max((int64_t)0, min((int64_t)V, A.C - c));
   const int last = q.to > q.from ? q.from + (q.to - q.from - 1) / MARK * MARK : q.from - MARK;
   int t1 = last + warp * STEPS;
-  char* mine = ring + warp * STEPS * ROW;
+  char* mine = ring + warp * STEPS * row_bytes(ODD);
   Input<T, ODD> f(A.f, A, q, tile, t1), x(A.x, A, q, tile, t1), d(A.dy, A, q, tile, t1), g(A.g, A, q, tile, t1);
-  const char *f0 = f.p, *x0 = x.p, *d0 = d.p, *g0 = g.p;  // ODD: as above
   auto fetch = [&](int half, int n) {
     char* to = mine + half * N * PIECE;
     f.copy(to, n, A.wide, -MARK);
@@ -461,14 +470,14 @@ __global__ void __launch_bounds__(WARPS * 32, 2) gated_scan_bwd_kernel(const __g
     copies_done();
     if (t0 > q.from) fetch(half ^ 1, n + MARK);
     const char* in = mine + half * N * PIECE;
-    auto x_of = [&](int l) { return read<T, ODD>(in + PIECE + l * ROW, x.skew(x0, x.row, l)); };
-    auto d_of = [&](int l) { return read<T, ODD>(in + 2 * PIECE + l * ROW, d.skew(d0, d.row, l)); };
-    auto g_of = [&](int l) { return read<T, ODD>(in + 3 * PIECE + l * ROW, g.skew(g0, g.row, l)); };
+    auto x_of = [&](int l) { return x.read(in + PIECE, l); };
+    auto d_of = [&](int l) { return d.read(in + 2 * PIECE, l); };
+    auto g_of = [&](int l) { return g.read(in + 3 * PIECE, l); };
     F a[STEPS], w[STEPS], e[STEPS];  // w = 1 - a, e = dh
     Map<V> m = Map<V>::none();
     F r = splat<V>(0.0f);
     auto take = [&](int l) {
-      sigmoid_pair(read<T, ODD>(in + l * ROW, f.skew(f0, f.row, l)), a[l], w[l]);
+      sigmoid_pair(f.read(in, l), a[l], w[l]);
       e[l] = d_of(l);
       if (GATE) {
         const F z = g_of(l);
