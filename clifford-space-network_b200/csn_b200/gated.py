@@ -14,12 +14,13 @@ and its gated product python/clifford_model.py:42-43.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _require_cuda, _workspace
+from .ops import _require_cuda
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _NAMES = {t: str(t).replace("torch.", "") for t in DTYPES}
@@ -39,6 +40,23 @@ def _launch(name, index, *args):
             rc = getattr(_lib.load(), name)(*args, _current_stream(index))
     if rc:
         raise _lib.CsnError(name, rc, _lib.load().csn_last_error().decode(errors="replace"))
+
+
+@functools.lru_cache(maxsize=1024)
+def _size(query, *sizes):
+    """A size query of the library, which is a function of its arguments alone."""
+    return getattr(_lib.load(), query)(*sizes)
+
+
+def _first_order(backward):
+    """once_differentiable, without its cost where no second backward pass can follow."""
+    once = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def call(ctx, *grads):
+        return once(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return call
 
 
 def _device_of(name, first, *rest):
@@ -118,7 +136,7 @@ def _scan_sizes(f, cu):
 
 
 def _scan_workspace(f, S, T, C, cu, backward):
-    nb = _lib.load().csn_gated_scan_workspace_bytes(S, T, C, int(cu is not None), DTYPES[f.dtype], backward)
+    nb = _size("csn_gated_scan_workspace_bytes", S, T, C, int(cu is not None), DTYPES[f.dtype], backward)
     return (f.new_empty((nb,), dtype=torch.uint8) if nb else None), nb
 
 
@@ -131,7 +149,7 @@ def _gated_scan_fwd(f, x, h0, gate, cu, keep):
     h_last = f.new_empty((S, C), dtype=torch.float32)
     marks = None
     if keep:
-        marks = f.new_empty((_lib.load().csn_gated_scan_marks(S, T, C, int(cu is not None)),), dtype=torch.float32)
+        marks = f.new_empty((_size("csn_gated_scan_marks", S, T, C, int(cu is not None)),), dtype=torch.float32)
     ws, nb = _scan_workspace(f, S, T, C, cu, 0)
     _launch("csn_gated_scan_fwd", index, _ptr(f), _ptr(x), _ptr(gate), _row_strides(f, x, gate), _ptr(h0), _ptr(cu),
             _ptr(y), _ptr(h_last), _ptr(marks), S, T, C, DTYPES[f.dtype], _ptr(ws), nb)
@@ -163,7 +181,7 @@ class GatedScanFunction(torch.autograd.Function):
         return y, h_last
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy, dh_last):
         if dy is None and dh_last is None:
             return None, None, None, None, None
@@ -256,8 +274,8 @@ def _silu_gated_linear_bwd(x, wg, wu, dy, need):
     dx = x.new_empty((R, C)) if need[0] else None
     dwg = x.new_empty((F, C)) if need[1] else None
     dwu = x.new_empty((F, C)) if need[2] else None
-    nb = _lib.load().csn_silu_gated_linear_bwd_workspace_bytes(R, C, F)
-    ws = _workspace(nb, x.device)
+    nb = _size("csn_silu_gated_linear_bwd_workspace_bytes", R, C, F)
+    ws = x.new_empty((nb,), dtype=torch.uint8)
     _launch("csn_silu_gated_linear_bwd", x.get_device(), _ptr(x), ldx, _ptr(wg), ldg, _ptr(wu), ldu, _ptr(dy),
             dy.stride(0), _ptr(dx), _ptr(dwg), _ptr(dwu), R, C, F, DTYPES[x.dtype], _ptr(ws), nb)
     return dx, dwg, dwu
@@ -270,7 +288,7 @@ class SiluGatedLinearFunction(torch.autograd.Function):
         return _silu_gated_linear_fwd(x, wg, wu)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy):
         return _silu_gated_linear_bwd(*ctx.saved_tensors, dy, ctx.needs_input_grad)
 
@@ -309,7 +327,7 @@ class DropoutAddFunction(torch.autograd.Function):
         return _dropout_add(x, residual, cut, rng)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy):
         (rng,) = ctx.saved_tensors
         dx = _dropout_add(dy, None, ctx.cut, rng) if ctx.needs_input_grad[0] else None

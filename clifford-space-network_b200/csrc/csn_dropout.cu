@@ -27,57 +27,85 @@ __device__ __forceinline__ uint4 philox4x32(uint4 c, uint32_t k0, uint32_t k1) {
   return c;
 }
 
+// 8 neighbouring elements, as the words that they lie in
+template <typename T>
+struct Block8 {
+  static constexpr int N = 2 * (int)sizeof(T);
+  uint32_t w[N];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const uint4 q = __ldg(reinterpret_cast<const uint4*>(p) + i / 4);
+      w[i] = q.x, w[i + 1] = q.y, w[i + 2] = q.z, w[i + 3] = q.w;
+    }
+  }
+  __device__ __forceinline__ void store(T* p) const {
+#pragma unroll
+    for (int i = 0; i < N; i += 4)
+      reinterpret_cast<uint4*>(p)[i / 4] = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+  }
+  // elements 2 i and 2 i + 1
+  __device__ __forceinline__ float2 get(int i) const;
+  __device__ __forceinline__ void set(int i, float a, float b) {
+    if (sizeof(T) == 4) w[N / 4 * i] = __float_as_uint(a), w[N / 4 * i + N / 4 - 1] = __float_as_uint(b);
+    else w[i] = pack<T>(a, b);
+  }
+};
+template <>
+__device__ __forceinline__ float2 Block8<float>::get(int i) const {
+  return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+}
+template <>
+__device__ __forceinline__ float2 Block8<__nv_bfloat16>::get(int i) const {
+  return make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ float2 Block8<__half>::get(int i) const {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+}
+
+// x * scale where the place is kept; a dropped one is 0 whatever stood there, an infinity or a NaN too
+__device__ __forceinline__ float kept(uint32_t bits, uint32_t cut, float x, float scale) {
+  return bits >= cut ? x * scale : 0.0f;
+}
+
 template <typename T, bool RES>
 __global__ void __launch_bounds__(256) dropout_add_kernel(const T* __restrict__ x, const T* __restrict__ res,
                                                           const int64_t* __restrict__ rng, T* __restrict__ y,
                                                           int64_t n, uint32_t cut, float scale) {
   const uint64_t seed = (uint64_t)rng[0], off = (uint64_t)rng[1];
-  const int64_t blocks = (n + 7) / 8;
-  for (int64_t j = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; j < blocks; j += (int64_t)gridDim.x * blockDim.x) {
-    T xv[8], rv[8];
-    const int64_t i0 = j * 8;
-    const bool whole = i0 + 8 <= n;
-    if (whole) {
-      *reinterpret_cast<Pack<T, 16 / sizeof(T)>*>(xv) = *reinterpret_cast<const Pack<T, 16 / sizeof(T)>*>(x + i0);
-      if (sizeof(T) == 4)
-        *reinterpret_cast<Pack<T, 4>*>(xv + 4) = *reinterpret_cast<const Pack<T, 4>*>(x + i0 + 4);
-      if (RES) {
-        *reinterpret_cast<Pack<T, 16 / sizeof(T)>*>(rv) = *reinterpret_cast<const Pack<T, 16 / sizeof(T)>*>(res + i0);
-        if (sizeof(T) == 4)
-          *reinterpret_cast<Pack<T, 4>*>(rv + 4) = *reinterpret_cast<const Pack<T, 4>*>(res + i0 + 4);
-      }
-    } else {
-      for (int e = 0; e < 8; ++e)
-        if (i0 + e < n) {
-          xv[e] = x[i0 + e];
-          if (RES) rv[e] = res[i0 + e];
-        }
-    }
-    const uint4 w = philox4x32(make_uint4((uint32_t)j, (uint32_t)((uint64_t)j >> 32), (uint32_t)off, (uint32_t)(off >> 32)),
-                               (uint32_t)seed, (uint32_t)(seed >> 32));
+  auto draw = [&](int64_t j) {
+    return philox4x32(make_uint4((uint32_t)j, (uint32_t)((uint64_t)j >> 32), (uint32_t)off, (uint32_t)(off >> 32)),
+                      (uint32_t)seed, (uint32_t)(seed >> 32));
+  };
+  const int64_t whole = n / 8;
+  for (int64_t j = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; j < whole; j += (int64_t)gridDim.x * blockDim.x) {
+    Block8<T> xv, rv;
+    xv.load(x + j * 8);
+    if (RES) rv.load(res + j * 8);
+    const uint4 w = draw(j);
     const uint32_t word[4] = {w.x, w.y, w.z, w.w};
-    T out[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t bits = e & 1 ? word[e / 2] >> 16 : word[e / 2] & 0xffffu;
-      // a dropped place is 0 whatever stood there, an infinity or a NaN too
-      const float v = bits >= cut ? to_float(xv[e]) * scale : 0.0f;
-      out[e] = from_float<T>(RES ? to_float(rv[e]) + v : v);
+    for (int i = 0; i < 4; ++i) {
+      const float2 v = xv.get(i), r = RES ? rv.get(i) : make_float2(0.0f, 0.0f);
+      const float a = kept(word[i] & 0xffffu, cut, v.x, scale), b = kept(word[i] >> 16, cut, v.y, scale);
+      xv.set(i, RES ? r.x + a : a, RES ? r.y + b : b);
     }
-    if (whole) {
-      *reinterpret_cast<Pack<T, 16 / sizeof(T)>*>(y + i0) = *reinterpret_cast<Pack<T, 16 / sizeof(T)>*>(out);
-      if (sizeof(T) == 4) *reinterpret_cast<Pack<T, 4>*>(y + i0 + 4) = *reinterpret_cast<Pack<T, 4>*>(out + 4);
-    } else {
-      for (int e = 0; e < 8; ++e)
-        if (i0 + e < n) y[i0 + e] = out[e];
-    }
+    xv.store(y + j * 8);
+  }
+  if (blockIdx.x == 0 && threadIdx.x < n % 8) {  // the last, short block
+    const int e = threadIdx.x;
+    const uint4 w = draw(whole);
+    const uint32_t u = e < 2 ? w.x : e < 4 ? w.y : e < 6 ? w.z : w.w;
+    const float v = kept(e & 1 ? u >> 16 : u & 0xffffu, cut, to_float(x[whole * 8 + e]), scale);
+    y[whole * 8 + e] = from_float<T>(RES ? to_float(res[whole * 8 + e]) + v : v);
   }
 }
 
 template <typename T>
 void launch_dropout(const void* x, const void* res, const int64_t* rng, void* y, int64_t n, int cut, cudaStream_t st) {
   const int64_t ctas = ((n + 7) / 8 + 255) / 256;
-  const unsigned grid = (unsigned)(ctas < 148 * 64 ? ctas : 148 * 64);
+  const unsigned grid = (unsigned)(ctas < 148 * 8 ? ctas : 148 * 8);  // 8 fit on an SM
   const float scale = cut < 65536 ? 65536.0f / (float)(65536 - cut) : 0.0f;
   const T* xt = static_cast<const T*>(x);
   const T* rt = static_cast<const T*>(res);

@@ -344,18 +344,23 @@ __global__ void __launch_bounds__(THREADS, 1) mm_kernel(const __grid_constant__ 
   if (warp == EPI_WARPS) tmem_free<2 * BN>(tmem);
 }
 
-// sums of the k ranges, in their order
+// Sums of the k ranges, in their order: element i of half h is out[h][i].
 template <bool BF16>
-__global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ part, void* out, int64_t n, int64_t stride,
-                                                   int splits, const uint32_t* amax) {
+__global__ void __launch_bounds__(128) join_kernel(const float* __restrict__ part, void* out0, void* out1, int64_t n,
+                                                   int halves, int splits, const uint32_t* amax) {
   const float down = scale_down(amax);
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
-    float v = 0.0f;
-    for (int s = 0; s < splits; ++s) v += part[s * stride + i];
-    v *= down;
-    if (BF16) static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(v);
-    else static_cast<__half*>(out)[i] = __float2half_rn(v);
-  }
+  const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x, stride = n * halves;
+  if (i >= stride) return;
+  const bool second = i >= n;
+  void* out = second ? out1 : out0;
+  if (!out) return;
+  float v = 0.0f;
+#pragma unroll 8
+  for (int s = 0; s < splits; ++s) v += part[s * stride + i];
+  v *= down;
+  const int64_t at = second ? i - n : i;
+  if (BF16) static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
+  else static_cast<__half*>(out)[at] = __float2half_rn(v);
 }
 
 // bits of the largest |dy| (0 before): a maximum does not depend on the order
@@ -499,14 +504,16 @@ __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(const __grid_cons
 // ---------------------------------------------------------------------------- host
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to; }
 
-// How a product of m x n over k blocks is cut up.  Narrow tiles where 256 columns would leave SMs idle (or the
-// columns are few); and where even those leave more than half of the SMs idle, ranges of k of at least 4 blocks.
+// How a product of m x n over k blocks is cut up: into tiles 256 or 128 columns wide, whichever takes less time when
+// SMS of them run at a time.  A k block of a wide tile counts 1 and of a narrow one 0.56 (measured: it reads more for
+// each product), what a tile costs besides 4 and 2.  Where tiles leave more than half of the SMs idle, k is cut into
+// ranges of at least 4 blocks, whose sums a second kernel adds.
 struct Plan {
   int bn, mt, nt, splits, kper;
   Plan(int64_t m, int64_t n, int64_t blocks, int halves, bool gate) {
     mt = (int)up(m, BM);
-    const int wide = gate ? 128 : 256;  // columns of a 256-wide tile
-    bn = n <= wide / 2 || mt * up(n, wide) * halves < SMS ? 128 : 256;
+    const int64_t wide = mt * up(n, gate ? 128 : 256) * halves, narrow = mt * up(n, gate ? 64 : 128) * halves;
+    bn = up(wide, SMS) * (blocks + 4.0) <= up(narrow, SMS) * (0.56 * blocks + 2.0) ? 256 : 128;
     nt = (int)up(n, gate ? bn / 2 : bn);
     splits = 1;
     const int64_t tiles = (int64_t)mt * nt * halves;
@@ -608,16 +615,13 @@ int forward(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void*
 }
 
 template <Mode MODE, bool BF16>
-int run_product(const Maps& maps, Args P, int64_t blocks, const Plan& p, float* part, int64_t outs, cudaStream_t st,
+int run_product(const Maps& maps, Args P, int64_t blocks, const Plan& p, float* part, cudaStream_t st,
                 const char* who) {
   P.mt = p.mt, P.nt = p.nt, P.kb = (int)(blocks / P.halves_k), P.splits = p.splits, P.kper = p.kper, P.part = part;
   int rc = p.bn == 256 ? run_mm<MODE, BF16, 256>(maps, P, st, who) : run_mm<MODE, BF16, 128>(maps, P, st, who);
   if (rc || p.splits == 1) return rc;
-  const int64_t n = (int64_t)P.m * P.n, ctas = up(n, 256);
-  for (int h = 0; h < outs; ++h)
-    if (P.out[h])
-      join_kernel<BF16><<<(unsigned)(ctas < 8 * SMS ? ctas : 8 * SMS), 256, 0, st>>>(part + h * n, P.out[h], n, outs * n,
-                                                                                     p.splits, P.amax);
+  const int64_t n = (int64_t)P.m * P.n;
+  join_kernel<BF16><<<(unsigned)up(n * P.halves_m, 128), 128, 0, st>>>(part, P.out[0], P.out[1], n, P.halves_m, p.splits, P.amax);
   return check_launch(who);
 }
 
@@ -644,7 +648,7 @@ int backward(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void
       return set_error(CSN_ERR_CUDA, "silu_gated_linear: cuTensorMapEncodeTiled");
     Args P = {};
     P.m = (int)R, P.n = (int)C, P.halves_m = 1, P.halves_k = 2, P.out[0] = dx, P.ldo = C, P.amax = amax;
-    if (int rc = run_product<DX, BF16>(maps, P, 2 * up(F, BK), p, part, 1, st, who)) return rc;
+    if (int rc = run_product<DX, BF16>(maps, P, 2 * up(F, BK), p, part, st, who)) return rc;
   }
   if (dwg || dwu) {
     const Plan p(F, C, up(R, BK), 2, false);
@@ -655,7 +659,7 @@ int backward(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void
     maps.b[1] = maps.b[0];
     Args P = {};
     P.m = (int)F, P.n = (int)C, P.halves_m = 2, P.halves_k = 1, P.out[0] = dwg, P.out[1] = dwu, P.ldo = C, P.amax = amax;
-    if (int rc = run_product<DW, BF16>(maps, P, up(R, BK), p, part, 2, st, who)) return rc;
+    if (int rc = run_product<DW, BF16>(maps, P, up(R, BK), p, part, st, who)) return rc;
   }
   return CSN_OK;
 }

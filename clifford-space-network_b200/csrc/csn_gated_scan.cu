@@ -100,16 +100,16 @@ struct Part {
   }
 };
 
-// bytes of a tile's row in shared memory: 128, and a word more (kept to 16 bytes) where rows are odd
-__host__ __device__ constexpr int row_bytes(bool odd) { return odd ? 144 : 128; }
-__host__ __device__ constexpr int piece_bytes(bool odd) { return MARK * row_bytes(odd); }  // of one tensor's rows of one CTA pass
+constexpr int ROW = 128;           // bytes of a tile's row in shared memory
+constexpr int PIECE = MARK * ROW;  // of one tensor's rows of one CTA pass
 
 template <typename T>
 struct Lane {
   static constexpr int V = sizeof(T) == 4 ? 1 : 2;  // channels of a lane
   using F = Vals<V>;
-  static constexpr int CHANNELS = 32 * V;           // of a tile
 };
+// channels of a tile: 32 words' worth, less a pair where rows are odd, so that 32 words hold them at either shift
+__host__ __device__ constexpr int channels(int size, bool odd) { return size == 4 ? 32 : odd ? 62 : 64; }
 
 template <typename T>
 __device__ __forceinline__ Vals<Lane<T>::V> unpack(uint32_t v);
@@ -150,7 +150,7 @@ struct Input {
   __device__ __forceinline__ Input(const Rows& r, const ScanArgs& A, const Part& part, int64_t tile, int t1) {
     p = q = nullptr;
     row = r.row * (int64_t)sizeof(T);
-    left = (int)min((int64_t)32 * Lane<T>::V, A.C - tile) * (int)sizeof(T);
+    left = (int)min((int64_t)channels(sizeof(T), ODD), A.C - tile) * (int)sizeof(T);
     skew[0] = skew[1] = 0;
     if (!r.p) return;
     const int lane = threadIdx.x & 31;
@@ -167,7 +167,6 @@ struct Input {
   }
   // the warp's n rows into shared memory at `to`, then `step` rows on
   __device__ __forceinline__ void copy(char* to, int n, bool wide, int step) {
-    constexpr int ROW = row_bytes(ODD);
     const int lane = threadIdx.x & 31;
     const uint32_t at = (uint32_t)__cvta_generic_to_shared(to);
     if (ODD) {
@@ -178,11 +177,6 @@ struct Input {
 #pragma unroll
           for (int l = o; l < STEPS; l += 2)
             if (l < n) copy4(at + l * ROW + lane * 4, w + (l - o) * row);
-        }
-        if (lane == 0 && 128 < left + skew[o] / 8) {
-#pragma unroll
-          for (int l = o; l < STEPS; l += 2)
-            if (l < n) copy4(at + l * ROW + 128, w + (l - o) * row + 128);
         }
       }
       q += step * row;
@@ -208,8 +202,9 @@ struct Input {
   }
   // this lane's channels of the warp's row l, which was copied to `at`
   __device__ __forceinline__ Vals<Lane<T>::V> read(const char* at, int l) const {
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(at + l * row_bytes(ODD)) + (threadIdx.x & 31);
-    return unpack<T>(ODD ? __funnelshift_r(w[0], w[1], skew[l & 1]) : w[0]);
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(at + l * ROW) + (threadIdx.x & 31);
+    // ODD: the last lane has no channels, and reads its own word twice
+    return unpack<T>(ODD ? __funnelshift_r(w[0], w[(threadIdx.x & 31) < 31], skew[l & 1]) : w[0]);
   }
 };
 
@@ -285,16 +280,16 @@ __device__ __forceinline__ Vals<V> enter(const ScanArgs& A, Map<V> (*maps)[32], 
 template <typename T, bool GATE, bool ODD, bool BACK>
 __global__ void __launch_bounds__(WARPS * 32, 3) reduce_kernel(const __grid_constant__ ScanArgs A) {
   using F = typename Lane<T>::F;
-  constexpr int V = Lane<T>::V, N = BACK && GATE ? 3 : 2, PIECE = piece_bytes(ODD);
+  constexpr int V = Lane<T>::V, N = BACK && GATE ? 3 : 2;
   extern __shared__ __align__(128) char ring[];  // [2][N][MARK rows]
   __shared__ Map<V> maps[WARPS][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Part q(A, blockIdx.x / A.tiles);
   if (q.s < 0 || (BACK ? q.k == 0 : q.to == q.len)) return;
-  const int64_t tile = (int64_t)(blockIdx.x % A.tiles) * Lane<T>::CHANNELS, c = tile + lane * V;
-  const int have = (int)max((int64_t)0, min((int64_t)V, A.C - c));
+  const int64_t tile = (int64_t)(blockIdx.x % A.tiles) * channels(sizeof(T), ODD), c = tile + lane * V;
+  const int have = (int)max((int64_t)0, min((int64_t)V, min(A.C, tile + channels(sizeof(T), ODD)) - c));
   const int share = A.chunk / WARPS, first = q.from + warp * share, past = min(first + share, q.to);
-  char* mine = ring + warp * STEPS * row_bytes(ODD);
+  char* mine = ring + warp * STEPS * ROW;
   // BACK goes from the last steps to the first
   int t = BACK ? first + (max(past - first, 1) - 1) / STEPS * STEPS : first;
   const int step = BACK ? -STEPS : STEPS;
@@ -351,16 +346,16 @@ __global__ void __launch_bounds__(WARPS * 32, 3) reduce_kernel(const __grid_cons
 template <typename T, bool GATE, bool ODD>
 __global__ void __launch_bounds__(WARPS * 32, 3) gated_scan_fwd_kernel(const __grid_constant__ ScanArgs A) {
   using F = typename Lane<T>::F;
-  constexpr int V = Lane<T>::V, N = GATE ? 3 : 2, PIECE = piece_bytes(ODD);
+  constexpr int V = Lane<T>::V, N = GATE ? 3 : 2;
   extern __shared__ __align__(128) char ring[];  // [2][N][MARK rows]
   __shared__ Map<V> maps[2][WARPS][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Part q(A, blockIdx.x / A.tiles);
   if (q.s < 0) return;
-  const int64_t tile = (int64_t)(blockIdx.x % A.tiles) * Lane<T>::CHANNELS, c = tile + lane * V;
-  const int have = (int)max((int64_t)0, min((int64_t)V, A.C - c));
+  const int64_t tile = (int64_t)(blockIdx.x % A.tiles) * channels(sizeof(T), ODD), c = tile + lane * V;
+  const int have = (int)max((int64_t)0, min((int64_t)V, min(A.C, tile + channels(sizeof(T), ODD)) - c));
   int t1 = q.from + warp * STEPS;
-  char* mine = ring + warp * STEPS * row_bytes(ODD);
+  char* mine = ring + warp * STEPS * ROW;
   Input<T, ODD> f(A.f, A, q, tile, t1), x(A.x, A, q, tile, t1), g(A.g, A, q, tile, t1);
   auto fetch = [&](int half, int n) {
     char* to = mine + half * N * PIECE;
@@ -432,7 +427,7 @@ __global__ void __launch_bounds__(WARPS * 32, 3) gated_scan_fwd_kernel(const __g
 template <typename T, bool GATE, bool ODD>
 __global__ void __launch_bounds__(WARPS * 32, 2) gated_scan_bwd_kernel(const __grid_constant__ ScanArgs A) {
   using F = typename Lane<T>::F;
-  constexpr int V = Lane<T>::V, N = GATE ? 4 : 3, PIECE = piece_bytes(ODD);
+  constexpr int V = Lane<T>::V, N = GATE ? 4 : 3;
   extern __shared__ __align__(128) char ring[];  // [2][N][MARK rows]
   // a warp's steps forward, and back: what leaves its first step when nothing enters its last
   __shared__ Map<V> maps[2][WARPS][32];
@@ -440,11 +435,11 @@ __global__ void __launch_bounds__(WARPS * 32, 2) gated_scan_bwd_kernel(const __g
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Part q(A, blockIdx.x / A.tiles);
   if (q.s < 0) return;
-  const int64_t tile = (int64_t)(blockIdx.x % A.tiles) * Lane<T>::CHANNELS, c = tile + lane * V;
-  const int have = (int)max((int64_t)0, min((int64_t)V, A.C - c));
+  const int64_t tile = (int64_t)(blockIdx.x % A.tiles) * channels(sizeof(T), ODD), c = tile + lane * V;
+  const int have = (int)max((int64_t)0, min((int64_t)V, min(A.C, tile + channels(sizeof(T), ODD)) - c));
   const int last = q.to > q.from ? q.from + (q.to - q.from - 1) / MARK * MARK : q.from - MARK;
   int t1 = last + warp * STEPS;
-  char* mine = ring + warp * STEPS * row_bytes(ODD);
+  char* mine = ring + warp * STEPS * ROW;
   Input<T, ODD> f(A.f, A, q, tile, t1), x(A.x, A, q, tile, t1), d(A.dy, A, q, tile, t1), g(A.g, A, q, tile, t1);
   auto fetch = [&](int half, int n) {
     char* to = mine + half * N * PIECE;
@@ -611,10 +606,10 @@ bool rows_align(const Rows& r, int size, int bytes) {
 struct Cut {
   int tiles, chunk, chunks;
   int64_t units;
-  Cut(int64_t S, int64_t T, int64_t C, bool packed, int dtype, bool bwd) {
-    const int channels = dtype == CSN_F32 ? 32 : 64;
+  Cut(int64_t S, int64_t T, int64_t C, bool packed, int dtype, bool odd, bool bwd) {
+    const int wide = channels(dtype == CSN_F32 ? 4 : 2, odd);
     const int64_t slots = 148 * (bwd ? 2 : 3);
-    tiles = (int)((C + channels - 1) / channels);
+    tiles = (int)((C + wide - 1) / wide);
     int64_t n = packed ? 1 : slots / (S * tiles);
     int64_t len = packed ? T * tiles / slots : n > 1 ? T / n : T;
     len = (len + MARK - 1) / MARK * MARK;
@@ -639,7 +634,7 @@ cudaError_t launch_part(K kernel, int64_t grid, int smem, const ScanArgs& A, cud
 template <typename T, bool GATE, bool ODD>
 cudaError_t launch_scan(const ScanArgs& A, bool bwd, const Cut& cut, cudaStream_t st) {
   const int64_t grid = cut.units * cut.tiles;
-  const int piece = 2 * piece_bytes(ODD);
+  const int piece = 2 * PIECE;
   if (cut.split(A.T)) {
     const cudaError_t e = bwd ? launch_part(reduce_kernel<T, GATE, ODD, true>, grid, (GATE ? 3 : 2) * piece, A, st)
                               : launch_part(reduce_kernel<T, false, ODD, false>, grid, 2 * piece, A, st);
@@ -655,17 +650,17 @@ cudaError_t launch_scan(const ScanArgs& A, bool bwd, const Cut& cut, cudaStream_
 
 int dispatch_scan(ScanArgs A, int dtype, bool bwd, void* workspace, size_t bytes, cudaStream_t st, const char* who) {
   const int size = width_of(dtype);
-  const Cut cut(A.S, A.T, A.C, A.cu != nullptr, dtype, bwd);
-  A.tiles = cut.tiles, A.chunk = cut.chunk, A.chunks = cut.chunks, A.maps = static_cast<float2*>(workspace);
-  if (cut.units * cut.tiles > 0x7fffffff) return set_error(CSN_ERR_INVALID, "csn_gated_scan: more than 2^31 - 1 tiles of work");
-  if (cut.split(A.T) && (!workspace || !aligned(workspace, 16) || bytes < (size_t)cut.units * A.C * sizeof(float2)))
-    return set_error(CSN_ERR_INVALID, "csn_gated_scan: workspace smaller than csn_gated_scan_workspace_bytes");
   auto all = [&](int to) {
     return A.C * size % to == 0 && rows_align(A.f, size, to) && rows_align(A.x, size, to) && rows_align(A.g, size, to) &&
            rows_align(A.dy, size, to);
   };
   A.wide = all(16);
   const bool odd = !all(4);
+  const Cut cut(A.S, A.T, A.C, A.cu != nullptr, dtype, odd, bwd);
+  A.tiles = cut.tiles, A.chunk = cut.chunk, A.chunks = cut.chunks, A.maps = static_cast<float2*>(workspace);
+  if (cut.units * cut.tiles > 0x7fffffff) return set_error(CSN_ERR_INVALID, "csn_gated_scan: more than 2^31 - 1 tiles of work");
+  if (cut.split(A.T) && (!workspace || !aligned(workspace, 16) || bytes < (size_t)cut.units * A.C * sizeof(float2)))
+    return set_error(CSN_ERR_INVALID, "csn_gated_scan: workspace smaller than csn_gated_scan_workspace_bytes");
   const cudaError_t e =
       dtype == CSN_F32 ? launch_scan<float, false>(A, bwd, cut, st)
       : dtype == CSN_BF16
@@ -677,7 +672,7 @@ int dispatch_scan(ScanArgs A, int dtype, bool bwd, void* workspace, size_t bytes
 int check_scan(const char* who, const ScanArgs& A, int dtype) {
   if (A.S < 0 || A.T < 0 || A.C < 0 || A.T > (1 << 30)) return set_error(CSN_ERR_INVALID, who);
   if (!width_of(dtype)) return set_error(CSN_ERR_UNSUPPORTED, who);
-  // a CTA for each 32 channels of a sequence
+  // a CTA for each 32 channels of a sequence at least
   if (A.S > 0 && A.C > 0 && (A.C + 31) / 32 > (int64_t)0x7fffffff / A.S) return set_error(CSN_ERR_INVALID, who);
   return CSN_OK;
 }
@@ -696,8 +691,13 @@ extern "C" size_t csn_gated_scan_workspace_bytes(int64_t S, int64_t T, int64_t C
   ScanArgs A = {};
   A.S = S, A.T = T, A.C = C;
   if (S <= 0 || T <= 0 || C <= 0 || check_scan("", A, dtype)) return 0;
-  const Cut cut(S, T, C, packed != 0, dtype, backward != 0);
-  return cut.split(T) ? (size_t)cut.units * C * sizeof(float2) : 0;
+  size_t most = 0;  // whichever way the rows turn out to lie
+  for (int odd = 0; odd < 2; ++odd) {
+    const Cut cut(S, T, C, packed != 0, dtype, odd != 0, backward != 0);
+    const size_t n = cut.split(T) ? (size_t)cut.units * C * sizeof(float2) : 0;
+    if (n > most) most = n;
+  }
+  return most;
 }
 
 extern "C" int csn_gated_scan_fwd(const void* f, const void* x, const void* gate, const int64_t* strides,
