@@ -9,12 +9,15 @@
 // whose smallest number is 2^-24, they are first scaled by the power of two that brings the largest |dy| into [1, 2),
 // and the products are scaled back in float32.
 //
-// mm_kernel is one persistent kernel for the four products (Mode).  A CTA owns an SM: one thread feeds a ring of
-// shared-memory stages by TMA, one issues tcgen05.mma into one of two accumulators in tensor memory, and eight warps
-// finish the other accumulator, so that loads, products and epilogue overlap across tiles.  A tile is 128 x BN.  For
-// the gate, BN = 2 FN: FN rows of Wg and the same FN rows of Wu lie one after the other in shared memory as one
-// operand, so g and u of a place sit in one tensor-memory lane and the gate is a per-lane epilogue.  The transposed
-// products read the same row-major tensors with an MN-major operand: nothing is transposed in memory.
+// mm_kernel is one persistent kernel for the four products (Mode).  A pair of CTAs on two SMs (cta_group::2) makes a
+// tile of 256 x BN: each loads 128 rows of A and half of B, so a k block of 64 moves 32 KB into an SM for the products
+// that take 48 KB when it works alone; what L2 delivers (about 60 bytes a clock and SM) is what bounds a large product.
+// In each CTA one thread feeds a ring of shared-memory stages by TMA, one of the pair issues tcgen05.mma into one of
+// two accumulators in tensor memory, and for each accumulator eight warps finish it, so that loads, products and both
+// epilogues overlap across tiles.  For the gate, BN = 2 FN: CTA 0 loads FN rows of Wg and CTA 1 the same FN rows of Wu
+// as the halves of one operand, so g and u of a place sit in one tensor-memory lane and the gate is a per-lane
+// epilogue.  The transposed products read the same row-major tensors with an MN-major operand: nothing is transposed in
+// memory.
 //
 // few_rows_kernel takes R <= 64 rows (generation): there the weights are what is read, so they take the 128-row side
 // of the product (64 rows of Wg and 64 of Wu) and x the narrow side, and a cluster splits C where F alone gives too
@@ -33,15 +36,15 @@ using namespace tc;
 
 enum Mode { GATE, GATE_BWD, DX, DW };
 
-constexpr int BM = 128, BK = 64;
-constexpr int EPI_WARPS = 8;
+constexpr int BM = 128, BK = 64;                    // rows of a CTA (a pair has 2 BM), k of a stage
+constexpr int EPI_WARPS = 16;                       // 8 for each accumulator
 constexpr int THREADS = (EPI_WARPS + 2) * 32;
 constexpr int STAGE_ROW = 80;                       // a lane's 64 bytes, padded against bank conflicts
 constexpr int STAGING = EPI_WARPS * 32 * STAGE_ROW;
-constexpr int SMS = 148;                            // what the work is cut up for
+constexpr int PAIRS = 74;                           // of SMs: what the work is cut up for
 
-__host__ __device__ constexpr int stage_bytes(int bn) { return (BM + bn) * BK * 2; }
-__host__ __device__ constexpr int stages(int bn) { return bn == 256 ? 4 : 6; }
+__host__ __device__ constexpr int stage_bytes(int bn) { return (BM + bn / 2) * BK * 2; }
+__host__ __device__ constexpr int stages(int bn) { return bn == 256 ? 5 : 7; }
 constexpr int smem_bytes(int bn) { return stages(bn) * stage_bytes(bn) + STAGING + 1024; }
 
 struct Maps {
@@ -90,32 +93,28 @@ __device__ __forceinline__ float2 unpack2(uint32_t v) {
   return __half22float2(*reinterpret_cast<__half2*>(&v));
 }
 
-// A warp's 32 rows x 64 bytes, one row a lane, to memory in whole row pieces (4 lanes a row, 8 rows an access);
-// `vec`: rows start on 16 bytes and hold multiples of 16.
-__device__ __forceinline__ void put_rows(char* stage, int lane, const uint32_t* v, char* out, int64_t row_bytes,
-                                         int rows, int bytes, bool vec) {
-  uint4* mine = reinterpret_cast<uint4*>(stage + lane * STAGE_ROW);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) mine[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+// A warp's 32 rows x 64 bytes pass between a lane's own row in `stage` and memory in whole row pieces (4 lanes a row,
+// 8 rows an access); `vec`: rows start on 16 bytes and hold multiples of 16.
+__device__ __forceinline__ void put_rows(const char* stage, int lane, char* out, int64_t row_bytes, int rows, int bytes,
+                                         bool vec) {
   __syncwarp();
   if (vec) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int r = i * 8 + lane / 4, at = lane % 4 * 16;
       if (r < rows && at < bytes)
-        *reinterpret_cast<uint4*>(out + r * row_bytes + at) = *reinterpret_cast<uint4*>(stage + r * STAGE_ROW + at);
+        *reinterpret_cast<uint4*>(out + r * row_bytes + at) = *reinterpret_cast<const uint4*>(stage + r * STAGE_ROW + at);
     }
   } else if (lane * 2 < bytes) {
     for (int r = 0; r < rows; ++r)
       *reinterpret_cast<uint16_t*>(out + r * row_bytes + lane * 2) =
-          *reinterpret_cast<uint16_t*>(stage + r * STAGE_ROW + lane * 2);
+          *reinterpret_cast<const uint16_t*>(stage + r * STAGE_ROW + lane * 2);
   }
   __syncwarp();
 }
-
-// the same the other way: what lies outside comes as 0
-__device__ __forceinline__ void get_rows(char* stage, int lane, uint32_t* v, const char* in, int64_t row_bytes, int rows,
-                                         int bytes, bool vec) {
+// what lies outside comes as 0
+__device__ __forceinline__ void get_rows(char* stage, int lane, const char* in, int64_t row_bytes, int rows, int bytes,
+                                         bool vec) {
   if (vec) {
     uint4 got[4];
 #pragma unroll
@@ -132,17 +131,19 @@ __device__ __forceinline__ void get_rows(char* stage, int lane, uint32_t* v, con
           r < rows && lane * 2 < bytes ? *reinterpret_cast<const uint16_t*>(in + r * row_bytes + lane * 2) : (uint16_t)0;
   }
   __syncwarp();
-  const uint4* mine = reinterpret_cast<const uint4*>(stage + lane * STAGE_ROW);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint4 q = mine[i];
-    v[4 * i] = q.x, v[4 * i + 1] = q.y, v[4 * i + 2] = q.z, v[4 * i + 3] = q.w;
-  }
-  __syncwarp();
+}
+// 8 words (32 bytes) of a lane's own row
+__device__ __forceinline__ void put8(char* p, const uint32_t* v) {
+  reinterpret_cast<uint4*>(p)[0] = make_uint4(v[0], v[1], v[2], v[3]);
+  reinterpret_cast<uint4*>(p)[1] = make_uint4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void get8(const char* p, uint32_t* v) {
+  const uint4 a = reinterpret_cast<const uint4*>(p)[0], b = reinterpret_cast<const uint4*>(p)[1];
+  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
 }
 
 // Tiles are walked in groups of 16 rows of tiles, column by column: the operands of the tiles under way at one time
-// (16 x 9) are read from HBM once and stay in L2.
+// (16 x 5 pairs') are read from HBM once and stay in L2.
 struct Tile {
   int m, n, half, split;
   __device__ __forceinline__ Tile(const Args& P, int t) {
@@ -159,17 +160,20 @@ struct Tile {
 };
 
 template <Mode MODE, bool BF16, int BN>
-__global__ void __launch_bounds__(THREADS, 1) mm_kernel(const __grid_constant__ Maps maps, const Args P) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+    mm_kernel(const __grid_constant__ Maps maps, const Args P) {
   constexpr int ST = stages(BN), SB = stage_bytes(BN);
   constexpr bool A_MN = MODE == DW, B_MN = MODE == DX || MODE == DW;
   constexpr int FN = BN / 2;
   extern __shared__ char raw[];
+  // full, acc_empty: those of CTA 0 count for the pair; empty, acc_full: each CTA's own
   __shared__ uint64_t full[ST], empty[ST], acc_full[2], acc_empty[2], drained;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile uint32_t gave_up;
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tiles = P.mt * P.nt * P.halves_m * P.splits;
+  const int rank = (int)cluster_rank();
+  const int tiles = P.mt * P.nt * P.halves_m * P.splits, first = blockIdx.x / 2, step = gridDim.x / 2;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < ST; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
@@ -178,9 +182,10 @@ __global__ void __launch_bounds__(THREADS, 1) mm_kernel(const __grid_constant__ 
     mbar_init_fence();
     gave_up = 0;
   }
-  if (warp == EPI_WARPS) tmem_alloc<2 * BN>(&tmem_slot);
+  if (warp == EPI_WARPS) tmem_alloc_pair<2 * BN>(&tmem_slot);
   fence_before();
   __syncthreads();
+  cluster_sync();  // the other CTA's barriers are there
   fence_after();
   const uint32_t tmem = tmem_slot;
 
@@ -188,160 +193,171 @@ __global__ void __launch_bounds__(THREADS, 1) mm_kernel(const __grid_constant__ 
     if (lane == 0) {  // TMA
       int it = 0;
       bool ok = true;
-      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      for (int t = first; t < tiles && ok; t += step) {
         const Tile T(P, t);
         const int k0 = T.split * P.kper, k1 = min(k0 + P.kper, P.kb * P.halves_k);
+        const int m = (T.m * 2 + rank) * BM;
         for (int k = k0; k < k1; ++k, ++it) {
           const int s = it % ST;
-          if (!(ok = mbar_wait(&empty[s], (it / ST + 1) & 1, &gave_up))) break;
-          mbar_expect(&full[s], SB);
+          if (!(ok = mbar_wait<true>(&empty[s], (it / ST + 1) & 1, &gave_up))) break;
+          if (rank == 0) mbar_expect(&full[s], 2 * SB);
+          const uint32_t bar = peer_addr(&full[s], 0);
           char* a = smem + s * SB;
           char* b = a + BM * BK * 2;
           if (MODE == GATE || MODE == GATE_BWD) {
-            tma_load(a, &maps.a[0], k * BK, T.m * BM, &full[s]);
-            tma_load(b, &maps.b[0], k * BK, T.n * FN, &full[s]);
-            tma_load(b + FN * BK * 2, &maps.b[1], k * BK, T.n * FN, &full[s]);
+            tma_load_pair(a, &maps.a[0], k * BK, m, bar);
+            tma_load_pair(b, &maps.b[rank], k * BK, T.n * FN, bar);
           } else if (MODE == DX) {
             const int h = k >= P.kb, kk = (k - h * P.kb) * BK;
-            tma_load(a, &maps.a[h], kk, T.m * BM, &full[s]);
+            tma_load_pair(a, &maps.a[h], kk, m, bar);
 #pragma unroll
-            for (int j = 0; j < BN / 64; ++j) tma_load(b + j * 8192, &maps.b[h], T.n * BN + j * 64, kk, &full[s]);
+            for (int j = 0; j < FN / 64; ++j)
+              tma_load_pair(b + j * 8192, &maps.b[h], T.n * BN + rank * FN + j * 64, kk, bar);
           } else {
 #pragma unroll
-            for (int j = 0; j < BM / 64; ++j) tma_load(a + j * 8192, &maps.a[T.half], T.m * BM + j * 64, k * BK, &full[s]);
+            for (int j = 0; j < BM / 64; ++j) tma_load_pair(a + j * 8192, &maps.a[T.half], m + j * 64, k * BK, bar);
 #pragma unroll
-            for (int j = 0; j < BN / 64; ++j) tma_load(b + j * 8192, &maps.b[0], T.n * BN + j * 64, k * BK, &full[s]);
+            for (int j = 0; j < FN / 64; ++j)
+              tma_load_pair(b + j * 8192, &maps.b[0], T.n * BN + rank * FN + j * 64, k * BK, bar);
           }
         }
       }
-      if (!ok)  // copies in flight end before the shared memory does
+      if (ok) {  // the pair's last commits arrive before this CTA leaves
+        for (int j = it > ST ? it - ST : 0; j < it; ++j) mbar_wait<true>(&empty[j % ST], (j / ST) & 1, &gave_up);
+      } else if (rank == 0)  // copies in flight end before the shared memory does (CTA 0's barriers count both CTAs')
         for (int j = it > ST ? it - ST : 0; j < it; ++j)
           for (uint32_t i = 0; i < POLLS && !mbar_try(&full[j % ST], (j / ST) & 1); ++i) {}
     }
   } else if (warp == EPI_WARPS + 1) {
-    if (lane == 0) {  // MMA
-      constexpr uint32_t IDESC = instruction(BF16, A_MN, B_MN, BM, BN);
+    if (lane == 0 && rank == 0) {  // MMA
+      constexpr uint32_t IDESC = instruction(BF16, A_MN, B_MN, 2 * BM, BN);
       int it = 0, n = 0;
       bool ok = true;
-      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++n) {
+      for (int t = first; t < tiles && ok; t += step, ++n) {
         const Tile T(P, t);
         const int k0 = T.split * P.kper, k1 = min(k0 + P.kper, P.kb * P.halves_k);
         const uint32_t d = tmem + (n & 1) * BN;
-        if (!(ok = mbar_wait(&acc_empty[n & 1], ((n >> 1) + 1) & 1, &gave_up))) break;
+        if (!(ok = mbar_wait<true>(&acc_empty[n & 1], ((n >> 1) + 1) & 1, &gave_up))) break;
         fence_after();
         for (int k = k0; k < k1; ++k, ++it) {
           const int s = it % ST;
-          if (!(ok = mbar_wait(&full[s], (it / ST) & 1, &gave_up))) break;
+          if (!(ok = mbar_wait<true>(&full[s], (it / ST) & 1, &gave_up))) break;
           fence_after();
           const uint32_t a = smem_addr(smem + s * SB), b = a + BM * BK * 2;
           const uint64_t ad = operand(a, 8192), bd = operand(b, 8192);
 #pragma unroll
           for (int j = 0; j < BK / 16; ++j)
-            mma(d, ad + j * (A_MN ? 2048 >> 4 : 32 >> 4), bd + j * (B_MN ? 2048 >> 4 : 32 >> 4), IDESC, k > k0 || j > 0);
-          mma_commit(&empty[s]);
+            mma_pair(d, ad + j * (A_MN ? 2048 >> 4 : 32 >> 4), bd + j * (B_MN ? 2048 >> 4 : 32 >> 4), IDESC, k > k0 || j > 0);
+          mma_commit_pair(&empty[s]);
         }
-        if (ok) mma_commit(&acc_full[n & 1]);
+        if (ok) mma_commit_pair(&acc_full[n & 1]);
       }
       if (!ok) {
-        mma_commit(&drained);
+        mma_commit_pair(&drained);
         for (uint32_t i = 0; i < POLLS && !mbar_try(&drained, 0); ++i) {}
       }
     }
   } else {
-    // epilogue: warp w reads the tensor-memory lanes of quarter w % 4 and half of the columns
+    // epilogue: warp w finishes accumulator w / 8, reads the tensor-memory lanes of quarter w % 4 and half of the columns
     char* stage = smem + ST * SB + warp * 32 * STAGE_ROW;
-    const int quarter = warp % 4, side = warp / 4;
+    char* own = stage + lane * STAGE_ROW;
+    const int acc = warp / 8, quarter = warp % 4, side = warp / 4 % 2;
     const float up = MODE == GATE_BWD ? scale_up(P.amax) : 1.0f;
     const float down = MODE == DX || MODE == DW ? scale_down(P.amax) : 1.0f;
-    int n = 0;
-    for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++n) {
+    const uint32_t d = tmem + acc * BN + ((uint32_t)(quarter * 32) << 16), release = peer_addr(&acc_empty[acc], 0);
+    const bool vec = (MODE == DX || MODE == DW) && P.splits > 1 ? P.n % 4 == 0 : P.ldo % 8 == 0;
+    const bool vec_dy = MODE == GATE_BWD && P.ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(P.dy) & 15) == 0 && P.n % 8 == 0;
+    uint32_t parity = 0;
+    for (int t = first + acc * step; t < tiles; t += 2 * step, parity ^= 1) {
       const Tile T(P, t);
-      const uint32_t d = tmem + (n & 1) * BN + ((uint32_t)(quarter * 32) << 16);
-      const int64_t row0 = (int64_t)T.m * BM + quarter * 32;
+      const int64_t row0 = (int64_t)(T.m * 2 + rank) * BM + quarter * 32;
       const int rows = (int)min((int64_t)32, P.m - row0);
-      const bool ok = mbar_wait(&acc_full[n & 1], (n >> 1) & 1, &gave_up);
+      const bool ok = mbar_wait(&acc_full[acc], parity, &gave_up);
       __syncwarp();
       fence_after();
-      if (MODE == GATE || MODE == GATE_BWD) {
-        const bool vec = P.ldo % 8 == 0;
-        const bool vec_dy = MODE == GATE_BWD && P.ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(P.dy) & 15) == 0 && P.n % 8 == 0;
+      const float nan = __int_as_float(0x7fffffff);
 #pragma unroll 1
-        for (int c = side * (FN / 2); c < (side + 1) * (FN / 2); c += 32) {
-          const int64_t col = (int64_t)T.n * FN + c;
-          const int bytes = (int)min((int64_t)32, P.n - col) * 2;
-          if (rows <= 0 || bytes <= 0) continue;
-          uint32_t dy[16];
-          if (MODE == GATE_BWD)
-            get_rows(stage, lane, dy, static_cast<const char*>(P.dy) + (row0 * P.ldy + col) * 2, P.ldy * 2, rows, bytes,
-                     vec_dy);
-          float g[32], u[32];
-          tmem_load32(d + c, g);
-          tmem_load32(d + FN + c, u);
-          tmem_load_wait();
-          if (!ok)
-#pragma unroll
-            for (int i = 0; i < 32; ++i) g[i] = __int_as_float(0x7fffffff);
-          uint32_t o0[16], o1[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float r0[2], r1[2];
-            const float2 dv = MODE == GATE_BWD ? unpack2<BF16>(dy[i]) : make_float2(0.0f, 0.0f);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const float gv = g[2 * i + j], uv = u[2 * i + j];
-              const float w = sigmoid(gv);
-              if (MODE == GATE) {
-                r0[j] = gv * w * uv;
-              } else {
-                const float e = (j ? dv.y : dv.x) * up;
-                r0[j] = e * uv * (w * fmaf(gv, 1.0f - w, 1.0f));
-                r1[j] = e * gv * w;
-              }
-            }
-            o0[i] = pack2<BF16>(r0[0], r0[1]);
-            if (MODE == GATE_BWD) o1[i] = pack2<BF16>(r1[0], r1[1]);
-          }
+      for (int c = side * (MODE <= GATE_BWD ? FN / 2 : FN); c < (side + 1) * (MODE <= GATE_BWD ? FN / 2 : FN); c += 32) {
+        const int64_t col = (int64_t)T.n * (MODE <= GATE_BWD ? FN : BN) + c;
+        const int cols = (int)min((int64_t)32, P.n - col);
+        if (rows <= 0 || cols <= 0) continue;
+        if (MODE == GATE || MODE == GATE_BWD) {
           const int64_t at = (row0 * P.ldo + col) * 2;
-          put_rows(stage, lane, o0, static_cast<char*>(P.out[0]) + at, P.ldo * 2, rows, bytes, vec);
-          if (MODE == GATE_BWD) put_rows(stage, lane, o1, static_cast<char*>(P.out[1]) + at, P.ldo * 2, rows, bytes, vec);
-        }
-      } else {
-#pragma unroll 1
-        for (int c = side * (BN / 2); c < (side + 1) * (BN / 2); c += 32) {
-          const int64_t col = (int64_t)T.n * BN + c;
-          const int cols = (int)min((int64_t)32, P.n - col);
-          if (rows <= 0 || cols <= 0) continue;
-          float v[32];
-          tmem_load32(d + c, v);
-          tmem_load_wait();
-          if (!ok)
+          if (MODE == GATE_BWD)
+            get_rows(stage, lane, static_cast<const char*>(P.dy) + (row0 * P.ldy + col) * 2, P.ldy * 2, rows, cols * 2, vec_dy);
+          uint32_t du[2][8];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = __int_as_float(0x7fffffff);
-          if (P.splits > 1) {
-            char* out = reinterpret_cast<char*>(P.part) +
-                        ((((int64_t)T.split * P.halves_m + T.half) * P.m + row0) * P.n + col) * 4;
-            put_rows(stage, lane, reinterpret_cast<uint32_t*>(v), out, (int64_t)P.n * 4, rows, min(cols, 16) * 4, P.n % 4 == 0);
-            if (cols > 16)
-              put_rows(stage, lane, reinterpret_cast<uint32_t*>(v + 16), out + 64, (int64_t)P.n * 4, rows, (cols - 16) * 4,
-                       P.n % 4 == 0);
-          } else if (void* to = T.half ? P.out[1] : P.out[0]) {
-            uint32_t o[16];
+          for (int h = 0; h < 2; ++h) {
+            float g[16], u[16];
+            tmem_load16(d + c + h * 16, g);
+            tmem_load16(d + FN + c + h * 16, u);
+            uint32_t dy[8], o[8];
+            if (MODE == GATE_BWD) get8(own + h * 32, dy);
+            tmem_load_wait();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = pack2<BF16>(v[2 * i] * down, v[2 * i + 1] * down);
-            put_rows(stage, lane, o, static_cast<char*>(to) + (row0 * P.ldo + col) * 2, P.ldo * 2, rows, cols * 2,
-                     P.ldo % 8 == 0);
+            for (int i = 0; i < 8; ++i) {
+              float r0[2], r1[2];
+              const float2 dv = MODE == GATE_BWD ? unpack2<BF16>(dy[i]) : make_float2(0.0f, 0.0f);
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const float gv = ok ? g[2 * i + j] : nan, uv = u[2 * i + j];
+                const float w = sigmoid(gv);
+                if (MODE == GATE) {
+                  r0[j] = gv * w * uv;
+                } else {
+                  const float e = (j ? dv.y : dv.x) * up;
+                  r0[j] = e * uv * (w * fmaf(gv, 1.0f - w, 1.0f));
+                  r1[j] = e * gv * w;
+                }
+              }
+              o[i] = pack2<BF16>(r0[0], r0[1]);
+              if (MODE == GATE_BWD) du[h][i] = pack2<BF16>(r1[0], r1[1]);
+            }
+            put8(own + h * 32, o);  // where this half's dy was
           }
+          put_rows(stage, lane, static_cast<char*>(P.out[0]) + at, P.ldo * 2, rows, cols * 2, vec);
+          if (MODE == GATE_BWD) {
+            put8(own, du[0]);
+            put8(own + 32, du[1]);
+            put_rows(stage, lane, static_cast<char*>(P.out[1]) + at, P.ldo * 2, rows, cols * 2, vec);
+          }
+        } else {
+          void* to = T.half ? P.out[1] : P.out[0];
+          if (!to) continue;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float v[16];
+            tmem_load16(d + c + h * 16, v);
+            tmem_load_wait();
+            if (!ok) v[0] = v[1] = v[2] = v[3] = v[4] = v[5] = v[6] = v[7] = v[8] = v[9] = v[10] = v[11] = v[12] = v[13] = v[14] = v[15] = nan;
+            if (P.splits > 1) {
+              if (h * 16 >= cols) continue;
+              put8(own, reinterpret_cast<uint32_t*>(v));
+              put8(own + 32, reinterpret_cast<uint32_t*>(v) + 8);
+              char* out = reinterpret_cast<char*>(P.part) +
+                          ((((int64_t)T.split * P.halves_m + T.half) * P.m + row0) * P.n + col + h * 16) * 4;
+              put_rows(stage, lane, out, (int64_t)P.n * 4, rows, min(cols - h * 16, 16) * 4, vec);
+            } else {
+              uint32_t o[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) o[i] = pack2<BF16>(v[2 * i] * down, v[2 * i + 1] * down);
+              put8(own + h * 32, o);
+            }
+          }
+          if (P.splits == 1)
+            put_rows(stage, lane, static_cast<char*>(to) + (row0 * P.ldo + col) * 2, P.ldo * 2, rows, cols * 2, vec);
         }
       }
       fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&acc_empty[n & 1]);
+      if (lane == 0) mbar_arrive_cluster(release);
     }
   }
   fence_before();
   __syncthreads();
+  cluster_sync();  // nothing of the pair is on its way to a CTA that has left
   fence_after();
-  if (warp == EPI_WARPS) tmem_free<2 * BN>(tmem);
+  if (warp == EPI_WARPS) tmem_free_pair<2 * BN>(tmem);
 }
 
 // Sums of the k ranges, in their order: element i of half h is out[h][i].
@@ -393,9 +409,6 @@ __device__ __forceinline__ float peer_float(uint32_t addr, uint32_t rank) {
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
   return v;
 }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 
 template <bool BF16, int NR>
 __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(const __grid_constant__ Maps maps, const FewArgs P) {
@@ -406,8 +419,8 @@ __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(const __grid_cons
   __shared__ volatile uint32_t gave_up;
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  uint32_t rank, ranks;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  const uint32_t rank = cluster_rank();
+  uint32_t ranks;
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
   const int f0 = blockIdx.x / ranks * HALF_ROWS;
   const int k0 = rank * P.kper, k1 = min(k0 + P.kper, P.kb);
@@ -465,16 +478,11 @@ __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(const __grid_cons
     const int row = warp * 32 + lane;
 #pragma unroll
     for (int c = 0; c < NR; c += 16) {
-      uint32_t r[16];
-      asm volatile(
-          "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-          : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-            "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-          : "r"(tmem + ((uint32_t)(warp * 32) << 16) + c));
+      float v[16];
+      tmem_load16(tmem + ((uint32_t)(warp * 32) << 16) + c, v);
       tmem_load_wait();
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        sums[row * (NR + 1) + c + i] = ok && !gave_up ? __uint_as_float(r[i]) : __int_as_float(0x7fffffff);
+      for (int i = 0; i < 16; ++i) sums[row * (NR + 1) + c + i] = ok && !gave_up ? v[i] : __int_as_float(0x7fffffff);
     }
     fence_before();
   }
@@ -505,20 +513,20 @@ __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(const __grid_cons
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to; }
 
 // How a product of m x n over k blocks is cut up: into tiles 256 or 128 columns wide, whichever takes less time when
-// SMS of them run at a time.  A k block of a wide tile counts 1 and of a narrow one 0.56 (measured: it reads more for
-// each product), what a tile costs besides 4 and 2.  Where tiles leave more than half of the SMs idle, k is cut into
-// ranges of at least 4 blocks, whose sums a second kernel adds.
+// PAIRS of them run at a time.  A k block of a wide tile counts 1 and of a narrow one 0.7 (it moves 24 KB an SM for half
+// the products of 32 KB), what a tile costs besides 4 and 2.  Where tiles leave more than half of the SMs idle, k is cut
+// into ranges of at least 4 blocks, whose sums a second kernel adds.
 struct Plan {
   int bn, mt, nt, splits, kper;
   Plan(int64_t m, int64_t n, int64_t blocks, int halves, bool gate) {
-    mt = (int)up(m, BM);
+    mt = (int)up(m, 2 * BM);
     const int64_t wide = mt * up(n, gate ? 128 : 256) * halves, narrow = mt * up(n, gate ? 64 : 128) * halves;
-    bn = up(wide, SMS) * (blocks + 4.0) <= up(narrow, SMS) * (0.56 * blocks + 2.0) ? 256 : 128;
+    bn = up(wide, PAIRS) * (blocks + 4.0) <= up(narrow, PAIRS) * (0.7 * blocks + 2.0) ? 256 : 128;
     nt = (int)up(n, gate ? bn / 2 : bn);
     splits = 1;
     const int64_t tiles = (int64_t)mt * nt * halves;
-    if (!gate && tiles * 2 <= SMS) {
-      int64_t s = SMS / tiles;
+    if (!gate && tiles * 2 <= PAIRS) {
+      int64_t s = PAIRS / tiles;
       s = s < blocks / 4 ? s : blocks / 4;
       splits = s > 1 ? (int)s : 1;
     }
@@ -555,7 +563,8 @@ template <Mode MODE, bool BF16, int BN>
 int run_mm(const Maps& maps, const Args& P, cudaStream_t st, const char* who) {
   if (cudaError_t e = allow_smem(mm_kernel<MODE, BF16, BN>, smem_bytes(BN))) return set_cuda_error(e, who);
   const int64_t tiles = (int64_t)P.mt * P.nt * P.halves_m * P.splits;
-  const unsigned grid = (unsigned)(tiles < sm_count() ? tiles : sm_count());
+  const int64_t pairs = sm_count() / 2;
+  const unsigned grid = 2 * (unsigned)(tiles < pairs ? tiles : pairs);
   mm_kernel<MODE, BF16, BN><<<grid, THREADS, smem_bytes(BN), st>>>(maps, P);
   return check_launch(who);
 }
@@ -608,7 +617,7 @@ int forward(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void*
   FewArgs P = {(int)R, (int)F, (int)up(C, BK), 0, y};
   // two CTAs fit on an SM: ranges of C (at least 4 blocks each) until there are as many
   int ranks = 1;
-  while (ranks < 8 && up(F, HALF_ROWS) * ranks * 2 <= 2 * SMS && P.kb >= ranks * 2 * 4) ranks *= 2;
+  while (ranks < 8 && up(F, HALF_ROWS) * ranks * 2 <= 4 * PAIRS && P.kb >= ranks * 2 * 4) ranks *= 2;
   P.kper = (int)up(P.kb, ranks);
   return nr == 16 ? run_few<BF16, 16>(maps, P, ranks, st, who)
                   : nr == 32 ? run_few<BF16, 32>(maps, P, ranks, st, who) : run_few<BF16, 64>(maps, P, ranks, st, who);
@@ -637,7 +646,7 @@ int backward(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void
   if (!BF16) {
     amax = reinterpret_cast<uint32_t*>(base + s.amax);
     if (cudaError_t e = cudaMemsetAsync(amax, 0, 4, st)) return set_cuda_error(e, who);
-    amax_kernel<<<(unsigned)(R < 8 * SMS ? R : 8 * SMS), 256, 0, st>>>(static_cast<const __half*>(dy), ldy, R, F, amax);
+    amax_kernel<<<(unsigned)(R < 16 * PAIRS ? R : 16 * PAIRS), 256, 0, st>>>(static_cast<const __half*>(dy), ldy, R, F, amax);
   }
   if (int rc = run_gate<BF16>(x, ldx, wg, ldg, wu, ldu, dy, ldy, dg, du, s.ld, amax, R, C, F, st, who)) return rc;
   if (dx) {
