@@ -171,7 +171,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   __shared__ uint32_t tmem_slot;
   __shared__ volatile uint32_t gave_up;
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = (int)cluster_rank();
   const int tiles = P.mt * P.nt * P.halves_m * P.splits, first = blockIdx.x / 2, step = gridDim.x / 2;
 
@@ -189,17 +189,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   fence_after();
   const uint32_t tmem = tmem_slot;
 
-  if (warp == EPI_WARPS) {
-    if (lane == 0) {  // TMA
-      int it = 0;
-      bool ok = true;
-      for (int t = first; t < tiles && ok; t += step) {
-        const Tile T(P, t);
-        const int k0 = T.split * P.kper, k1 = min(k0 + P.kper, P.kb * P.halves_k);
-        const int m = (T.m * 2 + rank) * BM;
-        for (int k = k0; k < k1; ++k, ++it) {
-          const int s = it % ST;
-          if (!(ok = mbar_wait<true>(&empty[s], (it / ST + 1) & 1, &gave_up))) break;
+  if (warp == EPI_WARPS) {  // TMA
+    int s = 0, it = 0;
+    uint32_t parity = 1;
+    bool ok = true;
+    for (int t = first; t < tiles && ok; t += step) {
+      const Tile T(P, t);
+      const int k0 = T.split * P.kper, k1 = min(k0 + P.kper, P.kb * P.halves_k);
+      const int m = (T.m * 2 + rank) * BM;
+      for (int k = k0; k < k1; ++k, ++it) {
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], parity, &gave_up)))) break;
+        if (elect_one()) {
           if (rank == 0) mbar_expect(&full[s], 2 * SB);
           const uint32_t bar = peer_addr(&full[s], 0);
           char* a = smem + s * SB;
@@ -221,39 +221,47 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
               tma_load_pair(b + j * 8192, &maps.b[0], T.n * BN + rank * FN + j * 64, k * BK, bar);
           }
         }
+        __syncwarp();
+        if (++s == ST) s = 0, parity ^= 1;
       }
-      if (ok) {  // the pair's last commits arrive before this CTA leaves
-        for (int j = it > ST ? it - ST : 0; j < it; ++j) mbar_wait<true>(&empty[j % ST], (j / ST) & 1, &gave_up);
-      } else if (rank == 0)  // copies in flight end before the shared memory does (CTA 0's barriers count both CTAs')
-        for (int j = it > ST ? it - ST : 0; j < it; ++j)
-          for (uint32_t i = 0; i < POLLS && !mbar_try(&full[j % ST], (j / ST) & 1); ++i) {}
+    }
+    if (ok) {  // the pair's last commits arrive before this CTA leaves
+      for (int j = it > ST ? it - ST : 0; j < it; ++j) mbar_wait(&empty[j % ST], (j / ST) & 1, &gave_up);
+    } else if (rank == 0) {  // copies in flight end before the shared memory does (CTA 0's barriers count both CTAs')
+      for (int j = it > ST ? it - ST : 0; j < it; ++j)
+        for (uint32_t i = 0; i < POLLS && !mbar_try(&full[j % ST], (j / ST) & 1); ++i) {}
     }
   } else if (warp == EPI_WARPS + 1) {
-    if (lane == 0 && rank == 0) {  // MMA
+    if (rank == 0) {  // MMA
       constexpr uint32_t IDESC = instruction(BF16, A_MN, B_MN, 2 * BM, BN);
-      int it = 0, n = 0;
+      const uint64_t desc0 = operand(smem_addr(smem), 8192);
+      int s = 0, n = 0;
+      uint32_t parity = 0;
       bool ok = true;
       for (int t = first; t < tiles && ok; t += step, ++n) {
         const Tile T(P, t);
         const int k0 = T.split * P.kper, k1 = min(k0 + P.kper, P.kb * P.halves_k);
         const uint32_t d = tmem + (n & 1) * BN;
-        if (!(ok = mbar_wait<true>(&acc_empty[n & 1], ((n >> 1) + 1) & 1, &gave_up))) break;
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[n & 1], ((n >> 1) + 1) & 1, &gave_up)))) break;
         fence_after();
-        for (int k = k0; k < k1; ++k, ++it) {
-          const int s = it % ST;
-          if (!(ok = mbar_wait<true>(&full[s], (it / ST) & 1, &gave_up))) break;
+        for (int k = k0; k < k1; ++k) {
+          if (!(ok = __all_sync(0xffffffffu, mbar_wait(&full[s], parity, &gave_up)))) break;
           fence_after();
-          const uint32_t a = smem_addr(smem + s * SB), b = a + BM * BK * 2;
-          const uint64_t ad = operand(a, 8192), bd = operand(b, 8192);
+          if (elect_one()) {
+            const uint64_t ad = desc0 + (uint32_t)(s * SB >> 4), bd = ad + (BM * BK * 2 >> 4);
 #pragma unroll
-          for (int j = 0; j < BK / 16; ++j)
-            mma_pair(d, ad + j * (A_MN ? 2048 >> 4 : 32 >> 4), bd + j * (B_MN ? 2048 >> 4 : 32 >> 4), IDESC, k > k0 || j > 0);
-          mma_commit_pair(&empty[s]);
+            for (int j = 0; j < BK / 16; ++j)
+              mma_pair(d, ad + j * (A_MN ? 2048 >> 4 : 32 >> 4), bd + j * (B_MN ? 2048 >> 4 : 32 >> 4), IDESC, k > k0 || j > 0);
+            mma_commit_pair(&empty[s]);
+            if (k == k1 - 1) mma_commit_pair(&acc_full[n & 1]);
+          }
+          __syncwarp();
+          if (++s == ST) s = 0, parity ^= 1;
         }
-        if (ok) mma_commit_pair(&acc_full[n & 1]);
       }
       if (!ok) {
-        mma_commit_pair(&drained);
+        if (elect_one()) mma_commit_pair(&drained);
+        __syncwarp();
         for (uint32_t i = 0; i < POLLS && !mbar_try(&drained, 0); ++i) {}
       }
     }
@@ -418,7 +426,7 @@ __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(const __grid_cons
   __shared__ uint32_t tmem_slot;
   __shared__ volatile uint32_t gave_up;
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   uint32_t ranks;
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
@@ -440,36 +448,39 @@ __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(const __grid_cons
 
   bool ok = true;
   if (warp == 4) {
-    if (lane == 0) {
-      int k = k0;
-      for (; k < k1; ++k) {
-        const int it = k - k0, s = it % ST;
-        if (!mbar_wait(&empty[s], (it / ST + 1) & 1, &gave_up)) break;
+    int k = k0;
+    for (; k < k1; ++k) {
+      const int it = k - k0, s = it % ST;
+      if (!__all_sync(0xffffffffu, mbar_wait(&empty[s], (it / ST + 1) & 1, &gave_up))) break;
+      if (elect_one()) {
         mbar_expect(&full[s], SB);
         char* a = smem + s * SB;
         tma_load(a, &maps.a[0], k * BK, f0, &full[s]);
         tma_load(a + HALF_ROWS * BK * 2, &maps.a[1], k * BK, f0, &full[s]);
         tma_load(a + 2 * HALF_ROWS * BK * 2, &maps.b[0], k * BK, 0, &full[s]);
       }
-      if (k < k1)
-        for (int j = max(0, k - k0 - ST); j < k - k0; ++j)
-          for (uint32_t i = 0; i < POLLS && !mbar_try(&full[j % ST], (j / ST) & 1); ++i) {}
+      __syncwarp();
     }
+    if (k < k1)
+      for (int j = max(0, k - k0 - ST); j < k - k0; ++j)
+        for (uint32_t i = 0; i < POLLS && !mbar_try(&full[j % ST], (j / ST) & 1); ++i) {}
   } else if (warp == 5) {
-    if (lane == 0) {
-      constexpr uint32_t IDESC = instruction(BF16, false, false, 128, NR);
-      for (int k = k0; k < k1; ++k) {
-        const int it = k - k0, s = it % ST;
-        if (!mbar_wait(&full[s], (it / ST) & 1, &gave_up)) break;
-        fence_after();
-        const uint32_t a = smem_addr(smem + s * SB);
-        const uint64_t ad = operand(a, 0), bd = operand(a + 2 * HALF_ROWS * BK * 2, 0);
+    constexpr uint32_t IDESC = instruction(BF16, false, false, 128, NR);
+    const uint64_t desc0 = operand(smem_addr(smem), 0);
+    for (int k = k0; k < k1; ++k) {
+      const int it = k - k0, s = it % ST;
+      if (!__all_sync(0xffffffffu, mbar_wait(&full[s], (it / ST) & 1, &gave_up))) break;
+      fence_after();
+      if (elect_one()) {
+        const uint64_t ad = desc0 + (uint32_t)(s * SB >> 4), bd = ad + (2 * HALF_ROWS * BK * 2 >> 4);
 #pragma unroll
         for (int j = 0; j < BK / 16; ++j) mma(tmem, ad + j * 2, bd + j * 2, IDESC, k > k0 || j > 0);
         mma_commit(&empty[s]);
       }
-      mma_commit(&done);
+      __syncwarp();
     }
+    if (elect_one()) mma_commit(&done);
+    __syncwarp();
   } else {
     // `done` counts the products issued: complete, unless a wait gave up
     ok = mbar_wait(&done, 0, &gave_up);
@@ -514,14 +525,14 @@ int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to; }
 
 // How a product of m x n over k blocks is cut up: into tiles 256 or 128 columns wide, whichever takes less time when
 // PAIRS of them run at a time.  A k block of a wide tile counts 1 and of a narrow one 0.7 (it moves 24 KB an SM for half
-// the products of 32 KB), what a tile costs besides 4 and 2.  Where tiles leave more than half of the SMs idle, k is cut
+// the products of 32 KB), what a tile costs besides 8 and 4.  Where tiles leave more than half of the SMs idle, k is cut
 // into ranges of at least 4 blocks, whose sums a second kernel adds.
 struct Plan {
   int bn, mt, nt, splits, kper;
   Plan(int64_t m, int64_t n, int64_t blocks, int halves, bool gate) {
     mt = (int)up(m, 2 * BM);
     const int64_t wide = mt * up(n, gate ? 128 : 256) * halves, narrow = mt * up(n, gate ? 64 : 128) * halves;
-    bn = up(wide, PAIRS) * (blocks + 4.0) <= up(narrow, PAIRS) * (0.7 * blocks + 2.0) ? 256 : 128;
+    bn = up(wide, PAIRS) * (blocks + 8.0) <= up(narrow, PAIRS) * (0.7 * blocks + 4.0) ? 256 : 128;
     nt = (int)up(n, gate ? bn / 2 : bn);
     splits = 1;
     const int64_t tiles = (int64_t)mt * nt * halves;
