@@ -23,6 +23,7 @@ from . import _lib
 from .ops import _require_cuda
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+MARK = 64  # steps between two kept states of the scan (csn_gated_scan_marks)
 _NAMES = {t: str(t).replace("torch.", "") for t in DTYPES}
 
 # a generation step is one small kernel, so what its call costs on the host is what it costs: the

@@ -3,7 +3,7 @@
 The same CUDA entry points as ``csn_b200.ops``, registered with ``torch.library`` so that
 they are first-class operators: they have a schema, a fake (shape-only) implementation for
 tracing on meta / fake tensors, and autograd through the matching ``*_bwd`` operator.
-Every operator computes in float32 on CUDA tensors and returns float32.
+The rotor operators compute in float32 on CUDA tensors and return float32.
 
     scan_fwd(M, C, h0?, two_sided, reverse) -> X            scan_bwd(...) -> (dM, dC, dh0)
     fused_rotor_scan_fwd(gens, dt, gamma?, S, h0?, basis, two_sided) -> X
@@ -12,6 +12,14 @@ Every operator computes in float32 on CUDA tensors and returns float32.
     cell_fwd(x, prev, W_rec, W_in, gamma_bias, dt) -> next   cell_bwd(...) -> 5 gradients
     ga3_scan_fwd(gens, dt, x, h0?) -> h                      ga3_scan_bwd(...) -> 4 gradients
     rotor_step(gens, dt, gamma?, S, h!, basis, two_sided)    (updates h in place)
+
+The gated recurrent block's operators (csn_b200.gated) take float32, bfloat16 and float16 as given:
+
+    gated_scan_fwd(f, x, h0?, gate?, cu_seqlens?) -> (y, h_last, marks)
+    gated_scan_bwd(f, x, gate?, cu_seqlens?, marks, dy, dh_last) -> (df, dx, dh0, dgate)
+    gated_step(f, x, h!, gate?) -> y                         (updates h in place)
+    silu_gated_linear_fwd(x, w_gate, w_up) -> y              silu_gated_linear_bwd(..., dy) -> 3 gradients
+    dropout_add(x, residual?, cut, rng) -> y                 (cut = 65536 p; its own backward)
 
 Optional gradients that do not exist (no h0, undamped) come back as empty tensors.
 The sequence-parallel scan takes a process group and stays a Python entry point
@@ -24,7 +32,7 @@ from typing import Optional, Tuple
 import torch
 from torch import Tensor
 
-from . import ops
+from . import gated, ops
 from .ops import _f32, _require_cuda
 
 _EMPTY = lambda ref: ref.new_empty((0,), dtype=torch.float32)
@@ -251,6 +259,121 @@ def rotor_step(gens: Tensor, dt: Tensor, gamma: Optional[Tensor], S: Tensor, h: 
 @rotor_step.register_fake
 def _(gens, dt, gamma, S, h, basis, two_sided):
     return None
+
+
+# ------------------------------------------------------- gated recurrent block
+@torch.library.custom_op("csn::gated_scan_fwd", mutates_args=())
+def gated_scan_fwd(f: Tensor, x: Tensor, h0: Optional[Tensor], gate: Optional[Tensor],
+                   cu_seqlens: Optional[Tensor]) -> Tuple[Tensor, Tensor, Tensor]:
+    gated._check_scan(f, x, h0, gate, cu_seqlens)
+    return gated._gated_scan_fwd(f, x, None if h0 is None else h0.float(), gate, cu_seqlens, True)
+
+
+@gated_scan_fwd.register_fake
+def _(f, x, h0, gate, cu_seqlens):
+    S, T, C = gated._scan_sizes(f, cu_seqlens)
+    rows = T if cu_seqlens is not None else S * T
+    n = (rows // gated.MARK + S) * C if S > 0 else 0
+    return (f.new_empty(f.shape), f.new_empty((S, C), dtype=torch.float32), f.new_empty((n,), dtype=torch.float32))
+
+
+@torch.library.custom_op("csn::gated_scan_bwd", mutates_args=())
+def gated_scan_bwd(f: Tensor, x: Tensor, gate: Optional[Tensor], cu_seqlens: Optional[Tensor], marks: Tensor,
+                   dy: Tensor, dh_last: Tensor) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    df, dx, dh0, dgate = gated._gated_scan_bwd(f, x, gate, cu_seqlens, marks, dy, dh_last, (True,) * 4)
+    return df, dx, dh0, (dgate if dgate is not None else f.new_empty((0,)))
+
+
+@gated_scan_bwd.register_fake
+def _(f, x, gate, cu_seqlens, marks, dy, dh_last):
+    S, _, C = gated._scan_sizes(f, cu_seqlens)
+    return (f.new_empty(f.shape), f.new_empty(f.shape), f.new_empty((S, C), dtype=torch.float32),
+            f.new_empty(f.shape) if gate is not None else f.new_empty((0,)))
+
+
+def _gated_scan_setup(ctx, inputs, output):
+    f, x, h0, gate, cu = inputs
+    ctx.save_for_backward(f, x, gate, cu, output[2])
+    ctx.h0_dtype = None if h0 is None else h0.dtype
+    ctx.set_materialize_grads(True)
+
+
+def _gated_scan_backward(ctx, dy, dh_last, dmarks):
+    f, x, gate, cu, marks = ctx.saved_tensors
+    df, dx, dh0, dgate = torch.ops.csn.gated_scan_bwd(f, x, gate, cu, marks, dy, dh_last)
+    return (df, dx, None if ctx.h0_dtype is None else dh0.to(ctx.h0_dtype), None if gate is None else dgate, None)
+
+
+gated_scan_fwd.register_autograd(_gated_scan_backward, setup_context=_gated_scan_setup)
+
+
+@torch.library.custom_op("csn::gated_step", mutates_args=("h",))
+def gated_step(f: Tensor, x: Tensor, h: Tensor, gate: Optional[Tensor]) -> Tensor:
+    return gated.gated_step(f.detach(), x.detach(), h, gate=None if gate is None else gate.detach())
+
+
+@gated_step.register_fake
+def _(f, x, h, gate):
+    return f.new_empty(f.shape)
+
+
+@torch.library.custom_op("csn::silu_gated_linear_fwd", mutates_args=())
+def silu_gated_linear_fwd(x: Tensor, w_gate: Tensor, w_up: Tensor) -> Tensor:
+    with torch.no_grad():
+        return gated.silu_gated_linear(x, w_gate, w_up)
+
+
+@silu_gated_linear_fwd.register_fake
+def _(x, w_gate, w_up):
+    return x.new_empty((*x.shape[:-1], w_gate.shape[0]))
+
+
+@torch.library.custom_op("csn::silu_gated_linear_bwd", mutates_args=())
+def silu_gated_linear_bwd(x: Tensor, w_gate: Tensor, w_up: Tensor, dy: Tensor) -> Tuple[Tensor, Tensor, Tensor]:
+    rows = lambda t: t.reshape(-1, t.shape[-1]) if t.shape[-1] else t.reshape(t.shape[:-1].numel(), 0)  # noqa: E731
+    dx, dwg, dwu = gated._silu_gated_linear_bwd(rows(x), w_gate, w_up, rows(dy), (True,) * 3)
+    return dx.view(x.shape), dwg, dwu
+
+
+@silu_gated_linear_bwd.register_fake
+def _(x, w_gate, w_up, dy):
+    return x.new_empty(x.shape), w_gate.new_empty(w_gate.shape), w_up.new_empty(w_up.shape)
+
+
+def _silu_gated_linear_setup(ctx, inputs, output):
+    ctx.save_for_backward(*inputs)
+
+
+def _silu_gated_linear_backward(ctx, dy):
+    return torch.ops.csn.silu_gated_linear_bwd(*ctx.saved_tensors, dy)
+
+
+silu_gated_linear_fwd.register_autograd(_silu_gated_linear_backward, setup_context=_silu_gated_linear_setup)
+
+
+@torch.library.custom_op("csn::dropout_add", mutates_args=())
+def dropout_add(x: Tensor, residual: Optional[Tensor], cut: int, rng: Tensor) -> Tensor:
+    with torch.no_grad():
+        return gated.dropout_add(x, residual, cut / 65536, rng)
+
+
+@dropout_add.register_fake
+def _(x, residual, cut, rng):
+    return x.new_empty(x.shape)
+
+
+def _dropout_setup(ctx, inputs, output):
+    x, residual, ctx.cut, rng = inputs
+    ctx.save_for_backward(rng)
+    ctx.has_residual = residual is not None
+
+
+def _dropout_backward(ctx, dy):
+    (rng,) = ctx.saved_tensors
+    return torch.ops.csn.dropout_add(dy, None, ctx.cut, rng), (dy if ctx.has_residual else None), None, None
+
+
+dropout_add.register_autograd(_dropout_backward, setup_context=_dropout_setup)
 
 
 # ------------------------------------------------------- sequence-parallel scan

@@ -1,5 +1,8 @@
-"""nn.Module front ends of the block kernels, parameter-compatible with torch.nn."""
+"""nn.Module front ends of the block kernels, parameter-compatible with torch.nn, and the gated
+recurrent block."""
 from __future__ import annotations
+
+from typing import Optional
 
 import torch
 import torch.nn as nn
@@ -50,3 +53,105 @@ def generator_inputs(x: torch.Tensor, biv_proj: nn.Linear, gamma_proj: nn.Linear
     b = torch.cat([biv_proj.bias, gamma_proj.bias, time_proj.bias], 0)
     raw = ops.linear(x, W, b)
     return ops.projection_epilogue(raw, omega_scale, dt_base, N, K, HT)
+
+
+# ------------------------------------------------------------- gated recurrent block
+class DropoutAdd(nn.Module):
+    """residual + dropout(x, p) in training, residual + x otherwise (residual None: without it), by
+    ops.dropout_add.  The buffer ``rng`` holds (seed, number of calls made): every call in training
+    draws with a copy of it and counts it up on the device, so each call of a captured training step
+    draws a new mask at every replay, the backward pass finds the numbers of its own call, and a saved
+    state_dict goes on where it stopped.  Drawn from torch's CPU generator, the seed follows
+    torch.manual_seed.  A forward pass that is run again (activation checkpointing) draws again."""
+
+    def __init__(self, p: float = 0.1):
+        super().__init__()
+        if not 0.0 <= p <= 1.0:
+            raise ValueError(f"DropoutAdd: 0 <= p <= 1 expected, got {p}")
+        self.p = p
+        self.register_buffer("rng", torch.stack([torch.randint(0, 1 << 62, ()), torch.zeros((), dtype=torch.int64)]))
+
+    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+        if not self.training or self.p == 0.0:
+            return x if residual is None else residual + x
+        numbers = self.rng.clone()
+        self.rng[1:].add_(1)
+        return ops.dropout_add(x, residual, self.p, numbers)
+
+
+class GatedRecurrence(nn.Module):
+    """The mixer of a gated recurrent block: one projection of x gives forget logits, inputs and output
+    gates, ops.gated_scan runs the recurrence over them as they lie, and a projection goes back.  The
+    channels' forget biases spread their memory from 2 steps to about 1000."""
+
+    def __init__(self, d_model: int, d_inner: Optional[int] = None):
+        super().__init__()
+        self.d_inner = d_model if d_inner is None else d_inner
+        self.in_proj = nn.Linear(d_model, 3 * self.d_inner)
+        self.out_proj = nn.Linear(self.d_inner, d_model)
+        with torch.no_grad():
+            self.in_proj.bias[:self.d_inner] = torch.linspace(0.0, 7.0, self.d_inner)
+
+    def init_state(self, batch_size: int, device=None) -> torch.Tensor:
+        device = device if device is not None else self.in_proj.weight.device
+        return torch.zeros(batch_size, self.d_inner, device=device)
+
+    def forward(self, x: torch.Tensor, h0: Optional[torch.Tensor] = None, cu_seqlens: Optional[torch.Tensor] = None):
+        """x [B, T, d_model], or [L, d_model] packed with cu_seqlens -> (out, float32 states [B, d_inner])."""
+        f, v, gate = ops.linear(x, self.in_proj.weight, self.in_proj.bias).split(self.d_inner, -1)
+        y, h = ops.gated_scan(f, v, h0=h0, gate=gate, cu_seqlens=cu_seqlens)
+        return ops.linear(y, self.out_proj.weight, self.out_proj.bias), h
+
+    @torch.no_grad()
+    def step(self, x_t: torch.Tensor, h: torch.Tensor) -> torch.Tensor:
+        """One token for each stream: x_t [B, d_model]; the state h [B, d_inner] is advanced in place."""
+        f, v, gate = self.in_proj(x_t).split(self.d_inner, -1)
+        return self.out_proj(ops.gated_step(f, v, h, gate=gate))
+
+
+class GatedFeedForward(nn.Module):
+    """w_down(silu(w_gate x) * w_up x) with the parameters of GeometricGatedLinearUnit
+    (python/clifford_model.py:29-43): 16-bit layers by ops.silu_gated_linear, float32 ones as that
+    module computes them."""
+
+    def __init__(self, d_model: int, d_ffn: Optional[int] = None):
+        super().__init__()
+        d_ffn = 2 * d_model if d_ffn is None else d_ffn
+        self.w_gate = nn.Linear(d_model, d_ffn, bias=False)
+        self.w_up = nn.Linear(d_model, d_ffn, bias=False)
+        self.w_down = nn.Linear(d_ffn, d_model, bias=False)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.dtype == torch.float32:
+            y = ops.silu_gate(ops.linear(x, torch.cat([self.w_gate.weight, self.w_up.weight], 0)))
+        else:
+            y = ops.silu_gated_linear(x, self.w_gate.weight, self.w_up.weight)
+        return ops.linear(y, self.w_down.weight)
+
+
+class GatedRecurrentBlock(nn.Module):
+    """x + drop(mixer(ln_1(x))), then + drop(ffn(ln_2(.))): the channelwise recurrence and the gated
+    feed-forward product as a residual block, trained with forward() and advanced one token at a time
+    with step()."""
+
+    def __init__(self, d_model: int, d_inner: Optional[int] = None, d_ffn: Optional[int] = None, dropout: float = 0.0):
+        super().__init__()
+        self.ln_1, self.ln_2 = LayerNorm(d_model), LayerNorm(d_model)
+        self.mixer = GatedRecurrence(d_model, d_inner)
+        self.ffn = GatedFeedForward(d_model, d_ffn)
+        self.drop_1, self.drop_2 = DropoutAdd(dropout), DropoutAdd(dropout)
+
+    def init_state(self, batch_size: int, device=None) -> torch.Tensor:
+        return self.mixer.init_state(batch_size, device)
+
+    def forward(self, x: torch.Tensor, h0: Optional[torch.Tensor] = None, cu_seqlens: Optional[torch.Tensor] = None):
+        """x [B, T, d_model], or [L, d_model] packed with cu_seqlens -> (out, states after the last steps)."""
+        mixed, h = self.mixer(self.ln_1(x), h0, cu_seqlens)
+        x = self.drop_1(mixed, x)
+        return self.drop_2(self.ffn(self.ln_2(x)), x), h
+
+    @torch.no_grad()
+    def step(self, x_t: torch.Tensor, h: torch.Tensor) -> torch.Tensor:
+        """One token, without dropout: x_t [B, d_model] -> out [B, d_model]; h is advanced in place."""
+        x_t = x_t + self.mixer.step(self.ln_1(x_t), h)
+        return x_t + self.ffn(self.ln_2(x_t))

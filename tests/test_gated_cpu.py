@@ -145,3 +145,60 @@ def test_dropout_refuses(lib):
     refused(lib, drop(x=fake(4)), 1, "misaligned")
     refused(lib, drop(rng=NULL), 1, "missing")
     assert drop(n=0) == 0
+
+
+@pytest.mark.parametrize("name", ["gated_scan_fwd", "gated_scan_bwd", "gated_step", "silu_gated_linear_fwd",
+                                  "silu_gated_linear_bwd", "dropout_add"])
+def test_operator_is_registered(name):
+    import torch
+    import csn_b200.ops  # noqa: F401
+    assert getattr(torch.ops.csn, name).default._schema.name == f"csn::{name}"
+
+
+def test_fake_shapes_on_meta(lib):
+    import torch
+    import csn_b200.ops  # noqa: F401
+    csn = torch.ops.csn
+    m = lambda *s, d=torch.bfloat16: torch.empty(*s, device="meta", dtype=d)  # noqa: E731
+    for f, cu, S in ((m(3, 70, 8), None, 3), (m(300, 8), m(6, d=torch.int32), 5)):
+        y, h, marks = csn.gated_scan_fwd(f, f, None, f, cu)
+        assert y.shape == f.shape and y.dtype == f.dtype and h.shape == (S, 8) and h.dtype == torch.float32
+        rows = f.shape[0] if cu is not None else f.shape[1]
+        assert marks.numel() == lib.csn_gated_scan_marks(S, rows, 8, int(cu is not None))
+        df, dx, dh0, dgate = csn.gated_scan_bwd(f, f, None, cu, marks, f, h)
+        assert df.shape == dx.shape == f.shape and dh0.shape == (S, 8) and dgate.numel() == 0
+    x, w = m(2, 5, 16), m(24, 16)
+    assert csn.silu_gated_linear_fwd(x, w, w).shape == (2, 5, 24)
+    assert [tuple(t.shape) for t in csn.silu_gated_linear_bwd(x, w, w, m(2, 5, 24))] == [(2, 5, 16), (24, 16), (24, 16)]
+    assert csn.dropout_add(x, None, 100, m(2, d=torch.int64)).shape == x.shape
+    assert csn.gated_step(m(4, 8), m(4, 8), m(4, 8, d=torch.float32), None).shape == (4, 8)
+
+
+def test_operators_want_cuda_tensors():
+    import torch
+    from csn_b200 import modules, ops
+    t = torch.zeros(2, 3, 8)
+    for call in (lambda: ops.gated_scan(t, t), lambda: ops.gated_step(t[0], t[0], t[0].clone()),
+                 lambda: ops.silu_gated_linear(t.bfloat16(), t[0].bfloat16(), t[0].bfloat16()),
+                 lambda: ops.dropout_add(t, None, 0.5, torch.zeros(2, dtype=torch.int64))):
+        with pytest.raises(RuntimeError, match="CUDA tensors"):
+            call()
+    with pytest.raises(ValueError):
+        modules.DropoutAdd(1.5)
+
+
+def test_feed_forward_shares_the_gglu_parameters():
+    from csn_b200.modules import GatedFeedForward
+    from python.clifford_model import GeometricGatedLinearUnit
+    a, b = GatedFeedForward(16, 24), GeometricGatedLinearUnit(16, 24)
+    assert {k: v.shape for k, v in a.state_dict().items()} == {k: v.shape for k, v in b.state_dict().items()}
+
+
+def test_dropout_seed_follows_the_generator():
+    import torch
+    from csn_b200.modules import DropoutAdd
+    torch.manual_seed(5)
+    a = DropoutAdd(0.1).rng
+    torch.manual_seed(5)
+    assert torch.equal(a, DropoutAdd(0.1).rng) and int(a[1]) == 0
+    assert not torch.equal(a, DropoutAdd(0.1).rng)
