@@ -4,7 +4,9 @@
 
 Each ``csrc/*.cu`` is compiled to an object in ``csrc/_build/`` (in parallel) and the
 objects are linked into ``csn_b200/libcsn_b200.so`` with the CUDA runtime linked
-statically, so the library depends only on the driver.
+statically, so the library depends only on the driver.  ``csrc/csn_torch.cpp``, the PyTorch binding
+of the gated block's entry points, is then compiled against the installed torch into
+``csn_b200/_gated.so``, which finds the library beside itself.
 
 The build is content-addressed: a SHA-256 over every source, header and the build flags is
 compiled into the library (``csn_version()`` ends in ``src <hash>``) and recorded beside it,
@@ -18,6 +20,7 @@ import hashlib
 import os
 import shutil
 import subprocess
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -25,6 +28,7 @@ ROOT = PKG.parent
 CSRC = ROOT / "csrc"
 OBJ = CSRC / "_build"
 LIB = PKG / "libcsn_b200.so"
+BINDING = PKG / "_gated.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-O2"]
@@ -48,7 +52,7 @@ last_action = None
 
 def source_hash() -> str:
     """SHA-256 (first 16 hex digits) over the build flags and every source and header."""
-    deps = sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h"))
+    deps = sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + sorted(CSRC.glob("*.cpp"))
     deps.append(ROOT.parent / "include" / "csn_b200.h")
     h = hashlib.sha256(" ".join(ARCH + FLAGS).encode())
     for p in deps:
@@ -59,9 +63,26 @@ def source_hash() -> str:
 
 
 def _stale(digest: str) -> bool:
-    if not LIB.exists() or not HASH_FILE.exists():
+    if not LIB.exists() or not BINDING.exists() or not HASH_FILE.exists():
         return True
     return HASH_FILE.read_text().strip() != digest
+
+
+def _build_binding() -> None:
+    from torch.utils import cpp_extension
+    # the compiler that torch's own libstdc++ goes with, and not $CXX: one that links its runtime statically
+    # makes a module whose streams crash beside torch's
+    cxx = next((c for c in ("/usr/bin/g++", shutil.which("g++")) if c and Path(c).exists()), "g++")
+    include = [f"-I{p}" for p in cpp_extension.include_paths(device_type="cuda") + [sysconfig.get_paths()["include"]]]
+    where = cpp_extension.library_paths(device_type="cuda")
+    tmp = BINDING.with_suffix(".so.tmp")
+    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", *include, str(CSRC / "csn_torch.cpp"),
+           "-o", str(tmp), f"-L{PKG}", "-l:libcsn_b200.so", "-Wl,-rpath,$ORIGIN", *[f"-L{p}" for p in where],
+           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{cxx} failed on csn_torch.cpp:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, BINDING)
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
@@ -93,6 +114,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB)
+    _build_binding()
     HASH_FILE.write_text(digest + "\n")
     last_action = "built"
     return LIB

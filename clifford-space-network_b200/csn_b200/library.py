@@ -32,7 +32,7 @@ from typing import Optional, Tuple
 import torch
 from torch import Tensor
 
-from . import gated, ops
+from . import _lib, gated, ops
 from .ops import _f32, _require_cuda
 
 _EMPTY = lambda ref: ref.new_empty((0,), dtype=torch.float32)
@@ -262,31 +262,36 @@ def _(gens, dt, gamma, S, h, basis, two_sided):
 
 
 # ------------------------------------------------------- gated recurrent block
+def _scan_sizes(f, cu):
+    n = f.shape
+    return (n[0], n[1], n[2]) if cu is None else (cu.shape[0] - 1, n[0], n[1])
+
+
 @torch.library.custom_op("csn::gated_scan_fwd", mutates_args=())
 def gated_scan_fwd(f: Tensor, x: Tensor, h0: Optional[Tensor], gate: Optional[Tensor],
                    cu_seqlens: Optional[Tensor]) -> Tuple[Tensor, Tensor, Tensor]:
-    gated._check_scan(f, x, h0, gate, cu_seqlens)
-    return gated._gated_scan_fwd(f, x, None if h0 is None else h0.float(), gate, cu_seqlens, True)
+    ext = gated._ext()
+    ext.gated_scan_check(f, x, h0, gate, cu_seqlens)
+    return ext.gated_scan_forward(f, x, None if h0 is None else h0.float(), gate, cu_seqlens, True)
 
 
 @gated_scan_fwd.register_fake
 def _(f, x, h0, gate, cu_seqlens):
-    S, T, C = gated._scan_sizes(f, cu_seqlens)
-    rows = T if cu_seqlens is not None else S * T
-    n = (rows // gated.MARK + S) * C if S > 0 else 0
+    S, T, C = _scan_sizes(f, cu_seqlens)
+    n = _lib.load().csn_gated_scan_marks(S, T, C, int(cu_seqlens is not None))
     return (f.new_empty(f.shape), f.new_empty((S, C), dtype=torch.float32), f.new_empty((n,), dtype=torch.float32))
 
 
 @torch.library.custom_op("csn::gated_scan_bwd", mutates_args=())
 def gated_scan_bwd(f: Tensor, x: Tensor, gate: Optional[Tensor], cu_seqlens: Optional[Tensor], marks: Tensor,
                    dy: Tensor, dh_last: Tensor) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
-    df, dx, dh0, dgate = gated._gated_scan_bwd(f, x, gate, cu_seqlens, marks, dy, dh_last, (True,) * 4)
+    df, dx, dh0, dgate = gated._ext().gated_scan_backward(f, x, gate, cu_seqlens, marks, dy, dh_last, True)
     return df, dx, dh0, (dgate if dgate is not None else f.new_empty((0,)))
 
 
 @gated_scan_bwd.register_fake
 def _(f, x, gate, cu_seqlens, marks, dy, dh_last):
-    S, _, C = gated._scan_sizes(f, cu_seqlens)
+    S, _, C = _scan_sizes(f, cu_seqlens)
     return (f.new_empty(f.shape), f.new_empty(f.shape), f.new_empty((S, C), dtype=torch.float32),
             f.new_empty(f.shape) if gate is not None else f.new_empty((0,)))
 
@@ -331,7 +336,7 @@ def _(x, w_gate, w_up):
 @torch.library.custom_op("csn::silu_gated_linear_bwd", mutates_args=())
 def silu_gated_linear_bwd(x: Tensor, w_gate: Tensor, w_up: Tensor, dy: Tensor) -> Tuple[Tensor, Tensor, Tensor]:
     rows = lambda t: t.reshape(-1, t.shape[-1]) if t.shape[-1] else t.reshape(t.shape[:-1].numel(), 0)  # noqa: E731
-    dx, dwg, dwu = gated._silu_gated_linear_bwd(rows(x), w_gate, w_up, rows(dy), (True,) * 3)
+    dx, dwg, dwu = gated._ext().silu_gated_linear_backward(rows(x), w_gate, w_up, rows(dy), True, True, True)
     return dx.view(x.shape), dwg, dwu
 
 
