@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(128) join_kernel(const float* __restrict__ par
   void* out = second ? out1 : out0;
   if (!out) return;
   float v = 0.0f;
-#pragma unroll 8
+#pragma unroll 16
   for (int s = 0; s < splits; ++s) v += part[s * stride + i];
   v *= down;
   const int64_t at = second ? i - n : i;
@@ -520,6 +520,50 @@ __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(const __grid_cons
   }
 }
 
+// ---------------------------------------------------------------------- padded copies
+// Rows that do not start on 16 bytes cannot be read by TMA: they are copied to rows that do, all operands in one launch,
+// 16 bytes a thread, in the widest loads that the source allows (N bytes).
+struct PadArgs {
+  const char* src[3];
+  char* dst[3];
+  int64_t end[3];  // 16-byte pieces up to and with this operand
+  int64_t ld[3];   // bytes of a source row
+  int pieces, bytes;  // of a row
+};
+
+template <int N>
+__device__ __forceinline__ void pad_piece(const char* p, int have, uint16_t* v) {
+#pragma unroll
+  for (int i = 0; i < 16; i += N) {
+    if (i + N <= have) {
+      if (N == 8) *reinterpret_cast<uint2*>(v + i / 2) = __ldg(reinterpret_cast<const uint2*>(p + i));
+      else if (N == 4) *reinterpret_cast<uint32_t*>(v + i / 2) = __ldg(reinterpret_cast<const uint32_t*>(p + i));
+      else v[i / 2] = __ldg(reinterpret_cast<const uint16_t*>(p + i));
+    } else {
+      for (int j = i; j < i + N; j += 2) v[j / 2] = j < have ? __ldg(reinterpret_cast<const uint16_t*>(p + j)) : (uint16_t)0;
+    }
+  }
+}
+
+__global__ void __launch_bounds__(256) pad_kernel(const PadArgs P) {
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < P.end[2]; i += (int64_t)gridDim.x * blockDim.x) {
+    const int o = i < P.end[0] ? 0 : i < P.end[1] ? 1 : 2;
+    const char* src = o == 0 ? P.src[0] : o == 1 ? P.src[1] : P.src[2];
+    char* dst = o == 0 ? P.dst[0] : o == 1 ? P.dst[1] : P.dst[2];
+    const int64_t ld = o == 0 ? P.ld[0] : o == 1 ? P.ld[1] : P.ld[2];
+    const int64_t k = i - (o == 0 ? 0 : o == 1 ? P.end[0] : P.end[1]), r = k / P.pieces;
+    const int at = (int)(k - r * P.pieces) * 16, have = min(16, P.bytes - at);
+    const char* p = src + r * ld + at;
+    uint4 v;
+    uint16_t* w = reinterpret_cast<uint16_t*>(&v);
+    const uintptr_t a = reinterpret_cast<uintptr_t>(src) | (uintptr_t)ld;
+    if (a % 8 == 0) pad_piece<8>(p, have, w);
+    else if (a % 4 == 0) pad_piece<4>(p, have, w);
+    else pad_piece<2>(p, have, w);
+    *reinterpret_cast<uint4*>(dst + k * 16) = v;
+  }
+}
+
 // ---------------------------------------------------------------------------- host
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to; }
 
@@ -548,18 +592,26 @@ struct Plan {
 
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// the backward pass's scratch: dg, du [R, ld], the largest |dy|, and the partial sums of split products
+// A pass's scratch: padded copies of the operands that need one (bits of `copies`: x, w_gate, w_up), and for the backward
+// pass dg, du [R, ld], the largest |dy|, and the partial sums of split products.
 struct Scratch {
   int64_t ld;
-  size_t dg, du, amax, part, total;
-  Scratch(int64_t R, int64_t C, int64_t F) {
+  size_t pad[3], dg, du, amax, part, total;
+  Scratch(int64_t R, int64_t C, int64_t F, int copies, bool bwd) {
+    size_t n = 0;
+    for (int i = 0; i < 3; ++i) {
+      pad[i] = n;
+      if (copies >> i & 1) n += align256((size_t)(i ? F : R) * up(C, 8) * 16);
+    }
+    total = n;
     ld = up(F, 8) * 8;
+    if (!bwd) return;
     const Plan px(R, C, 2 * up(F, BK), 1, false), pw(F, C, up(R, BK), 2, false);
     const size_t sx = px.splits > 1 ? (size_t)px.splits * R * C * 4 : 0;
     const size_t sw = pw.splits > 1 ? (size_t)pw.splits * 2 * F * C * 4 : 0;
-    dg = 0;
-    du = align256((size_t)R * ld * 2);
-    amax = 2 * du;
+    dg = n;
+    du = dg + align256((size_t)R * ld * 2);
+    amax = du + align256((size_t)R * ld * 2);
     part = amax + 256;
     total = part + align256(sx > sw ? sx : sw);
   }
@@ -647,9 +699,9 @@ int run_product(const Maps& maps, Args P, int64_t blocks, const Plan& p, float* 
 
 template <bool BF16>
 int backward(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void* wu, int64_t ldu, const void* dy,
-             int64_t ldy, void* dx, void* dwg, void* dwu, int64_t R, int64_t C, int64_t F, void* ws, cudaStream_t st) {
+             int64_t ldy, void* dx, void* dwg, void* dwu, int64_t R, int64_t C, int64_t F, const Scratch& s, void* ws,
+             cudaStream_t st) {
   const char* who = "csn_silu_gated_linear_bwd";
-  const Scratch s(R, C, F);
   char* base = static_cast<char*>(ws);
   void *dg = base + s.dg, *du = base + s.du;
   float* part = reinterpret_cast<float*>(base + s.part);
@@ -685,11 +737,44 @@ int backward(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void
 }
 
 bool al16b(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+bool even(const void* p) { return p && (reinterpret_cast<uintptr_t>(p) & 1) == 0; }
 
-// what TMA reads in place: rows that start on 16 bytes
+// whether TMA reads a matrix in place: its rows start on 16 bytes
 bool tiled(const void* p, int64_t rows, int64_t cols, int64_t ld) {
-  return p && al16b(p) && ld % 8 == 0 && (rows == 1 || ld >= cols) && ld > 0 && ld < ((int64_t)1 << 38);
+  return al16b(p) && ld % 8 == 0 && (rows == 1 || ld >= cols) && ld > 0 && ld < ((int64_t)1 << 38);
 }
+
+// The operands as TMA reads them: themselves, or their copies in the workspace.
+struct Operands {
+  const void* p[3];
+  int64_t ld[3];
+  int copies = 0;
+  Operands(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void* wu, int64_t ldu, int64_t R, int64_t C, int64_t F)
+      : p{x, wg, wu}, ld{ldx, ldg, ldu} {
+    for (int i = 0; i < 3; ++i) {
+      const int64_t rows = i ? F : R;
+      if (rows == 1) ld[i] = up(C, 8) * 8;  // the stride of one row says nothing
+      if (!tiled(p[i], rows, C, ld[i])) copies |= 1 << i;
+    }
+  }
+  int copy(int64_t R, int64_t C, int64_t F, const Scratch& s, void* ws, cudaStream_t st) {
+    if (!copies) return CSN_OK;
+    PadArgs A = {};
+    A.pieces = (int)up(C, 8), A.bytes = (int)C * 2;
+    int64_t n = 0;
+    for (int i = 0; i < 3; ++i) {
+      if (copies >> i & 1) {
+        A.src[i] = static_cast<const char*>(p[i]), A.dst[i] = static_cast<char*>(ws) + s.pad[i], A.ld[i] = ld[i] * 2;
+        n += (i ? F : R) * A.pieces;
+        p[i] = A.dst[i], ld[i] = up(C, 8) * 8;
+      }
+      A.end[i] = n;
+    }
+    const int64_t ctas = up(n, 256);
+    pad_kernel<<<(unsigned)(ctas < 32 * PAIRS ? ctas : 32 * PAIRS), 256, 0, st>>>(A);
+    return check_launch("csn_silu_gated_linear: padded copies");
+  }
+};
 
 int check_ffn(const char* who, int64_t R, int64_t C, int64_t F, int dtype) {
   // tile coordinates and counts are 32-bit
@@ -703,14 +788,19 @@ int check_ffn(const char* who, int64_t R, int64_t C, int64_t F, int dtype) {
 
 using namespace csn;
 
-extern "C" size_t csn_silu_gated_linear_bwd_workspace_bytes(int64_t R, int64_t C, int64_t F) {
+extern "C" int csn_silu_gated_linear_copies(const void* x, int64_t ldx, const void* w_gate, int64_t ld_gate, const void* w_up,
+                                            int64_t ld_up, int64_t R, int64_t C, int64_t F) {
+  return Operands(x, ldx, w_gate, ld_gate, w_up, ld_up, R, C, F).copies;
+}
+
+extern "C" size_t csn_silu_gated_linear_workspace_bytes(int64_t R, int64_t C, int64_t F, int copies, int backward) {
   if (R <= 0 || C <= 0 || F <= 0 || R > (1 << 21) || C > (1 << 21) || F > (1 << 21)) return 0;
-  return Scratch(R, C, F).total;
+  return Scratch(R, C, F, copies, backward != 0).total;
 }
 
 extern "C" int csn_silu_gated_linear_fwd(const void* x, int64_t ldx, const void* w_gate, int64_t ld_gate,
                                          const void* w_up, int64_t ld_up, void* y, int64_t R, int64_t C, int64_t F,
-                                         int dtype, void* stream) {
+                                         int dtype, void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = check_ffn("csn_silu_gated_linear_fwd: needs 0 <= R, C, F <= 2^21 and dtype bfloat16 or float16", R, C, F, dtype))
     return rc;
   if (R == 0 || F == 0) return CSN_OK;
@@ -720,12 +810,16 @@ extern "C" int csn_silu_gated_linear_fwd(const void* x, int64_t ldx, const void*
     const cudaError_t e = cudaMemsetAsync(y, 0, (size_t)R * F * 2, st);
     return e == cudaSuccess ? CSN_OK : set_cuda_error(e, "csn_silu_gated_linear_fwd");
   }
-  if (!tiled(x, R, C, ldx) || !tiled(w_gate, F, C, ld_gate) || !tiled(w_up, F, C, ld_up))
-    return set_error(CSN_ERR_INVALID, "csn_silu_gated_linear_fwd: x, w_gate and w_up need rows that start on 16 bytes "
-                                      "(row strides of at least C that are multiples of 8)");
+  if (!even(x) || !even(w_gate) || !even(w_up))
+    return set_error(CSN_ERR_INVALID, "csn_silu_gated_linear_fwd: x, w_gate and w_up are required, aligned to their type");
+  Operands o(x, ldx, w_gate, ld_gate, w_up, ld_up, R, C, F);
+  const Scratch s(R, C, F, o.copies, false);
+  if (s.total && (!workspace || !al16b(workspace) || workspace_bytes < s.total))
+    return set_error(CSN_ERR_INVALID, "csn_silu_gated_linear_fwd: workspace smaller than csn_silu_gated_linear_workspace_bytes");
   KernelTimer kt("silu_gated_linear_fwd", st);
-  return dtype == CSN_BF16 ? forward<true>(x, ldx, w_gate, ld_gate, w_up, ld_up, y, R, C, F, st)
-                           : forward<false>(x, ldx, w_gate, ld_gate, w_up, ld_up, y, R, C, F, st);
+  if (int rc = o.copy(R, C, F, s, workspace, st)) return rc;
+  return dtype == CSN_BF16 ? forward<true>(o.p[0], o.ld[0], o.p[1], o.ld[1], o.p[2], o.ld[2], y, R, C, F, st)
+                           : forward<false>(o.p[0], o.ld[0], o.p[1], o.ld[1], o.p[2], o.ld[2], y, R, C, F, st);
 }
 
 extern "C" int csn_silu_gated_linear_bwd(const void* x, int64_t ldx, const void* w_gate, int64_t ld_gate,
@@ -743,15 +837,16 @@ extern "C" int csn_silu_gated_linear_bwd(const void* x, int64_t ldx, const void*
         return set_error(CSN_ERR_CUDA, "csn_silu_gated_linear_bwd: cudaMemsetAsync");
     return CSN_OK;
   }
-  if (!dy || (reinterpret_cast<uintptr_t>(dy) & 1) || !al16b(dx) || !al16b(dw_gate) || !al16b(dw_up))
+  if (!even(dy) || !even(x) || !even(w_gate) || !even(w_up) || !al16b(dx) || !al16b(dw_gate) || !al16b(dw_up))
     return set_error(CSN_ERR_INVALID, "csn_silu_gated_linear_bwd: missing or misaligned pointer");
-  if (!tiled(x, R, C, ldx) || !tiled(w_gate, F, C, ld_gate) || !tiled(w_up, F, C, ld_up))
-    return set_error(CSN_ERR_INVALID, "csn_silu_gated_linear_bwd: x, w_gate and w_up need rows that start on 16 bytes "
-                                      "(row strides of at least C that are multiples of 8)");
-  if (!workspace || !al16b(workspace) || workspace_bytes < csn_silu_gated_linear_bwd_workspace_bytes(R, C, F))
-    return set_error(CSN_ERR_INVALID, "csn_silu_gated_linear_bwd: workspace smaller than csn_silu_gated_linear_bwd_workspace_bytes");
+  Operands o(x, ldx, w_gate, ld_gate, w_up, ld_up, R, C, F);
+  const Scratch s(R, C, F, o.copies, true);
+  if (!workspace || !al16b(workspace) || workspace_bytes < s.total)
+    return set_error(CSN_ERR_INVALID, "csn_silu_gated_linear_bwd: workspace smaller than csn_silu_gated_linear_workspace_bytes");
   KernelTimer kt("silu_gated_linear_bwd", st);
-  return dtype == CSN_BF16
-             ? backward<true>(x, ldx, w_gate, ld_gate, w_up, ld_up, dy, ld_dy, dx, dw_gate, dw_up, R, C, F, workspace, st)
-             : backward<false>(x, ldx, w_gate, ld_gate, w_up, ld_up, dy, ld_dy, dx, dw_gate, dw_up, R, C, F, workspace, st);
+  if (int rc = o.copy(R, C, F, s, workspace, st)) return rc;
+  return dtype == CSN_BF16 ? backward<true>(o.p[0], o.ld[0], o.p[1], o.ld[1], o.p[2], o.ld[2], dy, ld_dy, dx, dw_gate, dw_up, R, C,
+                                            F, s, workspace, st)
+                           : backward<false>(o.p[0], o.ld[0], o.p[1], o.ld[1], o.p[2], o.ld[2], dy, ld_dy, dx, dw_gate, dw_up, R,
+                                             C, F, s, workspace, st);
 }

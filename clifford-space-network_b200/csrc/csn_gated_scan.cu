@@ -11,6 +11,8 @@
 // memory; then every warp runs its steps again from the state that enters them.  So the inputs are read once: each
 // warp copies its rows into shared memory with cp.async one pass (MARK steps) ahead of their use.
 //
+// Sequences of at most 32 steps need fewer warps than a CTA has: it then takes 2, 4 or 8 of them.
+//
 // Where there are too few sequences and channels to fill the GPU, sequences are cut into chunks: reduce_kernel composes
 // the map of every chunk that another follows (it reads f and x once more, mostly from L2), and the CTA of a chunk
 // composes those before it into the state that enters it.  All sums, products and states are float32 and in an order
@@ -51,6 +53,7 @@ struct ScanArgs {
   int tiles;
   int chunk;     // steps of a chunk, a multiple of MARK
   int chunks;    // of a sequence, where all have one length
+  int group;     // warps that share a sequence; the others of a CTA have sequences of their own
   bool wide;  // every row starts on 16 bytes and holds multiples of 16
 };
 
@@ -350,11 +353,14 @@ __global__ void __launch_bounds__(WARPS * 32, 3) gated_scan_fwd_kernel(const __g
   extern __shared__ __align__(128) char ring[];  // [2][N][MARK rows]
   __shared__ Map<V> maps[2][WARPS][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Part q(A, blockIdx.x / A.tiles);
+  const int among = warp % A.group, head = warp - among;  // place in the sequence's warps, and the first of them
+  const int64_t unit = (int64_t)(blockIdx.x / A.tiles) * (WARPS / A.group) + head / A.group;
+  const bool spare = A.group < WARPS && unit >= A.S;  // goes through the motions of the last sequence
+  const Part q(A, spare ? A.S - 1 : unit);
   if (q.s < 0) return;
   const int64_t tile = (int64_t)(blockIdx.x % A.tiles) * channels(sizeof(T), ODD), c = tile + lane * V;
-  const int have = (int)max((int64_t)0, min((int64_t)V, min(A.C, tile + channels(sizeof(T), ODD)) - c));
-  int t1 = q.from + warp * STEPS;
+  const int have = spare ? 0 : (int)max((int64_t)0, min((int64_t)V, min(A.C, tile + channels(sizeof(T), ODD)) - c));
+  int t1 = q.from + among * STEPS;
   char* mine = ring + warp * STEPS * ROW;
   Input<T, ODD> f(A.f, A, q, tile, t1), x(A.x, A, q, tile, t1), g(A.g, A, q, tile, t1);
   auto fetch = [&](int half, int n) {
@@ -393,13 +399,20 @@ __global__ void __launch_bounds__(WARPS * 32, 3) gated_scan_fwd_kernel(const __g
     maps[half][warp][lane] = m;
     __syncthreads();
     F h;
+    if (A.group == WARPS) {
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      if (w == warp) h = carry;
-      carry = maps[half][w][lane].of(carry);
+      for (int w = 0; w < WARPS; ++w) {
+        if (w == warp) h = carry;
+        carry = maps[half][w][lane].of(carry);
+      }
+    } else {
+      for (int w = 0; w < A.group; ++w) {
+        if (w == among) h = carry;
+        carry = maps[half][head + w][lane].of(carry);
+      }
     }
     if (A.marks) {
-      if (warp == 0) store_state<V>(mark, h, have);
+      if (among == 0) store_state<V>(mark, h, have);
       mark += A.C;
     }
     auto finish = [&](int l) {
@@ -420,7 +433,7 @@ __global__ void __launch_bounds__(WARPS * 32, 3) gated_scan_fwd_kernel(const __g
         if (l < n) finish(l);
     }
   }
-  if (q.to == q.len && warp == 0 && A.h_last) store_state<V>(A.h_last + q.s * A.C + c, carry, have);
+  if (q.to == q.len && among == 0 && A.h_last) store_state<V>(A.h_last + q.s * A.C + c, carry, have);
   if (A.cu && q.k == 0) clear_outside<T, ODD>(A, q, c, have, A.y);
 }
 
@@ -433,12 +446,15 @@ __global__ void __launch_bounds__(WARPS * 32, 2) gated_scan_bwd_kernel(const __g
   __shared__ Map<V> maps[2][WARPS][32];
   __shared__ F back[2][WARPS][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Part q(A, blockIdx.x / A.tiles);
+  const int among = warp % A.group, head = warp - among;  // place in the sequence's warps, and the first of them
+  const int64_t unit = (int64_t)(blockIdx.x / A.tiles) * (WARPS / A.group) + head / A.group;
+  const bool spare = A.group < WARPS && unit >= A.S;  // goes through the motions of the last sequence
+  const Part q(A, spare ? A.S - 1 : unit);
   if (q.s < 0) return;
   const int64_t tile = (int64_t)(blockIdx.x % A.tiles) * channels(sizeof(T), ODD), c = tile + lane * V;
-  const int have = (int)max((int64_t)0, min((int64_t)V, min(A.C, tile + channels(sizeof(T), ODD)) - c));
+  const int have = spare ? 0 : (int)max((int64_t)0, min((int64_t)V, min(A.C, tile + channels(sizeof(T), ODD)) - c));
   const int last = q.to > q.from ? q.from + (q.to - q.from - 1) / MARK * MARK : q.from - MARK;
-  int t1 = last + warp * STEPS;
+  int t1 = last + among * STEPS;
   char* mine = ring + warp * STEPS * ROW;
   Input<T, ODD> f(A.f, A, q, tile, t1), x(A.x, A, q, tile, t1), d(A.dy, A, q, tile, t1), g(A.g, A, q, tile, t1);
   auto fetch = [&](int half, int n) {
@@ -495,13 +511,21 @@ __global__ void __launch_bounds__(WARPS * 32, 2) gated_scan_bwd_kernel(const __g
     maps[half][warp][lane] = m;
     back[half][warp][lane] = r;
     __syncthreads();
+    if (A.group == WARPS) {
 #pragma unroll
-    for (int k = 0; k < WARPS - 1; ++k)
-      if (k < warp) h = maps[half][k][lane].of(h);
+      for (int k = 0; k < WARPS - 1; ++k)
+        if (k < warp) h = maps[half][k][lane].of(h);
 #pragma unroll
-    for (int k = WARPS - 1; k >= 0; --k) {
-      if (k == warp) r = mu;
-      mu = fma(maps[half][k][lane].p, mu, back[half][k][lane]);
+      for (int k = WARPS - 1; k >= 0; --k) {
+        if (k == warp) r = mu;
+        mu = fma(maps[half][k][lane].p, mu, back[half][k][lane]);
+      }
+    } else {
+      for (int k = head; k < warp; ++k) h = maps[half][k][lane].of(h);
+      for (int k = head + A.group - 1; k >= head; --k) {
+        if (k == warp) r = mu;
+        mu = fma(maps[half][k][lane].p, mu, back[half][k][lane]);
+      }
     }
     // forward over the steps: D_t = h_{t-1} - x_t, and dg is done
     F D[STEPS];
@@ -536,7 +560,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) gated_scan_bwd_kernel(const __g
         if (l < n) finish(l);
     }
   }
-  if (q.k == 0 && warp == 0 && A.dh0) store_state<V>(A.dh0 + q.s * A.C + c, mu, have);
+  if (q.k == 0 && among == 0 && A.dh0) store_state<V>(A.dh0 + q.s * A.C + c, mu, have);
   if (A.cu && q.k == 0) {
     clear_outside<T, ODD>(A, q, c, have, A.df);
     clear_outside<T, ODD>(A, q, c, have, A.dx);
@@ -604,8 +628,8 @@ bool rows_align(const Rows& r, int size, int bytes) {
 // may be anything, are cut at an even share of all rows.  Chunks have 4 passes at least: below that the second
 // reading and its launch cost more than they bring.
 struct Cut {
-  int tiles, chunk, chunks;
-  int64_t units;
+  int tiles, chunk, chunks, group;
+  int64_t units, ctas;  // pieces of work; those of a tile that a CTA takes at a time
   Cut(int64_t S, int64_t T, int64_t C, bool packed, int dtype, bool odd, bool bwd) {
     const int wide = channels(dtype == CSN_F32 ? 4 : 2, odd);
     const int64_t slots = 148 * (bwd ? 2 : 3);
@@ -619,6 +643,8 @@ struct Cut {
     chunks = (int)((T + chunk - 1) / chunk);
     if (chunks == 0) chunks = 1;
     units = packed ? T / chunk + S : S * chunks;
+    group = packed || T > 32 ? WARPS : T > 16 ? 4 : T > 8 ? 2 : 1;
+    ctas = (units * group + WARPS - 1) / WARPS;
   }
   bool split(int64_t T) const { return T > chunk; }
 };
@@ -633,7 +659,7 @@ cudaError_t launch_part(K kernel, int64_t grid, int smem, const ScanArgs& A, cud
 
 template <typename T, bool GATE, bool ODD>
 cudaError_t launch_scan(const ScanArgs& A, bool bwd, const Cut& cut, cudaStream_t st) {
-  const int64_t grid = cut.units * cut.tiles;
+  const int64_t grid = cut.ctas * cut.tiles;
   const int piece = 2 * PIECE;
   if (cut.split(A.T)) {
     const cudaError_t e = bwd ? launch_part(reduce_kernel<T, GATE, ODD, true>, grid, (GATE ? 3 : 2) * piece, A, st)
@@ -657,7 +683,7 @@ int dispatch_scan(ScanArgs A, int dtype, bool bwd, void* workspace, size_t bytes
   A.wide = all(16);
   const bool odd = !all(4);
   const Cut cut(A.S, A.T, A.C, A.cu != nullptr, dtype, odd, bwd);
-  A.tiles = cut.tiles, A.chunk = cut.chunk, A.chunks = cut.chunks, A.maps = static_cast<float2*>(workspace);
+  A.tiles = cut.tiles, A.chunk = cut.chunk, A.chunks = cut.chunks, A.group = cut.group, A.maps = static_cast<float2*>(workspace);
   if (cut.units * cut.tiles > 0x7fffffff) return set_error(CSN_ERR_INVALID, "csn_gated_scan: more than 2^31 - 1 tiles of work");
   if (cut.split(A.T) && (!workspace || !aligned(workspace, 16) || bytes < (size_t)cut.units * A.C * sizeof(float2)))
     return set_error(CSN_ERR_INVALID, "csn_gated_scan: workspace smaller than csn_gated_scan_workspace_bytes");

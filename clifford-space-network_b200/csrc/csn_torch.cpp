@@ -223,39 +223,27 @@ Tensor gated_step(const Tensor& f_, const Tensor& x_, const Tensor& h, const May
 }
 
 // ---------------------------------------------------- gated feed-forward product
-// A 16-bit matrix whose rows start on 16 bytes, and its row stride: t itself where its rows do, otherwise a copy with
-// padded rows.
-std::pair<Tensor, int64_t> tiled(const Tensor& t_) {
-  const Tensor t = rows(t_);
-  const int64_t n = t.size(0), c = t.size(1), wide = (c + 7) / 8 * 8, ld = n > 1 ? t.stride(0) : wide;
-  if (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && ld % 8 == 0 && ld >= c) return {t, ld};
-  Tensor copy = room(t, {n, wide});
-  copy.narrow(1, 0, c).copy_(t);
-  return {copy, wide};
-}
-
 Tensor ffn_forward(const Tensor& x_, const Tensor& wg_, const Tensor& wu_) {
   const c10::cuda::CUDAGuard guard(x_.device());
-  auto [x, ldx] = tiled(x_);
-  auto [wg, ldg] = tiled(wg_);
-  auto [wu, ldu] = tiled(wu_);
-  Tensor y = room(x, {x_.size(0), wg_.size(0)});
-  check("csn_silu_gated_linear_fwd",
-        csn_silu_gated_linear_fwd(ptr(x), ldx, ptr(wg), ldg, ptr(wu), ldu, ptr(y), x_.size(0), x_.size(1), wg_.size(0),
-                                  code_of(x.scalar_type()), stream(x)));
+  const Tensor x = rows(x_), wg = rows(wg_), wu = rows(wu_);
+  const int64_t R = x.size(0), C = x.size(1), F = wg.size(0), ldx = x.stride(0), ldg = wg.stride(0), ldu = wu.stride(0);
+  Tensor y = room(x, {R, F});
+  const size_t nb = csn_silu_gated_linear_workspace_bytes(
+      R, C, F, csn_silu_gated_linear_copies(ptr(x), ldx, ptr(wg), ldg, ptr(wu), ldu, R, C, F), 0);
+  const Tensor ws = bytes(x, nb);
+  check("csn_silu_gated_linear_fwd", csn_silu_gated_linear_fwd(ptr(x), ldx, ptr(wg), ldg, ptr(wu), ldu, ptr(y), R, C, F,
+                                                               code_of(x.scalar_type()), ptr(ws), nb, stream(x)));
   return y;
 }
 
 std::tuple<Tensor, Tensor, Tensor> ffn_backward(const Tensor& x_, const Tensor& wg_, const Tensor& wu_, const Tensor& dy_,
                                                 bool need_x, bool need_g, bool need_u) {
   const c10::cuda::CUDAGuard guard(x_.device());
-  auto [x, ldx] = tiled(x_);
-  auto [wg, ldg] = tiled(wg_);
-  auto [wu, ldu] = tiled(wu_);
-  const Tensor dy = rows(dy_);
-  const int64_t R = x_.size(0), C = x_.size(1), F = wg_.size(0);
+  const Tensor x = rows(x_), wg = rows(wg_), wu = rows(wu_), dy = rows(dy_);
+  const int64_t R = x.size(0), C = x.size(1), F = wg.size(0), ldx = x.stride(0), ldg = wg.stride(0), ldu = wu.stride(0);
   Tensor dx = need_x ? room(x, {R, C}) : Tensor(), dg = need_g ? room(x, {F, C}) : Tensor(), du = need_u ? room(x, {F, C}) : Tensor();
-  const size_t nb = csn_silu_gated_linear_bwd_workspace_bytes(R, C, F);
+  const size_t nb = csn_silu_gated_linear_workspace_bytes(
+      R, C, F, csn_silu_gated_linear_copies(ptr(x), ldx, ptr(wg), ldg, ptr(wu), ldu, R, C, F), 1);
   const Tensor ws = bytes(x, nb);
   check("csn_silu_gated_linear_bwd",
         csn_silu_gated_linear_bwd(ptr(x), ldx, ptr(wg), ldg, ptr(wu), ldu, ptr(dy), dy.stride(0), ptr(dx), ptr(dg), ptr(du), R, C, F,

@@ -442,16 +442,23 @@ int csn_gated_step(const void* f, const void* x, const void* gate, const int64_t
                    void* y, int64_t B, int64_t C, int dtype, void* stream);
 
 /* y = silu(x w_gate^T) * (x w_up^T) in one pass (csn_silu_gate_fwd on the product that feeds it):
- * x [R, C], w_gate, w_up [F, C] with row strides ldx, ld_gate, ld_up (elements: multiples of 8, at
- * least C; pointers 16-byte aligned), y [R, F] contiguous; bfloat16 or float16, sums in float32.
- * The backward forms both products again and writes dx [R, C], dw_gate, dw_up [F, C]
- * (contiguous; each may be NULL) from dy [R, F] (any row stride ld_dy).  Its workspace is
- * required, 16-byte aligned.  R, C, F <= 2^21.  Should a device-side wait give up (it is bounded),
- * the results it concerns are NaN. */
-size_t csn_silu_gated_linear_bwd_workspace_bytes(int64_t R, int64_t C, int64_t F);
+ * x [R, C], w_gate, w_up [F, C] with row strides ldx, ld_gate, ld_up (elements), y [R, F]
+ * contiguous, 16-byte aligned; bfloat16 or float16, sums in float32.  The backward forms both
+ * products again and writes dx [R, C], dw_gate, dw_up [F, C] (contiguous; each may be NULL) from
+ * dy [R, F] (row stride ld_dy).  R, C, F <= 2^21.
+ * Operands whose rows do not start on 16 bytes (base, or row stride not a multiple of 8 elements
+ * or below C) are copied first: csn_silu_gated_linear_copies says which (bits 0, 1, 2 for x,
+ * w_gate, w_up), and the workspace query takes its answer.  The workspace is required where its
+ * size is not 0, 16-byte aligned.  Should a device-side wait give up (it is bounded), the results
+ * it concerns are NaN. */
+int csn_silu_gated_linear_copies(const void* x, int64_t ldx, const void* w_gate, int64_t ld_gate,
+                                 const void* w_up, int64_t ld_up, int64_t R, int64_t C, int64_t F);
+size_t csn_silu_gated_linear_workspace_bytes(int64_t R, int64_t C, int64_t F, int copies,
+                                             int backward);
 int csn_silu_gated_linear_fwd(const void* x, int64_t ldx, const void* w_gate, int64_t ld_gate,
                               const void* w_up, int64_t ld_up, void* y, int64_t R, int64_t C,
-                              int64_t F, int dtype, void* stream);
+                              int64_t F, int dtype, void* workspace, size_t workspace_bytes,
+                              void* stream);
 int csn_silu_gated_linear_bwd(const void* x, int64_t ldx, const void* w_gate, int64_t ld_gate,
                               const void* w_up, int64_t ld_up, const void* dy, int64_t ld_dy,
                               void* dx, void* dw_gate, void* dw_up, int64_t R, int64_t C, int64_t F,

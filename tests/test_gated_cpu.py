@@ -111,18 +111,17 @@ def test_step_refuses(lib):
 def test_ffn_refuses(lib):
     p = fake()
 
-    def fwd(x=p, y=p, R=4, C=8, F=8, ldx=8, dtype=1):
-        return lib.csn_silu_gated_linear_fwd(x, ldx, p, C, p, C, y, R, C, F, dtype, NULL)
+    def fwd(x=p, y=p, R=4, C=8, F=8, ldx=8, dtype=1, ws=NULL, nb=0):
+        return lib.csn_silu_gated_linear_fwd(x, ldx, p, C, p, C, y, R, C, F, dtype, ws, nb, NULL)
 
     refused(lib, fwd(R=-1), 1, "R, C, F")
     refused(lib, fwd(F=2 ** 22), 1, "R, C, F")
     refused(lib, fwd(dtype=0), 2, "dtype")
-    refused(lib, fwd(x=NULL), 1, "16 bytes")
-    refused(lib, fwd(x=fake(8)), 1, "16 bytes")
-    refused(lib, fwd(ldx=12), 1, "16 bytes")
-    refused(lib, fwd(ldx=0), 1, "16 bytes")
-    refused(lib, fwd(C=9, ldx=16), 1, "16 bytes")
+    refused(lib, fwd(x=NULL), 1, "required")
+    refused(lib, fwd(x=fake(1)), 1, "aligned")
     refused(lib, fwd(y=fake(2)), 1, "misaligned")
+    for odd in (dict(x=fake(8)), dict(ldx=12), dict(ldx=0), dict(C=9, ldx=16), dict(R=2, ldx=-8)):
+        refused(lib, fwd(**odd), 1, "workspace")  # a copy is needed, and there is no room for it
     assert fwd(R=0) == 0 and fwd(F=0) == 0
 
     def bwd(dy=p, dx=p, R=4, C=8, F=8, ws=p, nb=1 << 30):
@@ -133,6 +132,19 @@ def test_ffn_refuses(lib):
     refused(lib, bwd(ws=NULL, nb=0), 1, "workspace")
     refused(lib, bwd(nb=8), 1, "workspace")
     refused(lib, bwd(C=-2), 1, "R, C, F")
+
+
+def test_ffn_copies_and_their_room(lib):
+    copies = lambda x=fake(), ldx=64, ldg=64, ldu=64, R=5, C=64, F=7: lib.csn_silu_gated_linear_copies(  # noqa: E731
+        x, ldx, fake(), ldg, fake(), ldu, R, C, F)
+    assert copies() == 0 and copies(ldx=72) == 0 and copies(ldx=68) == 1 and copies(x=fake(2)) == 1
+    assert copies(ldg=65) == 2 and copies(ldu=0) == 4 and copies(C=63, ldx=63, ldg=63, ldu=63) == 7
+    assert copies(R=1, ldx=0) == 0  # the stride of one row says nothing
+    room = lib.csn_silu_gated_linear_workspace_bytes
+    assert room(5, 64, 7, 0, 0) == 0
+    assert room(5, 63, 7, 7, 0) >= (5 + 7 + 7) * 128
+    assert room(5, 63, 7, 7, 1) >= room(5, 63, 7, 7, 0) + 2 * 5 * 16
+    assert room(0, 64, 7, 7, 1) == 0
 
 
 def test_dropout_refuses(lib):

@@ -76,6 +76,16 @@ def test_scan_dense(ops, kind, B, T, C, gated):
     scan_case(ops, f, x, h0, gate, None, kind, dy=dy, dh=dh)
 
 
+@pytest.mark.parametrize("kind", ["bfloat16", "float32"])
+@pytest.mark.parametrize("T", [1, 2, 8, 9, 16, 17, 31, 32, 33])
+def test_scan_of_many_short_sequences(ops, kind, T):
+    """Several sequences to a CTA, and fewer of them than the last CTA has room for."""
+    for B, C in ((13, 66), (1, 33), (64, 64)):
+        f = (make((B, T, C), kind, 1).float() + bias(C)).to(TYPES[kind])
+        scan_case(ops, f, make((B, T, C), kind, 2), make((B, C), "float32", 4), make((B, T, C), kind, 3), None, kind,
+                  dy=make((B, T, C), kind, 5), dh=make((B, C), "float32", 6))
+
+
 @pytest.mark.parametrize("B,T,C", [(1, 5000, 64), (1, 1027, 40), (2, 2048, 128), (1, 4097, 6)])
 def test_scan_long(ops, B, T, C):
     for kind in ("bfloat16", "float32"):
