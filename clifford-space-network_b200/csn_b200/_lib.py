@@ -98,8 +98,8 @@ SIGNATURES = {
     "csn_gated_step": ([_f, _f, _f, _strides, _f, _f, _i64, _i64, _int, _f], _int),
     "csn_silu_gated_linear_copies": ([_f, _i64, _f, _i64, _f, _i64, _i64, _i64, _i64], _int),
     "csn_silu_gated_linear_workspace_bytes": ([_i64, _i64, _i64, _int, _int], _sz),
-    "csn_silu_gated_linear_fwd": ([_f, _i64, _f, _i64, _f, _i64, _f, _i64, _i64, _i64, _int, _f, _sz, _f], _int),
-    "csn_silu_gated_linear_bwd": ([_f, _i64, _f, _i64, _f, _i64, _f, _i64, _f, _f, _f, _i64, _i64, _i64, _int, _f,
+    "csn_silu_gated_linear_fwd": ([_f, _i64, _f, _i64, _f, _i64, _f, _f, _i64, _i64, _i64, _int, _f, _sz, _f], _int),
+    "csn_silu_gated_linear_bwd": ([_f, _i64, _f, _i64, _f, _i64, _f, _i64, _f, _f, _f, _f, _i64, _i64, _i64, _int, _f,
                                    _sz, _f], _int),
     "csn_dropout_add": ([_f, _f, _f, _f, _i64, _int, _int, _f], _int),
     "csn_timing_enable": ([_int], _int),

@@ -65,8 +65,9 @@ def gated_step(f, x, h, gate=None):
 def silu_gated_linear(x, w_gate, w_up):
     """silu(x w_gate^T) * (x w_up^T) in one kernel: x [..., C], w_gate and w_up [F, C], result [..., F]
     (what :func:`silu_gate` makes of the library product of both weights).  bfloat16 or float16 on the
-    tensor cores, sums in float32, one rounding at the end; the backward pass forms both products
-    again instead of keeping them.  float32 layers use ``silu_gate(linear(x, cat))``."""
+    tensor cores, sums in float32, one rounding at the end.  The backward pass forms both products
+    again, or, for C >= 1536, takes them from float32 copies that the forward pass keeps (8 bytes an
+    element of the result until then).  float32 layers use ``silu_gate(linear(x, cat))``."""
     return (_module or _ext()).silu_gated_linear(x, w_gate, w_up)
 
 

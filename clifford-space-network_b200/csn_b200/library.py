@@ -336,7 +336,7 @@ def _(x, w_gate, w_up):
 @torch.library.custom_op("csn::silu_gated_linear_bwd", mutates_args=())
 def silu_gated_linear_bwd(x: Tensor, w_gate: Tensor, w_up: Tensor, dy: Tensor) -> Tuple[Tensor, Tensor, Tensor]:
     rows = lambda t: t.reshape(-1, t.shape[-1]) if t.shape[-1] else t.reshape(t.shape[:-1].numel(), 0)  # noqa: E731
-    dx, dwg, dwu = gated._ext().silu_gated_linear_backward(rows(x), w_gate, w_up, rows(dy), True, True, True)
+    dx, dwg, dwu = gated._ext().silu_gated_linear_backward(rows(x), w_gate, w_up, rows(dy), None, True, True, True)
     return dx.view(x.shape), dwg, dwu
 
 

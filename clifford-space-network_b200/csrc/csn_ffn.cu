@@ -3,8 +3,9 @@
 //   g = x Wg^T,  u = x Wu^T,  y = silu(g) * u          x [R, C], Wg, Wu [F, C], y [R, F]
 // Adjoint, with w = sigmoid(g):
 //   dg = dy u w (1 + g (1 - w)),  du = dy g w,  dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x
-// The backward pass forms g and u again in float32 (they are never stored): keeping them would cost 8 bytes written
-// and read an element in float32, or, rounded to 16 bits, a third of the gradients' precision.
+// The backward pass takes g and u in float32 from what the forward pass kept ([2, R, F]), or forms them again.  Keeping
+// them costs 8 bytes an element written and read, forming them 4 C operations: at 6.5 TB/s and 1.4 PFLOP/s the two are
+// even near C = 1000, and the caller decides (rounded to 16 bits they would cost a third of the gradients' precision).
 // dg and du are rounded to the tensors' own type once, as the operands of the products that follow.  In float16,
 // whose smallest number is 2^-24, they are first scaled by the power of two that brings the largest |dy| into [1, 2),
 // and the products are scaled back in float32.
@@ -63,6 +64,7 @@ struct Args {
   const void* dy;
   int64_t ldy;
   float* part;        // splits > 1: [splits][halves_m][m][n]
+  float* pre;         // GATE: g and u are kept here, [2][m][n]
   const uint32_t* amax;  // float16 backward: bits of the largest |dy|
 };
 
@@ -275,6 +277,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     const uint32_t d = tmem + acc * BN + ((uint32_t)(quarter * 32) << 16), release = peer_addr(&acc_empty[acc], 0);
     const bool vec = (MODE == DX || MODE == DW) && P.splits > 1 ? P.n % 4 == 0 : P.ldo % 8 == 0;
     const bool vec_dy = MODE == GATE_BWD && P.ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(P.dy) & 15) == 0 && P.n % 8 == 0;
+    const bool vec_pre = P.n % 4 == 0;
     uint32_t parity = 0;
     for (int t = first + acc * step; t < tiles; t += 2 * step, parity ^= 1) {
       const Tile T(P, t);
@@ -293,7 +296,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           const int64_t at = (row0 * P.ldo + col) * 2;
           if (MODE == GATE_BWD)
             get_rows(stage, lane, static_cast<const char*>(P.dy) + (row0 * P.ldy + col) * 2, P.ldy * 2, rows, cols * 2, vec_dy);
-          uint32_t du[2][8];
+          uint32_t du[2][8];  // GATE: y
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             float g[16], u[16];
@@ -318,17 +321,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                   r1[j] = e * gv * w;
                 }
               }
-              o[i] = pack2<BF16>(r0[0], r0[1]);
-              if (MODE == GATE_BWD) du[h][i] = pack2<BF16>(r1[0], r1[1]);
+              if (MODE == GATE_BWD) {
+                o[i] = pack2<BF16>(r0[0], r0[1]);
+                du[h][i] = pack2<BF16>(r1[0], r1[1]);
+              } else {
+                du[h][i] = pack2<BF16>(r0[0], r0[1]);
+              }
             }
-            put8(own + h * 32, o);  // where this half's dy was
+            if (MODE == GATE_BWD) put8(own + h * 32, o);  // where this half's dy was
+            if (MODE == GATE && P.pre && h * 16 < cols) {
+              float* pre = P.pre + row0 * P.n + col + h * 16;
+              const int part = min(cols - h * 16, 16) * 4;
+              put8(own, reinterpret_cast<uint32_t*>(g));
+              put8(own + 32, reinterpret_cast<uint32_t*>(g) + 8);
+              put_rows(stage, lane, reinterpret_cast<char*>(pre), (int64_t)P.n * 4, rows, part, vec_pre);
+              put8(own, reinterpret_cast<uint32_t*>(u));
+              put8(own + 32, reinterpret_cast<uint32_t*>(u) + 8);
+              put_rows(stage, lane, reinterpret_cast<char*>(pre + (int64_t)P.m * P.n), (int64_t)P.n * 4, rows, part, vec_pre);
+            }
           }
-          put_rows(stage, lane, static_cast<char*>(P.out[0]) + at, P.ldo * 2, rows, cols * 2, vec);
-          if (MODE == GATE_BWD) {
-            put8(own, du[0]);
-            put8(own + 32, du[1]);
-            put_rows(stage, lane, static_cast<char*>(P.out[1]) + at, P.ldo * 2, rows, cols * 2, vec);
-          }
+          if (MODE == GATE_BWD)
+            put_rows(stage, lane, static_cast<char*>(P.out[0]) + at, P.ldo * 2, rows, cols * 2, vec);
+          put8(own, du[0]);
+          put8(own + 32, du[1]);
+          put_rows(stage, lane, static_cast<char*>(MODE == GATE ? P.out[0] : P.out[1]) + at, P.ldo * 2, rows, cols * 2, vec);
         } else {
           void* to = T.half ? P.out[1] : P.out[0];
           if (!to) continue;
@@ -385,6 +401,54 @@ __global__ void __launch_bounds__(128) join_kernel(const float* __restrict__ par
   const int64_t at = second ? i - n : i;
   if (BF16) static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
   else static_cast<__half*>(out)[at] = __float2half_rn(v);
+}
+
+// dg and du from the g and u that were kept: element (r, c) of g at r * F + c, of u R * F further.  A thread has 8
+// neighbouring elements where rows allow it (VEC), else one.  Memory bound: 14 bytes an element.
+template <bool BF16, bool VEC>
+__global__ void __launch_bounds__(256) gate_back_kernel(const float* __restrict__ pre, const uint16_t* __restrict__ dy, int64_t ldy,
+                                                        uint16_t* dg, uint16_t* du, int64_t ld, int64_t R, int64_t F,
+                                                        const uint32_t* amax) {
+  constexpr int N = VEC ? 8 : 1;
+  const float up = scale_up(amax);
+  const int64_t per = F / N, n = R * per;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / per, c = (i - r * per) * N;
+    float g[N], u[N], d[N], a[N], b[N];
+    const float* p = pre + r * F + c;
+    if (VEC) {
+#pragma unroll
+      for (int j = 0; j < N; j += 4) {
+        const float4 x = __ldg(reinterpret_cast<const float4*>(p + j)), y = __ldg(reinterpret_cast<const float4*>(p + R * F + j));
+        g[j] = x.x, g[j + 1] = x.y, g[j + 2] = x.z, g[j + 3] = x.w, u[j] = y.x, u[j + 1] = y.y, u[j + 2] = y.z, u[j + 3] = y.w;
+      }
+      const uint4 q = __ldg(reinterpret_cast<const uint4*>(dy + r * ldy + c));
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 v = unpack2<BF16>(w[j]);
+        d[2 * j] = v.x, d[2 * j + 1] = v.y;
+      }
+    } else {
+      g[0] = p[0], u[0] = p[R * F];
+      d[0] = unpack2<BF16>(dy[r * ldy + c]).x;
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float w = sigmoid(g[j]), e = d[j] * up;
+      a[j] = e * u[j] * (w * fmaf(g[j], 1.0f - w, 1.0f));
+      b[j] = e * g[j] * w;
+    }
+    if (VEC) {
+      *reinterpret_cast<uint4*>(dg + r * ld + c) =
+          make_uint4(pack2<BF16>(a[0], a[1]), pack2<BF16>(a[2], a[3]), pack2<BF16>(a[4], a[5]), pack2<BF16>(a[6], a[7]));
+      *reinterpret_cast<uint4*>(du + r * ld + c) =
+          make_uint4(pack2<BF16>(b[0], b[1]), pack2<BF16>(b[2], b[3]), pack2<BF16>(b[4], b[5]), pack2<BF16>(b[6], b[7]));
+    } else {
+      dg[r * ld + c] = (uint16_t)pack2<BF16>(a[0], 0.0f);
+      du[r * ld + c] = (uint16_t)pack2<BF16>(b[0], 0.0f);
+    }
+  }
 }
 
 // bits of the largest |dy| (0 before): a maximum does not depend on the order
@@ -634,7 +698,7 @@ int run_mm(const Maps& maps, const Args& P, cudaStream_t st, const char* who) {
 
 template <bool BF16>
 int run_gate(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void* wu, int64_t ldu, const void* dy,
-             int64_t ldy, void* o0, void* o1, int64_t ldo, const uint32_t* amax, int64_t R, int64_t C, int64_t F,
+             int64_t ldy, void* o0, void* o1, int64_t ldo, float* pre, const uint32_t* amax, int64_t R, int64_t C, int64_t F,
              cudaStream_t st, const char* who) {
   const Plan p(R, F, up(C, BK), 1, true);
   Maps maps;
@@ -644,7 +708,7 @@ int run_gate(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void
   maps.a[1] = maps.a[0];
   Args P = {};
   P.m = (int)R, P.n = (int)F, P.mt = p.mt, P.nt = p.nt, P.kb = (int)up(C, BK), P.halves_m = P.halves_k = 1;
-  P.splits = p.splits, P.kper = p.kper, P.out[0] = o0, P.out[1] = o1, P.ldo = ldo, P.dy = dy, P.ldy = ldy, P.amax = amax;
+  P.splits = p.splits, P.kper = p.kper, P.out[0] = o0, P.out[1] = o1, P.ldo = ldo, P.dy = dy, P.ldy = ldy, P.pre = pre, P.amax = amax;
   if (dy) return p.bn == 256 ? run_mm<GATE_BWD, BF16, 256>(maps, P, st, who) : run_mm<GATE_BWD, BF16, 128>(maps, P, st, who);
   return p.bn == 256 ? run_mm<GATE, BF16, 256>(maps, P, st, who) : run_mm<GATE, BF16, 128>(maps, P, st, who);
 }
@@ -667,10 +731,11 @@ int run_few(const Maps& maps, const FewArgs& P, int ranks, cudaStream_t st, cons
 }
 
 template <bool BF16>
-int forward(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void* wu, int64_t ldu, void* y, int64_t R,
+int forward(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void* wu, int64_t ldu, void* y, float* pre, int64_t R,
             int64_t C, int64_t F, cudaStream_t st) {
   const char* who = "csn_silu_gated_linear_fwd";
-  if (R > FEW) return run_gate<BF16>(x, ldx, wg, ldg, wu, ldu, nullptr, 0, y, nullptr, F, nullptr, R, C, F, st, who);
+  if (R > FEW || pre)
+    return run_gate<BF16>(x, ldx, wg, ldg, wu, ldu, nullptr, 0, y, nullptr, F, pre, nullptr, R, C, F, st, who);
   const int nr = R <= 16 ? 16 : R <= 32 ? 32 : 64;
   Maps maps;
   if (!make_map(&maps.a[0], wg, F, C, ldg, HALF_ROWS, BF16) || !make_map(&maps.a[1], wu, F, C, ldu, HALF_ROWS, BF16) ||
@@ -699,8 +764,8 @@ int run_product(const Maps& maps, Args P, int64_t blocks, const Plan& p, float* 
 
 template <bool BF16>
 int backward(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void* wu, int64_t ldu, const void* dy,
-             int64_t ldy, void* dx, void* dwg, void* dwu, int64_t R, int64_t C, int64_t F, const Scratch& s, void* ws,
-             cudaStream_t st) {
+             int64_t ldy, const float* pre, void* dx, void* dwg, void* dwu, int64_t R, int64_t C, int64_t F, const Scratch& s,
+             void* ws, cudaStream_t st) {
   const char* who = "csn_silu_gated_linear_bwd";
   char* base = static_cast<char*>(ws);
   void *dg = base + s.dg, *du = base + s.du;
@@ -711,7 +776,18 @@ int backward(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void
     if (cudaError_t e = cudaMemsetAsync(amax, 0, 4, st)) return set_cuda_error(e, who);
     amax_kernel<<<(unsigned)(R < 16 * PAIRS ? R : 16 * PAIRS), 256, 0, st>>>(static_cast<const __half*>(dy), ldy, R, F, amax);
   }
-  if (int rc = run_gate<BF16>(x, ldx, wg, ldg, wu, ldu, dy, ldy, dg, du, s.ld, amax, R, C, F, st, who)) return rc;
+  if (pre) {
+    const bool vec = F % 8 == 0 && ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(dy) & 15) == 0;
+    const int64_t ctas = up(R * (vec ? F / 8 : F), 256);
+    const unsigned grid = (unsigned)(ctas < 64 * PAIRS ? ctas : 64 * PAIRS);
+    const uint16_t* d = static_cast<const uint16_t*>(dy);
+    uint16_t *a = static_cast<uint16_t*>(dg), *b = static_cast<uint16_t*>(du);
+    if (vec) gate_back_kernel<BF16, true><<<grid, 256, 0, st>>>(pre, d, ldy, a, b, s.ld, R, F, amax);
+    else gate_back_kernel<BF16, false><<<grid, 256, 0, st>>>(pre, d, ldy, a, b, s.ld, R, F, amax);
+    if (int rc = check_launch(who)) return rc;
+  } else if (int rc = run_gate<BF16>(x, ldx, wg, ldg, wu, ldu, dy, ldy, dg, du, s.ld, nullptr, amax, R, C, F, st, who)) {
+    return rc;
+  }
   if (dx) {
     const Plan p(R, C, 2 * up(F, BK), 1, false);
     Maps maps;
@@ -799,15 +875,16 @@ extern "C" size_t csn_silu_gated_linear_workspace_bytes(int64_t R, int64_t C, in
 }
 
 extern "C" int csn_silu_gated_linear_fwd(const void* x, int64_t ldx, const void* w_gate, int64_t ld_gate,
-                                         const void* w_up, int64_t ld_up, void* y, int64_t R, int64_t C, int64_t F,
+                                         const void* w_up, int64_t ld_up, void* y, float* pre, int64_t R, int64_t C, int64_t F,
                                          int dtype, void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = check_ffn("csn_silu_gated_linear_fwd: needs 0 <= R, C, F <= 2^21 and dtype bfloat16 or float16", R, C, F, dtype))
     return rc;
   if (R == 0 || F == 0) return CSN_OK;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (!y || !al16b(y)) return set_error(CSN_ERR_INVALID, "csn_silu_gated_linear_fwd: y missing or misaligned");
+  if (!y || !al16b(y) || !al16b(pre)) return set_error(CSN_ERR_INVALID, "csn_silu_gated_linear_fwd: y missing, or y or pre misaligned");
   if (C == 0) {
-    const cudaError_t e = cudaMemsetAsync(y, 0, (size_t)R * F * 2, st);
+    cudaError_t e = cudaMemsetAsync(y, 0, (size_t)R * F * 2, st);
+    if (e == cudaSuccess && pre) e = cudaMemsetAsync(pre, 0, (size_t)R * F * 8, st);
     return e == cudaSuccess ? CSN_OK : set_cuda_error(e, "csn_silu_gated_linear_fwd");
   }
   if (!even(x) || !even(w_gate) || !even(w_up))
@@ -818,12 +895,12 @@ extern "C" int csn_silu_gated_linear_fwd(const void* x, int64_t ldx, const void*
     return set_error(CSN_ERR_INVALID, "csn_silu_gated_linear_fwd: workspace smaller than csn_silu_gated_linear_workspace_bytes");
   KernelTimer kt("silu_gated_linear_fwd", st);
   if (int rc = o.copy(R, C, F, s, workspace, st)) return rc;
-  return dtype == CSN_BF16 ? forward<true>(o.p[0], o.ld[0], o.p[1], o.ld[1], o.p[2], o.ld[2], y, R, C, F, st)
-                           : forward<false>(o.p[0], o.ld[0], o.p[1], o.ld[1], o.p[2], o.ld[2], y, R, C, F, st);
+  return dtype == CSN_BF16 ? forward<true>(o.p[0], o.ld[0], o.p[1], o.ld[1], o.p[2], o.ld[2], y, pre, R, C, F, st)
+                           : forward<false>(o.p[0], o.ld[0], o.p[1], o.ld[1], o.p[2], o.ld[2], y, pre, R, C, F, st);
 }
 
 extern "C" int csn_silu_gated_linear_bwd(const void* x, int64_t ldx, const void* w_gate, int64_t ld_gate,
-                                         const void* w_up, int64_t ld_up, const void* dy, int64_t ld_dy, void* dx,
+                                         const void* w_up, int64_t ld_up, const void* dy, int64_t ld_dy, const float* pre, void* dx,
                                          void* dw_gate, void* dw_up, int64_t R, int64_t C, int64_t F, int dtype,
                                          void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = check_ffn("csn_silu_gated_linear_bwd: needs 0 <= R, C, F <= 2^21 and dtype bfloat16 or float16", R, C, F, dtype))
@@ -837,7 +914,7 @@ extern "C" int csn_silu_gated_linear_bwd(const void* x, int64_t ldx, const void*
         return set_error(CSN_ERR_CUDA, "csn_silu_gated_linear_bwd: cudaMemsetAsync");
     return CSN_OK;
   }
-  if (!even(dy) || !even(x) || !even(w_gate) || !even(w_up) || !al16b(dx) || !al16b(dw_gate) || !al16b(dw_up))
+  if (!even(dy) || !even(x) || !even(w_gate) || !even(w_up) || !al16b(pre) || !al16b(dx) || !al16b(dw_gate) || !al16b(dw_up))
     return set_error(CSN_ERR_INVALID, "csn_silu_gated_linear_bwd: missing or misaligned pointer");
   Operands o(x, ldx, w_gate, ld_gate, w_up, ld_up, R, C, F);
   const Scratch s(R, C, F, o.copies, true);
@@ -845,8 +922,8 @@ extern "C" int csn_silu_gated_linear_bwd(const void* x, int64_t ldx, const void*
     return set_error(CSN_ERR_INVALID, "csn_silu_gated_linear_bwd: workspace smaller than csn_silu_gated_linear_workspace_bytes");
   KernelTimer kt("silu_gated_linear_bwd", st);
   if (int rc = o.copy(R, C, F, s, workspace, st)) return rc;
-  return dtype == CSN_BF16 ? backward<true>(o.p[0], o.ld[0], o.p[1], o.ld[1], o.p[2], o.ld[2], dy, ld_dy, dx, dw_gate, dw_up, R, C,
+  return dtype == CSN_BF16 ? backward<true>(o.p[0], o.ld[0], o.p[1], o.ld[1], o.p[2], o.ld[2], dy, ld_dy, pre, dx, dw_gate, dw_up, R, C,
                                             F, s, workspace, st)
-                           : backward<false>(o.p[0], o.ld[0], o.p[1], o.ld[1], o.p[2], o.ld[2], dy, ld_dy, dx, dw_gate, dw_up, R,
+                           : backward<false>(o.p[0], o.ld[0], o.p[1], o.ld[1], o.p[2], o.ld[2], dy, ld_dy, pre, dx, dw_gate, dw_up, R,
                                              C, F, s, workspace, st);
 }

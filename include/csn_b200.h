@@ -443,8 +443,9 @@ int csn_gated_step(const void* f, const void* x, const void* gate, const int64_t
 
 /* y = silu(x w_gate^T) * (x w_up^T) in one pass (csn_silu_gate_fwd on the product that feeds it):
  * x [R, C], w_gate, w_up [F, C] with row strides ldx, ld_gate, ld_up (elements), y [R, F]
- * contiguous, 16-byte aligned; bfloat16 or float16, sums in float32.  The backward forms both
- * products again and writes dx [R, C], dw_gate, dw_up [F, C] (contiguous; each may be NULL) from
+ * contiguous, 16-byte aligned; bfloat16 or float16, sums in float32.  pre: NULL, or 2 R F floats
+ * (16-byte aligned) in which the forward keeps both products and from which the backward takes
+ * them; with NULL it forms them again.  The backward writes dx [R, C], dw_gate, dw_up [F, C] (contiguous; each may be NULL) from
  * dy [R, F] (row stride ld_dy).  R, C, F <= 2^21.
  * Operands whose rows do not start on 16 bytes (base, or row stride not a multiple of 8 elements
  * or below C) are copied first: csn_silu_gated_linear_copies says which (bits 0, 1, 2 for x,
@@ -456,12 +457,12 @@ int csn_silu_gated_linear_copies(const void* x, int64_t ldx, const void* w_gate,
 size_t csn_silu_gated_linear_workspace_bytes(int64_t R, int64_t C, int64_t F, int copies,
                                              int backward);
 int csn_silu_gated_linear_fwd(const void* x, int64_t ldx, const void* w_gate, int64_t ld_gate,
-                              const void* w_up, int64_t ld_up, void* y, int64_t R, int64_t C,
-                              int64_t F, int dtype, void* workspace, size_t workspace_bytes,
+                              const void* w_up, int64_t ld_up, void* y, float* pre, int64_t R,
+                              int64_t C, int64_t F, int dtype, void* workspace, size_t workspace_bytes,
                               void* stream);
 int csn_silu_gated_linear_bwd(const void* x, int64_t ldx, const void* w_gate, int64_t ld_gate,
                               const void* w_up, int64_t ld_up, const void* dy, int64_t ld_dy,
-                              void* dx, void* dw_gate, void* dw_up, int64_t R, int64_t C, int64_t F,
+                              const float* pre, void* dx, void* dw_gate, void* dw_up, int64_t R, int64_t C, int64_t F,
                               int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /* y[i] = residual[i] + keep_i x[i] 65536 / (65536 - cut) over n elements (residual NULL: 0), a

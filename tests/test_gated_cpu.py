@@ -111,8 +111,8 @@ def test_step_refuses(lib):
 def test_ffn_refuses(lib):
     p = fake()
 
-    def fwd(x=p, y=p, R=4, C=8, F=8, ldx=8, dtype=1, ws=NULL, nb=0):
-        return lib.csn_silu_gated_linear_fwd(x, ldx, p, C, p, C, y, R, C, F, dtype, ws, nb, NULL)
+    def fwd(x=p, y=p, R=4, C=8, F=8, ldx=8, dtype=1, ws=NULL, nb=0, pre=NULL):
+        return lib.csn_silu_gated_linear_fwd(x, ldx, p, C, p, C, y, pre, R, C, F, dtype, ws, nb, NULL)
 
     refused(lib, fwd(R=-1), 1, "R, C, F")
     refused(lib, fwd(F=2 ** 22), 1, "R, C, F")
@@ -120,12 +120,13 @@ def test_ffn_refuses(lib):
     refused(lib, fwd(x=NULL), 1, "required")
     refused(lib, fwd(x=fake(1)), 1, "aligned")
     refused(lib, fwd(y=fake(2)), 1, "misaligned")
+    refused(lib, fwd(pre=fake(8)), 1, "misaligned")
     for odd in (dict(x=fake(8)), dict(ldx=12), dict(ldx=0), dict(C=9, ldx=16), dict(R=2, ldx=-8)):
         refused(lib, fwd(**odd), 1, "workspace")  # a copy is needed, and there is no room for it
     assert fwd(R=0) == 0 and fwd(F=0) == 0
 
     def bwd(dy=p, dx=p, R=4, C=8, F=8, ws=p, nb=1 << 30):
-        return lib.csn_silu_gated_linear_bwd(p, C, p, C, p, C, dy, F, dx, p, p, R, C, F, 1, ws, nb, NULL)
+        return lib.csn_silu_gated_linear_bwd(p, C, p, C, p, C, dy, F, NULL, dx, p, p, R, C, F, 1, ws, nb, NULL)
 
     refused(lib, bwd(dy=NULL), 1, "missing")
     refused(lib, bwd(dx=fake(2)), 1, "misaligned")

@@ -260,6 +260,16 @@ def test_ffn_of_few_rows(ops, R):
              make((F, C), "bfloat16", 3, scale=C ** -0.5), "bfloat16")
 
 
+@pytest.mark.parametrize("kind", ["bfloat16", "float16"])
+@pytest.mark.parametrize("R,C,F", [(70, 1536, 136), (130, 1541, 75), (300, 1600, 64), (65, 2048, 33)])
+def test_ffn_wide_layers_keep_their_products(ops, kind, R, C, F):
+    """From some width on the backward pass takes both products from the forward pass."""
+    x = make((R, C), kind, 1)
+    wg, wu = make((F, C), kind, 2, scale=C ** -0.5), make((F, C), kind, 3, scale=C ** -0.5)
+    ffn_case(ops, x, wg, wu, kind, make((R, F), kind, 4))
+    ffn_case(ops, x, wg, wu, kind, make((R, F + 1), kind, 4)[:, 1:])
+
+
 def test_ffn_many_rows_narrow_weights(ops):
     R, C, F = 5000, 64, 128
     ffn_case(ops, make((R, C), "bfloat16", 1), make((F, C), "bfloat16", 2, scale=0.1),
