@@ -470,7 +470,7 @@ __host__ __device__ constexpr int few_stages(int nr) { return nr == 64 ? 4 : 5; 
 constexpr int few_smem(int nr) { return few_stages(nr) * few_stage(nr) + 1024; }
 
 struct FewArgs {
-  int R, F, kb, kper;
+  int R, F, kb;
   void* y;
 };
 
@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(const __grid_cons
   uint32_t ranks;
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
   const int f0 = blockIdx.x / ranks * HALF_ROWS;
-  const int k0 = rank * P.kper, k1 = min(k0 + P.kper, P.kb);
+  const int k0 = P.kb * (int)rank / (int)ranks, k1 = P.kb * ((int)rank + 1) / (int)ranks;  // none is empty: kb >= 4 ranks
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < ST; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
@@ -742,11 +742,10 @@ int forward(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void*
       !make_map(&maps.b[0], x, R, C, ldx, nr, BF16))
     return set_error(CSN_ERR_CUDA, "silu_gated_linear: cuTensorMapEncodeTiled");
   maps.b[1] = maps.b[0];
-  FewArgs P = {(int)R, (int)F, (int)up(C, BK), 0, y};
+  const FewArgs P = {(int)R, (int)F, (int)up(C, BK), y};
   // two CTAs fit on an SM: ranges of C (at least 4 blocks each) until there are as many
   int ranks = 1;
   while (ranks < 8 && up(F, HALF_ROWS) * ranks * 2 <= 4 * PAIRS && P.kb >= ranks * 2 * 4) ranks *= 2;
-  P.kper = (int)up(P.kb, ranks);
   return nr == 16 ? run_few<BF16, 16>(maps, P, ranks, st, who)
                   : nr == 32 ? run_few<BF16, 32>(maps, P, ranks, st, who) : run_few<BF16, 64>(maps, P, ranks, st, who);
 }

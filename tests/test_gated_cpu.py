@@ -48,6 +48,47 @@ def test_marks_hold_every_pass_of_every_sequence(lib, packed, S, T):
             assert end * C <= have
 
 
+@pytest.mark.parametrize("seed", range(6))
+def test_any_borders_stay_inside(lib, seed):
+    """The scan's arithmetic for a packed batch (which sequence and chunk a unit works on, its marks and its
+    neighbours' maps), written out: every row, mark and map is inside its buffer for rising borders and,
+    though the results mean nothing then, for any others."""
+    import random
+    rng = random.Random(seed)
+    for _ in range(60):
+        S, T, C = rng.randint(1, 40), rng.randint(1, 3000), rng.choice([8, 64, 771])
+        cu = [rng.randint(-50, T + 50) for _ in range(S + 1)]
+        rising = rng.random() < 0.5
+        if rising:
+            cu = sorted(min(max(v, 0), T) for v in cu)
+        need = lib.csn_gated_scan_workspace_bytes(S, T, C, 1, 1, 0) // (C * 8)
+        units = need if need else S
+        # the chunk that this size has: units = T // chunk + S
+        for chunk in ([c for c in range(256, T + 64, 64) if T // c + S == units][:1] if need else [-(-T // 64) * 64]):
+            cut = [min(max(v, 0), T) for v in cu]
+            base = [cut[i] // chunk + i for i in range(S)]
+            done = [0] * T
+            for u in range(T // chunk + S):
+                s = max((i for i in range(S) if base[i] <= u), default=-1) if rising else rng.choice(
+                    [i for i in range(S) if base[i] <= u] or [-1])
+                if s < 0:
+                    continue
+                row0, length = cut[s], max(cut[s + 1], cut[s]) - cut[s]
+                k = u - base[s]
+                assert k >= 0
+                first, past = min(k * chunk, length), min(k * chunk + chunk, length)
+                if k > 0 and first >= length:
+                    continue
+                assert 0 <= row0 + first <= row0 + past <= T
+                for t in range(first, past):
+                    done[row0 + t] += 1
+                if past > first:
+                    assert row0 // 64 + s + (past - 1) // 64 < lib.csn_gated_scan_marks(S, T, C, 1) // C
+                    assert 0 <= u - k and u + (length - 1) // chunk - k < T // chunk + S
+            if rising:
+                assert all(n == (cut[0] <= t < cut[-1]) for t, n in enumerate(done))
+
+
 def test_marks_of_nothing(lib):
     assert lib.csn_gated_scan_marks(0, 5, 8, 0) == 0 and lib.csn_gated_scan_marks(5, 5, 0, 0) == 0
 

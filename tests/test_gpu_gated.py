@@ -260,6 +260,14 @@ def test_ffn_of_few_rows(ops, R):
              make((F, C), "bfloat16", 3, scale=C ** -0.5), "bfloat16")
 
 
+@pytest.mark.parametrize("C,F", [(2112, 64), (2240, 100), (2624, 576), (1088, 64), (512, 1000), (4160, 40), (9, 3)])
+def test_ffn_of_few_rows_over_every_split(ops, C, F):
+    """Cuts of the channels among the CTAs of a cluster that do not come out even."""
+    for R in (2, 40):
+        ffn_case(ops, make((R, C), "bfloat16", 1), make((F, C), "bfloat16", 2, scale=C ** -0.5),
+                 make((F, C), "bfloat16", 3, scale=C ** -0.5), "bfloat16")
+
+
 @pytest.mark.parametrize("kind", ["bfloat16", "float16"])
 @pytest.mark.parametrize("R,C,F", [(70, 1536, 136), (130, 1541, 75), (300, 1600, 64), (65, 2048, 33)])
 def test_ffn_wide_layers_keep_their_products(ops, kind, R, C, F):
