@@ -15,7 +15,7 @@
 // that take 48 KB when it works alone; what L2 delivers (about 60 bytes a clock and SM) is what bounds a large product.
 // In each CTA one thread feeds a ring of shared-memory stages by TMA, one of the pair issues tcgen05.mma into one of
 // two accumulators in tensor memory, and for each accumulator eight warps finish it, so that loads, products and both
-// epilogues overlap across tiles.  For the gate, BN = 2 FN: CTA 0 loads FN rows of Wg and CTA 1 the same FN rows of Wu
+// epilogues overlap across tiles (all sixteen on one after the other: R65536 C128 F256 forward 26.6 us against 20.8).  For the gate, BN = 2 FN: CTA 0 loads FN rows of Wg and CTA 1 the same FN rows of Wu
 // as the halves of one operand, so g and u of a place sit in one tensor-memory lane and the gate is a per-lane
 // epilogue.  The transposed products read the same row-major tensors with an MN-major operand: nothing is transposed in
 // memory.
@@ -353,7 +353,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             float v[16];
             tmem_load16(d + c + h * 16, v);
             tmem_load_wait();
-            if (!ok) v[0] = v[1] = v[2] = v[3] = v[4] = v[5] = v[6] = v[7] = v[8] = v[9] = v[10] = v[11] = v[12] = v[13] = v[14] = v[15] = nan;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (!ok) v[i] = nan;
             if (P.splits > 1) {
               if (h * 16 >= cols) continue;
               put8(own, reinterpret_cast<uint32_t*>(v));
@@ -681,14 +683,9 @@ struct Scratch {
   }
 };
 
-template <typename K>
-cudaError_t allow_smem(K kernel, int bytes) {
-  return cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-}
-
 template <Mode MODE, bool BF16, int BN>
 int run_mm(const Maps& maps, const Args& P, cudaStream_t st, const char* who) {
-  if (cudaError_t e = allow_smem(mm_kernel<MODE, BF16, BN>, smem_bytes(BN))) return set_cuda_error(e, who);
+  if (cudaError_t e = allow_smem<mm_kernel<MODE, BF16, BN>>(smem_bytes(BN))) return set_cuda_error(e, who);
   const int64_t tiles = (int64_t)P.mt * P.nt * P.halves_m * P.splits;
   const int64_t pairs = sm_count() / 2;
   const unsigned grid = 2 * (unsigned)(tiles < pairs ? tiles : pairs);
@@ -715,7 +712,7 @@ int run_gate(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void
 
 template <bool BF16, int NR>
 int run_few(const Maps& maps, const FewArgs& P, int ranks, cudaStream_t st, const char* who) {
-  if (cudaError_t e = allow_smem(few_rows_kernel<BF16, NR>, few_smem(NR))) return set_cuda_error(e, who);
+  if (cudaError_t e = allow_smem<few_rows_kernel<BF16, NR>>(few_smem(NR))) return set_cuda_error(e, who);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(up(P.F, HALF_ROWS) * ranks));
   cfg.blockDim = dim3(FEW_THREADS);

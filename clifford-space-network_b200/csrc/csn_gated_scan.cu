@@ -241,6 +241,11 @@ __device__ __forceinline__ void copies_done() {
   __syncwarp();
 }
 
+// The scan of a chunked batch is launched while its reduce pass runs (programmatic dependent launch): it has its rows
+// under way when it waits here for what that pass leaves in A.maps.
+__device__ __forceinline__ void others_done() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void others_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // A map h -> p h + b of V channels
 template <int V>
 struct alignas(8 * V) Map {
@@ -287,6 +292,7 @@ __global__ void __launch_bounds__(WARPS * 32, 3) reduce_kernel(const __grid_cons
   extern __shared__ __align__(128) char ring[];  // [2][N][MARK rows]
   __shared__ Map<V> maps[WARPS][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  others_may_start();
   const Part q(A, blockIdx.x / A.tiles);
   if (q.s < 0 || (BACK ? q.k == 0 : q.to == q.len)) return;
   const int64_t tile = (int64_t)(blockIdx.x % A.tiles) * channels(sizeof(T), ODD), c = tile + lane * V;
@@ -371,6 +377,7 @@ __global__ void __launch_bounds__(WARPS * 32, 3) gated_scan_fwd_kernel(const __g
     copies_queued();
   };
   fetch(0, q.to - t1);
+  others_done();
   F carry = A.h0 ? load_state<V>(A.h0 + q.s * A.C + c, have) : splat<V>(0.0f);
   if (q.k > 0) carry = enter<V>(A, maps[1], carry, q.unit - q.k, q.k, 1, c, have);
   T* out = static_cast<T*>(A.y) + (q.row0 + t1) * A.C + c;
@@ -466,6 +473,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) gated_scan_bwd_kernel(const __g
     copies_queued();
   };
   if (last >= q.from) fetch(0, q.to - t1);
+  others_done();
   // the gradient that enters from behind: a lam of the step after
   F mu = A.dh_last ? load_state<V>(A.dh_last + q.s * A.C + c, have) : splat<V>(0.0f);
   if (q.to < q.len) {
@@ -649,25 +657,34 @@ struct Cut {
   bool split(int64_t T) const { return T > chunk; }
 };
 
-template <typename K>
-cudaError_t launch_part(K kernel, int64_t grid, int smem, const ScanArgs& A, cudaStream_t st) {
-  if (cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, smem))
-    return e;
-  kernel<<<(unsigned)grid, WARPS * 32, smem, st>>>(A);
-  return cudaGetLastError();
+template <auto KERNEL>
+cudaError_t launch_part(int64_t grid, int smem, const ScanArgs& A, bool early, cudaStream_t st) {
+  if (cudaError_t e = allow_smem<KERNEL>(smem)) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(WARPS * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = early ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, KERNEL, A);
 }
 
 template <typename T, bool GATE, bool ODD>
 cudaError_t launch_scan(const ScanArgs& A, bool bwd, const Cut& cut, cudaStream_t st) {
   const int64_t grid = cut.ctas * cut.tiles;
-  const int piece = 2 * PIECE;
-  if (cut.split(A.T)) {
-    const cudaError_t e = bwd ? launch_part(reduce_kernel<T, GATE, ODD, true>, grid, (GATE ? 3 : 2) * piece, A, st)
-                              : launch_part(reduce_kernel<T, false, ODD, false>, grid, 2 * piece, A, st);
+  constexpr int piece = 2 * PIECE;
+  const bool split = cut.split(A.T);
+  if (split) {
+    const cudaError_t e = bwd ? launch_part<reduce_kernel<T, GATE, ODD, true>>(grid, (GATE ? 3 : 2) * piece, A, false, st)
+                              : launch_part<reduce_kernel<T, false, ODD, false>>(grid, 2 * piece, A, false, st);
     if (e != cudaSuccess) return e;
   }
-  return bwd ? launch_part(gated_scan_bwd_kernel<T, GATE, ODD>, grid, (GATE ? 4 : 3) * piece, A, st)
-             : launch_part(gated_scan_fwd_kernel<T, GATE, ODD>, grid, (GATE ? 3 : 2) * piece, A, st);
+  return bwd ? launch_part<gated_scan_bwd_kernel<T, GATE, ODD>>(grid, (GATE ? 4 : 3) * piece, A, split, st)
+             : launch_part<gated_scan_fwd_kernel<T, GATE, ODD>>(grid, (GATE ? 3 : 2) * piece, A, split, st);
 }
 template <typename T, bool ODD>
 cudaError_t launch_scan(const ScanArgs& A, bool bwd, const Cut& cut, cudaStream_t st) {

@@ -2,6 +2,9 @@
 #pragma once
 
 #include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <atomic>
 
 #include "../../include/csn_b200.h"
 
@@ -16,6 +19,20 @@ int check_launch(const char* where);
 }  // namespace csn
 
 namespace csn {
+
+// Allows KERNEL `bytes` of dynamic shared memory, once on each device (a call of the runtime costs as much as a launch).
+template <auto KERNEL>
+cudaError_t allow_smem(int bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load() & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(reinterpret_cast<const void*>(KERNEL), cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit);
+  return e;
+}
 
 // Optional per-kernel timing (off by default).  When enabled with
 // csn_timing_enable(1), every library launch wrapped in a KernelTimer records a pair
