@@ -482,11 +482,11 @@ struct FewArgs {
   void* y;
 };
 
-__device__ __forceinline__ float peer_float(uint32_t addr, uint32_t rank) {
+__device__ __forceinline__ float4 peer_float4(uint32_t addr, uint32_t rank) {
   uint32_t a;
-  float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  float4 v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
   return v;
 }
 
@@ -516,7 +516,9 @@ __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(const __grid_cons
   __syncthreads();
   fence_after();
   const uint32_t tmem = tmem_slot;
-  float* sums = reinterpret_cast<float*>(smem);  // [128][NR + 1], in the stages once they are done with
+  // [NR][128], in the stages once they are done with: neighbouring lanes write and read neighbouring places, which
+  // matters for what other CTAs read (in the other order a read took 32 trips: 20 thousand cycles for 41 rows)
+  float* sums = reinterpret_cast<float*>(smem);
 
   bool ok = true;
   if (warp == 4) {
@@ -565,25 +567,36 @@ __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(const __grid_cons
       tmem_load16(tmem + ((uint32_t)(warp * 32) << 16) + c, v);
       tmem_load_wait();
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sums[row * (NR + 1) + c + i] = ok && !gave_up ? v[i] : __int_as_float(0x7fffffff);
+      for (int i = 0; i < 16; ++i) sums[(c + i) * 2 * HALF_ROWS + row] = ok && !gave_up ? v[i] : __int_as_float(0x7fffffff);
     }
     fence_before();
   }
   __syncthreads();
   cluster_sync();
   const uint32_t base = smem_addr(sums);
-  for (int i = rank * FEW_THREADS + threadIdx.x; i < P.R * HALF_ROWS; i += ranks * FEW_THREADS) {
-    const int r = i / HALF_ROWS, f = i % HALF_ROWS;
-    if (f0 + f >= P.F) continue;
-    float g = 0.0f, u = 0.0f;
+  // a thread has 4 neighbouring hidden units of a row
+  for (int i = rank * FEW_THREADS + threadIdx.x; i < P.R * (HALF_ROWS / 4); i += ranks * FEW_THREADS) {
+    const int r = i / (HALF_ROWS / 4), f = i % (HALF_ROWS / 4) * 4, left = P.F - f0 - f;
+    if (left <= 0) continue;
+    float4 g = make_float4(0.0f, 0.0f, 0.0f, 0.0f), u = g;
+#pragma unroll 4
     for (uint32_t k = 0; k < ranks; ++k) {
-      g += peer_float(base + (f * (NR + 1) + r) * 4, k);
-      u += peer_float(base + ((f + HALF_ROWS) * (NR + 1) + r) * 4, k);
+      const float4 a = peer_float4(base + (r * 2 * HALF_ROWS + f) * 4, k);
+      const float4 b = peer_float4(base + (r * 2 * HALF_ROWS + HALF_ROWS + f) * 4, k);
+      g.x += a.x, g.y += a.y, g.z += a.z, g.w += a.w;
+      u.x += b.x, u.y += b.y, u.z += b.z, u.w += b.w;
     }
-    const float v = g * sigmoid(g) * u;
-    const int64_t at = (int64_t)r * P.F + f0 + f;
-    if (BF16) static_cast<__nv_bfloat16*>(P.y)[at] = __float2bfloat16_rn(v);
-    else static_cast<__half*>(P.y)[at] = __float2half_rn(v);
+    const uint32_t lo = pack2<BF16>(g.x * sigmoid(g.x) * u.x, g.y * sigmoid(g.y) * u.y);
+    const uint32_t hi = pack2<BF16>(g.z * sigmoid(g.z) * u.z, g.w * sigmoid(g.w) * u.w);
+    uint16_t* y = static_cast<uint16_t*>(P.y) + (int64_t)r * P.F + f0 + f;
+    if (P.F % 4 == 0) {
+      *reinterpret_cast<uint2*>(y) = make_uint2(lo, hi);
+    } else {
+      y[0] = (uint16_t)lo;
+      if (left > 1) y[1] = (uint16_t)(lo >> 16);
+      if (left > 2) y[2] = (uint16_t)hi;
+      if (left > 3) y[3] = (uint16_t)(hi >> 16);
+    }
   }
   cluster_sync();  // the peers have read this CTA's sums
   if (warp == 4) {
@@ -747,9 +760,10 @@ int forward(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void*
     return set_error(CSN_ERR_CUDA, "silu_gated_linear: cuTensorMapEncodeTiled");
   maps.b[1] = maps.b[0];
   const FewArgs P = {(int)R, (int)F, (int)up(C, BK), y};
-  // two CTAs fit on an SM: ranges of C (at least 4 blocks each) until there are as many
+  // Ranges of C, at least 4 blocks each, until there are one and a half CTAs an SM.  Two fit, but clusters do not fill
+  // every SM: R9 C1824 F4736 took 17.3 us with 296 CTAs and takes 10.6 with 148.
   int ranks = 1;
-  while (ranks < 8 && up(F, HALF_ROWS) * ranks * 2 <= 4 * PAIRS && P.kb >= ranks * 2 * 4) ranks *= 2;
+  while (ranks < 8 && up(F, HALF_ROWS) * ranks * 2 <= 3 * PAIRS && P.kb >= ranks * 2 * 4) ranks *= 2;
   return nr == 16 ? run_few<BF16, 16>(maps, P, ranks, st, who)
                   : nr == 32 ? run_few<BF16, 32>(maps, P, ranks, st, who) : run_few<BF16, 64>(maps, P, ranks, st, who);
 }
