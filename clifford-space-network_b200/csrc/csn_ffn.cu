@@ -655,8 +655,9 @@ int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to; }
 // How a product of m x n over k blocks is cut up: into tiles 256 or 128 columns wide, whichever takes less time when
 // PAIRS of them run at a time.  A k block of a wide tile counts 1 and of a narrow one 0.7 (it moves 24 KB an SM for half
 // the products of 32 KB), what a tile costs besides 8 and 4.  Forward, wide / narrow, us: R6509 C1152 F3440 71 / 86, R3000
-// C768 F1536 15.2 / 17.2, R178 C1736 F4112 17.6 / 14.1, R512 C256 F1024 8.0 / 6.3.  Where tiles leave more than half of the SMs idle, k is cut
-// into ranges of at least 4 blocks, whose sums a second kernel adds.
+// C768 F1536 15.2 / 17.2, R178 C1736 F4112 17.6 / 14.1, R512 C256 F1024 8.0 / 6.3.  Where tiles leave more than half of the SMs
+// idle and k has 32 blocks or more, k is cut into ranges of at least 8, whose sums a second kernel adds (shorter sums
+// take less time than that kernel's launch).
 struct Plan {
   int bn, mt, nt, splits, kper;
   Plan(int64_t m, int64_t n, int64_t blocks, int halves, bool gate) {
@@ -666,10 +667,9 @@ struct Plan {
     nt = (int)up(n, gate ? bn / 2 : bn);
     splits = 1;
     const int64_t tiles = (int64_t)mt * nt * halves;
-    if (!gate && tiles * 2 <= PAIRS) {
-      int64_t s = PAIRS / tiles;
-      s = s < blocks / 4 ? s : blocks / 4;
-      splits = s > 1 ? (int)s : 1;
+    if (!gate && tiles * 2 <= PAIRS && blocks >= 32) {
+      const int64_t s = PAIRS / tiles;
+      splits = (int)(s < blocks / 8 ? s : blocks / 8);
     }
     kper = (int)up(blocks, splits);
     splits = (int)up(blocks, kper);

@@ -115,10 +115,10 @@ def silu_gated_linear(x, wg, wu, kind, dy=None):
     return out
 
 
-def philox_halves(n, seed, offset):
-    """The 16-bit numbers of n places: Philox4x32-10 in Python's own whole numbers."""
+def philox_halves(n, seed, offset, block=0):
+    """The 16-bit numbers of n places from place 8 `block` on: Philox4x32-10 in Python's own whole numbers."""
     low, out = 0xFFFFFFFF, []
-    for j in range((n + 7) // 8):
+    for j in range(block, block + (n + 7) // 8):
         c = [j & low, j >> 32, offset & low, (offset >> 32) & low]
         k = [seed & low, (seed >> 32) & low]
         for _ in range(10):

@@ -436,6 +436,81 @@ def test_other_stream_and_captured_replay(ops):
             assert torch.equal(a, b)
 
 
+def test_calls_of_two_streams_at_once(ops):
+    f, x, gate = (make((3, 900, 96), "bfloat16", i) for i in (1, 2, 3))
+    a, wg, wu = make((700, 200), "bfloat16", 4), make((300, 200), "bfloat16", 5, 0.1), make((300, 200), "bfloat16", 6, 0.1)
+    dy, da = make((3, 900, 96), "bfloat16", 7), make((700, 300), "bfloat16", 8)
+
+    def run():
+        leaves = [t.detach().requires_grad_(True) for t in (f, x, gate, a, wg, wu)]
+        y, h = ops.gated_scan(*leaves[:2], gate=leaves[2])
+        z = ops.silu_gated_linear(*leaves[3:])
+        few = ops.silu_gated_linear(a[:20], wg, wu)
+        return [y, h, z, few, *torch.autograd.grad((y, z), leaves, (dy, da))]
+
+    want = run()
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(3)], []
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(run())
+    torch.cuda.synchronize()
+    for out in got:
+        for a_, b_ in zip(want, out):
+            assert torch.equal(a_, b_)
+
+
+def test_some_gradients_only(ops):
+    """What is not asked for does not change what is."""
+    R, C, F = 90, 72, 80
+    x, wg, wu, dy = make((R, C), "bfloat16", 1), make((F, C), "bfloat16", 2, 0.1), make((F, C), "bfloat16", 3, 0.1), make((R, F), "bfloat16", 4)
+    every = [t.detach().requires_grad_(True) for t in (x, wg, wu)]
+    want = torch.autograd.grad(ops.silu_gated_linear(*every), every, dy)
+    for keep in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 0, 1), (0, 1, 1)):
+        args = [t.detach().requires_grad_(bool(k)) for t, k in zip((x, wg, wu), keep)]
+        got = torch.autograd.grad(ops.silu_gated_linear(*args), [t for t, k in zip(args, keep) if k], dy)
+        for g, w in zip(got, [w for w, k in zip(want, keep) if k]):
+            assert torch.equal(g, w)
+    rng = torch.tensor([1, 2], device="cuda")
+    res = x.detach().requires_grad_(True)
+    (d,) = torch.autograd.grad(ops.dropout_add(x, res, 0.5, rng), res, x)
+    assert torch.equal(d, x)
+    (d,) = torch.autograd.grad(ops.dropout_add(res, x, 0.5, rng), res, x)
+    assert torch.equal(d, ops.dropout_add(x, None, 0.5, rng))
+    T = 70
+    f, v = make((2, T, C), "float16", 5), make((2, T, C), "float16", 6)
+    h0 = make((2, C), "float16", 7).requires_grad_(True)
+    y, h = ops.gated_scan(f, v, h0=h0)
+    (d,) = torch.autograd.grad(h, h0, torch.ones_like(h))
+    assert d.dtype == torch.float16
+    want = orc.gated_scan(to64(f).reshape(-1, C), to64(v).reshape(-1, C), to64(h0), None, [(0, T), (T, 2 * T)], None, np.ones((2, C)))
+    check(d, want["dh0"], "float16", "dh0")
+
+
+def test_offsets_past_32_bits(ops):
+    """Rows far apart, and a tensor of more than 2^31 elements."""
+    T, C, far = 70, 64, 1 << 25
+    big = torch.empty(T * far, device="cuda", dtype=torch.bfloat16).view(T, far)
+    big[:, :3 * C] = make((T, 3 * C), "bfloat16", 1)
+    f, x, gate = (big[:, i * C:(i + 1) * C] for i in range(3))
+    scan_case(ops, f[None], x[None], None, gate[None], None, "bfloat16", dy=make((1, T, C), "bfloat16", 5))
+    cu = torch.tensor([0, 33, T], dtype=torch.int32, device="cuda")
+    scan_case(ops, f, x, None, gate, cu, "bfloat16", dy=make((T, C), "bfloat16", 5))
+    w = make((2 * 72, C), "bfloat16", 6, scale=0.1)
+    ffn_case(ops, x, w[:72], w[72:], "bfloat16", make((T, 72), "bfloat16", 7))
+    ffn_case(ops, x[:40], w[:72], w[72:], "bfloat16")
+    h = torch.zeros(T, C, device="cuda")
+    assert torch.equal(ops.gated_step(f, x, h), ops.gated_step(f.contiguous(), x.contiguous(), torch.zeros_like(h)))
+    del big, f, x, gate
+    n = (1 << 31) + 29
+    one = torch.ones(n, device="cuda", dtype=torch.bfloat16)
+    y = ops.dropout_add(one, None, 0.5, torch.tensor([11, 12], device="cuda"))
+    first = (1 << 31) - 64  # a multiple of 8: block 2^28 - 8 on
+    halves = orc.philox_halves(64 + 29, 11, 12, first // 8)
+    assert torch.equal(y[first:].float().cpu(), torch.tensor(np.where(halves >= 32768, 2.0, 0.0), dtype=torch.float32))
+
+
 def test_same_inputs_same_bits(ops):
     f, x, dy = (make((2, 1500, 64), "bfloat16", i) for i in (1, 2, 3))
     xw, wg, wu, dw = (make(s, "bfloat16", 4, scale=0.2) for s in ((3000, 64), (128, 64), (128, 64), (3000, 128)))
