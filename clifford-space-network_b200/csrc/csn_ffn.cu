@@ -12,24 +12,24 @@
 //
 // mm_kernel is one persistent kernel for the four products (Mode).  A pair of CTAs on two SMs (cta_group::2) makes a
 // tile of 256 x BN: each loads 128 rows of A and half of B, so a k block of 64 moves 32 KB into an SM for the products
-// that take 48 KB when it works alone; what L2 delivers (about 60 bytes a clock and SM) is what bounds a large product.
-// In each CTA one thread feeds a ring of shared-memory stages by TMA, one of the pair issues tcgen05.mma into one of
-// two accumulators in tensor memory, and for each accumulator eight warps finish it, so that loads, products and both
-// epilogues overlap across tiles (all sixteen on one after the other: R65536 C128 F256 forward 26.6 us against 20.8).  For the gate, BN = 2 FN: CTA 0 loads FN rows of Wg and CTA 1 the same FN rows of Wu
-// as the halves of one operand, so g and u of a place sit in one tensor-memory lane and the gate is a per-lane
-// epilogue.  The transposed products read the same row-major tensors with an MN-major operand: nothing is transposed in
-// memory.
+// that take 48 KB when it works alone.  In each CTA a warp feeds a ring of shared-memory stages by TMA, a warp of the
+// pair issues tcgen05.mma into one of two accumulators in tensor memory, and for each accumulator eight warps finish it,
+// so that loads, products and both epilogues overlap across tiles (all sixteen on one accumulator after the other:
+// R65536 C128 F256 forward 26.6 us against 20.8).  For the gate, BN = 2 FN: CTA 0 loads FN rows of Wg and CTA 1 the same
+// FN rows of Wu as the halves of one operand, so g and u of a place sit in one tensor-memory lane and the gate is a
+// per-lane epilogue.  The transposed products read the same row-major tensors with an MN-major operand: nothing is
+// transposed in memory.
 //
-// What bounds it, bf16 on a B200: R2048 C4096 F8192 forward 174 us, 1.58 PFLOP/s, 0.94 of what the library's product
-// of 8192^3 reaches; training R8192 C4096 F8192 2.7 ms, 1.2 PFLOP/s of the 12 R C F that it cannot do without, under the
-// power cap.  With few channels the epilogue does: two MUFU operations and about 35 instructions an element of the gate,
-// R65536 C128 F256 forward 21 us against 7.7 us for its bytes.  Rows that start on 16 but not on 128 bytes cost the
-// loads a third (R1021 C1032 F2744 22 us, R1024 C1024 F2752 16).
+// What bounds it, bf16 on a B200: large products the tensor pipe, 94 to 98 % active.  R2048 C4096 F8192 forward 174 us,
+// 1.58 PFLOP/s, 0.94 of what the library's product of 8192^3 reaches; training R8192 C4096 F8192 2.75 ms, 1.2 PFLOP/s of
+// the 12 R C F that it cannot do without, under the power cap.  With few channels the gate's epilogue does, two MUFU
+// operations and about 35 instructions an element: R65536 C128 F256 forward 22 us against 7.7 us for its bytes.  Rows
+// that start on 16 but not on 128 bytes cost the loads a third (R1021 C1032 F2744 22 us, R1024 C1024 F2752 16).
 //
 // few_rows_kernel takes R <= 64 rows (generation): there the weights are what is read, so they take the 128-row side
 // of the product (64 rows of Wg and 64 of Wu) and x the narrow side, and a cluster splits C where F alone gives too
-// few CTAs, its partial sums joined through distributed shared memory in a fixed order.
-#include <atomic>
+// few CTAs, its partial sums joined through distributed shared memory in a fixed order.  Bound by the weights' bytes and
+// by the start and end of a short kernel: R4 C2048 F8192 15 us of 10.3 with the weights in HBM, R2 C256 F512 4.3 us.
 #include <cstdint>
 
 #include "csn_internal.h"

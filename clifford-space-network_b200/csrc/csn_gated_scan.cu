@@ -14,9 +14,9 @@
 // Sequences of at most 32 steps need fewer warps than a CTA has: it then takes 2, 4 or 8 of them.
 //
 // Where there are too few sequences and channels to fill the GPU, sequences are cut into chunks: reduce_kernel composes
-// the map of every chunk that another follows (it reads f and x once more, mostly from L2), and the CTA of a chunk
-// composes those before it into the state that enters it.  All sums, products and states are float32 and in an order
-// that the sizes alone fix.
+// the map of every chunk that another follows (it reads f and x once more, which the scan then finds in L2 where they
+// fit), and the CTA of a chunk composes those before it into the state that enters it.  All sums, products and states
+// are float32 and in an order that the sizes alone fix.
 //
 // What bounds it: issue and the latency of a pass, not memory.  An element costs about 37 instructions forward (two of
 // them on the MUFU for the decay, two for the gate) and 70 back, and with 256 to 444 CTAs of 8 warps the SMs issue 2 to
