@@ -819,6 +819,13 @@ void launch_step(StepArgs A, int64_t B, cudaStream_t st) {
   if (A.g) gated_step_kernel<T, V, true><<<grid, 256, 0, st>>>(A);
   else gated_step_kernel<T, V, false><<<grid, 256, 0, st>>>(A);
 }
+
+// whether the bytes of B rows of C elements at p reach into h
+bool shares(const StepArgs& A, const void* p, int64_t row, int64_t B, int size) {
+  if (!p) return false;
+  const intptr_t first = reinterpret_cast<intptr_t>(p), last = first + (B - 1) * row * size, h = reinterpret_cast<intptr_t>(A.h);
+  return (first < last ? first : last) < h + B * A.C * 4 && h < (first < last ? last : first) + A.C * size;
+}
 }  // namespace
 }  // namespace csn
 
@@ -832,6 +839,8 @@ extern "C" int csn_gated_step(const void* f, const void* x, const void* gate, co
       !aligned(h, 16) || !aligned(y, 16))
     return set_error(CSN_ERR_INVALID, "csn_gated_step: missing or misaligned pointer");
   StepArgs A = {f, x, gate, strides[0], strides[1], gate ? strides[2] : 0, h, y, 0, C};
+  if (shares(A, f, A.fr, B, size) || shares(A, x, A.xr, B, size) || shares(A, gate, A.gr, B, size) || shares(A, y, C, B, size))
+    return set_error(CSN_ERR_INVALID, "csn_gated_step: h shares memory with an input or the result");
   const bool two = C % 2 == 0 && strides[0] % 2 == 0 && strides[1] % 2 == 0 && A.gr % 2 == 0 && aligned(f, 4) &&
                    aligned(x, 4) && aligned(gate, 4);
   cudaStream_t st = static_cast<cudaStream_t>(stream);

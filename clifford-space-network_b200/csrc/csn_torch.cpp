@@ -215,10 +215,10 @@ Tensor gated_step(const Tensor& f_, const Tensor& x_, const Tensor& h, const May
   const c10::cuda::CUDAGuard guard(f_.device());
   const Tensor f = rows(f_), x = rows(x_), gate = rows(gate_);
   Tensor y = room(f, f.sizes());
+  h.unsafeGetTensorImpl()->bump_version();  // first: it raises where h may not be changed
   const int64_t st[3] = {f.stride(0), x.stride(0), gate.defined() ? gate.stride(0) : 0};
   check("csn_gated_step", csn_gated_step(ptr(f), ptr(x), ptr(gate), st, static_cast<float*>(ptr(h)), ptr(y), f.size(0), f.size(1),
                                          code_of(f.scalar_type()), stream(f)));
-  h.unsafeGetTensorImpl()->bump_version();
   return y;
 }
 

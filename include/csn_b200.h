@@ -437,7 +437,7 @@ int csn_gated_scan_bwd(const void* f, const void* x, const void* gate, const voi
                        size_t workspace_bytes, void* stream);
 
 /* One step of the same recurrence for B streams, h [B, C] in place (as csn_rotor_step):
- * f, x, gate element (b, c) at ptr + b * strides[i] + c; y [B, C]. */
+ * f, x, gate element (b, c) at ptr + b * strides[i] + c; y [B, C].  h shares no memory with them. */
 int csn_gated_step(const void* f, const void* x, const void* gate, const int64_t* strides, float* h,
                    void* y, int64_t B, int64_t C, int dtype, void* stream);
 

@@ -146,6 +146,11 @@ def test_step_refuses(lib):
     refused(lib, step(h=NULL), 1, "missing")
     refused(lib, step(h=fake(4)), 1, "misaligned")
     refused(lib, step(f=fake(1)), 1, "misaligned")
+    # a state that shares memory with what the step reads beside it (the first row, the last) or with its result
+    refused(lib, step(f=fake(1 << 20), h=p, y=fake(2 << 20)), 1, "shares memory")
+    refused(lib, lib.csn_gated_step(fake(1 << 20), p, NULL, (ctypes.c_int64 * 3)(64, 8, 0), fake((1 << 20) + 128), fake(2 << 20),
+                                    2, 8, 1, NULL), 1, "shares memory")
+    refused(lib, step(f=fake(1 << 20), h=fake(2 << 20), y=fake(2 << 20)), 1, "shares memory")
     assert step(B=0) == 0
 
 
