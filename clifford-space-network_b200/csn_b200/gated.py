@@ -77,6 +77,6 @@ def dropout_add(x, residual, p: float, rng):
     alone).  rng: int64 [2] on the device, (seed, offset): the mask is a function of these and of the
     place alone (Philox4x32-10, see csn_dropout_add in include/csn_b200.h), so equal numbers give equal
     masks and a captured graph draws a new one when the numbers are changed between replays
-    (csn_b200.modules.DropoutAdd counts for itself).  p is taken in steps of 2^-16 and kept places
+    (csn_b200.modules.DropoutAdd draws them itself).  p is taken in steps of 2^-16 and kept places
     are scaled by one over the probability of being kept."""
     return (_module or _ext()).dropout_add(x, residual, p, rng)

@@ -58,25 +58,26 @@ def generator_inputs(x: torch.Tensor, biv_proj: nn.Linear, gamma_proj: nn.Linear
 # ------------------------------------------------------------- gated recurrent block
 class DropoutAdd(nn.Module):
     """residual + dropout(x, p) in training, residual + x otherwise (residual None: without it), by
-    ops.dropout_add.  The buffer ``rng`` holds (seed, number of calls made): every call in training
-    draws with a copy of it and counts it up on the device, so each call of a captured training step
-    draws a new mask at every replay, the backward pass finds the numbers of its own call, and a saved
-    state_dict goes on where it stopped.  Drawn from torch's CPU generator, the seed follows
-    torch.manual_seed.  A forward pass that is run again (activation checkpointing) draws again."""
+    ops.dropout_add.  Each call in training draws its (seed, offset) from torch's generator of x's
+    device, as nn.Dropout draws its mask: it follows torch.manual_seed, a captured training step draws
+    a new mask at every replay, and a forward pass that is run again for activation checkpointing,
+    which puts the generator back first, has the mask of the first run."""
 
     def __init__(self, p: float = 0.1):
         super().__init__()
         if not 0.0 <= p <= 1.0:
             raise ValueError(f"DropoutAdd: 0 <= p <= 1 expected, got {p}")
         self.p = p
-        self.register_buffer("rng", torch.stack([torch.randint(0, 1 << 62, ()), torch.zeros((), dtype=torch.int64)]))
+
+    @staticmethod
+    def numbers(device) -> torch.Tensor:
+        """(seed, offset) of a call, from the device's generator."""
+        return torch.randint(1 << 62, (2,), device=device)
 
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         if not self.training or self.p == 0.0:
             return x if residual is None else residual + x
-        numbers = self.rng.clone()
-        self.rng[1:].add_(1)
-        return ops.dropout_add(x, residual, self.p, numbers)
+        return ops.dropout_add(x, residual, self.p, self.numbers(x.device))
 
 
 class GatedRecurrence(nn.Module):

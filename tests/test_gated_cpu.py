@@ -257,7 +257,9 @@ def test_dropout_seed_follows_the_generator():
     import torch
     from csn_b200.modules import DropoutAdd
     torch.manual_seed(5)
-    a = DropoutAdd(0.1).rng
+    drop = DropoutAdd(0.1)
+    a, b = drop.numbers("cpu"), drop.numbers("cpu")
+    assert a.dtype == torch.int64 and a.shape == (2,) and a[0] != b[0] and a[1] != b[1]
     torch.manual_seed(5)
-    assert torch.equal(a, DropoutAdd(0.1).rng) and int(a[1]) == 0
-    assert not torch.equal(a, DropoutAdd(0.1).rng)
+    assert torch.equal(a, drop.numbers("cpu")) and torch.equal(b, DropoutAdd(0.1).numbers("cpu"))
+    assert not drop.state_dict()  # nothing that copies of a layer, or the ranks of a job, would share

@@ -24,7 +24,8 @@ def build(d, f, p, dtype, seed=0):
 
 
 def written_out(blk, x, h0, borders):
-    """The block in float64 with torch's elementary operations and autograd: (out, states, parameters)."""
+    """The block in float64 with torch's elementary operations and autograd: (out, states, parameters).
+    Masks are drawn from where the generator stands."""
     P = {k: v.detach().double().requires_grad_(True) for k, v in blk.named_parameters()}
     norm = lambda v, n: ((v - v.mean(-1, keepdim=True)) / (v.var(-1, unbiased=False, keepdim=True) + 1e-5).sqrt()  # noqa: E731
                          * P[n + ".weight"] + P[n + ".bias"])
@@ -32,9 +33,9 @@ def written_out(blk, x, h0, borders):
     def dropped(v, drop):
         if not drop.training or drop.p == 0:
             return v
-        seed, offset = drop.rng.tolist()
+        seed, offset = drop.numbers(v.device).tolist()
         cut = round(drop.p * 65536)
-        keep = orc.philox_halves(v.numel(), seed, offset - 1) >= cut  # the call before counted up
+        keep = orc.philox_halves(v.numel(), seed, offset) >= cut
         return v * torch.tensor(keep, device=v.device).reshape(v.shape) * (65536 / (65536 - cut))
 
     rows = norm(x, "ln_1") @ P["mixer.in_proj.weight"].t() + P["mixer.in_proj.bias"]
@@ -74,7 +75,9 @@ def test_training_pass(dtype, p, packed):
     x = torch.randn(*shape, generator=g).to(dtype).cuda().requires_grad_(True)
     h0 = torch.randn(len(borders), d, generator=g).cuda().requires_grad_(True)
     dout, dh = torch.randn(*shape, generator=g).cuda(), torch.randn(len(borders), d, generator=g).cuda()
+    state = torch.cuda.get_rng_state()
     out, h = blk(x, h0, cu)
+    torch.cuda.set_rng_state(state)
     ((out.float() * dout).sum() + (h * dh).sum()).backward()
     x64, h64 = x.detach().double().reshape(-1, d).requires_grad_(True), h0.detach().double().requires_grad_(True)
     want, wh, P = written_out(blk, x64, h64, borders)
@@ -118,16 +121,14 @@ def test_captured_training_step_draws_new_masks():
     x, y = (torch.randn(B, T, d, generator=torch.Generator().manual_seed(i)).cuda() for i in (4, 5))
     loss = lambda out: ((out[0] - y) ** 2).mean()  # noqa: E731
     step = graphs.TrainStepGraph(blk, None, [x], loss_fn=loss)
-    before = blk.drop_1.rng.clone(), blk.drop_2.rng.clone()
+    state = torch.cuda.get_rng_state()
     outs, grads = [], []
     for _ in range(3):
         outs.append(step(x)[0].clone())
         grads.append([v.grad.clone() for v in blk.parameters()])
-    assert int(blk.drop_1.rng[1] - before[0][1]) == 3
     assert not torch.equal(outs[0], outs[1]) and not torch.equal(outs[1], outs[2])
     del step
-    blk.drop_1.rng.copy_(before[0])
-    blk.drop_2.rng.copy_(before[1])
+    torch.cuda.set_rng_state(state)
     for out, gr in zip(outs, grads):
         blk.zero_grad(set_to_none=True)
         o, _ = blk(x)
@@ -135,6 +136,44 @@ def test_captured_training_step_draws_new_masks():
         assert far(out, o.detach().double()) < 1e-5
         for a, v in zip(gr, blk.parameters()):
             assert far(a, v.grad.double()) < 1e-4
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_checkpointed_pass_keeps_its_masks(reentrant):
+    """A forward pass that is run again in the backward pass has the same masks: the same bits throughout."""
+    from torch.utils.checkpoint import checkpoint
+    blk = build(32, 72, 0.25, torch.bfloat16)
+    x = torch.randn(2, 40, 32, generator=torch.Generator().manual_seed(8)).bfloat16().cuda().requires_grad_(True)
+    leaves = [x, *blk.parameters()]
+    state = torch.cuda.get_rng_state()
+    got = []
+    for run in (lambda: blk(x), lambda: checkpoint(blk, x, use_reentrant=reentrant)):
+        torch.cuda.set_rng_state(state)
+        for v in leaves:
+            v.grad = None
+        out, h = run()
+        (out.float().square().sum() + h.sum()).backward()
+        got.append([out.detach(), *(v.grad for v in leaves)])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_copied_layers_draw_their_own_masks():
+    import copy
+    from csn_b200.modules import DropoutAdd
+    a = DropoutAdd(0.5)
+    x = torch.ones(4096, device="cuda")
+    assert not torch.equal(a(x), copy.deepcopy(a)(x))
+
+
+def test_generation_under_inference_mode():
+    blk = build(32, 72, 0.0, torch.bfloat16).eval()
+    x = torch.randn(3, 32, generator=torch.Generator().manual_seed(9)).bfloat16().cuda()
+    outs = []
+    for mode in (torch.no_grad, torch.inference_mode):
+        with mode():
+            h = blk.init_state(3)
+            outs.append((blk.step(x, h), h))
+    assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
 
 
 def test_registered_operators_and_their_gradients():
