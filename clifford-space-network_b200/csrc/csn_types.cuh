@@ -103,15 +103,18 @@ __device__ __forceinline__ float inverse_fast(float x) {
 }
 constexpr float LOG2E = 1.4426950408889634f;
 
-// q = sigmoid(-z) = 1 / (1 + exp(z)), off by a few units of its own (and 2 |z| 2^-24 relative, since the exponential's
-// argument is rounded), and a = 1 - q, rounded once.  So a near 1 has the rounding of a float32 number, without a
-// drift, and a near 0 is off by 2^-25: what a h loses by it is half a unit of h.  exp(z) too large for float32: q = 0.
+// a = sigmoid(z) and q = sigmoid(-z) = 1 / (1 + e) with e = exp(z), which is off by a few units of its own and, since its
+// argument is rounded, 2 |z| 2^-24 relative.  The smaller of the two takes that error relative to itself: q as it is, and
+// for z < 0 a = e q, so that what a closed gate leaves of a state and its gradients keep their precision (1 - q would
+// be off by 2^-25 whatever a is, and 0 from z = -17 on).  For z >= 0 a = 1 - q, rounded once: the long memory of a near 1
+// decays without a drift.  exp(z) too large for float32: q = 0, a = 1.
 template <int V>
 __device__ __forceinline__ void sigmoid_pair(Vals<V> z, Vals<V>& a, Vals<V>& q) {
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    q.v[i] = inverse_fast(1.0f + exp2_fast(LOG2E * z.v[i]));
-    a.v[i] = 1.0f - q.v[i];
+    const float e = exp2_fast(LOG2E * z.v[i]);
+    q.v[i] = inverse_fast(1.0f + e);
+    a.v[i] = e < 1.0f ? e * q.v[i] : 1.0f - q.v[i];
   }
 }
 

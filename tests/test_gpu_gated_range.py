@@ -1,0 +1,147 @@
+"""The gated block's operators over the whole range of what enters them, against 64-bit forms whose bounds are relative
+to what an output is made of: forget gates that close."""
+import numpy as np
+import pytest
+import torch
+
+import gated_oracle as orc
+
+pytestmark = pytest.mark.gpu
+TYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "float16": torch.float16}
+U = orc.U
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from csn_b200 import ops
+    return ops
+
+
+def to64(t):
+    return t.detach().double().cpu().numpy()
+
+
+def rand(shape, kind, seed, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * scale).to(TYPES[kind]).cuda()
+
+
+def check(got, want, kind, what):
+    used = orc.within(to64(got), want[0], want[1], kind)
+    assert used <= 1.0, f"{what}: {used:.2f} of the allowed error"
+
+
+# ------------------------------------------------------------------------ the scan
+# With e = exp(f), off by (4 + 2 |f|) U of itself (two steps of the fast exponential, and its rounded argument):
+# q = 1 / (1 + e) is off by that share of e q = a, by the sum's rounding (1 U) and the reciprocal's (4 U); for f < 0
+# a = e q is off by (4 + 2 |f|) U (its share of e, the smaller one of q included twice at most: 2 (4 + 2 |f|)), 5 U and its own
+# rounding, so by less than (16 + 4 |f|) U of itself; for f >= 0 a = 1 - q by q's error and one rounding of a number
+# in [1/2, 1], U.  The states are sums of terms, each a product along its way; `size` is the sum of the terms' sizes.  A
+# step multiplies a term by a (its error, and 1 U for the product) and rounds a sum (1 U of its size); composing steps first
+# and applying the maps after that rounds as many products and sums along any way, and one product and one sum more for
+# each of the up to three levels (steps of a warp, warps of a pass, chunks), so 4 U a step and 16 U at the end
+# cover any order.  A product of decays that falls below 2^-126 loses bits: SMALL of what it multiplies.
+SMALL = 2.0 ** -120
+
+
+def closed_scan(f, x, h0, gate, borders, dy, dh):
+    L, C = f.shape
+    a, q = orc.sigmoid(f), orc.sigmoid(-f)
+    rel = (16 + 4 * np.abs(f)) * U
+    a_off = np.where(f < 0, rel * a, rel * q + U)
+    q_off = rel * np.minimum(a, q) + 6 * U * q
+    w = orc.sigmoid(gate) if gate is not None else None
+    silu = gate * w if gate is not None else np.ones_like(f)
+    fast = (16 + 2 * np.abs(gate)) * U if gate is not None else 0.0
+    silu_off = fast * np.abs(silu)
+
+    def run(order, start, add, add_off):
+        """s_t = a_t s_{t-1} + add_t along `order`: (before, its error, its size) at each row, and those at the end."""
+        s, off, size = start.copy(), np.zeros(C), np.abs(start)
+        for t in order:
+            yield t, s, off + (16 * U + SMALL) * size, size
+            off = a[t] * off + (a_off[t] + 4 * U * a[t]) * size + add_off[t] + 4 * U * np.abs(add[t])
+            s, size = a[t] * s + add[t], a[t] * size + np.abs(add[t])
+        yield None, s, off + (16 * U + SMALL) * size, size
+
+    zero = lambda: np.zeros((L, C))  # noqa: E731
+    before, before_off, h, h_off = zero(), zero(), zero(), zero()
+    last, last_off = np.zeros_like(h0), np.zeros_like(h0)
+    for s, (b, e) in enumerate(borders):
+        seen = list(run(range(b, e), h0[s], q * x, q_off * np.abs(x) + U * np.abs(q * x)))
+        for (t, v, off, _), (_, v1, off1, _) in zip(seen, seen[1:]):
+            before[t], before_off[t], h[t], h_off[t] = v, off, v1, off1
+        last[s], last_off[s] = seen[-1][1:3]
+    out = {"y": (h * silu, h_off * np.abs(silu) + np.abs(h) * silu_off + 2 * U * np.abs(h * silu)), "h": (last, last_off)}
+    # lam_t = e_t + mu_t with mu_{t-1} = a_t lam_t: the same recurrence with a_t (e_t + mu_t)
+    e_t = dy * silu
+    e_off = np.abs(dy) * silu_off + 2 * U * np.abs(e_t)
+    lam, lam_off = zero(), zero()
+    dh0, dh0_off = np.zeros_like(h0), np.zeros_like(h0)
+    for s, (b, e) in enumerate(borders):
+        add = a * e_t
+        add_off = a_off * np.abs(e_t) + a * e_off + U * np.abs(add)
+        for t, mu, off, size in run(range(e - 1, b - 1, -1), dh[s], add, add_off):
+            if t is None:
+                dh0[s], dh0_off[s] = mu, off
+            else:
+                lam[t], lam_off[t] = e_t[t] + mu, e_off[t] + off + U * (np.abs(e_t[t]) + size)
+    D = before - x
+    D_off = before_off + U * np.abs(D)
+    df = lam * D * a * q
+    out["dx"] = (lam * q, q * lam_off + (q_off + 2 * U * q) * np.abs(lam))
+    out["df"] = (df, a * q * (np.abs(lam) * D_off + np.abs(D) * lam_off + lam_off * D_off)
+                 + (a_off * q + a * q_off) * np.abs(lam * D) + 6 * U * np.abs(df))
+    out["dh0"] = (dh0, dh0_off)
+    if gate is not None:
+        slope = w * (1 + gate * (1 - w))
+        slope_off = w * (fast * np.abs(gate) + 2 * fast * (1 + np.abs(gate) * (1 - w)))
+        out["dgate"] = (dy * h * slope, np.abs(dy) * (h_off * np.abs(slope) + np.abs(h) * slope_off + 3 * U * np.abs(h * slope)))
+    return out
+
+
+def closing(T, C, kind, seed):
+    """Forget logits from -30 to 30 in every row, and channels that stay at one of them."""
+    g = torch.Generator().manual_seed(seed)
+    f = torch.rand(T, C, generator=g) * 60 - 30
+    for i, v in enumerate((-8.0, -12.0, -15.0, -18.0, -25.0, 12.0)):
+        if i < C:
+            f[:, i] = v
+    return f.to(TYPES[kind]).cuda()
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("S,T,C,gated", [(3, 1, 8, False), (2, 5, 33, True), (2, 70, 40, True), (1, 130, 31, False), (1, 700, 24, True)])
+def test_scan_of_gates_that_close(ops, kind, S, T, C, gated):
+    """The decay of a closed gate keeps its own precision, and with it what is left of a large state and the gradients
+    of the logits and of the first state: one row, warps that share a CTA, several passes, chunks."""
+    f = closing(S * T, C, kind, 1)
+    x, dy = rand((S * T, C), kind, 2), rand((S * T, C), kind, 3)
+    gate = rand((S * T, C), kind, 4) if gated else None
+    h0, dh = rand((S, C), "float32", 5, scale=1e4), rand((S, C), "float32", 6)
+    want = closed_scan(*(to64(t) for t in (f, x, h0)), None if gate is None else to64(gate), [(s * T, s * T + T) for s in range(S)],
+                       to64(dy), to64(dh))
+    args = {"f": f, "x": x, "gate": gate}
+    for packed in (False, True):
+        leaves = {k: (t if packed else t.view(S, T, C)).detach().requires_grad_(True) for k, t in args.items() if t is not None}
+        leaves["h0"] = h0.detach().requires_grad_(True)
+        cu = torch.arange(0, S * T + 1, T, device="cuda", dtype=torch.int32) if packed else None
+        y, h = ops.gated_scan(leaves["f"], leaves["x"], h0=leaves["h0"], gate=leaves.get("gate"), cu_seqlens=cu)
+        grads = dict(zip(leaves, torch.autograd.grad((y, h), list(leaves.values()), (dy.view(y.shape), dh))))
+        check(y.reshape(-1, C), want["y"], kind, "y")
+        check(h, want["h"], "float32", "h")
+        for name, key in (("f", "df"), ("x", "dx"), ("gate", "dgate"), ("h0", "dh0")):
+            if name in grads:
+                check(grads[name].reshape(-1, C), want[key], "float32" if name == "h0" else kind, key)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_step_of_gates_that_close(ops, kind):
+    """What a closed gate leaves of a state far larger than its input."""
+    B, C = 5, 48
+    f, x, gate = closing(B, C, kind, 1), rand((B, C), kind, 2, scale=1e-3), rand((B, C), kind, 3)
+    h = rand((B, C), "float32", 4, scale=1e4)
+    want = closed_scan(*(to64(t) for t in (f, x, h)), to64(gate), [(b, b + 1) for b in range(B)], np.zeros((B, C)), np.zeros((B, C)))
+    y = ops.gated_step(f, x, h, gate=gate)
+    check(y, want["y"], kind, "y")
+    check(h, want["h"], "float32", "h")
