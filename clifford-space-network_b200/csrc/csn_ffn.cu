@@ -7,8 +7,11 @@
 // them costs 8 bytes an element written and read, forming them 4 C operations: at 6.5 TB/s and 1.4 PFLOP/s the two are
 // even near C = 1000, and the caller decides (rounded to 16 bits they would cost a third of the gradients' precision).
 // dg and du are rounded to the tensors' own type once, as the operands of the products that follow.  In float16,
-// whose smallest number is 2^-24, they are first scaled by the power of two that brings the largest |dy| into [1, 2),
-// and the products are scaled back in float32.
+// whose numbers end at 65504 and lose bits below 2^-14, they are first scaled by the power of two that brings the largest
+// finite |dy| into [2^10, 2^11), and the products are scaled back in float32.  So a row whose dy is 2^-24 of the largest
+// keeps its precision, and |dg / dy| and |du / dy| up to 32 fit.  The pass also notes the largest |dg| and |du|: where they do
+// not fit after all, it runs again with the scale that brings these into [2^14, 2^15).  This second pass is launched each
+// time, while the first runs, and ends at once where they do fit: at most 2 us (after the first: 6 to 8).
 //
 // mm_kernel is one persistent kernel for the four products (Mode).  A pair of CTAs on two SMs (cta_group::2) makes a
 // tile of 256 x BN: each loads 128 rows of A and half of B, so a k block of 64 moves 32 KB into an SM for the products
@@ -71,19 +74,39 @@ struct Args {
   int64_t ldy;
   float* part;        // splits > 1: [splits][halves_m][m][n]
   float* pre;         // GATE: g and u are kept here, [2][m][n]
-  const uint32_t* amax;  // float16 backward: bits of the largest |dy|
+  uint32_t* range;  // float16 backward: what scales dg and du
+  bool again;       // GATE_BWD: the pass that runs where the first scale was too large
 };
 
-// the power of two that brings amax into [1, 2), and its inverse; 1 where there is no such
-__device__ __forceinline__ float scale_up(const uint32_t* amax) {
-  if (!amax) return 1.0f;
-  const uint32_t b = *amax;
-  return b == 0 || b >= 0x7f800000u ? 1.0f : __uint_as_float((254u - (b >> 23)) << 23);
+// The scale of float16's dg and du.  range[0]: bits of the largest finite |dy|, range[1]: of the largest finite |dg| or
+// |du| under the first scale.
+constexpr uint32_t HALF_MAX = 0x477fe000;  // bits of 65504
+
+__device__ __forceinline__ bool too_large(const uint32_t* range) { return range[1] > HALF_MAX; }
+// its exponent as a float32 has it, and that of its inverse is 254 less this: |dy| is 0 or 2^-24 to 2^16, so the first is
+// 122 to 161, and the second 9 at least.
+__device__ __forceinline__ uint32_t scale_exponent(const uint32_t* range, bool again) {
+  if (range[0] == 0) return 127;
+  const uint32_t first = 127 + 10 + 127 - (range[0] >> 23);
+  return again ? first + 14 + 127 - (range[1] >> 23) : first;
 }
-__device__ __forceinline__ float scale_down(const uint32_t* amax) {
-  if (!amax) return 1.0f;
-  const uint32_t b = *amax;
-  return b == 0 || b >= 0x7f800000u ? 1.0f : __uint_as_float((b >> 23) << 23);
+// for dg and du
+__device__ __forceinline__ float scale_up(const uint32_t* range, bool again) {
+  return range ? __uint_as_float(scale_exponent(range, again) << 23) : 1.0f;
+}
+// for the products of dg and du
+__device__ __forceinline__ float scale_down(const uint32_t* range) {
+  return range ? __uint_as_float((254 - scale_exponent(range, too_large(range))) << 23) : 1.0f;
+}
+// the larger of `top` and what is finite of the larger of |a| and |b| (a NaN counts as nothing)
+__device__ __forceinline__ float finite_max(float top, float a, float b) {
+  const float m = fmaxf(fabsf(a), fabsf(b));
+  return fmaxf(top, m < __int_as_float(0x7f800000) ? m : 0.0f);
+}
+// a warp's maximum into the bits of *to: a maximum does not depend on the order
+__device__ __forceinline__ void note_max(uint32_t* to, float top) {
+  const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+  if ((threadIdx.x & 31) == 0) atomicMax(to, bits);
 }
 
 template <bool BF16>
@@ -182,6 +205,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = (int)cluster_rank();
   const int tiles = P.mt * P.nt * P.halves_m * P.splits, first = blockIdx.x / 2, step = gridDim.x / 2;
+  constexpr bool SCALED = MODE == GATE_BWD && !BF16;
+  if (SCALED && P.again) {  // launched early (programmatic dependent launch): what the first pass leaves is awaited
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (!too_large(P.range)) return;
+  } else if (SCALED) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  }
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < ST; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
@@ -278,8 +308,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     char* stage = smem + ST * SB + warp * 32 * STAGE_ROW;
     char* own = stage + lane * STAGE_ROW;
     const int acc = warp / 8, quarter = warp % 4, side = warp / 4 % 2;
-    const float up = MODE == GATE_BWD ? scale_up(P.amax) : 1.0f;
-    const float down = MODE == DX || MODE == DW ? scale_down(P.amax) : 1.0f;
+    const float up = SCALED ? scale_up(P.range, P.again) : 1.0f;
+    const float down = (MODE == DX || MODE == DW) && !BF16 ? scale_down(P.range) : 1.0f;
+    float top = 0.0f;  // SCALED: the largest finite |dg| and |du|
     const uint32_t d = tmem + acc * BN + ((uint32_t)(quarter * 32) << 16), release = peer_addr(&acc_empty[acc], 0);
     const bool vec = (MODE == DX || MODE == DW) && P.splits > 1 ? P.n % 4 == 0 : P.ldo % 8 == 0;
     const bool vec_dy = MODE == GATE_BWD && P.ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(P.dy) & 15) == 0 && P.n % 8 == 0;
@@ -325,6 +356,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                   const float e = (j ? dv.y : dv.x) * up;
                   r0[j] = e * uv * (w * fmaf(gv, 1.0f - w, 1.0f));
                   r1[j] = e * gv * w;
+                  if (SCALED) top = finite_max(top, r0[j], r1[j]);
                 }
               }
               if (MODE == GATE_BWD) {
@@ -384,6 +416,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(release);
     }
+    if (SCALED && !P.again) note_max(&P.range[1], top);
   }
   fence_before();
   __syncthreads();
@@ -395,8 +428,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 // Sums of the k ranges, in their order: element i of half h is out[h][i].
 template <bool BF16>
 __global__ void __launch_bounds__(128) join_kernel(const float* __restrict__ part, void* out0, void* out1, int64_t n,
-                                                   int halves, int splits, const uint32_t* amax) {
-  const float down = scale_down(amax);
+                                                   int halves, int splits, const uint32_t* range) {
+  const float down = BF16 ? 1.0f : scale_down(range);
   const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x, stride = n * halves;
   if (i >= stride) return;
   const bool second = i >= n;
@@ -416,9 +449,11 @@ __global__ void __launch_bounds__(128) join_kernel(const float* __restrict__ par
 template <bool BF16, bool VEC>
 __global__ void __launch_bounds__(256) gate_back_kernel(const float* __restrict__ pre, const uint16_t* __restrict__ dy, int64_t ldy,
                                                         uint16_t* dg, uint16_t* du, int64_t ld, int64_t R, int64_t F,
-                                                        const uint32_t* amax) {
+                                                        uint32_t* range, bool again) {
   constexpr int N = VEC ? 8 : 1;
-  const float up = scale_up(amax);
+  if (!BF16 && again && !too_large(range)) return;
+  const float up = BF16 ? 1.0f : scale_up(range, again);
+  float top = 0.0f;  // float16: the largest finite |dg| and |du|
   const int64_t per = F / N, n = R * per;
   for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
     const int64_t r = i / per, c = (i - r * per) * N;
@@ -446,6 +481,7 @@ __global__ void __launch_bounds__(256) gate_back_kernel(const float* __restrict_
       const float w = sigmoid(g[j]), e = d[j] * up;
       a[j] = e * u[j] * (w * fmaf(g[j], 1.0f - w, 1.0f));
       b[j] = e * g[j] * w;
+      if (!BF16) top = finite_max(top, a[j], b[j]);
     }
     if (VEC) {
       *reinterpret_cast<uint4*>(dg + r * ld + c) =
@@ -457,17 +493,30 @@ __global__ void __launch_bounds__(256) gate_back_kernel(const float* __restrict_
       du[r * ld + c] = (uint16_t)pack2<BF16>(b[0], 0.0f);
     }
   }
+  if (!BF16 && !again) note_max(&range[1], top);
 }
 
-// bits of the largest |dy| (0 before): a maximum does not depend on the order
-__global__ void __launch_bounds__(256) amax_kernel(const __half* __restrict__ dy, int64_t ld, int64_t R, int64_t F,
-                                                   uint32_t* amax) {
-  float m = 0.0f;
-  for (int64_t r = blockIdx.x; r < R; r += gridDim.x)
-    for (int64_t c = threadIdx.x; c < F; c += 256) m = fmaxf(m, fabsf(__half2float(dy[r * ld + c])));
+// range[0] (0 before): bits of the largest finite |dy|.  A thread has 8 neighbouring elements of a row; `vec`: in one access.
+__global__ void __launch_bounds__(256) amax_kernel(const __half* __restrict__ dy, int64_t ld, int64_t R, int64_t F, bool vec,
+                                                   uint32_t* range) {
+  float top = 0.0f;
+  const int64_t per = (F + 7) / 8, n = R * per;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / per, c = (i - r * per) * 8;
+    const __half* p = dy + r * ld + c;
+    if (vec) {
+      const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if ((threadIdx.x & 31) == 0) atomicMax(amax, __float_as_uint(m));
+      for (int j = 0; j < 4; ++j) {
+        const float2 v = unpack2<false>(w[j]);
+        top = finite_max(top, v.x, v.y);
+      }
+    } else {
+      for (int j = 0; j < 8 && c + j < F; ++j) top = finite_max(top, __half2float(p[j]), 0.0f);
+    }
+  }
+  note_max(range, top);
 }
 
 // ------------------------------------------------------------------------ few rows
@@ -679,10 +728,10 @@ struct Plan {
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // A pass's scratch: padded copies of the operands that need one (bits of `copies`: x, w_gate, w_up), and for the backward
-// pass dg, du [R, ld], the largest |dy|, and the partial sums of split products.
+// pass dg, du [R, ld], the scale of float16 ones, and the partial sums of split products.
 struct Scratch {
   int64_t ld;
-  size_t pad[3], dg, du, amax, part, total;
+  size_t pad[3], dg, du, range, part, total;
   Scratch(int64_t R, int64_t C, int64_t F, int copies, bool bwd) {
     size_t n = 0;
     for (int i = 0; i < 3; ++i) {
@@ -697,8 +746,8 @@ struct Scratch {
     const size_t sw = pw.splits > 1 ? (size_t)pw.splits * 2 * F * C * 4 : 0;
     dg = n;
     du = dg + align256((size_t)R * ld * 2);
-    amax = du + align256((size_t)R * ld * 2);
-    part = amax + 256;
+    range = du + align256((size_t)R * ld * 2);
+    part = range + 256;
     total = part + align256(sx > sw ? sx : sw);
   }
 };
@@ -709,13 +758,23 @@ int run_mm(const Maps& maps, const Args& P, cudaStream_t st, const char* who) {
   const int64_t tiles = (int64_t)P.mt * P.nt * P.halves_m * P.splits;
   const int64_t pairs = sm_count() / 2;
   const unsigned grid = 2 * (unsigned)(tiles < pairs ? tiles : pairs);
-  mm_kernel<MODE, BF16, BN><<<grid, THREADS, smem_bytes(BN), st>>>(maps, P);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem_bytes(BN);
+  cfg.stream = st;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = P.again ? 1 : 0;
+  if (cudaError_t e = cudaLaunchKernelEx(&cfg, mm_kernel<MODE, BF16, BN>, maps, P)) return set_cuda_error(e, who);
   return check_launch(who);
 }
 
 template <bool BF16>
 int run_gate(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void* wu, int64_t ldu, const void* dy,
-             int64_t ldy, void* o0, void* o1, int64_t ldo, float* pre, const uint32_t* amax, int64_t R, int64_t C, int64_t F,
+             int64_t ldy, void* o0, void* o1, int64_t ldo, float* pre, uint32_t* range, int64_t R, int64_t C, int64_t F,
              cudaStream_t st, const char* who) {
   const Plan p(R, F, up(C, BK), 1, true);
   Maps maps;
@@ -725,8 +784,13 @@ int run_gate(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void
   maps.a[1] = maps.a[0];
   Args P = {};
   P.m = (int)R, P.n = (int)F, P.mt = p.mt, P.nt = p.nt, P.kb = (int)up(C, BK), P.halves_m = P.halves_k = 1;
-  P.splits = p.splits, P.kper = p.kper, P.out[0] = o0, P.out[1] = o1, P.ldo = ldo, P.dy = dy, P.ldy = ldy, P.pre = pre, P.amax = amax;
-  if (dy) return p.bn == 256 ? run_mm<GATE_BWD, BF16, 256>(maps, P, st, who) : run_mm<GATE_BWD, BF16, 128>(maps, P, st, who);
+  P.splits = p.splits, P.kper = p.kper, P.out[0] = o0, P.out[1] = o1, P.ldo = ldo, P.dy = dy, P.ldy = ldy, P.pre = pre, P.range = range;
+  if (dy) {
+    int rc = p.bn == 256 ? run_mm<GATE_BWD, BF16, 256>(maps, P, st, who) : run_mm<GATE_BWD, BF16, 128>(maps, P, st, who);
+    P.again = true;
+    if (!BF16 && !rc) rc = p.bn == 256 ? run_mm<GATE_BWD, BF16, 256>(maps, P, st, who) : run_mm<GATE_BWD, BF16, 128>(maps, P, st, who);
+    return rc;
+  }
   return p.bn == 256 ? run_mm<GATE, BF16, 256>(maps, P, st, who) : run_mm<GATE, BF16, 128>(maps, P, st, who);
 }
 
@@ -775,7 +839,7 @@ int run_product(const Maps& maps, Args P, int64_t blocks, const Plan& p, float* 
   int rc = p.bn == 256 ? run_mm<MODE, BF16, 256>(maps, P, st, who) : run_mm<MODE, BF16, 128>(maps, P, st, who);
   if (rc || p.splits == 1) return rc;
   const int64_t n = (int64_t)P.m * P.n;
-  join_kernel<BF16><<<(unsigned)up(n * P.halves_m, 128), 128, 0, st>>>(part, P.out[0], P.out[1], n, P.halves_m, p.splits, P.amax);
+  join_kernel<BF16><<<(unsigned)up(n * P.halves_m, 128), 128, 0, st>>>(part, P.out[0], P.out[1], n, P.halves_m, p.splits, P.range);
   return check_launch(who);
 }
 
@@ -787,22 +851,26 @@ int backward(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void
   char* base = static_cast<char*>(ws);
   void *dg = base + s.dg, *du = base + s.du;
   float* part = reinterpret_cast<float*>(base + s.part);
-  uint32_t* amax = nullptr;
+  uint32_t* range = nullptr;
+  const bool vec = F % 8 == 0 && ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(dy) & 15) == 0;
   if (!BF16) {
-    amax = reinterpret_cast<uint32_t*>(base + s.amax);
-    if (cudaError_t e = cudaMemsetAsync(amax, 0, 4, st)) return set_cuda_error(e, who);
-    amax_kernel<<<(unsigned)(R < 16 * PAIRS ? R : 16 * PAIRS), 256, 0, st>>>(static_cast<const __half*>(dy), ldy, R, F, amax);
+    range = reinterpret_cast<uint32_t*>(base + s.range);
+    if (cudaError_t e = cudaMemsetAsync(range, 0, 8, st)) return set_cuda_error(e, who);
+    const int64_t ctas = up(R * up(F, 8), 256);
+    amax_kernel<<<(unsigned)(ctas < 16 * PAIRS ? ctas : 16 * PAIRS), 256, 0, st>>>(static_cast<const __half*>(dy), ldy, R, F, vec, range);
+    if (int rc = check_launch(who)) return rc;
   }
   if (pre) {
-    const bool vec = F % 8 == 0 && ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(dy) & 15) == 0;
     const int64_t ctas = up(R * (vec ? F / 8 : F), 256);
     const unsigned grid = (unsigned)(ctas < 64 * PAIRS ? ctas : 64 * PAIRS);
     const uint16_t* d = static_cast<const uint16_t*>(dy);
     uint16_t *a = static_cast<uint16_t*>(dg), *b = static_cast<uint16_t*>(du);
-    if (vec) gate_back_kernel<BF16, true><<<grid, 256, 0, st>>>(pre, d, ldy, a, b, s.ld, R, F, amax);
-    else gate_back_kernel<BF16, false><<<grid, 256, 0, st>>>(pre, d, ldy, a, b, s.ld, R, F, amax);
-    if (int rc = check_launch(who)) return rc;
-  } else if (int rc = run_gate<BF16>(x, ldx, wg, ldg, wu, ldu, dy, ldy, dg, du, s.ld, nullptr, amax, R, C, F, st, who)) {
+    for (int again = 0; again < (BF16 ? 1 : 2); ++again) {
+      if (vec) gate_back_kernel<BF16, true><<<grid, 256, 0, st>>>(pre, d, ldy, a, b, s.ld, R, F, range, again != 0);
+      else gate_back_kernel<BF16, false><<<grid, 256, 0, st>>>(pre, d, ldy, a, b, s.ld, R, F, range, again != 0);
+      if (int rc = check_launch(who)) return rc;
+    }
+  } else if (int rc = run_gate<BF16>(x, ldx, wg, ldg, wu, ldu, dy, ldy, dg, du, s.ld, nullptr, range, R, C, F, st, who)) {
     return rc;
   }
   if (dx) {
@@ -812,7 +880,7 @@ int backward(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void
         !make_map(&maps.b[0], wg, F, C, ldg, BK, BF16) || !make_map(&maps.b[1], wu, F, C, ldu, BK, BF16))
       return set_error(CSN_ERR_CUDA, "silu_gated_linear: cuTensorMapEncodeTiled");
     Args P = {};
-    P.m = (int)R, P.n = (int)C, P.halves_m = 1, P.halves_k = 2, P.out[0] = dx, P.ldo = C, P.amax = amax;
+    P.m = (int)R, P.n = (int)C, P.halves_m = 1, P.halves_k = 2, P.out[0] = dx, P.ldo = C, P.range = range;
     if (int rc = run_product<DX, BF16>(maps, P, 2 * up(F, BK), p, part, st, who)) return rc;
   }
   if (dwg || dwu) {
@@ -823,7 +891,7 @@ int backward(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void
       return set_error(CSN_ERR_CUDA, "silu_gated_linear: cuTensorMapEncodeTiled");
     maps.b[1] = maps.b[0];
     Args P = {};
-    P.m = (int)F, P.n = (int)C, P.halves_m = 2, P.halves_k = 1, P.out[0] = dwg, P.out[1] = dwu, P.ldo = C, P.amax = amax;
+    P.m = (int)F, P.n = (int)C, P.halves_m = 2, P.halves_k = 1, P.out[0] = dwg, P.out[1] = dwu, P.ldo = C, P.range = range;
     if (int rc = run_product<DW, BF16>(maps, P, up(R, BK), p, part, st, who)) return rc;
   }
   return CSN_OK;

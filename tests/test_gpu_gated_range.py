@@ -1,5 +1,5 @@
 """The gated block's operators over the whole range of what enters them, against 64-bit forms whose bounds are relative
-to what an output is made of: forget gates that close."""
+to what an output is made of: forget gates that close, float16 gradients of mixed sizes and products near the type's end."""
 import numpy as np
 import pytest
 import torch
@@ -145,3 +145,71 @@ def test_step_of_gates_that_close(ops, kind):
     y = ops.gated_step(f, x, h, gate=gate)
     check(y, want["y"], kind, "y")
     check(h, want["h"], "float32", "h")
+
+
+# ------------------------------------------------------- the gated product in float16
+# dg and du are float16 numbers under one scale that brings the largest finite |dy| to 2^10 or above, or where dg or du would not
+# fit then, the largest of these to 2^14 or above: they keep 2^-11 of themselves, or half of float16's smallest
+# step, 2^-25, over the scale.  With e = exp(-|g|), off by (4 + 2 |g|) U, 1 / (1 + e) is off by that share of e, a
+# sum and a reciprocal (5 U), and sigmoid of a negative number by a share of itself.
+def scaled_ffn(x, wg, wu, dy):
+    C, F, R = x.shape[1], wg.shape[0], x.shape[0]
+    sums = lambda k: (k + 16) * 2 * U  # noqa: E731
+    g, u = x @ wg.T, x @ wu.T
+    g_off, u_off = sums(C) * (np.abs(x) @ np.abs(wg).T), sums(C) * (np.abs(x) @ np.abs(wu).T)
+    w = orc.sigmoid(g)
+    w_rel = (4 + 2 * np.abs(g)) * U * orc.sigmoid(-g) + 8 * U
+    silu, slope = g * w, w * (1 + g * (1 - w))
+    # |silu'| <= 1.1, |silu''| <= 0.5, |g w (1 - w)| <= 0.3, and 1 - w is off by w's error and a rounding
+    silu_off = 1.1 * g_off + (w_rel + U) * np.abs(silu)
+    slope_off = 0.5 * g_off + w_rel * np.abs(slope) + w * (np.abs(g) * (w_rel * w + U) + 3 * U * (1 + np.abs(g) * (1 - w)))
+    dg, du = dy * u * slope, dy * silu
+    dg_off = np.abs(dy) * (u_off * (np.abs(slope) + slope_off) + np.abs(u) * slope_off) + 4 * U * np.abs(dg)
+    du_off = np.abs(dy) * silu_off + 2 * U * np.abs(du)
+    top, peak = np.abs(dy).max(), max(np.abs(dg).max(), np.abs(du).max())
+    floor = 2.0 ** -25 * max(top / 2 ** 10, peak / 2 ** 14)
+    dg_off, du_off = (o + orc.HALF_STEP["float16"] * np.abs(v) + floor for o, v in ((dg_off, dg), (du_off, du)))
+    aw, au, ax = np.abs(wg), np.abs(wu), np.abs(x)
+    return {"dx": (dg @ wg + du @ wu, dg_off @ aw + du_off @ au + sums(2 * F) * (np.abs(dg) @ aw + np.abs(du) @ au)),
+            "dwg": (dg.T @ x, dg_off.T @ ax + sums(R) * (np.abs(dg).T @ ax)),
+            "dwu": (du.T @ x, du_off.T @ ax + sums(R) * (np.abs(du).T @ ax))}
+
+
+def ffn_grads(ops, x, wg, wu, dy):
+    leaves = [t.detach().requires_grad_(True) for t in (x, wg, wu)]
+    return dict(zip(("dx", "dwg", "dwu"), torch.autograd.grad(ops.silu_gated_linear(*leaves), leaves, dy)))
+
+
+# forming the products again, and keeping them (C >= 1536); rows whose tiles are whole or cut, whole pieces or odd
+@pytest.mark.parametrize("R,C,F", [(200, 64, 64), (130, 72, 35), (150, 1536, 40), (70, 1541, 33)])
+@pytest.mark.parametrize("largest", [1e3, 1.0, 1e-3])
+def test_ffn_float16_gradients_of_mixed_sizes(ops, R, C, F, largest):
+    """A row of gradients keeps its precision beside one that is 10^7 times as large."""
+    x, wg, wu = rand((R, C), "float16", 1), rand((F, C), "float16", 2, C ** -0.5), rand((F, C), "float16", 3, C ** -0.5)
+    size = (10.0 ** (-7 * torch.arange(R) / (R - 1))).cuda()[:, None] * largest
+    dy = (rand((R, F), "float32", 4).sign() * size).half()
+    want = scaled_ffn(*(to64(t) for t in (x, wg, wu, dy)))
+    for name, got in ffn_grads(ops, x, wg, wu, dy).items():
+        check(got, want[name], "float16", name)
+    # a gradient that overflowed spoils its own row of dx alone
+    dy[3, 5] = float("inf")
+    dx = ffn_grads(ops, x, wg, wu, dy)["dx"]
+    rest = [r for r in range(R) if r != 3]
+    assert not torch.isfinite(dx[3]).all()
+    some = scaled_ffn(to64(x)[rest], to64(wg), to64(wu), to64(dy)[rest])["dx"]
+    check(dx[rest], some, "float16", "dx beside an infinity")
+
+
+@pytest.mark.parametrize("R,C,F", [(200, 64, 64), (130, 72, 35), (150, 1536, 40), (70, 1541, 33)])
+@pytest.mark.parametrize("large", ["gate", "up"])
+def test_ffn_float16_gradients_of_large_products(ops, R, C, F, large):
+    """Products near 10^5, with gradients that are small enough for the result."""
+    s = C ** -0.5
+    x = rand((R, C), "float16", 1, 64.0)
+    wg = rand((F, C), "float16", 2, 1024 * s if large == "gate" else s / 64)
+    wu = rand((F, C), "float16", 3, s / 2 ** 18 if large == "gate" else 1024 * s)
+    dy = rand((R, F), "float16", 4, 1e-4)
+    want = scaled_ffn(*(to64(t) for t in (x, wg, wu, dy)))
+    for name, got in ffn_grads(ops, x, wg, wu, dy).items():
+        assert torch.isfinite(got).all(), name
+        check(got, want[name], "float16", name)
