@@ -6,7 +6,7 @@ Unlike the rotor ops these read and write float32, bfloat16 and float16 tensors 
 tensors of a call of one type; recurrence states are float32) and take strided rows in place: only
 the last axis has to be contiguous, so slices of one projection's output are not copied.  Every op
 runs on the current stream of its tensors' device.  Gradients are first-order: a second backward
-pass through them raises.
+pass through them raises, and so does an input with a forward-mode tangent.
 
 The reference has no counterpart of these; its matrix recurrence is python/clifford_cl6.py:150-171
 and its gated product python/clifford_model.py:42-43.

@@ -314,7 +314,8 @@ gated_scan_fwd.register_autograd(_gated_scan_backward, setup_context=_gated_scan
 
 @torch.library.custom_op("csn::gated_step", mutates_args=("h",))
 def gated_step(f: Tensor, x: Tensor, h: Tensor, gate: Optional[Tensor]) -> Tensor:
-    return gated.gated_step(f.detach(), x.detach(), h, gate=None if gate is None else gate.detach())
+    with torch.no_grad():
+        return gated.gated_step(f, x, h, gate=gate)
 
 
 @gated_step.register_fake

@@ -71,6 +71,12 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
   return false;
 }
 
+// The kernels read and write through pointers, past which a forward-mode tangent would be lost without a word.
+void no_tangent(const char* name, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t || !t->defined() || !t->_fw_grad(0).defined(), name, ": forward-mode derivatives are not available");
+}
+
 // t with a contiguous last axis (itself where it has one)
 Tensor rows(const Tensor& t) { return !t.defined() || t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
 Tensor rows(const Maybe& t) { return there(t) ? rows(*t) : Tensor(); }
@@ -116,6 +122,7 @@ void put_strides(int64_t* to, const Tensor& t) {
 }
 
 void check_scan(const Tensor& f, const Tensor& x, const Maybe& h0, const Maybe& gate, const Maybe& cu) {
+  no_tangent("gated_scan", {&f, &x, at_of(h0), at_of(gate)});
   on_one_device("gated_scan", {&f, &x, at_of(h0), at_of(gate), at_of(cu)});
   of_one_type("gated_scan", true, {&f, &x, at_of(gate)});
   const bool shapes = f.dim() == (there(cu) ? 2 : 3) && x.sizes() == f.sizes() && (!there(gate) || gate->sizes() == f.sizes());
@@ -183,6 +190,7 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     if (!g[0].defined() && !g[1].defined()) return variable_list(5);
+    no_tangent("gated_scan", {&g[0], &g[1]});
     const auto s = ctx->get_saved_variables();
     auto [df, dx, dh0, dgate] = [&] {
       at::AutoGradMode off(false);
@@ -204,6 +212,7 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& f, const Tensor& x, const Ma
 }
 
 Tensor gated_step(const Tensor& f_, const Tensor& x_, const Tensor& h, const Maybe& gate_) {
+  no_tangent("gated_step", {&f_, &x_, &h, at_of(gate_)});
   on_one_device("gated_step", {&f_, &x_, &h, at_of(gate_)});
   of_one_type("gated_step", true, {&f_, &x_, at_of(gate_)});
   TORCH_CHECK_VALUE(f_.dim() == 2 && x_.sizes() == f_.sizes() && h.sizes() == f_.sizes() && (!there(gate_) || gate_->sizes() == f_.sizes()),
@@ -268,6 +277,7 @@ struct SiluGatedLinear : torch::autograd::Function<SiluGatedLinear> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto s = ctx->get_saved_variables();
+    no_tangent("silu_gated_linear", {&g[0]});
     auto [dx, dg, du] = [&] {
       at::AutoGradMode off(false);
       return ffn_backward(s[0], s[1], s[2], g[0], s[3], ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2));
@@ -277,6 +287,7 @@ struct SiluGatedLinear : torch::autograd::Function<SiluGatedLinear> {
 };
 
 Tensor silu_gated_linear(const Tensor& x, const Tensor& wg, const Tensor& wu) {
+  no_tangent("silu_gated_linear", {&x, &wg, &wu});
   on_one_device("silu_gated_linear", {&x, &wg, &wu});
   of_one_type("silu_gated_linear", false, {&x, &wg, &wu});
   TORCH_CHECK_VALUE(x.dim() >= 1 && wg.dim() == 2 && wu.sizes() == wg.sizes() && x.size(-1) == wg.size(1),
@@ -314,6 +325,7 @@ struct DropoutAdd : torch::autograd::Function<DropoutAdd> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const Tensor rng = ctx->get_saved_variables()[0];
+    no_tangent("dropout_add", {&g[0]});
     Tensor dx;
     if (ctx->saved_data["x"].toBool()) {
       at::AutoGradMode off(false);
@@ -324,6 +336,7 @@ struct DropoutAdd : torch::autograd::Function<DropoutAdd> {
 };
 
 Tensor dropout_add(const Tensor& x, const Maybe& residual, double p, const Tensor& rng) {
+  no_tangent("dropout_add", {&x, at_of(residual)});
   on_one_device("dropout_add", {&x, at_of(residual), &rng});
   of_one_type("dropout_add", true, {&x, at_of(residual)});
   TORCH_CHECK_VALUE(!there(residual) || residual->sizes() == x.sizes(), "dropout_add: x and residual of one shape expected");
