@@ -285,7 +285,7 @@ def _(f, x, h0, gate, cu_seqlens):
 @torch.library.custom_op("csn::gated_scan_bwd", mutates_args=())
 def gated_scan_bwd(f: Tensor, x: Tensor, gate: Optional[Tensor], cu_seqlens: Optional[Tensor], marks: Tensor,
                    dy: Tensor, dh_last: Tensor) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
-    df, dx, dh0, dgate = gated._ext().gated_scan_backward(f, x, gate, cu_seqlens, marks, dy, dh_last, True)
+    df, dx, dh0, dgate = gated._ext().gated_scan_backward(f, x, gate, cu_seqlens, marks, dy, dh_last)
     return df, dx, dh0, (dgate if dgate is not None else f.new_empty((0,)))
 
 
@@ -336,9 +336,7 @@ def _(x, w_gate, w_up):
 
 @torch.library.custom_op("csn::silu_gated_linear_bwd", mutates_args=())
 def silu_gated_linear_bwd(x: Tensor, w_gate: Tensor, w_up: Tensor, dy: Tensor) -> Tuple[Tensor, Tensor, Tensor]:
-    rows = lambda t: t.reshape(-1, t.shape[-1]) if t.shape[-1] else t.reshape(t.shape[:-1].numel(), 0)  # noqa: E731
-    dx, dwg, dwu = gated._ext().silu_gated_linear_backward(rows(x), w_gate, w_up, rows(dy), None, True, True, True)
-    return dx.view(x.shape), dwg, dwu
+    return gated._ext().silu_gated_linear_backward(x, w_gate, w_up, dy)
 
 
 @silu_gated_linear_bwd.register_fake

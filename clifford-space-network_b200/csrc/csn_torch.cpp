@@ -121,18 +121,25 @@ void put_strides(int64_t* to, const Tensor& t) {
   for (int64_t i = 0; i < n - 1; ++i) to[2 - (n - 1) + i] = t.size(i) > 1 ? t.stride(i) : 0;
 }
 
-void check_scan(const Tensor& f, const Tensor& x, const Maybe& h0, const Maybe& gate, const Maybe& cu) {
-  no_tangent("gated_scan", {&f, &x, at_of(h0), at_of(gate)});
-  on_one_device("gated_scan", {&f, &x, at_of(h0), at_of(gate), at_of(cu)});
+Sizes scan_sizes(const Tensor& f, const Tensor& x, const Maybe& gate, const Maybe& cu) {
   of_one_type("gated_scan", true, {&f, &x, at_of(gate)});
   const bool shapes = f.dim() == (there(cu) ? 2 : 3) && x.sizes() == f.sizes() && (!there(gate) || gate->sizes() == f.sizes());
   TORCH_CHECK_VALUE(shapes, "gated_scan: f, x and gate [B, T, C], or [L, C] with cu_seqlens, of one shape expected, got ",
                     f.sizes(), " and ", x.sizes());
   TORCH_CHECK_VALUE(!there(cu) || (cu->scalar_type() == at::kInt && cu->dim() == 1 && cu->size(0) >= 2 && cu->is_contiguous()),
                     "gated_scan: cu_seqlens is a contiguous int32 vector of at least 2 row numbers");
-  const Sizes n(f, there(cu), cu);
-  TORCH_CHECK_VALUE(!there(h0) || (h0->dim() == 2 && h0->size(0) == n.S && h0->size(1) == n.C && at::isFloatingType(h0->scalar_type())),
-                    "gated_scan: h0 [", n.S, ", ", n.C, "] of a floating type expected");
+  return Sizes(f, there(cu), cu);
+}
+
+void check_state(const char* what, const Maybe& h, const Sizes& n) {
+  TORCH_CHECK_VALUE(!there(h) || (h->dim() == 2 && h->size(0) == n.S && h->size(1) == n.C && at::isFloatingType(h->scalar_type())),
+                    "gated_scan: ", what, " [", n.S, ", ", n.C, "] of a floating type expected");
+}
+
+void check_scan(const Tensor& f, const Tensor& x, const Maybe& h0, const Maybe& gate, const Maybe& cu) {
+  no_tangent("gated_scan", {&f, &x, at_of(h0), at_of(gate)});
+  check_state("h0", h0, scan_sizes(f, x, gate, cu));
+  on_one_device("gated_scan", {&f, &x, at_of(h0), at_of(gate), at_of(cu)});
 }
 
 std::tuple<Tensor, Tensor, Tensor> scan_forward(const Tensor& f_, const Tensor& x_, const Maybe& h0_, const Maybe& gate_,
@@ -177,6 +184,22 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> scan_backward(const Tensor& f_, const
                            static_cast<const float*>(ptr(marks)), static_cast<const float*>(ptr(dlast)), ptr(df), ptr(dx),
                            ptr(dgate), static_cast<float*>(ptr(dh0)), n.S, n.T, n.C, code, ptr(ws), nb, stream(f)));
   return {df, dx, dh0, dgate};
+}
+
+// The backward pass on tensors of any origin, which are looked at first.
+std::tuple<Tensor, Tensor, Tensor, Tensor> gated_scan_backward(const Tensor& f, const Tensor& x, const Maybe& gate, const Maybe& cu,
+                                                               const Tensor& marks, const Tensor& dy, const Tensor& dlast) {
+  no_tangent("gated_scan", {&f, &x, at_of(gate), &marks, &dy, &dlast});
+  const Sizes n = scan_sizes(f, x, gate, cu);
+  of_one_type("gated_scan", true, {&f, &dy});
+  TORCH_CHECK_VALUE(dy.sizes() == f.sizes(), "gated_scan: dy of f's shape expected, got ", dy.sizes(), " and ", f.sizes());
+  check_state("dh_last", dlast, n);
+  const int64_t room = csn_gated_scan_marks(n.S, n.T, n.C, there(cu));
+  TORCH_CHECK_VALUE(marks.scalar_type() == at::kFloat && marks.dim() == 1 && marks.size(0) == room && marks.is_contiguous() &&
+                        reinterpret_cast<uintptr_t>(ptr(marks)) % 16 == 0,
+                    "gated_scan: marks are the ", room, " numbers that the forward pass kept");
+  on_one_device("gated_scan", {&f, &x, at_of(gate), at_of(cu), &marks, &dy, &dlast});
+  return scan_backward(f, x, gate, cu, marks, dy, dlast.to(at::kFloat), true);
 }
 
 struct GatedScan : torch::autograd::Function<GatedScan> {
@@ -286,23 +309,43 @@ struct SiluGatedLinear : torch::autograd::Function<SiluGatedLinear> {
   }
 };
 
-Tensor silu_gated_linear(const Tensor& x, const Tensor& wg, const Tensor& wu) {
-  no_tangent("silu_gated_linear", {&x, &wg, &wu});
-  on_one_device("silu_gated_linear", {&x, &wg, &wu});
+void check_ffn(const Tensor& x, const Tensor& wg, const Tensor& wu) {
   of_one_type("silu_gated_linear", false, {&x, &wg, &wu});
   TORCH_CHECK_VALUE(x.dim() >= 1 && wg.dim() == 2 && wu.sizes() == wg.sizes() && x.size(-1) == wg.size(1),
                     "silu_gated_linear: x [..., C] and w_gate, w_up [F, C] expected, got ", x.sizes(), ", ", wg.sizes(), ", ", wu.sizes());
-  Tensor flat = x;
-  if (x.dim() != 2) {
-    int64_t n = 1;
-    for (int64_t i = 0; i < x.dim() - 1; ++i) n *= x.size(i);
-    flat = x.reshape({n, x.size(-1)});
-  }
-  Tensor y = wants_grad({&x, &wg, &wu}) ? SiluGatedLinear::apply(flat, wg, wu) : std::get<0>(ffn_forward(flat, wg, wu, false));
+}
+
+// t [..., n] as a matrix
+Tensor flat(const Tensor& t) {
+  if (t.dim() == 2) return t;
+  int64_t n = 1;
+  for (int64_t i = 0; i < t.dim() - 1; ++i) n *= t.size(i);
+  return t.reshape({n, t.size(-1)});
+}
+
+Tensor silu_gated_linear(const Tensor& x, const Tensor& wg, const Tensor& wu) {
+  no_tangent("silu_gated_linear", {&x, &wg, &wu});
+  check_ffn(x, wg, wu);
+  on_one_device("silu_gated_linear", {&x, &wg, &wu});
+  const Tensor r = flat(x);
+  Tensor y = wants_grad({&x, &wg, &wu}) ? SiluGatedLinear::apply(r, wg, wu) : std::get<0>(ffn_forward(r, wg, wu, false));
   if (x.dim() == 2) return y;
   std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = wg.size(0);
   return y.view(shape);
+}
+
+// The backward pass on tensors of any origin, which are looked at first; both products are formed again.
+std::tuple<Tensor, Tensor, Tensor> silu_gated_linear_backward(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& dy) {
+  no_tangent("silu_gated_linear", {&x, &wg, &wu, &dy});
+  check_ffn(x, wg, wu);
+  of_one_type("silu_gated_linear", false, {&x, &dy});
+  const auto lead = x.sizes().slice(0, x.dim() - 1);
+  TORCH_CHECK_VALUE(dy.dim() == x.dim() && dy.sizes().slice(0, lead.size()) == lead && dy.size(-1) == wg.size(0),
+                    "silu_gated_linear: dy of the result's shape expected, got ", dy.sizes(), " for ", x.sizes(), " and ", wg.sizes());
+  on_one_device("silu_gated_linear", {&x, &wg, &wu, &dy});
+  auto [dx, dg, du] = ffn_backward(flat(x), wg, wu, flat(dy), std::nullopt, true, true, true);
+  return {dx.view(x.sizes()), dg, du};
 }
 
 // ------------------------------------------------------------------------ dropout
@@ -362,9 +405,9 @@ PYBIND11_MODULE(_gated, m) {
   m.def("gated_scan", &gated_scan);
   m.def("gated_scan_check", &check_scan);
   m.def("gated_scan_forward", &scan_forward);
-  m.def("gated_scan_backward", &scan_backward);
+  m.def("gated_scan_backward", &gated_scan_backward);
   m.def("gated_step", &gated_step);
   m.def("silu_gated_linear", &silu_gated_linear);
-  m.def("silu_gated_linear_backward", &ffn_backward);
+  m.def("silu_gated_linear_backward", &silu_gated_linear_backward);
   m.def("dropout_add", &dropout_add);
 }

@@ -51,3 +51,31 @@ def test_tangents_of_gradients_are_refused(ops):
         for call in (lambda: ops.dropout_add(dual, None, 0.5, rng), lambda: ops.dropout_add(x, dual, 0.5, rng)):
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 call()
+
+
+def test_registered_backward_operators(ops):
+    """They are the backward passes that autograd runs, and refuse what does not fit."""
+    csn = torch.ops.csn
+    f, x, gate, dy = (rand((3, 70, 24), i) for i in range(4))
+    h0, dh = rand((3, 24), 5, torch.float32), rand((3, 24), 6)
+    leaves = [t.detach().requires_grad_(True) for t in (f, x, h0, gate)]
+    y, h = ops.gated_scan(*leaves[:3], gate=leaves[3])
+    want = torch.autograd.grad((y, h), leaves, (dy, dh.float()))
+    marks = csn.gated_scan_fwd(f, x, h0, gate, None)[2]
+    got = csn.gated_scan_bwd(f, x, gate, None, marks, dy, dh)  # a state's gradient of any floating type
+    for a, b in zip(want, got):
+        assert torch.equal(a, b)
+    a, wg, wu, dz = rand((2, 50, 24), 7), rand((40, 24), 8), rand((40, 24), 9), rand((2, 50, 40), 10)
+    leaves = [t.detach().requires_grad_(True) for t in (a, wg, wu)]
+    want = torch.autograd.grad(ops.silu_gated_linear(*leaves), leaves, dz)
+    for p, q in zip(want, csn.silu_gated_linear_bwd(a, wg, wu, dz)):
+        assert p.shape == q.shape and torch.equal(p, q)
+    for bad in (lambda: csn.gated_scan_bwd(f, x, gate, None, marks[:-4].clone(), dy, dh), lambda: csn.gated_scan_bwd(f, x, gate, None, marks, dy[:2], dh),
+                lambda: csn.gated_scan_bwd(f, x, gate, None, marks, dy.float(), dh), lambda: csn.silu_gated_linear_bwd(a, wg, wu, dz[:, :-1]),
+                lambda: csn.silu_gated_linear_bwd(a, wg, wu, dz.half())):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (lambda: csn.gated_scan_bwd(f, x, gate, None, marks, dy, dh.cpu()), lambda: csn.gated_scan_bwd(f, x, gate, None, marks.cpu(), dy, dh),
+                lambda: csn.silu_gated_linear_bwd(a, wg, wu, dz.cpu())):
+        with pytest.raises(RuntimeError, match="CUDA tensors"):
+            bad()
