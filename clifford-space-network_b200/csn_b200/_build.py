@@ -11,7 +11,9 @@ of the gated block's entry points, is then compiled against the installed torch 
 The build is content-addressed: a SHA-256 over every source, header and the build flags is
 compiled into the library (``csn_version()`` ends in ``src <hash>``) and recorded beside it,
 so a library whose sources changed since it was linked is rebuilt whatever the file times
-say, and a caller can check that the library it loaded is the one these sources make.
+say, and a caller can check that the library it loaded is the one these sources make.  The binding is
+made for one torch, Python and C++ runtime as well: a second hash over these, its compiler and its flags
+is recorded beside it, and where that changes the binding alone is compiled again.
 """
 from __future__ import annotations
 
@@ -32,6 +34,7 @@ BINDING = PKG / "_gated.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-O2"]
+CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden"]
 
 
 def _nvcc() -> str:
@@ -46,6 +49,7 @@ def sources() -> list:
 
 
 HASH_FILE = LIB.with_name(LIB.name + ".srchash")
+BINDING_HASH_FILE = BINDING.with_name(BINDING.name + ".srchash")
 # what the last build() call did: "built" or "reused"
 last_action = None
 
@@ -62,37 +66,48 @@ def source_hash() -> str:
     return h.hexdigest()[:16]
 
 
-def _stale(digest: str) -> bool:
-    if not LIB.exists() or not BINDING.exists() or not HASH_FILE.exists():
-        return True
-    return HASH_FILE.read_text().strip() != digest
+def _recorded(product: Path, hash_file: Path, key: str) -> bool:
+    """Whether `product` is there and was built under `key`."""
+    return product.exists() and hash_file.exists() and hash_file.read_text().strip() == key
 
 
-def _build_binding() -> None:
-    from torch.utils import cpp_extension
+def _cxx() -> str:
     # the compiler that torch's own libstdc++ goes with, and not $CXX: one that links its runtime statically
     # makes a module whose streams crash beside torch's
-    cxx = next((c for c in ("/usr/bin/g++", shutil.which("g++")) if c and Path(c).exists()), "g++")
+    return next((c for c in ("/usr/bin/g++", shutil.which("g++")) if c and Path(c).exists()), "g++")
+
+
+def _cxx_version(cxx: str) -> str:
+    try:
+        return subprocess.run([cxx, "--version"], capture_output=True, text=True).stdout
+    except OSError:  # the build says so, if there is one to do
+        return ""
+
+
+def binding_key(digest: str) -> str:
+    """The hash that _gated.so is recorded under: the sources' (`digest`) and what it is built with and against."""
+    import torch
+    what = [digest, torch.__version__, str(torch._C._GLIBCXX_USE_CXX11_ABI), str(sysconfig.get_config_var("SOABI")),
+            _cxx_version(_cxx()), *CXX_FLAGS]
+    return hashlib.sha256("\0".join(what).encode()).hexdigest()[:16]
+
+
+def _build_binding(key: str) -> None:
+    from torch.utils import cpp_extension
     include = [f"-I{p}" for p in cpp_extension.include_paths(device_type="cuda") + [sysconfig.get_paths()["include"]]]
     where = cpp_extension.library_paths(device_type="cuda")
     tmp = BINDING.with_suffix(".so.tmp")
-    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", *include, str(CSRC / "csn_torch.cpp"),
-           "-o", str(tmp), f"-L{PKG}", "-l:libcsn_b200.so", "-Wl,-rpath,$ORIGIN", *[f"-L{p}" for p in where],
-           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    cxx = _cxx()
+    cmd = [cxx, *CXX_FLAGS, *include, str(CSRC / "csn_torch.cpp"), "-o", str(tmp), f"-L{PKG}", "-l:libcsn_b200.so",
+           "-Wl,-rpath,$ORIGIN", *[f"-L{p}" for p in where], "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"{cxx} failed on csn_torch.cpp:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, BINDING)
+    BINDING_HASH_FILE.write_text(key + "\n")
 
 
-def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile every CUDA source and link the shared library (skipped when the library was
-    built from exactly these sources)."""
-    global last_action
-    digest = source_hash()
-    if not force and not _stale(digest):
-        last_action = "reused"
-        return LIB
+def _build_library(digest: str, verbose: bool) -> None:
     nvcc = _nvcc()
     OBJ.mkdir(parents=True, exist_ok=True)
 
@@ -114,9 +129,22 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB)
-    _build_binding()
     HASH_FILE.write_text(digest + "\n")
-    last_action = "built"
+
+
+def build(force: bool = False, verbose: bool = False) -> Path:
+    """Compile every CUDA source and link the shared library, then the binding (each skipped when it was
+    built from exactly these sources, the binding also for this torch, Python and compiler)."""
+    global last_action
+    digest = source_hash()
+    key = binding_key(digest)
+    last_action = "reused"
+    if force or not _recorded(LIB, HASH_FILE, digest):
+        _build_library(digest, verbose)
+        last_action = "built"
+    if last_action == "built" or not _recorded(BINDING, BINDING_HASH_FILE, key):
+        _build_binding(key)
+        last_action = "built"
     return LIB
 
 
