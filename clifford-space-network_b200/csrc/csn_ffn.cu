@@ -68,6 +68,7 @@ struct Args {
   int halves_m;       // 2 for DW: dWg, then dWu
   int halves_k;       // 2 for DX: dg Wg, then du Wu
   int splits, kper;   // k blocks are cut into `splits` ranges of kper
+  uint32_t polls;     // the limit of a wait
   void* out[2];       // y; dg, du; dx; dWg, dWu
   int64_t ldo;
   const void* dy;
@@ -236,7 +237,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       const int k0 = T.split * P.kper, k1 = min(k0 + P.kper, P.kb * P.halves_k);
       const int m = (T.m * 2 + rank) * BM;
       for (int k = k0; k < k1; ++k, ++it) {
-        if (!(ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], parity, &gave_up)))) break;
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], parity, &gave_up, P.polls)))) break;
         if (elect_one()) {
           if (rank == 0) mbar_expect(&full[s], 2 * SB);
           const uint32_t bar = peer_addr(&full[s], 0);
@@ -264,7 +265,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       }
     }
     if (ok) {  // the pair's last commits arrive before this CTA leaves
-      for (int j = it > ST ? it - ST : 0; j < it; ++j) mbar_wait(&empty[j % ST], (j / ST) & 1, &gave_up);
+      for (int j = it > ST ? it - ST : 0; j < it; ++j) mbar_wait(&empty[j % ST], (j / ST) & 1, &gave_up, P.polls);
     } else if (rank == 0) {  // copies in flight end before the shared memory does (CTA 0's barriers count both CTAs')
       for (int j = it > ST ? it - ST : 0; j < it; ++j)
         for (uint32_t i = 0; i < POLLS && !mbar_try(&full[j % ST], (j / ST) & 1); ++i) {}
@@ -280,10 +281,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         const Tile T(P, t);
         const int k0 = T.split * P.kper, k1 = min(k0 + P.kper, P.kb * P.halves_k);
         const uint32_t d = tmem + (n & 1) * BN;
-        if (!(ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[n & 1], ((n >> 1) + 1) & 1, &gave_up)))) break;
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[n & 1], ((n >> 1) + 1) & 1, &gave_up, P.polls)))) break;
         fence_after();
         for (int k = k0; k < k1; ++k) {
-          if (!(ok = __all_sync(0xffffffffu, mbar_wait(&full[s], parity, &gave_up)))) break;
+          if (!(ok = __all_sync(0xffffffffu, mbar_wait(&full[s], parity, &gave_up, P.polls)))) break;
           fence_after();
           if (elect_one()) {
             const uint64_t ad = desc0 + (uint32_t)(s * SB >> 4), bd = ad + (BM * BK * 2 >> 4);
@@ -320,7 +321,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       const Tile T(P, t);
       const int64_t row0 = (int64_t)(T.m * 2 + rank) * BM + quarter * 32;
       const int rows = (int)min((int64_t)32, P.m - row0);
-      const bool ok = mbar_wait(&acc_full[acc], parity, &gave_up);
+      const bool ok = mbar_wait(&acc_full[acc], parity, &gave_up, P.polls);
       __syncwarp();
       fence_after();
       const float nan = __int_as_float(0x7fffffff);
@@ -370,6 +371,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             if (MODE == GATE && P.pre && h * 16 < cols) {
               float* pre = P.pre + row0 * P.n + col + h * 16;
               const int part = min(cols - h * 16, 16) * 4;
+              if (!ok) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) g[i] = u[i] = nan;
+              }
               put8(own, reinterpret_cast<uint32_t*>(g));
               put8(own + 32, reinterpret_cast<uint32_t*>(g) + 8);
               put_rows(stage, lane, reinterpret_cast<char*>(pre), (int64_t)P.n * 4, rows, part, vec_pre);
@@ -528,6 +533,7 @@ constexpr int few_smem(int nr) { return few_stages(nr) * few_stage(nr) + 1024; }
 
 struct FewArgs {
   int R, F, kb;
+  uint32_t polls;  // the limit of a wait
   void* y;
 };
 
@@ -574,7 +580,7 @@ __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(const __grid_cons
     int k = k0;
     for (; k < k1; ++k) {
       const int it = k - k0, s = it % ST;
-      if (!__all_sync(0xffffffffu, mbar_wait(&empty[s], (it / ST + 1) & 1, &gave_up))) break;
+      if (!__all_sync(0xffffffffu, mbar_wait(&empty[s], (it / ST + 1) & 1, &gave_up, P.polls))) break;
       if (elect_one()) {
         mbar_expect(&full[s], SB);
         char* a = smem + s * SB;
@@ -592,7 +598,7 @@ __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(const __grid_cons
     const uint64_t desc0 = operand(smem_addr(smem), 0);
     for (int k = k0; k < k1; ++k) {
       const int it = k - k0, s = it % ST;
-      if (!__all_sync(0xffffffffu, mbar_wait(&full[s], (it / ST) & 1, &gave_up))) break;
+      if (!__all_sync(0xffffffffu, mbar_wait(&full[s], (it / ST) & 1, &gave_up, P.polls))) break;
       fence_after();
       if (elect_one()) {
         const uint64_t ad = desc0 + (uint32_t)(s * SB >> 4), bd = ad + (2 * HALF_ROWS * BK * 2 >> 4);
@@ -606,7 +612,7 @@ __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(const __grid_cons
     __syncwarp();
   } else {
     // `done` counts the products issued: complete, unless a wait gave up
-    ok = mbar_wait(&done, 0, &gave_up);
+    ok = mbar_wait(&done, 0, &gave_up, P.polls);
     __syncwarp();
     fence_after();
     const int row = warp * 32 + lane;
@@ -784,7 +790,7 @@ int run_gate(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void
   maps.a[1] = maps.a[0];
   Args P = {};
   P.m = (int)R, P.n = (int)F, P.mt = p.mt, P.nt = p.nt, P.kb = (int)up(C, BK), P.halves_m = P.halves_k = 1;
-  P.splits = p.splits, P.kper = p.kper, P.out[0] = o0, P.out[1] = o1, P.ldo = ldo, P.dy = dy, P.ldy = ldy, P.pre = pre, P.range = range;
+  P.splits = p.splits, P.kper = p.kper, P.polls = poll_limit(p.kper), P.out[0] = o0, P.out[1] = o1, P.ldo = ldo, P.dy = dy, P.ldy = ldy, P.pre = pre, P.range = range;
   if (dy) {
     int rc = p.bn == 256 ? run_mm<GATE_BWD, BF16, 256>(maps, P, st, who) : run_mm<GATE_BWD, BF16, 128>(maps, P, st, who);
     P.again = true;
@@ -823,7 +829,7 @@ int forward(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void*
       !make_map(&maps.b[0], x, R, C, ldx, nr, BF16))
     return set_error(CSN_ERR_CUDA, "silu_gated_linear: cuTensorMapEncodeTiled");
   maps.b[1] = maps.b[0];
-  const FewArgs P = {(int)R, (int)F, (int)up(C, BK), y};
+  const FewArgs P = {(int)R, (int)F, (int)up(C, BK), poll_limit(up(C, BK)), y};
   // Ranges of C, at least 4 blocks each, until there are one and a half CTAs an SM.  Two fit, but clusters do not fill
   // every SM: R9 C1824 F4736 took 17.3 us with 296 CTAs and takes 10.6 with 148.
   int ranks = 1;
@@ -835,7 +841,7 @@ int forward(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void*
 template <Mode MODE, bool BF16>
 int run_product(const Maps& maps, Args P, int64_t blocks, const Plan& p, float* part, cudaStream_t st,
                 const char* who) {
-  P.mt = p.mt, P.nt = p.nt, P.kb = (int)(blocks / P.halves_k), P.splits = p.splits, P.kper = p.kper, P.part = part;
+  P.mt = p.mt, P.nt = p.nt, P.kb = (int)(blocks / P.halves_k), P.splits = p.splits, P.kper = p.kper, P.polls = poll_limit(p.kper), P.part = part;
   int rc = p.bn == 256 ? run_mm<MODE, BF16, 256>(maps, P, st, who) : run_mm<MODE, BF16, 128>(maps, P, st, who);
   if (rc || p.splits == 1) return rc;
   const int64_t n = (int64_t)P.m * P.n;

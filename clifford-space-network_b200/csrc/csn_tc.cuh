@@ -61,11 +61,13 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// Waits for the phase `parity` of b to end.  A poll takes tens of nanoseconds at least, so the limit is some tenths
-// of a second, a thousand times the longest tile.
+// Waits for the phase `parity` of b to end, for `polls` polls at most.  A poll takes tens of nanoseconds at least: POLLS are
+// some tenths of a second.  A wait can last as long as a tile: a k block takes 0.4 us of the tensor cores, or 0.7 where
+// nothing of it is in L2 and every SM reads, so 8192 of them 3 to 6 ms, and the limit is POLLS for each 8192 begun.
 constexpr uint32_t POLLS = 1u << 23;
-__device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, volatile uint32_t* gave_up) {
-  for (uint32_t i = 0; i < POLLS; ++i) {
+inline uint32_t poll_limit(int64_t k_blocks) { return POLLS * (uint32_t)(1 + k_blocks / 8192); }  // k_blocks <= 2^16
+__device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, volatile uint32_t* gave_up, uint32_t polls) {
+  for (uint32_t i = 0; i < polls; ++i) {
     if (mbar_try(b, parity)) return true;
     if ((i & 1023) == 1023 && *gave_up) return false;
   }
