@@ -213,3 +213,38 @@ def test_ffn_float16_gradients_of_large_products(ops, R, C, F, large):
     for name, got in ffn_grads(ops, x, wg, wu, dy).items():
         assert torch.isfinite(got).all(), name
         check(got, want[name], "float16", name)
+
+
+@pytest.mark.parametrize("R,C,F", [(200, 64, 72), (100, 1536, 40)])
+def test_ffn_float16_gradients_in_a_captured_pass(ops, R, C, F):
+    """A replayed pass forms dg and du again, or not, as its inputs of that replay ask for; and on several streams at once."""
+    ordinary = [rand(s, "float16", i, v) for i, (s, v) in enumerate((((R, C), 1.0), ((F, C), C ** -0.5), ((F, C), C ** -0.5), ((R, F), 1.0)))]
+    large = [ordinary[0] * 64, ordinary[1] * 1024, ordinary[2] / 2 ** 12, ordinary[3] * 1e-4]
+    at = [t.clone() for t in ordinary]
+    run = lambda: [v for _, v in sorted(ffn_grads(ops, *at).items())]  # noqa: E731
+    want = {}
+    for name, given in (("ordinary", ordinary), ("large", large)):
+        for a, b in zip(at, given):
+            a.copy_(b)
+        want[name] = [t.clone() for t in run()]
+        assert all(torch.isfinite(t).all() for t in want[name])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for name, given in (("large", large), ("ordinary", ordinary), ("large", large), ("large", large)):
+        for a, b in zip(at, given):
+            a.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, want[name]):
+            assert torch.equal(a, b)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(run())
+    torch.cuda.synchronize()
+    for outs in got:
+        for a, b in zip(outs, want["large"]):
+            assert torch.equal(a, b)
