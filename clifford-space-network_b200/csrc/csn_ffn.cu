@@ -5,7 +5,8 @@
 //   dg = dy u w (1 + g (1 - w)),  du = dy g w,  dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x
 // The backward pass takes g and u in float32 from what the forward pass kept ([2, R, F]), or forms them again.  Keeping
 // them costs 8 bytes an element written and read, forming them 4 C operations: at 6.5 TB/s and 1.4 PFLOP/s the two are
-// even near C = 1000, and the caller decides (rounded to 16 bits they would cost a third of the gradients' precision).
+// even near C = 1000, and the caller of these entry points decides (the PyTorch functions keep them from C = 1536 on; rounded to
+// 16 bits they would cost a third of the gradients' precision).
 // dg and du are rounded to the tensors' own type once, as the operands of the products that follow.  In float16,
 // whose numbers end at 65504 and lose bits below 2^-14, they are first scaled by the power of two that brings the largest
 // finite |dy| into [2^10, 2^11), and the products are scaled back in float32.  So a row whose dy is 2^-24 of the largest
@@ -32,7 +33,7 @@
 // few_rows_kernel takes R <= 64 rows (generation): there the weights are what is read, so they take the 128-row side
 // of the product (64 rows of Wg and 64 of Wu) and x the narrow side, and a cluster splits C where F alone gives too
 // few CTAs, its partial sums joined through distributed shared memory in a fixed order.  Bound by the weights' bytes and
-// by the start and end of a short kernel: R4 C2048 F8192 15 us of 10.3 with the weights in HBM, R2 C256 F512 4.3 us.
+// by the start and end of a short kernel: R4 C2048 F8192 15 us of 10.3 with the weights in HBM, R2 C256 F512 4.6 us.
 #include <cstdint>
 
 #include "csn_internal.h"
@@ -68,7 +69,6 @@ struct Args {
   int halves_m;       // 2 for DW: dWg, then dWu
   int halves_k;       // 2 for DX: dg Wg, then du Wu
   int splits, kper;   // k blocks are cut into `splits` ranges of kper
-  uint32_t polls;     // the limit of a wait
   void* out[2];       // y; dg, du; dx; dWg, dWu
   int64_t ldo;
   const void* dy;
@@ -237,7 +237,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       const int k0 = T.split * P.kper, k1 = min(k0 + P.kper, P.kb * P.halves_k);
       const int m = (T.m * 2 + rank) * BM;
       for (int k = k0; k < k1; ++k, ++it) {
-        if (!(ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], parity, &gave_up, P.polls)))) break;
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], parity, &gave_up)))) break;
         if (elect_one()) {
           if (rank == 0) mbar_expect(&full[s], 2 * SB);
           const uint32_t bar = peer_addr(&full[s], 0);
@@ -265,7 +265,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       }
     }
     if (ok) {  // the pair's last commits arrive before this CTA leaves
-      for (int j = it > ST ? it - ST : 0; j < it; ++j) mbar_wait(&empty[j % ST], (j / ST) & 1, &gave_up, P.polls);
+      for (int j = it > ST ? it - ST : 0; j < it; ++j) mbar_wait(&empty[j % ST], (j / ST) & 1, &gave_up);
     } else if (rank == 0) {  // copies in flight end before the shared memory does (CTA 0's barriers count both CTAs')
       for (int j = it > ST ? it - ST : 0; j < it; ++j)
         for (uint32_t i = 0; i < POLLS && !mbar_try(&full[j % ST], (j / ST) & 1); ++i) {}
@@ -281,10 +281,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         const Tile T(P, t);
         const int k0 = T.split * P.kper, k1 = min(k0 + P.kper, P.kb * P.halves_k);
         const uint32_t d = tmem + (n & 1) * BN;
-        if (!(ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[n & 1], ((n >> 1) + 1) & 1, &gave_up, P.polls)))) break;
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[n & 1], ((n >> 1) + 1) & 1, &gave_up)))) break;
         fence_after();
         for (int k = k0; k < k1; ++k) {
-          if (!(ok = __all_sync(0xffffffffu, mbar_wait(&full[s], parity, &gave_up, P.polls)))) break;
+          if (!(ok = __all_sync(0xffffffffu, mbar_wait(&full[s], parity, &gave_up)))) break;
           fence_after();
           if (elect_one()) {
             const uint64_t ad = desc0 + (uint32_t)(s * SB >> 4), bd = ad + (BM * BK * 2 >> 4);
@@ -321,7 +321,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       const Tile T(P, t);
       const int64_t row0 = (int64_t)(T.m * 2 + rank) * BM + quarter * 32;
       const int rows = (int)min((int64_t)32, P.m - row0);
-      const bool ok = mbar_wait(&acc_full[acc], parity, &gave_up, P.polls);
+      const bool ok = mbar_wait(&acc_full[acc], parity, &gave_up);
       __syncwarp();
       fence_after();
       const float nan = __int_as_float(0x7fffffff);
@@ -533,7 +533,6 @@ constexpr int few_smem(int nr) { return few_stages(nr) * few_stage(nr) + 1024; }
 
 struct FewArgs {
   int R, F, kb;
-  uint32_t polls;  // the limit of a wait
   void* y;
 };
 
@@ -580,7 +579,7 @@ __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(const __grid_cons
     int k = k0;
     for (; k < k1; ++k) {
       const int it = k - k0, s = it % ST;
-      if (!__all_sync(0xffffffffu, mbar_wait(&empty[s], (it / ST + 1) & 1, &gave_up, P.polls))) break;
+      if (!__all_sync(0xffffffffu, mbar_wait(&empty[s], (it / ST + 1) & 1, &gave_up))) break;
       if (elect_one()) {
         mbar_expect(&full[s], SB);
         char* a = smem + s * SB;
@@ -598,7 +597,7 @@ __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(const __grid_cons
     const uint64_t desc0 = operand(smem_addr(smem), 0);
     for (int k = k0; k < k1; ++k) {
       const int it = k - k0, s = it % ST;
-      if (!__all_sync(0xffffffffu, mbar_wait(&full[s], (it / ST) & 1, &gave_up, P.polls))) break;
+      if (!__all_sync(0xffffffffu, mbar_wait(&full[s], (it / ST) & 1, &gave_up))) break;
       fence_after();
       if (elect_one()) {
         const uint64_t ad = desc0 + (uint32_t)(s * SB >> 4), bd = ad + (2 * HALF_ROWS * BK * 2 >> 4);
@@ -612,7 +611,7 @@ __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(const __grid_cons
     __syncwarp();
   } else {
     // `done` counts the products issued: complete, unless a wait gave up
-    ok = mbar_wait(&done, 0, &gave_up, P.polls);
+    ok = mbar_wait(&done, 0, &gave_up);
     __syncwarp();
     fence_after();
     const int row = warp * 32 + lane;
@@ -790,7 +789,7 @@ int run_gate(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void
   maps.a[1] = maps.a[0];
   Args P = {};
   P.m = (int)R, P.n = (int)F, P.mt = p.mt, P.nt = p.nt, P.kb = (int)up(C, BK), P.halves_m = P.halves_k = 1;
-  P.splits = p.splits, P.kper = p.kper, P.polls = poll_limit(p.kper), P.out[0] = o0, P.out[1] = o1, P.ldo = ldo, P.dy = dy, P.ldy = ldy, P.pre = pre, P.range = range;
+  P.splits = p.splits, P.kper = p.kper, P.out[0] = o0, P.out[1] = o1, P.ldo = ldo, P.dy = dy, P.ldy = ldy, P.pre = pre, P.range = range;
   if (dy) {
     int rc = p.bn == 256 ? run_mm<GATE_BWD, BF16, 256>(maps, P, st, who) : run_mm<GATE_BWD, BF16, 128>(maps, P, st, who);
     P.again = true;
@@ -829,9 +828,9 @@ int forward(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void*
       !make_map(&maps.b[0], x, R, C, ldx, nr, BF16))
     return set_error(CSN_ERR_CUDA, "silu_gated_linear: cuTensorMapEncodeTiled");
   maps.b[1] = maps.b[0];
-  const FewArgs P = {(int)R, (int)F, (int)up(C, BK), poll_limit(up(C, BK)), y};
+  const FewArgs P = {(int)R, (int)F, (int)up(C, BK), y};
   // Ranges of C, at least 4 blocks each, until there are one and a half CTAs an SM.  Two fit, but clusters do not fill
-  // every SM: R9 C1824 F4736 took 17.3 us with 296 CTAs and takes 10.6 with 148.
+  // every SM: R9 C1824 F4736 took 17.3 us with 296 CTAs and takes 10.0 with 148.
   int ranks = 1;
   while (ranks < 8 && up(F, HALF_ROWS) * ranks * 2 <= 3 * PAIRS && P.kb >= ranks * 2 * 4) ranks *= 2;
   return nr == 16 ? run_few<BF16, 16>(maps, P, ranks, st, who)
@@ -841,7 +840,7 @@ int forward(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void*
 template <Mode MODE, bool BF16>
 int run_product(const Maps& maps, Args P, int64_t blocks, const Plan& p, float* part, cudaStream_t st,
                 const char* who) {
-  P.mt = p.mt, P.nt = p.nt, P.kb = (int)(blocks / P.halves_k), P.splits = p.splits, P.kper = p.kper, P.polls = poll_limit(p.kper), P.part = part;
+  P.mt = p.mt, P.nt = p.nt, P.kb = (int)(blocks / P.halves_k), P.splits = p.splits, P.kper = p.kper, P.part = part;
   int rc = p.bn == 256 ? run_mm<MODE, BF16, 256>(maps, P, st, who) : run_mm<MODE, BF16, 128>(maps, P, st, who);
   if (rc || p.splits == 1) return rc;
   const int64_t n = (int64_t)P.m * P.n;
