@@ -67,7 +67,8 @@ def silu_gated_linear(x, w_gate, w_up):
     (what :func:`silu_gate` makes of the library product of both weights).  bfloat16 or float16 on the
     tensor cores, sums in float32, one rounding at the end.  The backward pass forms both products
     again, or, for C >= 1536, takes them from float32 copies that the forward pass keeps (8 bytes an
-    element of the result until then).  float32 layers use ``silu_gate(linear(x, cat))``."""
+    element of the result until then; torch.ops.csn.silu_gated_linear_fwd never keeps them, and
+    activation checkpointing drops them).  At most 2^21 rows, C and F.  float32 layers use ``silu_gate(linear(x, cat))``."""
     return (_module or _ext()).silu_gated_linear(x, w_gate, w_up)
 
 

@@ -21,6 +21,10 @@ The gated recurrent block's operators (csn_b200.gated) take float32, bfloat16 an
     silu_gated_linear_fwd(x, w_gate, w_up) -> y              silu_gated_linear_bwd(..., dy) -> 3 gradients
     dropout_add(x, residual?, cut, rng) -> y                 (cut = 65536 p; its own backward)
 
+The backward operators check types, shapes and devices as the forward ones do.  silu_gated_linear_fwd
+keeps nothing for its backward, which forms both products again; csn_b200.ops.silu_gated_linear keeps
+them in wide layers, where that is faster.
+
 Optional gradients that do not exist (no h0, undamped) come back as empty tensors.
 The sequence-parallel scan takes a process group and stays a Python entry point
 (csn_b200.sequence_parallel.sequence_parallel_rotor_scan).

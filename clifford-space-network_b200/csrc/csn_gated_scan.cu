@@ -18,13 +18,15 @@
 // fit), and the CTA of a chunk composes those before it into the state that enters it.  All sums, products and states
 // are float32 and in an order that the sizes alone fix.
 //
-// What bounds it: issue and the latency of a pass, not memory.  An element costs about 37 instructions forward (two of
-// them on the MUFU for the decay, two for the gate) and 70 back, and with 256 to 444 CTAs of 8 warps the SMs issue 2 to
-// 2.5 a clock.  bf16 with a gate on a B200: B8 T2048 C2048 forward 73 us (3.7 TB/s of what has to move), backward 123 us
-// (3.8 TB/s); B24 T2048 C2048 181 us (4.5 TB/s) and 346 us (4.1 TB/s); one sequence of 65536 x 1024 48 us for the reduce
-// pass (5.6 TB/s) and 116 us for the scan (4.6 TB/s).  Slower: steps of 4 or 16 a warp, 4 or 16 warps a CTA, 2 or 4 CTAs an
-// SM forward and 1 or 3 back, packed float32 pairs (the same instruction count, in moves), and the time axis split over
-// clusters that pass maps every MARK steps (prompt 319 us with st.async, 419 with barrier.cluster).
+// What bounds it: the latency of a pass, not memory.  An element costs about 40 instructions forward (two of them on
+// the MUFU for the decay, two for the gate) and 73 back (two and four: the gate's sigmoid twice), and with 256 CTAs of
+// 8 warps the schedulers issue in 60 to 64 % of the cycles, MUFU 42 to 48 %, HBM 0.58 of its rate: nothing is full, and
+// a warp waits for fixed latencies, shared memory and MUFU results.  bf16 with a gate on a B200: B8 T2048 C2048 forward
+// 71 us (3.8 TB/s of what has to move), backward 124 us (3.8 TB/s); B24 T2048 C2048 181 us (4.5 TB/s) and 346 us (4.1
+// TB/s); one sequence of 65536 x 1024 50 us for the reduce pass (5.4 TB/s) and 114 us for the scan (4.7 TB/s).  Slower:
+// steps of 4 or 16 a warp, 4 or 16 warps a CTA, 2 or 4 CTAs an SM forward and 1 or 3 back, packed float32 pairs (the
+// same instruction count, in moves), and the time axis split over clusters that pass maps every MARK steps (prompt 319
+// us with st.async, 419 with barrier.cluster).
 //
 // The forward pass keeps the float32 state before every MARK-th step ("marks") where a backward pass will follow:
 // the adjoint forms the states between two marks again instead of reading rounded outputs (y is not h where there is
