@@ -19,8 +19,9 @@ Ops (reference functions they replace, paths relative to the reference root):
                                (layout include/clifford_configs.cuh:38-51)
 
 The gated recurrent block's ops (:func:`gated_scan`, :func:`gated_step`,
-:func:`silu_gated_linear`, :func:`dropout_add`, in ``gated.py``) take float32 and 16-bit tensors as
-they are instead.
+:func:`silu_gated_linear`, :func:`dropout_add`, in ``gated.py``) and the linear-attention block's
+(:func:`linear_attention`, :func:`linear_attention_step`, in ``linear_attention.py``) take float32 and
+16-bit tensors as they are instead, and so does :func:`layer_norm` with 16-bit ones.
 """
 from __future__ import annotations
 
@@ -34,7 +35,7 @@ from . import _lib
 __all__ = ["rotor_scan", "fused_rotor_scan", "fused_rotor_scan_heads", "cayley", "cell_step", "ga3_rotor_scan",
            "rotor_step", "RotorStepGraph", "state_spike", "layer_norm", "ln_conv_silu",
            "generator_action", "linear", "projection_epilogue", "silu_gate", "column_sum", "gated_scan", "gated_step",
-           "silu_gated_linear", "dropout_add", "BASIS"]
+           "silu_gated_linear", "dropout_add", "linear_attention", "linear_attention_step", "BASIS"]
 
 BASIS = {"triu": 0, "ga": 1}
 
@@ -547,13 +548,19 @@ LAYER_NORM_MAX_C = 1024
 
 
 def layer_norm_supported(C: int) -> bool:
-    """Feature counts the CUDA LayerNorm handles (C % 4 == 0, C <= 1024)."""
+    """Feature counts the CUDA LayerNorm handles in float32 (C % 4 == 0, C <= 1024)."""
     return 0 < C <= LAYER_NORM_MAX_C and C % 4 == 0
 
 
 def layer_norm(x, weight, bias, eps: float = 1e-5):
     """F.layer_norm(x, (C,), weight, bias, eps) over the last axis as one CUDA kernel each way
-    (the blocks' nn.LayerNorm, python/clifford_cl6.py:94,121,229); layer_norm_supported(C) only."""
+    (the blocks' nn.LayerNorm, python/clifford_cl6.py:94,121,229).  bfloat16 and float16 rows of any width
+    are read and written as they are (csrc/csn_layer_norm.cu; statistics and sums in float32, weights
+    of x's type or float32, once differentiable); others are float32, layer_norm_supported(C) only."""
+    if x.dtype in (torch.bfloat16, torch.float16):
+        if weight is None or bias is None:
+            raise ValueError("layer_norm: needs affine weight and bias")
+        return layer_norm_rows(x, weight, bias, eps)
     C = x.shape[-1]
     if not layer_norm_supported(C) or weight is None or bias is None:
         raise ValueError(f"layer_norm: needs affine weight and bias and C % 4 == 0, C <= {LAYER_NORM_MAX_C}")
@@ -841,7 +848,8 @@ def spatial_generators(in_proj, biv_proj, metric, lambda_sw, gamma_log, D: int):
     return SpatialGeneratorsFunction.apply(in_proj, biv_proj, metric, lambda_sw, gamma_log, D)
 
 
-# the gated recurrent block's ops and the torch.ops.csn.* registrations (both need the helpers
+# the gated recurrent and linear-attention blocks' ops and the torch.ops.csn.* registrations (both need the helpers
 # above; imported last on purpose)
 from .gated import dropout_add, gated_scan, gated_step, silu_gated_linear  # noqa: E402
+from .linear_attention import layer_norm_rows, linear_attention, linear_attention_step  # noqa: E402
 from . import library  # noqa: E402,F401

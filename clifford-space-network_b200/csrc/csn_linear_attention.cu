@@ -1,0 +1,473 @@
+// csn_linear_attention.cu -- linear attention with a decay for each head, its adjoint and its step.
+#include "csn_linear_attention.cuh"
+
+#include <algorithm>
+#include <cstdio>
+
+namespace csn {
+namespace {
+
+using namespace la;
+
+constexpr int MAX_D = 128;
+constexpr int BLOCK = 16;        // steps that are worked on together
+constexpr int LINE = BLOCK + 4;  // of shared memory: aligned, and a column of values is spread over the banks
+
+// n steps from X, in their order of processing (BACK: time runs down; X carried is Y, after its fade):
+//   out_i = so (l^(i+1) X^T a_i + sum over j <= i of l^(i-j) sb (a_i . b_j) v_j),   X <- l^n X + sum of l^(n-1-j) sb b_j v_j^T
+// (one power of l less before the first product and one more in the last sum where time runs down).  A thread has one
+// place of v and the K entries of the state beside it in registers: two FMA an entry and step, the products a . b shared by
+// all threads.  The state is rounded once a block: step by step, a memory of thousands of steps costs it a digit.
+// OUT: false for the first pass.
+template <typename T, int KP, int VP, bool OUT>
+__global__ void __launch_bounds__(VP) blocks_kernel(const Batch B, const Pass P) {
+  const Unit U(B, blockIdx.x);
+  if (U.s < 0 || (!OUT && U.ends(P.back))) return;
+  constexpr int NJ = BLOCK * BLOCK / VP;  // products of a thread
+  const int h = blockIdx.y, c = threadIdx.x, late = P.back ? 1 : 0;
+  const bool mine = c < P.V;
+  __shared__ __align__(16) float as[OUT ? KP : 1][LINE], bs[KP][LINE], prod[OUT ? BLOCK : 1][LINE];
+  __shared__ float power[BLOCK + 2];
+  if (c < BLOCK + 2) power[c] = fade(B.log_decay[h], c);
+  const int64_t size = (int64_t)P.K * P.V;
+  float x[KP];
+#pragma unroll
+  for (int i = 0; i < KP; ++i) x[i] = 0.0f;
+  if (OUT && P.state && mine) {
+    const float* p = P.state + ((P.by_unit ? U.unit : U.s) * B.H + h) * size + c * P.sc;
+#pragma unroll
+    for (int i = 0; i < KP; ++i)
+      if (i < P.K) x[i] = p[i * P.sr];
+  }
+  const T* a = static_cast<const T*>(P.a.p) + U.start(B, P.a) + h / P.a.shared * P.a.head;
+  const T* b = static_cast<const T*>(P.b.p) + U.start(B, P.b) + h / P.b.shared * P.b.head;
+  const T* v = static_cast<const T*>(P.v.p) + U.start(B, P.v) + h / P.v.shared * P.v.head;
+  for (int i = c; i < KP * LINE; i += VP) {
+    if (OUT) as[OUT ? i / LINE : 0][i % LINE] = 0.0f;
+    bs[i / LINE][i % LINE] = 0.0f;
+  }
+  const int steps = U.to - U.from;
+  for (int done = 0; done < steps; done += BLOCK) {
+    const int n = min(BLOCK, steps - done);
+    __syncthreads();
+    float vs[BLOCK];
+#pragma unroll
+    for (int i = 0; i < BLOCK; ++i) {
+      const bool in = i < n;
+      const int64_t t = P.back ? U.to - 1 - done - i : U.from + done + i;
+      vs[i] = in && mine ? to_float(v[t * P.v.row + c]) * P.sb : 0.0f;
+      for (int d = c; d < P.K; d += VP) {
+        if (OUT) as[OUT ? d : 0][i] = in ? to_float(a[t * P.a.row + d]) : 0.0f;
+        bs[d][i] = in ? to_float(b[t * P.b.row + d]) : 0.0f;
+      }
+    }
+    __syncthreads();
+    if (OUT) {
+      const int i = c % BLOCK, j0 = c / BLOCK * NJ;
+      float r[NJ] = {};
+#pragma unroll 8
+      for (int d = 0; d < KP; ++d) {
+        const float ai = as[OUT ? d : 0][i];
+        const Pack<float, NJ> bj = *reinterpret_cast<const Pack<float, NJ>*>(&bs[d][j0]);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) r[j] = fmaf(ai, bj.v[j], r[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) prod[OUT ? i : 0][j0 + j] = j0 + j <= i ? r[j] * power[i - j0 - j] : 0.0f;
+    }
+    float o[BLOCK] = {}, w[BLOCK];
+#pragma unroll
+    for (int i = 0; i < BLOCK; ++i) w[i] = i < n ? vs[i] * power[n - 1 - i + late] : 0.0f;
+    const float whole = power[n];
+#pragma unroll
+    for (int d = 0; d < KP; ++d) {
+      float t = 0.0f;
+#pragma unroll
+      for (int i = 0; i < BLOCK; i += 4) {
+        const float4 b4 = *reinterpret_cast<const float4*>(&bs[d][i]);
+        if (OUT) {
+          const float4 a4 = *reinterpret_cast<const float4*>(&as[OUT ? d : 0][i]);
+          o[i] = fmaf(a4.x, x[d], o[i]), o[i + 1] = fmaf(a4.y, x[d], o[i + 1]);
+          o[i + 2] = fmaf(a4.z, x[d], o[i + 2]), o[i + 3] = fmaf(a4.w, x[d], o[i + 3]);
+        }
+        t = fmaf(b4.x, w[i], t), t = fmaf(b4.y, w[i + 1], t);
+        t = fmaf(b4.z, w[i + 2], t), t = fmaf(b4.w, w[i + 3], t);
+      }
+      x[d] = fmaf(whole, x[d], t);
+    }
+    if (!OUT) continue;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < BLOCK; ++i) {
+      float r = 0.0f;
+#pragma unroll
+      for (int j = 0; j <= i; j += 4) {
+        const float4 p4 = *reinterpret_cast<const float4*>(&prod[OUT ? i : 0][j]);
+        const float pv[4] = {p4.x, p4.y, p4.z, p4.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (j + e <= i) r = fmaf(pv[e], vs[j + e], r);  // a later step's infinity has to stay out
+      }
+      if (i >= n || !mine) continue;
+      r = fmaf(power[i + 1 - late], o[i], r) * P.so;
+      const int64_t t = U.row0 + (P.back ? U.to - 1 - done - i : U.from + done + i), at = (t * B.H + h) * P.V + c;
+      if (P.wide) static_cast<float*>(P.out)[at] = r;
+      else static_cast<T*>(P.out)[at] = from_float<T>(r);
+    }
+  }
+  float* to = OUT ? (P.last && U.ends(P.back) ? P.last + (U.s * B.H + h) * size : nullptr) : P.made + (U.unit * B.H + h) * size;
+  if (to && mine) {
+#pragma unroll
+    for (int i = 0; i < KP; ++i)
+      if (i < P.K) to[i * P.sr + c * P.sc] = x[i];
+  }
+}
+
+// What enters each segment, in place of what it made: made[u] holds the sum of a unit's own steps.
+__global__ void __launch_bounds__(256) join_kernel(const Batch B, const float* __restrict__ enters, float* made, int size, bool back) {
+  const int64_t s = blockIdx.x;
+  const int h = blockIdx.y, i = blockIdx.z * 256 + threadIdx.x;
+  if (i >= size) return;
+  const int64_t row0 = B.cu ? Unit::border(B, s) : s * B.T;
+  const int64_t len = B.cu ? max(Unit::border(B, s + 1), row0) - row0 : B.T;
+  const int64_t first = B.cu ? row0 / B.seg + s : s * B.segs, n = max((len + B.seg - 1) / B.seg, (int64_t)1);
+  const float whole = fade(B.log_decay[h], B.seg);
+  float x = enters ? enters[(s * B.H + h) * size + i] : 0.0f;
+  for (int64_t j = 0; j < n; ++j) {
+    const int64_t m = back ? n - 1 - j : j;
+    float* p = made + ((first + m) * B.H + h) * size + i;
+    const float own = j + 1 < n ? *p : 0.0f;
+    *p = x;
+    const float f = (m + 1) * B.seg > len ? fade(B.log_decay[h], (int)(len - m * B.seg)) : whole;
+    x = fmaf(f, x, own);
+  }
+}
+
+// [rows][H][D] float32 to [rows][H / shared][D] of type T
+template <typename T>
+__global__ void __launch_bounds__(256) gather_kernel(const float* __restrict__ part, T* out, int64_t n, int D, int shared) {
+  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const float* p = part + i / D * shared * D + i % D;
+    float v = p[0];
+    for (int j = 1; j < shared; ++j) v += p[(int64_t)j * D];
+    out[i] = from_float<T>(v);
+  }
+}
+
+// Rows of no sequence are 0: those before the first border and from the last one on.
+__global__ void __launch_bounds__(256) outside_kernel(const Batch B, uint16_t* out, int64_t row) {
+  const int64_t a = Unit::border(B, 0) * row, b = max(Unit::border(B, B.S) * row, a), n = a + B.T * row - b;
+  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
+    out[i < a ? i : i - a + b] = 0;
+}
+
+// ------------------------------------------------------------------------- step
+struct StepArgs {
+  const void *q, *k, *v;
+  int64_t qs, qh, ks, kh, vs, vh;  // strides of stream and head
+  const float* log_decay;
+  float* s;
+  void* o;
+  int H, shared, Dk, Dv;
+  float scale;
+};
+
+// A CTA has one head of one stream.  VEC neighbouring entries of a row of the state belong to a thread, 1 << WIDE threads
+// take a row and the others the rows that follow, ROWS of them in flight.
+constexpr int STEP_THREADS = 256;
+template <typename T, int VEC, int ROWS>
+__global__ void __launch_bounds__(STEP_THREADS) step_kernel(const StepArgs A, int wide) {
+  __shared__ float qs[MAX_D], ks[MAX_D], vs[MAX_D];
+  __shared__ float part[STEP_THREADS * VEC];
+  const int h = blockIdx.x % A.H, tid = threadIdx.x;
+  const int64_t b = blockIdx.x / A.H;
+  const int c = (tid & ((1 << wide) - 1)) * VEC, r0 = tid >> wide, step = STEP_THREADS >> wide;
+  float* s = A.s + (b * A.H + h) * (int64_t)A.Dk * A.Dv + c;
+  const bool mine = c < A.Dv;
+  using Row = Pack<float, VEC>;
+  Row x[ROWS];
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i)
+    if (mine && r0 + i * step < A.Dk) x[i] = *reinterpret_cast<const Row*>(s + (int64_t)(r0 + i * step) * A.Dv);
+  if (tid < A.Dk) {
+    qs[tid] = to_float(static_cast<const T*>(A.q)[b * A.qs + h * A.qh + tid]) * A.scale;
+    ks[tid] = to_float(static_cast<const T*>(A.k)[b * A.ks + h / A.shared * A.kh + tid]);
+  }
+  if (tid < A.Dv) vs[tid] = to_float(static_cast<const T*>(A.v)[b * A.vs + h / A.shared * A.vh + tid]);
+  const float l = expf(A.log_decay[h]);
+  __syncthreads();
+  float o[VEC] = {}, v[VEC] = {};
+  if (mine) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = vs[c + e];
+    for (int r = r0;;) {
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) {
+        const int k = r + i * step;
+        if (k >= A.Dk) break;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          x[i].v[e] = fmaf(ks[k], v[e], l * x[i].v[e]);
+          o[e] = fmaf(qs[k], x[i].v[e], o[e]);
+        }
+        *reinterpret_cast<Row*>(s + (int64_t)k * A.Dv) = x[i];
+      }
+      r += ROWS * step;
+      if (r >= A.Dk) break;
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i)
+        if (r + i * step < A.Dk) x[i] = *reinterpret_cast<const Row*>(s + (int64_t)(r + i * step) * A.Dv);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) part[tid * VEC + e] = o[e];
+  __syncthreads();
+  if (tid < A.Dv) {
+    float r = 0.0f;
+    for (int i = 0; i < step; ++i) r += part[(i << wide) * VEC + tid];
+    static_cast<T*>(A.o)[(b * A.H + h) * A.Dv + tid] = from_float<T>(r);
+  }
+}
+
+// ------------------------------------------------------------------------- host
+int width_of(int dtype) { return dtype == CSN_F32 ? 4 : dtype == CSN_BF16 || dtype == CSN_F16 ? 2 : 0; }
+bool aligned(const void* p, int n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// The steps of a segment: enough segments for 12 warps on each of 148 SMs, none shorter than 128 steps.
+void cut(Batch& B, int V, bool packed) {
+  const int64_t warps = up(V, 32) * B.H * (packed ? 1 : B.S), want = up(148 * 12, warps);
+  B.seg = (int)(up(std::max(up(B.T, want), (int64_t)128), 64) * 64);
+  B.segs = packed ? 0 : (int)std::max(up(B.T, B.seg), (int64_t)1);
+  B.units = packed ? B.T / B.seg + B.S : B.S * B.segs;
+}
+bool is_cut(const Batch& B, bool packed) { return packed ? B.T > B.seg : B.segs > 1; }
+
+Batch batch(int64_t S, int64_t T, int H, int Dk, int Dv, const int32_t* cu, bool packed, const float* log_decay) {
+  Batch B = {cu, S, T, H, 0, 0, 0, log_decay};
+  cut(B, std::min(Dk, Dv), packed);
+  return B;
+}
+
+struct Room {  // in floats
+  int64_t states, dk, dv;
+  size_t bytes(bool backward) const { return sizeof(float) * (size_t)((backward ? 2 : 1) * states + dk + dv); }
+};
+Room room(const Batch& B, int Hk, int Dk, int Dv, bool packed, bool backward) {
+  const int64_t rows = packed ? B.T : B.S * B.T;
+  const bool shared = backward && Hk < B.H;
+  return {is_cut(B, packed) ? up(B.units * B.H * Dk * Dv, 4) * 4 : 0, shared ? up(rows * B.H * Dk, 4) * 4 : 0,
+          shared ? up(rows * B.H * Dv, 4) * 4 : 0};
+}
+
+template <typename T, int KP, int VP>
+void launch_blocks(const Batch& B, const Pass& P, bool first, cudaStream_t st) {
+  const dim3 grid((unsigned)B.units, (unsigned)B.H);
+  if (first) blocks_kernel<T, KP, VP, false><<<grid, VP, 0, st>>>(B, P);
+  else blocks_kernel<T, KP, VP, true><<<grid, VP, 0, st>>>(B, P);
+}
+template <typename T, int KP>
+void launch_blocks(const Batch& B, const Pass& P, bool first, cudaStream_t st) {
+  if (P.V <= 32) launch_blocks<T, KP, 32>(B, P, first, st);
+  else if (P.V <= 64) launch_blocks<T, KP, 64>(B, P, first, st);
+  else launch_blocks<T, KP, 128>(B, P, first, st);
+}
+template <typename T>
+void launch_blocks(const Batch& B, const Pass& P, bool first, cudaStream_t st) {
+  if (P.K <= 32) launch_blocks<T, 32>(B, P, first, st);
+  else if (P.K <= 64) launch_blocks<T, 64>(B, P, first, st);
+  else launch_blocks<T, 128>(B, P, first, st);
+}
+
+int run(const Batch& B, const Pass* passes, int count, bool first, int dtype, cudaStream_t st) {
+  for (int i = 0; i < count; ++i) {
+    KernelTimer kt(first ? "linear_attention_first" : "linear_attention", st);
+    if (dtype == CSN_F32) launch_blocks<float>(B, passes[i], first, st);
+    else if (dtype == CSN_BF16) launch_blocks<__nv_bfloat16>(B, passes[i], first, st);
+    else launch_blocks<__half>(B, passes[i], first, st);
+  }
+  return CSN_OK;
+}
+
+void join(const Batch& B, const float* enters, float* made, int size, bool back, cudaStream_t st) {
+  KernelTimer kt("linear_attention_join", st);
+  join_kernel<<<dim3((unsigned)B.S, (unsigned)B.H, (unsigned)up(size, 256)), 256, 0, st>>>(B, enters, made, size, back);
+}
+
+void clear_outside(const Batch& B, void* out, int64_t row_bytes, cudaStream_t st) {
+  if (B.cu) outside_kernel<<<64, 256, 0, st>>>(B, static_cast<uint16_t*>(out), row_bytes / 2);
+}
+
+int check_sizes(const char* name, int64_t S, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, int dtype) {
+  static thread_local char text[160];
+  const char* wrong = S < 0 || T < 0 || H < 0 || Hk < 0 ? "negative size" : nullptr;
+  if (!wrong && (H > 0 && (Hk < 1 || H % Hk))) wrong = "the heads of k and v have to divide those of q";
+  if (!wrong && (S > (1 << 30) || T > (1 << 30) || H > 65535)) wrong = "at most 2^30 sequences and steps and 65535 heads";
+  int code = CSN_ERR_INVALID;
+  if (!wrong && (Dk < 1 || Dv < 1 || Dk > MAX_D || Dv > MAX_D)) wrong = "head sizes of 1 to 128", code = CSN_ERR_UNSUPPORTED;
+  if (!wrong && !width_of(dtype)) wrong = "dtype is float32, bfloat16 or float16", code = CSN_ERR_UNSUPPORTED;
+  if (!wrong) return CSN_OK;
+  snprintf(text, sizeof text, "%s: %s", name, wrong);
+  return set_error(code, text);
+}
+
+Stream stream_of(const void* p, const int64_t* st, int shared) { return {p, st[0], st[1], st[2], shared}; }
+
+}  // namespace
+}  // namespace csn
+
+using namespace csn;
+using namespace csn::la;
+
+extern "C" size_t csn_linear_attention_workspace_bytes(int64_t S, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv,
+                                                       int packed, int dtype, int backward) {
+  if (S <= 0 || T <= 0 || H <= 0 || Hk <= 0 || check_sizes("csn_linear_attention_workspace_bytes", S, T, H, Hk, Dk, Dv, dtype) != CSN_OK)
+    return 0;
+  const Batch B = batch(S, T, (int)H, (int)Dk, (int)Dv, nullptr, packed != 0, nullptr);
+  return room(B, (int)Hk, (int)Dk, (int)Dv, packed != 0, backward != 0).bytes(backward != 0);
+}
+
+extern "C" int csn_linear_attention_fwd(const void* q, const void* k, const void* v, const int64_t* strides, const float* log_decay,
+                                        const float* s0, const int32_t* cu_seqlens, void* o, float* s_last, int64_t S, int64_t T,
+                                        int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, float scale, int dtype, void* workspace,
+                                        size_t workspace_bytes, void* stream) {
+  if (int rc = check_sizes("csn_linear_attention_fwd", S, T, H, Hk, Dk, Dv, dtype)) return rc;
+  if (S == 0 || H == 0) return CSN_OK;
+  const int size = width_of(dtype);
+  const bool packed = cu_seqlens != nullptr, rows = T > 0;
+  if (!log_decay || !aligned(s0, 16) || !aligned(s_last, 16) ||
+      (rows && (!q || !k || !v || !strides || !o || !aligned(q, size) || !aligned(k, size) || !aligned(v, size) || !aligned(o, 16))))
+    return set_error(CSN_ERR_INVALID, "csn_linear_attention_fwd: missing or misaligned pointer");
+  const Batch B = batch(S, T, (int)H, (int)Dk, (int)Dv, cu_seqlens, packed, log_decay);
+  const Room R = room(B, (int)Hk, (int)Dk, (int)Dv, packed, false);
+  if (R.bytes(false) && (!workspace || workspace_bytes < R.bytes(false) || !aligned(workspace, 16)))
+    return set_error(CSN_ERR_INVALID, "csn_linear_attention_fwd: workspace smaller than csn_linear_attention_workspace_bytes");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int shared = (int)(H / Hk), entries = (int)(Dk * Dv);
+  static const int64_t none[9] = {};
+  const int64_t* ss = strides ? strides : none;
+  Pass P = {stream_of(q, ss, 1), stream_of(k, ss + 3, shared), stream_of(v, ss + 6, shared), o, s0, s_last, nullptr, Dv, 1,
+            (int)Dk, (int)Dv, scale, 1.0f, false, false, false};
+  if (R.states) {
+    P.made = static_cast<float*>(workspace);
+    if (int rc = run(B, &P, 1, true, dtype, st)) return rc;
+    join(B, s0, P.made, entries, false, st);
+    P.state = P.made;
+    P.by_unit = true;
+  }
+  if (int rc = run(B, &P, 1, false, dtype, st)) return rc;
+  if (rows) clear_outside(B, o, H * Dv * size, st);
+  return check_launch("csn_linear_attention_fwd");
+}
+
+extern "C" int csn_linear_attention_bwd(const void* q, const void* k, const void* v, const void* d_o, const int64_t* strides,
+                                        const float* log_decay, const float* s0, const int32_t* cu_seqlens, const float* ds_last,
+                                        void* dq, void* dk, void* dv, float* ds0, int64_t S, int64_t T, int64_t H, int64_t Hk,
+                                        int64_t Dk, int64_t Dv, float scale, int dtype, void* workspace, size_t workspace_bytes,
+                                        void* stream) {
+  if (int rc = check_sizes("csn_linear_attention_bwd", S, T, H, Hk, Dk, Dv, dtype)) return rc;
+  if (S == 0 || H == 0) return CSN_OK;
+  const int size = width_of(dtype);
+  const bool packed = cu_seqlens != nullptr, rows = T > 0;
+  if (!log_decay || !aligned(s0, 16) || !aligned(ds_last, 16) || !aligned(ds0, 16) ||
+      (rows && (!q || !k || !v || !d_o || !strides || (ds0 && !dv) || !aligned(q, size) || !aligned(k, size) || !aligned(v, size) ||
+                !aligned(d_o, size) || !aligned(dq, 16) || !aligned(dk, 16) || !aligned(dv, 16))))
+    return set_error(CSN_ERR_INVALID, "csn_linear_attention_bwd: missing or misaligned pointer");
+  const Batch B = batch(S, T, (int)H, (int)Dk, (int)Dv, cu_seqlens, packed, log_decay);
+  const Room R = room(B, (int)Hk, (int)Dk, (int)Dv, packed, true);
+  if (R.bytes(true) && (!workspace || workspace_bytes < R.bytes(true) || !aligned(workspace, 16)))
+    return set_error(CSN_ERR_INVALID, "csn_linear_attention_bwd: workspace smaller than csn_linear_attention_workspace_bytes");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int shared = (int)(H / Hk), entries = (int)(Dk * Dv);
+  static const int64_t none[12] = {};
+  const int64_t* ss = strides ? strides : none;
+  const Stream Q = stream_of(q, ss, 1), K = stream_of(k, ss + 3, shared), V = stream_of(v, ss + 6, shared), O = stream_of(d_o, ss + 9, 1);
+  float* ws = static_cast<float*>(workspace);
+  float *made = ws, *back = ws + R.states, *dk32 = back + R.states, *dv32 = dk32 + R.dk;
+  Pass P[3] = {
+      {O, V, K, dq, s0, nullptr, nullptr, 1, Dv, (int)Dv, (int)Dk, scale, 1.0f, false, false, false},
+      {V, O, Q, shared > 1 ? dk32 : dk, ds_last, nullptr, nullptr, 1, Dv, (int)Dv, (int)Dk, 1.0f, scale, false, shared > 1, true},
+      {K, Q, O, shared > 1 ? dv32 : dv, ds_last, ds0, nullptr, Dv, 1, (int)Dk, (int)Dv, 1.0f, scale, false, shared > 1, true}};
+  if (R.states) {
+    P[0].made = made, P[2].made = back;
+    const int from = dq ? 0 : 2, to = dk || dv ? 2 : 0;  // the states of the forward direction are those that dq needs
+    for (int i = from; i <= to; i += 2)
+      if (int rc = run(B, &P[i], 1, true, dtype, st)) return rc;
+    if (dq) join(B, s0, made, entries, false, st);
+    if (dk || dv) join(B, ds_last, back, entries, true, st);
+    P[0].state = made, P[1].state = P[2].state = back;
+    for (Pass& p : P) p.by_unit = true;
+  }
+  Pass wanted[3];
+  int count = 0;
+  if (dq) wanted[count++] = P[0];
+  if (dk) wanted[count++] = P[1];
+  if (dv || ds0) wanted[count++] = P[2];
+  if (int rc = run(B, wanted, count, false, dtype, st)) return rc;
+  if (rows) {
+    const int64_t n = packed ? T : S * T;
+    if (shared > 1) {
+      KernelTimer kt("linear_attention_gather", st);
+      auto gather = [&](const float* part, void* out, int64_t D) {
+        const int64_t count = n * Hk * D;
+        const unsigned grid = (unsigned)std::min(up(count, 256), (int64_t)148 * 16);
+        if (dtype == CSN_F32) gather_kernel<<<grid, 256, 0, st>>>(part, static_cast<float*>(out), count, (int)D, shared);
+        else if (dtype == CSN_BF16) gather_kernel<<<grid, 256, 0, st>>>(part, static_cast<__nv_bfloat16*>(out), count, (int)D, shared);
+        else gather_kernel<<<grid, 256, 0, st>>>(part, static_cast<__half*>(out), count, (int)D, shared);
+      };
+      if (dk) gather(dk32, dk, Dk);
+      if (dv) gather(dv32, dv, Dv);
+    }
+    if (dq) clear_outside(B, dq, H * Dk * size, st);
+    if (dk) clear_outside(B, dk, Hk * Dk * size, st);
+    if (dv) clear_outside(B, dv, Hk * Dv * size, st);
+  }
+  return check_launch("csn_linear_attention_bwd");
+}
+
+namespace csn {
+namespace {
+// whether [p, p + its last element] meets the states
+bool shares(const float* s, int64_t states, const void* p, int64_t B, int64_t bs, int64_t H, int64_t hs, int64_t D, int size) {
+  const char *a = reinterpret_cast<const char*>(s), *b = reinterpret_cast<const char*>(s + states);
+  const int64_t first = std::min((B - 1) * bs, (int64_t)0) + std::min((H - 1) * hs, (int64_t)0);
+  const int64_t last = std::max((B - 1) * bs, (int64_t)0) + std::max((H - 1) * hs, (int64_t)0) + D;
+  const char* c = static_cast<const char*>(p);
+  return c + first * size < b && c + last * size > a;
+}
+
+template <typename T>
+void launch_step(const StepArgs& A, int64_t ctas, cudaStream_t st) {
+  const bool four = A.Dv % 4 == 0;
+  int wide = 0;
+  while ((four ? 4 : 1) << wide < A.Dv) ++wide;
+  if (four) step_kernel<T, 4, 8><<<(unsigned)ctas, STEP_THREADS, 0, st>>>(A, wide);
+  else step_kernel<T, 1, 8><<<(unsigned)ctas, STEP_THREADS, 0, st>>>(A, wide);
+}
+}  // namespace
+}  // namespace csn
+
+extern "C" int csn_linear_attention_step(const void* q, const void* k, const void* v, const int64_t* strides, const float* log_decay,
+                                         float* s, void* o, int64_t B, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, float scale,
+                                         int dtype, void* stream) {
+  if (int rc = check_sizes("csn_linear_attention_step", B, 1, H, Hk, Dk, Dv, dtype)) return rc;
+  if (B == 0 || H == 0) return CSN_OK;
+  const int size = width_of(dtype);
+  if (!q || !k || !v || !strides || !log_decay || !s || !o || !aligned(q, size) || !aligned(k, size) || !aligned(v, size) ||
+      !aligned(s, 16) || !aligned(o, 16))
+    return set_error(CSN_ERR_INVALID, "csn_linear_attention_step: missing or misaligned pointer");
+  if (B * H > 0x7fffffff) return set_error(CSN_ERR_UNSUPPORTED, "csn_linear_attention_step: at most 2^31 - 1 heads in all");
+  const int64_t states = B * H * Dk * Dv;
+  if (shares(s, states, q, B, strides[0], H, strides[1], Dk, size) || shares(s, states, k, B, strides[2], Hk, strides[3], Dk, size) ||
+      shares(s, states, v, B, strides[4], Hk, strides[5], Dv, size) || shares(s, states, o, B, H * Dv, H, Dv, Dv, size) ||
+      shares(s, states, log_decay, 1, 0, 1, 0, H, 4))
+    return set_error(CSN_ERR_INVALID, "csn_linear_attention_step: s shares memory with an input or the result");
+  const StepArgs A = {q, k, v, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], log_decay, s, o,
+                      (int)H, (int)(H / Hk), (int)Dk, (int)Dv, scale};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  KernelTimer kt("linear_attention_step", st);
+  if (dtype == CSN_F32) launch_step<float>(A, B * H, st);
+  else if (dtype == CSN_BF16) launch_step<__nv_bfloat16>(A, B * H, st);
+  else launch_step<__half>(A, B * H, st);
+  return check_launch("csn_linear_attention_step");
+}

@@ -1,4 +1,5 @@
-// csn_torch.cpp -- PyTorch binding of the gated recurrent block's entry points (python module csn_b200._gated).
+// csn_torch.cpp -- PyTorch binding of the gated recurrent and linear-attention blocks' entry points (python module
+// csn_b200._gated).
 //
 // The other entry points are bound with ctypes and torch.autograd.Function.  These are called once a token or once a
 // layer on small tensors, where the host's time for a call is the call's time, so their argument checks, allocations
@@ -348,6 +349,231 @@ std::tuple<Tensor, Tensor, Tensor> silu_gated_linear_backward(const Tensor& x, c
   return {dx.view(x.sizes()), dg, du};
 }
 
+// -------------------------------------------------------------- linear attention
+struct Heads {
+  int64_t S, T, H, Hk, Dk, Dv;
+  Heads(const Tensor& q, const Tensor& k, const Tensor& v, const Maybe& cu)
+      : S(there(cu) ? cu->size(0) - 1 : q.size(0)), T(there(cu) ? q.size(0) : q.size(1)), H(q.size(-2)), Hk(k.size(-2)), Dk(q.size(-1)),
+        Dv(v.size(-1)) {}
+};
+
+// strides of sequence, row and head, 0 where an axis has one entry
+void put_head_strides(int64_t* to, const Tensor& t) {
+  to[0] = 0;
+  const int64_t n = t.dim() - 1;
+  for (int64_t i = 0; i < n; ++i) to[3 - n + i] = t.size(i) > 1 ? t.stride(i) : 0;
+}
+
+// `lead`: axes before the heads
+void check_heads(const char* name, const char* form, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, int64_t lead) {
+  of_one_type(name, true, {&q, &k, &v});
+  bool fits = q.dim() == lead + 2 && k.dim() == q.dim() && v.dim() == q.dim();
+  for (int64_t i = 0; fits && i < lead; ++i) fits = k.size(i) == q.size(i) && v.size(i) == q.size(i);
+  TORCH_CHECK_VALUE(fits && k.size(-1) == q.size(-1) && v.size(-2) == k.size(-2), name, ": q ", form, " k and v with the same rows, k of q's last size, v of "
+                    "k's heads expected, got ", q.sizes(), ", ", k.sizes(), " and ", v.sizes());
+  TORCH_CHECK_VALUE(q.size(-2) >= 1 && k.size(-2) >= 1 && q.size(-2) % k.size(-2) == 0, name, ": the heads of k and v (", k.size(-2),
+                    ") have to divide those of q (", q.size(-2), ")");
+  TORCH_CHECK_VALUE(q.size(-1) >= 1 && q.size(-1) <= 128 && v.size(-1) >= 1 && v.size(-1) <= 128, name, ": head sizes of 1 to 128 expected, got ",
+                    q.size(-1), " and ", v.size(-1));
+  TORCH_CHECK_VALUE(log_decay.scalar_type() == at::kFloat && log_decay.dim() == 1 && log_decay.size(0) == q.size(-2) && log_decay.is_contiguous(),
+                    name, ": log_decay is a contiguous float32 vector with a number for each of the ", q.size(-2), " heads");
+  TORCH_CHECK_VALUE(!wants_grad({&log_decay}), name, ": log_decay has no gradient here: pass it detached");
+}
+
+Heads attention_sizes(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const Maybe& cu) {
+  TORCH_CHECK_VALUE(!there(cu) || (cu->scalar_type() == at::kInt && cu->dim() == 1 && cu->size(0) >= 2 && cu->is_contiguous()),
+                    "linear_attention: cu_seqlens is a contiguous int32 vector of at least 2 row numbers");
+  check_heads("linear_attention", "[B, T, H, D], or [L, H, D] with cu_seqlens,", q, k, v, log_decay, there(cu) ? 1 : 2);
+  return Heads(q, k, v, cu);
+}
+
+void check_states(const char* what, const Maybe& s, const Heads& n) {
+  TORCH_CHECK_VALUE(!there(s) || (s->dim() == 4 && s->size(0) == n.S && s->size(1) == n.H && s->size(2) == n.Dk && s->size(3) == n.Dv &&
+                                  at::isFloatingType(s->scalar_type())),
+                    "linear_attention: ", what, " [", n.S, ", ", n.H, ", ", n.Dk, ", ", n.Dv, "] of a floating type expected");
+}
+
+void check_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const Maybe& s0, const Maybe& cu) {
+  no_tangent("linear_attention", {&q, &k, &v, &log_decay, at_of(s0)});
+  check_states("s0", s0, attention_sizes(q, k, v, log_decay, cu));
+  on_one_device("linear_attention", {&q, &k, &v, &log_decay, at_of(s0), at_of(cu)});
+}
+
+double scale_of(const optional<double>& scale, int64_t Dk) { return scale ? *scale : 1.0 / std::sqrt((double)Dk); }
+
+std::tuple<Tensor, Tensor> attention_forward(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& log_decay, const Maybe& s0_,
+                                             const Maybe& cu, double scale) {
+  const c10::cuda::CUDAGuard guard(q_.device());
+  const Tensor q = rows(q_), k = rows(k_), v = rows(v_), s0 = packed(s0_);
+  const Heads n(q, k, v, cu);
+  const int code = code_of(q.scalar_type());
+  std::vector<int64_t> shape(q.sizes().begin(), q.sizes().end());
+  shape.back() = n.Dv;
+  Tensor o = room(q, shape), last = floats(q, {n.S, n.H, n.Dk, n.Dv});
+  const size_t nb = csn_linear_attention_workspace_bytes(n.S, n.T, n.H, n.Hk, n.Dk, n.Dv, there(cu), code, 0);
+  const Tensor ws = bytes(q, nb);
+  int64_t st[9];
+  put_head_strides(st, q), put_head_strides(st + 3, k), put_head_strides(st + 6, v);
+  check("csn_linear_attention_fwd",
+        csn_linear_attention_fwd(ptr(q), ptr(k), ptr(v), st, static_cast<const float*>(ptr(log_decay)), static_cast<const float*>(ptr(s0)),
+                                 static_cast<const int32_t*>(ptr(cu)), ptr(o), static_cast<float*>(ptr(last)), n.S, n.T, n.H, n.Hk, n.Dk,
+                                 n.Dv, (float)scale, code, ptr(ws), nb, stream(q)));
+  return {o, last};
+}
+
+// (dq, dk, dv, ds0), those that are wanted
+std::tuple<Tensor, Tensor, Tensor, Tensor> attention_backward(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& log_decay,
+                                                              const Maybe& s0_, const Maybe& cu, const Maybe& do_, const Maybe& dlast_,
+                                                              double scale, bool want_q, bool want_k, bool want_v, bool want_s0) {
+  const c10::cuda::CUDAGuard guard(q_.device());
+  const Tensor q = rows(q_), k = rows(k_), v = rows(v_), s0 = packed(s0_), dlast = packed(dlast_);
+  const Heads n(q, k, v, cu);
+  std::vector<int64_t> shape(q.sizes().begin(), q.sizes().end());
+  shape.back() = n.Dv;
+  // only the last states are used: a zero for every place
+  const Tensor d = there(do_) ? rows(*do_) : at::zeros(std::vector<int64_t>(q.dim() - 1, 1), q.options()).unsqueeze(-1).expand(shape).contiguous();
+  const int code = code_of(q.scalar_type());
+  Tensor dq = want_q ? room(q, q.sizes()) : Tensor(), dk = want_k ? room(k, k.sizes()) : Tensor();
+  Tensor dv = want_v || want_s0 ? room(v, v.sizes()) : Tensor(), ds0 = want_s0 ? floats(q, {n.S, n.H, n.Dk, n.Dv}) : Tensor();
+  const size_t nb = csn_linear_attention_workspace_bytes(n.S, n.T, n.H, n.Hk, n.Dk, n.Dv, there(cu), code, 1);
+  const Tensor ws = bytes(q, nb);
+  int64_t st[12];
+  put_head_strides(st, q), put_head_strides(st + 3, k), put_head_strides(st + 6, v), put_head_strides(st + 9, d);
+  check("csn_linear_attention_bwd",
+        csn_linear_attention_bwd(ptr(q), ptr(k), ptr(v), ptr(d), st, static_cast<const float*>(ptr(log_decay)),
+                                 static_cast<const float*>(ptr(s0)), static_cast<const int32_t*>(ptr(cu)),
+                                 static_cast<const float*>(ptr(dlast)), ptr(dq), ptr(dk), ptr(dv), static_cast<float*>(ptr(ds0)), n.S, n.T,
+                                 n.H, n.Hk, n.Dk, n.Dv, (float)scale, code, ptr(ws), nb, stream(q)));
+  return {dq, dk, want_v ? dv : Tensor(), ds0};
+}
+
+// The backward pass on tensors of any origin, which are looked at first.
+std::tuple<Tensor, Tensor, Tensor, Tensor> linear_attention_backward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay,
+                                                                     const Maybe& s0, const Maybe& cu, const Tensor& d, const Tensor& dlast,
+                                                                     optional<double> scale) {
+  no_tangent("linear_attention", {&q, &k, &v, &log_decay, at_of(s0), &d, &dlast});
+  const Heads n = attention_sizes(q, k, v, log_decay, cu);
+  check_states("s0", s0, n);
+  check_states("ds_last", dlast, n);
+  of_one_type("linear_attention", true, {&q, &d});
+  std::vector<int64_t> shape(q.sizes().begin(), q.sizes().end());
+  shape.back() = n.Dv;
+  TORCH_CHECK_VALUE(d.sizes() == at::IntArrayRef(shape), "linear_attention: do of the result's shape expected, got ", d.sizes());
+  on_one_device("linear_attention", {&q, &k, &v, &log_decay, at_of(s0), at_of(cu), &d, &dlast});
+  return attention_backward(q, k, v, log_decay, there(s0) ? Maybe(s0->to(at::kFloat)) : s0, cu, d, dlast.to(at::kFloat), scale_of(scale, n.Dk),
+                            true, true, true, true);
+}
+
+struct LinearAttention : torch::autograd::Function<LinearAttention> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay,
+                               const Maybe& s0, const Maybe& cu, double scale) {
+    ctx->set_materialize_grads(false);
+    auto [o, last] = attention_forward(q, k, v, log_decay, s0, cu, scale);
+    ctx->save_for_backward({q, k, v, log_decay, there(s0) ? *s0 : Tensor(), there(cu) ? *cu : Tensor()});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["s0"] = there(s0) && s0->requires_grad();
+    return {o, last};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    if (!g[0].defined() && !g[1].defined()) return variable_list(7);
+    no_tangent("linear_attention", {&g[0], &g[1]});
+    const auto s = ctx->get_saved_variables();
+    auto [dq, dk, dv, ds0] = [&] {
+      at::AutoGradMode off(false);
+      return attention_backward(s[0], s[1], s[2], s[3], s[4], s[5], g[0], g[1], ctx->saved_data["scale"].toDouble(), ctx->needs_input_grad(0),
+                                ctx->needs_input_grad(1), ctx->needs_input_grad(2), ctx->saved_data["s0"].toBool());
+    }();
+    return first_order({dq, dk, dv, Tensor(), ds0, Tensor(), Tensor()});
+  }
+};
+
+std::tuple<Tensor, Tensor> linear_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const Maybe& s0_,
+                                            const Maybe& cu, optional<double> scale_) {
+  check_attention(q, k, v, log_decay, s0_, cu);
+  const Maybe s0 = there(s0_) && s0_->scalar_type() != at::kFloat ? Maybe(s0_->to(at::kFloat)) : s0_;
+  const double scale = scale_of(scale_, q.size(-1));
+  if (!wants_grad({&q, &k, &v, at_of(s0)})) return attention_forward(q, k, v, log_decay, s0, cu, scale);
+  variable_list out = LinearAttention::apply(q, k, v, log_decay, s0, cu, scale);
+  return {out[0], out[1]};
+}
+
+Tensor linear_attention_step(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& log_decay, const Tensor& s,
+                             optional<double> scale) {
+  no_tangent("linear_attention_step", {&q_, &k_, &v_, &log_decay, &s});
+  on_one_device("linear_attention_step", {&q_, &k_, &v_, &log_decay, &s});
+  check_heads("linear_attention_step", "[B, H, D],", q_, k_, v_, log_decay, 1);
+  const int64_t B = q_.size(0), H = q_.size(1), Hk = k_.size(1), Dk = q_.size(2), Dv = v_.size(2);
+  TORCH_CHECK_VALUE(s.dim() == 4 && s.size(0) == B && s.size(1) == H && s.size(2) == Dk && s.size(3) == Dv && s.scalar_type() == at::kFloat &&
+                        s.is_contiguous() && reinterpret_cast<uintptr_t>(s.data_ptr()) % 16 == 0,
+                    "linear_attention_step: s is a contiguous float32 state [", B, ", ", H, ", ", Dk, ", ", Dv, "], 16-byte aligned");
+  TORCH_CHECK_VALUE(!wants_grad({&q_, &k_, &v_, &s}),
+                    "linear_attention_step: not differentiable; call it under torch.no_grad() or use linear_attention");
+  const c10::cuda::CUDAGuard guard(q_.device());
+  const Tensor q = rows(q_), k = rows(k_), v = rows(v_);
+  Tensor o = room(q, {B, H, Dv});
+  s.unsafeGetTensorImpl()->bump_version();  // first: it raises where s may not be changed
+  const int64_t st[6] = {q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1)};
+  check("csn_linear_attention_step",
+        csn_linear_attention_step(ptr(q), ptr(k), ptr(v), st, static_cast<const float*>(ptr(log_decay)), static_cast<float*>(ptr(s)), ptr(o), B,
+                                  H, Hk, Dk, Dv, (float)scale_of(scale, Dk), code_of(q.scalar_type()), stream(q)));
+  return o;
+}
+
+// --------------------------------------------------------- layer norm of 16-bit rows
+std::tuple<Tensor, Tensor> norm_forward(const Tensor& x, const Tensor& w_, const Tensor& b_, double eps, bool keep) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Tensor w = w_.contiguous(), b = b_.contiguous();
+  const int64_t R = x.size(0), C = x.size(1);
+  Tensor y = room(x, {R, C}), kept = keep ? floats(x, {2, R}) : Tensor();
+  float* k = static_cast<float*>(ptr(kept));
+  check("csn_layer_norm_rows_fwd", csn_layer_norm_rows_fwd(ptr(x), x.stride(0), ptr(w), ptr(b), ptr(y), k, k ? k + R : nullptr, R, C, (float)eps,
+                                                           code_of(x.scalar_type()), code_of(w.scalar_type()), stream(x)));
+  return {y, kept};
+}
+
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& b, double eps) {
+    auto [y, kept] = norm_forward(x, w, b, eps, true);
+    ctx->save_for_backward({x, w, kept});
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto s = ctx->get_saved_variables();
+    no_tangent("layer_norm", {&g[0]});
+    auto [dx, dw, db] = [&] {
+      at::AutoGradMode off(false);
+      const Tensor &x = s[0], w = s[1].contiguous(), &kept = s[2], dy = rows(g[0]);
+      const c10::cuda::CUDAGuard guard(x.device());
+      const int64_t R = x.size(0), C = x.size(1);
+      Tensor dx = ctx->needs_input_grad(0) ? room(x, {R, C}) : Tensor(), dw = ctx->needs_input_grad(1) ? room(w, {C}) : Tensor();
+      Tensor db = ctx->needs_input_grad(2) ? room(w, {C}) : Tensor();
+      const size_t nb = dw.defined() || db.defined() ? csn_layer_norm_rows_bwd_workspace_bytes(R, C) : 0;
+      const Tensor ws = bytes(x, nb);
+      const float* k = static_cast<const float*>(ptr(kept));
+      check("csn_layer_norm_rows_bwd",
+            csn_layer_norm_rows_bwd(ptr(dy), dy.stride(0), ptr(x), x.stride(0), k, k + R, ptr(w), ptr(dx), ptr(dw), ptr(db), R, C,
+                                    code_of(x.scalar_type()), code_of(w.scalar_type()), ptr(ws), nb, stream(x)));
+      return std::make_tuple(dx, dw, db);
+    }();
+    return first_order({dx, dw, db, Tensor()});
+  }
+};
+
+Tensor layer_norm_rows(const Tensor& x, const Tensor& w_, const Tensor& b_, double eps) {
+  no_tangent("layer_norm", {&x, &w_, &b_});
+  of_one_type("layer_norm", false, {&x});
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1 && w_.dim() == 1 && b_.dim() == 1 && w_.size(0) == x.size(-1) && b_.size(0) == x.size(-1),
+                    "layer_norm: x [..., C], weight and bias [C] expected, got ", x.sizes(), ", ", w_.sizes(), " and ", b_.sizes());
+  TORCH_CHECK_VALUE(at::isFloatingType(w_.scalar_type()) && at::isFloatingType(b_.scalar_type()), "layer_norm: weight and bias of a floating type expected");
+  on_one_device("layer_norm", {&x, &w_, &b_});
+  // weights of another type than the rows' are taken as float32
+  const bool same = w_.scalar_type() == x.scalar_type() && b_.scalar_type() == x.scalar_type();
+  const Tensor w = same ? w_ : w_.to(at::kFloat), b = same ? b_ : b_.to(at::kFloat);
+  const Tensor r = rows(flat(x));
+  Tensor y = wants_grad({&x, &w, &b}) ? LayerNorm::apply(r, w, b, eps) : std::get<0>(norm_forward(r, w, b, eps, false));
+  return x.dim() == 2 ? y : y.view(x.sizes());
+}
+
 // ------------------------------------------------------------------------ dropout
 Tensor dropout_run(const Tensor& x_, const Maybe& residual_, int64_t cut, const Tensor& rng) {
   const c10::cuda::CUDAGuard guard(x_.device());
@@ -410,4 +636,13 @@ PYBIND11_MODULE(_gated, m) {
   m.def("silu_gated_linear", &silu_gated_linear);
   m.def("silu_gated_linear_backward", &silu_gated_linear_backward);
   m.def("dropout_add", &dropout_add);
+  m.def("linear_attention", &linear_attention);
+  m.def("linear_attention_check", &check_attention);
+  m.def("linear_attention_forward", [](const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const Maybe& s0,
+                                       const Maybe& cu, optional<double> scale) {
+    return attention_forward(q, k, v, log_decay, s0, cu, scale_of(scale, q.size(-1)));
+  });
+  m.def("linear_attention_backward", &linear_attention_backward);
+  m.def("linear_attention_step", &linear_attention_step);
+  m.def("layer_norm_rows", &layer_norm_rows);
 }

@@ -474,6 +474,64 @@ int csn_silu_gated_linear_bwd(const void* x, int64_t ldx, const void* w_gate, in
 int csn_dropout_add(const void* x, const void* residual, const int64_t* rng, void* y, int64_t n,
                     int cut, int dtype, void* stream);
 
+/* --------------------------------------------------------------- linear attention */
+/* Attention without a softmax, whose memory of head h fades by l = exp(log_decay[h]) a step:
+ *     S_t = l S_{t-1} + k_t v_t^T,   o_t = scale S_t^T q_t        (S is Dk x Dv, S_{-1} = s0)
+ * q has H heads, k and v have Hk (H % Hk == 0): head h reads head h / (H / Hk) of them.  1 <= Dk,
+ * Dv <= 128.  q, k, v (and do, the backward pass's) element (s, t, h, d) at
+ * ptr + s * strides[3i] + t * strides[3i + 1] + h * strides[3i + 2] + d for i = 0, 1, 2 (3), in
+ * elements, a host array.  Two forms, as for csn_gated_scan_fwd: S sequences of T steps, o
+ * [S, T, H, Dv]; or, with cu_seqlens [S + 1] (device), T rows in all, of which sequence s has cu[s]
+ * .. cu[s+1] - 1, strides[3i] not used, o [T, H, Dv].  Rows of no sequence come out as 0.  Borders
+ * are cut to 0 .. T; they must not fall.
+ * log_decay [H] float32, at most 0 (-inf: nothing is remembered).  s0, s_last [S, H, Dk, Dv]
+ * float32 (NULL: 0, not wanted).
+ * Sums and states are float32.  16-bit tensors of 16-byte aligned rows (and head sizes that are
+ * multiples of 8) go through the tensor cores in blocks of 128 steps: there the products q k^T
+ * inside a block and the state, as an operand of its product with q, are rounded to the tensors'
+ * type, the state that is carried on is not.  An infinity or NaN in k or v can reach the outputs of
+ * its whole block.  Should a device-side wait give up (it is bounded), the results it concerns are
+ * NaN.
+ * The workspace is required where csn_linear_attention_workspace_bytes is not 0.  q, k, v, do
+ * aligned to their type; everything else 16-byte aligned. */
+size_t csn_linear_attention_workspace_bytes(int64_t S, int64_t T, int64_t H, int64_t Hk, int64_t Dk,
+                                            int64_t Dv, int packed, int dtype, int backward);
+int csn_linear_attention_fwd(const void* q, const void* k, const void* v, const int64_t* strides,
+                             const float* log_decay, const float* s0, const int32_t* cu_seqlens,
+                             void* o, float* s_last, int64_t S, int64_t T, int64_t H, int64_t Hk,
+                             int64_t Dk, int64_t Dv, float scale, int dtype, void* workspace,
+                             size_t workspace_bytes, void* stream);
+/* Its adjoint on the same inputs: do and ds_last [S, H, Dk, Dv] (NULL = 0) to dq, dk, dv
+ * (contiguous, in q's, k's and v's shapes; each may be NULL) and ds0 [S, H, Dk, Dv] (NULL = not
+ * wanted; it needs dv). */
+int csn_linear_attention_bwd(const void* q, const void* k, const void* v, const void* d_o,
+                             const int64_t* strides, const float* log_decay, const float* s0,
+                             const int32_t* cu_seqlens, const float* ds_last, void* dq, void* dk,
+                             void* dv, float* ds0, int64_t S, int64_t T, int64_t H, int64_t Hk,
+                             int64_t Dk, int64_t Dv, float scale, int dtype, void* workspace,
+                             size_t workspace_bytes, void* stream);
+/* One step of it for B streams, s [B, H, Dk, Dv] in place: q, k, v element (b, h, d) at
+ * ptr + b * strides[2i] + h * strides[2i + 1] + d; o [B, H, Dv].  s shares no memory with them. */
+int csn_linear_attention_step(const void* q, const void* k, const void* v, const int64_t* strides,
+                              const float* log_decay, float* s, void* o, int64_t B, int64_t H,
+                              int64_t Hk, int64_t Dk, int64_t Dv, float scale, int dtype,
+                              void* stream);
+
+/* csn_layer_norm_fwd for bfloat16 or float16 rows of any width, as they are: x [R, C] with row stride
+ * ldx (elements), y [R, C] contiguous, weight and bias [C] of the rows' type or float32
+ * (weight_dtype), mean and rstd [R] float32 (NULL: not wanted).  The backward pass reads dy (row
+ * stride ldy), x, mean and rstd and writes dx [R, C] (contiguous), dweight and dbias [C] (of
+ * weight_dtype; each of the three may be NULL); it needs the workspace for the last two.  y, dx and
+ * the workspace 16-byte aligned. */
+int csn_layer_norm_rows_fwd(const void* x, int64_t ldx, const void* weight, const void* bias, void* y,
+                            float* mean, float* rstd, int64_t R, int64_t C, float eps, int dtype,
+                            int weight_dtype, void* stream);
+size_t csn_layer_norm_rows_bwd_workspace_bytes(int64_t R, int64_t C);
+int csn_layer_norm_rows_bwd(const void* dy, int64_t ldy, const void* x, int64_t ldx, const float* mean,
+                            const float* rstd, const void* weight, void* dx, void* dweight,
+                            void* dbias, int64_t R, int64_t C, int dtype, int weight_dtype,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
 /* -------------------------------------------------------------- kernel timing */
 /* Measurement hook with no counterpart in the reference (which times with wall clock,
  * tests/profile_performance.py:41-71).  While enabled, every kernel the library
