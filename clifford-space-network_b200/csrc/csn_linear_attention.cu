@@ -234,18 +234,30 @@ int width_of(int dtype) { return dtype == CSN_F32 ? 4 : dtype == CSN_BF16 || dty
 bool aligned(const void* p, int n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// The steps of a segment: enough segments for 12 warps on each of 148 SMs, none shorter than 128 steps.
-void cut(Batch& B, int V, bool packed) {
-  const int64_t warps = up(V, 32) * B.H * (packed ? 1 : B.S), want = up(148 * 12, warps);
-  B.seg = (int)(up(std::max(up(B.T, want), (int64_t)128), 64) * 64);
+// The steps of a segment, a multiple of 128.  float32: enough segments for 12 warps on each SM.  16 bits, one CTA an SM: what
+// takes the fewest blocks of 128 steps one after another, where a CTA's start and end cost about 3 blocks and the first
+// pass, which cut sequences need, half as much again as the pass itself.
+void cut(Batch& B, int V, int passes, bool packed, bool half) {
+  const int64_t rows = up(B.T, 128), heads = (int64_t)B.H * (packed ? 1 : B.S);
+  int64_t best = 1;
+  if (half) {
+    int64_t least = INT64_MAX;
+    for (int64_t n = 1; n <= std::min(rows, (int64_t)64); ++n) {
+      const int64_t cost = up(heads * passes * n, 148) * (up(rows, n) + 3) * 2 + (n > 1 ? up(heads * std::min(passes, 2) * n, 148) * (up(rows, n) + 3) : 0);
+      if (cost < least) least = cost, best = n;
+    }
+  } else {
+    best = std::min(rows, up(148 * 12, heads * up(V, 32)));
+  }
+  B.seg = (int)(std::max(up(rows, std::max(best, (int64_t)1)), (int64_t)1) * 128);
   B.segs = packed ? 0 : (int)std::max(up(B.T, B.seg), (int64_t)1);
   B.units = packed ? B.T / B.seg + B.S : B.S * B.segs;
 }
 bool is_cut(const Batch& B, bool packed) { return packed ? B.T > B.seg : B.segs > 1; }
 
-Batch batch(int64_t S, int64_t T, int H, int Dk, int Dv, const int32_t* cu, bool packed, const float* log_decay) {
+Batch batch(int64_t S, int64_t T, int H, int Dk, int Dv, const int32_t* cu, bool packed, const float* log_decay, bool backward, int dtype) {
   Batch B = {cu, S, T, H, 0, 0, 0, log_decay};
-  cut(B, std::min(Dk, Dv), packed);
+  cut(B, std::min(Dk, Dv), backward ? 3 : 1, packed, dtype != CSN_F32);
   return B;
 }
 
@@ -280,6 +292,10 @@ void launch_blocks(const Batch& B, const Pass& P, bool first, cudaStream_t st) {
 }
 
 int run(const Batch& B, const Pass* passes, int count, bool first, int dtype, cudaStream_t st) {
+  bool tensor = dtype != CSN_F32 && B.T > 0;
+  for (int i = 0; i < count; ++i)
+    tensor = tensor && fits_tensor(B, passes[i].a, passes[i].K) && fits_tensor(B, passes[i].b, passes[i].K) && fits_tensor(B, passes[i].v, passes[i].V);
+  if (tensor) return tensor_passes(B, passes, count, first, dtype == CSN_BF16, st);
   for (int i = 0; i < count; ++i) {
     KernelTimer kt(first ? "linear_attention_first" : "linear_attention", st);
     if (dtype == CSN_F32) launch_blocks<float>(B, passes[i], first, st);
@@ -302,6 +318,7 @@ int check_sizes(const char* name, int64_t S, int64_t T, int64_t H, int64_t Hk, i
   static thread_local char text[160];
   const char* wrong = S < 0 || T < 0 || H < 0 || Hk < 0 ? "negative size" : nullptr;
   if (!wrong && (H > 0 && (Hk < 1 || H % Hk))) wrong = "the heads of k and v have to divide those of q";
+  if (!wrong && S * std::max(H, (int64_t)1) > (1 << 28)) wrong = "at most 2^28 heads in all";
   if (!wrong && (S > (1 << 30) || T > (1 << 30) || H > 65535)) wrong = "at most 2^30 sequences and steps and 65535 heads";
   int code = CSN_ERR_INVALID;
   if (!wrong && (Dk < 1 || Dv < 1 || Dk > MAX_D || Dv > MAX_D)) wrong = "head sizes of 1 to 128", code = CSN_ERR_UNSUPPORTED;
@@ -323,7 +340,7 @@ extern "C" size_t csn_linear_attention_workspace_bytes(int64_t S, int64_t T, int
                                                        int packed, int dtype, int backward) {
   if (S <= 0 || T <= 0 || H <= 0 || Hk <= 0 || check_sizes("csn_linear_attention_workspace_bytes", S, T, H, Hk, Dk, Dv, dtype) != CSN_OK)
     return 0;
-  const Batch B = batch(S, T, (int)H, (int)Dk, (int)Dv, nullptr, packed != 0, nullptr);
+  const Batch B = batch(S, T, (int)H, (int)Dk, (int)Dv, nullptr, packed != 0, nullptr, backward != 0, dtype);
   return room(B, (int)Hk, (int)Dk, (int)Dv, packed != 0, backward != 0).bytes(backward != 0);
 }
 
@@ -338,7 +355,7 @@ extern "C" int csn_linear_attention_fwd(const void* q, const void* k, const void
   if (!log_decay || !aligned(s0, 16) || !aligned(s_last, 16) ||
       (rows && (!q || !k || !v || !strides || !o || !aligned(q, size) || !aligned(k, size) || !aligned(v, size) || !aligned(o, 16))))
     return set_error(CSN_ERR_INVALID, "csn_linear_attention_fwd: missing or misaligned pointer");
-  const Batch B = batch(S, T, (int)H, (int)Dk, (int)Dv, cu_seqlens, packed, log_decay);
+  const Batch B = batch(S, T, (int)H, (int)Dk, (int)Dv, cu_seqlens, packed, log_decay, false, dtype);
   const Room R = room(B, (int)Hk, (int)Dk, (int)Dv, packed, false);
   if (R.bytes(false) && (!workspace || workspace_bytes < R.bytes(false) || !aligned(workspace, 16)))
     return set_error(CSN_ERR_INVALID, "csn_linear_attention_fwd: workspace smaller than csn_linear_attention_workspace_bytes");
@@ -373,7 +390,7 @@ extern "C" int csn_linear_attention_bwd(const void* q, const void* k, const void
       (rows && (!q || !k || !v || !d_o || !strides || (ds0 && !dv) || !aligned(q, size) || !aligned(k, size) || !aligned(v, size) ||
                 !aligned(d_o, size) || !aligned(dq, 16) || !aligned(dk, 16) || !aligned(dv, 16))))
     return set_error(CSN_ERR_INVALID, "csn_linear_attention_bwd: missing or misaligned pointer");
-  const Batch B = batch(S, T, (int)H, (int)Dk, (int)Dv, cu_seqlens, packed, log_decay);
+  const Batch B = batch(S, T, (int)H, (int)Dk, (int)Dv, cu_seqlens, packed, log_decay, true, dtype);
   const Room R = room(B, (int)Hk, (int)Dk, (int)Dv, packed, true);
   if (R.bytes(true) && (!workspace || workspace_bytes < R.bytes(true) || !aligned(workspace, 16)))
     return set_error(CSN_ERR_INVALID, "csn_linear_attention_bwd: workspace smaller than csn_linear_attention_workspace_bytes");

@@ -1,0 +1,518 @@
+// csn_linear_attention_tc.cu -- the passes of linear attention (csn_linear_attention.cuh) over 16-bit rows on the tensor cores.
+//
+// Blocks of 128 steps; with l = exp(log_decay), rows i, j of a block of n, X the state that enters (forward):
+//   P_ij = l^(i-j) (a_i . b_j) for j <= i,  out = so (diag(l^(i+1)) A X + P V),  X <- l^n X + (diag(l^(n-1-j)) B)^T V
+// and mirrored where time runs down.  A CTA runs through the blocks of one segment of one head:
+//   warp 8 loads the tiles of a, b (two stages) and v (one) by TMA;
+//   warp 9 issues the four products: A B^T and A X when the state is there, (l^.. B)^T V, P V;
+//   warps 0 to 3 turn A B^T into P and finish out, a row to a thread;
+//   warps 4 to 7 fade B and keep the state, a place of v to a thread, its entries along b in registers.
+// Shared memory has no room for a copy of each operand, so they follow one another in place: the state as an operand, then
+// P, then the next state; B, then the first part of the faded B; A, then its second part, then rows of out on their way.
+//
+// Roundings.  P and the state as an operand of A X are rounded to the tensors' type: out itself is, and these two add as
+// much again.  The state is not: it stays float32 in registers, and the faded B that enters it is split into parts that
+// hold 22 bits or more: three of bfloat16, two of float16.  float16 ends at 65504 and loses bits below 2^-14, so rows of P,
+// places of v of the state, and the faded B of a block are first scaled by a power of two that brings the
+// largest entry into [2^14, 2^15), and what comes of them is scaled back in float32.
+#include <algorithm>
+#include <cstdint>
+
+#include "csn_linear_attention.cuh"
+#include "csn_tc.cuh"
+
+namespace csn {
+namespace {
+
+using namespace tc;
+using namespace la;
+
+constexpr int STEPS = 128;      // of a block
+constexpr int BOX = 128 * 128;  // bytes of 128 rows x 64 places
+constexpr int THREADS = 10 * 32;
+constexpr int MAX_PASSES = 3;
+
+__host__ __device__ constexpr int tile_a(int nk) { return nk * BOX; }
+constexpr int smem_bytes(int nk, int nv, bool bf16) { return 4 * tile_a(nk) + nv * BOX + 2 * BOX + (bf16 ? tile_a(nk) : 0) + 1024; }
+
+struct Job {
+  CUtensorMap a, b, v;
+  Pass pass;
+};
+struct Jobs {
+  Job job[MAX_PASSES];
+};
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  return BF16 ? pack<__nv_bfloat16>(a, b) : pack<__half>(a, b);
+}
+template <bool BF16>
+__device__ __forceinline__ float2 unpack2(uint32_t v) {
+  if (BF16) return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+  return __half22float2(*reinterpret_cast<__half2*>(&v));
+}
+
+// the larger of `top` and |a|, unless that is not finite
+__device__ __forceinline__ float finite_max(float top, float a) {
+  a = fabsf(a);
+  return fmaxf(top, a < __int_as_float(0x7f800000) ? a : 0.0f);
+}
+// the power of two that brings `top` into [2^14, 2^15), as far as float32 has it and its inverse, and that inverse
+__device__ __forceinline__ float scale_up(float top, float& down) {
+  const uint32_t e = top == 0.0f ? 141u : max(__float_as_uint(top) >> 23, 15u);
+  down = __uint_as_float((e - 14) << 23);
+  return __uint_as_float((268 - e) << 23);
+}
+
+// 16 bytes: chunk c (8 places) of row r of a tile of boxes of `rows` rows
+__device__ __forceinline__ char* chunk_at(char* tile, int rows, int r, int c) {
+  return tile + (c / 8) * rows * 128 + r * 128 + ((c % 8) ^ (r & 7)) * 16;
+}
+__device__ __forceinline__ void arrive_warp(uint64_t* b) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(b);
+}
+
+template <bool BF16, int NK, int NV, bool OUT>
+__global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_constant__ Jobs jobs, const Batch B, int count) {
+  constexpr int TA = tile_a(NK), PARTS = BF16 ? 3 : 2;
+  extern __shared__ char raw[];
+  __shared__ uint64_t full_ab[2], full_v, ab_free[2], scores, keys, updated, probs, summed, state, out_read, drained;
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile uint32_t gave_up;
+  __shared__ float power[STEPS + 1], place_scale[2][128], tops[4];
+  char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  char* const tv = smem + 4 * TA;       // stage s: a at smem + 2 s TA, b behind it
+  char* const sp = tv + NV * BOX;       // the state as an operand, or P
+  char* const third = sp + 2 * BOX;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+
+  const Job& J = jobs.job[blockIdx.x % count];
+  const Pass& P = J.pass;
+  const int h = (int)(blockIdx.x / count % B.H);
+  const Unit U(B, blockIdx.x / count / B.H);
+  const bool back = P.back;
+  if (U.s < 0 || (!OUT && U.ends(back))) return;
+  const int steps = U.to - U.from, blocks = (steps + STEPS - 1) / STEPS;
+
+  if (threadIdx.x == 0) {
+    mbar_init(&full_ab[0], 1), mbar_init(&full_ab[1], 1), mbar_init(&full_v, 1), mbar_init(&ab_free[0], 4), mbar_init(&ab_free[1], 4);
+    mbar_init(&scores, 1), mbar_init(&keys, 4), mbar_init(&updated, 1), mbar_init(&probs, 4), mbar_init(&summed, 1);
+    mbar_init(&state, 4), mbar_init(&out_read, 4), mbar_init(&drained, 1);
+    mbar_init_fence();
+    gave_up = 0;
+  }
+  if (threadIdx.x <= STEPS) power[threadIdx.x] = fade(B.log_decay[h], threadIdx.x);
+  if (warp == 9) tmem_alloc<512>(&tmem_slot);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t t_scores = tmem_slot, t_inter = t_scores + 128, t_intra = t_inter + 64 * NV, t_update = t_intra + 64 * NV;
+  // steps of block n: first .. first + have - 1 of the sequence
+  auto block = [&](int n, int& have) {
+    const int b = back ? blocks - 1 - n : n;
+    have = min(STEPS, steps - b * STEPS);
+    return U.from + b * STEPS;
+  };
+
+  if (warp == 8) {  // ------------------------------------------------------------ loads
+    const int y_a = h / P.a.shared, y_b = h / P.b.shared, y_v = h / P.v.shared, w = B.cu ? 0 : (int)U.s;
+    const int row0 = B.cu ? (int)U.row0 : 0;
+    int ab = 0, vv = 0;  // blocks loaded
+    auto load_ab = [&](int n) {
+      int have;
+      const int row = row0 + block(n, have);
+      char* a = smem + (n & 1) * 2 * TA;
+      if (elect_one()) {
+        mbar_expect(&full_ab[n & 1], (OUT ? 2 : 1) * TA);
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+          if (OUT) tma_load(a + i * BOX, &J.a, i * 64, y_a, row, w, &full_ab[n & 1]);
+          tma_load(a + TA + i * BOX, &J.b, i * 64, y_b, row, w, &full_ab[n & 1]);
+        }
+      }
+      __syncwarp();
+      ++ab;
+    };
+    auto load_v = [&](int n) {
+      int have;
+      const int row = row0 + block(n, have);
+      if (elect_one()) {
+        mbar_expect(&full_v, NV * BOX);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) tma_load(tv + i * BOX, &J.v, i * 64, y_v, row, w, &full_v);
+      }
+      __syncwarp();
+      ++vv;
+    };
+    if (blocks > 0) load_ab(0), load_v(0);
+    if (blocks > 1) load_ab(1);
+    bool ok = true;
+    for (int n = 0; n + 1 < blocks && ok; ++n) {
+      if (!(ok = __all_sync(0xffffffffu, mbar_wait(OUT ? &summed : &updated, n & 1, &gave_up)))) break;
+      load_v(n + 1);
+      if (n + 2 >= blocks) continue;
+      if (OUT && !(ok = __all_sync(0xffffffffu, mbar_wait(&ab_free[n & 1], (n >> 1) & 1, &gave_up)))) break;
+      load_ab(n + 2);
+    }
+    // copies in flight end before the shared memory does: where a wait gave up, and otherwise these have long been awaited
+    for (int n = max(ab - 2, 0); n < ab; ++n)
+      for (uint32_t i = 0; i < POLLS && !mbar_try(&full_ab[n & 1], (n >> 1) & 1); ++i) {}
+    for (uint32_t i = 0; vv > 0 && i < POLLS && !mbar_try(&full_v, (vv - 1) & 1); ++i) {}
+  } else if (warp == 9) {  // -------------------------------------------------- products
+    constexpr uint32_t I_SCORES = instruction(BF16, false, false, 128, 128), I_INTER = instruction(BF16, false, false, 128, 64 * NV);
+    constexpr uint32_t I_INTRA = instruction(BF16, false, true, 128, 64 * NV), I_UPDATE = instruction(BF16, true, true, 128, 64 * NK);
+    const uint64_t d_v = operand(smem_addr(tv), BOX), d_sp = operand(smem_addr(sp), BOX), d_third = operand(smem_addr(third), BOX);
+    bool ok = true;
+    auto wait = [&](uint64_t* b, int n) {
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(b, n & 1, &gave_up));
+      return ok;
+    };
+    for (int n = 0; n < blocks && ok; ++n) {
+      const uint64_t d_a = operand(smem_addr(smem + (n & 1) * 2 * TA), BOX), d_b = d_a + (TA >> 4);
+      if (!wait(&full_ab[n & 1], n >> 1)) break;
+      if (OUT) {
+        if (!wait(&state, n) || (n > 0 && !wait(&out_read, n - 1))) break;
+        fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < 4 * NK; ++k) {
+            const uint32_t at = (k / 4) * (BOX >> 4) + (k % 4) * 2;
+            mma(t_scores, d_a + at, d_b + at, I_SCORES, k > 0);
+          }
+#pragma unroll
+          for (int k = 0; k < 4 * NK; ++k)
+            mma(t_inter, d_a + (k / 4) * (BOX >> 4) + (k % 4) * 2, d_sp + (k / 4) * (NV * BOX / 2 >> 4) + (k % 4) * 2, I_INTER, k > 0);
+          mma_commit(&scores);
+        }
+        __syncwarp();
+      }
+      if (!wait(&full_v, n) || !wait(&keys, n)) break;
+      fence_after();
+      if (elect_one()) {
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+          const uint64_t d = p == 0 ? d_b : p == 1 ? d_a : d_third;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) mma(t_update, d_v + k * (2048 >> 4), d + k * (2048 >> 4), I_UPDATE, p > 0 || k > 0);
+        }
+        mma_commit(&updated);
+      }
+      __syncwarp();
+      if (!OUT) continue;
+      if (!wait(&probs, n)) break;
+      fence_after();
+      if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          mma(t_intra, d_sp + (k / 4) * (BOX >> 4) + (k % 4) * 2, d_v + k * (2048 >> 4), I_INTRA, k > 0);
+        mma_commit(&summed);
+      }
+      __syncwarp();
+    }
+    if (!ok) {
+      if (elect_one()) mma_commit(&drained);
+      __syncwarp();
+      for (uint32_t i = 0; i < POLLS && !mbar_try(&drained, 0); ++i) {}
+    }
+  } else if (warp < 4) {  // ------------------------------------------------- P, and out
+    if (OUT) {
+      const int i = threadIdx.x;  // row of the block
+      const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+      const float both = P.so * P.sb, nan = __int_as_float(0x7fffffff);
+      for (int n = 0; n < blocks; ++n) {
+        int have;
+        const int first = block(n, have);
+        bool ok = mbar_wait(&scores, n & 1, &gave_up);
+        __syncwarp();
+        fence_after();
+        float down = 1.0f, up = both;
+        auto entry = [&](float v, int j, bool diagonal) {
+          const int d = back ? j - i : i - j;
+          if (back) return (diagonal && d < 0) || j >= have ? 0.0f : v * power[max(d, 0)];
+          return diagonal && d < 0 ? 0.0f : v * power[max(d, 0)];
+        };
+        if (!BF16) {
+          float top = 0.0f;
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            if (back ? c < warp : c > warp) continue;
+#pragma unroll
+            for (int q = 0; q < 32; q += 16) {
+              float v[16];
+              tmem_load16(t_scores + lanes + c * 32 + q, v);
+              tmem_load_wait();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) top = finite_max(top, entry(v[e], c * 32 + q + e, c == warp) * both);
+            }
+          }
+          up = scale_up(top, down) * both;
+        }
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          const bool none = back ? c < warp : c > warp;
+#pragma unroll
+          for (int q = 0; q < 32; q += 16) {
+            uint32_t w[8] = {};
+            if (!none) {
+              float v[16];
+              tmem_load16(t_scores + lanes + c * 32 + q, v);
+              tmem_load_wait();
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                w[e] = pack2<BF16>(entry(v[2 * e], c * 32 + q + 2 * e, c == warp) * up, entry(v[2 * e + 1], c * 32 + q + 2 * e + 1, c == warp) * up);
+            }
+            *reinterpret_cast<uint4*>(chunk_at(sp, 128, i, c * 4 + q / 8)) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(chunk_at(sp, 128, i, c * 4 + q / 8 + 1)) = make_uint4(w[4], w[5], w[6], w[7]);
+          }
+        }
+        fence_async();
+        fence_before();
+        arrive_warp(&probs);
+
+        ok = mbar_wait(&summed, n & 1, &gave_up) && ok;
+        __syncwarp();
+        fence_after();
+        const float inter = P.so * power[i < have ? (back ? have - 1 - i : i + 1) : 0];
+        char* const stage = smem + (n & 1) * 2 * TA + warp * 32 * 128;  // 32 rows x 128 bytes
+        const int rows = min(32, have - warp * 32);
+        const int size = P.wide ? 4 : 2, per = P.wide ? 32 : 64;  // places of a round
+        char* const out = static_cast<char*>(P.out) + ((U.row0 + first + warp * 32) * B.H + h) * (int64_t)P.V * size;
+        const int64_t pitch = (int64_t)B.H * P.V * size;
+        for (int c0 = 0; c0 < 64 * NV; c0 += per) {
+          for (int c = c0; c < c0 + per; c += 16) {
+            float a[16], v[16];
+            tmem_load16(t_inter + lanes + c, a);
+            tmem_load16(t_intra + lanes + c, v);
+            tmem_load_wait();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float x = BF16 ? a[e] : a[e] * place_scale[n & 1][c + e];
+              v[e] = ok ? fmaf(inter, x, v[e] * down) : nan;
+            }
+            if (P.wide) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                *reinterpret_cast<float4*>(stage + lane * 128 + (((c - c0) / 4 + e) ^ (lane & 7)) * 16) =
+                    make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                *reinterpret_cast<uint4*>(stage + lane * 128 + (((c - c0) / 8 + e) ^ (lane & 7)) * 16) =
+                    make_uint4(pack2<BF16>(v[8 * e], v[8 * e + 1]), pack2<BF16>(v[8 * e + 2], v[8 * e + 3]),
+                               pack2<BF16>(v[8 * e + 4], v[8 * e + 5]), pack2<BF16>(v[8 * e + 6], v[8 * e + 7]));
+            }
+          }
+          if (c0 + per >= 64 * NV) {
+            fence_before();
+            arrive_warp(&out_read);
+          }
+          __syncwarp();
+          const int at = c0 * size + lane % 8 * 16;
+          if (at < P.V * size) {
+            for (int r = lane / 8; r < rows; r += 4)
+              *reinterpret_cast<uint4*>(out + r * pitch + at) = *reinterpret_cast<const uint4*>(stage + r * 128 + ((lane % 8) ^ (r & 7)) * 16);
+          }
+          __syncwarp();
+        }
+        fence_async();
+        arrive_warp(&ab_free[n & 1]);
+      }
+    }
+  } else {  // ------------------------------------------------ the faded B, and the state
+    const int r = threadIdx.x - 128;  // row of the block; place of v
+    const uint32_t lanes = (uint32_t)((warp - 4) * 32) << 16;
+    const bool mine = r < P.V && r < 64 * NV;
+    const int64_t size = (int64_t)P.K * P.V;
+    float x[64 * NK];
+#pragma unroll
+    for (int k = 0; k < 64 * NK; ++k) x[k] = 0.0f;
+    if (OUT && P.state && mine) {
+      const float* p = P.state + ((P.by_unit ? U.unit : U.s) * B.H + h) * size + r * P.sc;
+#pragma unroll
+      for (int k = 0; k < 64 * NK; ++k)
+        if (k < P.K) x[k] = p[k * P.sr];
+    }
+    bool ok = true;
+    auto put_state = [&](int n) {  // as an operand of block n: row = place of v
+      float up = 1.0f;
+      if (!BF16) {
+        float top = 0.0f, down;
+#pragma unroll
+        for (int k = 0; k < 64 * NK; ++k) top = finite_max(top, x[k]);
+        up = scale_up(top, down);
+        place_scale[n & 1][r] = down;
+      }
+      if (r < 64 * NV) {
+#pragma unroll
+        for (int c = 0; c < 8 * NK; ++c) {
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = pack2<BF16>(x[c * 8 + 2 * e] * up, x[c * 8 + 2 * e + 1] * up);
+          *reinterpret_cast<uint4*>(chunk_at(sp, 64 * NV, r, c)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+      fence_async();
+      fence_before();
+      arrive_warp(&state);
+    };
+    if (OUT && blocks > 0) put_state(0);
+    for (int n = 0; n < blocks; ++n) {
+      int have;
+      block(n, have);
+      char* const ta = smem + (n & 1) * 2 * TA;
+      char* const tb = ta + TA;
+      ok = mbar_wait(&full_ab[n & 1], (n >> 1) & 1, &gave_up) && ok;
+      const float f = r < have ? power[back ? r + 1 : have - 1 - r] * P.sb : 0.0f;
+      float up = 1.0f, down = 1.0f;
+      if (!BF16) {
+        float top = 0.0f;
+        if (r < have) {
+#pragma unroll
+          for (int c = 0; c < 8 * NK; ++c) {
+            const uint4 q = *reinterpret_cast<const uint4*>(chunk_at(tb, 128, r, c));
+            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 v = unpack2<BF16>(w[e]);
+              top = finite_max(finite_max(top, v.x * f), v.y * f);
+            }
+          }
+        }
+        const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+        if (lane == 0) tops[warp - 4] = __uint_as_float(bits);
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        up = scale_up(top, down);
+      }
+      if (OUT) ok = mbar_wait(&scores, n & 1, &gave_up) && ok;  // A and B have been read
+      __syncwarp();
+#pragma unroll
+      for (int c = 0; c < 8 * NK; ++c) {
+        char* const at = chunk_at(tb, 128, r, c);
+        const uint4 q = *reinterpret_cast<const uint4*>(at);
+        const uint32_t in[4] = {q.x, q.y, q.z, q.w};
+        uint32_t w0[4], w1[4], w2[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float2 v = unpack2<BF16>(in[e]);
+          v.x = r < have ? v.x * f * up : 0.0f, v.y = r < have ? v.y * f * up : 0.0f;
+          w0[e] = pack2<BF16>(v.x, v.y);
+          const float2 v0 = unpack2<BF16>(w0[e]);
+          v.x -= v0.x, v.y -= v0.y;
+          w1[e] = pack2<BF16>(v.x, v.y);
+          if (BF16) {
+            const float2 v1 = unpack2<BF16>(w1[e]);
+            w2[e] = pack2<BF16>(v.x - v1.x, v.y - v1.y);
+          }
+        }
+        *reinterpret_cast<uint4*>(at) = make_uint4(w0[0], w0[1], w0[2], w0[3]);
+        *reinterpret_cast<uint4*>(chunk_at(ta, 128, r, c)) = make_uint4(w1[0], w1[1], w1[2], w1[3]);
+        if (BF16) *reinterpret_cast<uint4*>(chunk_at(third, 128, r, c)) = make_uint4(w2[0], w2[1], w2[2], w2[3]);
+      }
+      if (B.cu && have < STEPS) {  // rows of the next sequence, whatever they hold
+        ok = mbar_wait(&full_v, n & 1, &gave_up) && ok;
+        if (r >= have) {
+#pragma unroll
+          for (int c = 0; c < 8 * NV; ++c) *reinterpret_cast<uint4*>(chunk_at(tv, 128, r, c)) = make_uint4(0, 0, 0, 0);
+        }
+      }
+      fence_async();
+      fence_before();
+      arrive_warp(&keys);
+
+      const float whole = power[have];
+      ok = mbar_wait(&updated, n & 1, &gave_up) && ok;
+      __syncwarp();
+      fence_after();
+#pragma unroll
+      for (int c = 0; c < 64 * NK; c += 16) {
+        float u[16];
+        tmem_load16(t_update + lanes + c, u);
+        tmem_load_wait();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[c + e] = fmaf(whole, x[c + e], BF16 ? u[e] : u[e] * down);
+      }
+      fence_before();
+      if (OUT && n + 1 < blocks) {
+        ok = mbar_wait(&summed, n & 1, &gave_up) && ok;  // P has been read
+        __syncwarp();
+        put_state(n + 1);
+      }
+    }
+    float* to = OUT ? (P.last && U.ends(back) ? P.last + (U.s * B.H + h) * size : nullptr) : P.made + (U.unit * B.H + h) * size;
+    if (to && mine) {
+#pragma unroll
+      for (int k = 0; k < 64 * NK; ++k)
+        if (k < P.K) to[k * P.sr + r * P.sc] = ok ? x[k] : __int_as_float(0x7fffffff);
+    }
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (warp == 9) tmem_free<512>(tmem_slot);
+}
+
+template <bool BF16, int NK, int NV, bool OUT>
+cudaError_t launch(const Jobs& jobs, const Batch& B, int count, cudaStream_t st) {
+  constexpr int smem = smem_bytes(NK, NV, BF16);
+  if (cudaError_t e = allow_smem<blocks_tc_kernel<BF16, NK, NV, OUT>>(smem)) return e;
+  blocks_tc_kernel<BF16, NK, NV, OUT><<<(unsigned)(B.units * B.H * count), THREADS, smem, st>>>(jobs, B, count);
+  return cudaSuccess;
+}
+template <bool BF16, int NK, int NV>
+cudaError_t launch(const Jobs& jobs, const Batch& B, int count, bool first, cudaStream_t st) {
+  return first ? launch<BF16, NK, NV, false>(jobs, B, count, st) : launch<BF16, NK, NV, true>(jobs, B, count, st);
+}
+template <bool BF16>
+cudaError_t launch(const Jobs& jobs, const Batch& B, int nk, int nv, int count, bool first, cudaStream_t st) {
+  if (nk == 1 && nv == 1) return launch<BF16, 1, 1>(jobs, B, count, first, st);
+  if (nk == 1) return launch<BF16, 1, 2>(jobs, B, count, first, st);
+  if (nv == 1) return launch<BF16, 2, 1>(jobs, B, count, first, st);
+  return launch<BF16, 2, 2>(jobs, B, count, first, st);
+}
+
+bool map_stream(CUtensorMap* map, const Batch& B, const Stream& x, int D, bool bf16) {
+  const int64_t sizes[4] = {D, B.H / x.shared, B.T, B.cu ? 1 : B.S}, strides[3] = {x.head, x.row, x.seq};
+  return make_map4(map, x.p, sizes, strides, STEPS, bf16);
+}
+
+}  // namespace
+
+namespace la {
+
+bool fits_tensor(const Batch& B, const Stream& x, int D) {
+  auto step = [](int64_t n, int64_t stride) { return n <= 1 || (stride > 0 && stride % 8 == 0 && stride < (1ll << 38)); };
+  return D % 8 == 0 && reinterpret_cast<uintptr_t>(x.p) % 16 == 0 && step(B.H / x.shared, x.head) && step(B.T, x.row) &&
+         (B.cu || step(B.S, x.seq));
+}
+
+int tensor_passes(const Batch& B, const Pass* passes, int count, bool first, bool bf16, cudaStream_t st) {
+  // passes whose tiles have one shape run side by side in one launch
+  bool done[MAX_PASSES] = {};
+  for (int i = 0; i < count; ++i) {
+    if (done[i]) continue;
+    const int nk = passes[i].K > 64 ? 2 : 1, nv = passes[i].V > 64 ? 2 : 1;
+    Jobs jobs;
+    int n = 0;
+    for (int j = i; j < count; ++j) {
+      const Pass& p = passes[j];
+      if (done[j] || (p.K > 64 ? 2 : 1) != nk || (p.V > 64 ? 2 : 1) != nv) continue;
+      done[j] = true;
+      Job& job = jobs.job[n++];
+      job.pass = p;
+      if (!map_stream(&job.a, B, p.a, p.K, bf16) || !map_stream(&job.b, B, p.b, p.K, bf16) || !map_stream(&job.v, B, p.v, p.V, bf16))
+        return set_error(CSN_ERR_CUDA, "csn_linear_attention: tensor map");
+    }
+    for (int j = n; j < MAX_PASSES; ++j) jobs.job[j] = jobs.job[0];
+    KernelTimer kt(first ? "linear_attention_first" : "linear_attention", st);
+    const cudaError_t e = bf16 ? launch<true>(jobs, B, nk, nv, n, first, st) : launch<false>(jobs, B, nk, nv, n, first, st);
+    if (e != cudaSuccess) return set_cuda_error(e, "csn_linear_attention: shared memory");
+  }
+  return CSN_OK;
+}
+
+}  // namespace la
+}  // namespace csn

@@ -26,6 +26,19 @@ Encode encoder() {
 }
 }  // namespace
 
+bool make_map4(CUtensorMap* map, const void* p, const int64_t* sizes, const int64_t* strides, int box, bool bf16) {
+  Encode e = encoder();
+  int dev = 0;
+  if (!e || cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return false;
+  cuuint64_t dims[4], steps[3];
+  for (int i = 0; i < 4; ++i) dims[i] = (cuuint64_t)sizes[i];
+  for (int i = 0; i < 3; ++i) steps[i] = sizes[i + 1] > 1 ? (cuuint64_t)strides[i] * 2 : 16;
+  const cuuint32_t boxes[4] = {64, 1, (cuuint32_t)box, 1}, step[4] = {1, 1, 1, 1};
+  return e(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(p), dims, steps,
+           boxes, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 bool make_map(CUtensorMap* map, const void* p, int64_t rows, int64_t cols, int64_t ld, int box_rows, bool bf16) {
   Encode e = encoder();
   int dev = 0;

@@ -30,6 +30,9 @@ __device__ __forceinline__ void mbar_init(uint64_t* b, uint32_t count) {
 __device__ __forceinline__ void mbar_init_fence() {
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 }
+__device__ __forceinline__ void mbar_arrive(uint64_t* b) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(b)) : "memory");
+}
 __device__ __forceinline__ void mbar_expect(uint64_t* b, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(b)), "r"(bytes) : "memory");
 }
@@ -84,6 +87,17 @@ __device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int 
       "l"(map), "r"(x), "r"(y), "r"(smem_addr(b))
       : "memory");
 }
+
+// the box of a map of four axes
+__device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* b) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+          smem_addr(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_addr(b))
+      : "memory");
+}
+// what this thread has written to shared memory is seen by copies and products that follow
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // the same into this CTA's shared memory, counted on a barrier of either CTA of a pair
 __device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, int x, int y, uint32_t barrier) {
@@ -181,6 +195,9 @@ __device__ __forceinline__ void mma_commit_pair(uint64_t* b) {
 // Tensor map of a row-major 16-bit matrix [rows, cols] with `ld` elements a row (ld % 8 == 0, p 16-byte aligned),
 // read in boxes of 64 columns x box_rows rows with 128-byte swizzle; what lies outside reads as 0.
 bool make_map(CUtensorMap* map, const void* p, int64_t rows, int64_t cols, int64_t ld, int box_rows, bool bf16);
+// Tensor map of 16-bit elements over four axes (strides of the last three in elements, a multiple of 8 and not 0 where the
+// axis has more than one place), read in boxes of 64 x 1 x box x 1.
+bool make_map4(CUtensorMap* map, const void* p, const int64_t* sizes, const int64_t* strides, int box, bool bf16);
 int sm_count();
 
 }  // namespace tc
