@@ -3,10 +3,11 @@
 // Blocks of 128 steps; with l = exp(log_decay), rows i, j of a block of n, X the state that enters (forward):
 //   P_ij = l^(i-j) (a_i . b_j) for j <= i,  out = so (diag(l^(i+1)) A X + P V),  X <- l^n X + (diag(l^(n-1-j)) B)^T V
 // and mirrored where time runs down.  A CTA runs through the blocks of one segment of one head:
-//   warp 8 loads the tiles of a, b (two stages) and v (one) by TMA;
-//   warp 9 issues the four products: A B^T and A X when the state is there, (l^.. B)^T V, P V;
-//   warps 0 to 3 turn A B^T into P and finish out, a row to a thread;
-//   warps 4 to 7 fade B and keep the state, a place of v to a thread, its entries along b in registers.
+//   warp 16 loads the tiles of a, b (two stages) and v (one) by TMA;
+//   warp 17 issues the four products: A B^T and A X when the state is there, (l^.. B)^T V, P V.
+//   warps 0 to 7 turn A B^T into P and finish out, half a row to a thread;
+//   warps 8 to 15 fade B, half a row to a thread, and keep the state in registers: half of the entries along b at one
+//   place of v;
 // Shared memory has no room for a copy of each operand, so they follow one another in place: the state as an operand, then
 // P, then the next state; B, then the first part of the faded B; A, then its second part, then rows of out on their way.
 //
@@ -29,7 +30,7 @@ using namespace la;
 
 constexpr int STEPS = 128;      // of a block
 constexpr int BOX = 128 * 128;  // bytes of 128 rows x 64 places
-constexpr int THREADS = 10 * 32;
+constexpr int LOADS = 16, PRODUCTS = 17, THREADS = 18 * 32;
 constexpr int MAX_PASSES = 3;
 
 __host__ __device__ constexpr int tile_a(int nk) { return nk * BOX; }
@@ -52,6 +53,24 @@ __device__ __forceinline__ float2 unpack2(uint32_t v) {
   if (BF16) return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
   return __half22float2(*reinterpret_cast<__half2*>(&v));
 }
+
+// two float32 products, or sums, in one instruction
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 w, x, y, z;\n\tmov.b64 w, {%2, %3};\n\tmov.b64 x, {%4, %5};\n\tmov.b64 y, {%6, %7};\n\tfma.rn.f32x2 z, w, x, y;\n\t"
+      "mov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 twice(float a) { return make_float2(a, a); }
 
 // the larger of `top` and |a|, unless that is not finite
 __device__ __forceinline__ float finite_max(float top, float a) {
@@ -81,7 +100,9 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
   __shared__ uint64_t full_ab[2], full_v, ab_free[2], scores, keys, updated, probs, summed, state, out_read, drained;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile uint32_t gave_up;
-  __shared__ float power[STEPS + 1], place_scale[2][128], tops[4];
+  __shared__ float power[STEPS + 1], place_scale[2][128];
+  __shared__ float tops[2][128], place_top[2][128], warp_top[8];
+  __shared__ __align__(16) float near[32], fan[64];  // powers of the distances to a side of 32 steps, and to its diagonal
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   char* const tv = smem + 4 * TA;       // stage s: a at smem + 2 s TA, b behind it
   char* const sp = tv + NV * BOX;       // the state as an operand, or P
@@ -97,14 +118,16 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
   const int steps = U.to - U.from, blocks = (steps + STEPS - 1) / STEPS;
 
   if (threadIdx.x == 0) {
-    mbar_init(&full_ab[0], 1), mbar_init(&full_ab[1], 1), mbar_init(&full_v, 1), mbar_init(&ab_free[0], 4), mbar_init(&ab_free[1], 4);
-    mbar_init(&scores, 1), mbar_init(&keys, 4), mbar_init(&updated, 1), mbar_init(&probs, 4), mbar_init(&summed, 1);
-    mbar_init(&state, 4), mbar_init(&out_read, 4), mbar_init(&drained, 1);
+    mbar_init(&full_ab[0], 1), mbar_init(&full_ab[1], 1), mbar_init(&full_v, 1), mbar_init(&ab_free[0], 8), mbar_init(&ab_free[1], 8);
+    mbar_init(&scores, 1), mbar_init(&keys, 8), mbar_init(&updated, 1), mbar_init(&probs, 8), mbar_init(&summed, 1);
+    mbar_init(&state, 8), mbar_init(&out_read, 8), mbar_init(&drained, 1);
     mbar_init_fence();
     gave_up = 0;
   }
   if (threadIdx.x <= STEPS) power[threadIdx.x] = fade(B.log_decay[h], threadIdx.x);
-  if (warp == 9) tmem_alloc<512>(&tmem_slot);
+  else if (threadIdx.x - 256 < 32u) near[threadIdx.x - 256] = fade(B.log_decay[h], back ? threadIdx.x - 256 : 287 - threadIdx.x);
+  else if (threadIdx.x - 320 < 63u) fan[threadIdx.x - 320] = fade(B.log_decay[h], abs((int)threadIdx.x - 351));
+  if (warp == PRODUCTS) tmem_alloc<512>(&tmem_slot);
   fence_before();
   __syncthreads();
   fence_after();
@@ -116,7 +139,7 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
     return U.from + b * STEPS;
   };
 
-  if (warp == 8) {  // ------------------------------------------------------------ loads
+  if (warp == LOADS) {  // ------------------------------------------------------------ loads
     const int y_a = h / P.a.shared, y_b = h / P.b.shared, y_v = h / P.v.shared, w = B.cu ? 0 : (int)U.s;
     const int row0 = B.cu ? (int)U.row0 : 0;
     int ab = 0, vv = 0;  // blocks loaded
@@ -160,7 +183,7 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
     for (int n = max(ab - 2, 0); n < ab; ++n)
       for (uint32_t i = 0; i < POLLS && !mbar_try(&full_ab[n & 1], (n >> 1) & 1); ++i) {}
     for (uint32_t i = 0; vv > 0 && i < POLLS && !mbar_try(&full_v, (vv - 1) & 1); ++i) {}
-  } else if (warp == 9) {  // -------------------------------------------------- products
+  } else if (warp == PRODUCTS) {  // -------------------------------------------------- products
     constexpr uint32_t I_SCORES = instruction(BF16, false, false, 128, 128), I_INTER = instruction(BF16, false, false, 128, 64 * NV);
     constexpr uint32_t I_INTRA = instruction(BF16, false, true, 128, 64 * NV), I_UPDATE = instruction(BF16, true, true, 128, 64 * NK);
     const uint64_t d_v = operand(smem_addr(tv), BOX), d_sp = operand(smem_addr(sp), BOX), d_third = operand(smem_addr(third), BOX);
@@ -169,24 +192,35 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
       ok = ok && __all_sync(0xffffffffu, mbar_wait(b, n & 1, &gave_up));
       return ok;
     };
+    // A B^T of block n: as soon as its tiles are there and P of the block before has been read
+    auto issue_scores = [&](int n) {
+      if (!wait(&full_ab[n & 1], n >> 1)) return;
+      fence_after();
+      const uint64_t d_a = operand(smem_addr(smem + (n & 1) * 2 * TA), BOX);
+      if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < 4 * NK; ++k) {
+          const uint64_t at = d_a + (k / 4) * (BOX >> 4) + (k % 4) * 2;
+          mma(t_scores, at, at + (TA >> 4), I_SCORES, k > 0);
+        }
+      }
+      __syncwarp();
+    };
+    if (OUT && blocks > 0) issue_scores(0);
     for (int n = 0; n < blocks && ok; ++n) {
       const uint64_t d_a = operand(smem_addr(smem + (n & 1) * 2 * TA), BOX), d_b = d_a + (TA >> 4);
-      if (!wait(&full_ab[n & 1], n >> 1)) break;
       if (OUT) {
         if (!wait(&state, n) || (n > 0 && !wait(&out_read, n - 1))) break;
         fence_after();
         if (elect_one()) {
-#pragma unroll
-          for (int k = 0; k < 4 * NK; ++k) {
-            const uint32_t at = (k / 4) * (BOX >> 4) + (k % 4) * 2;
-            mma(t_scores, d_a + at, d_b + at, I_SCORES, k > 0);
-          }
 #pragma unroll
           for (int k = 0; k < 4 * NK; ++k)
             mma(t_inter, d_a + (k / 4) * (BOX >> 4) + (k % 4) * 2, d_sp + (k / 4) * (NV * BOX / 2 >> 4) + (k % 4) * 2, I_INTER, k > 0);
           mma_commit(&scores);
         }
         __syncwarp();
+      } else if (!wait(&full_ab[n & 1], n >> 1)) {
+        break;
       }
       if (!wait(&full_v, n) || !wait(&keys, n)) break;
       fence_after();
@@ -210,17 +244,46 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
         mma_commit(&summed);
       }
       __syncwarp();
+      if (n + 1 < blocks) issue_scores(n + 1);
     }
     if (!ok) {
       if (elect_one()) mma_commit(&drained);
       __syncwarp();
       for (uint32_t i = 0; i < POLLS && !mbar_try(&drained, 0); ++i) {}
     }
-  } else if (warp < 4) {  // ------------------------------------------------- P, and out
+  } else if (warp < 8) {  // ------------------------------------------------- P, and out
     if (OUT) {
-      const int i = threadIdx.x;  // row of the block
-      const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-      const float both = P.so * P.sb, nan = __int_as_float(0x7fffffff);
+      const int quarter = warp % 4, side = warp / 4, i = quarter * 32 + lane;  // row of the block
+      const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+      const float both = P.so * P.sb;
+      // 32 products of this thread's row, c of four, faded and times `up`; `have`: places of the block
+      auto products = [&](int c, int have, float up, float2 (&v)[16]) {
+        tmem_load16(t_scores + lanes + c * 32, reinterpret_cast<float*>(v));
+        tmem_load16(t_scores + lanes + c * 32 + 16, reinterpret_cast<float*>(v + 8));
+        const int apart = 32 * (back ? c - quarter : quarter - c);
+        if (apart == 0) {
+          const float* p = fan + 31 + lane;
+          const uint32_t in = back ? (c * 32 + 32 > have ? have > c * 32 ? (1u << (have - c * 32)) - 1 : 0u : ~0u) & ~0u << lane : (2u << lane) - 1;
+          tmem_load_wait();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float2 w = mul2(v[e], mul2(make_float2(p[-2 * e], p[-2 * e - 1]), twice(up)));
+            v[e] = make_float2(in & 1u << 2 * e ? w.x : 0.0f, in & 2u << 2 * e ? w.y : 0.0f);
+          }
+        } else {
+          const float2 edge = twice(power[apart - (back ? lane : 31 - lane)] * up);
+          tmem_load_wait();
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) {
+            const float4 f = *reinterpret_cast<const float4*>(&near[2 * e]);
+            v[e] = mul2(v[e], mul2(edge, make_float2(f.x, f.y))), v[e + 1] = mul2(v[e + 1], mul2(edge, make_float2(f.z, f.w)));
+          }
+          if (back && c * 32 + 32 > have) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = make_float2(c * 32 + 2 * e < have ? v[e].x : 0.0f, c * 32 + 2 * e + 1 < have ? v[e].y : 0.0f);
+          }
+        }
+      };
       for (int n = 0; n < blocks; ++n) {
         int have;
         const int first = block(n, have);
@@ -228,111 +291,108 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
         __syncwarp();
         fence_after();
         float down = 1.0f, up = both;
-        auto entry = [&](float v, int j, bool diagonal) {
-          const int d = back ? j - i : i - j;
-          if (back) return (diagonal && d < 0) || j >= have ? 0.0f : v * power[max(d, 0)];
-          return diagonal && d < 0 ? 0.0f : v * power[max(d, 0)];
-        };
         if (!BF16) {
           float top = 0.0f;
 #pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            if (back ? c < warp : c > warp) continue;
+          for (int c = 2 * side; c < 2 * side + 2; ++c) {
+            if (back ? c < quarter : c > quarter) continue;
+            float2 v[16];
+            products(c, have, both, v);
 #pragma unroll
-            for (int q = 0; q < 32; q += 16) {
-              float v[16];
-              tmem_load16(t_scores + lanes + c * 32 + q, v);
-              tmem_load_wait();
-#pragma unroll
-              for (int e = 0; e < 16; ++e) top = finite_max(top, entry(v[e], c * 32 + q + e, c == warp) * both);
-            }
+            for (int e = 0; e < 16; ++e) top = finite_max(finite_max(top, v[e].x), v[e].y);
           }
-          up = scale_up(top, down) * both;
+          tops[side][i] = top;
+          asm volatile("bar.sync 1, 256;" ::: "memory");
+          up = scale_up(fmaxf(tops[0][i], tops[1][i]), down) * both;
         }
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          const bool none = back ? c < warp : c > warp;
+        for (int c = 2 * side; c < 2 * side + 2; ++c) {
+          uint32_t w[16] = {};
+          if (back ? c >= quarter : c <= quarter) {
+            float2 v[16];
+            products(c, have, up, v);
 #pragma unroll
-          for (int q = 0; q < 32; q += 16) {
-            uint32_t w[8] = {};
-            if (!none) {
-              float v[16];
-              tmem_load16(t_scores + lanes + c * 32 + q, v);
-              tmem_load_wait();
-#pragma unroll
-              for (int e = 0; e < 8; ++e)
-                w[e] = pack2<BF16>(entry(v[2 * e], c * 32 + q + 2 * e, c == warp) * up, entry(v[2 * e + 1], c * 32 + q + 2 * e + 1, c == warp) * up);
-            }
-            *reinterpret_cast<uint4*>(chunk_at(sp, 128, i, c * 4 + q / 8)) = make_uint4(w[0], w[1], w[2], w[3]);
-            *reinterpret_cast<uint4*>(chunk_at(sp, 128, i, c * 4 + q / 8 + 1)) = make_uint4(w[4], w[5], w[6], w[7]);
+            for (int e = 0; e < 16; ++e) w[e] = pack2<BF16>(v[e].x, v[e].y);
           }
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            *reinterpret_cast<uint4*>(chunk_at(sp, 128, i, c * 4 + e)) = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
         }
         fence_async();
         fence_before();
         arrive_warp(&probs);
 
+        const float inter = P.so * power[i < have ? (back ? have - 1 - i : i + 1) : 0];
         ok = mbar_wait(&summed, n & 1, &gave_up) && ok;
         __syncwarp();
         fence_after();
-        const float inter = P.so * power[i < have ? (back ? have - 1 - i : i + 1) : 0];
         char* const stage = smem + (n & 1) * 2 * TA + warp * 32 * 128;  // 32 rows x 128 bytes
-        const int rows = min(32, have - warp * 32);
-        const int size = P.wide ? 4 : 2, per = P.wide ? 32 : 64;  // places of a round
-        char* const out = static_cast<char*>(P.out) + ((U.row0 + first + warp * 32) * B.H + h) * (int64_t)P.V * size;
+        char* const own = stage + lane * 128;
+        const int rows = min(32, have - quarter * 32), size = P.wide ? 4 : 2;
+        char* const out = static_cast<char*>(P.out) + ((U.row0 + first + quarter * 32) * B.H + h) * (int64_t)P.V * size;
         const int64_t pitch = (int64_t)B.H * P.V * size;
-        for (int c0 = 0; c0 < 64 * NV; c0 += per) {
-          for (int c = c0; c < c0 + per; c += 16) {
-            float a[16], v[16];
-            tmem_load16(t_inter + lanes + c, a);
-            tmem_load16(t_intra + lanes + c, v);
-            tmem_load_wait();
+        // the staged rows' `width` bytes go to `at` of the rows of out
+        auto copy = [&](int at, int width) {
+          __syncwarp();
+          const int x = lane % 8 * 16;
+          if (x < width && at + x < P.V * size) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float x = BF16 ? a[e] : a[e] * place_scale[n & 1][c + e];
-              v[e] = ok ? fmaf(inter, x, v[e] * down) : nan;
-            }
-            if (P.wide) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                *reinterpret_cast<float4*>(stage + lane * 128 + (((c - c0) / 4 + e) ^ (lane & 7)) * 16) =
-                    make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
-            } else {
-#pragma unroll
-              for (int e = 0; e < 2; ++e)
-                *reinterpret_cast<uint4*>(stage + lane * 128 + (((c - c0) / 8 + e) ^ (lane & 7)) * 16) =
-                    make_uint4(pack2<BF16>(v[8 * e], v[8 * e + 1]), pack2<BF16>(v[8 * e + 2], v[8 * e + 3]),
-                               pack2<BF16>(v[8 * e + 4], v[8 * e + 5]), pack2<BF16>(v[8 * e + 6], v[8 * e + 7]));
-            }
+            for (int r = lane / 8; r < 32; r += 4)
+              if (r < rows) *reinterpret_cast<uint4*>(out + r * pitch + at + x) = *reinterpret_cast<const uint4*>(stage + r * 128 + (x ^ (r & 7) * 16));
           }
-          if (c0 + per >= 64 * NV) {
+          __syncwarp();
+        };
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {  // 32 places at a time
+          const int c = (side * NV + k) * 32;
+          float a[32], v[32];
+          tmem_load16(t_inter + lanes + c, *reinterpret_cast<float(*)[16]>(a));
+          tmem_load16(t_inter + lanes + c + 16, *reinterpret_cast<float(*)[16]>(a + 16));
+          tmem_load16(t_intra + lanes + c, *reinterpret_cast<float(*)[16]>(v));
+          tmem_load16(t_intra + lanes + c + 16, *reinterpret_cast<float(*)[16]>(v + 16));
+          tmem_load_wait();
+          if (k == NV - 1) {
             fence_before();
             arrive_warp(&out_read);
           }
-          __syncwarp();
-          const int at = c0 * size + lane % 8 * 16;
-          if (at < P.V * size) {
-            for (int r = lane / 8; r < rows; r += 4)
-              *reinterpret_cast<uint4*>(out + r * pitch + at) = *reinterpret_cast<const uint4*>(stage + r * 128 + ((lane % 8) ^ (r & 7)) * 16);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = BF16 ? fmaf(inter, a[e], v[e]) : fmaf(inter, a[e] * place_scale[n & 1][c + e], v[e] * down);
+          if (!ok) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = __int_as_float(0x7fffffff);
           }
-          __syncwarp();
+          if (P.wide) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              *reinterpret_cast<float4*>(own + ((e ^ (lane & 7)) * 16)) = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+            copy(c * 4, 128);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              *reinterpret_cast<uint4*>(own + (((k * 4 + e) ^ (lane & 7)) * 16)) =
+                  make_uint4(pack2<BF16>(v[8 * e], v[8 * e + 1]), pack2<BF16>(v[8 * e + 2], v[8 * e + 3]),
+                             pack2<BF16>(v[8 * e + 4], v[8 * e + 5]), pack2<BF16>(v[8 * e + 6], v[8 * e + 7]));
+          }
         }
+        if (!P.wide) copy(side * NV * 64, NV * 64);
         fence_async();
         arrive_warp(&ab_free[n & 1]);
       }
     }
   } else {  // ------------------------------------------------ the faded B, and the state
-    const int r = threadIdx.x - 128;  // row of the block; place of v
-    const uint32_t lanes = (uint32_t)((warp - 4) * 32) << 16;
+    const int r = threadIdx.x & 127, side = (warp - 8) / 4;  // row of the block; place of v
+    const int k0 = side * 32 * NK;                           // entries k0 .. along b
+    const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
     const bool mine = r < P.V && r < 64 * NV;
     const int64_t size = (int64_t)P.K * P.V;
-    float x[64 * NK];
+    float x[32 * NK];
 #pragma unroll
-    for (int k = 0; k < 64 * NK; ++k) x[k] = 0.0f;
+    for (int k = 0; k < 32 * NK; ++k) x[k] = 0.0f;
     if (OUT && P.state && mine) {
-      const float* p = P.state + ((P.by_unit ? U.unit : U.s) * B.H + h) * size + r * P.sc;
+      const float* p = P.state + ((P.by_unit ? U.unit : U.s) * B.H + h) * size + k0 * P.sr + r * P.sc;
 #pragma unroll
-      for (int k = 0; k < 64 * NK; ++k)
-        if (k < P.K) x[k] = p[k * P.sr];
+      for (int k = 0; k < 32 * NK; ++k)
+        if (k0 + k < P.K) x[k] = p[k * P.sr];
     }
     bool ok = true;
     auto put_state = [&](int n) {  // as an operand of block n: row = place of v
@@ -340,17 +400,19 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
       if (!BF16) {
         float top = 0.0f, down;
 #pragma unroll
-        for (int k = 0; k < 64 * NK; ++k) top = finite_max(top, x[k]);
-        up = scale_up(top, down);
+        for (int k = 0; k < 32 * NK; ++k) top = finite_max(top, x[k]);
+        place_top[side][r] = top;
+        asm volatile("bar.sync 2, 256;" ::: "memory");
+        up = scale_up(fmaxf(place_top[0][r], place_top[1][r]), down);
         place_scale[n & 1][r] = down;
       }
       if (r < 64 * NV) {
 #pragma unroll
-        for (int c = 0; c < 8 * NK; ++c) {
+        for (int c = 0; c < 4 * NK; ++c) {
           uint32_t w[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) w[e] = pack2<BF16>(x[c * 8 + 2 * e] * up, x[c * 8 + 2 * e + 1] * up);
-          *reinterpret_cast<uint4*>(chunk_at(sp, 64 * NV, r, c)) = make_uint4(w[0], w[1], w[2], w[3]);
+          *reinterpret_cast<uint4*>(chunk_at(sp, 64 * NV, r, side * 4 * NK + c)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
       }
       fence_async();
@@ -364,14 +426,13 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
       char* const ta = smem + (n & 1) * 2 * TA;
       char* const tb = ta + TA;
       ok = mbar_wait(&full_ab[n & 1], (n >> 1) & 1, &gave_up) && ok;
-      const float f = r < have ? power[back ? r + 1 : have - 1 - r] * P.sb : 0.0f;
-      float up = 1.0f, down = 1.0f;
+      float f = r < have ? power[back ? r + 1 : have - 1 - r] * P.sb : 0.0f, down = 1.0f;
       if (!BF16) {
         float top = 0.0f;
         if (r < have) {
 #pragma unroll
-          for (int c = 0; c < 8 * NK; ++c) {
-            const uint4 q = *reinterpret_cast<const uint4*>(chunk_at(tb, 128, r, c));
+          for (int c = 0; c < 4 * NK; ++c) {
+            const uint4 q = *reinterpret_cast<const uint4*>(chunk_at(tb, 128, r, side * 4 * NK + c));
             const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -381,42 +442,44 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
           }
         }
         const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
-        if (lane == 0) tops[warp - 4] = __uint_as_float(bits);
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        up = scale_up(top, down);
+        if (lane == 0) warp_top[warp - 8] = __uint_as_float(bits);
+        asm volatile("bar.sync 2, 256;" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, warp_top[i]);
+        f *= scale_up(top, down);
       }
       if (OUT) ok = mbar_wait(&scores, n & 1, &gave_up) && ok;  // A and B have been read
       __syncwarp();
 #pragma unroll
-      for (int c = 0; c < 8 * NK; ++c) {
-        char* const at = chunk_at(tb, 128, r, c);
+      for (int c = 0; c < 4 * NK; ++c) {
+        char* const at = chunk_at(tb, 128, r, side * 4 * NK + c);
         const uint4 q = *reinterpret_cast<const uint4*>(at);
         const uint32_t in[4] = {q.x, q.y, q.z, q.w};
         uint32_t w0[4], w1[4], w2[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float2 v = unpack2<BF16>(in[e]);
-          v.x = r < have ? v.x * f * up : 0.0f, v.y = r < have ? v.y * f * up : 0.0f;
-          w0[e] = pack2<BF16>(v.x, v.y);
-          const float2 v0 = unpack2<BF16>(w0[e]);
-          v.x -= v0.x, v.y -= v0.y;
-          w1[e] = pack2<BF16>(v.x, v.y);
-          if (BF16) {
-            const float2 v1 = unpack2<BF16>(w1[e]);
-            w2[e] = pack2<BF16>(v.x - v1.x, v.y - v1.y);
+          float2 v = mul2(unpack2<BF16>(r < have ? in[e] : 0u), twice(f));
+          if (BF16) {  // the upper halves of what is left, cut off: each part takes 7 bits at least, and the last is rounded to 8 more
+            w0[e] = __byte_perm(__float_as_uint(v.x), __float_as_uint(v.y), 0x7632);
+            v = fma2(unpack2<BF16>(w0[e]), twice(-1.0f), v);
+            w1[e] = __byte_perm(__float_as_uint(v.x), __float_as_uint(v.y), 0x7632);
+            v = fma2(unpack2<BF16>(w1[e]), twice(-1.0f), v);
+            w2[e] = pack2<BF16>(v.x, v.y);
+          } else {
+            w0[e] = pack2<BF16>(v.x, v.y);
+            v = fma2(unpack2<BF16>(w0[e]), twice(-1.0f), v);
+            w1[e] = pack2<BF16>(v.x, v.y);
           }
         }
         *reinterpret_cast<uint4*>(at) = make_uint4(w0[0], w0[1], w0[2], w0[3]);
-        *reinterpret_cast<uint4*>(chunk_at(ta, 128, r, c)) = make_uint4(w1[0], w1[1], w1[2], w1[3]);
-        if (BF16) *reinterpret_cast<uint4*>(chunk_at(third, 128, r, c)) = make_uint4(w2[0], w2[1], w2[2], w2[3]);
+        *reinterpret_cast<uint4*>(at - tb + ta) = make_uint4(w1[0], w1[1], w1[2], w1[3]);
+        if (BF16) *reinterpret_cast<uint4*>(at - tb + third) = make_uint4(w2[0], w2[1], w2[2], w2[3]);
       }
       if (B.cu && have < STEPS) {  // rows of the next sequence, whatever they hold
         ok = mbar_wait(&full_v, n & 1, &gave_up) && ok;
         if (r >= have) {
 #pragma unroll
-          for (int c = 0; c < 8 * NV; ++c) *reinterpret_cast<uint4*>(chunk_at(tv, 128, r, c)) = make_uint4(0, 0, 0, 0);
+          for (int c = 0; c < 4 * NV; ++c) *reinterpret_cast<uint4*>(chunk_at(tv, 128, r, side * 4 * NV + c)) = make_uint4(0, 0, 0, 0);
         }
       }
       fence_async();
@@ -428,9 +491,9 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
       __syncwarp();
       fence_after();
 #pragma unroll
-      for (int c = 0; c < 64 * NK; c += 16) {
+      for (int c = 0; c < 32 * NK; c += 16) {
         float u[16];
-        tmem_load16(t_update + lanes + c, u);
+        tmem_load16(t_update + lanes + k0 + c, u);
         tmem_load_wait();
 #pragma unroll
         for (int e = 0; e < 16; ++e) x[c + e] = fmaf(whole, x[c + e], BF16 ? u[e] : u[e] * down);
@@ -445,14 +508,14 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
     float* to = OUT ? (P.last && U.ends(back) ? P.last + (U.s * B.H + h) * size : nullptr) : P.made + (U.unit * B.H + h) * size;
     if (to && mine) {
 #pragma unroll
-      for (int k = 0; k < 64 * NK; ++k)
-        if (k < P.K) to[k * P.sr + r * P.sc] = ok ? x[k] : __int_as_float(0x7fffffff);
+      for (int k = 0; k < 32 * NK; ++k)
+        if (k0 + k < P.K) to[(k0 + k) * P.sr + r * P.sc] = ok ? x[k] : __int_as_float(0x7fffffff);
     }
   }
   fence_before();
   __syncthreads();
   fence_after();
-  if (warp == 9) tmem_free<512>(tmem_slot);
+  if (warp == PRODUCTS) tmem_free<512>(tmem_slot);
 }
 
 template <bool BF16, int NK, int NV, bool OUT>
