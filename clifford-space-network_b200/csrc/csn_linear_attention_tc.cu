@@ -30,7 +30,10 @@ using namespace la;
 
 constexpr int STEPS = 128;      // of a block
 constexpr int BOX = 128 * 128;  // bytes of 128 rows x 64 places
-constexpr int LOADS = 16, PRODUCTS = 17, THREADS = 18 * 32;
+constexpr int LOADS = 16, PRODUCTS = 17, THREADS = 20 * 32;
+// Registers of a thread of warps 0 to 7, 8 to 15 and the rest: 256 x 88 + 256 x 128 + 128 x 40 = 60416 of the 640 x 96 = 61440
+// that a CTA is launched with.
+constexpr int FEW = 40, SOME = 88, MANY = 128;
 constexpr int MAX_PASSES = 3;
 
 __host__ __device__ constexpr int tile_a(int nk) { return nk * BOX; }
@@ -97,15 +100,16 @@ template <bool BF16, int NK, int NV, bool OUT>
 __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_constant__ Jobs jobs, const Batch B, int count) {
   constexpr int TA = tile_a(NK), PARTS = BF16 ? 3 : 2;
   extern __shared__ char raw[];
-  __shared__ uint64_t full_ab[2], full_v, ab_free[2], scores, keys, updated, probs, summed, state, out_read, drained;
+  __shared__ uint64_t full_ab[2], full_v, ab_free[2], scores, met, keys, updated, probs, summed, state, out_read, drained;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile uint32_t gave_up;
-  __shared__ float power[STEPS + 1], place_scale[2][128];
+  __shared__ __align__(16) float place_scale[2][128];
+  __shared__ float power[STEPS + 1];
   __shared__ float tops[2][128], place_top[2][128], warp_top[8];
   __shared__ __align__(16) float near[32], fan[64];  // powers of the distances to a side of 32 steps, and to its diagonal
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   char* const tv = smem + 4 * TA;       // stage s: a at smem + 2 s TA, b behind it
-  char* const sp = tv + NV * BOX;       // the state as an operand, or P
+  char* const sp = tv + NV * BOX;       // the state as an operand
   char* const third = sp + 2 * BOX;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
@@ -119,7 +123,7 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
 
   if (threadIdx.x == 0) {
     mbar_init(&full_ab[0], 1), mbar_init(&full_ab[1], 1), mbar_init(&full_v, 1), mbar_init(&ab_free[0], 8), mbar_init(&ab_free[1], 8);
-    mbar_init(&scores, 1), mbar_init(&keys, 8), mbar_init(&updated, 1), mbar_init(&probs, 8), mbar_init(&summed, 1);
+    mbar_init(&scores, 1), mbar_init(&met, 1), mbar_init(&keys, 8), mbar_init(&updated, 1), mbar_init(&probs, 8), mbar_init(&summed, 1);
     mbar_init(&state, 8), mbar_init(&out_read, 8), mbar_init(&drained, 1);
     mbar_init_fence();
     gave_up = 0;
@@ -139,6 +143,7 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
     return U.from + b * STEPS;
   };
 
+  if (warp >= 16) fewer_registers<FEW>();
   if (warp == LOADS) {  // ------------------------------------------------------------ loads
     const int y_a = h / P.a.shared, y_b = h / P.b.shared, y_v = h / P.v.shared, w = B.cu ? 0 : (int)U.s;
     const int row0 = B.cu ? (int)U.row0 : 0;
@@ -192,7 +197,7 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
       ok = ok && __all_sync(0xffffffffu, mbar_wait(b, n & 1, &gave_up));
       return ok;
     };
-    // A B^T of block n: as soon as its tiles are there and P of the block before has been read
+    // A B^T of block n, while the state is still on its way
     auto issue_scores = [&](int n) {
       if (!wait(&full_ab[n & 1], n >> 1)) return;
       fence_after();
@@ -203,6 +208,7 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
           const uint64_t at = d_a + (k / 4) * (BOX >> 4) + (k % 4) * 2;
           mma(t_scores, at, at + (TA >> 4), I_SCORES, k > 0);
         }
+        mma_commit(&scores);
       }
       __syncwarp();
     };
@@ -216,7 +222,7 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
 #pragma unroll
           for (int k = 0; k < 4 * NK; ++k)
             mma(t_inter, d_a + (k / 4) * (BOX >> 4) + (k % 4) * 2, d_sp + (k / 4) * (NV * BOX / 2 >> 4) + (k % 4) * 2, I_INTER, k > 0);
-          mma_commit(&scores);
+          mma_commit(&met);
         }
         __syncwarp();
       } else if (!wait(&full_ab[n & 1], n >> 1)) {
@@ -227,7 +233,7 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
       if (elect_one()) {
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) {
-          const uint64_t d = p == 0 ? d_b : p == 1 ? d_a : d_third;
+          const uint64_t d = p == 0 ? d_b : p == 2 || !BF16 ? d_a : d_third;
 #pragma unroll
           for (int k = 0; k < 8; ++k) mma(t_update, d_v + k * (2048 >> 4), d + k * (2048 >> 4), I_UPDATE, p > 0 || k > 0);
         }
@@ -240,11 +246,12 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
       if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          mma(t_intra, d_sp + (k / 4) * (BOX >> 4) + (k % 4) * 2, d_v + k * (2048 >> 4), I_INTRA, k > 0);
+          mma_tmem(t_intra, t_scores + k / 4 * 64 + k % 4 * 8, d_v + k * (2048 >> 4), I_INTRA, k > 0);
         mma_commit(&summed);
       }
       __syncwarp();
-      if (n + 1 < blocks) issue_scores(n + 1);
+      // P lies where the next scores go
+      if (n + 1 < blocks && wait(&summed, n)) issue_scores(n + 1);
     }
     if (!ok) {
       if (elect_one()) mma_commit(&drained);
@@ -252,6 +259,7 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
       for (uint32_t i = 0; i < POLLS && !mbar_try(&drained, 0); ++i) {}
     }
   } else if (warp < 8) {  // ------------------------------------------------- P, and out
+    fewer_registers<SOME>();
     if (OUT) {
       const int quarter = warp % 4, side = warp / 4, i = quarter * 32 + lane;  // row of the block
       const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
@@ -314,11 +322,9 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
 #pragma unroll
             for (int e = 0; e < 16; ++e) w[e] = pack2<BF16>(v[e].x, v[e].y);
           }
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            *reinterpret_cast<uint4*>(chunk_at(sp, 128, i, c * 4 + e)) = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+          tmem_store16(t_scores + lanes + side * 64 + (c & 1) * 16, w);  // over scores that this warp has read
         }
-        fence_async();
+        tmem_store_wait();
         fence_before();
         arrive_warp(&probs);
 
@@ -342,36 +348,40 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
           }
           __syncwarp();
         };
-#pragma unroll
-        for (int k = 0; k < NV; ++k) {  // 32 places at a time
-          const int c = (side * NV + k) * 32;
-          float a[32], v[32];
-          tmem_load16(t_inter + lanes + c, *reinterpret_cast<float(*)[16]>(a));
-          tmem_load16(t_inter + lanes + c + 16, *reinterpret_cast<float(*)[16]>(a + 16));
-          tmem_load16(t_intra + lanes + c, *reinterpret_cast<float(*)[16]>(v));
-          tmem_load16(t_intra + lanes + c + 16, *reinterpret_cast<float(*)[16]>(v + 16));
+#pragma unroll 1
+        for (int k = 0; k < 2 * NV; ++k) {  // 16 places at a time
+          const int c = (side * 2 * NV + k) * 16;
+          float2 a[8], v[8];
+          tmem_load16(t_inter + lanes + c, reinterpret_cast<float*>(a));
+          tmem_load16(t_intra + lanes + c, reinterpret_cast<float*>(v));
           tmem_load_wait();
-          if (k == NV - 1) {
+          if (k == 2 * NV - 1) {
             fence_before();
             arrive_warp(&out_read);
           }
 #pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = BF16 ? fmaf(inter, a[e], v[e]) : fmaf(inter, a[e] * place_scale[n & 1][c + e], v[e] * down);
+          for (int e = 0; e < 8; ++e) {
+            if (!BF16) {
+              a[e] = mul2(a[e], *reinterpret_cast<const float2*>(&place_scale[n & 1][c + 2 * e]));
+              v[e] = mul2(v[e], twice(down));
+            }
+            v[e] = fma2(twice(inter), a[e], v[e]);
+          }
           if (!ok) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = __int_as_float(0x7fffffff);
+            for (int e = 0; e < 8; ++e) v[e] = twice(__int_as_float(0x7fffffff));
           }
           if (P.wide) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              *reinterpret_cast<float4*>(own + ((e ^ (lane & 7)) * 16)) = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
-            copy(c * 4, 128);
+            for (int e = 0; e < 4; ++e)
+              *reinterpret_cast<float4*>(own + (((k % 2 * 4 + e) ^ (lane & 7)) * 16)) = make_float4(v[2 * e].x, v[2 * e].y, v[2 * e + 1].x, v[2 * e + 1].y);
+            if (k % 2) copy((c - 16) * 4, 128);
           } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              *reinterpret_cast<uint4*>(own + (((k * 4 + e) ^ (lane & 7)) * 16)) =
-                  make_uint4(pack2<BF16>(v[8 * e], v[8 * e + 1]), pack2<BF16>(v[8 * e + 2], v[8 * e + 3]),
-                             pack2<BF16>(v[8 * e + 4], v[8 * e + 5]), pack2<BF16>(v[8 * e + 6], v[8 * e + 7]));
+            for (int e = 0; e < 2; ++e)
+              *reinterpret_cast<uint4*>(own + (((k * 2 + e) ^ (lane & 7)) * 16)) =
+                  make_uint4(pack2<BF16>(v[4 * e].x, v[4 * e].y), pack2<BF16>(v[4 * e + 1].x, v[4 * e + 1].y),
+                             pack2<BF16>(v[4 * e + 2].x, v[4 * e + 2].y), pack2<BF16>(v[4 * e + 3].x, v[4 * e + 3].y));
           }
         }
         if (!P.wide) copy(side * NV * 64, NV * 64);
@@ -379,7 +389,8 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
         arrive_warp(&ab_free[n & 1]);
       }
     }
-  } else {  // ------------------------------------------------ the faded B, and the state
+  } else if (warp < 16) {  // --------------------------------- the faded B, and the state
+    more_registers<MANY>();
     const int r = threadIdx.x & 127, side = (warp - 8) / 4;  // row of the block; place of v
     const int k0 = side * 32 * NK;                           // entries k0 .. along b
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
@@ -448,14 +459,15 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
         for (int i = 0; i < 8; ++i) top = fmaxf(top, warp_top[i]);
         f *= scale_up(top, down);
       }
-      if (OUT) ok = mbar_wait(&scores, n & 1, &gave_up) && ok;  // A and B have been read
+      if (OUT) ok = mbar_wait(&scores, n & 1, &gave_up) && ok;  // B has been read
       __syncwarp();
+      uint32_t rest[16 * NK];  // the last part, kept until A has been read
 #pragma unroll
       for (int c = 0; c < 4 * NK; ++c) {
         char* const at = chunk_at(tb, 128, r, side * 4 * NK + c);
         const uint4 q = *reinterpret_cast<const uint4*>(at);
         const uint32_t in[4] = {q.x, q.y, q.z, q.w};
-        uint32_t w0[4], w1[4], w2[4];
+        uint32_t w0[4], w1[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float2 v = mul2(unpack2<BF16>(r < have ? in[e] : 0u), twice(f));
@@ -464,17 +476,19 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
             v = fma2(unpack2<BF16>(w0[e]), twice(-1.0f), v);
             w1[e] = __byte_perm(__float_as_uint(v.x), __float_as_uint(v.y), 0x7632);
             v = fma2(unpack2<BF16>(w1[e]), twice(-1.0f), v);
-            w2[e] = pack2<BF16>(v.x, v.y);
           } else {
             w0[e] = pack2<BF16>(v.x, v.y);
             v = fma2(unpack2<BF16>(w0[e]), twice(-1.0f), v);
-            w1[e] = pack2<BF16>(v.x, v.y);
           }
+          rest[4 * c + e] = pack2<BF16>(v.x, v.y);
         }
         *reinterpret_cast<uint4*>(at) = make_uint4(w0[0], w0[1], w0[2], w0[3]);
-        *reinterpret_cast<uint4*>(at - tb + ta) = make_uint4(w1[0], w1[1], w1[2], w1[3]);
-        if (BF16) *reinterpret_cast<uint4*>(at - tb + third) = make_uint4(w2[0], w2[1], w2[2], w2[3]);
+        if (BF16) *reinterpret_cast<uint4*>(at - tb + third) = make_uint4(w1[0], w1[1], w1[2], w1[3]);
       }
+      if (OUT) ok = mbar_wait(&met, n & 1, &gave_up) && ok;  // A has been read, and the state
+#pragma unroll
+      for (int c = 0; c < 4 * NK; ++c)
+        *reinterpret_cast<uint4*>(chunk_at(ta, 128, r, side * 4 * NK + c)) = make_uint4(rest[4 * c], rest[4 * c + 1], rest[4 * c + 2], rest[4 * c + 3]);
       if (B.cu && have < STEPS) {  // rows of the next sequence, whatever they hold
         ok = mbar_wait(&full_v, n & 1, &gave_up) && ok;
         if (r >= have) {
@@ -499,11 +513,7 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
         for (int e = 0; e < 16; ++e) x[c + e] = fmaf(whole, x[c + e], BF16 ? u[e] : u[e] * down);
       }
       fence_before();
-      if (OUT && n + 1 < blocks) {
-        ok = mbar_wait(&summed, n & 1, &gave_up) && ok;  // P has been read
-        __syncwarp();
-        put_state(n + 1);
-      }
+      if (OUT && n + 1 < blocks) put_state(n + 1);
     }
     float* to = OUT ? (P.last && U.ends(back) ? P.last + (U.s * B.H + h) * size : nullptr) : P.made + (U.unit * B.H + h) * size;
     if (to && mine) {
