@@ -5,11 +5,12 @@
 // and mirrored where time runs down.  A CTA runs through the blocks of one segment of one head:
 //   warp 16 loads the tiles of a, b (two stages) and v (one) by TMA;
 //   warp 17 issues the four products: A B^T and A X when the state is there, (l^.. B)^T V, P V.
-//   warps 0 to 7 turn A B^T into P and finish out, half a row to a thread;
+//   warps 0 to 7 turn A B^T into P, in its place in tensor memory, fade A X, which P V is then added to, and write out,
+//   half a row to a thread;
 //   warps 8 to 15 fade B, half a row to a thread, and keep the state in registers: half of the entries along b at one
 //   place of v;
-// Shared memory has no room for a copy of each operand, so they follow one another in place: the state as an operand, then
-// P, then the next state; B, then the first part of the faded B; A, then its second part, then rows of out on their way.
+// Shared memory has no room for a copy of each operand, so they follow one another in place: B, then the first part of the
+// faded B; A, then its last part.
 //
 // Roundings.  P and the state as an operand of A X are rounded to the tensors' type: out itself is, and these two add as
 // much again.  The state is not: it stays float32 in registers, and the faded B that enters it is split into parts that
@@ -31,9 +32,9 @@ using namespace la;
 constexpr int STEPS = 128;      // of a block
 constexpr int BOX = 128 * 128;  // bytes of 128 rows x 64 places
 constexpr int LOADS = 16, PRODUCTS = 17, THREADS = 20 * 32;
-// Registers of a thread of warps 0 to 7, 8 to 15 and the rest: 256 x 88 + 256 x 128 + 128 x 40 = 60416 of the 640 x 96 = 61440
+// Registers of a thread of warps 0 to 7, 8 to 15 and the rest: 256 x 72 + 256 x 152 + 128 x 24 = 60416 of the 640 x 96 = 61440
 // that a CTA is launched with.
-constexpr int FEW = 40, SOME = 88, MANY = 128;
+constexpr int FEW = 24, SOME = 72, MANY = 152;
 constexpr int MAX_PASSES = 3;
 
 __host__ __device__ constexpr int tile_a(int nk) { return nk * BOX; }
@@ -87,6 +88,13 @@ __device__ __forceinline__ float scale_up(float top, float& down) {
   return __uint_as_float((268 - e) << 23);
 }
 
+// 32 bytes in one access
+__device__ __forceinline__ void store8(void* p, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+               "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
 // 16 bytes: chunk c (8 places) of row r of a tile of boxes of `rows` rows
 __device__ __forceinline__ char* chunk_at(char* tile, int rows, int r, int c) {
   return tile + (c / 8) * rows * 128 + r * 128 + ((c % 8) ^ (r & 7)) * 16;
@@ -100,12 +108,12 @@ template <bool BF16, int NK, int NV, bool OUT>
 __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_constant__ Jobs jobs, const Batch B, int count) {
   constexpr int TA = tile_a(NK), PARTS = BF16 ? 3 : 2;
   extern __shared__ char raw[];
-  __shared__ uint64_t full_ab[2], full_v, ab_free[2], scores, met, keys, updated, probs, summed, state, out_read, drained;
+  __shared__ uint64_t full_ab[2], full_v, scores, met, keys[2], updated, probs, summed, state, out_read[2], drained;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile uint32_t gave_up;
   __shared__ __align__(16) float place_scale[2][128];
   __shared__ float power[STEPS + 1];
-  __shared__ float tops[2][128], place_top[2][128], warp_top[8];
+  __shared__ float tops[2][128], place_top[2][128], warp_top[2][8];
   __shared__ __align__(16) float near[32], fan[64];  // powers of the distances to a side of 32 steps, and to its diagonal
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   char* const tv = smem + 4 * TA;       // stage s: a at smem + 2 s TA, b behind it
@@ -122,9 +130,9 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
   const int steps = U.to - U.from, blocks = (steps + STEPS - 1) / STEPS;
 
   if (threadIdx.x == 0) {
-    mbar_init(&full_ab[0], 1), mbar_init(&full_ab[1], 1), mbar_init(&full_v, 1), mbar_init(&ab_free[0], 8), mbar_init(&ab_free[1], 8);
-    mbar_init(&scores, 1), mbar_init(&met, 1), mbar_init(&keys, 8), mbar_init(&updated, 1), mbar_init(&probs, 8), mbar_init(&summed, 1);
-    mbar_init(&state, 8), mbar_init(&out_read, 8), mbar_init(&drained, 1);
+    mbar_init(&full_ab[0], 1), mbar_init(&full_ab[1], 1), mbar_init(&full_v, 1),     mbar_init(&scores, 1), mbar_init(&met, 1), mbar_init(&updated, 1), mbar_init(&probs, 8), mbar_init(&summed, 1);
+    mbar_init(&state, 8), mbar_init(&out_read[0], 8), mbar_init(&out_read[1], 8), mbar_init(&drained, 1);
+    mbar_init(&keys[0], 8), mbar_init(&keys[1], 8);
     mbar_init_fence();
     gave_up = 0;
   }
@@ -135,7 +143,7 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t t_scores = tmem_slot, t_inter = t_scores + 128, t_intra = t_inter + 64 * NV, t_update = t_intra + 64 * NV;
+  const uint32_t t_scores = tmem_slot, t_update = t_scores + 128, t_out = t_update + 64 * NK;  // two of out
   // steps of block n: first .. first + have - 1 of the sequence
   auto block = [&](int n, int& have) {
     const int b = back ? blocks - 1 - n : n;
@@ -180,9 +188,7 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
     for (int n = 0; n + 1 < blocks && ok; ++n) {
       if (!(ok = __all_sync(0xffffffffu, mbar_wait(OUT ? &summed : &updated, n & 1, &gave_up)))) break;
       load_v(n + 1);
-      if (n + 2 >= blocks) continue;
-      if (OUT && !(ok = __all_sync(0xffffffffu, mbar_wait(&ab_free[n & 1], (n >> 1) & 1, &gave_up)))) break;
-      load_ab(n + 2);
+      if (n + 2 < blocks) load_ab(n + 2);
     }
     // copies in flight end before the shared memory does: where a wait gave up, and otherwise these have long been awaited
     for (int n = max(ab - 2, 0); n < ab; ++n)
@@ -216,37 +222,40 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
     for (int n = 0; n < blocks && ok; ++n) {
       const uint64_t d_a = operand(smem_addr(smem + (n & 1) * 2 * TA), BOX), d_b = d_a + (TA >> 4);
       if (OUT) {
-        if (!wait(&state, n) || (n > 0 && !wait(&out_read, n - 1))) break;
+        if (!wait(&state, n) || (n > 1 && !wait(&out_read[n & 1], (n >> 1) - 1))) break;
         fence_after();
         if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < 4 * NK; ++k)
-            mma(t_inter, d_a + (k / 4) * (BOX >> 4) + (k % 4) * 2, d_sp + (k / 4) * (NV * BOX / 2 >> 4) + (k % 4) * 2, I_INTER, k > 0);
+            mma(t_out + (n & 1) * 64 * NV, d_a + (k / 4) * (BOX >> 4) + (k % 4) * 2, d_sp + (k / 4) * (NV * BOX / 2 >> 4) + (k % 4) * 2, I_INTER, k > 0);
           mma_commit(&met);
         }
         __syncwarp();
       } else if (!wait(&full_ab[n & 1], n >> 1)) {
         break;
       }
-      if (!wait(&full_v, n) || !wait(&keys, n)) break;
-      fence_after();
-      if (elect_one()) {
+      if (!wait(&full_v, n)) break;
+      for (int q = 0; q < 2 && wait(&keys[q], n); ++q) {  // 64 rows of the faded B at a time
+        fence_after();
+        if (elect_one()) {
 #pragma unroll
-        for (int p = 0; p < PARTS; ++p) {
-          const uint64_t d = p == 0 ? d_b : p == 2 || !BF16 ? d_a : d_third;
+          for (int p = 0; p < PARTS; ++p) {
+            const uint64_t d = (p == 0 ? d_b : p == 2 || !BF16 ? d_a : d_third) + q * (8192 >> 4);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) mma(t_update, d_v + k * (2048 >> 4), d + k * (2048 >> 4), I_UPDATE, p > 0 || k > 0);
+            for (int k = 0; k < 4; ++k) mma(t_update, d_v + q * (8192 >> 4) + k * (2048 >> 4), d + k * (2048 >> 4), I_UPDATE, q > 0 || p > 0 || k > 0);
+          }
+          if (q == 1) mma_commit(&updated);
         }
-        mma_commit(&updated);
+        __syncwarp();
       }
-      __syncwarp();
+      if (!ok) break;
       if (!OUT) continue;
       if (!wait(&probs, n)) break;
       fence_after();
       if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          mma_tmem(t_intra, t_scores + k / 4 * 64 + k % 4 * 8, d_v + k * (2048 >> 4), I_INTRA, k > 0);
+          mma_tmem(t_out + (n & 1) * 64 * NV, t_scores + k / 4 * 64 + k % 4 * 8, d_v + k * (2048 >> 4), I_INTRA, true);
         mma_commit(&summed);
       }
       __syncwarp();
@@ -264,6 +273,7 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
       const int quarter = warp % 4, side = warp / 4, i = quarter * 32 + lane;  // row of the block
       const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
       const float both = P.so * P.sb;
+      const bool whole_sectors = !P.wide && P.V % 16 == 0 && (reinterpret_cast<uintptr_t>(P.out) & 31) == 0;
       // 32 products of this thread's row, c of four, faded and times `up`; `have`: places of the block
       auto products = [&](int c, int have, float up, float2 (&v)[16]) {
         tmem_load16(t_scores + lanes + c * 32, reinterpret_cast<float*>(v));
@@ -300,6 +310,7 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
         fence_after();
         float down = 1.0f, up = both;
         if (!BF16) {
+          // a row with an infinity is one in any case, and out has no use for what 2^60 leaves below 1
           float top = 0.0f;
 #pragma unroll 1
           for (int c = 2 * side; c < 2 * side + 2; ++c) {
@@ -307,11 +318,11 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
             float2 v[16];
             products(c, have, both, v);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) top = finite_max(finite_max(top, v[e].x), v[e].y);
+            for (int e = 0; e < 16; ++e) top = fmaxf(top, fmaxf(fabsf(v[e].x), fabsf(v[e].y)));
           }
           tops[side][i] = top;
           asm volatile("bar.sync 1, 256;" ::: "memory");
-          up = scale_up(fmaxf(tops[0][i], tops[1][i]), down) * both;
+          up = scale_up(fmaxf(fmaxf(tops[0][i], tops[1][i]), 0x1p-46f), down) * both;
         }
 #pragma unroll 1
         for (int c = 2 * side; c < 2 * side + 2; ++c) {
@@ -324,69 +335,70 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
           }
           tmem_store16(t_scores + lanes + side * 64 + (c & 1) * 16, w);  // over scores that this warp has read
         }
+        // A X, faded, is what P V is added to
+        const float inter = P.so * power[i < have ? (back ? have - 1 - i : i + 1) : 0] * (BF16 ? 1.0f : 1.0f / down);
+        const uint32_t t_mine = t_out + (n & 1) * 64 * NV + side * 32 * NV + lanes;
+        ok = mbar_wait(&met, n & 1, &gave_up) && ok;
+        __syncwarp();
+        fence_after();
+#pragma unroll 1
+        for (int c = 0; c < 32 * NV; c += 16) {
+          float2 a[8];
+          tmem_load16(t_mine + c, reinterpret_cast<float*>(a));
+          tmem_load_wait();
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            if (!BF16) a[e] = mul2(a[e], *reinterpret_cast<const float2*>(&place_scale[n & 1][side * 32 * NV + c + 2 * e]));
+            a[e] = mul2(a[e], twice(inter));
+          }
+          tmem_store16(t_mine + c, reinterpret_cast<const uint32_t*>(a));
+        }
         tmem_store_wait();
         fence_before();
         arrive_warp(&probs);
 
-        const float inter = P.so * power[i < have ? (back ? have - 1 - i : i + 1) : 0];
         ok = mbar_wait(&summed, n & 1, &gave_up) && ok;
         __syncwarp();
         fence_after();
-        char* const stage = smem + (n & 1) * 2 * TA + warp * 32 * 128;  // 32 rows x 128 bytes
-        char* const own = stage + lane * 128;
-        const int rows = min(32, have - quarter * 32), size = P.wide ? 4 : 2;
-        char* const out = static_cast<char*>(P.out) + ((U.row0 + first + quarter * 32) * B.H + h) * (int64_t)P.V * size;
-        const int64_t pitch = (int64_t)B.H * P.V * size;
-        // the staged rows' `width` bytes go to `at` of the rows of out
-        auto copy = [&](int at, int width) {
-          __syncwarp();
-          const int x = lane % 8 * 16;
-          if (x < width && at + x < P.V * size) {
-#pragma unroll
-            for (int r = lane / 8; r < 32; r += 4)
-              if (r < rows) *reinterpret_cast<uint4*>(out + r * pitch + at + x) = *reinterpret_cast<const uint4*>(stage + r * 128 + (x ^ (r & 7) * 16));
-          }
-          __syncwarp();
-        };
+        const bool there = i < have;
+        const int64_t at = ((U.row0 + first + i) * B.H + h) * (int64_t)P.V;
 #pragma unroll 1
         for (int k = 0; k < 2 * NV; ++k) {  // 16 places at a time
           const int c = (side * 2 * NV + k) * 16;
-          float2 a[8], v[8];
-          tmem_load16(t_inter + lanes + c, reinterpret_cast<float*>(a));
-          tmem_load16(t_intra + lanes + c, reinterpret_cast<float*>(v));
+          float2 v[8];
+          tmem_load16(t_mine + k * 16, reinterpret_cast<float*>(v));
           tmem_load_wait();
           if (k == 2 * NV - 1) {
             fence_before();
-            arrive_warp(&out_read);
+            arrive_warp(&out_read[n & 1]);
           }
+          if (!BF16) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            if (!BF16) {
-              a[e] = mul2(a[e], *reinterpret_cast<const float2*>(&place_scale[n & 1][c + 2 * e]));
-              v[e] = mul2(v[e], twice(down));
-            }
-            v[e] = fma2(twice(inter), a[e], v[e]);
+            for (int e = 0; e < 8; ++e) v[e] = mul2(v[e], twice(down));
           }
           if (!ok) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = twice(__int_as_float(0x7fffffff));
           }
+          if (!there || c >= P.V) continue;
+          // a row to a thread, whole sectors at a time; V is a multiple of 8
           if (P.wide) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              *reinterpret_cast<float4*>(own + (((k % 2 * 4 + e) ^ (lane & 7)) * 16)) = make_float4(v[2 * e].x, v[2 * e].y, v[2 * e + 1].x, v[2 * e + 1].y);
-            if (k % 2) copy((c - 16) * 4, 128);
+            float* to = static_cast<float*>(P.out) + at + c;
+            store8(to, reinterpret_cast<uint32_t*>(v));
+            if (c + 8 < P.V) store8(to + 8, reinterpret_cast<uint32_t*>(v + 4));
           } else {
+            uint32_t w[8];
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-              *reinterpret_cast<uint4*>(own + (((k * 2 + e) ^ (lane & 7)) * 16)) =
-                  make_uint4(pack2<BF16>(v[4 * e].x, v[4 * e].y), pack2<BF16>(v[4 * e + 1].x, v[4 * e + 1].y),
-                             pack2<BF16>(v[4 * e + 2].x, v[4 * e + 2].y), pack2<BF16>(v[4 * e + 3].x, v[4 * e + 3].y));
+            for (int e = 0; e < 8; ++e) w[e] = pack2<BF16>(v[e].x, v[e].y);
+            uint16_t* to = static_cast<uint16_t*>(P.out) + at + c;
+            if (whole_sectors) {
+              store8(to, w);
+            } else {
+              *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+              if (c + 8 < P.V) *reinterpret_cast<uint4*>(to + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+            }
           }
         }
-        if (!P.wide) copy(side * NV * 64, NV * 64);
-        fence_async();
-        arrive_warp(&ab_free[n & 1]);
       }
     }
   } else if (warp < 16) {  // --------------------------------- the faded B, and the state
@@ -411,7 +423,7 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
       if (!BF16) {
         float top = 0.0f, down;
 #pragma unroll
-        for (int k = 0; k < 32 * NK; ++k) top = finite_max(top, x[k]);
+        for (int k = 0; k < 32 * NK; ++k) top = fmaxf(top, fabsf(x[k]));
         place_top[side][r] = top;
         asm volatile("bar.sync 2, 256;" ::: "memory");
         up = scale_up(fmaxf(place_top[0][r], place_top[1][r]), down);
@@ -431,19 +443,48 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
       arrive_warp(&state);
     };
     if (OUT && blocks > 0) put_state(0);
-    for (int n = 0; n < blocks; ++n) {
+    // The faded B of a block is made 64 rows at a time, 2 NK chunks of a row to a thread, the first 64 while the products of
+    // the block before run.
+    const int row = (warp & 1) * 32 + lane, c0 = (warp - 8) / 2 * 2 * NK;
+    float down = 1.0f, next_down = 1.0f, up = P.sb;
+    uint32_t early[PARTS][8 * NK];
+    // the parts of chunk c of row `at` of B, whose factor is f; nothing of rows that are not the sequence's, whatever they hold
+    auto split = [&](const char* at, bool in, float2 f, uint32_t* w0, uint32_t* w1, uint32_t* w2) {
+      const uint4 x4 = in ? *reinterpret_cast<const uint4*>(at) : make_uint4(0, 0, 0, 0);
+      const uint32_t x[4] = {x4.x, x4.y, x4.z, x4.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float2 v = mul2(unpack2<BF16>(x[e]), f);
+        if (BF16) {  // the upper halves of what is left, cut off: each part takes 7 bits at least, and the last is rounded to 8 more
+          const uint32_t ux = __float_as_uint(v.x), uy = __float_as_uint(v.y);
+          w0[e] = __byte_perm(ux, uy, 0x7632);
+          v = fma2(make_float2(__uint_as_float(ux & 0xffff0000u), __uint_as_float(uy & 0xffff0000u)), twice(-1.0f), v);
+          const uint32_t sx = __float_as_uint(v.x), sy = __float_as_uint(v.y);
+          w1[e] = __byte_perm(sx, sy, 0x7632);
+          v = fma2(make_float2(__uint_as_float(sx & 0xffff0000u), __uint_as_float(sy & 0xffff0000u)), twice(-1.0f), v);
+          w2[e] = pack2<BF16>(v.x, v.y);
+        } else {
+          w0[e] = pack2<BF16>(v.x, v.y);
+          v = fma2(unpack2<BF16>(w0[e]), twice(-1.0f), v);
+          w1[e] = pack2<BF16>(v.x, v.y);
+        }
+      }
+    };
+    auto factor = [&](int i, int have) { return twice(i < have ? power[back ? i + 1 : have - 1 - i] * up : 0.0f); };
+    auto begin = [&](int n) {  // the first 64 rows of block n
       int have;
       block(n, have);
-      char* const ta = smem + (n & 1) * 2 * TA;
-      char* const tb = ta + TA;
+      const char* const tb = smem + (n & 1) * 2 * TA + TA;
       ok = mbar_wait(&full_ab[n & 1], (n >> 1) & 1, &gave_up) && ok;
-      float f = r < have ? power[back ? r + 1 : have - 1 - r] * P.sb : 0.0f, down = 1.0f;
+      __syncwarp();
       if (!BF16) {
         float top = 0.0f;
+        up = P.sb;
         if (r < have) {
+          const float f = factor(r, have).x;
 #pragma unroll
           for (int c = 0; c < 4 * NK; ++c) {
-            const uint4 q = *reinterpret_cast<const uint4*>(chunk_at(tb, 128, r, side * 4 * NK + c));
+            const uint4 q = *reinterpret_cast<const uint4*>(chunk_at(const_cast<char*>(tb), 128, r, side * 4 * NK + c));
             const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -453,52 +494,64 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
           }
         }
         const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
-        if (lane == 0) warp_top[warp - 8] = __uint_as_float(bits);
+        if (lane == 0) warp_top[n & 1][warp - 8] = __uint_as_float(bits);
         asm volatile("bar.sync 2, 256;" ::: "memory");
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, warp_top[i]);
-        f *= scale_up(top, down);
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, warp_top[n & 1][i]);
+        up *= scale_up(top, next_down);
       }
+      const float2 f = factor(row, have);
+#pragma unroll
+      for (int c = 0; c < 2 * NK; ++c)
+        split(chunk_at(const_cast<char*>(tb), 128, row, c0 + c), row < have, f, &early[0][4 * c], &early[1][4 * c], &early[PARTS - 1][4 * c]);
+    };
+    auto put = [&](char* tile, int i, int c, const uint32_t* w) {
+      *reinterpret_cast<uint4*>(chunk_at(tile, 128, i, c0 + c)) = make_uint4(w[0], w[1], w[2], w[3]);
+    };
+    if (blocks > 0) begin(0);
+    for (int n = 0; n < blocks; ++n) {
+      int have;
+      block(n, have);
+      char* const ta = smem + (n & 1) * 2 * TA;
+      char* const tb = ta + TA;
+      down = next_down;
       if (OUT) ok = mbar_wait(&scores, n & 1, &gave_up) && ok;  // B has been read
       __syncwarp();
-      uint32_t rest[16 * NK];  // the last part, kept until A has been read
 #pragma unroll
-      for (int c = 0; c < 4 * NK; ++c) {
-        char* const at = chunk_at(tb, 128, r, side * 4 * NK + c);
-        const uint4 q = *reinterpret_cast<const uint4*>(at);
-        const uint32_t in[4] = {q.x, q.y, q.z, q.w};
-        uint32_t w0[4], w1[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float2 v = mul2(unpack2<BF16>(r < have ? in[e] : 0u), twice(f));
-          if (BF16) {  // the upper halves of what is left, cut off: each part takes 7 bits at least, and the last is rounded to 8 more
-            w0[e] = __byte_perm(__float_as_uint(v.x), __float_as_uint(v.y), 0x7632);
-            v = fma2(unpack2<BF16>(w0[e]), twice(-1.0f), v);
-            w1[e] = __byte_perm(__float_as_uint(v.x), __float_as_uint(v.y), 0x7632);
-            v = fma2(unpack2<BF16>(w1[e]), twice(-1.0f), v);
-          } else {
-            w0[e] = pack2<BF16>(v.x, v.y);
-            v = fma2(unpack2<BF16>(w0[e]), twice(-1.0f), v);
-          }
-          rest[4 * c + e] = pack2<BF16>(v.x, v.y);
-        }
-        *reinterpret_cast<uint4*>(at) = make_uint4(w0[0], w0[1], w0[2], w0[3]);
-        if (BF16) *reinterpret_cast<uint4*>(at - tb + third) = make_uint4(w1[0], w1[1], w1[2], w1[3]);
+      for (int c = 0; c < 2 * NK; ++c) {
+        put(tb, row, c, &early[0][4 * c]);
+        if (BF16) put(third, row, c, &early[1][4 * c]);
       }
-      if (OUT) ok = mbar_wait(&met, n & 1, &gave_up) && ok;  // A has been read, and the state
-#pragma unroll
-      for (int c = 0; c < 4 * NK; ++c)
-        *reinterpret_cast<uint4*>(chunk_at(ta, 128, r, side * 4 * NK + c)) = make_uint4(rest[4 * c], rest[4 * c + 1], rest[4 * c + 2], rest[4 * c + 3]);
-      if (B.cu && have < STEPS) {  // rows of the next sequence, whatever they hold
+      if (B.cu && have < STEPS) {  // rows of the next sequence in v
         ok = mbar_wait(&full_v, n & 1, &gave_up) && ok;
-        if (r >= have) {
 #pragma unroll
-          for (int c = 0; c < 4 * NV; ++c) *reinterpret_cast<uint4*>(chunk_at(tv, 128, r, side * 4 * NV + c)) = make_uint4(0, 0, 0, 0);
+        for (int c = 0; c < 4 * NV; ++c)
+          if (r >= have) *reinterpret_cast<uint4*>(chunk_at(tv, 128, r, side * 4 * NV + c)) = make_uint4(0, 0, 0, 0);
+      }
+      const float2 f = factor(row + 64, have);
+      uint32_t rest[8 * NK];
+#pragma unroll
+      for (int c = 0; c < 2 * NK; ++c) {
+        uint32_t w0[4], w1[4];
+        split(chunk_at(tb, 128, row + 64, c0 + c), row + 64 < have, f, w0, BF16 ? w1 : &rest[4 * c], &rest[4 * c]);
+        put(tb, row + 64, c, w0);
+        if (BF16) put(third, row + 64, c, w1);
+        if (c == NK - 1) {
+          if (OUT) ok = mbar_wait(&met, n & 1, &gave_up) && ok;  // A has been read, and the state
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 2 * NK; ++i) put(ta, row, i, &early[PARTS - 1][4 * i]);
+          fence_async();
+          fence_before();
+          arrive_warp(&keys[0]);
         }
       }
+#pragma unroll
+      for (int c = 0; c < 2 * NK; ++c) put(ta, row + 64, c, &rest[4 * c]);
       fence_async();
       fence_before();
-      arrive_warp(&keys);
+      arrive_warp(&keys[1]);
+      if (n + 1 < blocks) begin(n + 1);
 
       const float whole = power[have];
       ok = mbar_wait(&updated, n & 1, &gave_up) && ok;
