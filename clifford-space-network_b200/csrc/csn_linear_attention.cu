@@ -131,15 +131,23 @@ __global__ void __launch_bounds__(256) join_kernel(const Batch B, const float* _
   const int64_t row0 = B.cu ? Unit::border(B, s) : s * B.T;
   const int64_t len = B.cu ? max(Unit::border(B, s + 1), row0) - row0 : B.T;
   const int64_t first = B.cu ? row0 / B.seg + s : s * B.segs, n = max((len + B.seg - 1) / B.seg, (int64_t)1);
-  const float whole = fade(B.log_decay[h], B.seg);
+  const float whole = fade(B.log_decay[h], B.seg), rest = fade(B.log_decay[h], (int)(len - (n - 1) * B.seg));
   float x = enters ? enters[(s * B.H + h) * size + i] : 0.0f;
-  for (int64_t j = 0; j < n; ++j) {
-    const int64_t m = back ? n - 1 - j : j;
-    float* p = made + ((first + m) * B.H + h) * size + i;
-    const float own = j + 1 < n ? *p : 0.0f;
-    *p = x;
-    const float f = (m + 1) * B.seg > len ? fade(B.log_decay[h], (int)(len - m * B.seg)) : whole;
-    x = fmaf(f, x, own);
+  const int64_t step = (back ? -1 : 1) * (int64_t)B.H * size;
+  float* p = made + ((first + (back ? n - 1 : 0)) * B.H + h) * size + i;
+  constexpr int N = 8;  // loads in flight
+  for (int64_t j0 = 0; j0 < n; j0 += N) {
+    float own[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (j0 + j + 1 < n) own[j] = p[j * step];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (j0 + j >= n) break;
+      p[j * step] = x;
+      if (j0 + j + 1 < n) x = fmaf(back && j0 + j == 0 ? rest : whole, x, own[j]);  // only the last segment in time may be short
+    }
+    p += N * step;
   }
 }
 
@@ -235,19 +243,21 @@ bool aligned(const void* p, int n) { return reinterpret_cast<uintptr_t>(p) % n =
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // The steps of a segment, a multiple of 128.  float32: enough segments for 12 warps on each SM.  16 bits, one CTA an SM: what
-// takes the fewest blocks of 128 steps one after another, where a CTA's start and end cost about 3 blocks and the first
-// pass, which cut sequences need, half as much again as the pass itself.
-void cut(Batch& B, int V, int passes, bool packed, bool half) {
-  const int64_t rows = up(B.T, 128), heads = (int64_t)B.H * (packed ? 1 : B.S);
+// takes the least time by these, measured with 128 x 128 states in bf16, in units of 0.1 us: a block of 128 steps 39, the start and end
+// of a CTA 90; where sequences are cut, in the first pass 27 and 70, and join_kernel 50, 5 a segment and its states' bytes.
+void cut(Batch& B, int Dk, int Dv, int passes, bool packed, bool half) {
+  const int64_t rows = up(B.T, 128), heads = (int64_t)B.H * (packed ? 1 : B.S), ways = std::min(passes, 2);
   int64_t best = 1;
   if (half) {
     int64_t least = INT64_MAX;
     for (int64_t n = 1; n <= std::min(rows, (int64_t)64); ++n) {
-      const int64_t cost = up(heads * passes * n, 148) * (up(rows, n) + 3) * 2 + (n > 1 ? up(heads * std::min(passes, 2) * n, 148) * (up(rows, n) + 3) : 0);
+      const int64_t blocks = up(rows, n);
+      int64_t cost = up(heads * passes * n, 148) * (39 * blocks + 90);
+      if (n > 1) cost += up(heads * ways * n, 148) * (27 * blocks + 70) + ways * (50 + 5 * n + heads * n * Dk * Dv / 50000);
       if (cost < least) least = cost, best = n;
     }
   } else {
-    best = std::min(rows, up(148 * 12, heads * up(V, 32)));
+    best = std::min(rows, up(148 * 12, heads * up(std::min(Dk, Dv), 32)));
   }
   B.seg = (int)(std::max(up(rows, std::max(best, (int64_t)1)), (int64_t)1) * 128);
   B.segs = packed ? 0 : (int)std::max(up(B.T, B.seg), (int64_t)1);
@@ -257,7 +267,7 @@ bool is_cut(const Batch& B, bool packed) { return packed ? B.T > B.seg : B.segs 
 
 Batch batch(int64_t S, int64_t T, int H, int Dk, int Dv, const int32_t* cu, bool packed, const float* log_decay, bool backward, int dtype) {
   Batch B = {cu, S, T, H, 0, 0, 0, log_decay};
-  cut(B, std::min(Dk, Dv), backward ? 3 : 1, packed, dtype != CSN_F32);
+  cut(B, Dk, Dv, backward ? 3 : 1, packed, dtype != CSN_F32);
   return B;
 }
 
@@ -407,9 +417,9 @@ extern "C" int csn_linear_attention_bwd(const void* q, const void* k, const void
       {K, Q, O, shared > 1 ? dv32 : dv, ds_last, ds0, nullptr, Dv, 1, (int)Dk, (int)Dv, 1.0f, scale, false, shared > 1, true}};
   if (R.states) {
     P[0].made = made, P[2].made = back;
-    const int from = dq ? 0 : 2, to = dk || dv ? 2 : 0;  // the states of the forward direction are those that dq needs
-    for (int i = from; i <= to; i += 2)
-      if (int rc = run(B, &P[i], 1, true, dtype, st)) return rc;
+    // the states of the forward direction are those that dq needs
+    const Pass firsts[2] = {dq ? P[0] : P[2], P[2]};
+    if (int rc = run(B, firsts, dq && (dk || dv) ? 2 : 1, true, dtype, st)) return rc;
     if (dq) join(B, s0, made, entries, false, st);
     if (dk || dv) join(B, ds_last, back, entries, true, st);
     P[0].state = made, P[1].state = P[2].state = back;

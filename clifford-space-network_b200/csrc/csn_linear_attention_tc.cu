@@ -130,20 +130,25 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
   const int steps = U.to - U.from, blocks = (steps + STEPS - 1) / STEPS;
 
   if (threadIdx.x == 0) {
-    mbar_init(&full_ab[0], 1), mbar_init(&full_ab[1], 1), mbar_init(&full_v, 1),     mbar_init(&scores, 1), mbar_init(&met, 1), mbar_init(&updated, 1), mbar_init(&probs, 8), mbar_init(&summed, 1);
+    mbar_init(&full_ab[0], 1), mbar_init(&full_ab[1], 1), mbar_init(&full_v, 1), mbar_init(&scores, 1), mbar_init(&met, 1);
+    mbar_init(&updated, 1), mbar_init(&probs, 8), mbar_init(&summed, 1);
     mbar_init(&state, 8), mbar_init(&out_read[0], 8), mbar_init(&out_read[1], 8), mbar_init(&drained, 1);
     mbar_init(&keys[0], 8), mbar_init(&keys[1], 8);
     mbar_init_fence();
     gave_up = 0;
   }
-  if (threadIdx.x <= STEPS) power[threadIdx.x] = fade(B.log_decay[h], threadIdx.x);
-  else if (threadIdx.x - 256 < 32u) near[threadIdx.x - 256] = fade(B.log_decay[h], back ? threadIdx.x - 256 : 287 - threadIdx.x);
-  else if (threadIdx.x - 320 < 63u) fan[threadIdx.x - 320] = fade(B.log_decay[h], abs((int)threadIdx.x - 351));
   if (warp == PRODUCTS) tmem_alloc<512>(&tmem_slot);
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t t_scores = tmem_slot, t_update = t_scores + 128, t_out = t_update + 64 * NK;  // two of out
+  if (warp < 16) {  // while the first tiles are on their way
+    const unsigned t = threadIdx.x;
+    if (t <= STEPS) power[t] = fade(B.log_decay[h], t);
+    else if (t - 256 < 32u) near[t - 256] = fade(B.log_decay[h], back ? t - 256 : 287 - t);
+    else if (t - 320 < 63u) fan[t - 320] = fade(B.log_decay[h], abs((int)t - 351));
+    asm volatile("bar.sync 3, 512;" ::: "memory");
+  }
   // steps of block n: first .. first + have - 1 of the sequence
   auto block = [&](int n, int& have) {
     const int b = back ? blocks - 1 - n : n;
