@@ -16,85 +16,409 @@ namespace {
 
 constexpr int THREADS = 256;
 
-template <typename T, int N>
-__device__ __forceinline__ void load(const T* p, float (&v)[N]) {
-  const Pack<T, N> x = *reinterpret_cast<const Pack<T, N>*>(p);
+// V neighbouring places in float32.  The arithmetic of 8 goes in pairs, one instruction each: one by one, with each place taken
+// out of its word and put back by itself, the kernels executed 20 and 40 instructions an element and were bound by them.
+template <int V>
+struct Floats {
+  float v[V];
+};
+template <int V>
+__device__ __forceinline__ Floats<V> all(float a) {
+  Floats<V> r;
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = to_float(x.v[i]);
+  for (int i = 0; i < V; ++i) r.v[i] = a;
+  return r;
 }
-template <typename T, int N>
-__device__ __forceinline__ void store(T* p, const float (&v)[N]) {
-  Pack<T, N> x;
+template <int V>
+__device__ __forceinline__ Floats<V> fma(const Floats<V>& a, const Floats<V>& b, const Floats<V>& c) {
+  Floats<V> r;
+  if constexpr (V % 2 == 0) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) x.v[i] = from_float<T>(v[i]);
-  *reinterpret_cast<Pack<T, N>*>(p) = x;
+    for (int i = 0; i < V; i += 2) {
+      const float2 x = fma2(make_float2(a.v[i], a.v[i + 1]), make_float2(b.v[i], b.v[i + 1]), make_float2(c.v[i], c.v[i + 1]));
+      r.v[i] = x.x, r.v[i + 1] = x.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.v[i] = fmaf(a.v[i], b.v[i], c.v[i]);
+  }
+  return r;
+}
+template <int V>
+__device__ __forceinline__ Floats<V> mul(const Floats<V>& a, const Floats<V>& b) {
+  Floats<V> r;
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const float2 x = mul2(make_float2(a.v[i], a.v[i + 1]), make_float2(b.v[i], b.v[i + 1]));
+      r.v[i] = x.x, r.v[i + 1] = x.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.v[i] = a.v[i] * b.v[i];
+  }
+  return r;
+}
+template <int V>
+__device__ __forceinline__ Floats<V> add(const Floats<V>& a, const Floats<V>& b) {
+  Floats<V> r;
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const float2 x = add2(make_float2(a.v[i], a.v[i + 1]), make_float2(b.v[i], b.v[i + 1]));
+      r.v[i] = x.x, r.v[i + 1] = x.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.v[i] = a.v[i] + b.v[i];
+  }
+  return r;
+}
+template <int V>
+__device__ __forceinline__ float sum(const Floats<V>& a) {
+  float r = a.v[0];
+#pragma unroll
+  for (int i = 1; i < V; ++i) r += a.v[i];
+  return r;
 }
 
-// Sum over a CTA, in a fixed order; every thread gets it.
-__device__ __forceinline__ float cta_sum(float v, float* room) {
+__device__ __forceinline__ float2 pair(uint32_t w, __nv_bfloat16) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+__device__ __forceinline__ float2 pair(uint32_t w, __half) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
+
+// V places as they lie in memory
+template <typename T, int V>
+struct Piece {
+  Pack<T, V> p;
+};
+template <typename T>
+struct Piece<T, 8> {
+  uint4 p;
+};
+template <typename T, int V>
+__device__ __forceinline__ Floats<V> floats(const Piece<T, V>& x) {
+  Floats<V> r;
+  if constexpr (V == 8) {
+    const uint32_t w[4] = {x.p.x, x.p.y, x.p.z, x.p.w};
 #pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) room[threadIdx.x / 32] = v;
-  __syncthreads();
-  v = 0.0f;
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = pair(w[i], T{});
+      r.v[2 * i] = f.x, r.v[2 * i + 1] = f.y;
+    }
+  } else {
+    r.v[0] = to_float(x.p.v[0]);
+  }
+  return r;
+}
+template <typename T, int V>
+__device__ __forceinline__ void store(T* to, const Floats<V>& a) {
+  if constexpr (V == 8)
+    *reinterpret_cast<uint4*>(to) = make_uint4(pack<T>(a.v[0], a.v[1]), pack<T>(a.v[2], a.v[3]), pack<T>(a.v[4], a.v[5]), pack<T>(a.v[6], a.v[7]));
+  else
+    to[0] = from_float<T>(a.v[0]);
+}
+// V neighbouring weights
+template <int V>
+__device__ __forceinline__ Floats<V> weights(const float* p) {
+  Floats<V> r;
+  if constexpr (V == 8) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    r.v[0] = a.x, r.v[1] = a.y, r.v[2] = a.z, r.v[3] = a.w, r.v[4] = b.x, r.v[5] = b.y, r.v[6] = b.z, r.v[7] = b.w;
+  } else {
+    r.v[0] = __ldg(p);
+  }
+  return r;
+}
+template <int V, typename T>
+__device__ __forceinline__ Floats<V> weights(const T* p) { return floats<T, V>(*reinterpret_cast<const Piece<T, V>*>(p)); }
+
+// Sums of n values over the TPR threads that share a row, in a fixed order; each of them gets them.  Rows of more than a
+// warp meet in `room`, whose two halves take turns, so that one barrier a call is enough.
+template <int TPR, int n>
+__device__ __forceinline__ void row_sums(float (&v)[n], float* room, int& turn) {
 #pragma unroll
-  for (int i = 0; i < THREADS / 32; ++i) v += room[i];
-  return v;
+  for (int o = (TPR < 32 ? TPR : 32) / 2; o; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < n; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+  if constexpr (TPR > 32) {
+    constexpr int WARPS = TPR / 32;
+    using Sums = Pack<float, n>;
+    Sums* mine = reinterpret_cast<Sums*>(room) + turn * (blockDim.x / 32);
+    turn ^= 1;
+    const int warp = threadIdx.x / 32, first = warp / WARPS * WARPS;
+    if ((threadIdx.x & 31) == 0) {
+      Sums own;
+#pragma unroll
+      for (int i = 0; i < n; ++i) own.v[i] = v[i];
+      mine[warp] = own;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < n; ++i) v[i] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const Sums other = mine[first + w];
+#pragma unroll
+      for (int i = 0; i < n; ++i) v[i] += other.v[i];
+    }
+  }
 }
 
-// A row to a CTA, read three times.
+// TPR threads take a row, NV pieces of V neighbouring places each, and ROWS rows at a time, to have enough loads in flight: a row
+// is read once and stays in registers, in its own type.  V = 8 where rows start on 16 bytes and C is a multiple of 8, else 1.
+// FWD_FIGURES
+template <typename T, typename W, int TPR, int NV, int V, int ROWS>
+__global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS, TPR > THREADS ? 1 : NV * V >= 64 ? 3 : 4)
+    forward_kernel(const T* __restrict__ x, int64_t ld, const W* __restrict__ w, const W* __restrict__ b, T* __restrict__ y, float* mean,
+                   float* rstd, int64_t R, int C, float eps) {
+  constexpr int N = TPR > THREADS ? TPR : THREADS, GROUPS = N / TPR;
+  __shared__ __align__(16) float room[2 * (TPR > 32 ? N / 32 : 1) * ROWS];
+  const int t = threadIdx.x % TPR;
+  const float over = 1.0f / C;
+  int turn = 0;
+  for (int64_t r0 = blockIdx.x * (int64_t)(GROUPS * ROWS); r0 < R; r0 += (int64_t)gridDim.x * (GROUPS * ROWS)) {
+    Piece<T, V> p[ROWS][NV];
+    float m[ROWS], s[ROWS];
+#pragma unroll
+    for (int j = 0; j < ROWS; ++j) {
+      const int64_t r = r0 + j * GROUPS + threadIdx.x / TPR;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int c = (k * TPR + t) * V;
+        if (r < R && c < C) p[j][k] = *reinterpret_cast<const Piece<T, V>*>(x + r * ld + c);
+        else p[j][k] = {};
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < ROWS; ++j) {
+      Floats<V> a = floats<T, V>(p[j][0]);
+#pragma unroll
+      for (int k = 1; k < NV; ++k) a = add<V>(a, floats<T, V>(p[j][k]));
+      s[j] = sum<V>(a);
+    }
+    row_sums<TPR>(s, room, turn);
+#pragma unroll
+    for (int j = 0; j < ROWS; ++j) {
+      m[j] = s[j] * over;
+      Floats<V> a = all<V>(0.0f);
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+        if ((k * TPR + t) * V < C) {
+          const Floats<V> d = add<V>(floats<T, V>(p[j][k]), all<V>(-m[j]));
+          a = fma<V>(d, d, a);
+        }
+      s[j] = sum<V>(a);
+    }
+    row_sums<TPR>(s, room, turn);
+#pragma unroll
+    for (int j = 0; j < ROWS; ++j) s[j] = 1.0f / sqrtf(s[j] * over + eps);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (k * TPR + t) * V;
+      if (c >= C) continue;
+      const Floats<V> wv = weights<V>(w + c), bv = weights<V>(b + c);
+#pragma unroll
+      for (int j = 0; j < ROWS; ++j) {
+        const int64_t r = r0 + j * GROUPS + threadIdx.x / TPR;
+        if (r >= R) continue;
+        const Floats<V> h = fma<V>(floats<T, V>(p[j][k]), all<V>(s[j]), all<V>(-m[j] * s[j]));
+        store<T, V>(y + r * C + c, fma<V>(h, wv, bv));
+      }
+    }
+    if (t == 0 && mean) {
+#pragma unroll
+      for (int j = 0; j < ROWS; ++j) {
+        const int64_t r = r0 + j * GROUPS + threadIdx.x / TPR;
+        if (r < R) mean[r] = m[j], rstd[r] = s[j];
+      }
+    }
+  }
+}
+
+// Rows too long for that: a CTA to a row, which is read three times.
 template <typename T, typename W>
-__global__ void __launch_bounds__(THREADS) forward_kernel(const T* __restrict__ x, int64_t ld, const W* __restrict__ w,
-                                                          const W* __restrict__ b, T* __restrict__ y, float* mean, float* rstd,
-                                                          int64_t R, int C, float eps) {
-  __shared__ float room[THREADS / 32];
+__global__ void __launch_bounds__(1024) long_forward_kernel(const T* __restrict__ x, int64_t ld, const W* __restrict__ w,
+                                                            const W* __restrict__ b, T* __restrict__ y, float* mean, float* rstd,
+                                                            int64_t R, int C, float eps) {
+  __shared__ __align__(16) float room[64];
+  const float over = 1.0f / C;
+  int turn = 0;
   for (int64_t r = blockIdx.x; r < R; r += gridDim.x) {
     const T* p = x + r * ld;
-    float s = 0.0f;
-    for (int c = threadIdx.x; c < C; c += THREADS) s += to_float(p[c]);
-    const float m = cta_sum(s, room) / C;
-    s = 0.0f;
-    for (int c = threadIdx.x; c < C; c += THREADS) {
+    float s[1] = {0.0f};
+    for (int c = threadIdx.x; c < C; c += 1024) s[0] += to_float(p[c]);
+    row_sums<1024>(s, room, turn);
+    const float m = s[0] * over;
+    s[0] = 0.0f;
+    for (int c = threadIdx.x; c < C; c += 1024) {
       const float d = to_float(p[c]) - m;
-      s = fmaf(d, d, s);
+      s[0] = fmaf(d, d, s[0]);
     }
-    const float k = 1.0f / sqrtf(cta_sum(s, room) / C + eps);
-    for (int c = threadIdx.x; c < C; c += THREADS)
+    row_sums<1024>(s, room, turn);
+    const float k = 1.0f / sqrtf(s[0] * over + eps);
+    for (int c = threadIdx.x; c < C; c += 1024)
       y[r * C + c] = from_float<T>(fmaf((to_float(p[c]) - m) * k, to_float(w[c]), to_float(b[c])));
     if (threadIdx.x == 0 && mean) mean[r] = m, rstd[r] = k;
   }
 }
 
+// The adjoint.  TPR threads take a row, NV pieces of V neighbouring places each.  A thread's places are the same in every row,
+// so it also gathers their sums of dy h and dy, which the CTA adds up at the end: part[CTA][0 and 1][C].  For V = 8 each
+// thread copies its own pieces of x and dy into shared memory DEPTH - 1 rows ahead (cp.async; no other thread reads them, so
+// that no barrier is needed): the registers that loads in flight would take leave room for more warps.
+// BWD_FIGURES
+template <typename T, typename W, int TPR, int NV, int V, int DEPTH>
+__global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS, TPR > THREADS ? 1 : NV > 1 ? 2 : 4)
+    backward_kernel(const T* __restrict__ dy, int64_t ldy, const T* __restrict__ x, int64_t ld, const float* __restrict__ mean,
+                    const float* __restrict__ rstd, const W* __restrict__ w, T* __restrict__ dx, float* __restrict__ part, int64_t R,
+                    int C) {
+  constexpr int N = TPR > THREADS ? TPR : THREADS, GROUPS = N / TPR;
+  using Piece = Piece<T, V>;
+  extern __shared__ __align__(16) char ring_bytes[];  // [DEPTH][2][NV][N] pieces, [DEPTH][2][N] mean and rstd; at the end the sums of the groups
+  Piece* const ring = reinterpret_cast<Piece*>(ring_bytes) + threadIdx.x;
+  float* const stats = reinterpret_cast<float*>(ring_bytes + DEPTH * 2 * NV * N * sizeof(Piece)) + threadIdx.x;
+  __shared__ __align__(16) float room[2 * (TPR > 32 ? N / 32 : 1) * 2];
+  const int t = threadIdx.x % TPR;
+  const float over = 1.0f / C;
+  const int64_t step = (int64_t)gridDim.x * GROUPS, first = blockIdx.x * (int64_t)GROUPS;
+  Piece ahead[V == 8 ? 1 : 2 * NV] = {};  // V = 1: cp.async takes 4 bytes at least
+  float ahead_mean = 0.0f, ahead_rstd = 0.0f;
+  auto fetch = [&](int64_t r0, int slot) {  // the pieces of a row
+    const int64_t r = r0 + threadIdx.x / TPR;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (k * TPR + t) * V;
+      if (r < R && c < C) {
+        Piece* const to = ring + (slot * 2 * NV + k) * N;
+        if constexpr (V == 8) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(x + r * ld + c) : "memory");
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to + NV * N)), "l"(dy + r * ldy + c)
+                       : "memory");
+        } else {
+          ahead[k] = *reinterpret_cast<const Piece*>(x + r * ld + c);
+          ahead[NV + k] = *reinterpret_cast<const Piece*>(dy + r * ldy + c);
+        }
+      }
+    }
+    if (r < R) {
+      float* const to = stats + slot * 2 * N;
+      if constexpr (V == 8) {
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(mean + r) : "memory");
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(to + N)), "l"(rstd + r) : "memory");
+      } else {
+        ahead_mean = __ldg(mean + r), ahead_rstd = __ldg(rstd + r);
+      }
+    }
+    if constexpr (V == 8) asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < DEPTH - 1; ++i) fetch(first + i * step, i);
+  Floats<V> dw[NV] = {}, db[NV] = {}, wv[NV] = {};
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+    if ((k * TPR + t) * V < C) wv[k] = weights<V>(w + (k * TPR + t) * V);
+  int turn = 0, slot = 0;
+  for (int64_t r0 = first; r0 < R; r0 += step) {
+    const int64_t r = r0 + threadIdx.x / TPR;
+    const bool there = r < R;
+    Piece now[V == 8 ? 1 : 2 * NV];
+    float k1 = ahead_rstd, m = ahead_mean;
+    if constexpr (V == 1) {
+#pragma unroll
+      for (int k = 0; k < 2 * NV; ++k) now[k] = ahead[k];
+    }
+    fetch(r0 + (DEPTH - 1) * step, slot == 0 ? DEPTH - 1 : slot - 1);
+    if constexpr (V == 8) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
+      m = stats[slot * 2 * N], k1 = stats[(slot * 2 + 1) * N];
+    }
+    if (!there) m = k1 = 0.0f;
+    const float off = -m * k1;  // h = k1 x + off
+    const Piece* const mine = ring + slot * 2 * NV * N;
+    auto of_x = [&](int k) { return floats<T, V>(V == 8 ? mine[k * N] : now[V == 8 ? 0 : k]); };
+    auto of_dy = [&](int k) { return floats<T, V>(V == 8 ? mine[(NV + k) * N] : now[V == 8 ? 0 : NV + k]); };
+    Floats<V> s0 = all<V>(0.0f), s1 = s0;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (there && (k * TPR + t) * V < C) {
+        const Floats<V> d = of_dy(k), h = fma<V>(of_x(k), all<V>(k1), all<V>(off));
+        const Floats<V> g = mul<V>(d, wv[k]);
+        s0 = add<V>(s0, g);
+        s1 = fma<V>(g, h, s1);
+        dw[k] = fma<V>(d, h, dw[k]);
+        db[k] = add<V>(db[k], d);
+      }
+    if (dx) {
+      float s[2] = {sum<V>(s0), sum<V>(s1)};
+      row_sums<TPR>(s, room, turn);
+      const float a = -k1 * s[0] * over, b = -k1 * s[1] * over;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int c = (k * TPR + t) * V;
+        if (!there || c >= C) continue;
+        const Floats<V> h = fma<V>(of_x(k), all<V>(k1), all<V>(off));
+        const Floats<V> g = mul<V>(of_dy(k), wv[k]);
+        store<T, V>(dx + r * C + c, fma<V>(g, all<V>(k1), fma<V>(h, all<V>(b), all<V>(a))));
+      }
+    }
+    slot = slot == DEPTH - 1 ? 0 : slot + 1;
+  }
+  if (!part) return;
+  float* const to = part + blockIdx.x * (int64_t)2 * C;
+  float* const gathered = reinterpret_cast<float*>(ring_bytes);
+  if constexpr (V == 8) asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if constexpr (GROUPS > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int e = 0; e < V; ++e) gathered[(threadIdx.x / TPR * NV + k) * TPR * V + t * V + e] = i ? db[k].v[e] : dw[k].v[e];
+      __syncthreads();
+      for (int c = threadIdx.x; c < C; c += N) {
+        float v = 0.0f;
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) v += gathered[g * NV * TPR * V + c];
+        to[i * C + c] = v;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if ((k * TPR + t) * V + e < C) to[i * C + (k * TPR + t) * V + e] = i ? db[k].v[e] : dw[k].v[e];
+    }
+  }
+}
+
 template <typename T, typename W>
-__global__ void __launch_bounds__(THREADS) backward_kernel(const T* __restrict__ dy, int64_t ldy, const T* __restrict__ x,
-                                                           int64_t ld, const float* __restrict__ mean,
-                                                           const float* __restrict__ rstd, const W* __restrict__ w,
-                                                           T* __restrict__ dx, int64_t R, int C) {
-  __shared__ float room[THREADS / 32];
+__global__ void __launch_bounds__(1024) long_backward_kernel(const T* __restrict__ dy, int64_t ldy, const T* __restrict__ x, int64_t ld,
+                                                             const float* __restrict__ mean, const float* __restrict__ rstd,
+                                                             const W* __restrict__ w, T* __restrict__ dx, int64_t R, int C) {
+  __shared__ __align__(16) float room[128];
+  const float over = 1.0f / C;
+  int turn = 0;
   for (int64_t r = blockIdx.x; r < R; r += gridDim.x) {
     const T *p = x + r * ld, *q = dy + r * ldy;
     const float m = mean[r], k = rstd[r];
-    float s = 0.0f, t = 0.0f;
-    for (int c = threadIdx.x; c < C; c += THREADS) {
+    float s[2] = {0.0f, 0.0f};
+    for (int c = threadIdx.x; c < C; c += 1024) {
       const float g = to_float(q[c]) * to_float(w[c]);
-      s += g;
-      t = fmaf(g, (to_float(p[c]) - m) * k, t);
+      s[0] += g;
+      s[1] = fmaf(g, (to_float(p[c]) - m) * k, s[1]);
     }
-    s = cta_sum(s, room) / C;
-    t = cta_sum(t, room) / C;
-    for (int c = threadIdx.x; c < C; c += THREADS) {
-      const float h = (to_float(p[c]) - m) * k;
-      dx[r * C + c] = from_float<T>(k * (to_float(q[c]) * to_float(w[c]) - s - h * t));
-    }
+    row_sums<1024>(s, room, turn);
+    const float a = s[0] * over, b = s[1] * over;
+    for (int c = threadIdx.x; c < C; c += 1024)
+      dx[r * C + c] = from_float<T>(k * (fmaf(to_float(q[c]), to_float(w[c]), -a) - (to_float(p[c]) - m) * k * b));
   }
 }
 
 // part[i][0 and 1][C]: the sums of dy h and dy over the rows i, i + gridDim.y, ...
 template <typename T>
-__global__ void __launch_bounds__(THREADS) weights_kernel(const T* __restrict__ dy, int64_t ldy, const T* __restrict__ x,
-                                                          int64_t ld, const float* __restrict__ mean,
-                                                          const float* __restrict__ rstd, float* part, int64_t R, int C) {
+__global__ void __launch_bounds__(THREADS) long_weights_kernel(const T* __restrict__ dy, int64_t ldy, const T* __restrict__ x,
+                                                               int64_t ld, const float* __restrict__ mean,
+                                                               const float* __restrict__ rstd, float* part, int64_t R, int C) {
   const int c = blockIdx.x * THREADS + threadIdx.x;
   if (c >= C) return;
   float s = 0.0f, t = 0.0f;
@@ -107,20 +431,30 @@ __global__ void __launch_bounds__(THREADS) weights_kernel(const T* __restrict__ 
   part[((int64_t)blockIdx.y * 2 + 1) * C + c] = t;
 }
 
+// The sums over the n parts: 32 columns of dw, then of db, to a CTA, its warps taking parts in turn, in a fixed order.
 template <typename W>
-__global__ void __launch_bounds__(THREADS) finish_kernel(const float* __restrict__ part, int n, int C, W* dw, W* db) {
-  const int c = blockIdx.x * THREADS + threadIdx.x;
-  if (c >= C) return;
-  float s = 0.0f, t = 0.0f;
-  for (int i = 0; i < n; ++i) {
-    s += part[(int64_t)i * 2 * C + c];
-    t += part[((int64_t)i * 2 + 1) * C + c];
+__global__ void __launch_bounds__(512) finish_kernel(const float* __restrict__ part, int n, int C, W* dw, W* db) {
+  __shared__ float sums[16][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+  const int64_t c = blockIdx.x * (int64_t)32 + lane;
+  float s = 0.0f;
+  if (c < 2 * (int64_t)C) {
+#pragma unroll 8
+    for (int i = warp; i < n; i += 16) s += __ldg(part + (int64_t)i * 2 * C + c);
   }
-  if (dw) dw[c] = from_float<W>(s);
-  if (db) db[c] = from_float<W>(t);
+  sums[warp][lane] = s;
+  __syncthreads();
+  if (warp == 0 && c < 2 * (int64_t)C) {
+    s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) s += sums[w][lane];
+    W* to = c < C ? dw : db;
+    if (to) to[c < C ? c : c - C] = from_float<W>(s);
+  }
 }
 
-int parts(int64_t R) { return (int)std::min<int64_t>(std::max<int64_t>(R, 1), 148 * 2); }
+// CTAs of the backward pass at most, and so partial sums of the weights' gradients
+int parts(int64_t R, int64_t C) { return (int)std::min<int64_t>(std::max<int64_t>(R, 1), C > 8192 ? 148 : 148 * 4); }
 bool aligned(const void* p, int n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 int check_rows(int64_t R, int64_t C, int dtype, int wtype) {
@@ -140,23 +474,117 @@ struct Back {
   int C;
 };
 template <typename T, typename W>
+struct Front {
+  const T* x;
+  int64_t ld;
+  const W *w, *b;
+  T* y;
+  float *mean, *rstd;
+  int64_t R;
+  int C;
+  float eps;
+  cudaStream_t st;
+
+  template <int TPR, int NV, int V>
+  void run() const {
+    constexpr int N = TPR > THREADS ? TPR : THREADS, ROWS = TPR > THREADS ? 2 : NV * V >= 32 ? 1 : NV * V >= 16 ? 2 : 4;
+    const int64_t ctas = (R + N / TPR * ROWS - 1) / (N / TPR * ROWS);
+    forward_kernel<T, W, TPR, NV, V, ROWS><<<(unsigned)std::min<int64_t>(ctas, 148 * 16), N, 0, st>>>(x, ld, w, b, y, mean, rstd, R, C, eps);
+  }
+  // A warp takes rows of up to 2048 places: it needs no barrier.
+  void lay_out(bool vec) const {
+    const int n = C / 8;
+    if (!vec) narrow();
+    else if (n <= 8) run<8, 1, 8>();
+    else if (n <= 16) run<16, 1, 8>();
+    else if (n <= 32) run<32, 1, 8>();
+    else if (n <= 64) run<32, 2, 8>();
+    else if (n <= 128) run<32, 4, 8>();
+    else if (n <= 256) run<32, 8, 8>();
+    else if (n <= 512) run<256, 2, 8>();
+    else if (n <= 1024) run<256, 4, 8>();
+    else if (n <= 2048) run<512, 4, 8>();
+    else run_long();
+  }
+  void narrow() const {
+    if (C <= 32) run<32, 1, 1>();
+    else if (C <= 128) run<32, 4, 1>();
+    else if (C <= 512) run<32, 16, 1>();
+    else if (C <= 1024) run<32, 32, 1>();
+    else if (C <= 4096) run<256, 16, 1>();
+    else if (C <= 8192) run<512, 16, 1>();
+    else run_long();
+  }
+  void run_long() const {
+    long_forward_kernel<T, W><<<(unsigned)std::min<int64_t>(R, 148 * 4), 1024, 0, st>>>(x, ld, w, b, y, mean, rstd, R, C, eps);
+  }
+};
+template <typename T, typename W>
+struct BackOf : Back {
+  cudaStream_t st;
+  template <int TPR, int NV, int V>
+  void run() const {
+    constexpr int N = TPR > THREADS ? TPR : THREADS, GROUPS = N / TPR, DEPTH = V == 8 ? (NV > 2 ? 3 : NV > 1 ? 5 : 6) : 2;
+    constexpr int ring = V == 8 ? DEPTH * (2 * NV * N * V * 2 + 2 * N * 4) : 0, sums = GROUPS > 1 ? N * NV * V * 4 : 0, smem = ring > sums ? ring : sums;
+    constexpr auto kernel = backward_kernel<T, W, TPR, NV, V, DEPTH>;
+    if (smem > 32 * 1024 && allow_smem<kernel>(smem) != cudaSuccess) return;  // its error is found after the call
+    // as many CTAs as the SMs hold at a time
+    const int n = (int)std::min<int64_t>(std::max<int64_t>((R + GROUPS - 1) / GROUPS, 1), 148 * (TPR > THREADS ? 1 : NV > 1 ? 2 : 4));
+    kernel<<<n, N, smem, st>>>(static_cast<const T*>(dy), ldy, static_cast<const T*>(x), ld, mean, rstd, static_cast<const W*>(w),
+                               static_cast<T*>(dx), dw || db ? part : nullptr, R, C);
+    finish(n);
+  }
+  // What a thread has of a row grows only where a CTA's threads do not reach: it keeps two sums for each of its places.
+  void lay_out(bool vec) const {
+    const int n = C / 8;
+    if (!vec) narrow();
+    else if (n <= 8) run<8, 1, 8>();
+    else if (n <= 16) run<8, 2, 8>();
+    else if (n <= 32) run<16, 2, 8>();
+    else if (n <= 64) run<32, 2, 8>();
+    else if (n <= 128) run<64, 2, 8>();
+    else if (n <= 256) run<128, 2, 8>();
+    else if (n <= 512) run<256, 2, 8>();
+    else if (n <= 1024) run<512, 2, 8>();
+    else if (n <= 2048) run<512, 4, 8>();
+    else run_long();
+  }
+  void narrow() const {
+    if (C <= 32) run<32, 1, 1>();
+    else if (C <= 128) run<32, 4, 1>();
+    else if (C <= 512) run<128, 4, 1>();
+    else if (C <= 1024) run<256, 4, 1>();
+    else if (C <= 4096) run<512, 8, 1>();
+    else if (C <= 8192) run<512, 16, 1>();
+    else run_long();
+  }
+  void run_long() const {
+    if (R && dx)
+      long_backward_kernel<T, W><<<(unsigned)std::min<int64_t>(R, 148 * 4), 1024, 0, st>>>(
+          static_cast<const T*>(dy), ldy, static_cast<const T*>(x), ld, mean, rstd, static_cast<const W*>(w), static_cast<T*>(dx), R, C);
+    const int n = (int)std::min<int64_t>(std::max<int64_t>(R, 1), parts(R, C));
+    if (dw || db)
+      long_weights_kernel<T><<<dim3((unsigned)((C + THREADS - 1) / THREADS), (unsigned)n), THREADS, 0, st>>>(
+          static_cast<const T*>(dy), ldy, static_cast<const T*>(x), ld, mean, rstd, part, R, C);
+    finish(n);
+  }
+  void finish(int n) const {
+    if (dw || db) finish_kernel<W><<<(unsigned)((2 * (int64_t)C + 31) / 32), 512, 0, st>>>(part, n, C, static_cast<W*>(dw), static_cast<W*>(db));
+  }
+};
+
+bool eights(const void* p, int64_t ld, int64_t R, int C) { return C % 8 == 0 && aligned(p, 16) && (R <= 1 || ld % 8 == 0); }
+
+template <typename T, typename W>
 void backward(const Back& A, cudaStream_t st) {
-  const unsigned grid = (unsigned)std::min<int64_t>(A.R, 148 * 8);
-  const T *dy = static_cast<const T*>(A.dy), *x = static_cast<const T*>(A.x);
-  if (A.R && A.dx)
-    backward_kernel<T, W><<<grid, THREADS, 0, st>>>(dy, A.ldy, x, A.ld, A.mean, A.rstd, static_cast<const W*>(A.w), static_cast<T*>(A.dx), A.R, A.C);
-  if (!A.dw && !A.db) return;
-  const int n = parts(A.R);
-  const unsigned tiles = (unsigned)((A.C + THREADS - 1) / THREADS);
-  weights_kernel<T><<<dim3(tiles, (unsigned)n), THREADS, 0, st>>>(dy, A.ldy, x, A.ld, A.mean, A.rstd, A.part, A.R, A.C);
-  finish_kernel<W><<<tiles, THREADS, 0, st>>>(A.part, n, A.C, static_cast<W*>(A.dw), static_cast<W*>(A.db));
+  const BackOf<T, W> f = {A, st};
+  f.lay_out(eights(A.dy, A.ldy, A.R, A.C) && eights(A.x, A.ld, A.R, A.C) && aligned(A.w, 16));
 }
 template <typename T, typename W>
 void forward(const void* x, int64_t ld, const void* w, const void* b, void* y, float* mean, float* rstd, int64_t R, int C, float eps,
              cudaStream_t st) {
-  const unsigned grid = (unsigned)std::min<int64_t>(R, 148 * 8);
-  forward_kernel<T, W><<<grid, THREADS, 0, st>>>(static_cast<const T*>(x), ld, static_cast<const W*>(w), static_cast<const W*>(b),
-                                                 static_cast<T*>(y), mean, rstd, R, C, eps);
+  const Front<T, W> f = {static_cast<const T*>(x), ld, static_cast<const W*>(w), static_cast<const W*>(b), static_cast<T*>(y), mean, rstd, R, C, eps, st};
+  f.lay_out(eights(x, ld, R, C) && aligned(w, 16) && aligned(b, 16));
 }
 
 }  // namespace
@@ -181,7 +609,7 @@ extern "C" int csn_layer_norm_rows_fwd(const void* x, int64_t ldx, const void* w
 
 extern "C" size_t csn_layer_norm_rows_bwd_workspace_bytes(int64_t R, int64_t C) {
   if (R < 0 || C < 1) return 0;
-  return (size_t)parts(R) * 2 * (size_t)C * sizeof(float);
+  return (size_t)parts(R, C) * 2 * (size_t)C * sizeof(float);
 }
 
 extern "C" int csn_layer_norm_rows_bwd(const void* dy, int64_t ldy, const void* x, int64_t ldx, const float* mean, const float* rstd,
