@@ -10,90 +10,140 @@ namespace {
 using namespace la;
 
 constexpr int MAX_D = 128;
-constexpr int BLOCK = 16;        // steps that are worked on together
-constexpr int LINE = BLOCK + 4;  // of shared memory: aligned, and a column of values is spread over the banks
+constexpr int BLOCK = 16;  // steps that are worked on together
 
 // n steps from X, in their order of processing (BACK: time runs down; X carried is Y, after its fade):
 //   out_i = so (l^(i+1) X^T a_i + sum over j <= i of l^(i-j) sb (a_i . b_j) v_j),   X <- l^n X + sum of l^(n-1-j) sb b_j v_j^T
 // (one power of l less before the first product and one more in the last sum where time runs down).  A thread has one
-// place of v and the K entries of the state beside it in registers: two FMA an entry and step, the products a . b shared by
-// all threads.  The state is rounded once a block: step by step, a memory of thousands of steps costs it a digit.
+// place of v and the K entries of the state beside it in registers: one packed pair of FMA an entry and step for each of the two
+// products, the products a . b shared by all threads.  The state is rounded once a block: step by step, a memory of
+// thousands of steps costs it a digit.
+// float32 rows come DEPTH - 1 blocks ahead by cp.async, 16 bytes at a time where they are aligned (WIDE); other types are
+// converted on their way.  Bound by the loads of a and b from shared memory, which every thread needs.
 // OUT: false for the first pass.
+constexpr int MAX_PASSES = 3;
+struct Passes {
+  Pass pass[MAX_PASSES];
+};
+__host__ __device__ constexpr int depth(int size) { return size == 4 ? 3 : 1; }
+__host__ __device__ constexpr int line(int places) { return places + 4; }  // aligned, and rows spread over the banks
+__host__ __device__ constexpr int stage_floats(int kp, int vp, bool out) { return BLOCK * ((out ? 2 : 1) * line(kp) + line(vp)); }
+
+__device__ __forceinline__ void copy_async(float* to, const float* from, bool wide) {
+  const uint32_t at = (uint32_t)__cvta_generic_to_shared(to);
+  if (wide) asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(at), "l"(from) : "memory");
+}
+
 template <typename T, int KP, int VP, bool OUT>
-__global__ void __launch_bounds__(VP) blocks_kernel(const Batch B, const Pass P) {
+__global__ void __launch_bounds__(VP) blocks_kernel(const Batch B, const __grid_constant__ Passes passes, bool wide) {
+  const Pass& P = passes.pass[blockIdx.z];
   const Unit U(B, blockIdx.x);
   if (U.s < 0 || (!OUT && U.ends(P.back))) return;
-  constexpr int NJ = BLOCK * BLOCK / VP;  // products of a thread
+  constexpr int NJ = BLOCK * BLOCK / VP, DEPTH = depth(sizeof(T)), LK = line(KP), LV = line(VP), STAGE = stage_floats(KP, VP, OUT);
   const int h = blockIdx.y, c = threadIdx.x, late = P.back ? 1 : 0;
   const bool mine = c < P.V;
-  __shared__ __align__(16) float as[OUT ? KP : 1][LINE], bs[KP][LINE], prod[OUT ? BLOCK : 1][LINE];
+  extern __shared__ __align__(16) float stages[];  // [DEPTH][b, v, a][BLOCK][places]
+  __shared__ __align__(16) float prod[OUT ? BLOCK : 1][BLOCK + 4];
   __shared__ float power[BLOCK + 2];
   if (c < BLOCK + 2) power[c] = fade(B.log_decay[h], c);
+  for (int i = c; i < DEPTH * STAGE; i += VP) stages[i] = 0.0f;
   const int64_t size = (int64_t)P.K * P.V;
-  float x[KP];
+  float2 x[KP / 2];
 #pragma unroll
-  for (int i = 0; i < KP; ++i) x[i] = 0.0f;
+  for (int i = 0; i < KP / 2; ++i) x[i] = make_float2(0.0f, 0.0f);
   if (OUT && P.state && mine) {
     const float* p = P.state + ((P.by_unit ? U.unit : U.s) * B.H + h) * size + c * P.sc;
 #pragma unroll
-    for (int i = 0; i < KP; ++i)
-      if (i < P.K) x[i] = p[i * P.sr];
+    for (int i = 0; i < KP / 2; ++i) {
+      if (2 * i < P.K) x[i].x = p[2 * i * P.sr];
+      if (2 * i + 1 < P.K) x[i].y = p[(2 * i + 1) * P.sr];
+    }
   }
   const T* a = static_cast<const T*>(P.a.p) + U.start(B, P.a) + h / P.a.shared * P.a.head;
   const T* b = static_cast<const T*>(P.b.p) + U.start(B, P.b) + h / P.b.shared * P.b.head;
   const T* v = static_cast<const T*>(P.v.p) + U.start(B, P.v) + h / P.v.shared * P.v.head;
-  for (int i = c; i < KP * LINE; i += VP) {
-    if (OUT) as[OUT ? i / LINE : 0][i % LINE] = 0.0f;
-    bs[i / LINE][i % LINE] = 0.0f;
-  }
   const int steps = U.to - U.from;
+  // the rows of a block, in their order of processing; what lies behind the last is left as it is
+  auto fetch = [&](int done) {
+    const int n = min(BLOCK, steps - done);
+    float* const to = stages + done / BLOCK % DEPTH * STAGE;
+    auto rows = [&](const T* from, int64_t pitch, int places, int l, float* at) {
+      const int w = sizeof(T) == 4 && wide ? 4 : 1, pieces = (places + w - 1) / w;
+      for (int i = c; i < n * pieces; i += VP) {
+        const int r = i / pieces, d = (i - r * pieces) * w;
+        const T* p = from + (P.back ? U.to - 1 - done - r : U.from + done + r) * pitch + d;
+        if constexpr (sizeof(T) == 4) copy_async(at + r * l + d, reinterpret_cast<const float*>(p), w == 4);
+        else at[r * l + d] = to_float(*p);
+      }
+    };
+    if (n > 0) {
+      rows(b, P.b.row, P.K, LK, to);
+      rows(v, P.v.row, P.V, LV, to + BLOCK * LK);
+      if (OUT) rows(a, P.a.row, P.K, LK, to + BLOCK * (LK + LV));
+    }
+    if constexpr (sizeof(T) == 4) asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  __syncthreads();
+  for (int i = 0; i < DEPTH - 1; ++i) fetch(i * BLOCK);
   for (int done = 0; done < steps; done += BLOCK) {
     const int n = min(BLOCK, steps - done);
+    if (DEPTH == 1) {
+      __syncthreads();  // the block before has been read
+      fetch(done);
+    } else {
+      asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH > 1 ? DEPTH - 2 : 0) : "memory");
+    }
     __syncthreads();
+    if (DEPTH > 1) fetch(done + (DEPTH - 1) * BLOCK);  // over the block before, which every thread is done with
+    const float* const bs = stages + done / BLOCK % DEPTH * STAGE;
+    const float *const vb = bs + BLOCK * LK, *const as = bs + BLOCK * (LK + LV);
+    if (OUT) {
+      const int i = c % BLOCK, j0 = c / BLOCK * NJ;
+      float2 r[NJ];
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) r[j] = make_float2(0.0f, 0.0f);
+#pragma unroll 4
+      for (int d = 0; d < KP; d += 4) {
+        const float4 a4 = *reinterpret_cast<const float4*>(as + i * LK + d);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          const float4 b4 = *reinterpret_cast<const float4*>(bs + (j0 + j) * LK + d);
+          r[j] = fma2(make_float2(a4.x, a4.y), make_float2(b4.x, b4.y), r[j]);
+          r[j] = fma2(make_float2(a4.z, a4.w), make_float2(b4.z, b4.w), r[j]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) prod[OUT ? i : 0][j0 + j] = j0 + j <= i ? (r[j].x + r[j].y) * power[i - j0 - j] : 0.0f;
+    }
+    float2 o[OUT ? BLOCK : 1];
     float vs[BLOCK];
 #pragma unroll
     for (int i = 0; i < BLOCK; ++i) {
-      const bool in = i < n;
-      const int64_t t = P.back ? U.to - 1 - done - i : U.from + done + i;
-      vs[i] = in && mine ? to_float(v[t * P.v.row + c]) * P.sb : 0.0f;
-      for (int d = c; d < P.K; d += VP) {
-        if (OUT) as[OUT ? d : 0][i] = in ? to_float(a[t * P.a.row + d]) : 0.0f;
-        bs[d][i] = in ? to_float(b[t * P.b.row + d]) : 0.0f;
-      }
+      vs[i] = i < n && mine ? vb[i * LV + c] * P.sb : 0.0f;
+      if (OUT) o[OUT ? i : 0] = make_float2(0.0f, 0.0f);
     }
-    __syncthreads();
-    if (OUT) {
-      const int i = c % BLOCK, j0 = c / BLOCK * NJ;
-      float r[NJ] = {};
-#pragma unroll 8
-      for (int d = 0; d < KP; ++d) {
-        const float ai = as[OUT ? d : 0][i];
-        const Pack<float, NJ> bj = *reinterpret_cast<const Pack<float, NJ>*>(&bs[d][j0]);
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) r[j] = fmaf(ai, bj.v[j], r[j]);
-      }
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) prod[OUT ? i : 0][j0 + j] = j0 + j <= i ? r[j] * power[i - j0 - j] : 0.0f;
-    }
-    float o[BLOCK] = {}, w[BLOCK];
+    const float whole = power[n];
+    // what rows behind the last hold does not count
+    float w[BLOCK];
 #pragma unroll
     for (int i = 0; i < BLOCK; ++i) w[i] = i < n ? vs[i] * power[n - 1 - i + late] : 0.0f;
-    const float whole = power[n];
 #pragma unroll
-    for (int d = 0; d < KP; ++d) {
-      float t = 0.0f;
+    for (int d = 0; d < KP; d += 4) {
+      float2 t0 = make_float2(0.0f, 0.0f), t1 = t0;
 #pragma unroll
-      for (int i = 0; i < BLOCK; i += 4) {
-        const float4 b4 = *reinterpret_cast<const float4*>(&bs[d][i]);
+      for (int i = 0; i < BLOCK; ++i) {
+        const float4 b4 = *reinterpret_cast<const float4*>(bs + i * LK + d);
+        t0 = fma2(make_float2(b4.x, b4.y), twice(w[i]), t0);
+        t1 = fma2(make_float2(b4.z, b4.w), twice(w[i]), t1);
         if (OUT) {
-          const float4 a4 = *reinterpret_cast<const float4*>(&as[OUT ? d : 0][i]);
-          o[i] = fmaf(a4.x, x[d], o[i]), o[i + 1] = fmaf(a4.y, x[d], o[i + 1]);
-          o[i + 2] = fmaf(a4.z, x[d], o[i + 2]), o[i + 3] = fmaf(a4.w, x[d], o[i + 3]);
+          const float4 a4 = *reinterpret_cast<const float4*>(as + i * LK + d);
+          o[OUT ? i : 0] = fma2(make_float2(a4.x, a4.y), x[d / 2], o[OUT ? i : 0]);
+          o[OUT ? i : 0] = fma2(make_float2(a4.z, a4.w), x[d / 2 + 1], o[OUT ? i : 0]);
         }
-        t = fmaf(b4.x, w[i], t), t = fmaf(b4.y, w[i + 1], t);
-        t = fmaf(b4.z, w[i + 2], t), t = fmaf(b4.w, w[i + 3], t);
       }
-      x[d] = fmaf(whole, x[d], t);
+      x[d / 2] = fma2(twice(whole), x[d / 2], t0);
+      x[d / 2 + 1] = fma2(twice(whole), x[d / 2 + 1], t1);
     }
     if (!OUT) continue;
     __syncthreads();
@@ -109,17 +159,20 @@ __global__ void __launch_bounds__(VP) blocks_kernel(const Batch B, const Pass P)
           if (j + e <= i) r = fmaf(pv[e], vs[j + e], r);  // a later step's infinity has to stay out
       }
       if (i >= n || !mine) continue;
-      r = fmaf(power[i + 1 - late], o[i], r) * P.so;
+      r = fmaf(power[i + 1 - late], o[OUT ? i : 0].x + o[OUT ? i : 0].y, r) * P.so;
       const int64_t t = U.row0 + (P.back ? U.to - 1 - done - i : U.from + done + i), at = (t * B.H + h) * P.V + c;
       if (P.wide) static_cast<float*>(P.out)[at] = r;
       else static_cast<T*>(P.out)[at] = from_float<T>(r);
     }
   }
+  if constexpr (sizeof(T) == 4) asm volatile("cp.async.wait_all;" ::: "memory");
   float* to = OUT ? (P.last && U.ends(P.back) ? P.last + (U.s * B.H + h) * size : nullptr) : P.made + (U.unit * B.H + h) * size;
   if (to && mine) {
 #pragma unroll
-    for (int i = 0; i < KP; ++i)
-      if (i < P.K) to[i * P.sr + c * P.sc] = x[i];
+    for (int i = 0; i < KP / 2; ++i) {
+      if (2 * i < P.K) to[2 * i * P.sr + c * P.sc] = x[i].x;
+      if (2 * i + 1 < P.K) to[(2 * i + 1) * P.sr + c * P.sc] = x[i].y;
+    }
   }
 }
 
@@ -257,7 +310,7 @@ void cut(Batch& B, int Dk, int Dv, int passes, bool packed, bool half) {
       if (cost < least) least = cost, best = n;
     }
   } else {
-    best = std::min(rows, up(148 * 12, heads * up(std::min(Dk, Dv), 32)));
+    best = std::min(rows, up(148 * 12, heads * passes * up(std::min(Dk, Dv), 32)));
   }
   B.seg = (int)(std::max(up(rows, std::max(best, (int64_t)1)), (int64_t)1) * 128);
   B.segs = packed ? 0 : (int)std::max(up(B.T, B.seg), (int64_t)1);
@@ -282,23 +335,25 @@ Room room(const Batch& B, int Hk, int Dk, int Dv, bool packed, bool backward) {
           shared ? up(rows * B.H * Dv, 4) * 4 : 0};
 }
 
-template <typename T, int KP, int VP>
-void launch_blocks(const Batch& B, const Pass& P, bool first, cudaStream_t st) {
-  const dim3 grid((unsigned)B.units, (unsigned)B.H);
-  if (first) blocks_kernel<T, KP, VP, false><<<grid, VP, 0, st>>>(B, P);
-  else blocks_kernel<T, KP, VP, true><<<grid, VP, 0, st>>>(B, P);
+template <typename T, int KP, int VP, bool OUT>
+cudaError_t launch_blocks(const Batch& B, const Passes& P, int count, bool wide, cudaStream_t st) {
+  constexpr int smem = depth(sizeof(T)) * stage_floats(KP, VP, OUT) * 4;
+  if (smem > 32 * 1024)
+    if (cudaError_t e = allow_smem<blocks_kernel<T, KP, VP, OUT>>(smem)) return e;
+  blocks_kernel<T, KP, VP, OUT><<<dim3((unsigned)B.units, (unsigned)B.H, (unsigned)count), VP, smem, st>>>(B, P, wide);
+  return cudaSuccess;
 }
 template <typename T, int KP>
-void launch_blocks(const Batch& B, const Pass& P, bool first, cudaStream_t st) {
-  if (P.V <= 32) launch_blocks<T, KP, 32>(B, P, first, st);
-  else if (P.V <= 64) launch_blocks<T, KP, 64>(B, P, first, st);
-  else launch_blocks<T, KP, 128>(B, P, first, st);
+cudaError_t launch_blocks(const Batch& B, const Passes& P, int count, int V, bool first, bool wide, cudaStream_t st) {
+  if (V <= 32) return first ? launch_blocks<T, KP, 32, false>(B, P, count, wide, st) : launch_blocks<T, KP, 32, true>(B, P, count, wide, st);
+  if (V <= 64) return first ? launch_blocks<T, KP, 64, false>(B, P, count, wide, st) : launch_blocks<T, KP, 64, true>(B, P, count, wide, st);
+  return first ? launch_blocks<T, KP, 128, false>(B, P, count, wide, st) : launch_blocks<T, KP, 128, true>(B, P, count, wide, st);
 }
 template <typename T>
-void launch_blocks(const Batch& B, const Pass& P, bool first, cudaStream_t st) {
-  if (P.K <= 32) launch_blocks<T, 32>(B, P, first, st);
-  else if (P.K <= 64) launch_blocks<T, 64>(B, P, first, st);
-  else launch_blocks<T, 128>(B, P, first, st);
+cudaError_t launch_blocks(const Batch& B, const Passes& P, int count, int K, int V, bool first, bool wide, cudaStream_t st) {
+  if (K <= 32) return launch_blocks<T, 32>(B, P, count, V, first, wide, st);
+  if (K <= 64) return launch_blocks<T, 64>(B, P, count, V, first, wide, st);
+  return launch_blocks<T, 128>(B, P, count, V, first, wide, st);
 }
 
 int run(const Batch& B, const Pass* passes, int count, bool first, int dtype, cudaStream_t st) {
@@ -306,11 +361,28 @@ int run(const Batch& B, const Pass* passes, int count, bool first, int dtype, cu
   for (int i = 0; i < count; ++i)
     tensor = tensor && fits_tensor(B, passes[i].a, passes[i].K) && fits_tensor(B, passes[i].b, passes[i].K) && fits_tensor(B, passes[i].v, passes[i].V);
   if (tensor) return tensor_passes(B, passes, count, first, dtype == CSN_BF16, st);
-  for (int i = 0; i < count; ++i) {
+  auto wide = [](const Stream& x, int places) {
+    return places % 4 == 0 && aligned(x.p, 16) && x.seq % 4 == 0 && x.row % 4 == 0 && x.head % 4 == 0;
+  };
+  bool done[MAX_PASSES] = {};
+  for (int i = 0; i < count; ++i) {  // passes of the same sizes run side by side in one launch
+    if (done[i]) continue;
+    Passes P;
+    int n = 0;
+    bool all_wide = dtype == CSN_F32;
+    for (int j = i; j < count; ++j) {
+      const Pass& p = passes[j];
+      if (done[j] || p.K != passes[i].K || p.V != passes[i].V) continue;
+      done[j] = true;
+      P.pass[n++] = p;
+      all_wide = all_wide && wide(p.a, p.K) && wide(p.b, p.K) && wide(p.v, p.V);
+    }
     KernelTimer kt(first ? "linear_attention_first" : "linear_attention", st);
-    if (dtype == CSN_F32) launch_blocks<float>(B, passes[i], first, st);
-    else if (dtype == CSN_BF16) launch_blocks<__nv_bfloat16>(B, passes[i], first, st);
-    else launch_blocks<__half>(B, passes[i], first, st);
+    const int K = passes[i].K, V = passes[i].V;
+    const cudaError_t e = dtype == CSN_F32    ? launch_blocks<float>(B, P, n, K, V, first, all_wide, st)
+                          : dtype == CSN_BF16 ? launch_blocks<__nv_bfloat16>(B, P, n, K, V, first, false, st)
+                                              : launch_blocks<__half>(B, P, n, K, V, first, false, st);
+    if (e != cudaSuccess) return set_cuda_error(e, "csn_linear_attention: shared memory");
   }
   return CSN_OK;
 }
