@@ -101,7 +101,8 @@ SIGNATURES = {
     "csn_silu_gated_linear_fwd": ([_f, _i64, _f, _i64, _f, _i64, _f, _f, _i64, _i64, _i64, _int, _f, _sz, _f], _int),
     "csn_silu_gated_linear_bwd": ([_f, _i64, _f, _i64, _f, _i64, _f, _i64, _f, _f, _f, _f, _i64, _i64, _i64, _int, _f,
                                    _sz, _f], _int),
-    "csn_linear_attention_workspace_bytes": ([_i64] * 6 + [_int, _int, _int], _sz),
+    "csn_linear_attention_copies": ([_f, _f, _f, _f, _strides] + [_i64] * 6 + [_int, _int], _int),
+    "csn_linear_attention_workspace_bytes": ([_i64] * 6 + [_int, _int, _int, _int], _sz),
     "csn_linear_attention_fwd": ([_f, _f, _f, _strides, _f, _f, _f, _f, _f] + [_i64] * 6 + [ctypes.c_float, _int, _f, _sz, _f], _int),
     "csn_linear_attention_bwd": ([_f, _f, _f, _f, _strides] + [_f] * 8 + [_i64] * 6 + [ctypes.c_float, _int, _f, _sz, _f], _int),
     "csn_linear_attention_step": ([_f, _f, _f, _strides, _f, _f, _f] + [_i64] * 5 + [ctypes.c_float, _int, _f], _int),

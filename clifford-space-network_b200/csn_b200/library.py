@@ -385,6 +385,64 @@ def _dropout_backward(ctx, dy):
 dropout_add.register_autograd(_dropout_backward, setup_context=_dropout_setup)
 
 
+# ------------------------------------------------------------ linear attention
+def _state_shape(q, v, cu):
+    return ((q.shape[0] if cu is None else cu.shape[0] - 1), q.shape[-2], q.shape[-1], v.shape[-1])
+
+
+@torch.library.custom_op("csn::linear_attention_fwd", mutates_args=())
+def linear_attention_fwd(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, s0: Optional[Tensor],
+                         cu_seqlens: Optional[Tensor], scale: Optional[float]) -> Tuple[Tensor, Tensor]:
+    ext = gated._ext()
+    ext.linear_attention_check(q, k, v, log_decay.detach(), s0, cu_seqlens)
+    return ext.linear_attention_forward(q, k, v, log_decay, None if s0 is None else s0.float(), cu_seqlens, scale)
+
+
+@linear_attention_fwd.register_fake
+def _(q, k, v, log_decay, s0, cu_seqlens, scale):
+    return q.new_empty((*q.shape[:-1], v.shape[-1])), q.new_empty(_state_shape(q, v, cu_seqlens), dtype=torch.float32)
+
+
+@torch.library.custom_op("csn::linear_attention_bwd", mutates_args=())
+def linear_attention_bwd(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, s0: Optional[Tensor], cu_seqlens: Optional[Tensor],
+                         do: Tensor, ds_last: Tensor, scale: Optional[float]) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    return gated._ext().linear_attention_backward(q, k, v, log_decay.detach(), s0, cu_seqlens, do, ds_last, scale)
+
+
+@linear_attention_bwd.register_fake
+def _(q, k, v, log_decay, s0, cu_seqlens, do, ds_last, scale):
+    return (q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape),
+            q.new_empty(_state_shape(q, v, cu_seqlens), dtype=torch.float32))
+
+
+def _linear_attention_setup(ctx, inputs, output):
+    q, k, v, log_decay, s0, cu, ctx.scale = inputs
+    if log_decay.requires_grad:
+        raise ValueError("linear_attention: log_decay has no gradient here: pass it detached")
+    ctx.save_for_backward(q, k, v, log_decay, s0, cu)
+    ctx.set_materialize_grads(True)
+
+
+def _linear_attention_backward(ctx, do, ds_last):
+    q, k, v, log_decay, s0, cu = ctx.saved_tensors
+    dq, dk, dv, ds0 = torch.ops.csn.linear_attention_bwd(q, k, v, log_decay, s0, cu, do, ds_last, ctx.scale)
+    return dq, dk, dv, None, None if s0 is None else ds0.to(s0.dtype), None, None
+
+
+linear_attention_fwd.register_autograd(_linear_attention_backward, setup_context=_linear_attention_setup)
+
+
+@torch.library.custom_op("csn::linear_attention_step", mutates_args=("s",))
+def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, s: Tensor, scale: Optional[float]) -> Tensor:
+    with torch.no_grad():
+        return gated._ext().linear_attention_step(q, k, v, log_decay, s, scale)
+
+
+@linear_attention_step.register_fake
+def _(q, k, v, log_decay, s, scale):
+    return q.new_empty((*q.shape[:-1], v.shape[-1]))
+
+
 # ------------------------------------------------------- sequence-parallel scan
 def _resolve_group(group_name: str):
     """The process group registered under `group_name` ("" = the default group)."""

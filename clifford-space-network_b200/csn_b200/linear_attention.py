@@ -27,10 +27,10 @@ def linear_attention(q, k, v, log_decay, s0=None, cu_seqlens=None, scale=None):
     s_last: the float32 states after the last ones, s0 for a sequence without steps.  scale: Dk ** -0.5 if absent.
     Differentiable in q, k, v and s0.
 
-    Sums and states are float32.  16-bit tensors whose rows start on 16 bytes, with head sizes that are multiples of 8, go
-    through the tensor cores in blocks of 128 steps (one more rounding to 16 bits of q k^T inside a block and of
-    the state where it meets q, none of the state that is carried); there an infinity or NaN in k or v can
-    reach the outputs of its whole block.  Other tensors are computed step by step."""
+    Sums and states are float32.  16-bit tensors go through the tensor cores in blocks of 128 steps (one more rounding
+    to 16 bits of q k^T inside a block and of the state where it meets q, none of the state that is carried); there an
+    infinity or NaN in k or v can reach the outputs of its whole block.  16-bit rows that do not start on 16 bytes, and expanded
+    ones, are copied first."""
     return (gated._module or gated._ext()).linear_attention(q, k, v, log_decay, s0, cu_seqlens, scale)
 
 

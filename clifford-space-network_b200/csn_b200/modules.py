@@ -1,5 +1,5 @@
 """nn.Module front ends of the block kernels, parameter-compatible with torch.nn, and the gated
-recurrent block."""
+recurrent and linear-attention blocks."""
 from __future__ import annotations
 
 from typing import Optional
@@ -13,13 +13,13 @@ from . import ops
 
 class LayerNorm(nn.LayerNorm):
     """nn.LayerNorm (same parameters, state_dict keys and eps) computed by the CUDA LayerNorm
-    kernels (csn_layer_norm_fwd / _bwd) for one normalised axis of C % 4 == 0, C <= 1024
-    features with affine weight and bias; other shapes go to F.layer_norm."""
+    kernels for one normalised axis with affine weight and bias: bfloat16 and float16 features of any number,
+    others of C % 4 == 0, C <= 1024; other shapes go to F.layer_norm."""
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         C = x.shape[-1]
         if (len(self.normalized_shape) == 1 and self.weight is not None and self.bias is not None
-                and ops.layer_norm_supported(C)):
+                and (x.dtype in (torch.bfloat16, torch.float16) or ops.layer_norm_supported(C))):
             return ops.layer_norm(x, self.weight, self.bias, self.eps)
         return F.layer_norm(x, self.normalized_shape, self.weight, self.bias, self.eps)
 
@@ -155,4 +155,80 @@ class GatedRecurrentBlock(nn.Module):
     def step(self, x_t: torch.Tensor, h: torch.Tensor) -> torch.Tensor:
         """One token, without dropout: x_t [B, d_model] -> out [B, d_model]; h is advanced in place."""
         x_t = x_t + self.mixer.step(self.ln_1(x_t), h)
+        return x_t + self.ffn(self.ln_2(x_t))
+
+
+# ------------------------------------------------------------- linear-attention block
+class LinearAttention(nn.Module):
+    """The mixer of a linear-attention block: one projection of x gives queries, keys and values, ops.linear_attention
+    runs over them as they lie, each head's output is normalised, and a projection goes back.  The heads'
+    memories run from 2^5 to 2^12 steps and are not trained (a buffer, float32 whatever the layer's type)."""
+
+    def __init__(self, d_model: int, num_heads: int, num_kv_heads: Optional[int] = None, head_dim: Optional[int] = None):
+        super().__init__()
+        self.num_heads = num_heads
+        self.num_kv_heads = num_heads if num_kv_heads is None else num_kv_heads
+        self.head_dim = d_model // num_heads if head_dim is None else head_dim
+        if num_heads < 1 or self.num_kv_heads < 1 or num_heads % self.num_kv_heads or not 1 <= self.head_dim <= 128:
+            raise ValueError(f"LinearAttention: num_kv_heads has to divide num_heads and heads have 1 to 128 places, got "
+                             f"{self.num_kv_heads}, {num_heads} and {self.head_dim}")
+        self.in_proj = nn.Linear(d_model, (num_heads + 2 * self.num_kv_heads) * self.head_dim, bias=False)
+        self.norm = LayerNorm(self.head_dim)
+        self.out_proj = nn.Linear(num_heads * self.head_dim, d_model, bias=False)
+        self.register_buffer("log_decay", torch.log1p(-torch.exp2(-torch.linspace(5.0, 12.0, num_heads))), persistent=False)
+
+    def _apply(self, fn, *args, **kwargs):
+        decay = self.log_decay
+        super()._apply(fn, *args, **kwargs)
+        # .bfloat16() and the like change the layer's type, not the decays': 16 bits have no number next to 1 - 2^-12
+        if self.log_decay.dtype != torch.float32:
+            self.log_decay = decay.to(self.log_decay.device)
+        return self
+
+    def init_state(self, batch_size: int, device=None) -> torch.Tensor:
+        device = device if device is not None else self.in_proj.weight.device
+        return torch.zeros(batch_size, self.num_heads, self.head_dim, self.head_dim, device=device)
+
+    def _heads(self, x: torch.Tensor):
+        h, hk, d = self.num_heads, self.num_kv_heads, self.head_dim
+        q, k, v = ops.linear(x, self.in_proj.weight).split([h * d, hk * d, hk * d], -1)
+        return q.unflatten(-1, (h, d)), k.unflatten(-1, (hk, d)), v.unflatten(-1, (hk, d))
+
+    def forward(self, x: torch.Tensor, s0: Optional[torch.Tensor] = None, cu_seqlens: Optional[torch.Tensor] = None):
+        """x [B, T, d_model], or [L, d_model] packed with cu_seqlens -> (out, float32 states [B, H, D, D])."""
+        o, s = ops.linear_attention(*self._heads(x), self.log_decay, s0=s0, cu_seqlens=cu_seqlens)
+        return ops.linear(self.norm(o).flatten(-2), self.out_proj.weight), s
+
+    @torch.no_grad()
+    def step(self, x_t: torch.Tensor, s: torch.Tensor) -> torch.Tensor:
+        """One token for each stream: x_t [B, d_model]; the states s [B, H, D, D] are advanced in place."""
+        o = ops.linear_attention_step(*self._heads(x_t), self.log_decay, s)
+        return ops.linear(self.norm(o).flatten(-2), self.out_proj.weight)
+
+
+class LinearAttentionBlock(nn.Module):
+    """x + drop(mixer(ln_1(x))), then + drop(ffn(ln_2(.))): linear attention and the gated feed-forward product as a residual
+    block, trained with forward() and advanced one token at a time with step()."""
+
+    def __init__(self, d_model: int, num_heads: int, num_kv_heads: Optional[int] = None, head_dim: Optional[int] = None,
+                 d_ffn: Optional[int] = None, dropout: float = 0.0):
+        super().__init__()
+        self.ln_1, self.ln_2 = LayerNorm(d_model), LayerNorm(d_model)
+        self.mixer = LinearAttention(d_model, num_heads, num_kv_heads, head_dim)
+        self.ffn = GatedFeedForward(d_model, d_ffn)
+        self.drop_1, self.drop_2 = DropoutAdd(dropout), DropoutAdd(dropout)
+
+    def init_state(self, batch_size: int, device=None) -> torch.Tensor:
+        return self.mixer.init_state(batch_size, device)
+
+    def forward(self, x: torch.Tensor, s0: Optional[torch.Tensor] = None, cu_seqlens: Optional[torch.Tensor] = None):
+        """x [B, T, d_model], or [L, d_model] packed with cu_seqlens -> (out, states after the last steps)."""
+        mixed, s = self.mixer(self.ln_1(x), s0, cu_seqlens)
+        x = self.drop_1(mixed, x)
+        return self.drop_2(self.ffn(self.ln_2(x)), x), s
+
+    @torch.no_grad()
+    def step(self, x_t: torch.Tensor, s: torch.Tensor) -> torch.Tensor:
+        """One token, without dropout: x_t [B, d_model] -> out [B, d_model]; s is advanced in place."""
+        x_t = x_t + self.mixer.step(self.ln_1(x_t), s)
         return x_t + self.ffn(self.ln_2(x_t))

@@ -18,14 +18,14 @@ constexpr int BLOCK = 16;  // steps that are worked on together
 // place of v and the K entries of the state beside it in registers: one packed pair of FMA an entry and step for each of the two
 // products, the products a . b shared by all threads.  The state is rounded once a block: step by step, a memory of
 // thousands of steps costs it a digit.
-// float32 rows come DEPTH - 1 blocks ahead by cp.async, 16 bytes at a time where they are aligned (WIDE); other types are
-// converted on their way.  Bound by the loads of a and b from shared memory, which every thread needs.
+// The rows come DEPTH - 1 blocks ahead by cp.async, 16 bytes at a time where they are aligned (`wide`).  Bound by the loads of
+// a and b from shared memory, which every thread needs.
 // OUT: false for the first pass.
 constexpr int MAX_PASSES = 3;
 struct Passes {
   Pass pass[MAX_PASSES];
 };
-__host__ __device__ constexpr int depth(int size) { return size == 4 ? 3 : 1; }
+constexpr int DEPTH = 3;
 __host__ __device__ constexpr int line(int places) { return places + 4; }  // aligned, and rows spread over the banks
 __host__ __device__ constexpr int stage_floats(int kp, int vp, bool out) { return BLOCK * ((out ? 2 : 1) * line(kp) + line(vp)); }
 
@@ -35,12 +35,12 @@ __device__ __forceinline__ void copy_async(float* to, const float* from, bool wi
   else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(at), "l"(from) : "memory");
 }
 
-template <typename T, int KP, int VP, bool OUT>
+template <int KP, int VP, bool OUT>
 __global__ void __launch_bounds__(VP) blocks_kernel(const Batch B, const __grid_constant__ Passes passes, bool wide) {
   const Pass& P = passes.pass[blockIdx.z];
   const Unit U(B, blockIdx.x);
   if (U.s < 0 || (!OUT && U.ends(P.back))) return;
-  constexpr int NJ = BLOCK * BLOCK / VP, DEPTH = depth(sizeof(T)), LK = line(KP), LV = line(VP), STAGE = stage_floats(KP, VP, OUT);
+  constexpr int NJ = BLOCK * BLOCK / VP, LK = line(KP), LV = line(VP), STAGE = stage_floats(KP, VP, OUT);
   const int h = blockIdx.y, c = threadIdx.x, late = P.back ? 1 : 0;
   const bool mine = c < P.V;
   extern __shared__ __align__(16) float stages[];  // [DEPTH][b, v, a][BLOCK][places]
@@ -60,21 +60,19 @@ __global__ void __launch_bounds__(VP) blocks_kernel(const Batch B, const __grid_
       if (2 * i + 1 < P.K) x[i].y = p[(2 * i + 1) * P.sr];
     }
   }
-  const T* a = static_cast<const T*>(P.a.p) + U.start(B, P.a) + h / P.a.shared * P.a.head;
-  const T* b = static_cast<const T*>(P.b.p) + U.start(B, P.b) + h / P.b.shared * P.b.head;
-  const T* v = static_cast<const T*>(P.v.p) + U.start(B, P.v) + h / P.v.shared * P.v.head;
+  const float* a = static_cast<const float*>(P.a.p) + U.start(B, P.a) + h / P.a.shared * P.a.head;
+  const float* b = static_cast<const float*>(P.b.p) + U.start(B, P.b) + h / P.b.shared * P.b.head;
+  const float* v = static_cast<const float*>(P.v.p) + U.start(B, P.v) + h / P.v.shared * P.v.head;
   const int steps = U.to - U.from;
   // the rows of a block, in their order of processing; what lies behind the last is left as it is
   auto fetch = [&](int done) {
     const int n = min(BLOCK, steps - done);
     float* const to = stages + done / BLOCK % DEPTH * STAGE;
-    auto rows = [&](const T* from, int64_t pitch, int places, int l, float* at) {
-      const int w = sizeof(T) == 4 && wide ? 4 : 1, pieces = (places + w - 1) / w;
+    auto rows = [&](const float* from, int64_t pitch, int places, int l, float* at) {
+      const int w = wide ? 4 : 1, pieces = (places + w - 1) / w;
       for (int i = c; i < n * pieces; i += VP) {
         const int r = i / pieces, d = (i - r * pieces) * w;
-        const T* p = from + (P.back ? U.to - 1 - done - r : U.from + done + r) * pitch + d;
-        if constexpr (sizeof(T) == 4) copy_async(at + r * l + d, reinterpret_cast<const float*>(p), w == 4);
-        else at[r * l + d] = to_float(*p);
+        copy_async(at + r * l + d, from + (P.back ? U.to - 1 - done - r : U.from + done + r) * pitch + d, wide);
       }
     };
     if (n > 0) {
@@ -82,20 +80,15 @@ __global__ void __launch_bounds__(VP) blocks_kernel(const Batch B, const __grid_
       rows(v, P.v.row, P.V, LV, to + BLOCK * LK);
       if (OUT) rows(a, P.a.row, P.K, LK, to + BLOCK * (LK + LV));
     }
-    if constexpr (sizeof(T) == 4) asm volatile("cp.async.commit_group;" ::: "memory");
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
   __syncthreads();
   for (int i = 0; i < DEPTH - 1; ++i) fetch(i * BLOCK);
   for (int done = 0; done < steps; done += BLOCK) {
     const int n = min(BLOCK, steps - done);
-    if (DEPTH == 1) {
-      __syncthreads();  // the block before has been read
-      fetch(done);
-    } else {
-      asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH > 1 ? DEPTH - 2 : 0) : "memory");
-    }
+    asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 2) : "memory");
     __syncthreads();
-    if (DEPTH > 1) fetch(done + (DEPTH - 1) * BLOCK);  // over the block before, which every thread is done with
+    fetch(done + (DEPTH - 1) * BLOCK);  // over the block before, which every thread is done with
     const float* const bs = stages + done / BLOCK % DEPTH * STAGE;
     const float *const vb = bs + BLOCK * LK, *const as = bs + BLOCK * (LK + LV);
     if (OUT) {
@@ -161,11 +154,10 @@ __global__ void __launch_bounds__(VP) blocks_kernel(const Batch B, const __grid_
       if (i >= n || !mine) continue;
       r = fmaf(power[i + 1 - late], o[OUT ? i : 0].x + o[OUT ? i : 0].y, r) * P.so;
       const int64_t t = U.row0 + (P.back ? U.to - 1 - done - i : U.from + done + i), at = (t * B.H + h) * P.V + c;
-      if (P.wide) static_cast<float*>(P.out)[at] = r;
-      else static_cast<T*>(P.out)[at] = from_float<T>(r);
+      static_cast<float*>(P.out)[at] = r;
     }
   }
-  if constexpr (sizeof(T) == 4) asm volatile("cp.async.wait_all;" ::: "memory");
+  asm volatile("cp.async.wait_all;" ::: "memory");
   float* to = OUT ? (P.last && U.ends(P.back) ? P.last + (U.s * B.H + h) * size : nullptr) : P.made + (U.unit * B.H + h) * size;
   if (to && mine) {
 #pragma unroll
@@ -324,43 +316,39 @@ Batch batch(int64_t S, int64_t T, int H, int Dk, int Dv, const int32_t* cu, bool
   return B;
 }
 
+size_t copy_floats(int64_t rows, int64_t heads, int64_t D) { return (size_t)up(rows * heads * up(D, 8) * 8 * 2, 16) * 4; }
 struct Room {  // in floats
-  int64_t states, dk, dv;
-  size_t bytes(bool backward) const { return sizeof(float) * (size_t)((backward ? 2 : 1) * states + dk + dv); }
+  int64_t states, dk, dv, copies;
+  size_t bytes(bool backward) const { return sizeof(float) * (size_t)((backward ? 2 : 1) * states + dk + dv + copies); }
 };
-Room room(const Batch& B, int Hk, int Dk, int Dv, bool packed, bool backward) {
+Room room(const Batch& B, int Hk, int Dk, int Dv, bool packed, bool backward, int mask) {
   const int64_t rows = packed ? B.T : B.S * B.T;
   const bool shared = backward && Hk < B.H;
+  int64_t copies = 0;
+  const int64_t heads[4] = {B.H, Hk, Hk, B.H}, D[4] = {Dk, Dk, Dv, Dv};
+  for (int i = 0; i < 4; ++i)
+    if (mask >> i & 1) copies += copy_floats(rows, heads[i], D[i]);
   return {is_cut(B, packed) ? up(B.units * B.H * Dk * Dv, 4) * 4 : 0, shared ? up(rows * B.H * Dk, 4) * 4 : 0,
-          shared ? up(rows * B.H * Dv, 4) * 4 : 0};
+          shared ? up(rows * B.H * Dv, 4) * 4 : 0, copies};
 }
 
-template <typename T, int KP, int VP, bool OUT>
+template <int KP, int VP, bool OUT>
 cudaError_t launch_blocks(const Batch& B, const Passes& P, int count, bool wide, cudaStream_t st) {
-  constexpr int smem = depth(sizeof(T)) * stage_floats(KP, VP, OUT) * 4;
+  constexpr int smem = DEPTH * stage_floats(KP, VP, OUT) * 4;
   if (smem > 32 * 1024)
-    if (cudaError_t e = allow_smem<blocks_kernel<T, KP, VP, OUT>>(smem)) return e;
-  blocks_kernel<T, KP, VP, OUT><<<dim3((unsigned)B.units, (unsigned)B.H, (unsigned)count), VP, smem, st>>>(B, P, wide);
+    if (cudaError_t e = allow_smem<blocks_kernel<KP, VP, OUT>>(smem)) return e;
+  blocks_kernel<KP, VP, OUT><<<dim3((unsigned)B.units, (unsigned)B.H, (unsigned)count), VP, smem, st>>>(B, P, wide);
   return cudaSuccess;
 }
-template <typename T, int KP>
+template <int KP>
 cudaError_t launch_blocks(const Batch& B, const Passes& P, int count, int V, bool first, bool wide, cudaStream_t st) {
-  if (V <= 32) return first ? launch_blocks<T, KP, 32, false>(B, P, count, wide, st) : launch_blocks<T, KP, 32, true>(B, P, count, wide, st);
-  if (V <= 64) return first ? launch_blocks<T, KP, 64, false>(B, P, count, wide, st) : launch_blocks<T, KP, 64, true>(B, P, count, wide, st);
-  return first ? launch_blocks<T, KP, 128, false>(B, P, count, wide, st) : launch_blocks<T, KP, 128, true>(B, P, count, wide, st);
-}
-template <typename T>
-cudaError_t launch_blocks(const Batch& B, const Passes& P, int count, int K, int V, bool first, bool wide, cudaStream_t st) {
-  if (K <= 32) return launch_blocks<T, 32>(B, P, count, V, first, wide, st);
-  if (K <= 64) return launch_blocks<T, 64>(B, P, count, V, first, wide, st);
-  return launch_blocks<T, 128>(B, P, count, V, first, wide, st);
+  if (V <= 32) return first ? launch_blocks<KP, 32, false>(B, P, count, wide, st) : launch_blocks<KP, 32, true>(B, P, count, wide, st);
+  if (V <= 64) return first ? launch_blocks<KP, 64, false>(B, P, count, wide, st) : launch_blocks<KP, 64, true>(B, P, count, wide, st);
+  return first ? launch_blocks<KP, 128, false>(B, P, count, wide, st) : launch_blocks<KP, 128, true>(B, P, count, wide, st);
 }
 
 int run(const Batch& B, const Pass* passes, int count, bool first, int dtype, cudaStream_t st) {
-  bool tensor = dtype != CSN_F32 && B.T > 0;
-  for (int i = 0; i < count; ++i)
-    tensor = tensor && fits_tensor(B, passes[i].a, passes[i].K) && fits_tensor(B, passes[i].b, passes[i].K) && fits_tensor(B, passes[i].v, passes[i].V);
-  if (tensor) return tensor_passes(B, passes, count, first, dtype == CSN_BF16, st);
+  if (dtype != CSN_F32 && B.T > 0) return tensor_passes(B, passes, count, first, dtype == CSN_BF16, st);
   auto wide = [](const Stream& x, int places) {
     return places % 4 == 0 && aligned(x.p, 16) && x.seq % 4 == 0 && x.row % 4 == 0 && x.head % 4 == 0;
   };
@@ -369,7 +357,7 @@ int run(const Batch& B, const Pass* passes, int count, bool first, int dtype, cu
     if (done[i]) continue;
     Passes P;
     int n = 0;
-    bool all_wide = dtype == CSN_F32;
+    bool all_wide = true;
     for (int j = i; j < count; ++j) {
       const Pass& p = passes[j];
       if (done[j] || p.K != passes[i].K || p.V != passes[i].V) continue;
@@ -379,12 +367,55 @@ int run(const Batch& B, const Pass* passes, int count, bool first, int dtype, cu
     }
     KernelTimer kt(first ? "linear_attention_first" : "linear_attention", st);
     const int K = passes[i].K, V = passes[i].V;
-    const cudaError_t e = dtype == CSN_F32    ? launch_blocks<float>(B, P, n, K, V, first, all_wide, st)
-                          : dtype == CSN_BF16 ? launch_blocks<__nv_bfloat16>(B, P, n, K, V, first, false, st)
-                                              : launch_blocks<__half>(B, P, n, K, V, first, false, st);
+    const cudaError_t e = K <= 32   ? launch_blocks<32>(B, P, n, V, first, all_wide, st)
+                          : K <= 64 ? launch_blocks<64>(B, P, n, V, first, all_wide, st)
+                                    : launch_blocks<128>(B, P, n, V, first, all_wide, st);
     if (e != cudaSuccess) return set_cuda_error(e, "csn_linear_attention: shared memory");
   }
   return CSN_OK;
+}
+
+// Rows of 16-bit streams that TMA cannot read, copied to rows that it can: [rows][heads][D up to a multiple of 8].
+struct Copy {
+  const uint16_t* from;
+  uint16_t* to;
+  int64_t seq, row, head, T, n;  // n: places in all
+  int heads, D, pitch;
+};
+struct Copies {
+  Copy copy[4];
+};
+__global__ void __launch_bounds__(256) copy_kernel(const __grid_constant__ Copies copies) {
+  const Copy& C = copies.copy[blockIdx.y];
+  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < C.n; i += (int64_t)gridDim.x * 256) {
+    const int d = (int)(i % C.D), h = (int)(i / C.D % C.heads);
+    const int64_t r = i / C.D / C.heads;
+    C.to[(r * C.heads + h) * C.pitch + d] = C.from[r / C.T * C.seq + r % C.T * C.row + h * C.head + d];
+  }
+}
+bool tma_reads(const void* p, const int64_t* st, int64_t S, int64_t T, int64_t heads) {
+  auto step = [](int64_t n, int64_t stride) { return n <= 1 || (stride > 0 && stride % 8 == 0 && stride < (1ll << 38)); };
+  return aligned(p, 16) && step(S, st[0]) && step(T, st[1]) && step(heads, st[2]);
+}
+// Puts copies of the streams of `mask` at `to` and the streams' new places into them.
+void copy_streams(Stream* const* streams, const int64_t* heads, const int64_t* D, int count, int mask, int64_t S, int64_t T, bool packed,
+                  float* to, cudaStream_t st) {
+  Copies C;
+  int n = 0;
+  int64_t most = 0;
+  for (int i = 0; i < count; ++i) {
+    if (!(mask >> i & 1)) continue;
+    Stream& x = *streams[i];
+    const int64_t rows = packed ? T : S * T, pitch = up(D[i], 8) * 8;
+    C.copy[n++] = {static_cast<const uint16_t*>(x.p), reinterpret_cast<uint16_t*>(to), x.seq, x.row, x.head, T, rows * heads[i] * D[i],
+                   (int)heads[i], (int)D[i], (int)pitch};
+    most = std::max(most, C.copy[n - 1].n);
+    x = {to, T * heads[i] * pitch, heads[i] * pitch, pitch, x.shared};
+    to += copy_floats(rows, heads[i], D[i]);
+  }
+  if (!n) return;
+  KernelTimer kt("linear_attention_copies", st);
+  copy_kernel<<<dim3((unsigned)std::min(up(most, 256), (int64_t)148 * 8), (unsigned)n), 256, 0, st>>>(C);
 }
 
 void join(const Batch& B, const float* enters, float* made, int size, bool back, cudaStream_t st) {
@@ -418,12 +449,20 @@ Stream stream_of(const void* p, const int64_t* st, int shared) { return {p, st[0
 using namespace csn;
 using namespace csn::la;
 
+extern "C" int csn_linear_attention_copies(const void* q, const void* k, const void* v, const void* d_o, const int64_t* strides, int64_t S,
+                                           int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, int packed, int dtype) {
+  if (dtype == CSN_F32 || !strides || T <= 0) return 0;
+  const int64_t n = packed ? 1 : S;
+  return (tma_reads(q, strides, n, T, H) ? 0 : 1) | (tma_reads(k, strides + 3, n, T, Hk) ? 0 : 2) |
+         (tma_reads(v, strides + 6, n, T, Hk) ? 0 : 4) | (!d_o || tma_reads(d_o, strides + 9, n, T, H) ? 0 : 8);
+}
+
 extern "C" size_t csn_linear_attention_workspace_bytes(int64_t S, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv,
-                                                       int packed, int dtype, int backward) {
+                                                       int packed, int dtype, int copies, int backward) {
   if (S <= 0 || T <= 0 || H <= 0 || Hk <= 0 || check_sizes("csn_linear_attention_workspace_bytes", S, T, H, Hk, Dk, Dv, dtype) != CSN_OK)
     return 0;
   const Batch B = batch(S, T, (int)H, (int)Dk, (int)Dv, nullptr, packed != 0, nullptr, backward != 0, dtype);
-  return room(B, (int)Hk, (int)Dk, (int)Dv, packed != 0, backward != 0).bytes(backward != 0);
+  return room(B, (int)Hk, (int)Dk, (int)Dv, packed != 0, backward != 0, dtype == CSN_F32 ? 0 : copies).bytes(backward != 0);
 }
 
 extern "C" int csn_linear_attention_fwd(const void* q, const void* k, const void* v, const int64_t* strides, const float* log_decay,
@@ -438,7 +477,8 @@ extern "C" int csn_linear_attention_fwd(const void* q, const void* k, const void
       (rows && (!q || !k || !v || !strides || !o || !aligned(q, size) || !aligned(k, size) || !aligned(v, size) || !aligned(o, 16))))
     return set_error(CSN_ERR_INVALID, "csn_linear_attention_fwd: missing or misaligned pointer");
   const Batch B = batch(S, T, (int)H, (int)Dk, (int)Dv, cu_seqlens, packed, log_decay, false, dtype);
-  const Room R = room(B, (int)Hk, (int)Dk, (int)Dv, packed, false);
+  const int mask = csn_linear_attention_copies(q, k, v, nullptr, strides, S, T, H, Hk, Dk, Dv, packed, dtype);
+  const Room R = room(B, (int)Hk, (int)Dk, (int)Dv, packed, false, mask);
   if (R.bytes(false) && (!workspace || workspace_bytes < R.bytes(false) || !aligned(workspace, 16)))
     return set_error(CSN_ERR_INVALID, "csn_linear_attention_fwd: workspace smaller than csn_linear_attention_workspace_bytes");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -447,6 +487,9 @@ extern "C" int csn_linear_attention_fwd(const void* q, const void* k, const void
   const int64_t* ss = strides ? strides : none;
   Pass P = {stream_of(q, ss, 1), stream_of(k, ss + 3, shared), stream_of(v, ss + 6, shared), o, s0, s_last, nullptr, Dv, 1,
             (int)Dk, (int)Dv, scale, 1.0f, false, false, false};
+  Stream* const streams[3] = {&P.a, &P.b, &P.v};
+  const int64_t heads[3] = {H, Hk, Hk}, places[3] = {Dk, Dk, Dv};
+  copy_streams(streams, heads, places, 3, mask, S, T, packed, static_cast<float*>(workspace) + R.states, st);
   if (R.states) {
     P.made = static_cast<float*>(workspace);
     if (int rc = run(B, &P, 1, true, dtype, st)) return rc;
@@ -473,16 +516,20 @@ extern "C" int csn_linear_attention_bwd(const void* q, const void* k, const void
                 !aligned(d_o, size) || !aligned(dq, 16) || !aligned(dk, 16) || !aligned(dv, 16))))
     return set_error(CSN_ERR_INVALID, "csn_linear_attention_bwd: missing or misaligned pointer");
   const Batch B = batch(S, T, (int)H, (int)Dk, (int)Dv, cu_seqlens, packed, log_decay, true, dtype);
-  const Room R = room(B, (int)Hk, (int)Dk, (int)Dv, packed, true);
+  const int mask = csn_linear_attention_copies(q, k, v, d_o, strides, S, T, H, Hk, Dk, Dv, packed, dtype);
+  const Room R = room(B, (int)Hk, (int)Dk, (int)Dv, packed, true, mask);
   if (R.bytes(true) && (!workspace || workspace_bytes < R.bytes(true) || !aligned(workspace, 16)))
     return set_error(CSN_ERR_INVALID, "csn_linear_attention_bwd: workspace smaller than csn_linear_attention_workspace_bytes");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int shared = (int)(H / Hk), entries = (int)(Dk * Dv);
   static const int64_t none[12] = {};
   const int64_t* ss = strides ? strides : none;
-  const Stream Q = stream_of(q, ss, 1), K = stream_of(k, ss + 3, shared), V = stream_of(v, ss + 6, shared), O = stream_of(d_o, ss + 9, 1);
+  Stream Q = stream_of(q, ss, 1), K = stream_of(k, ss + 3, shared), V = stream_of(v, ss + 6, shared), O = stream_of(d_o, ss + 9, 1);
   float* ws = static_cast<float*>(workspace);
   float *made = ws, *back = ws + R.states, *dk32 = back + R.states, *dv32 = dk32 + R.dk;
+  Stream* const streams[4] = {&Q, &K, &V, &O};
+  const int64_t heads[4] = {H, Hk, Hk, H}, places[4] = {Dk, Dk, Dv, Dv};
+  copy_streams(streams, heads, places, 4, mask, S, T, packed, dv32 + R.dv, st);
   Pass P[3] = {
       {O, V, K, dq, s0, nullptr, nullptr, 1, Dv, (int)Dv, (int)Dk, scale, 1.0f, false, false, false},
       {V, O, Q, shared > 1 ? dk32 : dk, ds_last, nullptr, nullptr, 1, Dv, (int)Dv, (int)Dk, 1.0f, scale, false, shared > 1, true},

@@ -93,9 +93,8 @@ struct Unit {
 // l^n without the rounding of log_decay * n (a product of 1000 would cost exp its last 10 bits); l^0 = 1 for l = 0 too
 __device__ __forceinline__ float fade(float log_decay, int n) { return n == 0 ? 1.0f : (float)exp((double)log_decay * n); }
 
-// Passes over 16-bit rows on the tensor cores; `first`: only the states that units make of nothing.  fits_tensor: whether
-// TMA can read a stream with heads of D places.  seg is a multiple of 128.
-bool fits_tensor(const Batch& B, const Stream& x, int D);
+// Passes over 16-bit rows on the tensor cores; `first`: only the states that units make of nothing.  Rows of the streams start on
+// 16 bytes, their strides are multiples of that and not 0 where an axis has more than one place.  seg is a multiple of 128.
 int tensor_passes(const Batch& B, const Pass* passes, int count, bool first, bool bf16, cudaStream_t st);
 
 }  // namespace la

@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
       const int quarter = warp % 4, side = warp / 4, i = quarter * 32 + lane;  // row of the block
       const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
       const float both = P.so * P.sb;
-      const bool whole_sectors = !P.wide && P.V % 16 == 0 && (reinterpret_cast<uintptr_t>(P.out) & 31) == 0;
+      const bool eights = P.V % 8 == 0, whole_sectors = P.V % 16 == 0 && (reinterpret_cast<uintptr_t>(P.out) & 31) == 0;
       // 32 products of this thread's row, c of four, faded and times `up`; `have`: places of the block
       auto products = [&](int c, int have, float up, float2 (&v)[16]) {
         tmem_load16(t_scores + lanes + c * 32, reinterpret_cast<float*>(v));
@@ -368,22 +368,30 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
             for (int e = 0; e < 8; ++e) v[e] = twice(__int_as_float(0x7fffffff));
           }
           if (!there || c >= P.V) continue;
-          // a row to a thread, whole sectors at a time; V is a multiple of 8
-          if (P.wide) {
+          // a row to a thread, whole sectors at a time
+          uint32_t w[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w[e] = pack2<BF16>(v[e].x, v[e].y);
+          if (P.wide && eights) {
             float* to = static_cast<float*>(P.out) + at + c;
             store8(to, reinterpret_cast<uint32_t*>(v));
             if (c + 8 < P.V) store8(to + 8, reinterpret_cast<uint32_t*>(v + 4));
-          } else {
-            uint32_t w[8];
+          } else if (P.wide) {
+            float* to = static_cast<float*>(P.out) + at + c;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = pack2<BF16>(v[e].x, v[e].y);
+            for (int e = 0; e < 16; ++e)
+              if (c + e < P.V) to[e] = e % 2 ? v[e / 2].y : v[e / 2].x;
+          } else if (whole_sectors) {
+            store8(static_cast<uint16_t*>(P.out) + at + c, w);
+          } else if (eights) {
             uint16_t* to = static_cast<uint16_t*>(P.out) + at + c;
-            if (whole_sectors) {
-              store8(to, w);
-            } else {
-              *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
-              if (c + 8 < P.V) *reinterpret_cast<uint4*>(to + 8) = make_uint4(w[4], w[5], w[6], w[7]);
-            }
+            *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+            if (c + 8 < P.V) *reinterpret_cast<uint4*>(to + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+          } else {
+            uint16_t* to = static_cast<uint16_t*>(P.out) + at + c;
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (c + e < P.V) to[e] = (uint16_t)(w[e / 2] >> (e % 2 * 16));
           }
         }
       }
@@ -595,12 +603,6 @@ bool map_stream(CUtensorMap* map, const Batch& B, const Stream& x, int D, bool b
 }  // namespace
 
 namespace la {
-
-bool fits_tensor(const Batch& B, const Stream& x, int D) {
-  auto step = [](int64_t n, int64_t stride) { return n <= 1 || (stride > 0 && stride % 8 == 0 && stride < (1ll << 38)); };
-  return D % 8 == 0 && reinterpret_cast<uintptr_t>(x.p) % 16 == 0 && step(B.H / x.shared, x.head) && step(B.T, x.row) &&
-         (B.cu || step(B.S, x.seq));
-}
 
 int tensor_passes(const Batch& B, const Pass* passes, int count, bool first, bool bf16, cudaStream_t st) {
   // passes whose tiles have one shape run side by side in one launch

@@ -410,10 +410,11 @@ std::tuple<Tensor, Tensor> attention_forward(const Tensor& q_, const Tensor& k_,
   std::vector<int64_t> shape(q.sizes().begin(), q.sizes().end());
   shape.back() = n.Dv;
   Tensor o = room(q, shape), last = floats(q, {n.S, n.H, n.Dk, n.Dv});
-  const size_t nb = csn_linear_attention_workspace_bytes(n.S, n.T, n.H, n.Hk, n.Dk, n.Dv, there(cu), code, 0);
-  const Tensor ws = bytes(q, nb);
   int64_t st[9];
   put_head_strides(st, q), put_head_strides(st + 3, k), put_head_strides(st + 6, v);
+  const int copies = csn_linear_attention_copies(ptr(q), ptr(k), ptr(v), nullptr, st, n.S, n.T, n.H, n.Hk, n.Dk, n.Dv, there(cu), code);
+  const size_t nb = csn_linear_attention_workspace_bytes(n.S, n.T, n.H, n.Hk, n.Dk, n.Dv, there(cu), code, copies, 0);
+  const Tensor ws = bytes(q, nb);
   check("csn_linear_attention_fwd",
         csn_linear_attention_fwd(ptr(q), ptr(k), ptr(v), st, static_cast<const float*>(ptr(log_decay)), static_cast<const float*>(ptr(s0)),
                                  static_cast<const int32_t*>(ptr(cu)), ptr(o), static_cast<float*>(ptr(last)), n.S, n.T, n.H, n.Hk, n.Dk,
@@ -435,10 +436,11 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> attention_backward(const Tensor& q_, 
   const int code = code_of(q.scalar_type());
   Tensor dq = want_q ? room(q, q.sizes()) : Tensor(), dk = want_k ? room(k, k.sizes()) : Tensor();
   Tensor dv = want_v || want_s0 ? room(v, v.sizes()) : Tensor(), ds0 = want_s0 ? floats(q, {n.S, n.H, n.Dk, n.Dv}) : Tensor();
-  const size_t nb = csn_linear_attention_workspace_bytes(n.S, n.T, n.H, n.Hk, n.Dk, n.Dv, there(cu), code, 1);
-  const Tensor ws = bytes(q, nb);
   int64_t st[12];
   put_head_strides(st, q), put_head_strides(st + 3, k), put_head_strides(st + 6, v), put_head_strides(st + 9, d);
+  const int copies = csn_linear_attention_copies(ptr(q), ptr(k), ptr(v), ptr(d), st, n.S, n.T, n.H, n.Hk, n.Dk, n.Dv, there(cu), code);
+  const size_t nb = csn_linear_attention_workspace_bytes(n.S, n.T, n.H, n.Hk, n.Dk, n.Dv, there(cu), code, copies, 1);
+  const Tensor ws = bytes(q, nb);
   check("csn_linear_attention_bwd",
         csn_linear_attention_bwd(ptr(q), ptr(k), ptr(v), ptr(d), st, static_cast<const float*>(ptr(log_decay)),
                                  static_cast<const float*>(ptr(s0)), static_cast<const int32_t*>(ptr(cu)),
@@ -500,7 +502,6 @@ std::tuple<Tensor, Tensor> linear_attention(const Tensor& q, const Tensor& k, co
 Tensor linear_attention_step(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& log_decay, const Tensor& s,
                              optional<double> scale) {
   no_tangent("linear_attention_step", {&q_, &k_, &v_, &log_decay, &s});
-  on_one_device("linear_attention_step", {&q_, &k_, &v_, &log_decay, &s});
   check_heads("linear_attention_step", "[B, H, D],", q_, k_, v_, log_decay, 1);
   const int64_t B = q_.size(0), H = q_.size(1), Hk = k_.size(1), Dk = q_.size(2), Dv = v_.size(2);
   TORCH_CHECK_VALUE(s.dim() == 4 && s.size(0) == B && s.size(1) == H && s.size(2) == Dk && s.size(3) == Dv && s.scalar_type() == at::kFloat &&
@@ -508,6 +509,7 @@ Tensor linear_attention_step(const Tensor& q_, const Tensor& k_, const Tensor& v
                     "linear_attention_step: s is a contiguous float32 state [", B, ", ", H, ", ", Dk, ", ", Dv, "], 16-byte aligned");
   TORCH_CHECK_VALUE(!wants_grad({&q_, &k_, &v_, &s}),
                     "linear_attention_step: not differentiable; call it under torch.no_grad() or use linear_attention");
+  on_one_device("linear_attention_step", {&q_, &k_, &v_, &log_decay, &s});
   const c10::cuda::CUDAGuard guard(q_.device());
   const Tensor q = rows(q_), k = rows(k_), v = rows(v_);
   Tensor o = room(q, {B, H, Dv});

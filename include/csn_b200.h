@@ -486,16 +486,22 @@ int csn_dropout_add(const void* x, const void* residual, const int64_t* rng, voi
  * are cut to 0 .. T; they must not fall.
  * log_decay [H] float32, at most 0 (-inf: nothing is remembered).  s0, s_last [S, H, Dk, Dv]
  * float32 (NULL: 0, not wanted).
- * Sums and states are float32.  16-bit tensors of 16-byte aligned rows (and head sizes that are
- * multiples of 8) go through the tensor cores in blocks of 128 steps: there the products q k^T
- * inside a block and the state, as an operand of its product with q, are rounded to the tensors'
- * type, the state that is carried on is not.  An infinity or NaN in k or v can reach the outputs of
- * its whole block.  Should a device-side wait give up (it is bounded), the results it concerns are
- * NaN.
- * The workspace is required where csn_linear_attention_workspace_bytes is not 0.  q, k, v, do
- * aligned to their type; everything else 16-byte aligned. */
+ * Sums and states are float32.  16-bit tensors go through the tensor cores in blocks of 128 steps:
+ * there the products q k^T inside a block and the state, as an operand of its product with q, are
+ * rounded to the tensors' type, the state that is carried on is not.  An infinity or NaN in k or v
+ * can reach the outputs of its whole block.  Should a device-side wait give up (it is bounded), the
+ * results it concerns are NaN.
+ * 16-bit operands whose rows do not start on 16 bytes (base, or a stride that is no multiple of 8
+ * elements, or 0 over more than one place) are copied first: csn_linear_attention_copies says which
+ * (bits 0 to 3 for q, k, v, do; do NULL in a forward pass), and the workspace query takes its
+ * answer.  The workspace is required where its size is not 0.  q, k, v, do aligned to their type;
+ * everything else 16-byte aligned. */
+int csn_linear_attention_copies(const void* q, const void* k, const void* v, const void* d_o,
+                                const int64_t* strides, int64_t S, int64_t T, int64_t H, int64_t Hk,
+                                int64_t Dk, int64_t Dv, int packed, int dtype);
 size_t csn_linear_attention_workspace_bytes(int64_t S, int64_t T, int64_t H, int64_t Hk, int64_t Dk,
-                                            int64_t Dv, int packed, int dtype, int backward);
+                                            int64_t Dv, int packed, int dtype, int copies,
+                                            int backward);
 int csn_linear_attention_fwd(const void* q, const void* k, const void* v, const int64_t* strides,
                              const float* log_decay, const float* s0, const int32_t* cu_seqlens,
                              void* o, float* s_last, int64_t S, int64_t T, int64_t H, int64_t Hk,
