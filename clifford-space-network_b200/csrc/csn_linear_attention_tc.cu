@@ -111,13 +111,48 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
   if (U.s < 0 || (!OUT && U.ends(back))) return;
   const int steps = U.to - U.from, blocks = (steps + STEPS - 1) / STEPS;
 
-  if (threadIdx.x == 0) {
-    mbar_init(&full_ab[0], 1), mbar_init(&full_ab[1], 1), mbar_init(&full_v, 1), mbar_init(&scores, 1), mbar_init(&met, 1);
-    mbar_init(&updated, 1), mbar_init(&probs, 8), mbar_init(&summed, 1);
-    mbar_init(&state, 8), mbar_init(&out_read[0], 8), mbar_init(&out_read[1], 8), mbar_init(&drained, 1);
-    mbar_init(&keys[0], 8), mbar_init(&keys[1], 8);
-    mbar_init_fence();
-    gave_up = 0;
+  // steps of block n: first .. first + have - 1 of the sequence
+  auto block = [&](int n, int& have) {
+    const int b = back ? blocks - 1 - n : n;
+    have = min(STEPS, steps - b * STEPS);
+    return U.from + b * STEPS;
+  };
+  auto load_ab = [&](int n) {
+    int have;
+    const int row = (B.cu ? (int)U.row0 : 0) + block(n, have), w = B.cu ? 0 : (int)U.s;
+    char* a = smem + (n & 1) * 2 * TA;
+    if (elect_one()) {
+      mbar_expect(&full_ab[n & 1], (OUT ? 2 : 1) * TA);
+#pragma unroll
+      for (int i = 0; i < NK; ++i) {
+        if (OUT) tma_load(a + i * BOX, &J.a, i * 64, h / P.a.shared, row, w, &full_ab[n & 1]);
+        tma_load(a + TA + i * BOX, &J.b, i * 64, h / P.b.shared, row, w, &full_ab[n & 1]);
+      }
+    }
+    __syncwarp();
+  };
+  auto load_v = [&](int n) {
+    int have;
+    const int row = (B.cu ? (int)U.row0 : 0) + block(n, have), w = B.cu ? 0 : (int)U.s;
+    if (elect_one()) {
+      mbar_expect(&full_v, NV * BOX);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) tma_load(tv + i * BOX, &J.v, i * 64, h / P.v.shared, row, w, &full_v);
+    }
+    __syncwarp();
+  };
+  if (warp == LOADS) {  // the first tiles are on their way while the rest is set up
+    if (elect_one()) {
+      mbar_init(&full_ab[0], 1), mbar_init(&full_ab[1], 1), mbar_init(&full_v, 1), mbar_init(&scores, 1), mbar_init(&met, 1);
+      mbar_init(&updated, 1), mbar_init(&probs, 8), mbar_init(&summed, 1);
+      mbar_init(&state, 8), mbar_init(&out_read[0], 8), mbar_init(&out_read[1], 8), mbar_init(&drained, 1);
+      mbar_init(&keys[0], 8), mbar_init(&keys[1], 8);
+      mbar_init_fence();
+      gave_up = 0;
+    }
+    __syncwarp();
+    if (blocks > 0) load_ab(0), load_v(0);
+    if (blocks > 1) load_ab(1);
   }
   if (warp == PRODUCTS) tmem_alloc<512>(&tmem_slot);
   fence_before();
@@ -131,51 +166,14 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
     else if (t - 320 < 63u) fan[t - 320] = fade(B.log_decay[h], abs((int)t - 351));
     asm volatile("bar.sync 3, 512;" ::: "memory");
   }
-  // steps of block n: first .. first + have - 1 of the sequence
-  auto block = [&](int n, int& have) {
-    const int b = back ? blocks - 1 - n : n;
-    have = min(STEPS, steps - b * STEPS);
-    return U.from + b * STEPS;
-  };
-
   if (warp >= 16) fewer_registers<FEW>();
   if (warp == LOADS) {  // ------------------------------------------------------------ loads
-    const int y_a = h / P.a.shared, y_b = h / P.b.shared, y_v = h / P.v.shared, w = B.cu ? 0 : (int)U.s;
-    const int row0 = B.cu ? (int)U.row0 : 0;
-    int ab = 0, vv = 0;  // blocks loaded
-    auto load_ab = [&](int n) {
-      int have;
-      const int row = row0 + block(n, have);
-      char* a = smem + (n & 1) * 2 * TA;
-      if (elect_one()) {
-        mbar_expect(&full_ab[n & 1], (OUT ? 2 : 1) * TA);
-#pragma unroll
-        for (int i = 0; i < NK; ++i) {
-          if (OUT) tma_load(a + i * BOX, &J.a, i * 64, y_a, row, w, &full_ab[n & 1]);
-          tma_load(a + TA + i * BOX, &J.b, i * 64, y_b, row, w, &full_ab[n & 1]);
-        }
-      }
-      __syncwarp();
-      ++ab;
-    };
-    auto load_v = [&](int n) {
-      int have;
-      const int row = row0 + block(n, have);
-      if (elect_one()) {
-        mbar_expect(&full_v, NV * BOX);
-#pragma unroll
-        for (int i = 0; i < NV; ++i) tma_load(tv + i * BOX, &J.v, i * 64, y_v, row, w, &full_v);
-      }
-      __syncwarp();
-      ++vv;
-    };
-    if (blocks > 0) load_ab(0), load_v(0);
-    if (blocks > 1) load_ab(1);
+    int ab = min(blocks, 2), vv = min(blocks, 1);  // blocks loaded
     bool ok = true;
     for (int n = 0; n + 1 < blocks && ok; ++n) {
       if (!(ok = __all_sync(0xffffffffu, mbar_wait(OUT ? &summed : &updated, n & 1, &gave_up)))) break;
-      load_v(n + 1);
-      if (n + 2 < blocks) load_ab(n + 2);
+      load_v(n + 1), ++vv;
+      if (n + 2 < blocks) load_ab(n + 2), ++ab;
     }
     // copies in flight end before the shared memory does: where a wait gave up, and otherwise these have long been awaited
     for (int n = max(ab - 2, 0); n < ab; ++n)
