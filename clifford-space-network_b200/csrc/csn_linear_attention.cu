@@ -52,8 +52,10 @@ __global__ void __launch_bounds__(VP) blocks_kernel(const Batch B, const __grid_
   float2 x[KP / 2];
 #pragma unroll
   for (int i = 0; i < KP / 2; ++i) x[i] = make_float2(0.0f, 0.0f);
-  if (OUT && P.state && mine) {
-    const float* p = P.state + ((P.by_unit ? U.unit : U.s) * B.H + h) * size + c * P.sc;
+  const bool cut = U.len > B.seg;
+  const float* const enters = cut ? P.made : P.state;
+  if (OUT && enters && mine) {
+    const float* p = enters + ((cut ? U.unit : U.s) * B.H + h) * size + c * P.sc;
 #pragma unroll
     for (int i = 0; i < KP / 2; ++i) {
       if (2 * i < P.K) x[i].x = p[2 * i * P.sr];
@@ -168,15 +170,19 @@ __global__ void __launch_bounds__(VP) blocks_kernel(const Batch B, const __grid_
   }
 }
 
-// What enters each segment, in place of what it made: made[u] holds the sum of a unit's own steps.
+// What enters each segment of the sequences that are cut, in place of what it made: made[u] holds the sum of a unit's own steps.
 __global__ void __launch_bounds__(256) join_kernel(const Batch B, const float* __restrict__ enters, float* made, int size, bool back) {
   const int64_t s = blockIdx.x;
   const int h = blockIdx.y, i = blockIdx.z * 256 + threadIdx.x;
-  if (i >= size) return;
   const int64_t row0 = B.cu ? Unit::border(B, s) : s * B.T;
   const int64_t len = B.cu ? max(Unit::border(B, s + 1), row0) - row0 : B.T;
-  const int64_t first = B.cu ? row0 / B.seg + s : s * B.segs, n = max((len + B.seg - 1) / B.seg, (int64_t)1);
-  const float whole = fade(B.log_decay[h], B.seg), rest = fade(B.log_decay[h], (int)(len - (n - 1) * B.seg));
+  const int64_t first = B.cu ? row0 / B.seg + s : s * B.segs, n = (len + B.seg - 1) / B.seg;
+  if (n < 2) return;
+  __shared__ float fades[2];  // of a whole segment and of the last one
+  if (threadIdx.x < 2) fades[threadIdx.x] = fade(B.log_decay[h], threadIdx.x == 0 ? B.seg : (int)(len - (n - 1) * B.seg));
+  __syncthreads();
+  if (i >= size) return;
+  const float whole = fades[0], rest = fades[1];
   float x = enters ? enters[(s * B.H + h) * size + i] : 0.0f;
   const int64_t step = (back ? -1 : 1) * (int64_t)B.H * size;
   float* p = made + ((first + (back ? n - 1 : 0)) * B.H + h) * size + i;
@@ -196,15 +202,32 @@ __global__ void __launch_bounds__(256) join_kernel(const Batch B, const float* _
   }
 }
 
-// [rows][H][D] float32 to [rows][H / shared][D] of type T
-template <typename T>
+// [rows][H][D] float32 to [rows][H / shared][D] of type T; N places to a thread
+template <typename T, int N>
 __global__ void __launch_bounds__(256) gather_kernel(const float* __restrict__ part, T* out, int64_t n, int D, int shared) {
+  const int per = D / N;
   for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const float* p = part + i / D * shared * D + i % D;
-    float v = p[0];
-    for (int j = 1; j < shared; ++j) v += p[(int64_t)j * D];
-    out[i] = from_float<T>(v);
+    // (a 64-bit division costs as much as the loads)
+    const int64_t row = i <= 0x7fffffff ? (int64_t)((uint32_t)i / (uint32_t)per) : i / per;
+    const float* p = part + row * shared * D + (i - row * per) * N;
+    Pack<float, N> v = *reinterpret_cast<const Pack<float, N>*>(p);
+    for (int j = 1; j < shared; ++j) {
+      const Pack<float, N> w = *reinterpret_cast<const Pack<float, N>*>(p + (int64_t)j * D);
+#pragma unroll
+      for (int e = 0; e < N; ++e) v.v[e] += w.v[e];
+    }
+    Pack<T, N> o;
+#pragma unroll
+    for (int e = 0; e < N; ++e) o.v[e] = from_float<T>(v.v[e]);
+    reinterpret_cast<Pack<T, N>*>(out)[i] = o;
   }
+}
+template <typename T>
+void gather(const float* part, void* out, int64_t n, int D, int shared, cudaStream_t st) {
+  const int N = D % 4 ? 1 : 4;
+  const unsigned grid = (unsigned)std::min((n / N + 255) / 256, (int64_t)148 * 16);
+  if (N == 4) gather_kernel<T, 4><<<grid, 256, 0, st>>>(part, static_cast<T*>(out), n / 4, D, shared);
+  else gather_kernel<T, 1><<<grid, 256, 0, st>>>(part, static_cast<T*>(out), n, D, shared);
 }
 
 // Rows of no sequence are 0: those before the first border and from the last one on.
@@ -486,7 +509,7 @@ extern "C" int csn_linear_attention_fwd(const void* q, const void* k, const void
   static const int64_t none[9] = {};
   const int64_t* ss = strides ? strides : none;
   Pass P = {stream_of(q, ss, 1), stream_of(k, ss + 3, shared), stream_of(v, ss + 6, shared), o, s0, s_last, nullptr, Dv, 1,
-            (int)Dk, (int)Dv, scale, 1.0f, false, false, false};
+            (int)Dk, (int)Dv, scale, 1.0f, false, false};
   Stream* const streams[3] = {&P.a, &P.b, &P.v};
   const int64_t heads[3] = {H, Hk, Hk}, places[3] = {Dk, Dk, Dv};
   copy_streams(streams, heads, places, 3, mask, S, T, packed, static_cast<float*>(workspace) + R.states, st);
@@ -494,8 +517,6 @@ extern "C" int csn_linear_attention_fwd(const void* q, const void* k, const void
     P.made = static_cast<float*>(workspace);
     if (int rc = run(B, &P, 1, true, dtype, st)) return rc;
     join(B, s0, P.made, entries, false, st);
-    P.state = P.made;
-    P.by_unit = true;
   }
   if (int rc = run(B, &P, 1, false, dtype, st)) return rc;
   if (rows) clear_outside(B, o, H * Dv * size, st);
@@ -531,18 +552,16 @@ extern "C" int csn_linear_attention_bwd(const void* q, const void* k, const void
   const int64_t heads[4] = {H, Hk, Hk, H}, places[4] = {Dk, Dk, Dv, Dv};
   copy_streams(streams, heads, places, 4, mask, S, T, packed, dv32 + R.dv, st);
   Pass P[3] = {
-      {O, V, K, dq, s0, nullptr, nullptr, 1, Dv, (int)Dv, (int)Dk, scale, 1.0f, false, false, false},
-      {V, O, Q, shared > 1 ? dk32 : dk, ds_last, nullptr, nullptr, 1, Dv, (int)Dv, (int)Dk, 1.0f, scale, false, shared > 1, true},
-      {K, Q, O, shared > 1 ? dv32 : dv, ds_last, ds0, nullptr, Dv, 1, (int)Dk, (int)Dv, 1.0f, scale, false, shared > 1, true}};
+      {O, V, K, dq, s0, nullptr, nullptr, 1, Dv, (int)Dv, (int)Dk, scale, 1.0f, false, false},
+      {V, O, Q, shared > 1 ? dk32 : dk, ds_last, nullptr, nullptr, 1, Dv, (int)Dv, (int)Dk, 1.0f, scale, shared > 1, true},
+      {K, Q, O, shared > 1 ? dv32 : dv, ds_last, ds0, nullptr, Dv, 1, (int)Dk, (int)Dv, 1.0f, scale, shared > 1, true}};
   if (R.states) {
-    P[0].made = made, P[2].made = back;
+    P[0].made = made, P[1].made = P[2].made = back;
     // the states of the forward direction are those that dq needs
     const Pass firsts[2] = {dq ? P[0] : P[2], P[2]};
     if (int rc = run(B, firsts, dq && (dk || dv) ? 2 : 1, true, dtype, st)) return rc;
     if (dq) join(B, s0, made, entries, false, st);
     if (dk || dv) join(B, ds_last, back, entries, true, st);
-    P[0].state = made, P[1].state = P[2].state = back;
-    for (Pass& p : P) p.by_unit = true;
   }
   Pass wanted[3];
   int count = 0;
@@ -554,15 +573,9 @@ extern "C" int csn_linear_attention_bwd(const void* q, const void* k, const void
     const int64_t n = packed ? T : S * T;
     if (shared > 1) {
       KernelTimer kt("linear_attention_gather", st);
-      auto gather = [&](const float* part, void* out, int64_t D) {
-        const int64_t count = n * Hk * D;
-        const unsigned grid = (unsigned)std::min(up(count, 256), (int64_t)148 * 16);
-        if (dtype == CSN_F32) gather_kernel<<<grid, 256, 0, st>>>(part, static_cast<float*>(out), count, (int)D, shared);
-        else if (dtype == CSN_BF16) gather_kernel<<<grid, 256, 0, st>>>(part, static_cast<__nv_bfloat16*>(out), count, (int)D, shared);
-        else gather_kernel<<<grid, 256, 0, st>>>(part, static_cast<__half*>(out), count, (int)D, shared);
-      };
-      if (dk) gather(dk32, dk, Dk);
-      if (dv) gather(dv32, dv, Dv);
+      auto* add = dtype == CSN_F32 ? gather<float> : dtype == CSN_BF16 ? gather<__nv_bfloat16> : gather<__half>;
+      if (dk) add(dk32, dk, n * Hk * Dk, (int)Dk, shared, st);
+      if (dv) add(dv32, dv, n * Hk * Dv, (int)Dv, shared, st);
     }
     if (dq) clear_outside(B, dq, H * Dk * size, st);
     if (dk) clear_outside(B, dk, Hk * Dk * size, st);

@@ -41,13 +41,13 @@ struct Batch {
 struct Pass {
   Stream a, b, v;
   void* out;             // [rows][H][V] contiguous; float32 where `wide`, the tensors' type elsewhere
-  const float* state;    // [S or units][H][K V] float32: what enters, NULL for 0
-  float* last;           // [S][H][K V]: what leaves each sequence, NULL: not wanted
-  float* made;           // first pass: [units][H][K V]
+  const float* state;    // [S][H][K V] float32: what enters each sequence, NULL for 0
+  float* last;           // [S][H][K V]: what leaves it, NULL: not wanted
+  float* made;           // [units][H][K V], of cut sequences: what the first pass leaves, and then what enters each segment
   int64_t sr, sc;        // entry (place of b, place of v) of a state at sr, sc
   int K, V;              // places of b and of v
   float so, sb;
-  bool by_unit, wide, back;
+  bool wide, back;
 };
 
 // The part of a sequence that a unit has: steps from .. to - 1 of len.

@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
   const Pass& P = J.pass;
   const int h = (int)(blockIdx.x / count % B.H);
   const Unit U(B, blockIdx.x / count / B.H);
-  const bool back = P.back;
+  const bool back = P.back, cut = U.len > B.seg;
   if (U.s < 0 || (!OUT && U.ends(back))) return;
   const int steps = U.to - U.from, blocks = (steps + STEPS - 1) / STEPS;
 
@@ -404,8 +404,9 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
     float x[32 * NK];
 #pragma unroll
     for (int k = 0; k < 32 * NK; ++k) x[k] = 0.0f;
-    if (OUT && P.state && mine) {
-      const float* p = P.state + ((P.by_unit ? U.unit : U.s) * B.H + h) * size + k0 * P.sr + r * P.sc;
+    const float* const enters = cut ? P.made : P.state;
+    if (OUT && enters && mine) {
+      const float* p = enters + ((cut ? U.unit : U.s) * B.H + h) * size + k0 * P.sr + r * P.sc;
 #pragma unroll
       for (int k = 0; k < 32 * NK; ++k)
         if (k0 + k < P.K) x[k] = p[k * P.sr];
