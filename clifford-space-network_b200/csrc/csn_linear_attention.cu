@@ -38,7 +38,7 @@ __device__ __forceinline__ void copy_async(float* to, const float* from, bool wi
 template <int KP, int VP, bool OUT>
 __global__ void __launch_bounds__(VP) blocks_kernel(const Batch B, const __grid_constant__ Passes passes, bool wide) {
   const Pass& P = passes.pass[blockIdx.z];
-  const Unit U(B, blockIdx.x);
+  const Unit U(B, blockIdx.x, !OUT, P.back);
   if (U.s < 0 || (!OUT && U.ends(P.back))) return;
   constexpr int NJ = BLOCK * BLOCK / VP, LK = line(KP), LV = line(VP), STAGE = stage_floats(KP, VP, OUT);
   const int h = blockIdx.y, c = threadIdx.x, late = P.back ? 1 : 0;
@@ -360,7 +360,7 @@ cudaError_t launch_blocks(const Batch& B, const Passes& P, int count, bool wide,
   constexpr int smem = DEPTH * stage_floats(KP, VP, OUT) * 4;
   if (smem > 32 * 1024)
     if (cudaError_t e = allow_smem<blocks_kernel<KP, VP, OUT>>(smem)) return e;
-  blocks_kernel<KP, VP, OUT><<<dim3((unsigned)B.units, (unsigned)B.H, (unsigned)count), VP, smem, st>>>(B, P, wide);
+  blocks_kernel<KP, VP, OUT><<<dim3((unsigned)unit_grid(B, !OUT), (unsigned)B.H, (unsigned)count), VP, smem, st>>>(B, P, wide);
   return cudaSuccess;
 }
 template <int KP>

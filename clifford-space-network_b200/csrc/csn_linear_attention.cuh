@@ -58,19 +58,25 @@ struct Unit {
   static __device__ __forceinline__ int64_t border(const Batch& B, int64_t i) {
     return min(max((int64_t)B.cu[i], (int64_t)0), B.T);
   }
-  __device__ __forceinline__ Unit(const Batch& B, int64_t u) : unit(u) {
+  // Unit u; or, `first`, in a packed batch the unit that row u seg lies in, and the next one where time runs down: each whole
+  // segment has one such row, so that the first pass, which is for these (those behind them) alone, need not start a CTA for
+  // every short sequence.
+  __device__ __forceinline__ Unit(const Batch& B, int64_t u, bool first, bool back) : unit(u) {
     int64_t m;
     if (B.cu) {
-      int64_t lo = 0, n = B.S;  // the last s whose units begin at u or before lies in lo .. lo + n - 1
+      const int64_t at = first ? u * B.seg : u;
+      int64_t lo = 0, n = B.S;  // the last s that begins at `at` or before lies in lo .. lo + n - 1
       while (n > 1) {
-        const int64_t half = n / 2, i = lo + half;
-        if (border(B, i) / B.seg + i <= u) lo = i, n -= half;
+        const int64_t half = n / 2, i = lo + half, row = border(B, i);
+        if ((first ? row : row / B.seg + i) <= at) lo = i, n -= half;
         else n = half;
       }
       s = lo;
       row0 = border(B, s);
       len = (int)(max(border(B, s + 1), row0) - row0);
-      m = u - (row0 / B.seg + s);
+      const int64_t base = row0 / B.seg + s;
+      if (first) unit = row0 <= at ? base + (at - row0) / B.seg + (back ? 1 : 0) : -1;
+      m = unit - base;
     } else {
       s = u / B.segs;
       row0 = s * B.T;
@@ -89,6 +95,9 @@ struct Unit {
   // elements from a stream's p to step 0 of the sequence
   __device__ __forceinline__ int64_t start(const Batch& B, const Stream& x) const { return B.cu ? row0 * x.row : s * x.seq; }
 };
+
+// CTAs along the units: all of them, or what the first pass needs
+inline int64_t unit_grid(const Batch& B, bool first) { return first && B.cu ? (B.T + B.seg - 1) / B.seg : B.units; }
 
 // l^n without the rounding of log_decay * n (a product of 1000 would cost exp its last 10 bits); l^0 = 1 for l = 0 too
 __device__ __forceinline__ float fade(float log_decay, int n) { return n == 0 ? 1.0f : (float)exp((double)log_decay * n); }

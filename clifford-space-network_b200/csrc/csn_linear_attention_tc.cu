@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
   const Job& J = jobs.job[blockIdx.x % count];
   const Pass& P = J.pass;
   const int h = (int)(blockIdx.x / count % B.H);
-  const Unit U(B, blockIdx.x / count / B.H);
+  const Unit U(B, blockIdx.x / count / B.H, !OUT, P.back);
   const bool back = P.back, cut = U.len > B.seg;
   if (U.s < 0 || (!OUT && U.ends(back))) return;
   const int steps = U.to - U.from, blocks = (steps + STEPS - 1) / STEPS;
@@ -579,7 +579,7 @@ template <bool BF16, int NK, int NV, bool OUT>
 cudaError_t launch(const Jobs& jobs, const Batch& B, int count, cudaStream_t st) {
   constexpr int smem = smem_bytes(NK, NV, BF16);
   if (cudaError_t e = allow_smem<blocks_tc_kernel<BF16, NK, NV, OUT>>(smem)) return e;
-  blocks_tc_kernel<BF16, NK, NV, OUT><<<(unsigned)(B.units * B.H * count), THREADS, smem, st>>>(jobs, B, count);
+  blocks_tc_kernel<BF16, NK, NV, OUT><<<(unsigned)(unit_grid(B, !OUT) * B.H * count), THREADS, smem, st>>>(jobs, B, count);
   return cudaSuccess;
 }
 template <bool BF16, int NK, int NV>
