@@ -13,13 +13,13 @@ from . import ops
 
 class LayerNorm(nn.LayerNorm):
     """nn.LayerNorm (same parameters, state_dict keys and eps) computed by the CUDA LayerNorm
-    kernels for one normalised axis with affine weight and bias: bfloat16 and float16 features of any number,
+    kernels for one normalised axis with affine weight and bias: any number of bfloat16 and float16 features on CUDA,
     others of C % 4 == 0, C <= 1024; other shapes go to F.layer_norm."""
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         C = x.shape[-1]
         if (len(self.normalized_shape) == 1 and self.weight is not None and self.bias is not None
-                and (x.dtype in (torch.bfloat16, torch.float16) or ops.layer_norm_supported(C))):
+                and (x.is_cuda and x.dtype in (torch.bfloat16, torch.float16) or ops.layer_norm_supported(C))):
             return ops.layer_norm(x, self.weight, self.bias, self.eps)
         return F.layer_norm(x, self.normalized_shape, self.weight, self.bias, self.eps)
 

@@ -188,6 +188,32 @@ def test_long_offsets(ops):
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("borders", [[-5, 60, 30, 400], [0, 500, 100, 100], [200, 150, 100, 50], [1 << 30, -(1 << 30), 7, 9]])
+def test_any_borders_stay_inside(ops, kind, borders):
+    """Borders outside the rows, or falling ones, are cut to what is there: every access stays inside, and what a sequence with good
+    borders of its own gives is finite."""
+    cu = torch.tensor(borders, dtype=torch.int32, device="cuda")
+    L, S = 300, len(borders) - 1
+    q, k, v = (make((L, 2, 64), kind, i).requires_grad_(True) for i in range(3))
+    o, s = ops.linear_attention(q, k, v, decays(2), s0=make((S, 2, 64, 64), "float32", 4), cu_seqlens=cu)
+    torch.autograd.grad((o, s), (q, k, v), (torch.ones_like(o), torch.ones_like(s)))
+    torch.cuda.synchronize()
+    good = [(a, b) for a, b in zip(borders[:-1], borders[1:]) if 0 <= a < b <= L]
+    for a, b in good[:1]:
+        assert torch.isfinite(o[a:b]).all()
+
+
+def test_no_rows(ops):
+    """Packed sequences without a row: the states pass through, and so do their gradients."""
+    for kind in TYPES:
+        q = torch.zeros(0, 2, 16, device="cuda", dtype=TYPES[kind])
+        s0 = make((3, 2, 16, 16), "float32", 1).requires_grad_(True)
+        o, s = ops.linear_attention(q, q, q, decays(2), s0=s0, cu_seqlens=torch.zeros(4, dtype=torch.int32, device="cuda"))
+        ds = make((3, 2, 16, 16), "float32", 2)
+        assert o.shape == (0, 2, 16) and torch.equal(s, s0) and torch.equal(torch.autograd.grad(s, s0, ds)[0], ds)
+
+
 def test_registered_operators(ops):
     csn = torch.ops.csn
     q, k, v = (make((2, 140, 2, 32), "bfloat16", i).requires_grad_(True) for i in range(3))

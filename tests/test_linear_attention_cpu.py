@@ -199,6 +199,14 @@ def test_modules_keep_their_decays():
     assert LinearAttention(64, 4).to(torch.float16).to("meta").log_decay.device.type == "meta"
 
 
+def test_layer_norm_module_off_the_gpu():
+    """What went to the library's layer norm on the CPU still does."""
+    from csn_b200.modules import LayerNorm
+    m = LayerNorm(6).bfloat16()
+    x = torch.randn(3, 6).bfloat16()
+    assert torch.equal(m(x), torch.nn.functional.layer_norm(x, (6,), m.weight, m.bias, m.eps))
+
+
 @pytest.mark.parametrize("kw", [{"num_heads": 4, "num_kv_heads": 3}, {"num_heads": 0}, {"num_heads": 1, "head_dim": 129}, {"num_heads": 4, "num_kv_heads": 0}])
 def test_modules_refuse(kw):
     with pytest.raises((ValueError, ZeroDivisionError)):
