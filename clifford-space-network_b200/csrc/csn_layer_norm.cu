@@ -268,10 +268,11 @@ __global__ void __launch_bounds__(1024) long_forward_kernel(const T* __restrict_
 // so it also gathers their sums of dy h and dy, which the CTA adds up at the end: part[CTA][0 and 1][C].  For V = 8 each
 // thread copies its own pieces of x and dy into shared memory DEPTH - 1 rows ahead (cp.async; no other thread reads them, so
 // that no barrier is needed): the registers that loads in flight would take leave room for more warps.
-// bf16 on a B200, with the sums: R32768 C2048 93 us (4.3 TB/s), R524288 C128 80 (5.0), R8192 C8192 108 (3.7).  An SM issues in
-// two thirds of its cycles: shuffles, the meeting of a row's warps and addresses cost a row 130 instructions a thread, so a
-// thread has 16 places of it (8: 108 us for C2048).  Slower: loads into registers (160 us), mean and rstd read when a row's turn
-// comes (140 us for C8192), more CTAs than the SMs hold at a time.
+// bf16 on a B200, with the sums: R32768 C2048 93 us (4.3 TB/s), R524288 C128 80 (5.0), R8192 C8192 108 (3.7).  Neither memory nor
+// issue is full (an SM issues in 41 to 62 % of its cycles, with 15 of 64 warps): a row's meeting at its barrier and the chain from
+// its sums to its gradient are what a few warps wait for.  Slower: 8 places to a thread 108 us for C2048 (shuffles, the meeting
+// and addresses cost a row 130 instructions a thread, whatever it has of it), loads into registers 160, mean and rstd
+// read when a row's turn comes 140 for C8192, more CTAs than the SMs hold at a time.
 template <typename T, typename W, int TPR, int NV, int V, int DEPTH>
 __global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS, TPR > THREADS ? 1 : NV > 1 ? 2 : 4)
     backward_kernel(const T* __restrict__ dy, int64_t ldy, const T* __restrict__ x, int64_t ld, const float* __restrict__ mean,
