@@ -19,8 +19,9 @@ constexpr int BLOCK = 16;  // steps that are worked on together
 // products, the products a . b shared by all threads.  The state is rounded once a block: step by step, a memory of
 // thousands of steps costs it a digit.
 // The rows come DEPTH - 1 blocks ahead by cp.async, 16 bytes at a time where they are aligned (`wide`).  Bound by the loads of
-// a and b from shared memory, which every thread needs, one for two packed FMA: B32 T2048 H4 D32 forward 158 us with the first
-// pass, B8 T4096 H16 D64 874.  Slower: step by step 540 us (three roundings a step, too), rows loaded when their turn comes 706.
+// a and b from shared memory, which every thread needs, one for two packed FMA: forward, with the first pass, B32 T2048 H4 D32
+// 161 us, B8 T4096 H16 D64 780, B2 T2048 H16 D128 386.  Slower: step by step (three roundings a step, too) and rows loaded when
+// their turn comes, 706 us for the first; half as many segments 158, 874 and 457.
 // OUT: false for the first pass.
 constexpr int MAX_PASSES = 3;
 struct Passes {
@@ -312,7 +313,7 @@ int width_of(int dtype) { return dtype == CSN_F32 ? 4 : dtype == CSN_BF16 || dty
 bool aligned(const void* p, int n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// The steps of a segment, a multiple of 128.  float32: enough segments for 12 warps on each SM.  16 bits, one CTA an SM: what
+// The steps of a segment, a multiple of 128.  float32: enough segments for 24 warps on each SM.  16 bits, one CTA an SM: what
 // takes the least time by these, measured with 128 x 128 states in bf16, in units of 0.1 us: a block of 128 steps 39, the start and end
 // of a CTA 90; where sequences are cut, in the first pass 27 and 70, and join_kernel 50, 5 a segment and its states' bytes.
 void cut(Batch& B, int Dk, int Dv, int passes, bool packed, bool half) {
@@ -327,7 +328,7 @@ void cut(Batch& B, int Dk, int Dv, int passes, bool packed, bool half) {
       if (cost < least) least = cost, best = n;
     }
   } else {
-    best = std::min(rows, up(148 * 12, heads * passes * up(std::min(Dk, Dv), 32)));
+    best = std::min(rows, up(148 * 24, heads * passes * up(std::min(Dk, Dv), 32)));
   }
   B.seg = (int)(std::max(up(rows, std::max(best, (int64_t)1)), (int64_t)1) * 128);
   B.segs = packed ? 0 : (int)std::max(up(B.T, B.seg), (int64_t)1);
