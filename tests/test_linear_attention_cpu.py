@@ -211,3 +211,32 @@ def test_layer_norm_module_off_the_gpu():
 def test_modules_refuse(kw):
     with pytest.raises((ValueError, ZeroDivisionError)):
         LinearAttention(64, **kw)
+
+
+# ------------------------------------------------------- the 64-bit forms that the kernels are held against
+def differences(value, leaves, grads):
+    """Central differences along one direction for each input, against the inner product of its gradient."""
+    for i, x in enumerate(leaves):
+        way, e = torch.randn(x.shape, dtype=torch.float64, generator=torch.Generator().manual_seed(i)), 1e-5
+        ends = [value(*[u + s * e * way if j == i else u for j, u in enumerate(leaves)]) for s in (1.0, -1.0)]
+        want, got = (ends[0] - ends[1]) / (2 * e), (grads[i] * way).sum()
+        # the third-order term is e^2 of values of a few units, the rounding of the ends 1e-16 / e of theirs
+        assert abs(want - got) <= 1e-7 * (1.0 + abs(want) + ends[0].abs())
+
+
+def test_oracles_gradients_are_differences():
+    import linear_attention_oracle as orc
+    r = lambda *s: torch.randn(*s, dtype=torch.float64, generator=torch.Generator().manual_seed(sum(s)))  # noqa: E731
+    L, H, Hk, Dk, Dv, borders = 11, 4, 2, 5, 3, [(0, 4), (4, 4), (4, 10)]
+    g, do, ds = -r(H).abs(), r(L, H, Dv), r(3, H, Dk, Dv)
+    ins = [r(L, H, Dk), r(L, Hk, Dk), r(L, Hk, Dv), r(3, H, Dk, Dv)]
+
+    def attention(q, k, v, s0):
+        out = orc.attention(q, k, v, g, s0, borders, 0.3)
+        return (out["o"][0] * do).sum() + (out["s"][0] * ds).sum()
+
+    got = orc.attention(*ins[:3], g, ins[3], borders, 0.3, do, ds)
+    differences(attention, ins, [got[n][0] for n in ("dq", "dk", "dv", "ds0")])
+    dy, ins = r(6, 9), [r(6, 9) + 2.0, r(9), r(1, 9)[0]]
+    got = orc.layer_norm(*ins, 1e-3, dy)
+    differences(lambda x, w, b: (orc.layer_norm(x, w, b, 1e-3)["y"][0] * dy).sum(), ins, [got[n][0] for n in ("dx", "dw", "db")])
