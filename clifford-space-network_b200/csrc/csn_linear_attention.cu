@@ -354,8 +354,9 @@ Room room(const Batch& B, int Hk, int Dk, int Dv, bool packed, bool backward, in
   const int64_t heads[4] = {B.H, Hk, Hk, B.H}, D[4] = {Dk, Dk, Dv, Dv};
   for (int i = 0; i < 4; ++i)
     if (mask >> i & 1) copies += copy_floats(rows, heads[i], D[i]);
-  return {is_cut(B, packed) ? up(B.units * B.H * Dk * Dv, 4) * 4 : 0, shared ? up(rows * B.H * Dk, 4) * 4 : 0,
-          shared ? up(rows * B.H * Dv, 4) * 4 : 0, copies};
+  // each part in whole sectors of 32 bytes, which the rows of the partial gradients are written in
+  return {is_cut(B, packed) ? up(B.units * B.H * Dk * Dv, 8) * 8 : 0, shared ? up(rows * B.H * Dk, 8) * 8 : 0,
+          shared ? up(rows * B.H * Dv, 8) * 8 : 0, copies};
 }
 
 template <int KP, int VP, bool OUT>

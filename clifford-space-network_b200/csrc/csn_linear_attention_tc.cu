@@ -80,7 +80,7 @@ __device__ __forceinline__ float scale_up(float top, float& down) {
   return __uint_as_float((268 - e) << 23);
 }
 
-// 32 bytes in one access
+// 32 bytes in one access, p on a multiple of them
 __device__ __forceinline__ void store8(void* p, const uint32_t* w) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
                "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
@@ -268,7 +268,8 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
       const int quarter = warp % 4, side = warp / 4, i = quarter * 32 + lane;  // row of the block
       const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
       const float both = P.so * P.sb;
-      const bool eights = P.V % 8 == 0, whole_sectors = P.V % 16 == 0 && (reinterpret_cast<uintptr_t>(P.out) & 31) == 0;
+      // rows whose pieces of 16 places (8, of float32) are sectors of 32 bytes, which store8 wants on such a border
+      const bool sectors = (reinterpret_cast<uintptr_t>(P.out) & 31) == 0, eights = P.V % 8 == 0, whole_sectors = P.V % 16 == 0 && sectors;
       // 32 products of this thread's row, c of four, faded and times `up`; `have`: places of the block
       auto products = [&](int c, int have, float up, float2 (&v)[16]) {
         tmem_load16(t_scores + lanes + c * 32, reinterpret_cast<float*>(v));
@@ -380,7 +381,7 @@ __global__ void __launch_bounds__(THREADS, 1) blocks_tc_kernel(const __grid_cons
           uint32_t w[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) w[e] = pack2<BF16>(v[e].x, v[e].y);
-          if (P.wide && eights) {
+          if (P.wide && eights && sectors) {
             float* to = static_cast<float*>(P.out) + at + c;
             store8(to, reinterpret_cast<uint32_t*>(v));
             if (c + 8 < P.V) store8(to + 8, reinterpret_cast<uint32_t*>(v + 4));
