@@ -5,7 +5,12 @@
 //   dx = r (g - mean(g) - h mean(g h)),  dw = sum over rows of dy h,  db = sum over rows of dy
 // Rows are read and written in their own type and computed in float32 (csn_block.cu has the float32 rows); w and b are
 // of the rows' type or float32.
+//
+// x - m is formed before anything else: r x - m r instead would put half a step of |m| r into h, which is 1 for a float16 row of one
+// value near 60000.  m is a quotient, and where C > 2^13, so that 24 bits do not hold the sum of C places of 11 bits, it
+// is corrected by the mean of x - m.  So rows of one value give h = 0 to the bit, whatever their width.
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 
 #include "csn_internal.h"
@@ -163,6 +168,19 @@ __device__ __forceinline__ void row_sums(float (&v)[n], float* room, int& turn) 
   }
 }
 
+// s / C, which is exact where float32 has it, as the product with 1 / C is not (Markstein's remainder step)
+__device__ __forceinline__ float mean_of(float s, float n, float over) {
+  const float m = s * over;
+  return fmaf(fmaf(-m, n, s), over, m);
+}
+// The mean m of a row corrected by that of x - m, whose part of the mean square of x - m is taken out.
+__device__ __forceinline__ void correct(float d, float& m, float& square) {
+  m += d;
+  const float var = fmaf(-d, d, square);
+  // a NaN stays one, and squares past float32's range an infinity
+  square = var < 0.0f ? 0.0f : square < INFINITY ? var : square;
+}
+
 // TPR threads take a row, NV pieces of V neighbouring places each, and ROWS rows at a time, to have enough loads in flight: a row
 // is read once and stays in registers, in its own type.  V = 8 where rows start on 16 bytes and C is a multiple of 8, else 1.
 // A warp takes rows of up to 2048 places: two reductions without a barrier.
@@ -174,13 +192,14 @@ __global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS, TPR > THREADS ?
     forward_kernel(const T* __restrict__ x, int64_t ld, const W* __restrict__ w, const W* __restrict__ b, T* __restrict__ y, float* mean,
                    float* rstd, int64_t R, int C, float eps) {
   constexpr int N = TPR > THREADS ? TPR : THREADS, GROUPS = N / TPR;
-  __shared__ __align__(16) float room[2 * (TPR > 32 ? N / 32 : 1) * ROWS];
+  constexpr bool FAR = TPR * NV * V > 8192;  // (all of them have C > 8192)
+  __shared__ __align__(16) float room[2 * (TPR > 32 ? N / 32 : 1) * (FAR ? 2 : 1) * ROWS];
   const int t = threadIdx.x % TPR;
-  const float over = 1.0f / C;
+  const float n = C, over = 1.0f / n;
   int turn = 0;
   for (int64_t r0 = blockIdx.x * (int64_t)(GROUPS * ROWS); r0 < R; r0 += (int64_t)gridDim.x * (GROUPS * ROWS)) {
     Piece<T, V> p[ROWS][NV];
-    float m[ROWS], s[ROWS];
+    float m[ROWS], s[ROWS], q[FAR ? 2 * ROWS : ROWS];  // q: the sums of (x - m)^2, and of x - m
 #pragma unroll
     for (int j = 0; j < ROWS; ++j) {
       const int64_t r = r0 + j * GROUPS + threadIdx.x / TPR;
@@ -201,19 +220,25 @@ __global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS, TPR > THREADS ?
     row_sums<TPR>(s, room, turn);
 #pragma unroll
     for (int j = 0; j < ROWS; ++j) {
-      m[j] = s[j] * over;
-      Floats<V> a = all<V>(0.0f);
+      m[j] = mean_of(s[j], n, over);
+      Floats<V> a = all<V>(0.0f), b = a;
 #pragma unroll
       for (int k = 0; k < NV; ++k)
         if ((k * TPR + t) * V < C) {
           const Floats<V> d = add<V>(floats<T, V>(p[j][k]), all<V>(-m[j]));
+          if (FAR) b = add<V>(b, d);
           a = fma<V>(d, d, a);
         }
-      s[j] = sum<V>(a);
+      q[j] = sum<V>(a);
+      if (FAR) q[FAR ? ROWS + j : 0] = sum<V>(b);
     }
-    row_sums<TPR>(s, room, turn);
+    row_sums<TPR>(q, room, turn);
 #pragma unroll
-    for (int j = 0; j < ROWS; ++j) s[j] = 1.0f / sqrtf(s[j] * over + eps);
+    for (int j = 0; j < ROWS; ++j) {
+      float square = q[j] * over;
+      if (FAR) correct(mean_of(q[FAR ? ROWS + j : 0], n, over), m[j], square);
+      s[j] = 1.0f / sqrtf(square + eps);
+    }
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int c = (k * TPR + t) * V;
@@ -223,7 +248,7 @@ __global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS, TPR > THREADS ?
       for (int j = 0; j < ROWS; ++j) {
         const int64_t r = r0 + j * GROUPS + threadIdx.x / TPR;
         if (r >= R) continue;
-        const Floats<V> h = fma<V>(floats<T, V>(p[j][k]), all<V>(s[j]), all<V>(-m[j] * s[j]));
+        const Floats<V> h = mul<V>(add<V>(floats<T, V>(p[j][k]), all<V>(-m[j])), all<V>(s[j]));
         store<T, V>(y + r * C + c, fma<V>(h, wv, bv));
       }
     }
@@ -242,22 +267,24 @@ template <typename T, typename W>
 __global__ void __launch_bounds__(1024) long_forward_kernel(const T* __restrict__ x, int64_t ld, const W* __restrict__ w,
                                                             const W* __restrict__ b, T* __restrict__ y, float* mean, float* rstd,
                                                             int64_t R, int C, float eps) {
-  __shared__ __align__(16) float room[64];
-  const float over = 1.0f / C;
+  __shared__ __align__(16) float room[128];
+  const float n = C, over = 1.0f / n;
   int turn = 0;
   for (int64_t r = blockIdx.x; r < R; r += gridDim.x) {
     const T* p = x + r * ld;
     float s[1] = {0.0f};
     for (int c = threadIdx.x; c < C; c += 1024) s[0] += to_float(p[c]);
     row_sums<1024>(s, room, turn);
-    const float m = s[0] * over;
-    s[0] = 0.0f;
+    float m = mean_of(s[0], n, over), q[2] = {0.0f, 0.0f};
     for (int c = threadIdx.x; c < C; c += 1024) {
       const float d = to_float(p[c]) - m;
-      s[0] = fmaf(d, d, s[0]);
+      q[0] = fmaf(d, d, q[0]);
+      q[1] += d;
     }
-    row_sums<1024>(s, room, turn);
-    const float k = 1.0f / sqrtf(s[0] * over + eps);
+    row_sums<1024>(q, room, turn);
+    float square = q[0] * over;
+    correct(mean_of(q[1], n, over), m, square);
+    const float k = 1.0f / sqrtf(square + eps);
     for (int c = threadIdx.x; c < C; c += 1024)
       y[r * C + c] = from_float<T>(fmaf((to_float(p[c]) - m) * k, to_float(w[c]), to_float(b[c])));
     if (threadIdx.x == 0 && mean) mean[r] = m, rstd[r] = k;
@@ -339,7 +366,6 @@ __global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS, TPR > THREADS ?
       m = stats[slot * 2 * N], k1 = stats[(slot * 2 + 1) * N];
     }
     if (!there) m = k1 = 0.0f;
-    const float off = -m * k1;  // h = k1 x + off
     const Piece* const mine = ring + slot * 2 * NV * N;
     auto of_x = [&](int k) { return floats<T, V>(V == 8 ? mine[k * N] : now[V == 8 ? 0 : k]); };
     auto of_dy = [&](int k) { return floats<T, V>(V == 8 ? mine[(NV + k) * N] : now[V == 8 ? 0 : NV + k]); };
@@ -347,7 +373,7 @@ __global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS, TPR > THREADS ?
 #pragma unroll
     for (int k = 0; k < NV; ++k)
       if (there && (k * TPR + t) * V < C) {
-        const Floats<V> d = of_dy(k), h = fma<V>(of_x(k), all<V>(k1), all<V>(off));
+        const Floats<V> d = of_dy(k), h = mul<V>(add<V>(of_x(k), all<V>(-m)), all<V>(k1));
         const Floats<V> g = mul<V>(d, wv[k]);
         s0 = add<V>(s0, g);
         s1 = fma<V>(g, h, s1);
@@ -362,7 +388,7 @@ __global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS, TPR > THREADS ?
       for (int k = 0; k < NV; ++k) {
         const int c = (k * TPR + t) * V;
         if (!there || c >= C) continue;
-        const Floats<V> h = fma<V>(of_x(k), all<V>(k1), all<V>(off));
+        const Floats<V> h = mul<V>(add<V>(of_x(k), all<V>(-m)), all<V>(k1));
         const Floats<V> g = mul<V>(of_dy(k), wv[k]);
         store<T, V>(dx + r * C + c, fma<V>(g, all<V>(k1), fma<V>(h, all<V>(b), all<V>(a))));
       }
