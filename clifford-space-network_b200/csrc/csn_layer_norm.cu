@@ -562,7 +562,7 @@ struct BackOf : Back {
     constexpr auto kernel = backward_kernel<T, W, TPR, NV, V, DEPTH>;
     if (smem > 32 * 1024 && allow_smem<kernel>(smem) != cudaSuccess) return;  // its error is found after the call
     // as many CTAs as the SMs hold at a time
-    const int n = (int)std::min<int64_t>(std::max<int64_t>((R + GROUPS - 1) / GROUPS, 1), 148 * (TPR > THREADS ? 1 : NV > 1 ? 2 : 4));
+    const int n = (int)std::min<int64_t>((R + GROUPS - 1) / GROUPS, 148 * (TPR > THREADS ? 1 : NV > 1 ? 2 : 4));
     kernel<<<n, N, smem, st>>>(static_cast<const T*>(dy), ldy, static_cast<const T*>(x), ld, mean, rstd, static_cast<const W*>(w),
                                static_cast<T*>(dx), dw || db ? part : nullptr, R, C);
     finish(n);
@@ -592,10 +592,10 @@ struct BackOf : Back {
     else run_long();
   }
   void run_long() const {
-    if (R && dx)
+    if (dx)
       long_backward_kernel<T, W><<<(unsigned)std::min<int64_t>(R, 148 * 4), 1024, 0, st>>>(
           static_cast<const T*>(dy), ldy, static_cast<const T*>(x), ld, mean, rstd, static_cast<const W*>(w), static_cast<T*>(dx), R, C);
-    const int n = (int)std::min<int64_t>(std::max<int64_t>(R, 1), parts(R, C));
+    const int n = parts(R, C);
     if (dw || db)
       long_weights_kernel<T><<<dim3((unsigned)((C + THREADS - 1) / THREADS), (unsigned)n), THREADS, 0, st>>>(
           static_cast<const T*>(dy), ldy, static_cast<const T*>(x), ld, mean, rstd, part, R, C);
@@ -656,6 +656,12 @@ extern "C" int csn_layer_norm_rows_bwd(const void* dy, int64_t ldy, const void* 
   if ((dweight || dbias) && (!workspace || !aligned(workspace, 16) || workspace_bytes < csn_layer_norm_rows_bwd_workspace_bytes(R, C)))
     return set_error(CSN_ERR_INVALID, "csn_layer_norm_rows_bwd: workspace smaller than csn_layer_norm_rows_bwd_workspace_bytes");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (R == 0) {  // nothing is read: the weight may be missing
+    for (void* to : {dweight, dbias})
+      if (to)
+        if (cudaError_t e = cudaMemsetAsync(to, 0, (size_t)C * ws, st)) return set_cuda_error(e, "csn_layer_norm_rows_bwd");
+    return CSN_OK;
+  }
   KernelTimer kt("layer_norm_rows_bwd", st);
   const Back A = {dy, x, weight, ldy, ldx, mean, rstd, dx, dweight, dbias, static_cast<float*>(workspace), R, (int)C};
   auto* f = dtype == CSN_BF16 ? (weight_dtype == CSN_F32 ? backward<__nv_bfloat16, float> : backward<__nv_bfloat16, __nv_bfloat16>)

@@ -527,8 +527,9 @@ int csn_linear_attention_step(const void* q, const void* k, const void* v, const
  * ldx (elements), y [R, C] contiguous, weight and bias [C] of the rows' type or float32
  * (weight_dtype), mean and rstd [R] float32 (NULL: not wanted).  The backward pass reads dy (row
  * stride ldy), x, mean and rstd and writes dx [R, C] (contiguous), dweight and dbias [C] (of
- * weight_dtype; each of the three may be NULL); it needs the workspace for the last two.  y, dx and
- * the workspace 16-byte aligned. */
+ * weight_dtype; each of the three may be NULL); it needs the workspace for the last two.
+ * Without rows (R = 0) these are 0, and what would be read may be NULL.  y, dx and the workspace
+ * 16-byte aligned. */
 int csn_layer_norm_rows_fwd(const void* x, int64_t ldx, const void* weight, const void* bias, void* y,
                             float* mean, float* rstd, int64_t R, int64_t C, float eps, int dtype,
                             int weight_dtype, void* stream);

@@ -89,3 +89,21 @@ def test_squares_past_the_range(ops, C):  # noqa: F811
     w, b = make((C,), torch.bfloat16, 1, 0.3, 1.0), make((C,), torch.bfloat16, 2)
     y = ops.layer_norm(x, w, b)
     assert torch.equal(y[0], b) and torch.equal(y[2], b) and y[1].isnan().all() and y[3].isnan().all()
+
+
+@pytest.mark.parametrize("C", [64, 771, 20000])
+def test_backward_without_rows_or_weight(C):
+    """A caller of the C ABI that has no rows need not have a weight: the sums over rows are 0."""
+    import ctypes
+    from csn_b200 import _lib
+    null = ctypes.c_void_p(0)
+    nbytes = _lib.load().csn_layer_norm_rows_bwd_workspace_bytes(0, C)
+    work = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+    for code, typ in ((1, torch.bfloat16), (0, torch.float32)):
+        for which in ((0, 1), (0,), (1,)):
+            sums = [torch.full((C + 8,), 7.0, device="cuda", dtype=typ) for _ in range(2)]
+            out = [ctypes.c_void_p(t.data_ptr()) if i in which else null for i, t in enumerate(sums)]
+            _lib.call("csn_layer_norm_rows_bwd", null, C, null, C, null, null, null, null, *out, 0, C, 1, code, ctypes.c_void_p(work.data_ptr()),
+                      nbytes, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+            for i, t in enumerate(sums):
+                assert (t[:C] == (0.0 if i in which else 7.0)).all() and (t[C:] == 7.0).all()
