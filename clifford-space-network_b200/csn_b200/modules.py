@@ -13,15 +13,28 @@ from . import ops
 
 class LayerNorm(nn.LayerNorm):
     """nn.LayerNorm (same parameters, state_dict keys and eps) computed by the CUDA LayerNorm
-    kernels for one normalised axis with affine weight and bias: any number of bfloat16 and float16 features on CUDA,
-    others of C % 4 == 0, C <= 1024; other shapes go to F.layer_norm."""
+    kernels (ops.layer_norm) for one normalised axis of C % 4 == 0, C <= 1024 features with affine
+    weight and bias; other shapes go to F.layer_norm, and keep what only that has: second
+    derivatives, forward-mode tangents, tracing, and a float32 result under autocast."""
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         C = x.shape[-1]
         if (len(self.normalized_shape) == 1 and self.weight is not None and self.bias is not None
-                and (x.is_cuda and x.dtype in (torch.bfloat16, torch.float16) or ops.layer_norm_supported(C))):
+                and ops.layer_norm_supported(C)):
             return ops.layer_norm(x, self.weight, self.bias, self.eps)
         return F.layer_norm(x, self.normalized_shape, self.weight, self.bias, self.eps)
+
+
+class BlockLayerNorm(LayerNorm):
+    """LayerNorm of the gated recurrent and linear-attention blocks, whose other operators are
+    differentiable once and not traced either: bfloat16 and float16 features on CUDA go to
+    ops.layer_norm at every width."""
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if (x.is_cuda and x.dtype in (torch.bfloat16, torch.float16) and len(self.normalized_shape) == 1
+                and self.weight is not None and self.bias is not None):
+            return ops.layer_norm(x, self.weight, self.bias, self.eps)
+        return super().forward(x)
 
 
 def causal_conv_input(ln: nn.LayerNorm, conv: nn.Conv1d, x: torch.Tensor) -> torch.Tensor:
@@ -137,7 +150,7 @@ class GatedRecurrentBlock(nn.Module):
 
     def __init__(self, d_model: int, d_inner: Optional[int] = None, d_ffn: Optional[int] = None, dropout: float = 0.0):
         super().__init__()
-        self.ln_1, self.ln_2 = LayerNorm(d_model), LayerNorm(d_model)
+        self.ln_1, self.ln_2 = BlockLayerNorm(d_model), BlockLayerNorm(d_model)
         self.mixer = GatedRecurrence(d_model, d_inner)
         self.ffn = GatedFeedForward(d_model, d_ffn)
         self.drop_1, self.drop_2 = DropoutAdd(dropout), DropoutAdd(dropout)
@@ -173,7 +186,7 @@ class LinearAttention(nn.Module):
             raise ValueError(f"LinearAttention: num_kv_heads has to divide num_heads and heads have 1 to 128 places, got "
                              f"{self.num_kv_heads}, {num_heads} and {self.head_dim}")
         self.in_proj = nn.Linear(d_model, (num_heads + 2 * self.num_kv_heads) * self.head_dim, bias=False)
-        self.norm = LayerNorm(self.head_dim)
+        self.norm = BlockLayerNorm(self.head_dim)
         self.out_proj = nn.Linear(num_heads * self.head_dim, d_model, bias=False)
         self.register_buffer("log_decay", torch.log1p(-torch.exp2(-torch.linspace(5.0, 12.0, num_heads))), persistent=False)
 
@@ -213,7 +226,7 @@ class LinearAttentionBlock(nn.Module):
     def __init__(self, d_model: int, num_heads: int, num_kv_heads: Optional[int] = None, head_dim: Optional[int] = None,
                  d_ffn: Optional[int] = None, dropout: float = 0.0):
         super().__init__()
-        self.ln_1, self.ln_2 = LayerNorm(d_model), LayerNorm(d_model)
+        self.ln_1, self.ln_2 = BlockLayerNorm(d_model), BlockLayerNorm(d_model)
         self.mixer = LinearAttention(d_model, num_heads, num_kv_heads, head_dim)
         self.ffn = GatedFeedForward(d_model, d_ffn)
         self.drop_1, self.drop_2 = DropoutAdd(dropout), DropoutAdd(dropout)
