@@ -98,12 +98,12 @@ Tensor bytes(const Tensor& like, size_t n) {
 void* stream(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 
 // Gradients are first-order: where a second backward pass could follow, what comes out raises in it.
-variable_list first_order(variable_list grads) {
+variable_list first_order(const char* name, variable_list grads) {
   if (!at::GradMode::is_enabled()) return grads;
   for (auto& g : grads)
     if (g.defined()) g = g.detach().set_requires_grad(true);
   auto error = std::make_shared<torch::autograd::DelayedError>(
-      "the gated operators are differentiable once: a second backward pass through them is not available", grads.size());
+      std::string(name) + " is differentiable once: a second backward pass through it is not available", grads.size());
   return (*error)(std::move(grads));
 }
 
@@ -220,7 +220,7 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
       at::AutoGradMode off(false);
       return scan_backward(s[0], s[1], s[2], s[3], s[4], g[0], g[1], ctx->saved_data["h0"].toBool());
     }();
-    return first_order({df, dx, dh0, dgate, Tensor()});
+    return first_order("gated_scan", {df, dx, dh0, dgate, Tensor()});
   }
 };
 
@@ -306,7 +306,7 @@ struct SiluGatedLinear : torch::autograd::Function<SiluGatedLinear> {
       at::AutoGradMode off(false);
       return ffn_backward(s[0], s[1], s[2], g[0], s[3], ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2));
     }();
-    return first_order({dx, dg, du});
+    return first_order("silu_gated_linear", {dx, dg, du});
   }
 };
 
@@ -485,7 +485,7 @@ struct LinearAttention : torch::autograd::Function<LinearAttention> {
       return attention_backward(s[0], s[1], s[2], s[3], s[4], s[5], g[0], g[1], ctx->saved_data["scale"].toDouble(), ctx->needs_input_grad(0),
                                 ctx->needs_input_grad(1), ctx->needs_input_grad(2), ctx->saved_data["s0"].toBool());
     }();
-    return first_order({dq, dk, dv, Tensor(), ds0, Tensor(), Tensor()});
+    return first_order("linear_attention", {dq, dk, dv, Tensor(), ds0, Tensor(), Tensor()});
   }
 };
 
@@ -557,7 +557,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
                                     code_of(x.scalar_type()), code_of(w.scalar_type()), ptr(ws), nb, stream(x)));
       return std::make_tuple(dx, dw, db);
     }();
-    return first_order({dx, dw, db, Tensor()});
+    return first_order("layer_norm", {dx, dw, db, Tensor()});
   }
 };
 
@@ -602,7 +602,7 @@ struct DropoutAdd : torch::autograd::Function<DropoutAdd> {
       at::AutoGradMode off(false);
       dx = dropout_run(g[0], std::nullopt, ctx->saved_data["cut"].toInt(), rng);
     }
-    return first_order({dx, ctx->saved_data["residual"].toBool() ? g[0] : Tensor(), Tensor(), Tensor()});
+    return first_order("dropout_add", {dx, ctx->saved_data["residual"].toBool() ? g[0] : Tensor(), Tensor(), Tensor()});
   }
 };
 
