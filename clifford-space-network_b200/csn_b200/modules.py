@@ -108,7 +108,7 @@ class GatedRecurrence(nn.Module):
 
     def init_state(self, batch_size: int, device=None) -> torch.Tensor:
         device = device if device is not None else self.in_proj.weight.device
-        return torch.zeros(batch_size, self.d_inner, device=device)
+        return torch.zeros(batch_size, self.d_inner, device=device, dtype=torch.float32)
 
     def forward(self, x: torch.Tensor, h0: Optional[torch.Tensor] = None, cu_seqlens: Optional[torch.Tensor] = None):
         """x [B, T, d_model], or [L, d_model] packed with cu_seqlens -> (out, float32 states [B, d_inner])."""
@@ -188,7 +188,7 @@ class LinearAttention(nn.Module):
         self.in_proj = nn.Linear(d_model, (num_heads + 2 * self.num_kv_heads) * self.head_dim, bias=False)
         self.norm = BlockLayerNorm(self.head_dim)
         self.out_proj = nn.Linear(num_heads * self.head_dim, d_model, bias=False)
-        self.register_buffer("log_decay", torch.log1p(-torch.exp2(-torch.linspace(5.0, 12.0, num_heads))), persistent=False)
+        self.register_buffer("log_decay", torch.log1p(-torch.exp2(-torch.linspace(5.0, 12.0, num_heads, dtype=torch.float32))), persistent=False)
 
     def _apply(self, fn, *args, **kwargs):
         decay = self.log_decay
@@ -200,7 +200,7 @@ class LinearAttention(nn.Module):
 
     def init_state(self, batch_size: int, device=None) -> torch.Tensor:
         device = device if device is not None else self.in_proj.weight.device
-        return torch.zeros(batch_size, self.num_heads, self.head_dim, self.head_dim, device=device)
+        return torch.zeros(batch_size, self.num_heads, self.head_dim, self.head_dim, device=device, dtype=torch.float32)
 
     def _heads(self, x: torch.Tensor):
         h, hk, d = self.num_heads, self.num_kv_heads, self.head_dim
