@@ -188,14 +188,20 @@ class LinearAttention(nn.Module):
         self.in_proj = nn.Linear(d_model, (num_heads + 2 * self.num_kv_heads) * self.head_dim, bias=False)
         self.norm = BlockLayerNorm(self.head_dim)
         self.out_proj = nn.Linear(num_heads * self.head_dim, d_model, bias=False)
-        self.register_buffer("log_decay", torch.log1p(-torch.exp2(-torch.linspace(5.0, 12.0, num_heads, dtype=torch.float32))), persistent=False)
+        self.register_buffer("log_decay", self._decays(), persistent=False)
+
+    def _decays(self, **kw) -> torch.Tensor:
+        return torch.log1p(-torch.exp2(-torch.linspace(5.0, 12.0, self.num_heads, dtype=torch.float32, **kw)))
 
     def _apply(self, fn, *args, **kwargs):
         decay = self.log_decay
         super()._apply(fn, *args, **kwargs)
-        # .bfloat16() and the like change the layer's type, not the decays': 16 bits have no number next to 1 - 2^-12
-        if self.log_decay.dtype != torch.float32:
-            self.log_decay = decay.to(self.log_decay.device)
+        # .bfloat16() and the like change the layer's type, not the decays': 16 bits have no number next to 1 - 2^-12.
+        # .to_empty() leaves them as well, and makes those of a module that had no memory: no state_dict brings them.
+        device = self.log_decay.device
+        if decay.is_meta and device.type != "meta":
+            decay = self._decays(device="cpu")
+        self.log_decay = decay.to(device)
         return self
 
     def init_state(self, batch_size: int, device=None) -> torch.Tensor:
