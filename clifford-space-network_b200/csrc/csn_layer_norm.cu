@@ -559,10 +559,13 @@ struct BackOf : Back {
   void run() const {
     constexpr int N = TPR > THREADS ? TPR : THREADS, GROUPS = N / TPR, DEPTH = V == 8 ? (NV > 2 ? 3 : NV > 1 ? 5 : 6) : 2;
     constexpr int ring = V == 8 ? DEPTH * (2 * NV * N * V * 2 + 2 * N * 4) : 0, sums = GROUPS > 1 ? N * NV * V * 4 : 0, smem = ring > sums ? ring : sums;
+    // That an SM holds at a time; more of them start a second, mostly empty round.  C <= 64: 3 of 6 rows' depth, R1048576 C64 88 us;
+    // 4 CTAs of that depth 92, 4 of a depth of 5, which do fit, 96.
+    constexpr int CTAS = TPR > THREADS ? 1 : NV > 1 ? 2 : V == 8 ? 3 : 4;
+    static_assert((smem + 2048) * CTAS <= 228 * 1024, "1 KB of an SM's shared memory goes to each CTA, and some to its static part");
     constexpr auto kernel = backward_kernel<T, W, TPR, NV, V, DEPTH>;
     if (smem > 32 * 1024 && allow_smem<kernel>(smem) != cudaSuccess) return;  // its error is found after the call
-    // as many CTAs as the SMs hold at a time
-    const int n = (int)std::min<int64_t>((R + GROUPS - 1) / GROUPS, 148 * (TPR > THREADS ? 1 : NV > 1 ? 2 : 4));
+    const int n = (int)std::min<int64_t>((R + GROUPS - 1) / GROUPS, 148 * CTAS);
     kernel<<<n, N, smem, st>>>(static_cast<const T*>(dy), ldy, static_cast<const T*>(x), ld, mean, rstd, static_cast<const W*>(w),
                                static_cast<T*>(dx), dw || db ? part : nullptr, R, C);
     finish(n);
