@@ -29,8 +29,9 @@ def linear_attention(q, k, v, log_decay, s0=None, cu_seqlens=None, scale=None):
 
     Sums and states are float32.  16-bit tensors go through the tensor cores in blocks of 128 steps (one more rounding
     to 16 bits of q k^T inside a block and of the state where it meets q, none of the state that is carried); there an
-    infinity or NaN in k or v can reach the outputs of its whole block.  16-bit rows that do not start on 16 bytes, and expanded
-    ones, are copied first."""
+    infinity or NaN in k or v can reach the outputs of its whole block, one in q, k, v or the gradient of o the gradients of its
+    block, and what depends on it may be NaN where it would be infinite; other blocks, heads and sequences that do not depend on
+    it keep their bits.  16-bit rows that do not start on 16 bytes, and expanded ones, are copied first."""
     return (gated._module or gated._ext()).linear_attention(q, k, v, log_decay, s0, cu_seqlens, scale)
 
 

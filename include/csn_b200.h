@@ -489,7 +489,8 @@ int csn_dropout_add(const void* x, const void* residual, const int64_t* rng, voi
  * Sums and states are float32.  16-bit tensors go through the tensor cores in blocks of 128 steps:
  * there the products q k^T inside a block and the state, as an operand of its product with q, are
  * rounded to the tensors' type, the state that is carried on is not.  An infinity or NaN in k or v
- * can reach the outputs of its whole block.  Should a device-side wait give up (it is bounded), the
+ * can reach the outputs of its whole block, one in q, k, v or do the gradients of its block, and what
+ * depends on it may be NaN where it would be infinite.  Should a device-side wait give up (it is bounded), the
  * results it concerns are NaN.
  * 16-bit operands whose rows do not start on 16 bytes (base, or a stride that is no multiple of 8
  * elements, or 0 over more than one place) are copied first: csn_linear_attention_copies says which
