@@ -184,8 +184,8 @@ __device__ __forceinline__ void correct(float d, float& m, float& square) {
 // TPR threads take a row, NV pieces of V neighbouring places each, and ROWS rows at a time, to have enough loads in flight: a row
 // is read once and stays in registers, in its own type.  V = 8 where rows start on 16 bytes and C is a multiple of 8, else 1.
 // A warp takes rows of up to 2048 places: two reductions without a barrier.
-// bf16 on a B200: R32768 C2048 50 us (5.4 TB/s), R524288 C128 54 (5.0), R8192 C8192 51 (5.3), where a CTA to a row that read it
-// three times took 93, 812 and 88.  Bound by memory and, where rows are short, by the instructions that rows cost besides
+// bf16 on a B200: R32768 C2048 51 us (5.3 TB/s), R524288 C128 59 (4.6), R8192 C8192 51 (5.2), R4096 C16384 76 (3.5; the second mean is
+// 10 of it), where a CTA to a row that read it three times took 93, 812 and 88 for the first three.  Bound by memory and, where rows are short, by the instructions that rows cost besides
 // their places.  Slower: C2048 with a CTA to a row 80 us (barriers), with 173 registers a thread 64 (8 warps an SM).
 template <typename T, typename W, int TPR, int NV, int V, int ROWS>
 __global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS, TPR > THREADS ? 1 : NV * V >= 64 ? 3 : 4)
@@ -295,8 +295,8 @@ __global__ void __launch_bounds__(1024) long_forward_kernel(const T* __restrict_
 // so it also gathers their sums of dy h and dy, which the CTA adds up at the end: part[CTA][0 and 1][C].  For V = 8 each
 // thread copies its own pieces of x and dy into shared memory DEPTH - 1 rows ahead (cp.async; no other thread reads them, so
 // that no barrier is needed): the registers that loads in flight would take leave room for more warps.
-// bf16 on a B200, with the sums: R32768 C2048 93 us (4.3 TB/s), R524288 C128 80 (5.0), R8192 C8192 108 (3.7).  Neither memory nor
-// issue is full (an SM issues in 41 to 62 % of its cycles, with 15 of 64 warps): a row's meeting at its barrier and the chain from
+// bf16 on a B200, with the sums: R32768 C2048 91 us (4.4 TB/s), R524288 C128 76 (5.3), R8192 C8192 109 (3.7), R1048576 C64 83 (4.8).
+// Neither memory nor issue is full (an SM issues in 42 to 68 % of its cycles, with 15 to 21 of 64 warps): a row's meeting at its barrier and the chain from
 // its sums to its gradient are what a few warps wait for.  Slower: 8 places to a thread 108 us for C2048 (shuffles, the meeting
 // and addresses cost a row 130 instructions a thread, whatever it has of it), loads into registers 160, mean and rstd
 // read when a row's turn comes 140 for C8192, more CTAs than the SMs hold at a time.
@@ -559,8 +559,8 @@ struct BackOf : Back {
   void run() const {
     constexpr int N = TPR > THREADS ? TPR : THREADS, GROUPS = N / TPR, DEPTH = V == 8 ? (NV > 2 ? 3 : NV > 1 ? 5 : 6) : 2;
     constexpr int ring = V == 8 ? DEPTH * (2 * NV * N * V * 2 + 2 * N * 4) : 0, sums = GROUPS > 1 ? N * NV * V * 4 : 0, smem = ring > sums ? ring : sums;
-    // That an SM holds at a time; more of them start a second, mostly empty round.  C <= 64: 3 of 6 rows' depth, R1048576 C64 88 us;
-    // 4 CTAs of that depth 92, 4 of a depth of 5, which do fit, 96.
+    // That an SM holds at a time; more of them start a second, mostly empty round.  C <= 64: 3 of 6 rows' depth, R1048576 C64 88 us with
+    // events around the call; 4 CTAs of that depth 92, 4 of a depth of 5, which do fit, 96.
     constexpr int CTAS = TPR > THREADS ? 1 : NV > 1 ? 2 : V == 8 ? 3 : 4;
     static_assert((smem + 2048) * CTAS <= 228 * 1024, "1 KB of an SM's shared memory goes to each CTA, and some to its static part");
     constexpr auto kernel = backward_kernel<T, W, TPR, NV, V, DEPTH>;

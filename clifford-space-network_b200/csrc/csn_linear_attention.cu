@@ -18,8 +18,10 @@ constexpr int BLOCK = 16;  // steps that are worked on together
 // place of v and the K entries of the state beside it in registers: one packed pair of FMA an entry and step for each of the two
 // products, the products a . b shared by all threads.  The state is rounded once a block: step by step, a memory of
 // thousands of steps costs it a digit.
-// The rows come DEPTH - 1 blocks ahead by cp.async, 16 bytes at a time where they are aligned (`wide`).  Bound by the loads of
-// a and b from shared memory, which every thread needs, one for two packed FMA: forward, with the first pass, B32 T2048 H4 D32
+// The rows come DEPTH - 1 blocks ahead by cp.async, 16 bytes at a time where they are aligned (`wide`).  What it does most is load a
+// and b from shared memory, which every thread needs, one load for two packed FMA: at B32 T2048 H4 D32 that pipe is busy for 48 to
+// 64 % of the time and issue for 41 to 53 %, with 2 to 3 warps a scheduler, which wait for such loads.  At B8 T1024 H4 D32, 2 warps an
+// SM, it is 13 % and 25 %: there a single warp's chain is the time.  Forward, with the first pass, B32 T2048 H4 D32
 // 161 us, B8 T4096 H16 D64 780, B2 T2048 H16 D128 386.  Slower: step by step (three roundings a step, too) and rows loaded when
 // their turn comes, 706 us for the first; half as many segments 158, 874 and 457.
 // OUT: false for the first pass.
@@ -315,7 +317,10 @@ int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // The steps of a segment, a multiple of 128.  float32: enough segments for 24 warps on each SM.  16 bits, one CTA an SM: what
 // takes the least time by these, measured with 128 x 128 states in bf16, in units of 0.1 us: a block of 128 steps 39, the start and end
-// of a CTA 90; where sequences are cut, in the first pass 27 and 70, and join_kernel 50, 5 a segment and its states' bytes.
+// of a CTA 90; where sequences are cut, in the first pass 27 and 70, and join_kernel 50, 5 a segment and its states' bytes.  Other
+// passes are taken to have these times in the same proportion (a block of 64 places takes about 0.7 of them, one of float16 1.2), and
+// a packed batch to be one sequence, since its borders are not known here: none may be as long as a segment, and the first
+// pass and join_kernel find nothing to do (3 x 15 us of 664 for L20011 H12 Dk72 Dv104 float16 and 37 sequences).
 void cut(Batch& B, int Dk, int Dv, int passes, bool packed, bool half) {
   const int64_t rows = up(B.T, 128), heads = (int64_t)B.H * (packed ? 1 : B.S), ways = std::min(passes, 2);
   int64_t best = 1;
