@@ -184,9 +184,10 @@ __device__ __forceinline__ void correct(float d, float& m, float& square) {
 // TPR threads take a row, NV pieces of V neighbouring places each, and ROWS rows at a time, to have enough loads in flight: a row
 // is read once and stays in registers, in its own type.  V = 8 where rows start on 16 bytes and C is a multiple of 8, else 1.
 // A warp takes rows of up to 2048 places: two reductions without a barrier.
-// bf16 on a B200: R32768 C2048 51 us (5.3 TB/s), R524288 C128 59 (4.6), R8192 C8192 51 (5.2), R4096 C16384 76 (3.5; the second mean is
-// 10 of it), where a CTA to a row that read it three times took 93, 812 and 88 for the first three.  Bound by memory and, where rows are short, by the instructions that rows cost besides
-// their places.  Slower: C2048 with a CTA to a row 80 us (barriers), with 173 registers a thread 64 (8 warps an SM).
+// bf16 on a B200: R32768 C2048 51 us (5.3 TB/s), R524288 C128 59 (4.6), R8192 C8192 51 (5.2), R4096 C16384 76 (3.5; the second
+// mean is 10 of it), where a CTA to a row that read it three times took 93, 812 and 88 for the first three.  Bound by memory
+// and, where rows are short, by the instructions that rows cost besides their places.  Slower: C2048 with a CTA to a row 80 us
+// (barriers), with 173 registers a thread 64 (8 warps an SM).
 template <typename T, typename W, int TPR, int NV, int V, int ROWS>
 __global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS, TPR > THREADS ? 1 : NV * V >= 64 ? 3 : 4)
     forward_kernel(const T* __restrict__ x, int64_t ld, const W* __restrict__ w, const W* __restrict__ b, T* __restrict__ y, float* mean,
